@@ -1,0 +1,148 @@
+// What the kernels of the training step share (cross_entropy.cu, norm_residual.cu, rotary.cu, adamw.cu).
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+#include <stdio.h>
+
+#include "../../include/ffcv_b200.h"
+
+namespace ffcvb {
+
+constexpr int kSms = 148;
+
+// The message of the calling thread's last failure; returns `code`.
+int training_fail(int code, const char *fmt, ...) __attribute__((format(printf, 2, 3)));
+
+// Makes `device` current for a call's launches, and the one before it again afterwards.
+class OnDevice {
+  public:
+    explicit OnDevice(int device) {
+        if (cudaGetDevice(&before_) != cudaSuccess) before_ = -1;
+        ok_ = before_ == device || cudaSetDevice(device) == cudaSuccess;
+        if (before_ == device) before_ = -1;
+    }
+    ~OnDevice() {
+        if (before_ >= 0) cudaSetDevice(before_);
+    }
+    bool ok() const { return ok_; }
+
+  private:
+    int before_ = -1;
+    bool ok_ = false;
+};
+
+inline int launched(const char *what) {
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? FFCVB_OK : training_fail(FFCVB_E_CUDA, "%s: %s", what, cudaGetErrorString(e));
+}
+
+// Calls f with a value of the type that a FFCVB_TYPE_* stands for.
+template <typename F>
+bool with_type(int type, F &&f) {
+    switch (type) {
+    case FFCVB_TYPE_F32: f(float{}); return true;
+    case FFCVB_TYPE_F16: f(__half{}); return true;
+    case FFCVB_TYPE_BF16: f(__nv_bfloat16{}); return true;
+    }
+    return false;
+}
+inline int type_size(int type) { return type == FFCVB_TYPE_F32 ? 4 : 2; }
+
+#ifdef __CUDACC__
+
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T from_float(float v);
+template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// N values that are loaded and stored at once: 16 bytes of them, or one.
+template <typename T, int N> struct Pack;
+template <typename T> struct Pack<T, 1> {
+    T raw;
+    __device__ __forceinline__ void load(const T *p) { raw = *p; }
+    __device__ __forceinline__ void load_once(const T *p) { raw = __ldcs(p); }
+    __device__ __forceinline__ void store(T *p) const { *p = raw; }
+    __device__ __forceinline__ void store_once(T *p) const { __stcs(p, raw); }
+    __device__ __forceinline__ void get(float (&v)[1]) const { v[0] = to_float(raw); }
+    __device__ __forceinline__ void set(const float (&v)[1]) { raw = from_float<T>(v[0]); }
+};
+template <typename T> struct Pack16 {
+    uint4 raw;
+    __device__ __forceinline__ void load(const T *p) { raw = *reinterpret_cast<const uint4 *>(p); }
+    // (what is read or written once and not soon again need not displace what is)
+    __device__ __forceinline__ void load_once(const T *p) { raw = __ldcs(reinterpret_cast<const uint4 *>(p)); }
+    __device__ __forceinline__ void store(T *p) const { *reinterpret_cast<uint4 *>(p) = raw; }
+    __device__ __forceinline__ void store_once(T *p) const { __stcs(reinterpret_cast<uint4 *>(p), raw); }
+};
+template <> struct Pack<float, 4> : Pack16<float> {
+    __device__ __forceinline__ void get(float (&v)[4]) const {
+        v[0] = __uint_as_float(raw.x);
+        v[1] = __uint_as_float(raw.y);
+        v[2] = __uint_as_float(raw.z);
+        v[3] = __uint_as_float(raw.w);
+    }
+    __device__ __forceinline__ void set(const float (&v)[4]) {
+        raw = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+    }
+};
+template <> struct Pack<__nv_bfloat16, 8> : Pack16<__nv_bfloat16> {
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            v[2 * k] = __uint_as_float(w[k] << 16);
+            v[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
+        }
+    }
+    __device__ __forceinline__ void set(const float (&v)[8]) {
+        uint32_t w[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const __nv_bfloat162 two = __floats2bfloat162_rn(v[2 * k], v[2 * k + 1]);
+            w[k] = *reinterpret_cast<const uint32_t *>(&two);
+        }
+        raw = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+};
+template <> struct Pack<__half, 8> : Pack16<__half> {
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const float2 two = __half22float2(*reinterpret_cast<const __half2 *>(&w[k]));
+            v[2 * k] = two.x;
+            v[2 * k + 1] = two.y;
+        }
+    }
+    __device__ __forceinline__ void set(const float (&v)[8]) {
+        uint32_t w[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const __half2 two = __floats2half2_rn(v[2 * k], v[2 * k + 1]);
+            w[k] = *reinterpret_cast<const uint32_t *>(&two);
+        }
+        raw = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+};
+template <typename T> constexpr int kWide = 16 / (int)sizeof(T);
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+
+#endif
+
+} // namespace ffcvb

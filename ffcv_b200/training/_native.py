@@ -1,0 +1,58 @@
+"""Calls of ``libffcv_b200.so`` for the training step: arguments are packed into the C structures of
+``include/ffcv_b200.h`` (all 8-byte members first, so that there is no padding)."""
+import struct
+from ctypes import c_char_p, c_int, c_int32, c_int64, c_void_p
+
+import torch as ch
+
+from ..libffcv import lib
+
+TYPES = {ch.float32: 0, ch.float16: 1, ch.bfloat16: 2}
+
+CROSS_ENTROPY = struct.Struct('=8Q6q8i2f')
+NORM_RESIDUAL = struct.Struct('=22Q8q6i2f')
+ROTARY = struct.Struct('=6Q19q6ifi')
+ADAMW = struct.Struct('=7Qq4id')
+ADAMW_GROUP = struct.Struct('=5d')
+ADAMW_BLOCK = 256
+NORM_MAX_WIDTH = 16384
+
+lib.ffcvb_training_error.argtypes = []
+lib.ffcvb_training_error.restype = c_char_p
+for _name in ('ffcvb_cross_entropy', 'ffcvb_norm_residual', 'ffcvb_norm_residual_backward', 'ffcvb_rotary'):
+    getattr(lib, _name).argtypes = [c_char_p, c_void_p]
+    getattr(lib, _name).restype = c_int
+lib.ffcvb_norm_residual_workspace.argtypes = [c_char_p]
+lib.ffcvb_norm_residual_workspace.restype = c_int64
+lib.ffcvb_adamw_layout.argtypes = [c_int32, c_void_p, c_void_p, c_void_p]
+lib.ffcvb_adamw_layout.restype = c_int64
+lib.ffcvb_adamw_table.argtypes = [c_int32, c_void_p, c_void_p, c_void_p]
+lib.ffcvb_adamw_table.restype = c_int
+lib.ffcvb_adamw_step.argtypes = [c_char_p, c_void_p, c_void_p, c_void_p, c_void_p, c_char_p, c_int32, c_void_p]
+lib.ffcvb_adamw_step.restype = c_int
+
+
+def check(rc):
+    if rc != 0:
+        raise RuntimeError(f'{lib.ffcvb_training_error().decode()} (error {rc})')
+
+
+def stream_of(tensor):
+    return ch.cuda.current_stream(tensor.device).cuda_stream
+
+
+def ptr(tensor):
+    return 0 if tensor is None else tensor.data_ptr()
+
+
+def require(tensor, name, like=None):
+    """A CUDA tensor of a type the kernels know, on the device of `like`."""
+    if not isinstance(tensor, ch.Tensor):
+        raise TypeError(f'{name} is not a tensor')
+    if not tensor.is_cuda:
+        raise TypeError(f'{name} is not on a GPU; ffcv_b200 has no CPU form of this operator')
+    if tensor.dtype not in TYPES:
+        raise TypeError(f'{name}: {tensor.dtype} is none of float32, float16, bfloat16')
+    if like is not None and tensor.device != like.device:
+        raise ValueError(f'{name} is on {tensor.device}, not on {like.device}')
+    return TYPES[tensor.dtype]

@@ -1,0 +1,209 @@
+"""AdamW over all tensors of a network in one launch, with moments in 32 or in 8 bits."""
+import numpy as np
+import torch as ch
+
+from . import _native as N
+
+_BLOCK = N.ADAMW_BLOCK
+
+
+class AdamW(ch.optim.Optimizer):
+    """Adam with decoupled weight decay.
+
+    Parameters
+    ----------
+    params : iterable
+        Parameters or groups of them, all of one floating type and on one GPU.
+    lr, betas, eps, weight_decay
+        As in ``torch.optim.AdamW``; each may differ from group to group and change from step to step.
+    state_bits : 32 or 8
+        8 keeps the first moment as an e4m3 and the second as an e5m2 number, with one power of two as scale per 256
+        values, rounded stochastically.
+    max_grad_norm : float
+        Gradients are scaled down together so that their norm is at most this.  Where the norm is not finite, the step
+        changes nothing (but counts).  ``grad_norm`` holds the last step's norm, on the GPU.
+    seed : int
+        Of the stochastic rounding: the same seed, steps and gradients give the same weights.
+
+    16-bit parameters have 32-bit masters, which the steps are made on.  The state lies in flat tensors, ``exp_avg``,
+    ``exp_avg_sq``, ``scales`` (8 bits) and ``master`` (16-bit parameters), of which ``state[p]`` has views; every
+    parameter begins a block of 256 values, the rest of its last block is zero.  A parameter without a gradient is left alone,
+    and its step is not counted.  The kernels read the current learning rates from the groups and take gradients and
+    parameters wherever they lie at the time of the step.
+    """
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, state_bits=32, max_grad_norm=None,
+                 seed=0):
+        if state_bits not in (8, 32):
+            raise ValueError(f'state_bits must be 8 or 32, not {state_bits}')
+        if max_grad_norm is not None and not max_grad_norm > 0:
+            raise ValueError(f'max_grad_norm must be positive, not {max_grad_norm}')
+        self.state_bits, self.max_grad_norm, self.seed = state_bits, max_grad_norm, int(seed)
+        self.exp_avg = self.exp_avg_sq = self.scales = self.master = self.grad_norm = None
+        self._params, self._numel, self._steps = [], None, np.zeros(0, np.int64)
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+
+    @staticmethod
+    def _check_group(group):
+        b1, b2 = group['betas']
+        if not (group['lr'] >= 0 and group['eps'] >= 0 and group['weight_decay'] >= 0 and 0 <= b1 < 1 and 0 <= b2 < 1):
+            raise ValueError('lr, eps and weight_decay must not be negative, betas must be in [0, 1): '
+                             f"{ {k: group[k] for k in ('lr', 'betas', 'eps', 'weight_decay')} }")
+
+    def add_param_group(self, group):
+        super().add_param_group(group)
+        group = self.param_groups[-1]
+        try:
+            self._check_group(group)
+            for p in group['params']:
+                N.require(p, 'parameter')
+                like = self._params[0] if self._params else group['params'][0]
+                if p.dtype != like.dtype or p.device != like.device:
+                    raise TypeError(f'parameters must be of one type on one GPU: {p.dtype} on {p.device}, {like.dtype} on {like.device}')
+                if not _dense(p):
+                    raise ValueError('parameters must lie together in memory, without gaps or overlaps')
+        except Exception:
+            self.param_groups.pop()
+            raise
+        self._lay_out()
+
+    def _lay_out(self):
+        """Flat state for all parameters of all groups; what there was keeps its values."""
+        old = {id(p): (start, step) for p, start, step in zip(self._params, self._start if self._params else (), self._steps)}
+        before = self.exp_avg, self.exp_avg_sq, self.scales, self.master
+        self._params = [p for group in self.param_groups for p in group['params']]
+        n, device, dtype = len(self._params), self._params[0].device, self._params[0].dtype
+        self._numel = np.array([p.numel() for p in self._params], np.int64)
+        self._start, sizes = np.zeros(n, np.int64), np.zeros(2, np.int64)
+        total = N.lib.ffcvb_adamw_layout(n, self._numel.ctypes.data, self._start.ctypes.data, sizes.ctypes.data)
+        zeros = lambda t: ch.zeros(total, dtype=t, device=device)  # noqa: E731
+        eight = self.state_bits == 8
+        self.exp_avg = zeros(ch.uint8).view(ch.float8_e4m3fn) if eight else zeros(ch.float32)
+        self.exp_avg_sq = zeros(ch.uint8).view(ch.float8_e5m2) if eight else zeros(ch.float32)
+        self.scales = ch.ones((total // _BLOCK, 2), device=device) if eight else None
+        self.master = None if dtype == ch.float32 else zeros(ch.float32)
+        self._table = ch.empty(int(sizes[0]), dtype=ch.uint8, device=device)
+        self._workspace = ch.empty(max(16, int(sizes[1])), dtype=ch.uint8, device=device) if self.max_grad_norm else None
+        self.grad_norm = ch.zeros((), device=device) if self.max_grad_norm else None
+        self._table_size, self._at = int(sizes[0]), None
+        self._group_of = np.repeat(np.arange(len(self.param_groups), dtype=np.int32), [len(g['params']) for g in self.param_groups])
+        steps = np.zeros(n, np.int64)
+        for i, p in enumerate(self._params):
+            a, b = int(self._start[i]), int(self._start[i]) + -(-p.numel() // _BLOCK) * _BLOCK
+            if id(p) in old:
+                was, steps[i] = old[id(p)]
+                for now, then in zip((self.exp_avg, self.exp_avg_sq, self.master), before[:2] + before[3:]):
+                    if now is not None:
+                        _bytes(now)[a * now.itemsize:b * now.itemsize].copy_(_bytes(then)[was * now.itemsize:(was + b - a) * now.itemsize])
+                if eight:
+                    self.scales[a // _BLOCK:b // _BLOCK].copy_(before[2][was // _BLOCK:(was + b - a) // _BLOCK])
+            elif self.master is not None:
+                self._of(self.master, i).copy_(p.detach())
+            entry = self.state[p] = dict(step=int(steps[i]), exp_avg=self._of(self.exp_avg, i), exp_avg_sq=self._of(self.exp_avg_sq, i))
+            if eight:
+                entry['scales'] = self.scales[a // _BLOCK:b // _BLOCK]
+            if self.master is not None:
+                entry['master'] = self._of(self.master, i)
+        self._steps = steps
+
+    def _of(self, flat, i):
+        """Parameter i's part of a flat tensor, in the parameter's shape and order in memory."""
+        p = self._params[i]
+        return ch.as_strided(flat, p.shape, p.stride(), int(self._start[i]))
+
+    def _gradients(self):
+        """Addresses of the gradients, 0 without one, and tensors that must live until the launch."""
+        kept, at = [], []
+        for p in self._params:
+            g = p.grad
+            if g is None:
+                at.append(0)
+                continue
+            if g.stride() != p.stride() or g.dtype != p.dtype:
+                if g.is_sparse or g.dtype != p.dtype:
+                    raise TypeError(f'gradients must be dense and of the parameters\' type, not {g.dtype} {g.layout}')
+                g = ch.empty_like(p).copy_(g)
+                kept.append(g)
+            if g.device != p.device:
+                raise ValueError(f'a gradient is on {g.device}, its parameter on {p.device}')
+            at.append(g.data_ptr())
+        return np.array(at, np.uint64), kept
+
+    @ch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with ch.enable_grad():
+                loss = closure()
+        params = self._params
+        device = params[0].device
+        grads, kept = self._gradients()
+        at = [p.data_ptr() for p in params]
+        if at != self._at:  # the first step, or parameters that have moved
+            host = np.empty(max(1, self._table_size), np.uint8)
+            where = np.array(at, np.uint64)
+            N.check(N.lib.ffcvb_adamw_table(len(params), self._numel.ctypes.data, where.ctypes.data, host.ctypes.data))
+            self._table.copy_(ch.from_numpy(host[:self._table_size]))
+            self._at = at
+        groups = bytearray()
+        for group in self.param_groups:
+            self._check_group(group)
+            groups += N.ADAMW_GROUP.pack(group['lr'], *group['betas'], group['eps'], group['weight_decay'])
+        args = N.ADAMW.pack(self._table.data_ptr(), self.exp_avg.data_ptr(), self.exp_avg_sq.data_ptr(), N.ptr(self.scales),
+                            N.ptr(self.master), N.ptr(self.grad_norm), N.ptr(self._workspace), self.seed, device.index,
+                            N.TYPES[params[0].dtype], self.state_bits, len(params), self.max_grad_norm or 0.0)
+        N.check(N.lib.ffcvb_adamw_step(args, self._numel.ctypes.data, grads.ctypes.data, self._steps.ctypes.data,
+                                       self._group_of.ctypes.data, bytes(groups), len(self.param_groups),
+                                       N.stream_of(params[0])))
+        del kept
+        return loss
+
+    def state_dict(self):
+        for p, step in zip(self._params, self._steps):
+            self.state[p]['step'] = int(step)
+        saved = super().state_dict()
+        saved['state_bits'] = self.state_bits
+        return saved
+
+    @ch.no_grad()
+    def load_state_dict(self, saved):
+        """State as :meth:`state_dict` gives it, of the same parameters in the same groups; with ``state_bits=32`` also
+        that of ``torch.optim.AdamW``.  Values are copied into the flat tensors."""
+        groups = saved['param_groups']
+        if [len(g['params']) for g in groups] != [len(g['params']) for g in self.param_groups]:
+            raise ValueError('the saved state has other parameter groups')
+        if saved.get('state_bits', 32) != self.state_bits:
+            raise ValueError(f"the saved state has {saved.get('state_bits', 32)}-bit moments, not {self.state_bits}-bit ones")
+        for group, theirs in zip(self.param_groups, groups):
+            for key, value in theirs.items():
+                if key != 'params' and key in group:
+                    group[key] = value
+            self._check_group(group)
+        ids = [i for g in groups for i in g['params']]
+        for i, (p, key) in enumerate(zip(self._params, ids)):
+            entry, own = saved['state'].get(key), self.state[p]
+            if entry is None:
+                continue
+            for name, view in own.items():
+                if name == 'step' or (name == 'master' and name not in entry):
+                    continue
+                if entry[name].shape != view.shape or entry[name].dtype != view.dtype:
+                    raise ValueError(f'saved {name}: {entry[name].dtype} {tuple(entry[name].shape)}, not {view.dtype} {tuple(view.shape)}')
+                view.copy_(entry[name])
+            if 'master' in own and 'master' not in entry:
+                own['master'].copy_(p.detach())
+            self._steps[i] = int(entry['step'])
+
+
+def _dense(p):
+    """Whether a tensor's values fill a stretch of memory, each once, in whatever order."""
+    size = 1
+    for stride, n in sorted((s, n) for s, n in zip(p.stride(), p.shape) if n != 1):
+        if stride != size:
+            return p.numel() == 0
+        size *= n
+    return True
+
+
+def _bytes(t):
+    return t.view(-1).view(ch.uint8)

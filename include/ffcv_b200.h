@@ -307,6 +307,120 @@ int ffcvb_onehot_mix(ffcvb_ctx *ctx, void *stream, int n, int classes, const int
 int ffcvb_poison(ffcvb_ctx *ctx, void *stream, uint8_t *images_dev, int n, int64_t count, const uint8_t *apply,
                  const double *one_minus_alpha_dev, const double *mask_dev, double clamp_lo, double clamp_hi);
 
+/* ---- operators of a training step ---------------------------------------------------------
+ * No counterpart in the reference, whose work ends with the batch: what an image network's training
+ * step does with that batch, on the stream it arrives on.  They need no context.  All pointers are
+ * DEVICE pointers unless said otherwise; every call queues its work on `stream` of `device` and
+ * returns FFCVB_OK or a negative code, whose message ffcvb_training_error() gives (of the calling
+ * thread's last failure).  Nothing is allocated and nothing is kept from one call for the next.
+ * Strides count values. */
+enum { FFCVB_TYPE_F32 = 0, FFCVB_TYPE_F16 = 1, FFCVB_TYPE_BF16 = 2 };
+
+const char *ffcvb_training_error(void);
+
+/* Cross entropy of logits [rows, classes] and its gradient.  Row i has target probabilities
+ *   T = (1 - smoothing) * P + smoothing / classes,
+ * P being 1 at labels[i]; lambda at the first and 1 - lambda at the second label of a row of LabelMixup
+ * (ffcv/transforms/mixup.py:66-90), added where the two are the same; or given.  With S = sum T
+ *   loss_i = S * lse_i - sum over T > 0 of T * x,   lse_i = log sum exp x,
+ *   grad_i = k_i * (S * exp(x - lse_i) - T),        k_i = scale * upstream / counted rows (mean) or * 1.
+ * Rows with the label ignore_index (has_ignore) give 0 and a gradient of 0 and are not counted; rows whose logits
+ * are all -inf give 0 and a gradient of 0 and are; rows with another label outside 0 .. classes - 1 give NaN.  Where no
+ * row is counted the mean is 0. */
+enum { FFCVB_TARGET_LABELS = 0, FFCVB_TARGET_MIXED = 1, FFCVB_TARGET_SOFT = 2 };
+typedef struct {
+    const void *logits;     /* [rows, classes], neighbouring classes next to one another */
+    const void *target;     /* int64 [rows]; float [rows, 3]: label, label, lambda; or probabilities [rows, classes] */
+    const float *upstream;  /* one factor of the gradient, or one per row (upstream_per_row), or NULL */
+    void *grad;             /* [rows, classes] of the logits' type, or NULL: no gradient */
+    float *loss;            /* one value, the mean or the sum, or NULL */
+    float *row_loss;        /* [rows]: written unless from_stats */
+    float *stats;           /* [rows, 2]: largest logit and 1 / sum exp(x - it); written, or read with from_stats, or NULL */
+    float *counted;         /* one value of workspace; needed with has_ignore and mean */
+    int64_t rows, classes, logits_stride, target_stride, grad_stride, ignore_index;
+    int32_t device, type, target_kind, target_type, has_ignore, mean, upstream_per_row;
+    int32_t from_stats;     /* the gradient alone, with stats of an earlier call */
+    float smoothing, scale;
+} ffcvb_cross_entropy_args;
+int ffcvb_cross_entropy(const ffcvb_cross_entropy_args *args, void *stream);
+
+/* The seam between two blocks of a residual network, on rows of `width` values (at most FFCVB_NORM_MAX_WIDTH):
+ *   u = post(h), or h;   y = x + scale * gate * u;   z = norm(y)
+ * where a norm is (a - mean) / sqrt(var + eps) * weight + bias (layer) or a / sqrt(mean a^2 + eps) * weight (rms), in 32
+ * bits throughout: y is rounded when it is stored, z is made from what it was before.  Without h, y = x and only z is
+ * written; without `norm` only y is.  Weights, biases and scale (per channel) are of param_type or NULL (1, 0, 1);
+ * `number` is one more factor of the branch.  The gate is of the rows' type, one row per row or per `tokens` rows. */
+enum { FFCVB_NORM_NONE = 0, FFCVB_NORM_LAYER = 1, FFCVB_NORM_RMS = 2 };
+enum { FFCVB_GATE_NONE = 0, FFCVB_GATE_SAMPLE = 1, FFCVB_GATE_TOKEN = 2 };
+#define FFCVB_NORM_MAX_WIDTH 16384
+typedef struct {
+    const void *x, *h, *gate;
+    const void *weight, *bias, *post_weight, *post_bias, *scale;
+    float *stats;           /* [rows, 4]: mean and 1 / deviation of y and of h; written forward, read backward */
+    void *y, *z;            /* contiguous; forward only */
+    const void *dy, *dz;    /* gradients of y and z, or NULL: 0; backward only, like the following */
+    void *dx, *dh, *dgate;  /* contiguous, or NULL: not wanted */
+    void *dweight, *dbias, *dpost_weight, *dpost_bias, *dscale; /* of param_type, or NULL */
+    void *workspace;        /* ffcvb_norm_residual_workspace() bytes, 16-byte aligned; backward only */
+    int64_t rows, width, tokens, x_stride, h_stride, gate_stride, dy_stride, dz_stride;
+    int32_t device, type, param_type, norm, post_norm, gate_kind;
+    float eps, number;
+} ffcvb_norm_residual_args;
+int ffcvb_norm_residual(const ffcvb_norm_residual_args *args, void *stream);
+int ffcvb_norm_residual_backward(const ffcvb_norm_residual_args *args, void *stream);
+int64_t ffcvb_norm_residual_workspace(const ffcvb_norm_residual_args *args);
+
+/* Rotary positions: pair i of a head's first rotary_dim values, (a, b), becomes
+ *   amplitude * (a cos t - b sin t, a sin t + b cos t),   t = position * 2 pi * turns[i],
+ * the other values are copied.  Pairs are neighbours (interleaved) or rotary_dim / 2 apart (half).  With two axes
+ * the first half of the pairs turns by the first position of a token and the second half by its second.  `transpose` turns
+ * the other way: the gradient.  Queries [batch, tokens, heads, head_dim] and keys (k NULL: none) go in one
+ * launch; their last dimension lies together, the other strides are free.  out may be in. */
+typedef struct {
+    const void *q, *k;
+    void *q_out, *k_out;
+    const void *positions;  /* int64 or float [batch, tokens, axes], contiguous but for the batch stride (may be 0) */
+    const double *turns;    /* [rotary_dim / 2], per unit of position */
+    int64_t batch, tokens, heads, kv_heads, head_dim, rotary_dim, positions_stride;
+    int64_t q_stride[3], k_stride[3], q_out_stride[3], k_out_stride[3]; /* batch, token, head */
+    int32_t device, type, positions_float, axes, interleaved, transpose;
+    float amplitude;
+    int32_t unused;
+} ffcvb_rotary_args;
+int ffcvb_rotary(const ffcvb_rotary_args *args, void *stream);
+
+/* One AdamW step over many tensors.  In units of FFCVB_ADAMW_BLOCK values, every tensor beginning a unit, the flat
+ * arrays hold the state: moments as float, or (bits = 8) as e4m3 and e5m2 numbers with two float scales per unit; float masters of
+ * 16-bit weights.  With t the tensor's steps, counted from 1 and this one among them,
+ *   g = grad * c;  m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2;
+ *   w = w (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps),
+ * c = 1, or min(1, max_norm / (norm + 1e-6)) with max_norm > 0, norm being that of all gradients; where that is not
+ * finite, nothing is changed.  8-bit moments are rounded stochastically: the numbers come from a hash of seed, t and
+ * a value's place in the flat arrays.  Tensors whose gradient is NULL are left alone. */
+#define FFCVB_ADAMW_BLOCK 256
+typedef struct {
+    double lr, beta1, beta2, eps, weight_decay;
+} ffcvb_adamw_group;
+typedef struct {
+    const void *tensors;    /* DEVICE table that ffcvb_adamw_layout() made */
+    void *exp_avg, *exp_avg_sq;
+    float *scales, *master; /* NULL without */
+    float *norm;            /* one value: the gradients' norm; with max_norm */
+    void *workspace;        /* ffcvb_adamw_layout() says its size; with max_norm */
+    int64_t seed;
+    int32_t device, type, bits, n_tensors;
+    double max_norm;
+} ffcvb_adamw_args;
+/* HOST: for n tensors of numel[i] values, writes start[i], their first values' places in the flat arrays; returns
+ * the flat arrays' length.  sizes[0] is set to the table's bytes, sizes[1] to the workspace's. */
+int64_t ffcvb_adamw_layout(int32_t n, const int64_t *numel, int64_t *start, int64_t *sizes);
+/* HOST: writes the table, to be copied to the device: params[i] is the DEVICE address of tensor i. */
+int ffcvb_adamw_table(int32_t n, const int64_t *numel, const uint64_t *params, void *table);
+/* numel, grads (DEVICE addresses, or 0), steps and group_of are HOST arrays of n_tensors entries; steps[i] of tensors
+ * with a gradient is advanced. */
+int ffcvb_adamw_step(const ffcvb_adamw_args *args, const int64_t *numel, const uint64_t *grads, int64_t *steps,
+                     const int32_t *group_of, const ffcvb_adamw_group *groups, int32_t n_groups, void *stream);
+
 /* ---- decode without allocating -----------------------------------------------------------
  * No counterpart in the reference.  For callers that must not allocate GPU memory while they
  * run: a process that handed all device memory to its own pool at start-up, a plugin living
