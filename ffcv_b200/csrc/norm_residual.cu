@@ -7,6 +7,7 @@
 // again from x and h, in 32 bits: its rounded copy would cost the weights' gradients their last digits.
 // Sums over columns of the gradient go through one partial row per CTA, added up in a fixed order by a second kernel.
 #include "training.h"
+#include "two.h"
 
 namespace ffcvb {
 
@@ -16,62 +17,132 @@ using Args = ffcvb_norm_residual_args;
 
 template <int V> struct Int { static constexpr int value = V; };
 
-// N parameters from column `at` on, which is inside the row; `otherwise` without any.
-template <int N>
-__device__ __forceinline__ void load_params(float (&v)[N], const void *p, int type, int at, float otherwise) {
-    if (!p) {
+// A thread's part of a row: eight columns, as 8 / N packs of N; the packs of all threads of a row lie next to one another.
+// Arithmetic is on pairs of them.
+constexpr int kPairs = 4;
+using Eight = Two[kPairs];
+
+template <int N, bool MULTI> struct Columns {
+    int first, step, width;
+    __device__ __forceinline__ Columns(long long w, int ctas, int rank) : width((int)w) {
+        first = (MULTI ? rank * blockDim.x + threadIdx.x : threadIdx.x) * N;
+        step = (MULTI ? ctas * blockDim.x : 32) * N;
+    }
+    __device__ __forceinline__ int at(int k) const { return first + k * step; }
+    __device__ __forceinline__ bool in(int k) const { return at(k) < width; } // (a pack is inside the row or not)
+};
+
+__device__ __forceinline__ void fill(Eight &v, float value) {
 #pragma unroll
-        for (int j = 0; j < N; j++) v[j] = otherwise;
-    } else if constexpr (N == 1) {
-        v[0] = type == FFCVB_TYPE_F32 ? static_cast<const float *>(p)[at]
-               : type == FFCVB_TYPE_F16 ? to_float(static_cast<const __half *>(p)[at])
-                                        : to_float(static_cast<const __nv_bfloat16 *>(p)[at]);
-    } else if (type == FFCVB_TYPE_F32) {
+    for (int p = 0; p < kPairs; p++) v[p] = Two(value, value);
+}
+template <typename T, int N>
+__device__ __forceinline__ void to_pairs(Eight &v, const Pack<T, N> (&packs)[8 / N]) {
+    float f[8];
 #pragma unroll
-        for (int j = 0; j < N; j += 4)
-            *reinterpret_cast<float4 *>(v + j) = *reinterpret_cast<const float4 *>(static_cast<const float *>(p) + at + j);
-    } else {
-        uint32_t w[N / 2];
+    for (int k = 0; k < 8 / N; k++) packs[k].get(*reinterpret_cast<float(*)[N]>(f + k * N));
 #pragma unroll
-        for (int j = 0; j < N / 2; j += 2)
-            *reinterpret_cast<uint2 *>(w + j) = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(p) + at + 2 * j);
+    for (int p = 0; p < kPairs; p++) v[p] = Two(f[2 * p], f[2 * p + 1]);
+}
+// Columns of a row in global memory; 0 beyond it.
+template <typename T, int N, bool MULTI>
+__device__ __forceinline__ void load_row(Eight &v, const void *p, long long offset, const Columns<N, MULTI> &c) {
+    Pack<T, N> packs[8 / N] = {};
 #pragma unroll
-        for (int j = 0; j < N / 2; j++) {
-            const float2 two = type == FFCVB_TYPE_F16 ? __half22float2(*reinterpret_cast<const __half2 *>(w + j))
-                                                      : make_float2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u));
-            v[2 * j] = two.x;
-            v[2 * j + 1] = two.y;
+    for (int k = 0; k < 8 / N; k++)
+        if (p && c.in(k)) packs[k].load(static_cast<const T *>(p) + offset + c.at(k));
+    to_pairs<T, N>(v, packs);
+}
+template <typename T, int N, bool MULTI>
+__device__ __forceinline__ void store_row(const Eight &v, void *p, long long offset, const Columns<N, MULTI> &c) {
+    float f[8];
+#pragma unroll
+    for (int q = 0; q < kPairs; q++) {
+        f[2 * q] = v[q].lo();
+        f[2 * q + 1] = v[q].hi();
+    }
+#pragma unroll
+    for (int k = 0; k < 8 / N; k++)
+        if (c.in(k)) {
+            Pack<T, N> pack;
+            pack.set(*reinterpret_cast<const float(*)[N]>(f + k * N));
+            pack.store(static_cast<T *>(p) + offset + c.at(k));
+        }
+}
+// Parameters of the columns; `otherwise` without any, `beyond` beyond the row.
+template <int N, bool MULTI>
+__device__ __forceinline__ void load_params(Eight &v, const void *p, int type, const Columns<N, MULTI> &c, float otherwise, float beyond) {
+    float f[8];
+#pragma unroll
+    for (int k = 0; k < 8 / N; k++) {
+#pragma unroll
+        for (int j = 0; j < N; j++) f[k * N + j] = c.in(k) ? otherwise : beyond;
+        if (!p || !c.in(k)) continue;
+        const int at = c.at(k);
+        if constexpr (N == 1) {
+            f[k] = type == FFCVB_TYPE_F32 ? static_cast<const float *>(p)[at]
+                   : type == FFCVB_TYPE_F16 ? to_float(static_cast<const __half *>(p)[at])
+                                            : to_float(static_cast<const __nv_bfloat16 *>(p)[at]);
+        } else if (type == FFCVB_TYPE_F32) {
+#pragma unroll
+            for (int j = 0; j < N; j += 4) {
+                const float4 w = *reinterpret_cast<const float4 *>(static_cast<const float *>(p) + at + j);
+                f[k * N + j] = w.x, f[k * N + j + 1] = w.y, f[k * N + j + 2] = w.z, f[k * N + j + 3] = w.w;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; j += 4) {
+                const uint2 w = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(p) + at + j);
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const uint32_t u = i ? w.y : w.x;
+                    const float2 two = type == FFCVB_TYPE_F16 ? __half22float2(*reinterpret_cast<const __half2 *>(&u))
+                                                              : make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+                    f[k * N + j + 2 * i] = two.x;
+                    f[k * N + j + 2 * i + 1] = two.y;
+                }
+            }
         }
     }
+#pragma unroll
+    for (int q = 0; q < kPairs; q++) v[q] = Two(f[2 * q], f[2 * q + 1]);
+}
+template <int N, bool MULTI>
+__device__ __forceinline__ void store_floats(const Eight &v, float *to, const Columns<N, MULTI> &c) {
+#pragma unroll
+    for (int k = 0; k < 8 / N; k++)
+        if (c.in(k)) {
+#pragma unroll
+            for (int j = 0; j < N; j++) to[c.at(k) + j] = v[(k * N + j) / 2].half((k * N + j) & 1);
+        }
 }
 
-// Sums over the threads of a row: a warp, a CTA, or (wide rows, backward) the CTAs of a cluster, whose sums travel through
-// distributed shared memory.  Consecutive sums use `s` in turn, so that one barrier is enough.
+// Two sums over the threads of a row: a warp, a CTA, or (wide rows) the CTAs of a cluster, whose sums travel through distributed
+// shared memory.  In a warp the halves exchange what they do not go on with, so that two sums take little more than one.
+// Consecutive sums use `s`, zero at the start, in turn, so that one barrier is enough.
 template <bool MULTI> struct RowSum {
     float2 *s; // [2][32 + 4]
-    int ctas = 1;
+    int ctas;
     int turn = 0;
-    __device__ __forceinline__ float operator()(float a) { return (*this)(make_float2(a, 0.0f), false).x; }
-    __device__ __forceinline__ float2 operator()(float2 v, bool both = true) {
-        v.x = warp_sum(v.x);
-        if (both) v.y = warp_sum(v.y);
-        if constexpr (MULTI) {
-            const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
+    __device__ __forceinline__ float2 operator()(float a, float b) {
+        const int lane = threadIdx.x & 31;
+        float v = lane & 16 ? b : a;
+        v += __shfl_xor_sync(0xffffffffu, lane & 16 ? a : b, 16);
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        if constexpr (!MULTI) {
+            return make_float2(__shfl_sync(0xffffffffu, v, 0), __shfl_sync(0xffffffffu, v, 16));
+        } else {
+            const int warps = blockDim.x >> 5;
             float2 *to = s + turn * 36;
             turn ^= 1;
-            if (lane == 0) to[threadIdx.x >> 5] = v;
+            if ((lane & 15) == 0) reinterpret_cast<float *>(to + (threadIdx.x >> 5))[lane >> 4] = v;
             __syncthreads();
-            if (warps <= 8) {
-                v = to[0];
-                for (int k = 1; k < warps; k++) {
-                    const float2 w = to[k];
-                    v.x += w.x;
-                    v.y += w.y;
-                }
-            } else {
-                v = lane < warps ? to[lane] : make_float2(0.0f, 0.0f);
-                v.x = warp_sum(v.x);
-                if (both) v.y = warp_sum(v.y);
+            float2 r = make_float2(0.0f, 0.0f);
+            for (int k = 0; k < warps; k += 2) {
+                const float4 w = *reinterpret_cast<const float4 *>(to + k);
+                r.x += w.x + w.z;
+                r.y += w.y + w.w;
             }
             if (ctas > 1) {
                 if ((int)threadIdx.x < ctas) {
@@ -79,31 +150,38 @@ template <bool MULTI> struct RowSum {
                     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
                     mine = (uint32_t)__cvta_generic_to_shared(to + 32 + rank);
                     asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(mine), "r"(threadIdx.x));
-                    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(there), "f"(v.x), "f"(v.y) : "memory");
+                    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(there), "f"(r.x), "f"(r.y) : "memory");
                 }
-                asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-                v = to[32];
+                cluster_barrier();
+                r = to[32];
                 for (int k = 1; k < ctas; k++) {
                     const float2 w = to[32 + k];
-                    v.x += w.x;
-                    v.y += w.y;
+                    r.x += w.x;
+                    r.y += w.y;
                 }
             }
+            return r;
         }
-        return v;
+    }
+    static __device__ __forceinline__ void cluster_barrier() {
+        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    }
+    // (all of a cluster's CTAs have begun before one writes into another's memory)
+    __device__ __forceinline__ void begin() {
+        if constexpr (MULTI) {
+            for (int k = threadIdx.x; k < 72; k += blockDim.x) s[k] = make_float2(0.0f, 0.0f);
+            __syncthreads();
+            if (ctas > 1) cluster_barrier();
+        }
     }
 };
 
-// A thread's columns: VPT packs of N, the packs of all threads of a row next to one another.
-template <int N, int VPT, bool MULTI> struct Columns {
-    int first, step, width;
-    __device__ __forceinline__ Columns(long long w, int ctas = 1, int rank = 0) : width((int)w) {
-        first = (MULTI ? rank * blockDim.x + threadIdx.x : threadIdx.x & 31) * N;
-        step = (MULTI ? ctas * blockDim.x : 32) * N;
-    }
-    __device__ __forceinline__ int at(int k) const { return first + k * step; }
-    __device__ __forceinline__ bool in(int k) const { return at(k) < width; } // (a pack is inside the row or not)
-};
+__device__ __forceinline__ float sum_of(const Eight &v) {
+    Two a = v[0];
+#pragma unroll
+    for (int p = 1; p < kPairs; p++) a = add_rn(a, v[p]);
+    return a.lo() + a.hi();
+}
 
 // Packs of coming rows on their way into shared memory, every thread's in places of its own, so that it waits for nobody
 // else's.  Slots are used in turn.
@@ -111,7 +189,7 @@ __device__ __forceinline__ void copy16(void *to, const void *from) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
 }
 __device__ __forceinline__ void copies_made() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void copies_wait(int ahead) { // for the oldest of `ahead` (1 to 3) rows
+__device__ __forceinline__ void copies_wait(int ahead) { // for the oldest of `ahead` (1 to 3) rounds
     if (ahead == 3)
         asm volatile("cp.async.wait_group 2;" ::: "memory");
     else if (ahead == 2)
@@ -119,180 +197,200 @@ __device__ __forceinline__ void copies_wait(int ahead) { // for the oldest of `a
     else
         asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
-// As many rows ahead, at most `most`, as shared memory has room for: it is shared by a CTA of 16 warps, or by CTAs of together as many.
-constexpr size_t kRoom = 208 * 1024;
-int rows_ahead(int most, size_t per_thread, size_t besides) {
-    while (most > 1 && 512 * (most * per_thread + besides) > kRoom) most--;
-    return most;
+// A thread's packs of one stream in a slot.
+template <typename T, int N, bool MULTI>
+__device__ __forceinline__ void copy_packs(uint4 *&to, const void *from, long long offset, const Columns<N, MULTI> &c) {
+#pragma unroll
+    for (int k = 0; k < 8 / N; k++)
+        if (c.in(k)) copy16(to + k * blockDim.x, static_cast<const T *>(from) + offset + c.at(k));
+    to += 8 / N * blockDim.x;
+}
+template <typename T, int N, bool MULTI>
+__device__ __forceinline__ void copied(Eight &v, const uint4 *&from, const Columns<N, MULTI> &c) {
+    Pack<T, N> packs[8 / N] = {};
+#pragma unroll
+    for (int k = 0; k < 8 / N; k++)
+        if (c.in(k)) packs[k].raw = from[k * blockDim.x];
+    to_pairs<T, N>(v, packs);
+    from += 8 / N * blockDim.x;
 }
 
-template <typename T, int N, int VPT, bool MULTI>
-__device__ __forceinline__ void load_packs(Pack<T, N> (&v)[VPT], const void *p, long long offset, const Columns<N, VPT, MULTI> &c) {
-#pragma unroll
-    for (int k = 0; k < VPT; k++)
-        if (c.in(k)) v[k].load(static_cast<const T *>(p) + offset + c.at(k));
-}
-// Values of packs, 0 beyond the row.
-template <typename T, int N, int VPT, bool MULTI>
-__device__ __forceinline__ void unpack(float (&v)[VPT][N], const Pack<T, N> (&p)[VPT], const Columns<N, VPT, MULTI> &c) {
-#pragma unroll
-    for (int k = 0; k < VPT; k++) {
-        p[k].get(v[k]);
-        if (!c.in(k)) {
-#pragma unroll
-            for (int j = 0; j < N; j++) v[k][j] = 0.0f;
-        }
-    }
-}
-template <typename T, int N, int VPT, bool MULTI>
-__device__ __forceinline__ void load_row(float (&v)[VPT][N], const void *p, long long offset, const Columns<N, VPT, MULTI> &c) {
-    Pack<T, N> raw[VPT];
-    load_packs<T, N, VPT, MULTI>(raw, p, offset, c);
-    unpack<T, N, VPT, MULTI>(v, raw, c);
-}
-template <typename T, int N, int VPT, bool MULTI>
-__device__ __forceinline__ void store_row(const float (&v)[VPT][N], void *p, long long offset, const Columns<N, VPT, MULTI> &c) {
-#pragma unroll
-    for (int k = 0; k < VPT; k++)
-        if (c.in(k)) {
-            Pack<T, N> pack;
-            pack.set(v[k]);
-            pack.store(static_cast<T *>(p) + offset + c.at(k));
-        }
-}
+// How rows are shared out: threads of a CTA, CTAs of a cluster, clusters; streams that are copied ahead and for how many rounds.
+struct Shape {
+    int threads, ctas_per_row, rows_at_once;
+    int streams, ahead;
+};
 
-// Mean (0 for rms) and 1 / deviation of a row: the mean first, then the squares of what is left.
-template <int N, int VPT, bool MULTI>
-__device__ __forceinline__ float2 row_stats(const float (&v)[VPT][N], int kind, const Columns<N, VPT, MULTI> &c, float eps, RowSum<MULTI> &sum) {
+// Means and 1 / deviations of two rows: the means first (0 for rms), then the squares of what is left.
+template <int N, bool MULTI>
+__device__ __forceinline__ void two_stats(const Eight (&v)[2], int kind, const Columns<N, MULTI> &c, float eps, RowSum<MULTI> &sum, float (&mean)[2], float (&r)[2]) {
     const float over = 1.0f / (float)c.width;
-    float mean = 0.0f;
+    mean[0] = mean[1] = 0.0f;
     if (kind == FFCVB_NORM_LAYER) {
-        float a = 0.0f;
-#pragma unroll
-        for (int k = 0; k < VPT; k++)
-#pragma unroll
-            for (int j = 0; j < N; j++) a += v[k][j];
-        mean = sum(a) * over;
+        const float2 both = sum(sum_of(v[0]), sum_of(v[1]));
+        mean[0] = both.x * over;
+        mean[1] = both.y * over;
     }
-    float q = 0.0f;
+    float q[2];
 #pragma unroll
-    for (int k = 0; k < VPT; k++)
-        if (c.in(k)) {
+    for (int i = 0; i < 2; i++) {
+        const Two m(-mean[i], -mean[i]);
+        Eight d;
 #pragma unroll
-            for (int j = 0; j < N; j++) q += (v[k][j] - mean) * (v[k][j] - mean);
+        for (int p = 0; p < kPairs; p++) {
+            d[p] = add_rn(v[i][p], m);
+            d[p] = mul_rn(d[p], d[p]);
+            if constexpr (N == 1)
+                d[p] = Two(c.in(2 * p) ? d[p].lo() : 0.0f, c.in(2 * p + 1) ? d[p].hi() : 0.0f);
+            else if (!c.in(2 * p / N))
+                d[p] = Two(0.0f, 0.0f);
         }
-    return make_float2(mean, rsqrtf(sum(q) * over + eps));
+        q[i] = sum_of(d);
+    }
+    const float2 both = sum(q[0], q[1]);
+    r[0] = rsqrtf(both.x * over + eps);
+    r[1] = rsqrtf(both.y * over + eps);
+}
+// (v - mean) r
+__device__ __forceinline__ void normalise(Eight &v, float mean, float r) {
+    const Two rr(r, r), m(-mean, -mean);
+#pragma unroll
+    for (int p = 0; p < kPairs; p++) v[p] = mul_rn(add_rn(v[p], m), rr);
 }
 
-// A row per warp, or (MULTI) per CTA.  Packs of more than one value need rows of a multiple of N values on 16-byte boundaries; the
-// next rows of x and h (two, where there is room) are then on their way while one is worked on.
-template <typename T, int N, int VPT, bool MULTI>
-__global__ void __launch_bounds__(MULTI ? 512 : 128, MULTI ? 1 : 4)
-forward_kernel(const __grid_constant__ Args a, const int ahead) {
+// Two rows per CTA (or cluster, or warp) at a time, so that the sums of both take one barrier; with packs of 16 bytes those of the next
+// rounds are on their way meanwhile.  POST: with an inner norm.
+template <typename T, int N, bool MULTI, bool POST>
+__global__ void __launch_bounds__(MULTI ? 512 : 32, MULTI ? 1 : 16)
+forward_kernel(const __grid_constant__ Args a, const Shape shape) {
     constexpr bool RING = N > 1;
-    __shared__ float2 s_sum[72];
-    extern __shared__ uint4 s_ring[]; // [ahead][2][VPT][threads]
-    RowSum<MULTI> sum{s_sum};
-    const Columns<N, VPT, MULTI> c(a.width);
-    const long long step = MULTI ? gridDim.x : gridDim.x * 4ll;
-    const long long begin = MULTI ? blockIdx.x : blockIdx.x * 4ll + (threadIdx.x >> 5);
-    uint4 *const mine = s_ring + threadIdx.x;
-    auto fetch = [&](long long row, int slot) {
-        if (row < a.rows) {
+    __shared__ __align__(16) float2 s_sum[72];
+    extern __shared__ uint4 s_ring[]; // [ahead][2][streams][8 / N][threads]
+    int rank = 0, cluster = blockIdx.x;
+    if (MULTI && shape.ctas_per_row > 1) {
+        rank = blockIdx.x % shape.ctas_per_row;
+        cluster = blockIdx.x / shape.ctas_per_row;
+    }
+    RowSum<MULTI> sum{s_sum, shape.ctas_per_row};
+    sum.begin();
+    const Columns<N, MULTI> c(a.width, shape.ctas_per_row, rank);
+    Eight w, b, f, pw, pb; // (f is 0 beyond the row, which keeps y 0 there)
+    load_params(w, a.weight, a.param_type, c, 1.0f, 1.0f);
+    load_params(b, a.bias, a.param_type, c, 0.0f, 0.0f);
+    load_params(f, a.scale, a.param_type, c, 1.0f, 0.0f);
+    if (POST) {
+        load_params(pw, a.post_weight, a.param_type, c, 1.0f, 1.0f);
+        load_params(pb, a.post_bias, a.param_type, c, 0.0f, 0.0f);
+    }
 #pragma unroll
-            for (int k = 0; k < VPT; k++)
-                if (c.in(k)) {
-                    copy16(mine + (slot * 2 * VPT + k) * blockDim.x, static_cast<const T *>(a.x) + row * a.x_stride + c.at(k));
-                    if (a.h) copy16(mine + (slot * 2 * VPT + VPT + k) * blockDim.x, static_cast<const T *>(a.h) + row * a.h_stride + c.at(k));
-                }
+    for (int p = 0; p < kPairs; p++) f[p] = mul_rn(f[p], Two(a.number, a.number));
+    const bool gated = a.gate_kind != FFCVB_GATE_NONE, per_sample = a.gate_kind == FFCVB_GATE_SAMPLE;
+    const long long step = 2ll * shape.rows_at_once, begin = 2ll * cluster;
+    // the sample of the next row to be fetched, and the row's place in it
+    long long next_sample = per_sample ? begin / a.tokens : 0, next_place = per_sample ? begin % a.tokens : 0;
+    const long long sample_step = per_sample ? step / a.tokens : 0, place_step = per_sample ? step % a.tokens : 0;
+    uint4 *const mine = s_ring + threadIdx.x;
+    const int slot_size = 2 * shape.streams * (8 / N) * blockDim.x;
+    auto gate_row = [&](long long row, int i) { return per_sample ? next_sample + (i && next_place + 1 == a.tokens) : row + i; };
+    auto fetched = [&]() {
+        if (!per_sample) return;
+        next_sample += sample_step;
+        next_place += place_step;
+        if (next_place >= a.tokens) {
+            next_place -= a.tokens;
+            next_sample++;
         }
+    };
+    auto fetch = [&](long long row, int slot) {
+        uint4 *to = mine + slot * slot_size;
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+            if (row + i < a.rows) {
+                copy_packs<T>(to, a.x, (row + i) * a.x_stride, c);
+                if (a.h) copy_packs<T>(to, a.h, (row + i) * a.h_stride, c);
+                if (gated) copy_packs<T>(to, a.gate, gate_row(row, i) * a.gate_stride, c);
+            }
         copies_made();
+        fetched();
     };
     if constexpr (RING)
-        for (int k = 0; k < ahead; k++) fetch(begin + k * step, k);
+        for (int k = 0; k < shape.ahead; k++) fetch(begin + k * step, k);
     int slot = 0;
     for (long long row = begin; row < a.rows; row += step) {
-        float y[VPT][N];
-        float4 stats = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        Pack<T, N> raw[VPT], raw_h[VPT];
+        const int rows = row + 1 < a.rows ? 2 : 1;
+        Eight y[2], u[2], g[2];
+        float4 stats[2] = {};
         if constexpr (RING) {
-            copies_wait(ahead);
+            copies_wait(shape.ahead);
+            const uint4 *from = mine + slot * slot_size;
 #pragma unroll
-            for (int k = 0; k < VPT; k++)
-                if (c.in(k)) {
-                    raw[k].raw = mine[(slot * 2 * VPT + k) * blockDim.x];
-                    if (a.h) raw_h[k].raw = mine[(slot * 2 * VPT + VPT + k) * blockDim.x];
-                }
-            fetch(row + ahead * step, slot);
-            slot = slot + 1 == ahead ? 0 : slot + 1;
+            for (int i = 0; i < 2; i++) {
+                if (i == 1 && rows == 1) from = mine + slot * slot_size; // (the same row again, to no effect)
+                copied<T>(y[i], from, c);
+                if (a.h) copied<T>(u[i], from, c);
+                if (gated) copied<T>(g[i], from, c);
+            }
+            fetch(row + shape.ahead * step, slot);
+            slot = slot + 1 == shape.ahead ? 0 : slot + 1;
         } else {
-            load_packs<T, N, VPT, MULTI>(raw, a.x, row * a.x_stride, c);
-            if (a.h) load_packs<T, N, VPT, MULTI>(raw_h, a.h, row * a.h_stride, c);
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const int k = i < rows ? i : 0;
+                load_row<T>(y[i], a.x, (row + k) * a.x_stride, c);
+                if (a.h) load_row<T>(u[i], a.h, (row + k) * a.h_stride, c);
+                if (gated) load_row<T>(g[i], a.gate, gate_row(row, k) * a.gate_stride, c);
+            }
+            fetched();
         }
         if (a.h) {
-            float u[VPT][N];
-            unpack<T, N, VPT, MULTI>(u, raw_h, c);
-            if (a.post_norm != FFCVB_NORM_NONE) {
-                const float2 inner = row_stats<N, VPT, MULTI>(u, a.post_norm, c, a.eps, sum);
-                stats.z = inner.x;
-                stats.w = inner.y;
+            if (POST) {
+                float mean[2], r[2];
+                two_stats<N, MULTI>(u, a.post_norm, c, a.eps, sum, mean, r);
 #pragma unroll
-                for (int k = 0; k < VPT; k++)
-                    if (c.in(k)) {
-                        float w[N], b[N];
-                        load_params<N>(w, a.post_weight, a.param_type, c.at(k), 1.0f);
-                        load_params<N>(b, a.post_bias, a.param_type, c.at(k), 0.0f);
+                for (int i = 0; i < 2; i++) {
+                    stats[i].z = mean[i];
+                    stats[i].w = r[i];
+                    normalise(u[i], mean[i], r[i]);
 #pragma unroll
-                        for (int j = 0; j < N; j++) u[k][j] = (u[k][j] - inner.x) * inner.y * w[j] + b[j];
-                    }
-            }
-            if (a.gate_kind != FFCVB_GATE_NONE) {
-                float gate[VPT][N];
-                load_row<T, N, VPT, MULTI>(gate, a.gate, (a.gate_kind == FFCVB_GATE_SAMPLE ? row / a.tokens : row) * a.gate_stride, c);
-#pragma unroll
-                for (int k = 0; k < VPT; k++)
-#pragma unroll
-                    for (int j = 0; j < N; j++) u[k][j] *= gate[k][j];
-            }
-            unpack<T, N, VPT, MULTI>(y, raw, c);
-#pragma unroll
-            for (int k = 0; k < VPT; k++)
-                if (c.in(k)) {
-                    float f[N];
-                    load_params<N>(f, a.scale, a.param_type, c.at(k), 1.0f);
-#pragma unroll
-                    for (int j = 0; j < N; j++) y[k][j] += u[k][j] * (a.number * f[j]);
+                    for (int p = 0; p < kPairs; p++) u[i][p] = fma_rn(u[i][p], pw[p], pb[p]);
                 }
-            store_row<T, N, VPT, MULTI>(y, a.y, row * a.width, c);
-        } else {
-            unpack<T, N, VPT, MULTI>(y, raw, c);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                if (gated)
+#pragma unroll
+                    for (int p = 0; p < kPairs; p++) u[i][p] = mul_rn(u[i][p], g[i][p]);
+#pragma unroll
+                for (int p = 0; p < kPairs; p++) y[i][p] = fma_rn(u[i][p], f[p], y[i][p]);
+                if (i < rows) store_row<T>(y[i], a.y, (row + i) * a.width, c);
+            }
         }
         if (a.norm != FFCVB_NORM_NONE) {
-            const float2 outer = row_stats<N, VPT, MULTI>(y, a.norm, c, a.eps, sum);
-            stats.x = outer.x;
-            stats.y = outer.y;
+            float mean[2], r[2];
+            two_stats<N, MULTI>(y, a.norm, c, a.eps, sum, mean, r);
 #pragma unroll
-            for (int k = 0; k < VPT; k++)
-                if (c.in(k)) {
-                    float w[N], b[N];
-                    load_params<N>(w, a.weight, a.param_type, c.at(k), 1.0f);
-                    load_params<N>(b, a.bias, a.param_type, c.at(k), 0.0f);
+            for (int i = 0; i < 2; i++) {
+                stats[i].x = mean[i];
+                stats[i].y = r[i];
+                normalise(y[i], mean[i], r[i]);
 #pragma unroll
-                    for (int j = 0; j < N; j++) y[k][j] = (y[k][j] - outer.x) * outer.y * w[j] + b[j];
-                }
-            store_row<T, N, VPT, MULTI>(y, a.z, row * a.width, c);
+                for (int p = 0; p < kPairs; p++) y[i][p] = fma_rn(y[i][p], w[p], b[p]);
+                if (i < rows) store_row<T>(y[i], a.z, (row + i) * a.width, c);
+            }
         }
-        if (a.stats && c.first == 0) reinterpret_cast<float4 *>(a.stats)[row] = stats;
+        if (c.first == 0) {
+            reinterpret_cast<float4 *>(a.stats)[row] = stats[0];
+            if (rows == 2) reinterpret_cast<float4 *>(a.stats)[row + 1] = stats[1];
+        }
     }
 }
 
 // How the backward pass deals its rows out.  A unit is a run of rows of one sample (with a gate per sample, whose
 // gradient is a sum over them) or of all rows.
 struct Deal {
+    Shape shape;
     long long samples, tokens, splits, units;
-    int threads, ctas_per_row, rows_at_once; // of a CTA; a cluster's CTAs; clusters
-    int columns;                             // column sums of each cluster: weight, bias, post_weight, post_bias, scale
-    int streams, ahead;                      // that are read; rows of them that are on their way (packs of 16 bytes)
+    int columns; // column sums of each cluster: weight, bias, post_weight, post_bias, scale
 };
 // Partial rows: [rows_at_once][columns][width] of the column sums, then [units][width] of the gate's with more than one split.
 struct Partials {
@@ -301,234 +399,204 @@ struct Partials {
 
 constexpr int kColumns = 5;
 
-template <int N, int VPT, bool MULTI>
-__device__ __forceinline__ void store_floats(const float (&v)[VPT][N], float *to, const Columns<N, VPT, MULTI> &c) {
-#pragma unroll
-    for (int k = 0; k < VPT; k++)
-        if (c.in(k)) {
-#pragma unroll
-            for (int j = 0; j < N; j++) to[c.at(k) + j] = v[k][j];
-        }
-}
-
-// One row per CTA, or per cluster, at a time; with packs of 16 bytes those of the next are on their way meanwhile.
+// One row per CTA (or cluster, or warp) at a time; with packs of 16 bytes those of the next are on their way meanwhile.
 // POST: with an inner norm.  Of the branch's side two sums are kept per column and unit, A = sum t u and B = sum t (t with the gate,
 // if it is one per token), u without weight and bias: all other gradients are made of them at a unit's end,
 //   gate: f (pw A + pb B);  times the sample's gate:  scale: pw A + pb B,  post_weight: f A,  post_bias: f B.
-template <typename T, int N, int VPT, bool MULTI, bool POST>
+template <typename T, int N, bool MULTI, bool POST>
 __global__ void __launch_bounds__(MULTI ? 512 : 32, MULTI ? 1 : 16)
 backward_kernel(const __grid_constant__ Args a, const Deal deal, const Partials part) {
     constexpr bool RING = N > 1;
-    __shared__ float2 s_sum[72];
-    extern __shared__ uint4 s_ring[]; // [deal.ahead][deal.streams][VPT][threads], then floats [3][VPT * N][threads]: see below
+    const Shape &shape = deal.shape;
+    __shared__ __align__(16) float2 s_sum[72];
+    extern __shared__ uint4 s_ring[]; // [ahead][streams][8 / N][threads], then floats [8][3][threads]: see below
     int rank = 0, cluster = blockIdx.x;
-    if (MULTI && deal.ctas_per_row > 1) {
-        rank = blockIdx.x % deal.ctas_per_row;
-        cluster = blockIdx.x / deal.ctas_per_row;
+    if (MULTI && shape.ctas_per_row > 1) {
+        rank = blockIdx.x % shape.ctas_per_row;
+        cluster = blockIdx.x / shape.ctas_per_row;
     }
-    RowSum<MULTI> sum{s_sum, deal.ctas_per_row};
-    const Columns<N, VPT, MULTI> c(a.width, deal.ctas_per_row, rank);
+    RowSum<MULTI> sum{s_sum, shape.ctas_per_row};
+    sum.begin();
+    const Columns<N, MULTI> c(a.width, shape.ctas_per_row, rank);
     const float over = 1.0f / (float)a.width;
-    const bool per_sample = a.gate_kind == FFCVB_GATE_SAMPLE;
+    const bool per_sample = a.gate_kind == FFCVB_GATE_SAMPLE, per_token = a.gate_kind == FFCVB_GATE_TOKEN;
+    const int slot_size = shape.streams * (8 / N) * blockDim.x;
     // with a gate per sample the sums over units are kept here, the thread's own
-    float *const kept = reinterpret_cast<float *>(s_ring + (RING ? deal.ahead * deal.streams * VPT * blockDim.x : 0)) + threadIdx.x;
+    float *const kept = reinterpret_cast<float *>(s_ring + (RING ? shape.ahead * slot_size : 0)) + threadIdx.x;
     if (per_sample)
-        for (int k = 0; k < 3 * VPT * N; k++) kept[k * blockDim.x] = 0.0f;
-    float dw[VPT][N] = {}, db[VPT][N] = {}, sa[VPT][N] = {}, sb[VPT][N] = {};
-    float w[VPT][N], f[VPT][N];
+        for (int k = 0; k < 24; k++) kept[k * blockDim.x] = 0.0f;
+    Eight dw, db, sa, sb, w, f; // f: with the sample's gate; 0 beyond the row, which keeps everything of the branch 0 there
+    fill(dw, 0.0f);
+    fill(db, 0.0f);
+    fill(sa, 0.0f);
+    fill(sb, 0.0f);
+    load_params(w, a.weight, a.param_type, c, 1.0f, 0.0f);
+    auto load_f = [&]() {
+        load_params(f, a.scale, a.param_type, c, 1.0f, 0.0f);
 #pragma unroll
-    for (int k = 0; k < VPT; k++) {
-        const int at = c.in(k) ? c.at(k) : 0;
-        load_params<N>(w[k], a.weight, a.param_type, at, 1.0f);
-        load_params<N>(f[k], a.scale, a.param_type, at, 1.0f);
-#pragma unroll
-        for (int j = 0; j < N; j++) f[k][j] *= a.number;
-    }
+        for (int p = 0; p < kPairs; p++) f[p] = mul_rn(f[p], Two(a.number, a.number));
+    };
+    load_f();
     uint4 *const mine = s_ring + threadIdx.x;
-    if (MULTI && deal.ctas_per_row > 1) // (all of a cluster's CTAs have begun before one writes into another's memory)
-        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-    for (long long unit = cluster; unit < deal.units; unit += deal.rows_at_once) {
+    for (long long unit = cluster; unit < deal.units; unit += shape.rows_at_once) {
         const long long sample = unit / deal.splits, split = unit % deal.splits;
         const long long begin = sample * deal.tokens + deal.tokens * split / deal.splits;
         const long long end = sample * deal.tokens + deal.tokens * (split + 1) / deal.splits;
-        float gate[VPT][N];
+        if (per_sample) {
+            Eight gate;
+            load_f();
+            load_row<T>(gate, a.gate, sample * a.gate_stride, c);
 #pragma unroll
-        for (int k = 0; k < VPT; k++)
-#pragma unroll
-            for (int j = 0; j < N; j++) gate[k][j] = 1.0f;
-        if (per_sample) load_row<T, N, VPT, MULTI>(gate, a.gate, sample * a.gate_stride, c);
+            for (int p = 0; p < kPairs; p++) f[p] = mul_rn(f[p], gate[p]);
+        }
         auto fetch = [&](long long row, int slot) {
             if (row < end) {
-                uint4 *to = mine + slot * deal.streams * VPT * blockDim.x;
-                auto one = [&](const void *from, long long stride) {
-                    if (!from) return;
-#pragma unroll
-                    for (int k = 0; k < VPT; k++)
-                        if (c.in(k)) copy16(to + k * blockDim.x, static_cast<const T *>(from) + row * stride + c.at(k));
-                    to += VPT * blockDim.x;
-                };
-                one(a.x, a.x_stride);
-                one(a.h, a.h_stride);
-                one(a.dy, a.dy_stride);
-                one(a.dz, a.dz_stride);
-                if (a.gate_kind == FFCVB_GATE_TOKEN) one(a.gate, a.gate_stride);
+                uint4 *to = mine + slot * slot_size;
+                copy_packs<T>(to, a.x, row * a.x_stride, c);
+                if (a.h) copy_packs<T>(to, a.h, row * a.h_stride, c);
+                if (a.dy) copy_packs<T>(to, a.dy, row * a.dy_stride, c);
+                if (a.dz) copy_packs<T>(to, a.dz, row * a.dz_stride, c);
+                if (per_token) copy_packs<T>(to, a.gate, row * a.gate_stride, c);
             }
             copies_made();
         };
         if constexpr (RING)
-            for (int k = 0; k < deal.ahead; k++) fetch(begin + k, k);
+            for (int k = 0; k < shape.ahead; k++) fetch(begin + k, k);
+        float4 next = {};
+        if (begin < end) next = reinterpret_cast<const float4 *>(a.stats)[begin];
         int slot = 0;
         for (long long row = begin; row < end; row++) {
-            float y[VPT][N], u[VPT][N], t[VPT][N], dz[VPT][N];
-            const float4 stats = reinterpret_cast<const float4 *>(a.stats)[row];
+            Eight y, u, t, dz, gate;
+            const float4 stats = next;
+            if (row + 1 < end) next = reinterpret_cast<const float4 *>(a.stats)[row + 1];
+            fill(u, 0.0f);
+            fill(t, 0.0f);
+            fill(dz, 0.0f);
             if constexpr (RING) {
-                copies_wait(deal.ahead);
-                const uint4 *from = mine + slot * deal.streams * VPT * blockDim.x;
-                auto one = [&](float(&v)[VPT][N], const void *there) {
-                    Pack<T, N> raw[VPT] = {};
-                    if (there) {
-#pragma unroll
-                        for (int k = 0; k < VPT; k++)
-                            if (c.in(k)) raw[k].raw = from[k * blockDim.x];
-                        from += VPT * blockDim.x;
-                    }
-#pragma unroll
-                    for (int k = 0; k < VPT; k++) raw[k].get(v[k]);
-                };
-                one(y, a.x);
-                one(u, a.h);
-                one(t, a.dy);
-                one(dz, a.dz);
-                if (a.gate_kind == FFCVB_GATE_TOKEN) one(gate, a.gate);
-                fetch(row + deal.ahead, slot);
-                slot = slot + 1 == deal.ahead ? 0 : slot + 1;
+                copies_wait(shape.ahead);
+                const uint4 *from = mine + slot * slot_size;
+                copied<T>(y, from, c);
+                if (a.h) copied<T>(u, from, c);
+                if (a.dy) copied<T>(t, from, c);
+                if (a.dz) copied<T>(dz, from, c);
+                if (per_token) copied<T>(gate, from, c);
+                fetch(row + shape.ahead, slot);
+                slot = slot + 1 == shape.ahead ? 0 : slot + 1;
             } else {
-                auto one = [&](float(&v)[VPT][N], const void *from, long long stride) {
-#pragma unroll
-                    for (int k = 0; k < VPT; k++)
-#pragma unroll
-                        for (int j = 0; j < N; j++) v[k][j] = from && c.in(k) ? to_float(static_cast<const T *>(from)[row * stride + c.at(k) + j]) : 0.0f;
-                };
-                one(y, a.x, a.x_stride);
-                one(u, a.h, a.h_stride);
-                one(t, a.dy, a.dy_stride);
-                one(dz, a.dz, a.dz_stride);
-                if (a.gate_kind == FFCVB_GATE_TOKEN) one(gate, a.gate, a.gate_stride);
+                load_row<T>(y, a.x, row * a.x_stride, c);
+                load_row<T>(u, a.h, row * a.h_stride, c);
+                load_row<T>(t, a.dy, row * a.dy_stride, c);
+                load_row<T>(dz, a.dz, row * a.dz_stride, c);
+                if (per_token) load_row<T>(gate, a.gate, row * a.gate_stride, c);
             }
-            if (POST) { // u: normalised, without weight and bias
-#pragma unroll
-                for (int k = 0; k < VPT; k++)
-#pragma unroll
-                    for (int j = 0; j < N; j++) u[k][j] = (u[k][j] - stats.z) * stats.w;
-            }
-            // the inner norm's parameters are fetched again for every row, from L1: there are no registers for them
-            auto post_params = [&](int k, float(&pw)[N], float(&pb)[N]) {
-                load_params<N>(pw, a.post_weight, a.param_type, c.in(k) ? c.at(k) : 0, 1.0f);
-                load_params<N>(pb, a.post_bias, a.param_type, c.in(k) ? c.at(k) : 0, 0.0f);
-            };
-            if (a.norm != FFCVB_NORM_NONE) {
-                float2 means = make_float2(0.0f, 0.0f);
-#pragma unroll
-                for (int k = 0; k < VPT; k++) {
-                    float pw[N], pb[N];
-                    if (POST) post_params(k, pw, pb);
-#pragma unroll
-                    for (int j = 0; j < N; j++) {
-                        const float whole = POST ? u[k][j] * pw[j] + pb[j] : u[k][j];
-                        y[k][j] = (y[k][j] + whole * (f[k][j] * gate[k][j]) - stats.x) * stats.y;
-                        dw[k][j] += dz[k][j] * y[k][j];
-                        db[k][j] += dz[k][j];
-                        dz[k][j] *= w[k][j];
-                        means.x += dz[k][j];
-                        means.y += dz[k][j] * y[k][j];
-                    }
-                }
-                means = sum(means);
-                const float m = a.norm == FFCVB_NORM_LAYER ? means.x * over : 0.0f, my = means.y * over;
-#pragma unroll
-                for (int k = 0; k < VPT; k++)
-#pragma unroll
-                    for (int j = 0; j < N; j++) t[k][j] = c.in(k) ? t[k][j] + stats.y * (dz[k][j] - m - y[k][j] * my) : 0.0f;
-            }
-            if (a.dx) store_row<T, N, VPT, MULTI>(t, a.dx, row * a.width, c);
-            if (!a.h) continue;
-            float2 means = make_float2(0.0f, 0.0f);
-#pragma unroll
-            for (int k = 0; k < VPT; k++) {
-                float pw[N], pb[N];
-                if (POST) post_params(k, pw, pb);
-#pragma unroll
-                for (int j = 0; j < N; j++) {
-                    if (a.gate_kind == FFCVB_GATE_TOKEN) { // (dz is not needed any more)
-                        dz[k][j] = t[k][j] * (POST ? u[k][j] * pw[j] + pb[j] : u[k][j]) * f[k][j];
-                        t[k][j] *= gate[k][j];
-                    }
-                    sa[k][j] += t[k][j] * u[k][j];
-                    if (POST) sb[k][j] += t[k][j];
-                    t[k][j] *= f[k][j];
-                    if (per_sample) t[k][j] *= gate[k][j];
-                    if (POST) {
-                        t[k][j] *= pw[j];
-                        means.x += t[k][j];
-                        means.y += t[k][j] * u[k][j];
-                    }
-                }
-            }
-            if (a.gate_kind == FFCVB_GATE_TOKEN && a.dgate) store_row<T, N, VPT, MULTI>(dz, a.dgate, row * a.width, c);
+            Eight pw, pb; // fetched again for every row, from L1: there are no registers to keep them in
             if (POST) {
-                means = sum(means);
-                const float m = a.post_norm == FFCVB_NORM_LAYER ? means.x * over : 0.0f, mu = means.y * over;
-#pragma unroll
-                for (int k = 0; k < VPT; k++)
-#pragma unroll
-                    for (int j = 0; j < N; j++) t[k][j] = stats.w * (t[k][j] - m - u[k][j] * mu);
+                normalise(u, stats.z, stats.w); // without weight and bias
+                load_params(pw, a.post_weight, a.param_type, c, 1.0f, 1.0f);
+                load_params(pb, a.post_bias, a.param_type, c, 0.0f, 0.0f);
             }
-            if (a.dh) store_row<T, N, VPT, MULTI>(t, a.dh, row * a.width, c);
+            if (a.norm != FFCVB_NORM_NONE) {
+#pragma unroll
+                for (int p = 0; p < kPairs; p++) {
+                    const Two whole = POST ? fma_rn(u[p], pw[p], pb[p]) : u[p];
+                    y[p] = fma_rn(per_token ? mul_rn(whole, gate[p]) : whole, f[p], y[p]);
+                }
+                normalise(y, stats.x, stats.y);
+                Two first(0.0f, 0.0f), second(0.0f, 0.0f);
+#pragma unroll
+                for (int p = 0; p < kPairs; p++) {
+                    dw[p] = fma_rn(dz[p], y[p], dw[p]);
+                    db[p] = add_rn(db[p], dz[p]);
+                    dz[p] = mul_rn(dz[p], w[p]);
+                    first = add_rn(first, dz[p]);
+                    second = fma_rn(dz[p], y[p], second);
+                }
+                const float2 means = sum(first.lo() + first.hi(), second.lo() + second.hi());
+                const float m = a.norm == FFCVB_NORM_LAYER ? means.x * over : 0.0f, my = means.y * over;
+                const Two minus_m(-m, -m), minus_my(-my, -my), r(stats.y, stats.y);
+#pragma unroll
+                for (int p = 0; p < kPairs; p++) t[p] = fma_rn(fma_rn(y[p], minus_my, add_rn(dz[p], minus_m)), r, t[p]);
+            }
+            if (a.dx) store_row<T>(t, a.dx, row * a.width, c);
+            if (!a.h) continue;
+            if (per_token) {
+                Eight scale, dgate;
+                load_params(scale, a.scale, a.param_type, c, 1.0f, 0.0f);
+#pragma unroll
+                for (int p = 0; p < kPairs; p++) {
+                    const Two whole = POST ? fma_rn(u[p], pw[p], pb[p]) : u[p];
+                    dgate[p] = mul_rn(mul_rn(t[p], whole), mul_rn(scale[p], Two(a.number, a.number)));
+                    t[p] = mul_rn(t[p], gate[p]);
+                }
+                if (a.dgate) store_row<T>(dgate, a.dgate, row * a.width, c);
+            }
+            Two first(0.0f, 0.0f), second(0.0f, 0.0f);
+#pragma unroll
+            for (int p = 0; p < kPairs; p++) {
+                sa[p] = fma_rn(t[p], u[p], sa[p]);
+                if (POST) sb[p] = add_rn(sb[p], t[p]);
+                t[p] = mul_rn(t[p], f[p]);
+                if (POST) {
+                    t[p] = mul_rn(t[p], pw[p]);
+                    first = add_rn(first, t[p]);
+                    second = fma_rn(t[p], u[p], second);
+                }
+            }
+            if (POST) {
+                const float2 means = sum(first.lo() + first.hi(), second.lo() + second.hi());
+                const float m = a.post_norm == FFCVB_NORM_LAYER ? means.x * over : 0.0f, mu = means.y * over;
+                const Two minus_m(-m, -m), minus_mu(-mu, -mu), r(stats.w, stats.w);
+#pragma unroll
+                for (int p = 0; p < kPairs; p++) t[p] = mul_rn(fma_rn(u[p], minus_mu, add_rn(t[p], minus_m)), r);
+            }
+            if (a.dh) store_row<T>(t, a.dh, row * a.width, c);
         }
         if (per_sample) {
-            float dg[VPT][N];
+            Eight dg, gate, pw, pb;
+            load_params(pw, a.post_weight, a.param_type, c, 1.0f, 1.0f);
+            load_params(pb, a.post_bias, a.param_type, c, 0.0f, 0.0f);
+            load_row<T>(gate, a.gate, sample * a.gate_stride, c);
+            load_f();
 #pragma unroll
-            for (int k = 0; k < VPT; k++) {
-                float pw[N], pb[N];
-                load_params<N>(pw, a.post_weight, a.param_type, c.in(k) ? c.at(k) : 0, 1.0f);
-                load_params<N>(pb, a.post_bias, a.param_type, c.in(k) ? c.at(k) : 0, 0.0f);
+            for (int p = 0; p < kPairs; p++) {
+                const Two whole = fma_rn(pw[p], sa[p], mul_rn(pb[p], sb[p])), fg = mul_rn(f[p], gate[p]);
+                const Two add[3] = {mul_rn(fg, sa[p]), mul_rn(fg, sb[p]), mul_rn(gate[p], whole)};
 #pragma unroll
-                for (int j = 0; j < N; j++) {
-                    const float whole = pw[j] * sa[k][j] + pb[j] * sb[k][j];
-                    float *to = kept + 3 * (k * N + j) * blockDim.x;
-                    to[0] += f[k][j] * gate[k][j] * sa[k][j];
-                    to[blockDim.x] += f[k][j] * gate[k][j] * sb[k][j];
-                    to[2 * blockDim.x] += gate[k][j] * whole;
-                    dg[k][j] = f[k][j] * whole;
-                    sa[k][j] = sb[k][j] = 0.0f;
-                }
+                for (int j = 0; j < 6; j++) kept[(p * 6 + j) * blockDim.x] += add[j >> 1].half(j & 1);
+                dg[p] = mul_rn(f[p], whole);
+                sa[p] = sb[p] = Two(0.0f, 0.0f);
             }
             if (a.dgate && deal.splits == 1)
-                store_row<T, N, VPT, MULTI>(dg, a.dgate, sample * a.width, c);
+                store_row<T>(dg, a.dgate, sample * a.width, c);
             else if (a.dgate)
-                store_floats<N, VPT, MULTI>(dg, part.gate + unit * a.width, c);
+                store_floats(dg, part.gate + unit * a.width, c);
         }
     }
     float *to = part.columns + (long long)cluster * deal.columns * a.width;
-    auto put = [&](const float(&v)[VPT][N], const void *wanted) {
+    auto put = [&](const Eight &v, const void *wanted) {
         if (!wanted) return;
-        store_floats<N, VPT, MULTI>(v, to, c);
+        store_floats(v, to, c);
         to += a.width;
     };
     put(dw, a.dweight);
     put(db, a.dbias);
+    Eight pw, pb;
+    load_params(pw, a.post_weight, a.param_type, c, 1.0f, 1.0f);
+    load_params(pb, a.post_bias, a.param_type, c, 0.0f, 0.0f);
 #pragma unroll
-    for (int k = 0; k < VPT; k++) {
-        float pw[N], pb[N];
-        load_params<N>(pw, a.post_weight, a.param_type, c.in(k) ? c.at(k) : 0, 1.0f);
-        load_params<N>(pb, a.post_bias, a.param_type, c.in(k) ? c.at(k) : 0, 0.0f);
-#pragma unroll
-        for (int j = 0; j < N; j++) {
-            const float *from = kept + 3 * (k * N + j) * blockDim.x;
-            dw[k][j] = per_sample ? from[0] : f[k][j] * sa[k][j];
-            db[k][j] = per_sample ? from[blockDim.x] : f[k][j] * sb[k][j];
-            f[k][j] = a.number * (per_sample ? from[2 * blockDim.x] : pw[j] * sa[k][j] + pb[j] * sb[k][j]);
+    for (int p = 0; p < kPairs; p++) {
+        const float *from = kept + p * 6 * blockDim.x;
+        const int next = blockDim.x;
+        if (per_sample) {
+            dw[p] = Two(from[0], from[next]);
+            db[p] = Two(from[2 * next], from[3 * next]);
+            f[p] = Two(from[4 * next], from[5 * next]);
+        } else {
+            dw[p] = mul_rn(f[p], sa[p]);
+            db[p] = mul_rn(f[p], sb[p]);
+            f[p] = fma_rn(pw[p], sa[p], mul_rn(pb[p], sb[p]));
         }
+        f[p] = mul_rn(f[p], Two(a.number, a.number));
     }
     put(dw, a.dpost_weight);
     put(db, a.dpost_bias);
@@ -578,34 +646,63 @@ bool wide_rows(const Args &a) {
                                (a.dz ? a.dz_stride : 0)) % n == 0;
 }
 
-// A thread of the backward pass has eight columns; up to 4096 of them are a CTA's, beyond that a cluster shares a row.
+// Rows of up to 4096 values are a CTA's (of up to 256 a warp's), wider ones a cluster's; as many rounds ahead, at most `most`, as shared
+// memory has room for, which 16 warps per SM share.
+constexpr size_t kRoom = 208 * 1024;
+Shape shape_of(const Args &a, int streams, int most_ahead, size_t besides) {
+    Shape s{};
+    s.ctas_per_row = (int)((a.width + 4095) / 4096);
+    const int eights = (int)((a.width + 7) / 8);
+    s.threads = ((eights + s.ctas_per_row - 1) / s.ctas_per_row + 31) / 32 * 32;
+    s.rows_at_once = kSms * (512 / s.threads) / s.ctas_per_row;
+    s.streams = streams;
+    s.ahead = most_ahead;
+    while (s.ahead > 1 && 512 * ((size_t)s.ahead * streams * 8 * type_size(a.type) + besides) > kRoom) s.ahead--;
+    return s;
+}
 Deal deal_of(const Args &a) {
     Deal d{};
-    d.ctas_per_row = (int)((a.width + 4095) / 4096);
-    const int eights = (int)((a.width + 7) / 8);
-    d.threads = ((eights + d.ctas_per_row - 1) / d.ctas_per_row + 31) / 32 * 32;
-    const long long most = (long long)kSms * (512 / d.threads) / d.ctas_per_row; // 16 warps per SM
+    int streams = 0;
+    for (const void *p : {a.x, a.h, a.dy, a.dz, a.gate_kind == FFCVB_GATE_TOKEN ? a.gate : nullptr}) streams += p != nullptr;
+    d.shape = shape_of(a, streams, 3, a.gate_kind == FFCVB_GATE_SAMPLE ? 96 : 0);
+    const long long most = d.shape.rows_at_once;
     d.samples = a.gate_kind == FFCVB_GATE_SAMPLE ? a.rows / a.tokens : 1;
     d.tokens = a.gate_kind == FFCVB_GATE_SAMPLE ? a.tokens : a.rows;
     if (d.samples < 1) d.samples = 1; // no rows
     // splits of a sample: those with which the longest turn of a cluster is shortest
-    d.splits = 1;
+    const long long least = d.samples >= most ? 1 : most / d.samples, upto = d.samples >= most ? 8 : least;
     long long best = 0;
-    const long long upto = d.samples >= most ? 8 : most / d.samples;
-    for (long long s = d.samples >= most ? 1 : upto; s <= upto && s <= (d.tokens > 1 ? d.tokens : 1); s++) {
-        const long long turn = (d.samples * s + most - 1) / most * ((d.tokens + s - 1) / s);
+    d.splits = 1;
+    for (long long s = least; s <= upto; s++) {
+        const long long splits = s < d.tokens ? s : d.tokens > 1 ? d.tokens : 1;
+        const long long turn = (d.samples * splits + most - 1) / most * ((d.tokens + splits - 1) / splits);
         if (!best || turn < best) {
             best = turn;
-            d.splits = s;
+            d.splits = splits;
         }
     }
-    if (d.samples < most && d.splits == 1) d.splits = d.tokens < upto ? (d.tokens > 1 ? d.tokens : 1) : upto;
     d.units = d.samples * d.splits;
-    d.rows_at_once = (int)(d.units < most ? d.units : most);
+    if (d.units < most) d.shape.rows_at_once = (int)d.units;
     for (const void *p : {a.dweight, a.dbias, a.dpost_weight, a.dpost_bias, a.dscale}) d.columns += p != nullptr;
-    for (const void *p : {a.x, a.h, a.dy, a.dz, a.gate_kind == FFCVB_GATE_TOKEN ? a.gate : nullptr}) d.streams += p != nullptr;
-    d.ahead = rows_ahead(3, d.streams * 8 * type_size(a.type), a.gate_kind == FFCVB_GATE_SAMPLE ? 96 : 0);
     return d;
+}
+
+template <typename Kernel, typename... More>
+void launch(Kernel kernel, const Shape &shape, size_t room, cudaStream_t stream, const More &...more) {
+    // (what a CTA may have without being asked includes the static part)
+    if (room > 40 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)room);
+    cudaLaunchConfig_t how{};
+    cudaLaunchAttribute cluster{};
+    cluster.id = cudaLaunchAttributeClusterDimension;
+    cluster.val.clusterDim.x = shape.ctas_per_row;
+    cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+    how.gridDim = dim3(shape.rows_at_once * shape.ctas_per_row);
+    how.blockDim = dim3(shape.threads);
+    how.dynamicSmemBytes = room;
+    how.stream = stream;
+    how.attrs = &cluster;
+    how.numAttrs = shape.ctas_per_row > 1;
+    cudaLaunchKernelEx(&how, kernel, more...);
 }
 
 int check(const Args *args, bool backward) {
@@ -644,31 +741,25 @@ int ffcvb_norm_residual(const ffcvb_norm_residual_args *args, void *stream) {
     OnDevice here(a.device);
     if (!here.ok()) return training_fail(FFCVB_E_NODEVICE, "ffcvb_norm_residual: no device %d", a.device);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    // up to 1024 values a warp has a row, then a CTA of a warp for every 1024; a lane has 8, 16, 24 or 32 of them
-    const int warps = (int)((a.width + 1023) / 1024);
-    const int eights = (int)((a.width + warps * 256 - 1) / (warps * 256));
+    Shape shape = shape_of(a, 1 + (a.h != nullptr) + (a.gate_kind != FFCVB_GATE_NONE), 2, 0);
+    shape.streams *= 2; // (of two rows)
+    while (shape.ahead > 1 && 512ull * shape.ahead * shape.streams * 8 * type_size(a.type) > kRoom) shape.ahead--;
+    if ((a.rows + 1) / 2 < shape.rows_at_once) shape.rows_at_once = (int)((a.rows + 1) / 2);
+    const bool wide = wide_rows(a), warp = shape.threads == 32 && shape.ctas_per_row == 1, post = a.post_norm != FFCVB_NORM_NONE;
+    const size_t room = wide ? (size_t)shape.threads * shape.ahead * shape.streams * 8 * type_size(a.type) : 0;
+    shape.streams /= 2;
     with_type(a.type, [&](auto zero) {
         using T = decltype(zero);
-        constexpr int W = 16 / (int)sizeof(T);
         auto sized = [&](auto n) {
-            constexpr int N = decltype(n)::value, V = 8 / N;
-            auto run = [&](auto kernel, int per, long long ctas, int threads) {
-                const int ahead = rows_ahead(2, 2 * per * V * 16, 0);
-                const size_t room = N > 1 ? (size_t)ahead * 2 * per * V * threads * 16 : 0;
-                if (room > 40 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)room);
-                kernel<<<(unsigned)ctas, threads, room, st>>>(a, ahead);
-            };
-            if (warps == 1) {
-                const long long all = (a.rows + 3) / 4, most = kSms * 16ll;
-                run(eights == 1 ? forward_kernel<T, N, V, false> : eights == 2 ? forward_kernel<T, N, 2 * V, false>
-                    : eights == 3 ? forward_kernel<T, N, 3 * V, false> : forward_kernel<T, N, 4 * V, false>, eights, all < most ? all : most, 128);
-            } else {
-                const long long most = kSms * (64ll / warps < 32 ? 64ll / warps : 32);
-                run(eights <= 3 ? forward_kernel<T, N, 3 * V, true> : forward_kernel<T, N, 4 * V, true>, eights <= 3 ? 3 : 4, a.rows < most ? a.rows : most, 32 * warps);
-            }
+            constexpr int N = decltype(n)::value;
+            auto run = [&](auto kernel) { launch(kernel, shape, room, st, a, shape); };
+            if (post)
+                run(warp ? forward_kernel<T, N, false, true> : forward_kernel<T, N, true, true>);
+            else
+                run(warp ? forward_kernel<T, N, false, false> : forward_kernel<T, N, true, false>);
         };
-        if (wide_rows(a))
-            sized(Int<W>{});
+        if (wide)
+            sized(Int<16 / (int)sizeof(T)>{});
         else
             sized(Int<1>{});
     });
@@ -678,7 +769,7 @@ int ffcvb_norm_residual(const ffcvb_norm_residual_args *args, void *stream) {
 int64_t ffcvb_norm_residual_workspace(const ffcvb_norm_residual_args *args) {
     if (!args || args->rows < 0 || args->width < 1 || (args->gate_kind == FFCVB_GATE_SAMPLE && args->tokens < 1)) return 0;
     const Deal d = deal_of(*args);
-    return ((int64_t)d.rows_at_once * d.columns + (args->gate_kind == FFCVB_GATE_SAMPLE && d.splits > 1 ? d.units : 0)) * args->width * 4 + 16;
+    return ((int64_t)d.shape.rows_at_once * d.columns + (args->gate_kind == FFCVB_GATE_SAMPLE && d.splits > 1 ? d.units : 0)) * args->width * 4 + 16;
 }
 
 int ffcvb_norm_residual_backward(const ffcvb_norm_residual_args *args, void *stream) {
@@ -688,41 +779,25 @@ int ffcvb_norm_residual_backward(const ffcvb_norm_residual_args *args, void *str
     if (!here.ok()) return training_fail(FFCVB_E_NODEVICE, "ffcvb_norm_residual_backward: no device %d", a.device);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const Deal d = deal_of(a);
-    Partials part{static_cast<float *>(a.workspace), static_cast<float *>(a.workspace) + (long long)d.rows_at_once * d.columns * a.width};
+    Partials part{static_cast<float *>(a.workspace), static_cast<float *>(a.workspace) + (long long)d.shape.rows_at_once * d.columns * a.width};
     if (a.rows > 0)
         with_type(a.type, [&](auto zero) {
             using T = decltype(zero);
-            auto sized = [&](auto n, auto post) {
-                constexpr int N = decltype(n)::value, V = 8 / N;
-                constexpr bool P = decltype(post)::value;
-                const size_t room = (size_t)d.threads * V * ((N > 1 ? d.ahead * d.streams * 16 : 0) + (a.gate_kind == FFCVB_GATE_SAMPLE ? 12 * N : 0));
-                auto run = [&](auto kernel) {
-                    if (room > 40 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)room);
-                    cudaLaunchConfig_t how{};
-                    cudaLaunchAttribute cluster{};
-                    cluster.id = cudaLaunchAttributeClusterDimension;
-                    cluster.val.clusterDim.x = d.ctas_per_row;
-                    cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
-                    how.gridDim = dim3(d.rows_at_once * d.ctas_per_row);
-                    how.blockDim = dim3(d.threads);
-                    how.dynamicSmemBytes = room;
-                    how.stream = st;
-                    how.attrs = &cluster;
-                    how.numAttrs = d.ctas_per_row > 1;
-                    cudaLaunchKernelEx(&how, kernel, a, d, part);
-                };
-                run(d.threads == 32 && d.ctas_per_row == 1 ? backward_kernel<T, N, V, false, P> : backward_kernel<T, N, V, true, P>);
+            const Shape &shape = d.shape;
+            const bool wide = wide_rows(a), warp = shape.threads == 32 && shape.ctas_per_row == 1, post = a.post_norm != FFCVB_NORM_NONE;
+            const size_t room = (size_t)shape.threads * ((wide ? shape.ahead * shape.streams * 8 * sizeof(T) : 0) + (a.gate_kind == FFCVB_GATE_SAMPLE ? 96 : 0));
+            auto sized = [&](auto n) {
+                constexpr int N = decltype(n)::value;
+                auto run = [&](auto kernel) { launch(kernel, shape, room, st, a, d, part); };
+                if (post)
+                    run(warp ? backward_kernel<T, N, false, true> : backward_kernel<T, N, true, true>);
+                else
+                    run(warp ? backward_kernel<T, N, false, false> : backward_kernel<T, N, true, false>);
             };
-            constexpr int W = 16 / (int)sizeof(T);
-            const bool post = a.post_norm != FFCVB_NORM_NONE;
-            if (wide_rows(a) && post)
-                sized(Int<W>{}, Int<1>{});
-            else if (wide_rows(a))
-                sized(Int<W>{}, Int<0>{});
-            else if (post)
-                sized(Int<1>{}, Int<1>{});
+            if (wide)
+                sized(Int<16 / (int)sizeof(T)>{});
             else
-                sized(Int<1>{}, Int<0>{});
+                sized(Int<1>{});
         });
     Sums s{};
     int n = 0;
@@ -732,7 +807,7 @@ int ffcvb_norm_residual_backward(const ffcvb_norm_residual_args *args, void *str
             s.to[n++] = p;
         }
     s.width = a.width;
-    s.count = a.rows > 0 ? d.rows_at_once : 0;
+    s.count = a.rows > 0 ? d.shape.rows_at_once : 0;
     s.stride = d.columns * a.width;
     s.type = a.param_type;
     const unsigned across = (unsigned)((a.width + 31) / 32);
