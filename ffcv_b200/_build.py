@@ -7,8 +7,9 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, 'csrc')
 LIB = os.path.join(HERE, 'libffcv_b200.so')
 SOURCES = ['context.cu', 'entropy.cu', 'idct.cu', 'gather.cu', 'resize.cu', 'pixel_ops.cu', 'static_decode.cu', 'training.cu',
-           'cross_entropy.cu', 'norm_residual.cu', 'rotary.cu', 'adamw.cu', 'jpeg_header.cpp']
-HEADERS = ['types.h', 'kernels.h', 'jpeg_header.h', 'huffman.h', 'color.h', 'two.h', 'decode_index.h', 'table_store.h', 'training.h', os.path.join('..', '..', 'include', 'ffcv_b200.h')]
+           'cross_entropy.cu', 'norm_residual.cu', 'norm_forward.cu', 'norm_backward.cu', 'rotary.cu', 'adamw.cu', 'jpeg_header.cpp']
+HEADERS = ['types.h', 'kernels.h', 'jpeg_header.h', 'huffman.h', 'color.h', 'two.h', 'decode_index.h', 'table_store.h', 'training.h', 'norm_residual.h',
+           os.path.join('..', '..', 'include', 'ffcv_b200.h')]
 
 
 def _nvcc():
@@ -31,7 +32,7 @@ def build_native(force=False, verbose=False):
     if not force and not is_stale():
         return LIB
     cmd = [_nvcc(), '-gencode', 'arch=compute_100a,code=sm_100a', '-lineinfo', '-O3', '-std=c++17',
-           '-Xcompiler', '-fPIC,-O3,-pthread', '-shared', '-o', LIB]
+           '--threads', '0', '-Xcompiler', '-fPIC,-O3,-pthread', '-shared', '-o', LIB]
     if verbose:
         cmd += ['-Xptxas', '-v']
     cmd += [os.path.join(CSRC, f) for f in SOURCES]

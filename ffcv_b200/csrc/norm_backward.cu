@@ -1,0 +1,260 @@
+// Backward pass of the seam between two blocks (sm_100a): see norm_residual.cu.
+#include "norm_residual.h"
+
+namespace ffcvb {
+
+namespace norms {
+
+namespace {
+
+// One row per CTA (or cluster, or warp) at a time; with packs of 16 bytes those of the next are on their way meanwhile.
+// POST: with an inner norm.  Of the branch's side two sums are kept per column and unit, A = sum t u and B = sum t (t with the gate,
+// if it is one per token), u without weight and bias: all other gradients are made of them at a unit's end,
+//   gate: f (pw A + pb B);  times the sample's gate:  scale: pw A + pb B,  post_weight: f A,  post_bias: f B.
+template <typename T, int N, bool MULTI, bool POST, int FORM>
+__global__ void __launch_bounds__(MULTI ? 512 : 32, MULTI ? 1 : 16)
+backward_kernel(const __grid_constant__ Args a, const Deal deal, const Partials part) {
+    constexpr bool RING = N > 1;
+    const Shape &shape = deal.shape;
+    __shared__ __align__(16) float2 s_sum[72];
+    extern __shared__ uint4 s_ring[]; // [ahead][streams][8 / N][threads], then floats [8][3][threads]: see below
+    int rank = 0, cluster = blockIdx.x;
+    if (MULTI && shape.ctas_per_row > 1) {
+        rank = blockIdx.x % shape.ctas_per_row;
+        cluster = blockIdx.x / shape.ctas_per_row;
+    }
+    RowSum<MULTI> sum{s_sum, shape.ctas_per_row};
+    sum.begin();
+    const Columns<N, MULTI> c(a.width, shape.ctas_per_row, rank);
+    const float over = 1.0f / (float)a.width;
+    const bool per_sample = FORM == kGated || (FORM == kAny && a.gate_kind == FFCVB_GATE_SAMPLE);
+    const bool per_token = FORM == kAny && a.gate_kind == FFCVB_GATE_TOKEN;
+    const bool branch = FORM != kAny || a.h, normed = FORM != kAny || a.norm != FFCVB_NORM_NONE;
+    const bool given_dy = FORM != kAny || a.dy, given_dz = FORM != kAny || a.dz, want_dx = FORM != kAny || a.dx, want_dh = FORM != kAny || a.dh;
+    const uint32_t mine = (uint32_t)__cvta_generic_to_shared(s_ring + threadIdx.x), slot_size = shape.streams * (8 / N) * blockDim.x * 16;
+    const uint32_t ring_end = mine + shape.ahead * slot_size;
+    // with a gate per sample the sums over units are kept here, the thread's own
+    float *const kept = reinterpret_cast<float *>(s_ring + (RING ? shape.ahead * shape.streams * (8 / N) * blockDim.x : 0)) + threadIdx.x;
+    if (per_sample)
+        for (int k = 0; k < 24; k++) kept[k * blockDim.x] = 0.0f;
+    Eight dw, db, sa, sb, w, f; // f: with the sample's gate; 0 beyond the row, which keeps everything of the branch 0 there
+    fill(dw, 0.0f);
+    fill(db, 0.0f);
+    fill(sa, 0.0f);
+    fill(sb, 0.0f);
+    load_params(w, a.weight, a.param_type, c, 1.0f, 0.0f);
+    auto load_f = [&]() {
+        load_params(f, a.scale, a.param_type, c, 1.0f, 0.0f);
+#pragma unroll
+        for (int p = 0; p < kPairs; p++) f[p] = mul_rn(f[p], Two(a.number, a.number));
+    };
+    load_f();
+    for (long long unit = cluster; unit < deal.units; unit += shape.rows_at_once) {
+        const long long sample = unit / deal.splits, split = unit % deal.splits;
+        const long long begin = sample * deal.tokens + deal.tokens * split / deal.splits;
+        const long long end = sample * deal.tokens + deal.tokens * (split + 1) / deal.splits;
+        if (per_sample) {
+            Eight gate;
+            load_f();
+            load_row<T>(gate, a.gate, sample * a.gate_stride, c);
+#pragma unroll
+            for (int p = 0; p < kPairs; p++) f[p] = mul_rn(f[p], gate[p]);
+        }
+        const T *next_x = static_cast<const T *>(a.x) + begin * a.x_stride, *next_h = static_cast<const T *>(a.h) + begin * a.h_stride;
+        const T *next_dy = static_cast<const T *>(a.dy) + begin * a.dy_stride, *next_dz = static_cast<const T *>(a.dz) + begin * a.dz_stride;
+        auto fetch = [&](long long row, uint32_t to) {
+            if (row < end) {
+                copy_packs(to, next_x, c);
+                if (branch) copy_packs(to, next_h, c);
+                if (given_dy) copy_packs(to, next_dy, c);
+                if (given_dz) copy_packs(to, next_dz, c);
+                if (per_token) copy_packs(to, static_cast<const T *>(a.gate) + row * a.gate_stride, c);
+            }
+            copies_made();
+            next_x += a.x_stride;
+            next_h += a.h_stride;
+            next_dy += a.dy_stride;
+            next_dz += a.dz_stride;
+        };
+        if constexpr (RING)
+            for (int k = 0; k < shape.ahead; k++) fetch(begin + k, mine + k * slot_size);
+        float4 next = {};
+        if (begin < end) next = reinterpret_cast<const float4 *>(a.stats)[begin];
+        uint32_t slot = mine;
+        T *to_dx = static_cast<T *>(a.dx) + begin * a.width, *to_dh = static_cast<T *>(a.dh) + begin * a.width;
+        for (long long row = begin; row < end; row++, to_dx += a.width, to_dh += a.width) {
+            Eight y, u, t, dz, gate;
+            const float4 stats = next;
+            if (row + 1 < end) next = reinterpret_cast<const float4 *>(a.stats)[row + 1];
+            if (!branch) fill(u, 0.0f);
+            if (!given_dy) fill(t, 0.0f);
+            if (!given_dz) fill(dz, 0.0f);
+            if constexpr (RING) {
+                copies_wait(shape.ahead);
+                uint32_t from = slot;
+                copied<T, N>(y, from);
+                if (branch) copied<T, N>(u, from);
+                if (given_dy) copied<T, N>(t, from);
+                if (given_dz) copied<T, N>(dz, from);
+                if (per_token) copied<T, N>(gate, from);
+                fetch(row + shape.ahead, slot);
+                slot += slot_size;
+                if (slot == ring_end) slot = mine;
+            } else {
+                load_row<T>(y, a.x, row * a.x_stride, c);
+                load_row<T>(u, a.h, row * a.h_stride, c);
+                load_row<T>(t, a.dy, row * a.dy_stride, c);
+                load_row<T>(dz, a.dz, row * a.dz_stride, c);
+                if (per_token) load_row<T>(gate, a.gate, row * a.gate_stride, c);
+            }
+            Eight pw, pb; // fetched again for every row, from L1: there are no registers to keep them in
+            if (POST) {
+                normalise(u, stats.z, stats.w); // without weight and bias
+                load_params(pw, a.post_weight, a.param_type, c, 1.0f, 1.0f);
+                load_params(pb, a.post_bias, a.param_type, c, 0.0f, 0.0f);
+            }
+            if (normed) {
+#pragma unroll
+                for (int p = 0; p < kPairs; p++) {
+                    const Two whole = POST ? fma_rn(u[p], pw[p], pb[p]) : u[p];
+                    y[p] = fma_rn(per_token ? mul_rn(whole, gate[p]) : whole, f[p], y[p]);
+                }
+                normalise(y, stats.x, stats.y);
+                Two first(0.0f, 0.0f), second(0.0f, 0.0f);
+#pragma unroll
+                for (int p = 0; p < kPairs; p++) {
+                    dw[p] = fma_rn(dz[p], y[p], dw[p]);
+                    db[p] = add_rn(db[p], dz[p]);
+                    dz[p] = mul_rn(dz[p], w[p]);
+                    first = add_rn(first, dz[p]);
+                    second = fma_rn(dz[p], y[p], second);
+                }
+                const float2 means = sum(first.lo() + first.hi(), second.lo() + second.hi());
+                const float m = a.norm == FFCVB_NORM_LAYER ? means.x * over : 0.0f, my = means.y * over;
+                const Two minus_m(-m, -m), minus_my(-my, -my), r(stats.y, stats.y);
+#pragma unroll
+                for (int p = 0; p < kPairs; p++) t[p] = fma_rn(fma_rn(y[p], minus_my, add_rn(dz[p], minus_m)), r, t[p]);
+            }
+            if (want_dx) store_row<T>(t, to_dx, 0, c);
+            if (!branch) continue;
+            if (per_token) {
+                Eight scale, dgate;
+                load_params(scale, a.scale, a.param_type, c, 1.0f, 0.0f);
+#pragma unroll
+                for (int p = 0; p < kPairs; p++) {
+                    const Two whole = POST ? fma_rn(u[p], pw[p], pb[p]) : u[p];
+                    dgate[p] = mul_rn(mul_rn(t[p], whole), mul_rn(scale[p], Two(a.number, a.number)));
+                    t[p] = mul_rn(t[p], gate[p]);
+                }
+                if (a.dgate) store_row<T>(dgate, a.dgate, row * a.width, c);
+            }
+            Two first(0.0f, 0.0f), second(0.0f, 0.0f);
+#pragma unroll
+            for (int p = 0; p < kPairs; p++) {
+                sa[p] = fma_rn(t[p], u[p], sa[p]);
+                if (POST) sb[p] = add_rn(sb[p], t[p]);
+                t[p] = mul_rn(t[p], f[p]);
+                if (POST) {
+                    t[p] = mul_rn(t[p], pw[p]);
+                    first = add_rn(first, t[p]);
+                    second = fma_rn(t[p], u[p], second);
+                }
+            }
+            if (POST) {
+                const float2 means = sum(first.lo() + first.hi(), second.lo() + second.hi());
+                const float m = a.post_norm == FFCVB_NORM_LAYER ? means.x * over : 0.0f, mu = means.y * over;
+                const Two minus_m(-m, -m), minus_mu(-mu, -mu), r(stats.w, stats.w);
+#pragma unroll
+                for (int p = 0; p < kPairs; p++) t[p] = mul_rn(fma_rn(u[p], minus_mu, add_rn(t[p], minus_m)), r);
+            }
+            if (want_dh) store_row<T>(t, to_dh, 0, c);
+        }
+        if (per_sample) {
+            Eight dg, gate, pw, pb;
+            load_params(pw, a.post_weight, a.param_type, c, 1.0f, 1.0f);
+            load_params(pb, a.post_bias, a.param_type, c, 0.0f, 0.0f);
+            load_row<T>(gate, a.gate, sample * a.gate_stride, c);
+            load_f();
+#pragma unroll
+            for (int p = 0; p < kPairs; p++) {
+                const Two whole = fma_rn(pw[p], sa[p], mul_rn(pb[p], sb[p])), fg = mul_rn(f[p], gate[p]);
+                const Two add[3] = {mul_rn(fg, sa[p]), mul_rn(fg, sb[p]), mul_rn(gate[p], whole)};
+#pragma unroll
+                for (int j = 0; j < 6; j++) kept[(p * 6 + j) * blockDim.x] += add[j >> 1].half(j & 1);
+                dg[p] = mul_rn(f[p], whole);
+                sa[p] = sb[p] = Two(0.0f, 0.0f);
+            }
+            if (a.dgate && deal.splits == 1)
+                store_row<T>(dg, a.dgate, sample * a.width, c);
+            else if (a.dgate)
+                store_floats(dg, part.gate + unit * a.width, c);
+        }
+    }
+    float *to = part.columns + (long long)cluster * deal.columns * a.width;
+    auto put = [&](const Eight &v, const void *wanted) {
+        if (!wanted) return;
+        store_floats(v, to, c);
+        to += a.width;
+    };
+    put(dw, a.dweight);
+    put(db, a.dbias);
+    Eight pw, pb;
+    load_params(pw, a.post_weight, a.param_type, c, 1.0f, 1.0f);
+    load_params(pb, a.post_bias, a.param_type, c, 0.0f, 0.0f);
+#pragma unroll
+    for (int p = 0; p < kPairs; p++) {
+        const float *from = kept + p * 6 * blockDim.x;
+        const int next = blockDim.x;
+        if (per_sample) {
+            dw[p] = Two(from[0], from[next]);
+            db[p] = Two(from[2 * next], from[3 * next]);
+            f[p] = Two(from[4 * next], from[5 * next]);
+        } else {
+            dw[p] = mul_rn(f[p], sa[p]);
+            db[p] = mul_rn(f[p], sb[p]);
+            f[p] = fma_rn(pw[p], sa[p], mul_rn(pb[p], sb[p]));
+        }
+        f[p] = mul_rn(f[p], Two(a.number, a.number));
+    }
+    put(dw, a.dpost_weight);
+    put(db, a.dpost_bias);
+    put(f, a.dscale);
+}
+
+template <typename T, int N, bool POST, int FORM>
+void sized(const Args &a, const Deal &d, const Partials &part, size_t room, cudaStream_t stream) {
+    if (d.shape.threads == 32 && d.shape.ctas_per_row == 1)
+        launch(backward_kernel<T, N, false, POST, FORM>, d.shape, room, stream, a, d, part);
+    else
+        launch(backward_kernel<T, N, true, POST, FORM>, d.shape, room, stream, a, d, part);
+}
+
+} // namespace
+
+void launch_backward(const Args &a, const Deal &d, const Partials &part, bool wide, cudaStream_t stream) {
+    const bool post = a.post_norm != FFCVB_NORM_NONE;
+    const size_t room = (size_t)d.shape.threads * ((wide ? d.shape.ahead * d.shape.streams * 8 * type_size(a.type) : 0) + (a.gate_kind == FFCVB_GATE_SAMPLE ? 96 : 0));
+    with_type(a.type, [&](auto zero) {
+        using T = decltype(zero);
+        constexpr int W = 16 / (int)sizeof(T);
+        auto formed = [&](auto post_norm) {
+            constexpr bool P = decltype(post_norm)::value;
+            if (!wide)
+                sized<T, 1, P, kAny>(a, d, part, room, stream);
+            else if (form_of(a, true) == kPlain)
+                sized<T, W, P, kPlain>(a, d, part, room, stream);
+            else if (form_of(a, true) == kGated)
+                sized<T, W, P, kGated>(a, d, part, room, stream);
+            else
+                sized<T, W, P, kAny>(a, d, part, room, stream);
+        };
+        if (post)
+            formed(Int<1>{});
+        else
+            formed(Int<0>{});
+    });
+}
+
+} // namespace norms
+
+} // namespace ffcvb

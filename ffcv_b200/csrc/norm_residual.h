@@ -1,0 +1,311 @@
+// The seam between two blocks of a residual network: what its kernels share (sm_100a).
+#pragma once
+
+#include "training.h"
+#include "two.h"
+
+namespace ffcvb {
+
+namespace norms {
+
+using Args = ffcvb_norm_residual_args;
+
+template <int V> struct Int { static constexpr int value = V; };
+
+// A thread's part of a row: eight columns, as 8 / N packs of N; the packs of all threads of a row lie next to one another.
+// Arithmetic is on pairs of them.
+constexpr int kPairs = 4;
+using Eight = Two[kPairs];
+
+template <int N, bool MULTI> struct Columns {
+    int first, step, width;
+    __device__ __forceinline__ Columns(long long w, int ctas, int rank) : width((int)w) {
+        first = (MULTI ? rank * blockDim.x + threadIdx.x : threadIdx.x) * N;
+        step = (MULTI ? ctas * blockDim.x : 32) * N;
+    }
+    __device__ __forceinline__ int at(int k) const { return first + k * step; }
+    __device__ __forceinline__ bool in(int k) const { return at(k) < width; } // (a pack is inside the row or not)
+    __device__ __forceinline__ int inside(int k) const { return in(k) ? at(k) : 0; }
+};
+
+__device__ __forceinline__ void fill(Eight &v, float value) {
+#pragma unroll
+    for (int p = 0; p < kPairs; p++) v[p] = Two(value, value);
+}
+template <typename T, int N>
+__device__ __forceinline__ void to_pairs(Eight &v, const Pack<T, N> (&packs)[8 / N]) {
+    float f[8];
+#pragma unroll
+    for (int k = 0; k < 8 / N; k++) packs[k].get(*reinterpret_cast<float(*)[N]>(f + k * N));
+#pragma unroll
+    for (int p = 0; p < kPairs; p++) v[p] = Two(f[2 * p], f[2 * p + 1]);
+}
+// Columns of a row in global memory; 0 beyond it.
+template <typename T, int N, bool MULTI>
+__device__ __forceinline__ void load_row(Eight &v, const void *p, long long offset, const Columns<N, MULTI> &c) {
+    Pack<T, N> packs[8 / N] = {};
+#pragma unroll
+    for (int k = 0; k < 8 / N; k++)
+        if (p && c.in(k)) packs[k].load(static_cast<const T *>(p) + offset + c.at(k));
+    to_pairs<T, N>(v, packs);
+}
+template <typename T, int N, bool MULTI>
+__device__ __forceinline__ void store_row(const Eight &v, void *p, long long offset, const Columns<N, MULTI> &c) {
+    float f[8];
+#pragma unroll
+    for (int q = 0; q < kPairs; q++) {
+        f[2 * q] = v[q].lo();
+        f[2 * q + 1] = v[q].hi();
+    }
+#pragma unroll
+    for (int k = 0; k < 8 / N; k++)
+        if (c.in(k)) {
+            Pack<T, N> pack;
+            pack.set(*reinterpret_cast<const float(*)[N]>(f + k * N));
+            pack.store(static_cast<T *>(p) + offset + c.at(k));
+        }
+}
+// Parameters of the columns; `otherwise` without any, `beyond` beyond the row.
+template <int N, bool MULTI>
+__device__ __forceinline__ void load_params(Eight &v, const void *p, int type, const Columns<N, MULTI> &c, float otherwise, float beyond) {
+    float f[8];
+#pragma unroll
+    for (int k = 0; k < 8 / N; k++) {
+#pragma unroll
+        for (int j = 0; j < N; j++) f[k * N + j] = c.in(k) ? otherwise : beyond;
+        if (!p || !c.in(k)) continue;
+        const int at = c.at(k);
+        if constexpr (N == 1) {
+            f[k] = type == FFCVB_TYPE_F32 ? static_cast<const float *>(p)[at]
+                   : type == FFCVB_TYPE_F16 ? to_float(static_cast<const __half *>(p)[at])
+                                            : to_float(static_cast<const __nv_bfloat16 *>(p)[at]);
+        } else if (type == FFCVB_TYPE_F32) {
+#pragma unroll
+            for (int j = 0; j < N; j += 4) {
+                const float4 w = *reinterpret_cast<const float4 *>(static_cast<const float *>(p) + at + j);
+                f[k * N + j] = w.x, f[k * N + j + 1] = w.y, f[k * N + j + 2] = w.z, f[k * N + j + 3] = w.w;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; j += 4) {
+                const uint2 w = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(p) + at + j);
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const uint32_t u = i ? w.y : w.x;
+                    const float2 two = type == FFCVB_TYPE_F16 ? __half22float2(*reinterpret_cast<const __half2 *>(&u))
+                                                              : make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+                    f[k * N + j + 2 * i] = two.x;
+                    f[k * N + j + 2 * i + 1] = two.y;
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int q = 0; q < kPairs; q++) v[q] = Two(f[2 * q], f[2 * q + 1]);
+}
+template <int N, bool MULTI>
+__device__ __forceinline__ void store_floats(const Eight &v, float *to, const Columns<N, MULTI> &c) {
+#pragma unroll
+    for (int k = 0; k < 8 / N; k++)
+        if (c.in(k)) {
+#pragma unroll
+            for (int j = 0; j < N; j++) to[c.at(k) + j] = v[(k * N + j) / 2].half((k * N + j) & 1);
+        }
+}
+
+// Two sums over the threads of a row: a warp, a CTA, or (wide rows) the CTAs of a cluster, whose sums travel through distributed
+// shared memory.  In a warp the halves exchange what they do not go on with, so that two sums take little more than one.
+// Consecutive sums use `s`, zero at the start, in turn, so that one barrier is enough.
+template <bool MULTI> struct RowSum {
+    float2 *s; // [2][32 + 4]
+    int ctas;
+    int turn = 0;
+    __device__ __forceinline__ float2 operator()(float a, float b) {
+        const int lane = threadIdx.x & 31;
+        float v = lane & 16 ? b : a;
+        v += __shfl_xor_sync(0xffffffffu, lane & 16 ? a : b, 16);
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        if constexpr (!MULTI) {
+            return make_float2(__shfl_sync(0xffffffffu, v, 0), __shfl_sync(0xffffffffu, v, 16));
+        } else {
+            const int warps = blockDim.x >> 5;
+            float2 *to = s + turn * 36;
+            turn ^= 1;
+            if ((lane & 15) == 0) reinterpret_cast<float *>(to + (threadIdx.x >> 5))[lane >> 4] = v;
+            __syncthreads();
+            float2 r;
+            {
+                const float4 w = *reinterpret_cast<const float4 *>(to), x = *reinterpret_cast<const float4 *>(to + 2);
+                r = make_float2((w.x + w.z) + (x.x + x.z), (w.y + w.w) + (x.y + x.w)); // (0 without a warp)
+            }
+            for (int k = 4; k < warps; k += 2) {
+                const float4 w = *reinterpret_cast<const float4 *>(to + k);
+                r.x += w.x + w.z;
+                r.y += w.y + w.w;
+            }
+            if (ctas > 1) {
+                if ((int)threadIdx.x < ctas) {
+                    uint32_t mine, rank, there;
+                    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+                    mine = (uint32_t)__cvta_generic_to_shared(to + 32 + rank);
+                    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(mine), "r"(threadIdx.x));
+                    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(there), "f"(r.x), "f"(r.y) : "memory");
+                }
+                cluster_barrier();
+                r = to[32];
+                for (int k = 1; k < ctas; k++) {
+                    const float2 w = to[32 + k];
+                    r.x += w.x;
+                    r.y += w.y;
+                }
+            }
+            return r;
+        }
+    }
+    static __device__ __forceinline__ void cluster_barrier() {
+        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    }
+    // (all of a cluster's CTAs have begun before one writes into another's memory)
+    __device__ __forceinline__ void begin() {
+        if constexpr (MULTI) {
+            for (int k = threadIdx.x; k < 72; k += blockDim.x) s[k] = make_float2(0.0f, 0.0f);
+            __syncthreads();
+            if (ctas > 1) cluster_barrier();
+        }
+    }
+};
+
+__device__ __forceinline__ float sum_of(const Eight &v) {
+    Two a = v[0];
+#pragma unroll
+    for (int p = 1; p < kPairs; p++) a = add_rn(a, v[p]);
+    return a.lo() + a.hi();
+}
+
+// Packs of coming rows on their way into shared memory, every thread's in places of its own, so that it waits for nobody
+// else's; zeros beyond the row.  Slots are used in turn.
+__device__ __forceinline__ void copy16(uint32_t to, const void *from, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copies_made() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void copies_wait(int ahead) { // for the oldest of `ahead` (1 to 3) rounds
+    if (ahead == 3)
+        asm volatile("cp.async.wait_group 2;" ::: "memory");
+    else if (ahead == 2)
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+    else
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+// A thread's packs of one stream of a row that begins at `from`; `to` goes on to the next stream's places.
+template <typename T, int N, bool MULTI>
+__device__ __forceinline__ void copy_packs(uint32_t &to, const T *from, const Columns<N, MULTI> &c) {
+#pragma unroll
+    for (int k = 0; k < 8 / N; k++) {
+        copy16(to, from + c.inside(k), c.in(k) ? 16 : 0);
+        to += blockDim.x * 16;
+    }
+}
+template <typename T, int N>
+__device__ __forceinline__ void copied(Eight &v, uint32_t &from) {
+    Pack<T, N> packs[8 / N];
+#pragma unroll
+    for (int k = 0; k < 8 / N; k++) {
+        uint4 &r = packs[k].raw;
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(from) : "memory");
+        from += blockDim.x * 16;
+    }
+    to_pairs<T, N>(v, packs);
+}
+
+// How rows are shared out: threads of a CTA, CTAs of a cluster, clusters; streams that are copied ahead and for how many rounds.
+struct Shape {
+    int threads, ctas_per_row, rows_at_once;
+    int streams, ahead;
+};
+
+// Means and 1 / deviations of two rows: the means first (0 for rms), then the squares of what is left.
+template <int N, bool MULTI>
+__device__ __forceinline__ void two_stats(const Eight (&v)[2], int kind, const Columns<N, MULTI> &c, float eps, RowSum<MULTI> &sum, float (&mean)[2], float (&r)[2]) {
+    const float over = 1.0f / (float)c.width;
+    mean[0] = mean[1] = 0.0f;
+    if (kind == FFCVB_NORM_LAYER) {
+        const float2 both = sum(sum_of(v[0]), sum_of(v[1]));
+        mean[0] = both.x * over;
+        mean[1] = both.y * over;
+    }
+    float q[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const Two m(-mean[i], -mean[i]);
+        Eight d;
+#pragma unroll
+        for (int p = 0; p < kPairs; p++) {
+            d[p] = add_rn(v[i][p], m);
+            d[p] = mul_rn(d[p], d[p]);
+            if constexpr (N == 1)
+                d[p] = Two(c.in(2 * p) ? d[p].lo() : 0.0f, c.in(2 * p + 1) ? d[p].hi() : 0.0f);
+            else if (!c.in(2 * p / N))
+                d[p] = Two(0.0f, 0.0f);
+        }
+        q[i] = sum_of(d);
+    }
+    const float2 both = sum(q[0], q[1]);
+    r[0] = rsqrtf(both.x * over + eps);
+    r[1] = rsqrtf(both.y * over + eps);
+}
+// (v - mean) r
+__device__ __forceinline__ void normalise(Eight &v, float mean, float r) {
+    const Two rr(r, r), m(-mean, -mean);
+#pragma unroll
+    for (int p = 0; p < kPairs; p++) v[p] = mul_rn(add_rn(v[p], m), rr);
+}
+
+// How the backward pass deals its rows out.  A unit is a run of rows of one sample (with a gate per sample, whose
+// gradient is a sum over them) or of all rows.
+struct Deal {
+    Shape shape;
+    long long samples, tokens, splits, units;
+    int columns; // column sums of each cluster: weight, bias, post_weight, post_bias, scale
+};
+// Partial rows: [rows_at_once][columns][width] of the column sums, then [units][width] of the gate's with more than one split.
+struct Partials {
+    float *columns, *gate;
+};
+
+constexpr int kColumns = 5;
+
+// What is known of a call when its kernel is compiled: nothing; or that there are a branch, a norm behind it and (backward) gradients of both
+// results, and all streams' gradients wanted, with no gate or one per sample.
+enum Form { kAny, kPlain, kGated };
+inline Form form_of(const Args &a, bool backward) {
+    if (!a.h || a.norm == FFCVB_NORM_NONE || a.gate_kind == FFCVB_GATE_TOKEN || (backward && (!a.dy || !a.dz || !a.dx || !a.dh))) return kAny;
+    return a.gate_kind == FFCVB_GATE_SAMPLE ? kGated : kPlain;
+}
+
+template <typename Kernel, typename... More>
+void launch(Kernel kernel, const Shape &shape, size_t room, cudaStream_t stream, const More &...more) {
+    // (what a CTA may have without being asked includes the static part)
+    if (room > 40 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)room);
+    cudaLaunchConfig_t how{};
+    cudaLaunchAttribute cluster{};
+    cluster.id = cudaLaunchAttributeClusterDimension;
+    cluster.val.clusterDim.x = shape.ctas_per_row;
+    cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+    how.gridDim = dim3(shape.rows_at_once * shape.ctas_per_row);
+    how.blockDim = dim3(shape.threads);
+    how.dynamicSmemBytes = room;
+    how.stream = stream;
+    how.attrs = &cluster;
+    how.numAttrs = shape.ctas_per_row > 1;
+    cudaLaunchKernelEx(&how, kernel, more...);
+}
+
+
+// wide: rows in packs of 16 bytes.
+void launch_forward(const Args &a, const Shape &shape, bool wide, cudaStream_t stream);
+void launch_backward(const Args &a, const Deal &deal, const Partials &part, bool wide, cudaStream_t stream);
+
+} // namespace norms
+
+} // namespace ffcvb
