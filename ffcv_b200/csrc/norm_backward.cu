@@ -17,7 +17,8 @@ backward_kernel(const __grid_constant__ Args a, const Deal deal, const Partials 
     constexpr bool RING = N > 1;
     const Shape &shape = deal.shape;
     __shared__ __align__(16) float2 s_sum[72];
-    extern __shared__ uint4 s_ring[]; // [ahead][streams][8 / N][threads], then floats [8][3][threads]: see below
+    extern __shared__ uint4 s_ring[]; // [ahead][streams][8 / N][threads], then with an inner norm its parameters, float4 [4][threads],
+    // and with a gate per sample sums, floats [24][threads]
     int rank = 0, cluster = blockIdx.x;
     if (MULTI && shape.ctas_per_row > 1) {
         rank = blockIdx.x % shape.ctas_per_row;
@@ -34,7 +35,27 @@ backward_kernel(const __grid_constant__ Args a, const Deal deal, const Partials 
     const uint32_t mine = (uint32_t)__cvta_generic_to_shared(s_ring + threadIdx.x), slot_size = shape.streams * (8 / N) * blockDim.x * 16;
     const uint32_t ring_end = mine + shape.ahead * slot_size;
     // with a gate per sample the sums over units are kept here, the thread's own
-    float *const kept = reinterpret_cast<float *>(s_ring + (RING ? shape.ahead * shape.streams * (8 / N) * blockDim.x : 0)) + threadIdx.x;
+    float4 *const post = reinterpret_cast<float4 *>(s_ring + (RING ? shape.ahead * shape.streams * (8 / N) * blockDim.x : 0)) + threadIdx.x;
+    float *const kept = reinterpret_cast<float *>(post - threadIdx.x + (POST ? 4 * blockDim.x : 0)) + threadIdx.x;
+    const bool post_bias = a.post_bias;
+    if (POST) { // (there are no registers for them)
+        Eight pw, pb;
+        load_params(pw, a.post_weight, a.param_type, c, 1.0f, 1.0f);
+        load_params(pb, a.post_bias, a.param_type, c, 0.0f, 0.0f);
+#pragma unroll
+        for (int p = 0; p < 2; p++) {
+            post[p * blockDim.x] = make_float4(pw[2 * p].lo(), pw[2 * p].hi(), pw[2 * p + 1].lo(), pw[2 * p + 1].hi());
+            post[(p + 2) * blockDim.x] = make_float4(pb[2 * p].lo(), pb[2 * p].hi(), pb[2 * p + 1].lo(), pb[2 * p + 1].hi());
+        }
+    }
+    auto post_params = [&](Eight &v, int bias) {
+#pragma unroll
+        for (int p = 0; p < 2; p++) {
+            const float4 w = post[(p + 2 * bias) * blockDim.x];
+            v[2 * p] = Two(w.x, w.y);
+            v[2 * p + 1] = Two(w.z, w.w);
+        }
+    };
     if (per_sample)
         for (int k = 0; k < 24; k++) kept[k * blockDim.x] = 0.0f;
     Eight dw, db, sa, sb, w, f; // f: with the sample's gate; 0 beyond the row, which keeps everything of the branch 0 there
@@ -107,18 +128,26 @@ backward_kernel(const __grid_constant__ Args a, const Deal deal, const Partials 
                 load_row<T>(dz, a.dz, row * a.dz_stride, c);
                 if (per_token) load_row<T>(gate, a.gate, row * a.gate_stride, c);
             }
-            Eight pw, pb; // fetched again for every row, from L1: there are no registers to keep them in
+            Eight pw;
             if (POST) {
                 normalise(u, stats.z, stats.w); // without weight and bias
-                load_params(pw, a.post_weight, a.param_type, c, 1.0f, 1.0f);
-                load_params(pb, a.post_bias, a.param_type, c, 0.0f, 0.0f);
+                post_params(pw, 0);
             }
-            if (normed) {
+            auto whole = [&](Eight &v) {
 #pragma unroll
-                for (int p = 0; p < kPairs; p++) {
-                    const Two whole = POST ? fma_rn(u[p], pw[p], pb[p]) : u[p];
-                    y[p] = fma_rn(per_token ? mul_rn(whole, gate[p]) : whole, f[p], y[p]);
+                for (int p = 0; p < kPairs; p++) v[p] = POST ? mul_rn(u[p], pw[p]) : u[p];
+                if (POST && post_bias) {
+                    Eight pb;
+                    post_params(pb, 1);
+#pragma unroll
+                    for (int p = 0; p < kPairs; p++) v[p] = add_rn(v[p], pb[p]);
                 }
+            };
+            if (normed) {
+                Eight full;
+                whole(full);
+#pragma unroll
+                for (int p = 0; p < kPairs; p++) y[p] = fma_rn(per_token ? mul_rn(full[p], gate[p]) : full[p], f[p], y[p]);
                 normalise(y, stats.x, stats.y);
                 Two first(0.0f, 0.0f), second(0.0f, 0.0f);
 #pragma unroll
@@ -138,12 +167,11 @@ backward_kernel(const __grid_constant__ Args a, const Deal deal, const Partials 
             if (want_dx) store_row<T>(t, to_dx, 0, c);
             if (!branch) continue;
             if (per_token) {
-                Eight scale, dgate;
-                load_params(scale, a.scale, a.param_type, c, 1.0f, 0.0f);
+                Eight full, dgate;
+                whole(full);
 #pragma unroll
                 for (int p = 0; p < kPairs; p++) {
-                    const Two whole = POST ? fma_rn(u[p], pw[p], pb[p]) : u[p];
-                    dgate[p] = mul_rn(mul_rn(t[p], whole), mul_rn(scale[p], Two(a.number, a.number)));
+                    dgate[p] = mul_rn(mul_rn(t[p], full[p]), f[p]);
                     t[p] = mul_rn(t[p], gate[p]);
                 }
                 if (a.dgate) store_row<T>(dgate, a.dgate, row * a.width, c);
@@ -233,7 +261,7 @@ void sized(const Args &a, const Deal &d, const Partials &part, size_t room, cuda
 
 void launch_backward(const Args &a, const Deal &d, const Partials &part, bool wide, cudaStream_t stream) {
     const bool post = a.post_norm != FFCVB_NORM_NONE;
-    const size_t room = (size_t)d.shape.threads * ((wide ? d.shape.ahead * d.shape.streams * 8 * type_size(a.type) : 0) + (a.gate_kind == FFCVB_GATE_SAMPLE ? 96 : 0));
+    const size_t room = (size_t)d.shape.threads * ((wide ? d.shape.ahead * d.shape.streams * 8 * type_size(a.type) : 0) + (post ? 64 : 0) + (a.gate_kind == FFCVB_GATE_SAMPLE ? 96 : 0));
     with_type(a.type, [&](auto zero) {
         using T = decltype(zero);
         constexpr int W = 16 / (int)sizeof(T);

@@ -14,37 +14,53 @@ namespace norms {
 
 namespace {
 
-// Adds up partial rows: 32 columns per CTA, 32 runs of rows side by side.
+// Adds up partial rows: eight columns per CTA, 128 runs of rows side by side (740 rows of 768 columns: six values per thread, all on
+// their way at once).
 struct Sums {
     const float *from[kColumns];
     void *to[kColumns];
-    long long width, count, stride, from_z, to_z; // rows to add, from one to the next; from one sum (blockIdx.z) to the next
+    long long width, count, stride; // rows to add, from one to the next
     int type;
 };
 __global__ void __launch_bounds__(1024)
 add_up_kernel(const __grid_constant__ Sums s) {
-    __shared__ float s_part[32][33];
-    const int lane = threadIdx.x & 31, run = threadIdx.x >> 5;
-    const long long c = blockIdx.x * 32ll + lane;
-    const float *from = s.from[blockIdx.y] + blockIdx.z * s.from_z;
+    __shared__ float s_part[8][129];
+    const int column = threadIdx.x & 7, run = threadIdx.x >> 3;
+    const long long c = blockIdx.x * 8ll + column;
+    const float *from = s.from[blockIdx.y];
     float v = 0.0f;
     if (c < s.width) {
 #pragma unroll 8
-        for (long long r = run; r < s.count; r += 32) v += from[r * s.stride + c];
+        for (long long r = run; r < s.count; r += 128) v += from[r * s.stride + c];
     }
-    s_part[run][lane] = v;
+    s_part[column][run] = v;
     __syncthreads();
-    v = warp_sum(s_part[lane][run]); // column `run`
-    const long long mine = blockIdx.x * 32ll + run;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (warp >= 8) return;
+    v = warp_sum((s_part[warp][lane] + s_part[warp][lane + 32]) + (s_part[warp][lane + 64] + s_part[warp][lane + 96]));
+    const long long mine = blockIdx.x * 8ll + warp;
     if (lane == 0 && mine < s.width) {
-        const long long at = blockIdx.z * s.to_z + mine;
         if (s.type == FFCVB_TYPE_F32)
-            static_cast<float *>(s.to[blockIdx.y])[at] = v;
+            static_cast<float *>(s.to[blockIdx.y])[mine] = v;
         else if (s.type == FFCVB_TYPE_F16)
-            static_cast<__half *>(s.to[blockIdx.y])[at] = __float2half_rn(v);
+            static_cast<__half *>(s.to[blockIdx.y])[mine] = __float2half_rn(v);
         else
-            static_cast<__nv_bfloat16 *>(s.to[blockIdx.y])[at] = __float2bfloat16_rn(v);
+            static_cast<__nv_bfloat16 *>(s.to[blockIdx.y])[mine] = __float2bfloat16_rn(v);
     }
+}
+
+// A gate's gradient per sample: the sums of its splits.
+template <typename T>
+__global__ void __launch_bounds__(256)
+gates_kernel(const float *__restrict__ partial, T *__restrict__ dgate, long long width, long long splits, long long values) {
+    const long long at = blockIdx.x * 256ll + threadIdx.x;
+    if (at >= values) return;
+    const long long sample = at / width;
+    const float *from = partial + sample * splits * width + at % width;
+    float v = 0.0f;
+#pragma unroll 4
+    for (long long k = 0; k < splits; k++) v += from[k * width];
+    dgate[at] = from_float<T>(v);
 }
 
 bool wide_rows(const Args &a) {
@@ -75,7 +91,7 @@ Deal deal_of(const Args &a) {
     Deal d{};
     int streams = 0;
     for (const void *p : {a.x, a.h, a.dy, a.dz, a.gate_kind == FFCVB_GATE_TOKEN ? a.gate : nullptr}) streams += p != nullptr;
-    d.shape = shape_of(a, streams, 3, a.gate_kind == FFCVB_GATE_SAMPLE ? 96 : 0);
+    d.shape = shape_of(a, streams, 3, (a.gate_kind == FFCVB_GATE_SAMPLE ? 96 : 0) + (a.post_norm != FFCVB_NORM_NONE ? 64 : 0));
     const long long most = d.shape.rows_at_once;
     d.samples = a.gate_kind == FFCVB_GATE_SAMPLE ? a.rows / a.tokens : 1;
     d.tokens = a.gate_kind == FFCVB_GATE_SAMPLE ? a.tokens : a.rows;
@@ -170,19 +186,14 @@ int ffcvb_norm_residual_backward(const ffcvb_norm_residual_args *args, void *str
     s.count = a.rows > 0 ? d.shape.rows_at_once : 0;
     s.stride = d.columns * a.width;
     s.type = a.param_type;
-    const unsigned across = (unsigned)((a.width + 31) / 32);
+    const unsigned across = (unsigned)((a.width + 7) / 8);
     if (n) add_up_kernel<<<dim3(across, n), 1024, 0, st>>>(s);
-    if (a.dgate && a.gate_kind == FFCVB_GATE_SAMPLE && d.splits > 1 && a.rows > 0) {
-        Sums g{};
-        g.from[0] = part.gate;
-        g.to[0] = a.dgate;
-        g.width = g.stride = g.to_z = a.width;
-        g.count = d.splits;
-        g.from_z = d.splits * a.width;
-        g.type = a.type;
-        // (more than one split means that there are fewer samples than CTAs)
-        add_up_kernel<<<dim3(across, 1, (unsigned)d.samples), 1024, 0, st>>>(g);
-    }
+    if (a.dgate && a.gate_kind == FFCVB_GATE_SAMPLE && d.splits > 1 && a.rows > 0) // (then there are fewer samples than CTAs, or few splits)
+        with_type(a.type, [&](auto zero) {
+            using T = decltype(zero);
+            const long long values = d.samples * a.width;
+            gates_kernel<T><<<(unsigned)((values + 255) / 256), 256, 0, st>>>(part.gate, static_cast<T *>(a.dgate), a.width, d.splits, values);
+        });
     return launched("ffcvb_norm_residual_backward");
 }
 
