@@ -12,8 +12,10 @@
 // grid too and is not rounded again, which would add up to a noise of several times the value over 1 / (1 - beta2) steps.
 // Second moments above zero stay above zero.
 #include "training.h"
+#include "two.h"
 
 #include <math.h>
+#include <type_traits>
 
 namespace ffcvb {
 
@@ -63,77 +65,175 @@ __host__ __device__ inline uint32_t mix(uint32_t x) {
     return x ^ (x >> 16);
 }
 
-// Four values from place `at` of a tensor of n; 0 beyond its end.
-template <typename T>
-__device__ __forceinline__ void load4(float (&v)[4], const T *p, long long at, long long n, bool aligned) {
-    if (aligned && at + 4 <= n) {
-        if constexpr (sizeof(T) == 4) {
-            const float4 f = __ldcs(reinterpret_cast<const float4 *>(p + at));
-            v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+// Four neighbouring values as two pairs.
+__device__ __forceinline__ void four(Two *v, float4 f) {
+    v[0] = Two(f.x, f.y);
+    v[1] = Two(f.z, f.w);
+}
+__device__ __forceinline__ float4 four(const Two *v) { return make_float4(v[0].lo(), v[0].hi(), v[1].lo(), v[1].hi()); }
+
+// Four values from place `at` of a tensor of n; 0 beyond its end.  WHOLE: none is, and the tensor lies on boundaries of four values.
+template <bool WHOLE, typename T>
+__device__ __forceinline__ float4 load4(const T *p, long long at, long long n) {
+    if constexpr (WHOLE && sizeof(T) == 4) {
+        return __ldcs(reinterpret_cast<const float4 *>(p + at));
+    } else if constexpr (WHOLE) {
+        const uint2 w = __ldcs(reinterpret_cast<const uint2 *>(p + at));
+        float2 lo, hi;
+        if constexpr (std::is_same<T, __half>::value) {
+            lo = __half22float2(*reinterpret_cast<const __half2 *>(&w.x));
+            hi = __half22float2(*reinterpret_cast<const __half2 *>(&w.y));
         } else {
-            const uint2 w = __ldcs(reinterpret_cast<const uint2 *>(p + at));
-            T t[4];
-            *reinterpret_cast<uint2 *>(t) = w;
-#pragma unroll
-            for (int j = 0; j < 4; j++) v[j] = to_float(t[j]);
+            lo = make_float2(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u));
+            hi = make_float2(__uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
         }
+        return make_float4(lo.x, lo.y, hi.x, hi.y);
     } else {
-#pragma unroll
-        for (int j = 0; j < 4; j++) v[j] = at + j < n ? to_float(p[at + j]) : 0.0f;
+        return make_float4(at < n ? to_float(p[at]) : 0.0f, at + 1 < n ? to_float(p[at + 1]) : 0.0f,
+                           at + 2 < n ? to_float(p[at + 2]) : 0.0f, at + 3 < n ? to_float(p[at + 3]) : 0.0f);
     }
 }
-template <typename T>
-__device__ __forceinline__ void store4(const float (&v)[4], T *p, long long at, long long n, bool aligned) {
-    if (aligned && at + 4 <= n) {
-        if constexpr (sizeof(T) == 4) {
-            __stcs(reinterpret_cast<float4 *>(p + at), make_float4(v[0], v[1], v[2], v[3]));
+template <bool WHOLE, typename T>
+__device__ __forceinline__ void store4(float4 v, T *p, long long at, long long n) {
+    if constexpr (WHOLE && sizeof(T) == 4) {
+        __stcs(reinterpret_cast<float4 *>(p + at), v);
+    } else if constexpr (WHOLE) {
+        uint2 w;
+        if constexpr (std::is_same<T, __half>::value) {
+            const __half2 lo = __floats2half2_rn(v.x, v.y), hi = __floats2half2_rn(v.z, v.w);
+            w = make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
         } else {
-            T t[4];
-#pragma unroll
-            for (int j = 0; j < 4; j++) t[j] = from_float<T>(v[j]);
-            __stcs(reinterpret_cast<uint2 *>(p + at), *reinterpret_cast<const uint2 *>(t));
+            const __nv_bfloat162 lo = __floats2bfloat162_rn(v.x, v.y), hi = __floats2bfloat162_rn(v.z, v.w);
+            w = make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
         }
+        __stcs(reinterpret_cast<uint2 *>(p + at), w);
     } else {
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-            if (at + j < n) p[at + j] = from_float<T>(v[j]);
+        if (at < n) p[at] = from_float<T>(v.x);
+        if (at + 1 < n) p[at + 1] = from_float<T>(v.y);
+        if (at + 2 < n) p[at + 2] = from_float<T>(v.z);
+        if (at + 3 < n) p[at + 3] = from_float<T>(v.w);
     }
 }
 
 // 2^e as a number, -127 < e < 128.
 __device__ __forceinline__ float power(int e) { return __int_as_float((e + 127) << 23); }
 
-// Codes of eight values of a lane, and the unit's scale; the largest becomes 2^TOP .. 2^(TOP + 1).
-template <int TOP, int BIAS, int DROPPED>
-__device__ __forceinline__ float to_eight(const float (&v)[8], const uint32_t (&noise)[8], uint32_t (&code)[2]) {
-    float most = 0.0f;
-#pragma unroll
-    for (int j = 0; j < 8; j++) most = fmaxf(most, fabsf(v[j]));
-    bool odd = false; // not a number: fmaxf does not see it
-#pragma unroll
-    for (int j = 0; j < 8; j++) odd |= v[j] != v[j];
-    uint32_t top = __reduce_max_sync(0xffffffffu, odd ? 0x7fc00000u : __float_as_uint(most)) >> 23;
-    if (top >= 255) {
-        code[0] = code[1] = 0x01010101u;
-        return NAN; // infinities and what is no number make the unit none
-    }
-    const int e = max((int)top, 1) - 127;
-    const float down = power(-e), bias = __int_as_float((127 + TOP - BIAS) << 23);
-    code[0] = code[1] = 0;
-#pragma unroll
-    for (int j = 0; j < 8; j++) {
-        uint32_t c = (__float_as_uint(__fmul_rn(__fmul_rn(fabsf(v[j]), down), bias)) + noise[j]) >> DROPPED;
-        if (DROPPED == 21) c = max(c, v[j] > 0.0f ? 1u : 0u);
-        if (DROPPED == 20 && v[j] < 0.0f) c |= 128u;
-        code[j >> 2] |= c << (8 * (j & 3));
-    }
-    return __fmul_rn(power(e), __int_as_float((127 - TOP) << 23));
+// The largest of three sizes; what is no number is larger.
+__device__ __forceinline__ float largest(float a, float b, float c) {
+    float r;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
 }
-template <int TOP, int BIAS, int DROPPED>
-__device__ __forceinline__ float from_eight(uint32_t code, int j, float scale) {
-    const uint32_t c = code >> (8 * j);
-    const float v = __int_as_float((c & 127u) << DROPPED | (c & 128u) << 24);
-    return __fmul_rn(__fmul_rn(v, __int_as_float((127 + BIAS) << 23)), scale);
+
+// The unit's scale for eight values of every lane, of which the largest becomes 2^TOP .. 2^(TOP + 1); v becomes the 32-bit numbers
+// that have an 8-bit type's codes as their upper bits.  Infinities and what is no number make the unit none.
+template <int TOP, int BIAS>
+__device__ __forceinline__ float scale_down(Two (&v)[4]) {
+    float most = largest(v[0].lo(), v[0].hi(), v[1].lo());
+    most = largest(most, v[1].hi(), v[2].lo());
+    most = largest(most, v[2].hi(), v[3].lo());
+    most = largest(most, v[3].hi(), 0.0f);
+    const int e = max((int)(__reduce_max_sync(0xffffffffu, __float_as_uint(most)) >> 23), 1) - 127;
+    const float down = e < 128 ? power(-e) : 0.0f, bias = __int_as_float((127 + TOP - BIAS) << 23);
+#pragma unroll
+    for (int p = 0; p < 4; p++) v[p] = mul_rn(mul_rn(v[p], Two(down, down)), Two(bias, bias));
+    return e < 128 ? __fmul_rn(power(e), __int_as_float((127 - TOP) << 23)) : NAN;
+}
+// The upper bytes of four words, the first lowest.
+__device__ __forceinline__ uint32_t top_bytes(const uint32_t *w) {
+    return __byte_perm(__byte_perm(w[0], w[1], 0x0073), __byte_perm(w[2], w[3], 0x0073), 0x5410);
+}
+
+// One unit.  WHOLE: all of it inside a tensor on boundaries of four values.
+template <typename T, int BITS, bool WHOLE, typename Args>
+__device__ __forceinline__ void step_unit(const Args &a, const Set &set, float clip, const T *grad, T *param, long long first, long long n, long long flat) {
+    const int lane = threadIdx.x & 31;
+    Two g[4], w[4], m[4], v[4];
+    float *const exp_avg = static_cast<float *>(a.exp_avg), *const exp_avg_sq = static_cast<float *>(a.exp_avg_sq);
+    uint32_t *const m_codes = static_cast<uint32_t *>(a.exp_avg), *const v_codes = static_cast<uint32_t *>(a.exp_avg_sq);
+    uint32_t mc[2], vc[2];
+    float2 scale;
+    if (BITS == 8) scale = *reinterpret_cast<const float2 *>(a.scales + flat / kUnit * 2);
+#pragma unroll
+    for (int half = 0; half < 2; half++) { // (a lane has four neighbours in either half of a unit)
+        const long long at = first + half * 128 + lane * 4, place = flat + half * 128 + lane * 4;
+        four(g + 2 * half, load4<WHOLE>(grad, at, n));
+        four(w + 2 * half, sizeof(T) == 4 ? load4<WHOLE>(param, at, n) : __ldcs(reinterpret_cast<const float4 *>(a.master + place)));
+        if (BITS == 32) {
+            four(m + 2 * half, __ldcs(reinterpret_cast<const float4 *>(exp_avg + place)));
+            four(v + 2 * half, __ldcs(reinterpret_cast<const float4 *>(exp_avg_sq + place)));
+        } else {
+            mc[half] = __ldcs(m_codes + place / 4);
+            vc[half] = __ldcs(v_codes + place / 4);
+        }
+    }
+    if (BITS == 8) {
+#pragma unroll
+        for (int p = 0; p < 4; p++) { // through 16-bit floats, which hold either type: e5m2 numbers are their upper bytes
+            const uint32_t two_m = mc[p >> 1] >> (16 * (p & 1));
+            uint32_t halves;
+            asm("{ .reg .b16 c; cvt.u16.u32 c, %1; cvt.rn.f16x2.e4m3x2 %0, c; }" : "=r"(halves) : "r"(two_m));
+            const float2 fm = __half22float2(*reinterpret_cast<const __half2 *>(&halves));
+            m[p] = mul_rn(Two(fm.x, fm.y), Two(scale.x, scale.x));
+            halves = __byte_perm(vc[p >> 1], 0, p & 1 ? 0x3424 : 0x1404);
+            const float2 fv = __half22float2(*reinterpret_cast<const __half2 *>(&halves));
+            v[p] = mul_rn(Two(fv.x, fv.y), Two(scale.y, scale.y));
+        }
+    }
+    const Two c2(clip, clip), b1(set.b1, set.b1), d1(set.c1, set.c1), b2(set.b2, set.b2), d2(set.c2, set.c2);
+#pragma unroll
+    for (int p = 0; p < 4; p++) {
+        g[p] = mul_rn(g[p], c2);
+        m[p] = add_rn(mul_rn(m[p], b1), mul_rn(g[p], d1));
+        v[p] = add_rn(mul_rn(v[p], b2), mul_rn(mul_rn(g[p], g[p]), d2));
+        // (a root and a quotient to within two units of the last place: they change a weight by a thousandth of its size at most)
+        float root[2], u[2];
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            asm("sqrt.approx.f32 %0, %1;" : "=f"(root[j]) : "f"(v[p].half(j)));
+            asm("div.approx.ftz.f32 %0, %1, %2;" : "=f"(u[j]) : "f"(m[p].half(j)), "f"(fmaf(root[j], set.over_root, set.eps)));
+        }
+        w[p] = fma_rn(Two(u[0], u[1]), Two(-set.rate, -set.rate), mul_rn(w[p], Two(set.decay, set.decay)));
+    }
+    if (BITS == 8) {
+        uint32_t lifted[4]; // (v's smallest code: above zero; values below 2^-128 may still become zero)
+        scale.x = scale_down<7, 120>(m);
+        Two down[4] = {v[0], v[1], v[2], v[3]};
+        scale.y = scale_down<14, 112>(down);
+        const uint32_t base = ((uint32_t)flat + set.key + (uint32_t)(flat >> 32) * 0x9E3779B9u + lane * 4) * 0xE4C6EF2Bu;
+#pragma unroll
+        for (int half = 0; half < 2; half++) {
+            uint32_t m_word[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                uint32_t x = base + (half * 128 + j) * 0xE4C6EF2Bu; // mix(place + key)
+                x ^= x >> 15;
+                x *= 0x87EA99B3u;
+                const uint32_t upper = x >> 16;
+                const uint32_t y = __float_as_uint(m[2 * half + (j >> 1)].half(j & 1)) + (((x ^ upper) & 0xffffu) << 4);
+                m_word[j] = (y & 0x80000000u) | ((y << 4) & 0x7fffffffu);
+                uint32_t z = __float_as_uint(down[2 * half + (j >> 1)].half(j & 1)) + (upper << 5);
+                z = max(z, min(__float_as_uint(v[2 * half + (j >> 1)].half(j & 1)), 1u << 21));
+                lifted[j] = z << 3;
+            }
+            mc[half] = top_bytes(m_word);
+            vc[half] = top_bytes(lifted);
+        }
+        if (lane == 0) *reinterpret_cast<float2 *>(a.scales + flat / kUnit * 2) = scale;
+    }
+#pragma unroll
+    for (int half = 0; half < 2; half++) {
+        const long long at = first + half * 128 + lane * 4, place = flat + half * 128 + lane * 4;
+        store4<WHOLE>(four(w + 2 * half), param, at, n);
+        if (sizeof(T) != 4) __stcs(reinterpret_cast<float4 *>(a.master + place), four(w + 2 * half));
+        if (BITS == 32) {
+            __stcs(reinterpret_cast<float4 *>(exp_avg + place), four(m + 2 * half));
+            __stcs(reinterpret_cast<float4 *>(exp_avg_sq + place), four(v + 2 * half));
+        } else {
+            __stcs(m_codes + place / 4, mc[half]);
+            __stcs(v_codes + place / 4, vc[half]);
+        }
+    }
 }
 
 template <typename T, int BITS, int MOST>
@@ -150,78 +250,16 @@ step_kernel(const __grid_constant__ Launch<MOST> a) {
         clip = fminf(1.0f, a.max_norm / (norm + 1e-6f));
     }
     const Tensor tensor = a.tensors[local];
-    const Set set = a.sets[a.set[local]];
+    const Set &set = a.sets[a.set[local]];
     T *param = reinterpret_cast<T *>(tensor.param);
-    const long long n = tensor.numel;
     const bool aligned = ((reinterpret_cast<uintptr_t>(grad) | reinterpret_cast<uintptr_t>(param)) & (4 * sizeof(T) - 1)) == 0;
-    const int lane = threadIdx.x & 31;
     for (int unit = threadIdx.x >> 5; unit < kUnitsPerChunk; unit += kThreads / 32) {
         const long long first = chunk.index * kChunk + unit * kUnit; // in the tensor
-        if (first >= n) break;
-        const long long flat = tensor.start + first;
-        float g[8], w[8], m[8], v[8];
-#pragma unroll
-        for (int half = 0; half < 2; half++) {
-            const long long at = first + half * 128 + lane * 4;
-            const long long place = flat + half * 128 + lane * 4;
-            float(&g4)[4] = *reinterpret_cast<float(*)[4]>(g + 4 * half);
-            float(&w4)[4] = *reinterpret_cast<float(*)[4]>(w + 4 * half);
-            load4(g4, grad, at, n, aligned);
-            if (sizeof(T) == 4)
-                load4(w4, param, at, n, aligned);
-            else
-                *reinterpret_cast<float4 *>(w4) = __ldcs(reinterpret_cast<const float4 *>(a.master + place));
-            if (BITS == 32) {
-                *reinterpret_cast<float4 *>(m + 4 * half) = __ldcs(reinterpret_cast<const float4 *>(static_cast<const float *>(a.exp_avg) + place));
-                *reinterpret_cast<float4 *>(v + 4 * half) = __ldcs(reinterpret_cast<const float4 *>(static_cast<const float *>(a.exp_avg_sq) + place));
-            } else {
-                const float2 scale = *reinterpret_cast<const float2 *>(a.scales + flat / kUnit * 2);
-                const uint32_t mc = __ldcs(reinterpret_cast<const uint32_t *>(static_cast<const uint8_t *>(a.exp_avg) + place));
-                const uint32_t vc = __ldcs(reinterpret_cast<const uint32_t *>(static_cast<const uint8_t *>(a.exp_avg_sq) + place));
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    m[4 * half + j] = from_eight<7, 120, 20>(mc, j, scale.x);
-                    v[4 * half + j] = from_eight<14, 112, 21>(vc, j, scale.y);
-                }
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const float gj = __fmul_rn(g[j], clip);
-            m[j] = __fadd_rn(__fmul_rn(m[j], set.b1), __fmul_rn(gj, set.c1));
-            v[j] = __fadd_rn(__fmul_rn(v[j], set.b2), __fmul_rn(__fmul_rn(gj, gj), set.c2));
-            w[j] = w[j] * set.decay - set.rate * (m[j] / (sqrtf(v[j]) * set.over_root + set.eps));
-        }
-        uint32_t mc[2], vc[2];
-        if (BITS == 8) {
-            const uint32_t base = (uint32_t)flat + set.key + (uint32_t)(flat >> 32) * 0x9E3779B9u;
-            uint32_t m_noise[8], v_noise[8];
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const uint32_t r = mix(base + (j >> 2) * 128 + lane * 4 + (j & 3));
-                m_noise[j] = (r & 0xffffu) << 4;
-                v_noise[j] = (r >> 16) << 5;
-            }
-            float2 scale;
-            scale.x = to_eight<7, 120, 20>(m, m_noise, mc);
-            scale.y = to_eight<14, 112, 21>(v, v_noise, vc);
-            if (lane == 0) *reinterpret_cast<float2 *>(a.scales + flat / kUnit * 2) = scale;
-        }
-#pragma unroll
-        for (int half = 0; half < 2; half++) {
-            const long long at = first + half * 128 + lane * 4;
-            const long long place = flat + half * 128 + lane * 4;
-            const float(&w4)[4] = *reinterpret_cast<const float(*)[4]>(w + 4 * half);
-            store4(w4, param, at, n, aligned);
-            if (sizeof(T) != 4) __stcs(reinterpret_cast<float4 *>(a.master + place), make_float4(w4[0], w4[1], w4[2], w4[3]));
-            if (BITS == 32) {
-                __stcs(reinterpret_cast<float4 *>(static_cast<float *>(a.exp_avg) + place), make_float4(m[4 * half], m[4 * half + 1], m[4 * half + 2], m[4 * half + 3]));
-                __stcs(reinterpret_cast<float4 *>(static_cast<float *>(a.exp_avg_sq) + place), make_float4(v[4 * half], v[4 * half + 1], v[4 * half + 2], v[4 * half + 3]));
-            } else {
-                __stcs(reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(a.exp_avg) + place), mc[half]);
-                __stcs(reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(a.exp_avg_sq) + place), vc[half]);
-            }
-        }
+        if (first >= tensor.numel) break;
+        if (aligned && first + kUnit <= tensor.numel)
+            step_unit<T, BITS, true>(a, set, clip, grad, param, first, tensor.numel, tensor.start + first);
+        else
+            step_unit<T, BITS, false>(a, set, clip, grad, param, first, tensor.numel, tensor.start + first);
     }
 }
 
@@ -238,11 +276,17 @@ squares_kernel(const __grid_constant__ Launch<MOST> a) {
         const long long n = a.tensors[local].numel;
         const bool aligned = (reinterpret_cast<uintptr_t>(grad) & (4 * sizeof(T) - 1)) == 0;
         const long long first = chunk.index * kChunk;
-        for (int k = threadIdx.x; k < kChunk / 4 && first + k * 4 < n; k += kThreads) {
-            float g[4];
-            load4(g, grad, first + k * 4, n, aligned);
+        if (aligned && first + kChunk <= n) {
+            float4 g[kChunk / 4 / kThreads];
 #pragma unroll
-            for (int j = 0; j < 4; j++) sum += g[j] * g[j];
+            for (int k = 0; k < kChunk / 4 / kThreads; k++) g[k] = load4<true>(grad, first + (k * kThreads + threadIdx.x) * 4, n);
+#pragma unroll
+            for (int k = 0; k < kChunk / 4 / kThreads; k++) sum += (g[k].x * g[k].x + g[k].y * g[k].y) + (g[k].z * g[k].z + g[k].w * g[k].w);
+        } else {
+            for (int k = threadIdx.x; k < kChunk / 4 && first + k * 4 < n; k += kThreads) {
+                const float4 g = load4<false>(grad, first + k * 4, n);
+                sum += (g.x * g.x + g.y * g.y) + (g.z * g.z + g.w * g.w);
+            }
         }
     }
     sum = warp_sum(sum);
