@@ -4,6 +4,7 @@
 // memory, then the heads.  Angles are counted in turns: the product of position and turns per position is made in 64 bits and
 // whole turns are taken off there, which leaves nothing of a long context's angles to lose in 32.
 #include "training.h"
+#include "two.h"
 
 namespace ffcvb {
 
@@ -13,12 +14,23 @@ using Args = ffcvb_rotary_args;
 
 constexpr int kThreads = 256;
 constexpr int kTileAngles = 2048; // angles of a tile (16 KB)
+constexpr int kAtOnce = 4;        // tokens that a thread has on their way
 
+// (a, b) -> (a c - b s, a s + b c) for pairs of either.
+__device__ __forceinline__ void turn(Two &a, Two &b, Two c, Two s) {
+    const Two x = fma_rn(b, s, mul_rn(a, c)); // (s: with the sign of the first)
+    b = fma_rn(a, mul_rn(s, Two(-1.0f, -1.0f)), mul_rn(b, c));
+    a = x;
+}
+
+// A head's slots: packs that turn (with their partners, half the rotated part on), then packs that are copied.  A thread has the same slot of the same
+// head of several tokens, one after the other; where a token has fewer slots than a CTA threads, tokens lie side by side.
 template <typename T, int N, bool INTERLEAVED>
 __global__ void __launch_bounds__(kThreads)
 rotary_kernel(const __grid_constant__ Args a, int tile) {
-    extern __shared__ float2 s_turn[]; // [tile][pairs]
-    const int pairs = (int)(a.rotary_dim / 2);
+    extern __shared__ float s_cos[]; // [tile][pairs], then the sines
+    const int pairs = (int)a.rotary_dim / 2;
+    float *const s_sin = s_cos + tile * pairs;
     const long long tiles = (a.tokens + tile - 1) / tile;
     const long long b = blockIdx.x / tiles, first = blockIdx.x % tiles * tile;
     const int tokens = (int)min((long long)tile, a.tokens - first);
@@ -30,62 +42,82 @@ rotary_kernel(const __grid_constant__ Args a, int tile) {
         const double turns = where * a.turns[i];
         float sine, cosine;
         sincospif((float)(2.0 * (turns - rint(turns))), &sine, &cosine);
-        s_turn[k] = make_float2(cosine * a.amplitude, (a.transpose ? -sine : sine) * a.amplitude);
+        s_cos[k] = cosine * a.amplitude;
+        s_sin[k] = (a.transpose ? sine : -sine) * a.amplitude;
     }
     __syncthreads();
-    // slots of a head: packs (and their partners, half the rotated part on) that turn, then packs that are copied
+    constexpr int PER = INTERLEAVED && N == 1 ? 2 : N; // values of a turning slot, or of a half of it
     const int half = (int)a.rotary_dim / 2;
-    const int turning = (INTERLEAVED ? (int)a.rotary_dim : half) / (INTERLEAVED && N == 1 ? 2 : N);
+    const int turning = (INTERLEAVED ? (int)a.rotary_dim : half) / PER;
     const int slots = turning + (int)(a.head_dim - a.rotary_dim) / N;
-    const int heads = (int)(a.heads + a.kv_heads);
-    for (int k = threadIdx.x; k < tokens * heads * slots; k += kThreads) {
-        const int slot = k % slots, h = k / slots % heads, t = k / slots / heads;
+    const int items = (int)(a.heads + a.kv_heads) * slots;
+    const int abreast = items < kThreads ? kThreads / items : 1; // tokens side by side
+    for (int item = items < kThreads ? threadIdx.x % items : threadIdx.x; item < items; item += kThreads) {
+        int t = items < kThreads ? threadIdx.x / items : 0;
+        if (t >= abreast) return;
+        const int slot = item % slots, h = item / slots;
         const bool key = h >= a.heads;
         const int64_t *in_stride = key ? a.k_stride : a.q_stride, *out_stride = key ? a.k_out_stride : a.q_out_stride;
-        const long long hh = key ? h - a.heads : h;
-        const T *in = static_cast<const T *>(key ? a.k : a.q) + b * in_stride[0] + (first + t) * in_stride[1] + hh * in_stride[2];
-        T *out = static_cast<T *>(key ? a.k_out : a.q_out) + b * out_stride[0] + (first + t) * out_stride[1] + hh * out_stride[2];
-        const float2 *turn = s_turn + t * pairs;
-        if (slot >= turning) {
-            const int at = (int)a.rotary_dim + (slot - turning) * N;
-            if (in != out) {
-                Pack<T, N> p;
-                p.load(in + at);
-                p.store(out + at);
-            }
-        } else if (!INTERLEAVED || N == 1) {
-            const int at = INTERLEAVED ? 2 * slot : slot * N, other = INTERLEAVED ? at + 1 : at + half;
-            Pack<T, N> p, q;
-            p.load(in + at);
-            q.load(in + other);
-            float u[N], v[N];
-            p.get(u);
-            q.get(v);
+        const long long head = key ? h - a.heads : h;
+        const bool turns = slot < turning;
+        const int at = turns ? slot * PER : (int)a.rotary_dim + (slot - turning) * N;
+        const int other = INTERLEAVED ? 1 : half; // from a value to its partner, where it is in another pack
+        const T *in = static_cast<const T *>(key ? a.k : a.q) + b * in_stride[0] + (first + t) * in_stride[1] + head * in_stride[2] + at;
+        T *out = static_cast<T *>(key ? a.k_out : a.q_out) + b * out_stride[0] + (first + t) * out_stride[1] + head * out_stride[2] + at;
+        const long long in_step = abreast * in_stride[1], out_step = abreast * out_stride[1];
+        if (!turns && in == out) continue;
+        constexpr bool TWO = !INTERLEAVED || N == 1; // partners in two packs
+        for (; t < tokens; t += kAtOnce * abreast, in += kAtOnce * in_step, out += kAtOnce * out_step) {
+            Pack<T, N> p[kAtOnce], q[kAtOnce];
 #pragma unroll
-            for (int j = 0; j < N; j++) {
-                const float2 cs = turn[slot * N + j];
-                const float x = u[j] * cs.x - v[j] * cs.y;
-                v[j] = u[j] * cs.y + v[j] * cs.x;
-                u[j] = x;
-            }
-            p.set(u);
-            q.set(v);
-            p.store(out + at);
-            q.store(out + other);
-        } else {
-            Pack<T, N> p;
-            p.load(in + slot * N);
-            float u[N];
-            p.get(u);
+            for (int i = 0; i < kAtOnce; i++)
+                if (t + i * abreast < tokens) {
+                    p[i].load_once(in + i * in_step);
+                    if (TWO && turns) q[i].load_once(in + i * in_step + other);
+                }
 #pragma unroll
-            for (int j = 0; j + 1 < N; j += 2) {
-                const float2 cs = turn[slot * (N / 2) + j / 2];
-                const float x = u[j] * cs.x - u[j + 1] * cs.y;
-                u[j + 1] = u[j] * cs.y + u[j + 1] * cs.x;
-                u[j] = x;
+            for (int i = 0; i < kAtOnce; i++) {
+                if (t + i * abreast >= tokens) break;
+                if (turns) {
+                    const int angle = (t + i * abreast) * pairs + (INTERLEAVED ? slot * PER / 2 : slot * N);
+                    const float *c = s_cos + angle, *s = s_sin + angle;
+                    if constexpr (N == 1) {
+                        float u[1], v[1];
+                        p[i].get(u);
+                        q[i].get(v);
+                        const float x[1] = {u[0] * c[0] + v[0] * s[0]}, y[1] = {v[0] * c[0] - u[0] * s[0]};
+                        p[i].set(x);
+                        q[i].set(y);
+                    } else if constexpr (INTERLEAVED) {
+                        float u[N];
+                        p[i].get(u);
+#pragma unroll
+                        for (int j = 0; j < N; j += 2) {
+                            const Two x = fma_rn(Two(u[j + 1], u[j]), Two(s[j / 2], -s[j / 2]), mul_rn(Two(u[j], u[j + 1]), Two(c[j / 2], c[j / 2])));
+                            u[j] = x.lo();
+                            u[j + 1] = x.hi();
+                        }
+                        p[i].set(u);
+                    } else {
+                        float u[N], v[N];
+                        p[i].get(u);
+                        q[i].get(v);
+#pragma unroll
+                        for (int j = 0; j < N; j += 4) {
+                            const float4 cc = *reinterpret_cast<const float4 *>(c + j), ss = *reinterpret_cast<const float4 *>(s + j);
+                            Two u0(u[j], u[j + 1]), u1(u[j + 2], u[j + 3]), v0(v[j], v[j + 1]), v1(v[j + 2], v[j + 3]);
+                            turn(u0, v0, Two(cc.x, cc.y), Two(ss.x, ss.y));
+                            turn(u1, v1, Two(cc.z, cc.w), Two(ss.z, ss.w));
+                            u[j] = u0.lo(), u[j + 1] = u0.hi(), u[j + 2] = u1.lo(), u[j + 3] = u1.hi();
+                            v[j] = v0.lo(), v[j + 1] = v0.hi(), v[j + 2] = v1.lo(), v[j + 3] = v1.hi();
+                        }
+                        p[i].set(u);
+                        q[i].set(v);
+                    }
+                }
+                p[i].store_once(out + i * out_step);
+                if (TWO && turns) q[i].store_once(out + i * out_step + other);
             }
-            p.set(u);
-            p.store(out + slot * N);
         }
     }
 }
@@ -111,6 +143,8 @@ extern "C" int ffcvb_rotary(const ffcvb_rotary_args *args, void *stream) {
     int tile = kTileAngles / pairs;
     if (tile > 16) tile = 16;
     if (tile < 1) tile = 1;
+    // fewer tokens per CTA where there are few: two CTAs for every SM
+    while (tile > 2 && a.batch * ((a.tokens + tile - 1) / tile) < 2 * kSms) tile /= 2;
     const long long ctas = a.batch * ((a.tokens + tile - 1) / tile);
     if (ctas > 0x7fffffff) return training_fail(FFCVB_E_LIMIT, "ffcvb_rotary: too many tokens");
     with_type(a.type, [&](auto zero) {
@@ -124,7 +158,7 @@ extern "C" int ffcvb_rotary(const ffcvb_rotary_args *args, void *stream) {
         if (a.kv_heads) low |= reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.k_out);
         const bool wide = (low & 15) == 0 && sizes % W == 0;
         auto run = [&](auto kernel) {
-            kernel<<<(unsigned)ctas, kThreads, (size_t)tile * pairs * sizeof(float2), static_cast<cudaStream_t>(stream)>>>(a, tile);
+            kernel<<<(unsigned)ctas, kThreads, (size_t)tile * pairs * 2 * sizeof(float), static_cast<cudaStream_t>(stream)>>>(a, tile);
         };
         if (wide)
             run(a.interleaved ? rotary_kernel<T, W, true> : rotary_kernel<T, W, false>);
