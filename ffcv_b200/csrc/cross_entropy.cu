@@ -55,74 +55,91 @@ __device__ __forceinline__ Picks picks_of(const ffcvb_cross_entropy_args &a, lon
     return p;
 }
 
-// N probabilities from place `at` on, those of classes [from, to) of the pack; 0 for the others.
+// N probabilities from class c of a row on.
 template <int N>
-__device__ __forceinline__ void probabilities(float (&p)[N], const ffcvb_cross_entropy_args &a, long long at, int from, int to, bool wide) {
+__device__ __forceinline__ void probabilities(float (&p)[N], const ffcvb_cross_entropy_args &a, long long at, bool wide) {
     if (N > 1 && wide && a.target_type == FFCVB_TYPE_F32) {
 #pragma unroll
         for (int j = 0; j < N; j += 4) {
-            float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (j < to && j + 4 > from) f = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.target) + at + j);
+            const float4 f = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.target) + at + j);
             p[j] = f.x, p[j + 1] = f.y, p[j + 2] = f.z, p[j + 3] = f.w;
         }
-#pragma unroll
-        for (int j = 0; j < N; j++)
-            if (j < from || j >= to) p[j] = 0.0f;
         return;
     }
 #pragma unroll
-    for (int j = 0; j < N; j++) {
-        p[j] = 0.0f;
-        if (j < from || j >= to) continue;
-        if (a.target_type == FFCVB_TYPE_F32)
-            p[j] = static_cast<const float *>(a.target)[at + j];
-        else if (a.target_type == FFCVB_TYPE_F16)
-            p[j] = to_float(static_cast<const __half *>(a.target)[at + j]);
-        else
-            p[j] = to_float(static_cast<const __nv_bfloat16 *>(a.target)[at + j]);
-    }
+    for (int j = 0; j < N; j++)
+        p[j] = a.target_type == FFCVB_TYPE_F32   ? static_cast<const float *>(a.target)[at + j]
+               : a.target_type == FFCVB_TYPE_F16 ? to_float(static_cast<const __half *>(a.target)[at + j])
+                                                 : to_float(static_cast<const __nv_bfloat16 *>(a.target)[at + j]);
 }
 
 __device__ __forceinline__ void copy16(uint32_t to, const void *from) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
 }
 
-// The largest logit of a row and the sum of exponentials relative to it, and what else is summed up.
+// The largest logit of a part of a row, at least kLowest, and the sum of exponentials relative to it; what else is summed up.  (Where all
+// logits are -inf the sum is 0: no difference here is that of two infinities of one sign, unless a logit is +inf.)
+constexpr float kLowest = -3.402823466e38f;
 struct Found {
     float top, sum, dot, mass;
-    // joins two parts of a row
     __device__ __forceinline__ void join(float t, float s, float d, float m) {
         const float most = fmaxf(top, t);
-        // (nothing but what is no number is added to a part without a maximum)
-        sum = (top == -INFINITY ? sum : sum * exp_of(top - most)) + (t == -INFINITY ? s : s * exp_of(t - most));
+        sum = sum * exp_of(top - most) + s * exp_of(t - most);
         top = most;
         dot += d;
         mass += m;
     }
-    template <bool MORE> __device__ __forceinline__ void join_warp() {
-        float most = warp_max(top);
-        sum = warp_sum(top == -INFINITY ? sum : sum * exp_of(top - most));
+    // joins those of groups of LANES lanes; `more`: dot and mass too
+    template <int LANES> __device__ __forceinline__ void join_lanes(bool more) {
+        float most = top;
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+        sum *= exp_of(top - most);
         top = most;
-        if (MORE) {
-            dot = warp_sum(dot);
-            mass = warp_sum(mass);
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (!more) return;
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) mass += __shfl_xor_sync(0xffffffffu, mass, o);
+    }
+    template <int N> __device__ __forceinline__ void add(const float (&v)[N]) {
+        float most = fmaxf(top, v[0]);
+#pragma unroll
+        for (int j = 1; j < N; j++) most = fmaxf(most, v[j]);
+        sum *= exp_of(top - most);
+        top = most;
+        if constexpr (N == 1) {
+            sum += exp_of(v[0] - top);
+        } else {
+            Two part[2] = {Two(0.0f, 0.0f), Two(0.0f, 0.0f)};
+            const Two minus(-top, -top), log2e(kLog2e, kLog2e);
+#pragma unroll
+            for (int j = 0; j < N; j += 2) {
+                const Two d = mul_rn(add_rn(Two(v[j], v[j + 1]), minus), log2e);
+                part[j / 2 & 1] = add_rn(part[j / 2 & 1], Two(exp2_of(d.lo()), exp2_of(d.hi())));
+            }
+            part[0] = add_rn(part[0], part[1]);
+            sum += part[0].lo() + part[0].hi();
         }
     }
 };
 
-// How rows are dealt out: packs of a CTA's part of a row; whether parts are copied to shared memory; whether probabilities can be read
-// 16 bytes at a time.
+// How rows are dealt out: whether logits and gradient lie alike to 16-byte boundaries; packs of a CTA's part of a row; whether
+// probabilities can be read 16 bytes at a time.
 struct Deal {
-    int part, staged, soft_wide;
+    int wide, part, soft_wide;
 };
 
-// WIDE: 16 bytes at a time from the 16-byte boundary at or before the row on (what lies before the row there is left out); logits and
-// gradient then lie alike to these boundaries.  WARP: a row per warp, four warps per CTA.
-template <typename T, bool WIDE, bool SOFT, bool WARP>
-__global__ void __launch_bounds__(WARP ? 128 : 512)
+// A row's packs of 16 bytes are dealt out to its threads in turn; the few logits before and behind them (all, where logits and
+// gradient lie differently to 16-byte boundaries) are taken one by one.  WARP: a row per warp, four warps per CTA; else a row per
+// CTA or cluster.  STAGED: the packs go through shared memory; else they are read where they are needed.
+template <typename T, bool STAGED, bool SOFT, bool WARP>
+__global__ void __launch_bounds__(WARP ? 128 : 256)
 rows_kernel(const __grid_constant__ ffcvb_cross_entropy_args a, const Deal deal) {
-    constexpr int N = WIDE ? kWide<T> : 1;
-    __shared__ float4 s_part[16];
+    constexpr int N = kWide<T>, BATCH = STAGED ? 2 : 4; // packs that a thread works on together
+    __shared__ float4 s_part[8];
     __shared__ float4 s_there[8]; // from the cluster's CTAs
     extern __shared__ uint4 s_row[];
     uint32_t rank = 0, ranks = 1;
@@ -137,34 +154,33 @@ rows_kernel(const __grid_constant__ ffcvb_cross_entropy_args a, const Deal deal)
     const int classes = (int)a.classes;
     const T *x = static_cast<const T *>(a.logits) + row * a.logits_stride;
     T *g = a.grad ? static_cast<T *>(a.grad) + row * a.grad_stride : nullptr;
-    const int lead = WIDE ? (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T)) : 0;
-    const int packs = (lead + classes + N - 1) / N;
-    // this CTA's packs, [first, last); the row's first and last are not wholly of the row
-    const int first = (int)rank * deal.part, last = min(packs, first + deal.part);
-    const int head = lead > 0 ? 0 : -1, tail = (lead + classes) % N ? packs - 1 : -1;
-    const T *x0 = x - lead;
+    // logits before the packs, packs of the row and of this CTA's part, logits besides packs
+    const int lead = (int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / (int)sizeof(T);
+    const int before = deal.wide && lead < classes ? lead : classes;
+    const int packs = (classes - before) / N, singles = classes - packs * N;
+    const int first = (int)rank * deal.part, count = max(0, min(packs - first, deal.part));
+    const T *x0 = x + before + (long long)first * N;
     const uint32_t mine = (uint32_t)__cvta_generic_to_shared(s_row + (WARP ? (threadIdx.x >> 5) * deal.part : 0) + thread);
-    const bool staged = WIDE && deal.staged && !a.from_stats;
-    if (staged) {
+    if (STAGED) {
         uint32_t to = mine;
-        for (int k = first + thread; k < last; k += threads, to += threads * 16) copy16(to, x0 + (long long)k * N);
+        for (int k = thread; k < count; k += threads, to += threads * 16) copy16(to, x0 + (long long)k * N);
         asm volatile("cp.async.commit_group;" ::: "memory");
     }
+    auto single = [&](int k) { return k < before ? k : k + packs * N; }; // class of the k-th besides packs
     const Picks p = picks_of(a, row);
     if (p.ignored || p.bad) { // (all of a cluster's CTAs alike)
-        if (ranks > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
-        const float v = p.ignored ? 0.0f : NAN;
+        const T v = from_float<T>(p.ignored ? 0.0f : NAN);
         if (g)
-            for (long long c = (long long)first * N - lead + thread; c < (long long)last * N - lead && c < classes; c += threads)
-                if (c >= 0) g[c] = from_float<T>(v);
+            for (int c = (int)rank * threads + thread; c < classes; c += (int)ranks * threads) g[c] = v;
         if (thread == 0 && rank == 0 && !a.from_stats) {
-            a.row_loss[row] = v;
-            if (a.stats) reinterpret_cast<float2 *>(a.stats)[row] = make_float2(v, v);
+            a.row_loss[row] = to_float(v);
+            if (a.stats) reinterpret_cast<float2 *>(a.stats)[row] = make_float2(to_float(v), to_float(v));
         }
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        if (STAGED) asm volatile("cp.async.wait_group 0;" ::: "memory");
+        if (ranks > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
         return;
     }
-    const long long soft_row = row * a.target_stride - lead;
+    const long long soft_row = row * a.target_stride;
     const float sure = 1.0f - a.smoothing;
     float picked = 0.0f; // of the labels' logits
     if (!SOFT && thread == 0 && rank == 0 && !a.from_stats) {
@@ -172,87 +188,71 @@ rows_kernel(const __grid_constant__ ffcvb_cross_entropy_args a, const Deal deal)
         for (int k = 0; k < 2; k++)
             if (p.weight[k] != 0.0f) picked += p.weight[k] * to_float(x[p.label[k]]);
     }
-    // classes [from, to) of pack k are the row's
-    auto ends = [&](int k, int &from, int &to) {
-        from = k == head ? lead : 0;
-        to = k == tail ? lead + classes - k * N : N;
-    };
-    auto fetch = [&](Pack<T, N> &pack, int k, uint32_t from) {
-        if (staged) {
-            if constexpr (WIDE)
-                asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(pack.raw.x), "=r"(pack.raw.y), "=r"(pack.raw.z), "=r"(pack.raw.w) : "r"(from) : "memory");
-        } else {
-            pack.load(x0 + (long long)k * N);
+    // Calls f(values, class of the first) for this thread's packs, of which BATCH are on their way at a time.
+    auto each_pack = [&](auto &&f) {
+        uint32_t at = mine;
+        for (int k = thread; k < count; k += BATCH * threads, at += BATCH * threads * 16) {
+            Pack<T, N> pack[BATCH];
+#pragma unroll
+            for (int i = 0; i < BATCH; i++)
+                if (k + i * threads < count) {
+                    if constexpr (STAGED) {
+                        uint4 &r = pack[i].raw;
+                        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(at + i * threads * 16) : "memory");
+                    } else {
+                        pack[i].load(x0 + (long long)(k + i * threads) * N);
+                    }
+                }
+#pragma unroll
+            for (int i = 0; i < BATCH; i++)
+                if (k + i * threads < count) {
+                    float v[N];
+                    pack[i].get(v);
+                    f(v, before + (first + k + i * threads) * N);
+                }
         }
+    };
+    auto each_single = [&](auto &&f) {
+        for (int k = (int)rank * threads + thread; k < singles; k += (int)ranks * threads) f(single(k));
     };
     if (ranks > 1 && a.from_stats) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
     float row_top, over, total = p.total; // (over: 1 / sum of exp(x - row_top), 0 where there is nothing)
     if (!a.from_stats) {
-        Found f{-INFINITY, 0.0f, 0.0f, 0.0f};
-        float base = 0.0f; // top, where there is one
-        if (staged) asm volatile("cp.async.wait_group 0;" ::: "memory");
-        uint32_t at = mine;
-#pragma unroll 2
-        for (int k = first + thread; k < last; k += threads, at += threads * 16) {
-            Pack<T, N> pack;
-            fetch(pack, k, at);
-            float v[N];
-            pack.get(v);
-            if (WIDE && (k == head || k == tail)) {
-                int from, to;
-                ends(k, from, to);
-#pragma unroll
-                for (int j = 0; j < N; j++)
-                    if (j < from || j >= to) v[j] = -INFINITY;
-            }
+        Found f{kLowest, 0.0f, 0.0f, 0.0f};
+        auto take = [&](auto &v, int c) {
+            constexpr int M = sizeof(v) / 4;
             if (SOFT) {
-                int from, to;
-                ends(k, from, to);
-                float t[N];
-                probabilities<N>(t, a, soft_row + (long long)k * N, from, to, deal.soft_wide);
+                float t[M];
+                probabilities<M>(t, a, soft_row + c, deal.soft_wide);
 #pragma unroll
-                for (int j = 0; j < N; j++) {
-                    t[j] = j >= from && j < to ? sure * t[j] + p.flat : 0.0f;
+                for (int j = 0; j < M; j++) {
+                    t[j] = sure * t[j] + p.flat;
                     f.mass += t[j];
                     if (t[j] > 0.0f) f.dot += t[j] * v[j];
                 }
             } else if (p.flat > 0.0f) {
-                int from, to;
-                ends(k, from, to);
-                float part = 0.0f;
+                float part = v[0];
 #pragma unroll
-                for (int j = 0; j < N; j++) part += j >= from && j < to ? v[j] : 0.0f;
+                for (int j = 1; j < M; j++) part += v[j];
                 f.dot += p.flat * part;
             }
-            float most = v[0];
-#pragma unroll
-            for (int j = 1; j < N; j++) most = fmaxf(most, v[j]);
-            if (most > f.top) {
-                if (f.top != -INFINITY) f.sum *= exp_of(f.top - most);
-                f.top = base = most;
-            }
-            if constexpr (N == 1) {
-                f.sum += exp_of(v[0] - base);
-            } else {
-                Two part(0.0f, 0.0f);
-                const Two minus(-base, -base), log2e(kLog2e, kLog2e);
-#pragma unroll
-                for (int j = 0; j < N; j += 2) {
-                    const Two d = mul_rn(add_rn(Two(v[j], v[j + 1]), minus), log2e);
-                    part = add_rn(part, Two(exp2_of(d.lo()), exp2_of(d.hi())));
-                }
-                f.sum += part.lo() + part.hi();
-            }
-        }
-        f.dot += picked;
-        f.join_warp<true>();
+            f.add(v);
+        };
+        each_single([&](int c) {
+            const float v[1] = {to_float(x[c])};
+            take(v, c);
+        });
+        if (STAGED) asm volatile("cp.async.wait_group 0;" ::: "memory");
+        each_pack(take);
+        const bool more = SOFT || p.flat > 0.0f;
+        f.join_lanes<32>(more);
         if (!WARP) {
             const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
             if (lane == 0) s_part[threadIdx.x >> 5] = make_float4(f.top, f.sum, f.dot, f.mass);
             __syncthreads();
-            const float4 other = lane < warps ? s_part[lane] : make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
+            const float4 other = (lane & 7) < warps ? s_part[lane & 7] : make_float4(kLowest, 0.0f, 0.0f, 0.0f); // (at most eight)
             f = Found{other.x, other.y, other.z, other.w};
-            f.join_warp<true>();
+            f.join_lanes<8>(more);
             if (ranks > 1) {
                 asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); // all have begun
                 if (threadIdx.x < ranks) {
@@ -265,11 +265,11 @@ rows_kernel(const __grid_constant__ ffcvb_cross_entropy_args a, const Deal deal)
                 for (uint32_t k = 1; k < ranks; k++) f.join(s_there[k].x, s_there[k].y, s_there[k].z, s_there[k].w);
             }
         }
-        row_top = f.top == -INFINITY ? 0.0f : f.top;
+        row_top = f.top;
         over = f.sum == 0.0f ? 0.0f : 1.0f / f.sum;
         if (SOFT) total = f.mass;
         if (thread == 0 && rank == 0) {
-            a.row_loss[row] = f.sum == 0.0f ? 0.0f : total * (row_top + logf(f.sum)) - f.dot;
+            a.row_loss[row] = f.sum == 0.0f ? 0.0f : total * (row_top + logf(f.sum)) - (f.dot + picked);
             if (a.stats) reinterpret_cast<float2 *>(a.stats)[row] = make_float2(row_top, over);
         }
     } else {
@@ -278,13 +278,10 @@ rows_kernel(const __grid_constant__ ffcvb_cross_entropy_args a, const Deal deal)
         over = stats.y;
         if (SOFT) { // the whole row's, by every CTA of a cluster
             float mass = 0.0f;
-            for (int k = thread; k < packs; k += threads) {
-                int from, to;
-                ends(k, from, to);
-                float t[N];
-                probabilities<N>(t, a, soft_row + (long long)k * N, from, to, deal.soft_wide);
-#pragma unroll
-                for (int j = 0; j < N; j++) mass += j >= from && j < to ? sure * t[j] + p.flat : 0.0f;
+            for (int c = thread; c < classes; c += threads) {
+                float t[1];
+                probabilities<1>(t, a, soft_row + c, false);
+                mass += sure * t[0] + p.flat;
             }
             mass = warp_sum(mass);
             if (!WARP) {
@@ -302,52 +299,46 @@ rows_kernel(const __grid_constant__ ffcvb_cross_entropy_args a, const Deal deal)
     if (a.mean) k_row /= a.has_ignore ? fmaxf(a.counted[0], 1.0f) : (float)a.rows;
     if (over == 0.0f) k_row = 0.0f;
     const float factor = k_row * total * over, flat = k_row * p.flat;
-    T *g0 = g - lead;
-    // packs of the labels
-    const int at0 = p.label[0] < 0 ? -1 : ((int)p.label[0] + lead) / N, at1 = p.label[1] < 0 ? -1 : ((int)p.label[1] + lead) / N;
-    uint32_t at = mine;
-#pragma unroll 2
-    for (int k = first + thread; k < last; k += threads, at += threads * 16) {
-        Pack<T, N> pack;
-        fetch(pack, k, at);
-        float v[N];
-        pack.get(v);
-        if constexpr (N == 1) {
-            v[0] = factor * exp_of(v[0] - row_top) - flat;
+    each_single([&](int c) {
+        float v = factor * exp_of(to_float(x[c]) - row_top) - flat;
+        if (SOFT) {
+            float t[1];
+            probabilities<1>(t, a, soft_row + c, false);
+            v -= k_row * sure * t[0];
         } else {
-            const Two minus(-row_top, -row_top), log2e(kLog2e, kLog2e), less(-flat, -flat), times(factor, factor);
 #pragma unroll
-            for (int j = 0; j < N; j += 2) {
-                const Two d = mul_rn(add_rn(Two(v[j], v[j + 1]), minus), log2e);
-                const Two e = fma_rn(Two(exp2_of(d.lo()), exp2_of(d.hi())), times, less);
-                v[j] = e.lo();
-                v[j + 1] = e.hi();
-            }
+            for (int k = 0; k < 2; k++)
+                if (c == (int)p.label[k]) v -= k_row * p.weight[k];
+        }
+        g[c] = from_float<T>(v);
+    });
+    const Two minus(-row_top, -row_top), log2e(kLog2e, kLog2e), less(-flat, -flat), times(factor, factor);
+    each_pack([&](float(&v)[N], int c) {
+#pragma unroll
+        for (int j = 0; j < N; j += 2) {
+            const Two d = mul_rn(add_rn(Two(v[j], v[j + 1]), minus), log2e);
+            const Two e = fma_rn(Two(exp2_of(d.lo()), exp2_of(d.hi())), times, less);
+            v[j] = e.lo();
+            v[j + 1] = e.hi();
         }
         if (SOFT) {
-            int from, to;
-            ends(k, from, to);
             float t[N];
-            probabilities<N>(t, a, soft_row + (long long)k * N, from, to, deal.soft_wide);
+            probabilities<N>(t, a, soft_row + c, deal.soft_wide);
 #pragma unroll
             for (int j = 0; j < N; j++) v[j] -= k_row * sure * t[j];
-        } else if (k == at0 || k == at1) {
-#pragma unroll
-            for (int j = 0; j < N; j++) {
-                const int c = k * N + j - lead;
-                if (c == (int)p.label[0]) v[j] -= k_row * p.weight[0];
-                if (c == (int)p.label[1]) v[j] -= k_row * p.weight[1];
-            }
         }
+        Pack<T, N> pack;
         pack.set(v);
-        if (!WIDE || (k != head && k != tail)) {
-            pack.store_once(g0 + (long long)k * N);
-        } else {
-            int from, to;
-            ends(k, from, to);
+        pack.store_once(g + c);
+    });
+    if (!SOFT) { // the labels' classes in packs: the thread that has just written them writes them again
 #pragma unroll
-            for (int j = 0; j < N; j++)
-                if (j >= from && j < to) g0[(long long)k * N + j] = from_float<T>(v[j]);
+        for (int k = 0; k < 2; k++) {
+            const int c = (int)p.label[k], in = c - before;
+            if (c < 0 || in < 0 || in >= packs * N || in / N < first || (in / N - first) % threads != thread || in / N - first >= count) continue;
+            float v = factor * exp_of(to_float(x[c]) - row_top) - flat - k_row * p.weight[k];
+            if (p.label[0] == p.label[1]) v -= k_row * p.weight[k ^ 1];
+            g[c] = from_float<T>(v);
         }
     }
 }
@@ -392,27 +383,29 @@ template <typename T>
 void launch_rows(const ffcvb_cross_entropy_args &a, cudaStream_t stream) {
     constexpr int W = 16 / (int)sizeof(T);
     const uintptr_t apart = reinterpret_cast<uintptr_t>(a.logits) ^ reinterpret_cast<uintptr_t>(a.grad);
-    const bool wide = !a.grad || ((apart & 15) == 0 && (a.logits_stride - a.grad_stride) * (long long)sizeof(T) % 16 == 0);
-    const bool soft = a.target_kind == FFCVB_TARGET_SOFT;
-    const long long packs = wide ? (a.classes + W - 1) / W + 1 : a.classes; // (at most one more than without a lead)
+    const bool soft = a.target_kind == FFCVB_TARGET_SOFT, both = a.grad && !a.from_stats; // (both passes)
     Deal deal{};
-    deal.staged = wide && a.grad && !a.from_stats;
-    // probabilities lie to 16-byte boundaries as the logits' packs do: same stride, both begin on one
+    deal.wide = !a.grad || ((apart & 15) == 0 && (a.logits_stride - a.grad_stride) % W == 0);
+    // probabilities lie to 16-byte boundaries as the logits' packs do: strides differ by whole packs, both begin on one
     deal.soft_wide = soft && ((reinterpret_cast<uintptr_t>(a.logits) | reinterpret_cast<uintptr_t>(a.target)) & 15) == 0 &&
                      (a.logits_stride - a.target_stride) % W == 0;
+    const long long packs = deal.wide ? a.classes / W : 0; // (at most)
     cudaLaunchConfig_t how{};
     cudaLaunchAttribute cluster{};
     how.stream = stream;
     auto run = [&](auto kernel) {
-        if (how.dynamicSmemBytes > 40 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)how.dynamicSmemBytes);
+        if (how.dynamicSmemBytes > 40 * 1024) {
+            cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)how.dynamicSmemBytes);
+            cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+        }
         cudaLaunchKernelEx(&how, kernel, a, deal);
     };
     if (a.classes <= kWarpClasses) {
         deal.part = (int)packs;
         how.gridDim = dim3((unsigned)((a.rows + 3) / 4));
         how.blockDim = dim3(128);
-        how.dynamicSmemBytes = deal.staged ? 4 * packs * 16 : 0;
-        if (wide)
+        how.dynamicSmemBytes = both ? 4 * packs * 16 : 0;
+        if (both)
             run(soft ? rows_kernel<T, true, true, true> : rows_kernel<T, true, false, true>);
         else
             run(soft ? rows_kernel<T, false, true, true> : rows_kernel<T, false, false, true>);
@@ -420,19 +413,19 @@ void launch_rows(const ffcvb_cross_entropy_args &a, cudaStream_t stream) {
     }
     // CTAs per row: until a part fits, and until there are two CTAs per SM (with few rows) of parts that are worth it
     int ctas = 1;
-    while (ctas < 8 && ((deal.staged && (packs + ctas - 1) / ctas * 16 > kPartBytes) || (a.rows * ctas * 2 <= 2 * kSms && packs > 2048 * ctas))) ctas *= 2;
+    while (ctas < 8 && ((both && (packs + ctas - 1) / ctas * 16 > kPartBytes) || (a.rows * ctas <= kSms && packs > 2048 * ctas))) ctas *= 2;
     deal.part = (int)((packs + ctas - 1) / ctas);
-    if (deal.staged && deal.part * 16ll > kPartBytes) deal.staged = 0; // (then the second pass reads what the caches still have)
-    const int threads = (deal.part / 8 + 31) / 32 * 32;
+    const bool staged = both && deal.part * 16ll <= kPartBytes; // (else the second pass reads what the caches still have)
+    const int threads = (deal.part / 16 + 31) / 32 * 32;
     how.gridDim = dim3((unsigned)(a.rows * ctas));
-    how.blockDim = dim3(threads < 64 ? 64 : threads > 320 ? 320 : threads);
-    how.dynamicSmemBytes = deal.staged ? deal.part * 16ll : 0;
+    how.blockDim = dim3(!deal.wide || threads > 256 ? 256 : threads < 64 ? 64 : threads);
+    how.dynamicSmemBytes = staged ? deal.part * 16ll : 0;
     cluster.id = cudaLaunchAttributeClusterDimension;
     cluster.val.clusterDim.x = ctas;
     cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
     how.attrs = &cluster;
     how.numAttrs = ctas > 1;
-    if (wide)
+    if (staged)
         run(soft ? rows_kernel<T, true, true, false> : rows_kernel<T, true, false, false>);
     else
         run(soft ? rows_kernel<T, false, true, false> : rows_kernel<T, false, false, false>);
