@@ -253,6 +253,7 @@ step_kernel(const __grid_constant__ Launch<MOST> a) {
     if (!grad) return;
     float clip = 1.0f;
     if (a.norm) {
+        wait_for_previous();
         const float norm = *a.norm;
         if (!isfinite(norm)) return;
         clip = fminf(1.0f, a.max_norm / (norm + 1e-6f));
@@ -277,6 +278,7 @@ template <typename T, int MOST>
 __global__ void __launch_bounds__(kThreads)
 squares_kernel(const __grid_constant__ Launch<MOST> a) {
     __shared__ float s_part[kThreads / 32];
+    let_next_begin();
     const unsigned which = gridDim.x - 1 - blockIdx.x;
     const Chunk chunk = a.chunks[which];
     const int local = chunk.tensor - a.first;
@@ -312,6 +314,8 @@ squares_kernel(const __grid_constant__ Launch<MOST> a) {
 __global__ void __launch_bounds__(1024)
 norm_kernel(const float *__restrict__ partial, long long n, float *norm) {
     __shared__ double s_sum[32];
+    wait_for_previous();
+    let_next_begin();
     double sum = 0.0;
     for (long long k = threadIdx.x; k < n; k += 1024) sum += partial[k];
 #pragma unroll
@@ -388,12 +392,13 @@ void launch_all(const ffcvb_adamw_args &args, const Tensors &t, bool squares, cu
         a.max_norm = (float)args.max_norm;
         a.partial = static_cast<float *>(args.workspace) + at;
         if (count > 0 && (any || squares)) {
+            auto step = args.bits == 8 ? step_kernel<T, 8, MOST> : step_kernel<T, 32, MOST>;
             if (squares)
                 squares_kernel<T, MOST><<<(unsigned)count, kThreads, 0, st>>>(a);
-            else if (args.bits == 8)
-                step_kernel<T, 8, MOST><<<(unsigned)count, kThreads, 0, st>>>(a);
+            else if (a.norm && first == 0) // right behind the norm
+                launch_early(step, (unsigned)count, kThreads, 0, st, a);
             else
-                step_kernel<T, 32, MOST><<<(unsigned)count, kThreads, 0, st>>>(a);
+                step<<<(unsigned)count, kThreads, 0, st>>>(a);
         }
         first += n;
         at += count;
@@ -465,7 +470,7 @@ int ffcvb_adamw_step(const ffcvb_adamw_args *args, const int64_t *numel, const u
         };
         if (a.max_norm > 0.0) {
             all(true);
-            norm_kernel<<<1, 1024, 0, st>>>(static_cast<const float *>(a.workspace), t.chunks, a.norm);
+            launch_early(norm_kernel, 1, 1024, 0, st, static_cast<const float *>(a.workspace), t.chunks, a.norm);
         }
         all(false);
     });

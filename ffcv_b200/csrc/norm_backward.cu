@@ -218,6 +218,7 @@ backward_kernel(const __grid_constant__ Args a, const Deal deal, const Partials 
                 store_floats(dg, part.gate + unit * a.width, c);
         }
     }
+    let_next_begin();
     float *to = part.columns + (long long)cluster * deal.columns * a.width;
     auto put = [&](const Eight &v, const void *wanted) {
         if (!wanted) return;

@@ -25,6 +25,7 @@ struct Sums {
 __global__ void __launch_bounds__(1024)
 add_up_kernel(const __grid_constant__ Sums s) {
     __shared__ float s_part[8][129];
+    wait_for_previous();
     const int column = threadIdx.x & 7, run = threadIdx.x >> 3;
     const long long c = blockIdx.x * 8ll + column;
     const float *from = s.from[blockIdx.y];
@@ -53,6 +54,7 @@ add_up_kernel(const __grid_constant__ Sums s) {
 template <typename T>
 __global__ void __launch_bounds__(256)
 gates_kernel(const float *__restrict__ partial, T *__restrict__ dgate, long long width, long long splits, long long values) {
+    wait_for_previous();
     const long long at = blockIdx.x * 256ll + threadIdx.x;
     if (at >= values) return;
     const long long sample = at / width;
@@ -187,12 +189,12 @@ int ffcvb_norm_residual_backward(const ffcvb_norm_residual_args *args, void *str
     s.stride = d.columns * a.width;
     s.type = a.param_type;
     const unsigned across = (unsigned)((a.width + 7) / 8);
-    if (n) add_up_kernel<<<dim3(across, n), 1024, 0, st>>>(s);
+    if (n) launch_early(add_up_kernel, dim3(across, n), 1024, 0, st, s);
     if (a.dgate && a.gate_kind == FFCVB_GATE_SAMPLE && d.splits > 1 && a.rows > 0) // (then there are fewer samples than CTAs, or few splits)
         with_type(a.type, [&](auto zero) {
             using T = decltype(zero);
             const long long values = d.samples * a.width;
-            gates_kernel<T><<<(unsigned)((values + 255) / 256), 256, 0, st>>>(part.gate, static_cast<T *>(a.dgate), a.width, d.splits, values);
+            launch_early(gates_kernel<T>, (unsigned)((values + 255) / 256), 256, 0, st, part.gate, static_cast<T *>(a.dgate), a.width, d.splits, values);
         });
     return launched("ffcvb_norm_residual_backward");
 }

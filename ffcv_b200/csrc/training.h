@@ -53,6 +53,25 @@ inline int type_size(int type) { return type == FFCVB_TYPE_F32 ? 4 : 2; }
 
 #ifdef __CUDACC__
 
+// Programmatic launches: a kernel launched by launch_early may begin once every CTA of the one before it has called let_next_begin() or
+// ended; it calls wait_for_previous() before it touches what earlier kernels of the stream wrote or read.
+template <typename... Params, typename... Given>
+cudaError_t launch_early(void (*kernel)(Params...), dim3 grid, dim3 block, size_t room, cudaStream_t stream, Given &&...given) {
+    cudaLaunchConfig_t how{};
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    how.gridDim = grid;
+    how.blockDim = block;
+    how.dynamicSmemBytes = room;
+    how.stream = stream;
+    how.attrs = &early;
+    how.numAttrs = 1;
+    return cudaLaunchKernelEx(&how, kernel, static_cast<Params>(given)...);
+}
+__device__ __forceinline__ void let_next_begin() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 __device__ __forceinline__ float to_float(float v) { return v; }
 __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
 __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
