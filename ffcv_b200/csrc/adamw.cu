@@ -247,13 +247,14 @@ __device__ __forceinline__ void step_unit(const Args &a, const Set &set, float c
 template <typename T, int BITS, int MOST>
 __global__ void __launch_bounds__(kThreads)
 step_kernel(const __grid_constant__ Launch<MOST> a) {
+    wait_for_previous();
+    let_next_begin();
     const Chunk chunk = a.chunks[blockIdx.x];
     const int local = chunk.tensor - a.first;
     const T *grad = static_cast<const T *>(a.grads[local]);
     if (!grad) return;
     float clip = 1.0f;
     if (a.norm) {
-        wait_for_previous();
         const float norm = *a.norm;
         if (!isfinite(norm)) return;
         clip = fminf(1.0f, a.max_norm / (norm + 1e-6f));
@@ -278,6 +279,7 @@ template <typename T, int MOST>
 __global__ void __launch_bounds__(kThreads)
 squares_kernel(const __grid_constant__ Launch<MOST> a) {
     __shared__ float s_part[kThreads / 32];
+    wait_for_previous();
     let_next_begin();
     const unsigned which = gridDim.x - 1 - blockIdx.x;
     const Chunk chunk = a.chunks[which];
@@ -393,12 +395,7 @@ void launch_all(const ffcvb_adamw_args &args, const Tensors &t, bool squares, cu
         a.partial = static_cast<float *>(args.workspace) + at;
         if (count > 0 && (any || squares)) {
             auto step = args.bits == 8 ? step_kernel<T, 8, MOST> : step_kernel<T, 32, MOST>;
-            if (squares)
-                squares_kernel<T, MOST><<<(unsigned)count, kThreads, 0, st>>>(a);
-            else if (a.norm && first == 0) // right behind the norm
-                launch_early(step, (unsigned)count, kThreads, 0, st, a);
-            else
-                step<<<(unsigned)count, kThreads, 0, st>>>(a);
+            launch_early(squares ? squares_kernel<T, MOST> : step, (unsigned)count, kThreads, 0, st, a);
         }
         first += n;
         at += count;
@@ -441,8 +438,8 @@ int ffcvb_adamw_table(int32_t n, const int64_t *numel, const uint64_t *params, v
     return FFCVB_OK;
 }
 
-int ffcvb_adamw_step(const ffcvb_adamw_args *args, const int64_t *numel, const uint64_t *grads, int64_t *steps,
-                     const int32_t *group_of, const ffcvb_adamw_group *groups, int32_t n_groups, void *stream) {
+int ffcvb_adamw_step(const ffcvb_adamw_args *args, const int64_t *numel, int64_t *steps, const int32_t *group_of,
+                     const uint64_t *grads, const ffcvb_adamw_group *groups, int32_t n_groups, void *stream) {
     if (!args || args->n_tensors < 0) return training_fail(FFCVB_E_ARG, "ffcvb_adamw_step: no arguments");
     const ffcvb_adamw_args &a = *args;
     if (a.n_tensors == 0) return FFCVB_OK;

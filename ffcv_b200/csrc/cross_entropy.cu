@@ -142,6 +142,9 @@ rows_kernel(const __grid_constant__ ffcvb_cross_entropy_args a, const Deal deal)
     __shared__ float4 s_part[8];
     __shared__ float4 s_there[8]; // from the cluster's CTAs
     extern __shared__ uint4 s_row[];
+    const bool counted = a.has_ignore && a.mean; // by the kernel before this one, which waited for all before it
+    if (!counted) wait_for_previous();
+    let_next_begin();
     uint32_t rank = 0, ranks = 1;
     if (!WARP) {
         asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
@@ -178,6 +181,7 @@ rows_kernel(const __grid_constant__ ffcvb_cross_entropy_args a, const Deal deal)
         }
         if (STAGED) asm volatile("cp.async.wait_group 0;" ::: "memory");
         if (ranks > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+        if (counted) wait_for_previous();
         return;
     }
     const long long soft_row = row * a.target_stride;
@@ -293,9 +297,8 @@ rows_kernel(const __grid_constant__ ffcvb_cross_entropy_args a, const Deal deal)
             total = mass;
         }
     }
-    let_next_begin();
+    if (counted) wait_for_previous();
     if (!g) return;
-    if (a.has_ignore && a.mean) wait_for_previous(); // for the count, the only thing that the kernel before this one can have made
     float k_row = a.scale;
     if (a.upstream) k_row *= a.upstream[a.upstream_per_row ? row : 0];
     if (a.mean) k_row /= a.has_ignore ? fmaxf(a.counted[0], 1.0f) : (float)a.rows;
@@ -349,7 +352,8 @@ rows_kernel(const __grid_constant__ ffcvb_cross_entropy_args a, const Deal deal)
 __global__ void __launch_bounds__(1024)
 count_kernel(const int64_t *__restrict__ labels, long long rows, long long stride, long long ignore, float *counted) {
     __shared__ int s_count[32];
-    let_next_begin(); // (all that is before this kernel has ended)
+    wait_for_previous();
+    let_next_begin(); // (so all that is before this kernel has ended when the next one begins)
     int n = 0;
     for (long long i = threadIdx.x; i < rows; i += 1024) n += labels[i * stride] != ignore;
     n = __reduce_add_sync(0xffffffffu, n);
@@ -398,11 +402,9 @@ void launch_rows(const ffcvb_cross_entropy_args &a, cudaStream_t stream) {
     cudaLaunchAttribute with[2] = {};
     how.stream = stream;
     how.attrs = with;
-    if (a.has_ignore && a.mean) { // behind the count
-        with[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        with[0].val.programmaticStreamSerializationAllowed = 1;
-        how.numAttrs = 1;
-    }
+    with[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    with[0].val.programmaticStreamSerializationAllowed = 1;
+    how.numAttrs = 1;
     auto run = [&](auto kernel) {
         if (how.dynamicSmemBytes > 40 * 1024) {
             cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)how.dynamicSmemBytes);
@@ -461,7 +463,7 @@ extern "C" int ffcvb_cross_entropy(const ffcvb_cross_entropy_args *args, void *s
     OnDevice here(a.device);
     if (!here.ok()) return training_fail(FFCVB_E_NODEVICE, "ffcvb_cross_entropy: no device %d", a.device);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (needs_count) count_kernel<<<1, 1024, 0, st>>>(static_cast<const int64_t *>(a.target), a.rows, a.target_stride, a.ignore_index, a.counted);
+    if (needs_count) launch_early(count_kernel, 1, 1024, 0, st, static_cast<const int64_t *>(a.target), a.rows, a.target_stride, a.ignore_index, a.counted);
     if (a.rows > 0) with_type(a.type, [&](auto zero) { launch_rows<decltype(zero)>(a, st); });
     if (a.loss && !a.from_stats) launch_early(mean_kernel, 1, 1024, 0, st, a.row_loss, a.rows, needs_count ? a.counted : nullptr, a.mean, a.loss);
     return launched("ffcvb_cross_entropy");

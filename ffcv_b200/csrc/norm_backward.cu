@@ -26,6 +26,7 @@ backward_kernel(const __grid_constant__ Args a, const Deal deal, const Partials 
     }
     RowSum<MULTI> sum{s_sum, shape.ctas_per_row};
     sum.begin();
+    wait_for_previous();
     const Columns<N, MULTI> c(a.width, shape.ctas_per_row, rank);
     const float over = 1.0f / (float)a.width;
     const bool per_sample = FORM == kGated || (FORM == kAny && a.gate_kind == FFCVB_GATE_SAMPLE);

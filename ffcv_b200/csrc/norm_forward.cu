@@ -25,6 +25,7 @@ forward_kernel(const __grid_constant__ Args a, const Shape shape) {
     const bool per_sample = FORM == kGated || (FORM == kAny && a.gate_kind == FFCVB_GATE_SAMPLE);
     RowSum<MULTI> sum{s_sum, shape.ctas_per_row};
     sum.begin();
+    wait_for_previous();
     const Columns<N, MULTI> c(a.width, shape.ctas_per_row, rank);
     Eight w, b, f, pw, pb; // (f is 0 beyond the row, which keeps y 0 there)
     load_params(w, a.weight, a.param_type, c, 1.0f, 1.0f);
@@ -68,6 +69,7 @@ forward_kernel(const __grid_constant__ Args a, const Shape shape) {
     };
     if constexpr (RING)
         for (int k = 0; k < shape.ahead; k++) fetch(begin + k * step, mine + k * slot_size);
+    let_next_begin();
     uint32_t slot = mine;
     T *to_y = static_cast<T *>(a.y) + begin * a.width, *to_z = static_cast<T *>(a.z) + begin * a.width;
     for (long long row = begin; row < a.rows; row += step, to_y += step * a.width, to_z += step * a.width) {

@@ -288,16 +288,18 @@ void launch(Kernel kernel, const Shape &shape, size_t room, cudaStream_t stream,
     // (what a CTA may have without being asked includes the static part)
     if (room > 40 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)room);
     cudaLaunchConfig_t how{};
-    cudaLaunchAttribute cluster{};
-    cluster.id = cudaLaunchAttributeClusterDimension;
-    cluster.val.clusterDim.x = shape.ctas_per_row;
-    cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+    cudaLaunchAttribute with[2] = {};
+    with[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    with[0].val.programmaticStreamSerializationAllowed = 1;
+    with[1].id = cudaLaunchAttributeClusterDimension;
+    with[1].val.clusterDim.x = shape.ctas_per_row;
+    with[1].val.clusterDim.y = with[1].val.clusterDim.z = 1;
     how.gridDim = dim3(shape.rows_at_once * shape.ctas_per_row);
     how.blockDim = dim3(shape.threads);
     how.dynamicSmemBytes = room;
     how.stream = stream;
-    how.attrs = &cluster;
-    how.numAttrs = shape.ctas_per_row > 1;
+    how.attrs = with;
+    how.numAttrs = shape.ctas_per_row > 1 ? 2 : 1;
     cudaLaunchKernelEx(&how, kernel, more...);
 }
 

@@ -29,6 +29,8 @@ template <typename T, int N, bool INTERLEAVED>
 __global__ void __launch_bounds__(kThreads)
 rotary_kernel(const __grid_constant__ Args a, int tile) {
     extern __shared__ float s_cos[]; // [tile][pairs], then the sines
+    wait_for_previous();
+    let_next_begin();
     const int pairs = (int)a.rotary_dim / 2;
     float *const s_sin = s_cos + tile * pairs;
     const long long tiles = (a.tokens + tile - 1) / tile;
@@ -158,7 +160,7 @@ extern "C" int ffcvb_rotary(const ffcvb_rotary_args *args, void *stream) {
         if (a.kv_heads) low |= reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.k_out);
         const bool wide = (low & 15) == 0 && sizes % W == 0;
         auto run = [&](auto kernel) {
-            kernel<<<(unsigned)ctas, kThreads, (size_t)tile * pairs * 2 * sizeof(float), static_cast<cudaStream_t>(stream)>>>(a, tile);
+            launch_early(kernel, (unsigned)ctas, kThreads, (size_t)tile * pairs * 2 * sizeof(float), static_cast<cudaStream_t>(stream), a, tile);
         };
         if (wide)
             run(a.interleaved ? rotary_kernel<T, W, true> : rotary_kernel<T, W, false>);

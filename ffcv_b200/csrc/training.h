@@ -53,8 +53,9 @@ inline int type_size(int type) { return type == FFCVB_TYPE_F32 ? 4 : 2; }
 
 #ifdef __CUDACC__
 
-// Programmatic launches: a kernel launched by launch_early may begin once every CTA of the one before it has called let_next_begin() or
-// ended; it calls wait_for_previous() before it touches what earlier kernels of the stream wrote or read.
+// Programmatic launches, of all kernels here: such a kernel may begin once every CTA of the one before it has called let_next_begin() or
+// ended; it calls wait_for_previous() before it touches what earlier kernels of the stream wrote or read.  What it saves is the way from one
+// kernel's end to the next one's begin (rotary, queries and keys forward and backward in turn, 65 us each: 141 us a pair without, 137 with).
 template <typename... Params, typename... Given>
 cudaError_t launch_early(void (*kernel)(Params...), dim3 grid, dim3 block, size_t room, cudaStream_t stream, Given &&...given) {
     cudaLaunchConfig_t how{};

@@ -1,4 +1,6 @@
 """AdamW over all tensors of a network in one launch, with moments in 32 or in 8 bits."""
+import struct
+
 import numpy as np
 import torch as ch
 
@@ -85,7 +87,7 @@ class AdamW(ch.optim.Optimizer):
         self._table = ch.empty(int(sizes[0]), dtype=ch.uint8, device=device)
         self._workspace = ch.empty(max(16, int(sizes[1])), dtype=ch.uint8, device=device) if self.max_grad_norm else None
         self.grad_norm = ch.zeros((), device=device) if self.max_grad_norm else None
-        self._table_size, self._at = int(sizes[0]), None
+        self._table_size, self._at, self._contiguous = int(sizes[0]), None, False
         self._group_of = np.repeat(np.arange(len(self.param_groups), dtype=np.int32), [len(g['params']) for g in self.param_groups])
         steps = np.zeros(n, np.int64)
         for i, p in enumerate(self._params):
@@ -105,29 +107,18 @@ class AdamW(ch.optim.Optimizer):
             if self.master is not None:
                 entry['master'] = self._of(self.master, i)
         self._steps = steps
+        self._host = self._numel.ctypes.data, self._steps.ctypes.data, self._group_of.ctypes.data
 
     def _of(self, flat, i):
         """Parameter i's part of a flat tensor, in the parameter's shape and order in memory."""
         p = self._params[i]
         return ch.as_strided(flat, p.shape, p.stride(), int(self._start[i]))
 
-    def _gradients(self):
-        """Addresses of the gradients, 0 without one, and tensors that must live until the launch."""
-        kept, at = [], []
-        for p in self._params:
-            g = p.grad
-            if g is None:
-                at.append(0)
-                continue
-            if g.stride() != p.stride() or g.dtype != p.dtype:
-                if g.is_sparse or g.dtype != p.dtype:
-                    raise TypeError(f'gradients must be dense and of the parameters\' type, not {g.dtype} {g.layout}')
-                g = ch.empty_like(p).copy_(g)
-                kept.append(g)
-            if g.device != p.device:
-                raise ValueError(f'a gradient is on {g.device}, its parameter on {p.device}')
-            at.append(g.data_ptr())
-        return np.array(at, np.uint64), kept
+    def _as_parameter(self, p, g):
+        """A gradient that is laid out as its parameter."""
+        if g.layout != ch.strided or g.dtype != p.dtype or g.device != p.device:
+            raise TypeError(f'gradients must be dense, of the parameters\' type and on their GPU, not {g.dtype} {g.layout} on {g.device}')
+        return g if g.stride() == p.stride() else ch.empty_like(p).copy_(g)
 
     @ch.no_grad()
     def step(self, closure=None):
@@ -135,26 +126,31 @@ class AdamW(ch.optim.Optimizer):
         if closure is not None:
             with ch.enable_grad():
                 loss = closure()
-        params = self._params
-        device = params[0].device
-        grads, kept = self._gradients()
+        params, n = self._params, len(self._params)
+        dtype, index = params[0].dtype, params[0].get_device()
         at = [p.data_ptr() for p in params]
+        # addresses of gradients, 0 without one
+        grads, kept = [p.grad for p in params], None
+        if at == self._at and self._contiguous and all(
+                g is not None and g.dtype is dtype and g.is_contiguous() for g in grads):
+            grads_at = [g.data_ptr() for g in grads]
+        else:
+            kept = [None if g is None else self._as_parameter(p, g) for p, g in zip(params, grads)]
+            grads_at = [N.ptr(g) for g in kept]
         if at != self._at:  # the first step, or parameters that have moved
             host = np.empty(max(1, self._table_size), np.uint8)
             where = np.array(at, np.uint64)
-            N.check(N.lib.ffcvb_adamw_table(len(params), self._numel.ctypes.data, where.ctypes.data, host.ctypes.data))
+            N.check(N.lib.ffcvb_adamw_table(n, self._numel.ctypes.data, where.ctypes.data, host.ctypes.data))
             self._table.copy_(ch.from_numpy(host[:self._table_size]))
-            self._at = at
-        groups = bytearray()
+            self._at, self._contiguous = at, all(p.is_contiguous() for p in params)
+        groups = b''
         for group in self.param_groups:
             self._check_group(group)
             groups += N.ADAMW_GROUP.pack(group['lr'], *group['betas'], group['eps'], group['weight_decay'])
         args = N.ADAMW.pack(self._table.data_ptr(), self.exp_avg.data_ptr(), self.exp_avg_sq.data_ptr(), N.ptr(self.scales),
-                            N.ptr(self.master), N.ptr(self.grad_norm), N.ptr(self._workspace), self.seed, device.index,
-                            N.TYPES[params[0].dtype], self.state_bits, len(params), self.max_grad_norm or 0.0)
-        N.check(N.lib.ffcvb_adamw_step(args, self._numel.ctypes.data, grads.ctypes.data, self._steps.ctypes.data,
-                                       self._group_of.ctypes.data, bytes(groups), len(self.param_groups),
-                                       N.stream_of(params[0])))
+                            N.ptr(self.master), N.ptr(self.grad_norm), N.ptr(self._workspace), self.seed, index,
+                            N.TYPES[dtype], self.state_bits, n, self.max_grad_norm or 0.0)
+        N.check(N.lib.ffcvb_adamw_step(args, *self._host, struct.pack(f'={n}Q', *grads_at), groups, len(self.param_groups), N.raw_stream(index)))
         del kept
         return loss
 

@@ -27,11 +27,11 @@ class _Call:
             self.kind, target, shape = _LABELS, labels, (n,)
             if not isinstance(labels, ch.Tensor) or labels.dtype not in (ch.int64, ch.int32):
                 raise TypeError('labels must be an int64 or int32 tensor')
-            target = labels.long()
+            target = labels if labels.dtype == ch.int64 else labels.long()
         elif mixed is not None:
             self.kind, target, shape = _MIXED, mixed, (n, 3)
             N.require(mixed, 'mixed', logits)
-            target = mixed.float()
+            target = mixed if mixed.dtype == ch.float32 else mixed.float()
             if target.stride(1) != 1:
                 target = target.contiguous()
         else:
@@ -50,18 +50,19 @@ class _Call:
         self.logits = logits if logits.stride(1) == 1 else logits.contiguous()
         self.target, self.ignore, self.mean, self.smoothing = target, ignore_index, reduction == 'mean', float(smoothing)
 
+    # loss: a value per sample, and one more for their mean or sum
     def run(self, grad=None, loss=None, row_loss=None, stats=None, upstream=None, per_row=False, from_stats=False, scale=1.0):
         x, t = self.logits, self.target
         counted = ch.empty(1, device=x.device) if self.ignore is not None and self.mean else None
         args = N.CROSS_ENTROPY.pack(
-            x.data_ptr(), t.data_ptr(), N.ptr(upstream), N.ptr(grad), N.ptr(loss), N.ptr(row_loss), N.ptr(stats), N.ptr(counted),
+            x.data_ptr(), t.data_ptr(), N.ptr(upstream), N.ptr(grad), 0 if loss is None else loss.data_ptr() + 4 * x.shape[0], N.ptr(row_loss), N.ptr(stats), N.ptr(counted),
             x.shape[0], x.shape[1], x.stride(0), t.stride(0), x.shape[1], -1 if self.ignore is None else self.ignore,
-            x.device.index, self.type, self.kind, self.target_type, self.ignore is not None, self.mean, per_row, from_stats,
+            x.get_device(), self.type, self.kind, self.target_type, self.ignore is not None, self.mean, per_row, from_stats,
             self.smoothing, scale)
         N.check(N.lib.ffcvb_cross_entropy(args, N.stream_of(x)))
 
     def new_grad(self):
-        return ch.empty(self.logits.shape, dtype=self.logits.dtype, device=self.logits.device)
+        return N.new_like(self.logits)
 
 
 def cross_entropy_with_grad(logits, labels=None, *, mixed=None, soft=None, label_smoothing=0.0, ignore_index=None,
@@ -94,7 +95,7 @@ def cross_entropy_with_grad(logits, labels=None, *, mixed=None, soft=None, label
     n = logits.shape[0]
     loss = ch.empty(n + 1, device=logits.device)  # a value per sample, and their mean or sum
     grad = call.new_grad()
-    call.run(grad=grad, loss=None if reduction == 'none' else loss[n:], row_loss=loss, scale=grad_scale)
+    call.run(grad=grad, loss=None if reduction == 'none' else loss, row_loss=loss, scale=grad_scale)
     return loss[:n] if reduction == 'none' else loss[n], grad
 
 
@@ -103,7 +104,7 @@ class _CrossEntropy(ch.autograd.Function):
     def forward(ctx, logits, call, reduction):
         n = logits.shape[0]
         loss, stats = ch.empty(n + 1, device=logits.device), ch.empty((n, 2), device=logits.device)
-        call.run(loss=None if reduction == 'none' else loss[n:], row_loss=loss, stats=stats)
+        call.run(loss=None if reduction == 'none' else loss, row_loss=loss, stats=stats)
         ctx.per_row = reduction == 'none'
         ctx.save_for_backward(call.logits, call.target, stats)
         call.logits = call.target = None  # (autograd keeps them, and sees to it that nobody changes them)

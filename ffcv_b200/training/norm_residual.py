@@ -23,19 +23,16 @@ def _gate_kind(x, gate):
     return None, 1
 
 
-def _rows(t, width):
-    """(rows, width) with neighbouring values together: a view where the strides allow it."""
-    t = t.reshape(-1, width)
-    return t if t.stride(1) == 1 or width == 1 else t.contiguous()
-
-
 class _Call:
     """A checked call: what the forward and the backward pass have in common."""
+    __slots__ = ('x', 'h', 'gate', 'scale', 'width', 'rows', 'type', 'param_dtype', 'param_type', 'index', 'norm', 'post_norm', 'gate_kind',
+                 'tokens', 'eps', 'number', 'given', 'strides', 'kept')
 
     def __init__(self, x, h, norm, weight, bias, post_norm, post_weight, post_bias, gate, scale, eps):
         self.type = N.require(x, 'x')
-        if x.dim() < 1 or not 1 <= x.shape[-1] <= N.NORM_MAX_WIDTH:
-            raise ValueError(f'x must have 1 to {N.NORM_MAX_WIDTH} values in its last dimension, not {tuple(x.shape)}')
+        shape = x.shape
+        if len(shape) < 1 or not 1 <= shape[-1] <= N.NORM_MAX_WIDTH:
+            raise ValueError(f'x must have 1 to {N.NORM_MAX_WIDTH} values in its last dimension, not {tuple(shape)}')
         if norm not in _NORMS or post_norm not in _NORMS:
             raise ValueError("norms are 'layer', 'rms' or None")
         if h is None:
@@ -43,89 +40,103 @@ class _Call:
                 raise ValueError('nothing to do: neither a branch nor a norm')
             if post_norm is not None or gate is not None or scale is not None:
                 raise ValueError('post_norm, gate and scale go with a branch h')
-        elif N.require(h, 'h', x) != self.type or h.shape != x.shape:
-            raise ValueError(f'h must be {x.dtype} {tuple(x.shape)}, not {h.dtype} {tuple(h.shape)}')
+        elif N.require(h, 'h', x) != self.type or h.shape != shape:
+            raise ValueError(f'h must be {x.dtype} {tuple(shape)}, not {h.dtype} {tuple(h.shape)}')
         if norm is None and (weight is not None or bias is not None):
             raise ValueError('weight and bias go with a norm')
         if post_norm is None and (post_weight is not None or post_bias is not None):
             raise ValueError('post_weight and post_bias go with a post_norm')
-        self.number, self.scale = 1.0, scale
+        self.number = 1.0
         if scale is not None and not isinstance(scale, ch.Tensor):
-            self.number, self.scale = float(scale), None
-        self.width = width = x.shape[-1]
-        self.weight, self.bias, self.post_weight, self.post_bias = weight, bias, post_weight, post_bias
-        self.param_dtype, self.param_type = ch.float32, 0
-        first = True
-        for name in _PARAMS:
-            p = getattr(self, name)
+            self.number, scale = float(scale), None
+        self.x, self.h, self.gate, self.scale = x, h, gate, scale
+        self.width = width = shape[-1]
+        self.rows = x.numel() // width
+        self.index = x.get_device()
+        self.param_dtype, self.param_type, self.kept = None, 0, []
+        at = [0] * 8  # addresses of x, h, gate, and the parameters
+        for k, p in enumerate((weight, bias, post_weight, post_bias, scale)):
             if p is None:
                 continue
-            kind = N.require(p, name, x)
+            kind = N.require(p, _PARAMS[k], x)
             if p.shape != (width,):
-                raise ValueError(f'{name} must be of shape ({width},), not {tuple(p.shape)}')
-            if not first and p.dtype != self.param_dtype:
+                raise ValueError(f'{_PARAMS[k]} must be of shape ({width},), not {tuple(p.shape)}')
+            if self.param_dtype is None:
+                self.param_dtype, self.param_type = p.dtype, kind
+            elif p.dtype is not self.param_dtype:
                 raise TypeError('weights, biases and scale must be of one type')
-            self.param_dtype, self.param_type, first = p.dtype, kind, False
-            if width > 1 and p.stride(0) != 1:
-                setattr(self, name, p.contiguous())
+            if not p.is_contiguous():
+                p = p.contiguous()
+                self.kept.append(p)
+            at[3 + k] = p.data_ptr()
         self.gate_kind, self.tokens = _gate_kind(x, gate)
         if gate is not None and (N.require(gate, 'gate', x) != self.type or self.gate_kind is None):
-            raise ValueError(f'gate must be {x.dtype}, with a row per row or per sample of {tuple(x.shape)}, not {gate.dtype} {tuple(gate.shape)}')
-        self.shape, self.device = x.shape, x.device
-        self.x, self.h = _rows(x, width), None if h is None else _rows(h, width)
-        self.gate_shape = None if gate is None else gate.shape
-        self.gate = None if gate is None else _rows(gate, width)
+            raise ValueError(f'gate must be {x.dtype}, with a row per row or per sample of {tuple(shape)}, not {gate.dtype} {tuple(gate.shape)}')
+        at[0], x_stride = self.rows_of(x)
+        at[1], h_stride = self.rows_of(h)
+        at[2], gate_stride = self.rows_of(gate)
+        self.given, self.strides = at, (x_stride, h_stride, gate_stride)
         self.norm, self.post_norm, self.eps = _NORMS[norm], _NORMS[post_norm], float(eps)
+
+    def rows_of(self, t):
+        """Address of rows whose values lie together, and the stride from one to the next: a view where the strides allow it."""
+        if t is None:
+            return 0, 0
+        if t.is_contiguous():
+            return t.data_ptr(), self.width
+        t = t.reshape(-1, self.width)
+        if self.width > 1 and t.stride(1) != 1:
+            t = t.contiguous()
+        self.kept.append(t)
+        return t.data_ptr(), t.stride(0)
 
     def plain(self):
         """Whether the branch is added as it is, so that its gradient is the stream's."""
         return self.post_norm == 0 and self.gate is None and self.scale is None and self.number == 1.0
 
-    def pack(self, stats, y=None, z=None, dy=None, dz=None, dx=None, dh=None, dgate=None, params=(0,) * 5, workspace=0):
-        x, h, gate = self.x, self.h, self.gate
-        p = N.ptr
+    def pack(self, stats, y=0, z=0, dy=0, dz=0, dx=0, dh=0, dgate=0, params=(0,) * 5, workspace=0, dy_stride=0, dz_stride=0):
         return N.NORM_RESIDUAL.pack(
-            x.data_ptr(), p(h), p(gate), p(self.weight), p(self.bias), p(self.post_weight), p(self.post_bias), p(self.scale),
-            p(stats), p(y), p(z), p(dy), p(dz), p(dx), p(dh), p(dgate), *params, workspace,
-            x.shape[0], self.width, self.tokens, x.stride(0), 0 if h is None else h.stride(0), 0 if gate is None else gate.stride(0),
-            0 if dy is None else dy.stride(0), 0 if dz is None else dz.stride(0),
-            self.device.index, self.type, self.param_type, self.norm, self.post_norm, self.gate_kind, self.eps, self.number)
+            *self.given, stats.data_ptr(), y, z, dy, dz, dx, dh, dgate, *params, workspace, self.rows, self.width, self.tokens,
+            *self.strides, dy_stride, dz_stride, self.index, self.type, self.param_type, self.norm, self.post_norm, self.gate_kind,
+            self.eps, self.number)
 
     def forward(self):
-        new = lambda: ch.empty(self.shape, dtype=self.x.dtype, device=self.device)  # noqa: E731
-        y, z = None if self.h is None else new(), new() if self.norm else None
-        stats = ch.empty((self.x.shape[0], 4), device=self.device)
-        N.check(N.lib.ffcvb_norm_residual(self.pack(stats, y, z), N.stream_of(self.x)))
+        x = self.x
+        y, z = None if self.h is None else N.new_like(x), N.new_like(x) if self.norm else None
+        stats = ch.empty(4 * self.rows, device=x.device)
+        N.check(N.lib.ffcvb_norm_residual(self.pack(stats, N.ptr(y), N.ptr(z)), N.raw_stream(self.index)))
         return y, z, stats
 
     def backward(self, stats, dy, dz, wanted):
         """The gradients named in `wanted`, which holds only what the call was given."""
-        dtype, device = self.x.dtype, self.device
+        x = self.x
         for name, g in (('dy', dy), ('dz', dz)):
-            if g is not None and (N.require(g, name, self.x) != self.type or g.shape != self.shape):
-                raise ValueError(f'{name} must be {dtype} {tuple(self.shape)}, not {g.dtype} {tuple(g.shape)}')
+            if g is not None and (N.require(g, name, x) != self.type or g.shape != x.shape):
+                raise ValueError(f'{name} must be {x.dtype} {tuple(x.shape)}, not {g.dtype} {tuple(g.shape)}')
         if dz is not None and self.norm == 0:
             raise ValueError('dz goes with a norm')
-        dy, dz = (None if g is None else _rows(g, self.width) for g in (dy, dz))
         if dz is None and self.norm:  # the kernel reads one where there is a norm
-            dz = ch.zeros_like(self.x)
-        new = lambda: ch.empty(self.shape, dtype=dtype, device=device)  # noqa: E731
+            dz = ch.zeros_like(x, memory_format=ch.contiguous_format)
+        dy_at, dy_stride = self.rows_of(dy)
+        dz_at, dz_stride = self.rows_of(dz)
         plain = self.plain()
         out = {}
         if 'x' in wanted or (plain and 'h' in wanted):
-            out['x'] = new()
+            out['x'] = N.new_like(x)
         if 'h' in wanted:
-            out['h'] = out['x'] if plain else new()
-        for name in _PARAMS:
+            out['h'] = out['x'] if plain else N.new_like(x)
+        params = [0] * 5
+        for k, name in enumerate(_PARAMS):
             if name in wanted:
-                out[name] = ch.empty(self.width, dtype=self.param_dtype, device=device)
+                out[name] = g = ch.empty(self.width, dtype=self.param_dtype, device=x.device)
+                params[k] = g.data_ptr()
         if 'gate' in wanted:
-            out['gate'] = ch.empty(self.gate_shape, dtype=dtype, device=device)
-        how = dict(dy=dy, dz=dz, dx=out.get('x'), dh=None if plain else out.get('h'), dgate=out.get('gate'),
-                   params=tuple(N.ptr(out.get(name)) for name in _PARAMS))
+            out['gate'] = N.new_like(self.gate)
+        how = dict(dy=dy_at, dz=dz_at, dx=N.ptr(out.get('x')), dh=0 if plain else N.ptr(out.get('h')), dgate=N.ptr(out.get('gate')),
+                   params=params, dy_stride=dy_stride, dz_stride=dz_stride)
         room = N.lib.ffcvb_norm_residual_workspace(self.pack(stats, **how))
-        workspace = ch.empty(room, dtype=ch.uint8, device=device)
-        N.check(N.lib.ffcvb_norm_residual_backward(self.pack(stats, workspace=workspace.data_ptr(), **how), N.stream_of(self.x)))
+        workspace = ch.empty(room, dtype=ch.uint8, device=x.device)
+        N.check(N.lib.ffcvb_norm_residual_backward(self.pack(stats, workspace=workspace.data_ptr(), **how), N.raw_stream(self.index)))
         return out
 
 

@@ -18,13 +18,13 @@ class _Rotate(ch.autograd.Function):
     def forward(ctx, rotary, positions, q, k):
         ctx.rotary = rotary
         ctx.save_for_backward(positions)
-        return rotary._run(q, k, positions, False, False)
+        return rotary._run(q, k, *rotary._where(q, positions), False, False)
 
     @staticmethod
     @ch.autograd.function.once_differentiable
     def backward(ctx, dq, dk=None):
         positions, = ctx.saved_tensors
-        dq, dk = ctx.rotary._run(dq, dk, positions, True, False)
+        dq, dk = ctx.rotary._run(dq, dk, *ctx.rotary._where(dq, positions), True, False)
         return None, None, dq, dk
 
 
@@ -101,14 +101,14 @@ class RotaryPositions(ch.nn.Module):
             raise ValueError(f'positions are on {positions.device}, not on {q.device}')
         if positions.dtype not in (ch.int64, ch.float32):
             positions = positions.float() if positions.is_floating_point() else positions.long()
-        own = (tokens,) if self.axes == 1 else (tokens, 2)
-        if tuple(positions.shape) == own:
+        own, shape = (tokens,) if self.axes == 1 else (tokens, 2), positions.shape
+        if shape == own:
             return positions.contiguous(), 0
-        if tuple(positions.shape) == (1,) + own:
+        if shape == (1,) + own:
             return positions[0].contiguous(), 0
-        if tuple(positions.shape) == (batch,) + own:
+        if shape == (batch,) + own:
             return positions.contiguous(), tokens * self.axes
-        raise ValueError(f'positions must be of shape {own} or {(batch,) + own}, not {tuple(positions.shape)}')
+        raise ValueError(f'positions must be of shape {own} or {(batch,) + own}, not {tuple(shape)}')
 
     def _check(self, q, k):
         N.require(q, 'q')
@@ -116,34 +116,39 @@ class RotaryPositions(ch.nn.Module):
             raise ValueError(f'q must be (batch, tokens, heads, {self.head_dim}), not {tuple(q.shape)}')
         if k is not None:
             N.require(k, 'k', q)
-            if k.dtype != q.dtype or k.dim() != 4 or k.shape[:2] != q.shape[:2] or k.shape[3] != self.head_dim:
+            if k.dtype is not q.dtype or k.dim() != 4 or k.shape[:2] != q.shape[:2] or k.shape[3] != self.head_dim:
                 raise ValueError(f'k must be {q.dtype} {tuple(q.shape[:2])} + (heads, {self.head_dim}), not {k.dtype} {tuple(k.shape)}')
 
-    def _run(self, q, k, positions, transpose, inplace):
-        where, stride = self._where(q, positions)
+    def _run(self, q, k, where, stride, transpose, inplace):
         if inplace and (q.stride(3) != 1 or (k is not None and k.stride(3) != 1)):
             raise ValueError('in place the values of a head must lie next to one another')
         if q.stride(3) != 1:
             q = q.contiguous()
         if k is not None and k.stride(3) != 1:
             k = k.contiguous()
-        q_out = q if inplace else ch.empty(q.shape, dtype=q.dtype, device=q.device)
-        k_out = k if inplace or k is None else ch.empty(k.shape, dtype=k.dtype, device=k.device)
-        none = (0, 0, 0)
+        q_out = q if inplace else N.new_like(q)
+        k_out = k if inplace or k is None else N.new_like(k)
+        batch, tokens, heads, _ = q.shape
+        qb, qt, qh, _ = q.stride()
+        qob, qot, qoh, _ = q_out.stride()
+        kv_heads, kb, kt, kh, kob, kot, koh = 0, 0, 0, 0, 0, 0, 0
+        if k is not None:
+            kv_heads = k.shape[2]
+            kb, kt, kh, _ = k.stride()
+            kob, kot, koh, _ = k_out.stride()
+        index = q.get_device()
         args = N.ROTARY.pack(
             q.data_ptr(), N.ptr(k), q_out.data_ptr(), N.ptr(k_out), where.data_ptr(), self._turns_on(q.device).data_ptr(),
-            q.shape[0], q.shape[1], q.shape[2], 0 if k is None else k.shape[2], self.head_dim, self.rotary_dim, stride,
-            *q.stride()[:3], *(none if k is None else k.stride()[:3]), *q_out.stride()[:3],
-            *(none if k is None else k_out.stride()[:3]), q.device.index, N.TYPES[q.dtype], where.dtype == ch.float32,
-            self.axes, self.layout == 'interleaved', transpose, self.amplitude, 0)
-        N.check(N.lib.ffcvb_rotary(args, N.stream_of(q)))
+            batch, tokens, heads, kv_heads, self.head_dim, self.rotary_dim, stride, qb, qt, qh, kb, kt, kh, qob, qot, qoh, kob, kot, koh,
+            index, N.TYPES[q.dtype], where.dtype == ch.float32, self.axes, self.layout == 'interleaved', transpose, self.amplitude, 0)
+        N.check(N.lib.ffcvb_rotary(args, N.raw_stream(index)))
         return q_out, k_out
 
     def rotate(self, q, k=None, positions=None, transpose=False, inplace=False):
         """``(q, k)`` turned, without autograd.  ``transpose`` turns the other way, which is the gradient's way: given the
         gradients of what ``rotate`` returned, it returns those of what it was given."""
         self._check(q, k)
-        return self._run(q, k, positions, transpose, inplace)
+        return self._run(q, k, *self._where(q, positions), transpose, inplace)
 
     def forward(self, q, k=None, positions=None):
         """Queries and keys, (batch, tokens, heads, head_dim) with any strides, at integer or float positions of

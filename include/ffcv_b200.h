@@ -418,8 +418,8 @@ int64_t ffcvb_adamw_layout(int32_t n, const int64_t *numel, int64_t *start, int6
 int ffcvb_adamw_table(int32_t n, const int64_t *numel, const uint64_t *params, void *table);
 /* numel, grads (DEVICE addresses, or 0), steps and group_of are HOST arrays of n_tensors entries; steps[i] of tensors
  * with a gradient is advanced. */
-int ffcvb_adamw_step(const ffcvb_adamw_args *args, const int64_t *numel, const uint64_t *grads, int64_t *steps,
-                     const int32_t *group_of, const ffcvb_adamw_group *groups, int32_t n_groups, void *stream);
+int ffcvb_adamw_step(const ffcvb_adamw_args *args, const int64_t *numel, int64_t *steps, const int32_t *group_of,
+                     const uint64_t *grads, const ffcvb_adamw_group *groups, int32_t n_groups, void *stream);
 
 /* ---- decode without allocating -----------------------------------------------------------
  * No counterpart in the reference.  For callers that must not allocate GPU memory while they
