@@ -80,13 +80,12 @@ __device__ __forceinline__ void four(Two *v, float4 f) {
 __device__ __forceinline__ float4 four(const Two *v) { return make_float4(v[0].lo(), v[0].hi(), v[1].lo(), v[1].hi()); }
 
 // Four values from place `at` of a tensor of n; 0 beyond its end.  WHOLE: none is, and the tensor lies on boundaries of four values.
-// KEPT: to be read again soon.
-template <bool WHOLE, bool KEPT = false, typename T>
+template <bool WHOLE, typename T>
 __device__ __forceinline__ float4 load4(const T *p, long long at, long long n) {
     if constexpr (WHOLE && sizeof(T) == 4) {
-        return KEPT ? *reinterpret_cast<const float4 *>(p + at) : __ldcs(reinterpret_cast<const float4 *>(p + at));
+        return *reinterpret_cast<const float4 *>(p + at);
     } else if constexpr (WHOLE) {
-        const uint2 w = KEPT ? *reinterpret_cast<const uint2 *>(p + at) : __ldcs(reinterpret_cast<const uint2 *>(p + at));
+        const uint2 w = *reinterpret_cast<const uint2 *>(p + at);
         float2 lo, hi;
         if constexpr (std::is_same<T, __half>::value) {
             lo = __half22float2(*reinterpret_cast<const __half2 *>(&w.x));
@@ -104,7 +103,7 @@ __device__ __forceinline__ float4 load4(const T *p, long long at, long long n) {
 template <bool WHOLE, typename T>
 __device__ __forceinline__ void store4(float4 v, T *p, long long at, long long n) {
     if constexpr (WHOLE && sizeof(T) == 4) {
-        __stcs(reinterpret_cast<float4 *>(p + at), v);
+        *reinterpret_cast<float4 *>(p + at) = v;
     } else if constexpr (WHOLE) {
         uint2 w;
         if constexpr (std::is_same<T, __half>::value) {
@@ -114,7 +113,7 @@ __device__ __forceinline__ void store4(float4 v, T *p, long long at, long long n
             const __nv_bfloat162 lo = __floats2bfloat162_rn(v.x, v.y), hi = __floats2bfloat162_rn(v.z, v.w);
             w = make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
         }
-        __stcs(reinterpret_cast<uint2 *>(p + at), w);
+        *reinterpret_cast<uint2 *>(p + at) = w;
     } else {
         if (at < n) p[at] = from_float<T>(v.x);
         if (at + 1 < n) p[at + 1] = from_float<T>(v.y);
@@ -166,13 +165,13 @@ __device__ __forceinline__ void step_unit(const Args &a, const Set &set, float c
     for (int half = 0; half < 2; half++) { // (a lane has four neighbours in either half of a unit)
         const long long at = first + half * 128 + lane * 4, place = flat + half * 128 + lane * 4;
         four(g + 2 * half, load4<WHOLE>(grad, at, n));
-        four(w + 2 * half, sizeof(T) == 4 ? load4<WHOLE>(param, at, n) : __ldcs(reinterpret_cast<const float4 *>(a.master + place)));
+        four(w + 2 * half, sizeof(T) == 4 ? load4<WHOLE>(param, at, n) : *reinterpret_cast<const float4 *>(a.master + place));
         if (BITS == 32) {
-            four(m + 2 * half, __ldcs(reinterpret_cast<const float4 *>(exp_avg + place)));
-            four(v + 2 * half, __ldcs(reinterpret_cast<const float4 *>(exp_avg_sq + place)));
+            four(m + 2 * half, *reinterpret_cast<const float4 *>(exp_avg + place));
+            four(v + 2 * half, *reinterpret_cast<const float4 *>(exp_avg_sq + place));
         } else {
-            mc[half] = __ldcs(m_codes + place / 4);
-            vc[half] = __ldcs(v_codes + place / 4);
+            mc[half] = m_codes[place / 4];
+            vc[half] = v_codes[place / 4];
         }
     }
     if (BITS == 8) {
@@ -233,13 +232,13 @@ __device__ __forceinline__ void step_unit(const Args &a, const Set &set, float c
     for (int half = 0; half < 2; half++) {
         const long long at = first + half * 128 + lane * 4, place = flat + half * 128 + lane * 4;
         store4<WHOLE>(four(w + 2 * half), param, at, n);
-        if (sizeof(T) != 4) __stcs(reinterpret_cast<float4 *>(a.master + place), four(w + 2 * half));
+        if (sizeof(T) != 4) *reinterpret_cast<float4 *>(a.master + place) = four(w + 2 * half);
         if (BITS == 32) {
-            __stcs(reinterpret_cast<float4 *>(exp_avg + place), four(m + 2 * half));
-            __stcs(reinterpret_cast<float4 *>(exp_avg_sq + place), four(v + 2 * half));
+            *reinterpret_cast<float4 *>(exp_avg + place) = four(m + 2 * half);
+            *reinterpret_cast<float4 *>(exp_avg_sq + place) = four(v + 2 * half);
         } else {
-            __stcs(m_codes + place / 4, mc[half]);
-            __stcs(v_codes + place / 4, vc[half]);
+            m_codes[place / 4] = mc[half];
+            v_codes[place / 4] = vc[half];
         }
     }
 }
@@ -274,7 +273,8 @@ step_kernel(const __grid_constant__ Launch<MOST> a) {
 }
 
 // The sum of squares of a chunk's gradients.  The last chunks come first: what the first ones leave in the caches the step begins with
-// (101 M values in 32 bits: squares and step together 505 us, 508 with the first chunks first).
+// (101 M values in 32 bits: squares and step together 505 us, 508 with the first chunks first; 500 and 494 without and with the caches'
+// default policy for all loads and stores instead of one for what is used once).
 template <typename T, int MOST>
 __global__ void __launch_bounds__(kThreads)
 squares_kernel(const __grid_constant__ Launch<MOST> a) {
@@ -294,12 +294,12 @@ squares_kernel(const __grid_constant__ Launch<MOST> a) {
         if (aligned && first + a.chunk <= n && a.chunk == kLong) {
             float4 g[AT_ONCE];
 #pragma unroll
-            for (int k = 0; k < AT_ONCE; k++) g[k] = load4<true, true>(grad, first + (k * kThreads + threadIdx.x) * 4, n);
+            for (int k = 0; k < AT_ONCE; k++) g[k] = load4<true>(grad, first + (k * kThreads + threadIdx.x) * 4, n);
 #pragma unroll
             for (int k = 0; k < AT_ONCE; k++) sum += (g[k].x * g[k].x + g[k].y * g[k].y) + (g[k].z * g[k].z + g[k].w * g[k].w);
         } else {
             for (int k = threadIdx.x; k < a.chunk / 4 && first + k * 4 < n; k += kThreads) {
-                const float4 g = load4<false, true>(grad, first + k * 4, n);
+                const float4 g = load4<false>(grad, first + k * 4, n);
                 sum += (g.x * g.x + g.y * g.y) + (g.z * g.z + g.w * g.w);
             }
         }

@@ -334,7 +334,7 @@ rows_kernel(const __grid_constant__ ffcvb_cross_entropy_args a, const Deal deal)
         }
         Pack<T, N> pack;
         pack.set(v);
-        pack.store_once(g + c);
+        pack.store(g + c);
     });
     if (!SOFT) { // the labels' classes in packs: the thread that has just written them writes them again
 #pragma unroll

@@ -74,8 +74,8 @@ rotary_kernel(const __grid_constant__ Args a, int tile) {
 #pragma unroll
             for (int i = 0; i < kAtOnce; i++)
                 if (t + i * abreast < tokens) {
-                    p[i].load_once(in + i * in_step);
-                    if (TWO && turns) q[i].load_once(in + i * in_step + other);
+                    p[i].load(in + i * in_step);
+                    if (TWO && turns) q[i].load(in + i * in_step + other);
                 }
 #pragma unroll
             for (int i = 0; i < kAtOnce; i++) {
@@ -117,8 +117,8 @@ rotary_kernel(const __grid_constant__ Args a, int tile) {
                         q[i].set(v);
                     }
                 }
-                p[i].store_once(out + i * out_step);
-                if (TWO && turns) q[i].store_once(out + i * out_step + other);
+                p[i].store(out + i * out_step);
+                if (TWO && turns) q[i].store(out + i * out_step + other);
             }
         }
     }

@@ -86,19 +86,14 @@ template <typename T, int N> struct Pack;
 template <typename T> struct Pack<T, 1> {
     T raw;
     __device__ __forceinline__ void load(const T *p) { raw = *p; }
-    __device__ __forceinline__ void load_once(const T *p) { raw = __ldcs(p); }
     __device__ __forceinline__ void store(T *p) const { *p = raw; }
-    __device__ __forceinline__ void store_once(T *p) const { __stcs(p, raw); }
     __device__ __forceinline__ void get(float (&v)[1]) const { v[0] = to_float(raw); }
     __device__ __forceinline__ void set(const float (&v)[1]) { raw = from_float<T>(v[0]); }
 };
 template <typename T> struct Pack16 {
     uint4 raw;
     __device__ __forceinline__ void load(const T *p) { raw = *reinterpret_cast<const uint4 *>(p); }
-    // (what is read or written once and not soon again need not displace what is)
-    __device__ __forceinline__ void load_once(const T *p) { raw = __ldcs(reinterpret_cast<const uint4 *>(p)); }
     __device__ __forceinline__ void store(T *p) const { *reinterpret_cast<uint4 *>(p) = raw; }
-    __device__ __forceinline__ void store_once(T *p) const { __stcs(reinterpret_cast<uint4 *>(p), raw); }
 };
 template <> struct Pack<float, 4> : Pack16<float> {
     __device__ __forceinline__ void get(float (&v)[4]) const {
