@@ -11,32 +11,32 @@ namespace {
 // POST: with an inner norm.  Of the branch's side two sums are kept per column and unit, A = sum t u and B = sum t (t with the gate,
 // if it is one per token), u without weight and bias: all other gradients are made of them at a unit's end,
 //   gate: f (pw A + pb B);  times the sample's gate:  scale: pw A + pb B,  post_weight: f A,  post_bias: f B.
-template <typename T, int N, bool MULTI, bool POST, int FORM>
-__global__ void __launch_bounds__(MULTI ? 512 : 32, MULTI ? 1 : 16)
+template <typename T, int N, int LANES, bool POST, int FORM>
+__global__ void __launch_bounds__(LANES ? 32 : 512, LANES ? 16 : 1)
 backward_kernel(const __grid_constant__ Args a, const Deal deal, const Partials part) {
-    constexpr bool RING = N > 1;
+    constexpr bool PACKS = N > 1, MULTI = LANES == 0;
     const Shape &shape = deal.shape;
     __shared__ __align__(16) float2 s_sum[72];
-    extern __shared__ uint4 s_ring[]; // [ahead][streams][8 / N][threads], then with an inner norm its parameters, float4 [4][threads],
-    // and with a gate per sample sums, floats [24][threads]
-    int rank = 0, cluster = blockIdx.x;
-    if (MULTI && shape.ctas_per_row > 1) {
-        rank = blockIdx.x % shape.ctas_per_row;
-        cluster = blockIdx.x / shape.ctas_per_row;
-    }
-    RowSum<MULTI> sum{s_sum, shape.ctas_per_row};
+    // [ahead][streams][8 / N][threads], or windows [rows][ahead + 1][streams]; with an inner norm its parameters, float4 [4][threads]; with
+    // a gate per sample sums, floats [24][threads]
+    extern __shared__ uint4 s_ring[];
+    int rank;
+    const int cluster = first_row<LANES>(shape, rank);
+    RowSum<LANES> sum{s_sum, shape.ctas_per_row};
     sum.begin();
     wait_for_previous();
-    const Columns<N, MULTI> c(a.width, shape.ctas_per_row, rank);
+    const Columns<N, LANES> c(a.width, rank);
     const float over = 1.0f / (float)a.width;
     const bool per_sample = FORM == kGated || (FORM == kAny && a.gate_kind == FFCVB_GATE_SAMPLE);
     const bool per_token = FORM == kAny && a.gate_kind == FFCVB_GATE_TOKEN;
     const bool branch = FORM != kAny || a.h, normed = FORM != kAny || a.norm != FFCVB_NORM_NONE;
     const bool given_dy = FORM != kAny || a.dy, given_dz = FORM != kAny || a.dz, want_dx = FORM != kAny || a.dx, want_dh = FORM != kAny || a.dh;
-    const uint32_t mine = (uint32_t)__cvta_generic_to_shared(s_ring + threadIdx.x), slot_size = shape.streams * (8 / N) * blockDim.x * 16;
-    const uint32_t ring_end = mine + shape.ahead * slot_size;
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(s_ring), window_size = window_bytes<T>(c.threads);
+    const uint32_t slot_size = shape.streams * (PACKS ? (8 / N) * blockDim.x * 16 : window_size);
+    const int slots = PACKS ? shape.ahead : shape.ahead + 1;
+    const uint32_t mine = ring + (PACKS ? threadIdx.x * 16 : MULTI ? 0 : threadIdx.x / (MULTI ? 1 : LANES) * slots * slot_size), ring_end = mine + slots * slot_size;
     // with a gate per sample the sums over units are kept here, the thread's own
-    float4 *const post = reinterpret_cast<float4 *>(s_ring + (RING ? shape.ahead * shape.streams * (8 / N) * blockDim.x : 0)) + threadIdx.x;
+    float4 *const post = reinterpret_cast<float4 *>(s_ring + (PACKS ? shape.ahead * shape.streams * (8 / N) * blockDim.x : (int)(shape.ring / 16))) + threadIdx.x;
     float *const kept = reinterpret_cast<float *>(post - threadIdx.x + (POST ? 4 * blockDim.x : 0)) + threadIdx.x;
     const bool post_bias = a.post_bias;
     if (POST) { // (there are no registers for them)
@@ -86,11 +86,19 @@ backward_kernel(const __grid_constant__ Args a, const Deal deal, const Partials 
         const T *next_dy = static_cast<const T *>(a.dy) + begin * a.dy_stride, *next_dz = static_cast<const T *>(a.dz) + begin * a.dz_stride;
         auto fetch = [&](long long row, uint32_t to) {
             if (row < end) {
-                copy_packs(to, next_x, c);
-                if (branch) copy_packs(to, next_h, c);
-                if (given_dy) copy_packs(to, next_dy, c);
-                if (given_dz) copy_packs(to, next_dz, c);
-                if (per_token) copy_packs(to, static_cast<const T *>(a.gate) + row * a.gate_stride, c);
+                auto copy = [&](const T *from) {
+                    if constexpr (PACKS) {
+                        copy_packs(to, from, c);
+                    } else {
+                        copy_window(to, from, c);
+                        to += window_size;
+                    }
+                };
+                copy(next_x);
+                if (branch) copy(next_h);
+                if (given_dy) copy(next_dy);
+                if (given_dz) copy(next_dz);
+                if (per_token) copy(static_cast<const T *>(a.gate) + row * a.gate_stride);
             }
             copies_made();
             next_x += a.x_stride;
@@ -98,8 +106,8 @@ backward_kernel(const __grid_constant__ Args a, const Deal deal, const Partials 
             next_dy += a.dy_stride;
             next_dz += a.dz_stride;
         };
-        if constexpr (RING)
-            for (int k = 0; k < shape.ahead; k++) fetch(begin + k, mine + k * slot_size);
+        if (!PACKS) row_barrier<LANES>(sum.mask()); // (the unit before is through)
+        for (int k = 0; k < shape.ahead; k++) fetch(begin + k, mine + k * slot_size);
         float4 next = {};
         if (begin < end) next = reinterpret_cast<const float4 *>(a.stats)[begin];
         uint32_t slot = mine;
@@ -111,9 +119,9 @@ backward_kernel(const __grid_constant__ Args a, const Deal deal, const Partials 
             if (!branch) fill(u, 0.0f);
             if (!given_dy) fill(t, 0.0f);
             if (!given_dz) fill(dz, 0.0f);
-            if constexpr (RING) {
-                copies_wait(shape.ahead);
-                uint32_t from = slot;
+            copies_wait(shape.ahead);
+            uint32_t from = slot;
+            if constexpr (PACKS) {
                 copied<T, N>(y, from);
                 if (branch) copied<T, N>(u, from);
                 if (given_dy) copied<T, N>(t, from);
@@ -123,11 +131,19 @@ backward_kernel(const __grid_constant__ Args a, const Deal deal, const Partials 
                 slot += slot_size;
                 if (slot == ring_end) slot = mine;
             } else {
-                load_row<T>(y, a.x, row * a.x_stride, c);
-                load_row<T>(u, a.h, row * a.h_stride, c);
-                load_row<T>(t, a.dy, row * a.dy_stride, c);
-                load_row<T>(dz, a.dz, row * a.dz_stride, c);
-                if (per_token) load_row<T>(gate, a.gate, row * a.gate_stride, c);
+                row_barrier<LANES>(sum.mask()); // (all have the row, and none the one before any more, whose place is the next one's)
+                fetch(row + shape.ahead, slot == mine ? ring_end - slot_size : slot - slot_size);
+                auto read = [&](Eight &v, const void *rows, long long stride) {
+                    window(v, from, static_cast<const T *>(rows) + row * stride, c);
+                    from += window_size;
+                };
+                read(y, a.x, a.x_stride);
+                if (branch) read(u, a.h, a.h_stride);
+                if (given_dy) read(t, a.dy, a.dy_stride);
+                if (given_dz) read(dz, a.dz, a.dz_stride);
+                if (per_token) read(gate, a.gate, a.gate_stride);
+                slot += slot_size;
+                if (slot == ring_end) slot = mine;
             }
             Eight pw;
             if (POST) {
@@ -253,17 +269,22 @@ backward_kernel(const __grid_constant__ Args a, const Deal deal, const Partials 
 
 template <typename T, int N, bool POST, int FORM>
 void sized(const Args &a, const Deal &d, const Partials &part, size_t room, cudaStream_t stream) {
-    if (d.shape.threads == 32 && d.shape.ctas_per_row == 1)
-        launch(backward_kernel<T, N, false, POST, FORM>, d.shape, room, stream, a, d, part);
+    auto run = [&](auto kernel) { launch(kernel, d.shape, room, stream, a, d, part); };
+    if (d.shape.threads > 32 || d.shape.ctas_per_row > 1)
+        run(backward_kernel<T, N, 0, POST, FORM>);
+    else if (N == 1 || d.shape.lanes == 32) // (single values: always)
+        run(backward_kernel<T, N, 32, POST, FORM>);
+    else if (d.shape.lanes == 16)
+        run(backward_kernel<T, N, N == 1 ? 32 : 16, POST, FORM>);
     else
-        launch(backward_kernel<T, N, true, POST, FORM>, d.shape, room, stream, a, d, part);
+        run(backward_kernel<T, N, N == 1 ? 32 : 8, POST, FORM>);
 }
 
 } // namespace
 
 void launch_backward(const Args &a, const Deal &d, const Partials &part, bool wide, cudaStream_t stream) {
     const bool post = a.post_norm != FFCVB_NORM_NONE;
-    const size_t room = (size_t)d.shape.threads * ((wide ? d.shape.ahead * d.shape.streams * 8 * type_size(a.type) : 0) + (post ? 64 : 0) + (a.gate_kind == FFCVB_GATE_SAMPLE ? 96 : 0));
+    const size_t room = d.shape.ring + (size_t)d.shape.threads * ((post ? 64 : 0) + (a.gate_kind == FFCVB_GATE_SAMPLE ? 96 : 0));
     with_type(a.type, [&](auto zero) {
         using T = decltype(zero);
         constexpr int W = 16 / (int)sizeof(T);

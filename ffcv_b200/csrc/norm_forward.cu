@@ -9,24 +9,21 @@ namespace {
 
 // Two rows per CTA (or cluster, or warp) at a time, so that the sums of both take one barrier; with packs of 16 bytes those of the next
 // rounds are on their way meanwhile.  POST: with an inner norm.
-template <typename T, int N, bool MULTI, bool POST, int FORM>
-__global__ void __launch_bounds__(MULTI ? 512 : 32, MULTI ? 1 : 16)
+template <typename T, int N, int LANES, bool POST, int FORM>
+__global__ void __launch_bounds__(LANES ? 32 : 512, LANES ? 16 : 1)
 forward_kernel(const __grid_constant__ Args a, const Shape shape) {
-    constexpr bool RING = N > 1;
+    constexpr bool PACKS = N > 1, MULTI = LANES == 0;
     __shared__ __align__(16) float2 s_sum[72];
-    extern __shared__ uint4 s_ring[]; // [ahead][2][streams][8 / N][threads]
-    int rank = 0, cluster = blockIdx.x;
-    if (MULTI && shape.ctas_per_row > 1) {
-        rank = blockIdx.x % shape.ctas_per_row;
-        cluster = blockIdx.x / shape.ctas_per_row;
-    }
+    extern __shared__ uint4 s_ring[]; // [ahead][2][streams][8 / N][threads], or windows [rows][ahead + 1][2][streams]
+    int rank;
+    const int cluster = first_row<LANES>(shape, rank);
     const bool branch = FORM != kAny || a.h, normed = FORM != kAny || a.norm != FFCVB_NORM_NONE;
     const bool gated = FORM == kGated || (FORM == kAny && a.gate_kind != FFCVB_GATE_NONE);
     const bool per_sample = FORM == kGated || (FORM == kAny && a.gate_kind == FFCVB_GATE_SAMPLE);
-    RowSum<MULTI> sum{s_sum, shape.ctas_per_row};
+    RowSum<LANES> sum{s_sum, shape.ctas_per_row};
     sum.begin();
     wait_for_previous();
-    const Columns<N, MULTI> c(a.width, shape.ctas_per_row, rank);
+    const Columns<N, LANES> c(a.width, rank);
     Eight w, b, f, pw, pb; // (f is 0 beyond the row, which keeps y 0 there)
     load_params(w, a.weight, a.param_type, c, 1.0f, 1.0f);
     load_params(b, a.bias, a.param_type, c, 0.0f, 0.0f);
@@ -51,24 +48,34 @@ forward_kernel(const __grid_constant__ Args a, const Shape shape) {
             next_sample++;
         }
     };
-    const uint32_t mine = (uint32_t)__cvta_generic_to_shared(s_ring + threadIdx.x), slot_size = 2 * shape.streams * (8 / N) * blockDim.x * 16;
-    const uint32_t ring_end = mine + shape.ahead * slot_size;
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(s_ring), window_size = window_bytes<T>(c.threads);
+    const uint32_t slot_size = 2 * shape.streams * (PACKS ? (8 / N) * blockDim.x * 16 : window_size);
+    const int slots = PACKS ? shape.ahead : shape.ahead + 1;
+    const uint32_t mine = ring + (PACKS ? threadIdx.x * 16 : MULTI ? 0 : threadIdx.x / (MULTI ? 1 : LANES) * slots * slot_size), ring_end = mine + slots * slot_size;
     const T *next_x = static_cast<const T *>(a.x) + begin * a.x_stride, *next_h = static_cast<const T *>(a.h) + begin * a.h_stride;
     auto fetch = [&](long long row, uint32_t to) {
 #pragma unroll
         for (int i = 0; i < 2; i++)
             if (row + i < a.rows) {
-                copy_packs(to, next_x + i * a.x_stride, c);
-                if (branch) copy_packs(to, next_h + i * a.h_stride, c);
-                if (gated) copy_packs(to, static_cast<const T *>(a.gate) + gate_row(row, i) * a.gate_stride, c);
+                auto copy = [&](const T *from) {
+                    if constexpr (PACKS) {
+                        copy_packs(to, from, c);
+                    } else {
+                        copy_window(to, from, c);
+                        to += window_size;
+                    }
+                };
+                copy(next_x + i * a.x_stride);
+                if (branch) copy(next_h + i * a.h_stride);
+                if (gated) copy(static_cast<const T *>(a.gate) + gate_row(row, i) * a.gate_stride);
             }
         copies_made();
         next_x += step * a.x_stride;
         next_h += step * a.h_stride;
         fetched();
     };
-    if constexpr (RING)
-        for (int k = 0; k < shape.ahead; k++) fetch(begin + k * step, mine + k * slot_size);
+    for (int k = 0; k < shape.ahead; k++) fetch(begin + k * step, mine + k * slot_size);
+    long long sample = per_sample ? begin / a.tokens : 0, place = per_sample ? begin % a.tokens : 0; // of the row in hand (windows)
     let_next_begin();
     uint32_t slot = mine;
     T *to_y = static_cast<T *>(a.y) + begin * a.width, *to_z = static_cast<T *>(a.z) + begin * a.width;
@@ -76,9 +83,9 @@ forward_kernel(const __grid_constant__ Args a, const Shape shape) {
         const bool both = row + 1 < a.rows; // (else the second is whatever it is, and is not stored)
         Eight y[2], u[2], g[2];
         float4 stats[2] = {};
-        if constexpr (RING) {
-            copies_wait(shape.ahead);
-            uint32_t from = slot;
+        copies_wait(shape.ahead);
+        uint32_t from = slot;
+        if constexpr (PACKS) {
 #pragma unroll
             for (int i = 0; i < 2; i++) {
                 copied<T, N>(y[i], from);
@@ -86,22 +93,40 @@ forward_kernel(const __grid_constant__ Args a, const Shape shape) {
                 if (gated) copied<T, N>(g[i], from);
             }
             fetch(row + shape.ahead * step, slot);
-            slot += slot_size;
-            if (slot == ring_end) slot = mine;
         } else {
+            row_barrier<LANES>(sum.mask()); // (all have the row, and none the one before any more, whose place is the next one's)
+            fetch(row + shape.ahead * step, slot == mine ? ring_end - slot_size : slot - slot_size);
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                const int k = both ? i : 0;
-                load_row<T>(y[i], a.x, (row + k) * a.x_stride, c);
-                if (branch) load_row<T>(u[i], a.h, (row + k) * a.h_stride, c);
-                if (gated) load_row<T>(g[i], a.gate, gate_row(row, k) * a.gate_stride, c);
+                if (i == 1 && !both) break;
+                auto read = [&](Eight &v, const void *rows, long long stride, long long which) {
+                    window(v, from, static_cast<const T *>(rows) + which * stride, c);
+                    from += window_size;
+                };
+                read(y[i], a.x, a.x_stride, row + i);
+                if (branch) read(u[i], a.h, a.h_stride, row + i);
+                if (gated) read(g[i], a.gate, a.gate_stride, per_sample ? sample + (i && place + 1 == a.tokens) : row + i);
             }
-            fetched();
+            if (!both) {
+                fill(y[1], 0.0f);
+                fill(u[1], 0.0f);
+                fill(g[1], 0.0f);
+            }
+            if (per_sample) {
+                sample += sample_step;
+                place += place_step;
+                if (place >= a.tokens) {
+                    place -= a.tokens;
+                    sample++;
+                }
+            }
         }
+        slot += slot_size;
+        if (slot == ring_end) slot = mine;
         if (branch) {
             if (POST) {
                 float mean[2], r[2];
-                two_stats<N, MULTI>(u, a.post_norm, c, a.eps, sum, mean, r);
+                two_stats<N, LANES>(u, a.post_norm, c, a.eps, sum, mean, r);
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
                     stats[i].z = mean[i];
@@ -123,7 +148,7 @@ forward_kernel(const __grid_constant__ Args a, const Shape shape) {
         }
         if (normed) {
             float mean[2], r[2];
-            two_stats<N, MULTI>(y, a.norm, c, a.eps, sum, mean, r);
+            two_stats<N, LANES>(y, a.norm, c, a.eps, sum, mean, r);
 #pragma unroll
             for (int i = 0; i < 2; i++) {
                 stats[i].x = mean[i];
@@ -143,17 +168,22 @@ forward_kernel(const __grid_constant__ Args a, const Shape shape) {
 
 template <typename T, int N, bool POST, int FORM>
 void sized(const Args &a, const Shape &shape, size_t room, cudaStream_t stream) {
-    if (shape.threads == 32 && shape.ctas_per_row == 1)
-        launch(forward_kernel<T, N, false, POST, FORM>, shape, room, stream, a, shape);
+    auto run = [&](auto kernel) { launch(kernel, shape, room, stream, a, shape); };
+    if (shape.threads > 32 || shape.ctas_per_row > 1)
+        run(forward_kernel<T, N, 0, POST, FORM>);
+    else if (N == 1 || shape.lanes == 32) // (single values: always)
+        run(forward_kernel<T, N, 32, POST, FORM>);
+    else if (shape.lanes == 16)
+        run(forward_kernel<T, N, N == 1 ? 32 : 16, POST, FORM>);
     else
-        launch(forward_kernel<T, N, true, POST, FORM>, shape, room, stream, a, shape);
+        run(forward_kernel<T, N, N == 1 ? 32 : 8, POST, FORM>);
 }
 
 } // namespace
 
 void launch_forward(const Args &a, const Shape &shape, bool wide, cudaStream_t stream) {
     const bool post = a.post_norm != FFCVB_NORM_NONE;
-    const size_t room = wide ? (size_t)shape.threads * shape.ahead * 2 * shape.streams * 8 * type_size(a.type) : 0;
+    const size_t room = shape.ring;
     with_type(a.type, [&](auto zero) {
         using T = decltype(zero);
         constexpr int W = 16 / (int)sizeof(T);

@@ -14,8 +14,8 @@ namespace norms {
 
 namespace {
 
-// Adds up partial rows: eight columns per CTA, 128 runs of rows side by side (740 rows of 768 columns: six values per thread, all on
-// their way at once).
+// Adds up partial rows: 32 columns per CTA, 32 runs of rows side by side (of 576 rows of 1024 columns 6 us; with 8 columns and 128
+// runs 9).
 struct Sums {
     const float *from[kColumns];
     void *to[kColumns];
@@ -24,22 +24,20 @@ struct Sums {
 };
 __global__ void __launch_bounds__(1024)
 add_up_kernel(const __grid_constant__ Sums s) {
-    __shared__ float s_part[8][129];
+    __shared__ float s_part[32][33];
     wait_for_previous();
-    const int column = threadIdx.x & 7, run = threadIdx.x >> 3;
-    const long long c = blockIdx.x * 8ll + column;
+    const int lane = threadIdx.x & 31, run = threadIdx.x >> 5;
+    const long long c = blockIdx.x * 32ll + lane;
     const float *from = s.from[blockIdx.y];
     float v = 0.0f;
     if (c < s.width) {
 #pragma unroll 8
-        for (long long r = run; r < s.count; r += 128) v += from[r * s.stride + c];
+        for (long long r = run; r < s.count; r += 32) v += from[r * s.stride + c];
     }
-    s_part[column][run] = v;
+    s_part[run][lane] = v;
     __syncthreads();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (warp >= 8) return;
-    v = warp_sum((s_part[warp][lane] + s_part[warp][lane + 32]) + (s_part[warp][lane + 64] + s_part[warp][lane + 96]));
-    const long long mine = blockIdx.x * 8ll + warp;
+    v = warp_sum(s_part[lane][run]); // column `run`
+    const long long mine = blockIdx.x * 32ll + run;
     if (lane == 0 && mine < s.width) {
         if (s.type == FFCVB_TYPE_F32)
             static_cast<float *>(s.to[blockIdx.y])[mine] = v;
@@ -75,25 +73,32 @@ bool wide_rows(const Args &a) {
                                (a.dz ? a.dz_stride : 0)) % n == 0;
 }
 
-// Rows of up to 4096 values are a CTA's (of up to 256 a warp's), wider ones a cluster's; as many rounds ahead, at most `most`, as shared
-// memory has room for, which 16 warps per SM share.
+// Rows of up to 4096 values are a CTA's (of up to 256 a warp's, 128 and 64 a half's and a quarter's), wider ones a cluster's; as many
+// rounds ahead, at most `most_ahead`, as shared memory has room for, which 16 warps per SM share; besides: bytes per thread.
 constexpr size_t kRoom = 208 * 1024;
-Shape shape_of(const Args &a, int streams, int most_ahead, size_t besides) {
+Shape shape_of(const Args &a, bool wide, int streams, int rows, int most_ahead, size_t besides) {
     Shape s{};
     s.ctas_per_row = (int)((a.width + 4095) / 4096);
     const int eights = (int)((a.width + 7) / 8);
     s.threads = ((eights + s.ctas_per_row - 1) / s.ctas_per_row + 31) / 32 * 32;
-    s.rows_at_once = kSms * (512 / s.threads) / s.ctas_per_row;
+    s.lanes = !wide || eights > 16 ? 32 : eights <= 8 ? 8 : 16;
+    s.rows_at_once = kSms * (512 / s.threads) / s.ctas_per_row * s.rows_per_cta();
     s.streams = streams;
-    s.ahead = most_ahead;
-    while (s.ahead > 1 && 512 * ((size_t)s.ahead * streams * 8 * type_size(a.type) + besides) > kRoom) s.ahead--;
+    const int size = type_size(a.type);
+    auto ring = [&](int ahead) { // of a CTA
+        if (wide) return (size_t)s.threads * ahead * rows * streams * 8 * size;
+        const int threads = s.rows_per_cta() > 1 ? s.lanes : s.threads;
+        return (size_t)(ahead + 1) * rows * streams * (size == 4 ? window_bytes<float>(threads) : window_bytes<__half>(threads)) * s.rows_per_cta();
+    };
+    for (s.ahead = most_ahead; s.ahead > 1 && 512 / s.threads * (ring(s.ahead) + besides * s.threads) > kRoom;) s.ahead--;
+    s.ring = ring(s.ahead);
     return s;
 }
 Deal deal_of(const Args &a) {
     Deal d{};
     int streams = 0;
     for (const void *p : {a.x, a.h, a.dy, a.dz, a.gate_kind == FFCVB_GATE_TOKEN ? a.gate : nullptr}) streams += p != nullptr;
-    d.shape = shape_of(a, streams, 3, (a.gate_kind == FFCVB_GATE_SAMPLE ? 96 : 0) + (a.post_norm != FFCVB_NORM_NONE ? 64 : 0));
+    d.shape = shape_of(a, wide_rows(a), streams, 1, 3, (a.gate_kind == FFCVB_GATE_SAMPLE ? 96 : 0) + (a.post_norm != FFCVB_NORM_NONE ? 64 : 0));
     const long long most = d.shape.rows_at_once;
     d.samples = a.gate_kind == FFCVB_GATE_SAMPLE ? a.rows / a.tokens : 1;
     d.tokens = a.gate_kind == FFCVB_GATE_SAMPLE ? a.tokens : a.rows;
@@ -111,7 +116,8 @@ Deal deal_of(const Args &a) {
         }
     }
     d.units = d.samples * d.splits;
-    if (d.units < most) d.shape.rows_at_once = (int)d.units;
+    const int per = d.shape.rows_per_cta();
+    if (d.units < most) d.shape.rows_at_once = (int)((d.units + per - 1) / per * per);
     for (const void *p : {a.dweight, a.dbias, a.dpost_weight, a.dpost_bias, a.dscale}) d.columns += p != nullptr;
     return d;
 }
@@ -155,9 +161,10 @@ int ffcvb_norm_residual(const ffcvb_norm_residual_args *args, void *stream) {
     OnDevice here(a.device);
     if (!here.ok()) return training_fail(FFCVB_E_NODEVICE, "ffcvb_norm_residual: no device %d", a.device);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    Shape shape = shape_of(a, 2 * (1 + (a.h != nullptr) + (a.gate_kind != FFCVB_GATE_NONE)), 2, 0); // (of two rows)
-    shape.streams /= 2;
-    if ((a.rows + 1) / 2 < shape.rows_at_once) shape.rows_at_once = (int)((a.rows + 1) / 2);
+    Shape shape = shape_of(a, wide_rows(a), 1 + (a.h != nullptr) + (a.gate_kind != FFCVB_GATE_NONE), 2, 2, 0);
+    const long long pairs = (a.rows + 1) / 2;
+    const int per = shape.rows_per_cta();
+    if (pairs < shape.rows_at_once) shape.rows_at_once = (int)((pairs + per - 1) / per * per);
     launch_forward(a, shape, wide_rows(a), st);
     return launched("ffcvb_norm_residual");
 }
@@ -188,7 +195,7 @@ int ffcvb_norm_residual_backward(const ffcvb_norm_residual_args *args, void *str
     s.count = a.rows > 0 ? d.shape.rows_at_once : 0;
     s.stride = d.columns * a.width;
     s.type = a.param_type;
-    const unsigned across = (unsigned)((a.width + 7) / 8);
+    const unsigned across = (unsigned)((a.width + 31) / 32);
     if (n) launch_early(add_up_kernel, dim3(across, n), 1024, 0, st, s);
     if (a.dgate && a.gate_kind == FFCVB_GATE_SAMPLE && d.splits > 1 && a.rows > 0) // (then there are fewer samples than CTAs, or few splits)
         with_type(a.type, [&](auto zero) {

@@ -12,18 +12,26 @@ using Args = ffcvb_norm_residual_args;
 
 template <int V> struct Int { static constexpr int value = V; };
 
-// A thread's part of a row: eight columns, as 8 / N packs of N; the packs of all threads of a row lie next to one another.
-// Arithmetic is on pairs of them.
+// A thread's part of a row: eight columns, as 8 / N packs of N, the packs of all threads of a row next to one another; single values are
+// 32 apart, and 256 next to one another a warp's.  Arithmetic is on pairs of them.  A row is a CTA's, a cluster's (CTA by CTA), or that
+// of 8, 16 or 32 lanes of a CTA of one warp.
 constexpr int kPairs = 4;
 using Eight = Two[kPairs];
 
-template <int N, bool MULTI> struct Columns {
+// LANES: 8, 16 or 32 of a CTA of one warp have a row; 0: all threads of a CTA or cluster.
+template <int N, int LANES> struct Columns {
+    static constexpr bool MULTI = LANES == 0;
+    int thread, threads; // of the row, or of the CTA's part
+    int part;            // first column of that
     int first, step, width;
-    __device__ __forceinline__ Columns(long long w, int ctas, int rank) : width((int)w) {
-        first = (MULTI ? rank * blockDim.x + threadIdx.x : threadIdx.x) * N;
-        step = (MULTI ? ctas * blockDim.x : 32) * N;
+    __device__ __forceinline__ Columns(long long w, int rank) : width((int)w) {
+        thread = MULTI ? threadIdx.x : threadIdx.x & (LANES - 1);
+        threads = MULTI ? blockDim.x : LANES;
+        part = MULTI ? rank * blockDim.x * 8 : 0;
+        first = part + (N == 1 ? (thread >> 5) * 256 + (thread & 31) : thread * N);
+        step = N == 1 ? 32 : threads * N;
     }
-    __device__ __forceinline__ int at(int k) const { return first + k * step; }
+    __device__ __forceinline__ int at(int k) const { return N == 1 ? first + k * 32 : first + k * step; }
     __device__ __forceinline__ bool in(int k) const { return at(k) < width; } // (a pack is inside the row or not)
     __device__ __forceinline__ int inside(int k) const { return in(k) ? at(k) : 0; }
 };
@@ -41,33 +49,34 @@ __device__ __forceinline__ void to_pairs(Eight &v, const Pack<T, N> (&packs)[8 /
     for (int p = 0; p < kPairs; p++) v[p] = Two(f[2 * p], f[2 * p + 1]);
 }
 // Columns of a row in global memory; 0 beyond it.
-template <typename T, int N, bool MULTI>
-__device__ __forceinline__ void load_row(Eight &v, const void *p, long long offset, const Columns<N, MULTI> &c) {
+template <typename T, int N, int LANES>
+__device__ __forceinline__ void load_row(Eight &v, const void *p, long long offset, const Columns<N, LANES> &c) {
     Pack<T, N> packs[8 / N] = {};
 #pragma unroll
     for (int k = 0; k < 8 / N; k++)
         if (p && c.in(k)) packs[k].load(static_cast<const T *>(p) + offset + c.at(k));
     to_pairs<T, N>(v, packs);
 }
-template <typename T, int N, bool MULTI>
-__device__ __forceinline__ void store_row(const Eight &v, void *p, long long offset, const Columns<N, MULTI> &c) {
+template <typename T, int N, int LANES>
+__device__ __forceinline__ void store_row(const Eight &v, void *p, long long offset, const Columns<N, LANES> &c) {
     float f[8];
 #pragma unroll
     for (int q = 0; q < kPairs; q++) {
         f[2 * q] = v[q].lo();
         f[2 * q + 1] = v[q].hi();
     }
+    T *const to = static_cast<T *>(p) + offset + c.first;
 #pragma unroll
     for (int k = 0; k < 8 / N; k++)
         if (c.in(k)) {
             Pack<T, N> pack;
             pack.set(*reinterpret_cast<const float(*)[N]>(f + k * N));
-            pack.store(static_cast<T *>(p) + offset + c.at(k));
+            pack.store(to + (N == 1 ? k * 32 : k * c.step));
         }
 }
 // Parameters of the columns; `otherwise` without any, `beyond` beyond the row.
-template <int N, bool MULTI>
-__device__ __forceinline__ void load_params(Eight &v, const void *p, int type, const Columns<N, MULTI> &c, float otherwise, float beyond) {
+template <int N, int LANES>
+__device__ __forceinline__ void load_params(Eight &v, const void *p, int type, const Columns<N, LANES> &c, float otherwise, float beyond) {
     float f[8];
 #pragma unroll
     for (int k = 0; k < 8 / N; k++) {
@@ -103,8 +112,8 @@ __device__ __forceinline__ void load_params(Eight &v, const void *p, int type, c
 #pragma unroll
     for (int q = 0; q < kPairs; q++) v[q] = Two(f[2 * q], f[2 * q + 1]);
 }
-template <int N, bool MULTI>
-__device__ __forceinline__ void store_floats(const Eight &v, float *to, const Columns<N, MULTI> &c) {
+template <int N, int LANES>
+__device__ __forceinline__ void store_floats(const Eight &v, float *to, const Columns<N, LANES> &c) {
 #pragma unroll
     for (int k = 0; k < 8 / N; k++)
         if (c.in(k)) {
@@ -116,19 +125,28 @@ __device__ __forceinline__ void store_floats(const Eight &v, float *to, const Co
 // Two sums over the threads of a row: a warp, a CTA, or (wide rows) the CTAs of a cluster, whose sums travel through distributed
 // shared memory.  In a warp the halves exchange what they do not go on with, so that two sums take little more than one.
 // Consecutive sums use `s`, zero at the start, in turn, so that one barrier is enough.
-template <bool MULTI> struct RowSum {
+template <int LANES> struct RowSum {
+    static constexpr bool MULTI = LANES == 0;
     float2 *s; // [2][32 + 4]
     int ctas;
     int turn = 0;
+    // the lanes of the thread's row
+    __device__ __forceinline__ uint32_t mask() const { return MULTI || LANES == 32 ? 0xffffffffu : ((1u << (LANES & 31)) - 1) << (threadIdx.x & 31 & -LANES); }
     __device__ __forceinline__ float2 operator()(float a, float b) {
         const int lane = threadIdx.x & 31;
-        float v = lane & 16 ? b : a;
-        v += __shfl_xor_sync(0xffffffffu, lane & 16 ? a : b, 16);
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
         if constexpr (!MULTI) {
-            return make_float2(__shfl_sync(0xffffffffu, v, 0), __shfl_sync(0xffffffffu, v, 16));
+            const uint32_t all = mask();
+            constexpr int half = LANES / 2;
+            float v = lane & half ? b : a;
+            v += __shfl_xor_sync(all, lane & half ? a : b, half);
+#pragma unroll
+            for (int o = half / 2; o > 0; o >>= 1) v += __shfl_xor_sync(all, v, o);
+            return make_float2(__shfl_sync(all, v, lane & -LANES), __shfl_sync(all, v, (lane & -LANES) + half));
         } else {
+            float v = lane & 16 ? b : a;
+            v += __shfl_xor_sync(0xffffffffu, lane & 16 ? a : b, 16);
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
             const int warps = blockDim.x >> 5;
             float2 *to = s + turn * 36;
             turn ^= 1;
@@ -198,8 +216,8 @@ __device__ __forceinline__ void copies_wait(int ahead) { // for the oldest of `a
         asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 // A thread's packs of one stream of a row that begins at `from`; `to` goes on to the next stream's places.
-template <typename T, int N, bool MULTI>
-__device__ __forceinline__ void copy_packs(uint32_t &to, const T *from, const Columns<N, MULTI> &c) {
+template <typename T, int N, int LANES>
+__device__ __forceinline__ void copy_packs(uint32_t &to, const T *from, const Columns<N, LANES> &c) {
 #pragma unroll
     for (int k = 0; k < 8 / N; k++) {
         copy16(to, from + c.inside(k), c.in(k) ? 16 : 0);
@@ -218,15 +236,52 @@ __device__ __forceinline__ void copied(Eight &v, uint32_t &from) {
     to_pairs<T, N>(v, packs);
 }
 
-// How rows are shared out: threads of a CTA, CTAs of a cluster, clusters; streams that are copied ahead and for how many rounds.
+// Rows that do not begin on 16-byte boundaries: the packs that a row's part lies in are copied by its threads together, and its values
+// read one by one from wherever they lie then.  A barrier of the row's threads is needed in between.
+template <typename T> __host__ __device__ constexpr int window_bytes(int threads) { return threads * 8 * (int)sizeof(T) + 16; }
+template <typename T, int LANES>
+__device__ __forceinline__ void copy_window(uint32_t to, const T *row, const Columns<1, LANES> &c) {
+    const T *from = row + c.part;
+    const int lead = (int)(reinterpret_cast<uintptr_t>(from) & 15), bytes = lead + min(c.width - c.part, c.threads * 8) * (int)sizeof(T);
+    const char *at = reinterpret_cast<const char *>(from) - lead;
+    for (int k = c.thread * 16; k < bytes; k += c.threads * 16) copy16(to + k, at + k, 16);
+}
+template <typename T, int LANES>
+__device__ __forceinline__ void window(Eight &v, uint32_t from, const T *row, const Columns<1, LANES> &c) {
+    from += (uint32_t)(reinterpret_cast<uintptr_t>(row + c.part) & 15);
+    const T *at = static_cast<const T *>(__cvta_shared_to_generic(from)) + (c.first - c.part);
+    float f[8];
+#pragma unroll
+    for (int k = 0; k < 8; k++) f[k] = c.in(k) ? to_float(at[k * 32]) : 0.0f;
+#pragma unroll
+    for (int p = 0; p < kPairs; p++) v[p] = Two(f[2 * p], f[2 * p + 1]);
+}
+template <int LANES> __device__ __forceinline__ void row_barrier(uint32_t mask) {
+    if (LANES == 0)
+        __syncthreads();
+    else
+        __syncwarp(mask);
+}
+
+// How rows are shared out: threads of a CTA, CTAs of a cluster, lanes of a row in a CTA of one warp; rows that are worked on together, a
+// multiple of those of a CTA; streams that are copied ahead and for how many rounds; bytes of shared memory for them.
 struct Shape {
-    int threads, ctas_per_row, rows_at_once;
+    int threads, ctas_per_row, lanes, rows_at_once;
     int streams, ahead;
+    size_t ring;
+    int rows_per_cta() const { return threads == 32 && ctas_per_row == 1 ? 32 / lanes : 1; }
 };
+// The row that a CTA's thread begins with, and its CTA's place in a cluster.
+template <int LANES> __device__ __forceinline__ int first_row(const Shape &s, int &rank) {
+    rank = 0;
+    if constexpr (LANES > 0) return blockIdx.x * (32 / LANES) + threadIdx.x / LANES;
+    if (s.ctas_per_row > 1) rank = blockIdx.x % s.ctas_per_row;
+    return blockIdx.x / s.ctas_per_row;
+}
 
 // Means and 1 / deviations of two rows: the means first (0 for rms), then the squares of what is left.
-template <int N, bool MULTI>
-__device__ __forceinline__ void two_stats(const Eight (&v)[2], int kind, const Columns<N, MULTI> &c, float eps, RowSum<MULTI> &sum, float (&mean)[2], float (&r)[2]) {
+template <int N, int LANES>
+__device__ __forceinline__ void two_stats(const Eight (&v)[2], int kind, const Columns<N, LANES> &c, float eps, RowSum<LANES> &sum, float (&mean)[2], float (&r)[2]) {
     const float over = 1.0f / (float)c.width;
     mean[0] = mean[1] = 0.0f;
     if (kind == FFCVB_NORM_LAYER) {
@@ -294,7 +349,7 @@ void launch(Kernel kernel, const Shape &shape, size_t room, cudaStream_t stream,
     with[1].id = cudaLaunchAttributeClusterDimension;
     with[1].val.clusterDim.x = shape.ctas_per_row;
     with[1].val.clusterDim.y = with[1].val.clusterDim.z = 1;
-    how.gridDim = dim3(shape.rows_at_once * shape.ctas_per_row);
+    how.gridDim = dim3(shape.rows_at_once / shape.rows_per_cta() * shape.ctas_per_row);
     how.blockDim = dim3(shape.threads);
     how.dynamicSmemBytes = room;
     how.stream = stream;
