@@ -272,12 +272,12 @@ void sized(const Args &a, const Deal &d, const Partials &part, size_t room, cuda
     auto run = [&](auto kernel) { launch(kernel, d.shape, room, stream, a, d, part); };
     if (d.shape.threads > 32 || d.shape.ctas_per_row > 1)
         run(backward_kernel<T, N, 0, POST, FORM>);
-    else if (N == 1 || d.shape.lanes == 32) // (single values: always)
+    else if (d.shape.lanes == 32)
         run(backward_kernel<T, N, 32, POST, FORM>);
     else if (d.shape.lanes == 16)
-        run(backward_kernel<T, N, N == 1 ? 32 : 16, POST, FORM>);
+        run(backward_kernel<T, N, 16, POST, FORM>);
     else
-        run(backward_kernel<T, N, N == 1 ? 32 : 8, POST, FORM>);
+        run(backward_kernel<T, N, 8, POST, FORM>);
 }
 
 } // namespace

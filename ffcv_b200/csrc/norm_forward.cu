@@ -171,12 +171,12 @@ void sized(const Args &a, const Shape &shape, size_t room, cudaStream_t stream) 
     auto run = [&](auto kernel) { launch(kernel, shape, room, stream, a, shape); };
     if (shape.threads > 32 || shape.ctas_per_row > 1)
         run(forward_kernel<T, N, 0, POST, FORM>);
-    else if (N == 1 || shape.lanes == 32) // (single values: always)
+    else if (shape.lanes == 32)
         run(forward_kernel<T, N, 32, POST, FORM>);
     else if (shape.lanes == 16)
-        run(forward_kernel<T, N, N == 1 ? 32 : 16, POST, FORM>);
+        run(forward_kernel<T, N, 16, POST, FORM>);
     else
-        run(forward_kernel<T, N, N == 1 ? 32 : 8, POST, FORM>);
+        run(forward_kernel<T, N, 8, POST, FORM>);
 }
 
 } // namespace

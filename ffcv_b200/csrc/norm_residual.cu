@@ -81,7 +81,7 @@ Shape shape_of(const Args &a, bool wide, int streams, int rows, int most_ahead, 
     s.ctas_per_row = (int)((a.width + 4095) / 4096);
     const int eights = (int)((a.width + 7) / 8);
     s.threads = ((eights + s.ctas_per_row - 1) / s.ctas_per_row + 31) / 32 * 32;
-    s.lanes = !wide || eights > 16 ? 32 : eights <= 8 ? 8 : 16;
+    s.lanes = eights > 16 ? 32 : eights <= 8 ? 8 : 16;
     s.rows_at_once = kSms * (512 / s.threads) / s.ctas_per_row * s.rows_per_cta();
     s.streams = streams;
     const int size = type_size(a.type);

@@ -13,7 +13,7 @@ using Args = ffcvb_norm_residual_args;
 template <int V> struct Int { static constexpr int value = V; };
 
 // A thread's part of a row: eight columns, as 8 / N packs of N, the packs of all threads of a row next to one another; single values are
-// 32 apart, and 256 next to one another a warp's.  Arithmetic is on pairs of them.  A row is a CTA's, a cluster's (CTA by CTA), or that
+// 32 apart (or as many as lanes have the row), and 256 next to one another a warp's.  Arithmetic is on pairs of them.  A row is a CTA's, a cluster's (CTA by CTA), or that
 // of 8, 16 or 32 lanes of a CTA of one warp.
 constexpr int kPairs = 4;
 using Eight = Two[kPairs];
@@ -29,9 +29,10 @@ template <int N, int LANES> struct Columns {
         threads = MULTI ? blockDim.x : LANES;
         part = MULTI ? rank * blockDim.x * 8 : 0;
         first = part + (N == 1 ? (thread >> 5) * 256 + (thread & 31) : thread * N);
-        step = N == 1 ? 32 : threads * N;
+        step = N == 1 ? kApart : threads * N;
     }
-    __device__ __forceinline__ int at(int k) const { return N == 1 ? first + k * 32 : first + k * step; }
+    static constexpr int kApart = MULTI ? 32 : LANES; // of single values
+    __device__ __forceinline__ int at(int k) const { return first + k * (N == 1 ? kApart : step); }
     __device__ __forceinline__ bool in(int k) const { return at(k) < width; } // (a pack is inside the row or not)
     __device__ __forceinline__ int inside(int k) const { return in(k) ? at(k) : 0; }
 };
@@ -71,7 +72,7 @@ __device__ __forceinline__ void store_row(const Eight &v, void *p, long long off
         if (c.in(k)) {
             Pack<T, N> pack;
             pack.set(*reinterpret_cast<const float(*)[N]>(f + k * N));
-            pack.store(to + (N == 1 ? k * 32 : k * c.step));
+            pack.store(to + k * (N == 1 ? c.kApart : c.step));
         }
 }
 // Parameters of the columns; `otherwise` without any, `beyond` beyond the row.
@@ -252,7 +253,7 @@ __device__ __forceinline__ void window(Eight &v, uint32_t from, const T *row, co
     const T *at = static_cast<const T *>(__cvta_shared_to_generic(from)) + (c.first - c.part);
     float f[8];
 #pragma unroll
-    for (int k = 0; k < 8; k++) f[k] = c.in(k) ? to_float(at[k * 32]) : 0.0f;
+    for (int k = 0; k < 8; k++) f[k] = c.in(k) ? to_float(at[k * Columns<1, LANES>::kApart]) : 0.0f;
 #pragma unroll
     for (int p = 0; p < kPairs; p++) v[p] = Two(f[2 * p], f[2 * p + 1]);
 }
