@@ -1,8 +1,9 @@
 // Rotary positions of queries and keys (sm_100a): pair (a, b) of a head at angle t becomes
 // amplitude * (a cos t - b sin t, a sin t + b cos t).
 // A CTA takes a tile of tokens: first the sines and cosines of all their pairs, once for all heads, into shared
-// memory, then the heads.  Angles are counted in turns: the product of position and turns per position is made in 64 bits and
-// whole turns are taken off there, which leaves nothing of a long context's angles to lose in 32.
+// memory, then the heads.  Angles are counted in turns.  Whole positions multiply turns in units of 2^-64 of a turn: the product's low
+// 64 bits are what is left of it without whole turns, whatever the position; its upper 32 are the angle, to 2^-33 of a turn.  Positions
+// that are floats multiply in 64-bit floats.  So nothing of a long context's angles is lost.
 #include "training.h"
 #include "two.h"
 
@@ -13,8 +14,8 @@ namespace {
 using Args = ffcvb_rotary_args;
 
 constexpr int kThreads = 256;
-constexpr int kTileAngles = 2048; // angles of a tile (16 KB)
-constexpr int kAtOnce = 4;        // tokens that a thread has on their way
+constexpr int kTileAngles = 4096; // angles of a tile at most (32 KB)
+constexpr int kTileBytes = 32 * 1024; // of queries and keys of a tile at least, where that many angles allow it
 
 // (a, b) -> (a c - b s, a s + b c) for pairs of either.
 __device__ __forceinline__ void turn(Two &a, Two &b, Two c, Two s) {
@@ -26,8 +27,10 @@ __device__ __forceinline__ void turn(Two &a, Two &b, Two c, Two s) {
 // A head's slots: packs that turn (with their partners, half the rotated part on), then packs that are copied.  A thread has the same slot of the same
 // head of several tokens, one after the other; where a token has fewer slots than a CTA threads, tokens lie side by side.
 template <typename T, int N, bool INTERLEAVED>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 5)
 rotary_kernel(const __grid_constant__ Args a, int tile) {
+    // tokens that a thread has on their way: four packs (with eight 65536 tokens of 40 half-turned heads of 128 take 667 us, not 462)
+    constexpr int kAtOnce = INTERLEAVED || N * sizeof(T) < 16 ? 4 : 2;
     extern __shared__ float s_cos[]; // [tile][pairs], then the sines
     wait_for_previous();
     let_next_begin();
@@ -36,16 +39,28 @@ rotary_kernel(const __grid_constant__ Args a, int tile) {
     const long long tiles = (a.tokens + tile - 1) / tile;
     const long long b = blockIdx.x / tiles, first = blockIdx.x % tiles * tile;
     const int tokens = (int)min((long long)tile, a.tokens - first);
-    for (int k = threadIdx.x; k < tokens * pairs; k += kThreads) {
-        const int t = k / pairs, i = k % pairs;
-        const long long at = b * a.positions_stride + (first + t) * a.axes + (a.axes == 2 && i >= pairs / 2);
-        const double where = a.positions_float ? (double)static_cast<const float *>(a.positions)[at]
-                                               : (double)static_cast<const int64_t *>(a.positions)[at];
-        const double turns = where * a.turns[i];
-        float sine, cosine;
-        sincospif((float)(2.0 * (turns - rint(turns))), &sine, &cosine);
-        s_cos[k] = cosine * a.amplitude;
-        s_sin[k] = (a.transpose ? sine : -sine) * a.amplitude;
+    // a thread makes the angles of one pair, of several tokens, or (more pairs than threads) of several pairs
+    const int across = min(pairs, kThreads), beside = kThreads / across;
+    for (int i = threadIdx.x % across; i < pairs && threadIdx.x < across * beside; i += across) {
+        const double turns = a.turns[i];
+        const uint64_t steps = a.steps[i];
+        const long long begin = b * a.positions_stride + first * a.axes + (a.axes == 2 && i >= pairs / 2);
+#pragma unroll 2
+        for (int t = threadIdx.x / across; t < tokens; t += beside) {
+            const long long at = begin + t * a.axes;
+            float angle; // in half turns, -1 .. 1
+            if (a.positions_float) {
+                const double turned = static_cast<const float *>(a.positions)[at] * turns;
+                angle = (float)(2.0 * (turned - rint(turned)));
+            } else {
+                const uint64_t turned = (uint64_t)static_cast<const int64_t *>(a.positions)[at] * steps;
+                angle = (float)(int32_t)(turned >> 32) * 4.656612873077393e-10f; // 2^-31
+            }
+            float sine, cosine;
+            sincospif(angle, &sine, &cosine);
+            s_cos[t * pairs + i] = cosine * a.amplitude;
+            s_sin[t * pairs + i] = (a.transpose ? sine : -sine) * a.amplitude;
+        }
     }
     __syncthreads();
     constexpr int PER = INTERLEAVED && N == 1 ? 2 : N; // values of a turning slot, or of a half of it
@@ -104,8 +119,13 @@ rotary_kernel(const __grid_constant__ Args a, int tile) {
                         float u[N], v[N];
                         p[i].get(u);
                         q[i].get(v);
+        if constexpr (N == 2) {
+                            Two x(u[0], u[1]), y(v[0], v[1]);
+                            turn(x, y, Two(c[0], c[1]), Two(s[0], s[1]));
+                            u[0] = x.lo(), u[1] = x.hi(), v[0] = y.lo(), v[1] = y.hi();
+                        }
 #pragma unroll
-                        for (int j = 0; j < N; j += 4) {
+                        for (int j = 0; j + 3 < N; j += 4) {
                             const float4 cc = *reinterpret_cast<const float4 *>(c + j), ss = *reinterpret_cast<const float4 *>(s + j);
                             Two u0(u[j], u[j + 1]), u1(u[j + 2], u[j + 3]), v0(v[j], v[j + 1]), v1(v[j + 2], v[j + 3]);
                             turn(u0, v0, Two(cc.x, cc.y), Two(ss.x, ss.y));
@@ -137,13 +157,15 @@ extern "C" int ffcvb_rotary(const ffcvb_rotary_args *args, void *stream) {
         (a.axes != 1 && a.axes != 2) || a.rotary_dim % (2 * a.axes) || a.heads + a.kv_heads > 0xffff || (a.type != FFCVB_TYPE_F32 && a.type != FFCVB_TYPE_F16 && a.type != FFCVB_TYPE_BF16))
         return training_fail(FFCVB_E_ARG, "ffcvb_rotary: bad size or type");
     if (a.batch * a.tokens * (a.heads + a.kv_heads) == 0) return FFCVB_OK;
-    if (!a.positions || !a.turns || (a.heads > 0 && (!a.q || !a.q_out)) || (a.kv_heads > 0 && (!a.k || !a.k_out)))
+    if (!a.positions || !a.turns || !a.steps || (a.heads > 0 && (!a.q || !a.q_out)) || (a.kv_heads > 0 && (!a.k || !a.k_out)))
         return training_fail(FFCVB_E_ARG, "ffcvb_rotary: bad argument");
     OnDevice here(a.device);
     if (!here.ok()) return training_fail(FFCVB_E_NODEVICE, "ffcvb_rotary: no device %d", a.device);
     const int pairs = (int)a.rotary_dim / 2;
-    int tile = kTileAngles / pairs;
-    if (tile > 16) tile = 16;
+    const long long token = (a.heads + a.kv_heads) * a.head_dim * type_size(a.type);
+    int tile = (int)(kTileBytes / token);
+    if (tile < 16) tile = 16;
+    if (tile > kTileAngles / pairs) tile = kTileAngles / pairs;
     if (tile < 1) tile = 1;
     // fewer tokens per CTA where there are few: two CTAs for every SM
     while (tile > 2 && a.batch * ((a.tokens + tile - 1) / tile) < 2 * kSms) tile /= 2;
@@ -158,12 +180,14 @@ extern "C" int ffcvb_rotary(const ffcvb_rotary_args *args, void *stream) {
             sizes |= (a.heads ? a.q_stride[k] | a.q_out_stride[k] : 0) | (a.kv_heads ? a.k_stride[k] | a.k_out_stride[k] : 0);
         if (a.heads) low |= reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.q_out);
         if (a.kv_heads) low |= reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.k_out);
-        const bool wide = (low & 15) == 0 && sizes % W == 0;
+        const bool wide = (low & 15) == 0 && sizes % W == 0, half_wide = (low & 7) == 0 && sizes % (W / 2) == 0;
         auto run = [&](auto kernel) {
             launch_early(kernel, (unsigned)ctas, kThreads, (size_t)tile * pairs * 2 * sizeof(float), static_cast<cudaStream_t>(stream), a, tile);
         };
         if (wide)
             run(a.interleaved ? rotary_kernel<T, W, true> : rotary_kernel<T, W, false>);
+        else if (half_wide)
+            run(a.interleaved ? rotary_kernel<T, W / 2, true> : rotary_kernel<T, W / 2, false>);
         else
             run(a.interleaved ? rotary_kernel<T, 1, true> : rotary_kernel<T, 1, false>);
     });

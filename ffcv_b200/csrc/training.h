@@ -95,6 +95,41 @@ template <typename T> struct Pack16 {
     __device__ __forceinline__ void load(const T *p) { raw = *reinterpret_cast<const uint4 *>(p); }
     __device__ __forceinline__ void store(T *p) const { *reinterpret_cast<uint4 *>(p) = raw; }
 };
+// Half as much: 8 bytes.
+template <typename T> struct Pack8 {
+    uint2 raw;
+    __device__ __forceinline__ void load(const T *p) { raw = *reinterpret_cast<const uint2 *>(p); }
+    __device__ __forceinline__ void store(T *p) const { *reinterpret_cast<uint2 *>(p) = raw; }
+};
+template <> struct Pack<float, 2> : Pack8<float> {
+    __device__ __forceinline__ void get(float (&v)[2]) const {
+        v[0] = __uint_as_float(raw.x);
+        v[1] = __uint_as_float(raw.y);
+    }
+    __device__ __forceinline__ void set(const float (&v)[2]) { raw = make_uint2(__float_as_uint(v[0]), __float_as_uint(v[1])); }
+};
+template <> struct Pack<__nv_bfloat16, 4> : Pack8<__nv_bfloat16> {
+    __device__ __forceinline__ void get(float (&v)[4]) const {
+        v[0] = __uint_as_float(raw.x << 16);
+        v[1] = __uint_as_float(raw.x & 0xffff0000u);
+        v[2] = __uint_as_float(raw.y << 16);
+        v[3] = __uint_as_float(raw.y & 0xffff0000u);
+    }
+    __device__ __forceinline__ void set(const float (&v)[4]) {
+        const __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]), b = __floats2bfloat162_rn(v[2], v[3]);
+        raw = make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
+    }
+};
+template <> struct Pack<__half, 4> : Pack8<__half> {
+    __device__ __forceinline__ void get(float (&v)[4]) const {
+        const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&raw.x)), b = __half22float2(*reinterpret_cast<const __half2 *>(&raw.y));
+        v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
+    }
+    __device__ __forceinline__ void set(const float (&v)[4]) {
+        const __half2 a = __floats2half2_rn(v[0], v[1]), b = __floats2half2_rn(v[2], v[3]);
+        raw = make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
+    }
+};
 template <> struct Pack<float, 4> : Pack16<float> {
     __device__ __forceinline__ void get(float (&v)[4]) const {
         v[0] = __uint_as_float(raw.x);

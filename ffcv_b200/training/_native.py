@@ -11,7 +11,7 @@ TYPES = {ch.float32: 0, ch.float16: 1, ch.bfloat16: 2}
 
 CROSS_ENTROPY = struct.Struct('=8Q6q8i2f')
 NORM_RESIDUAL = struct.Struct('=22Q8q6i2f')
-ROTARY = struct.Struct('=6Q19q6ifi')
+ROTARY = struct.Struct('=7Q19q6ifi')
 ADAMW = struct.Struct('=7Qq4id')
 ADAMW_GROUP = struct.Struct('=5d')
 ADAMW_BLOCK = 256

@@ -1,6 +1,7 @@
 """Rotary positions of queries and keys: of tokens in a row, or of an image's patches by row and column."""
 import math
 
+import numpy as np
 import torch as ch
 
 from . import _native as N
@@ -77,8 +78,10 @@ class RotaryPositions(ch.nn.Module):
             keep = ((original_length * f / (2 * math.pi) - 1) / (32 - 1)).clamp(0, 1)
             f = f * ((1 - keep) / factor + keep)
             self.amplitude = 0.1 * math.log(factor) + 1 if factor > 1 else 1.0
-        # turns per unit of position, in 64 bits whatever type the module is cast to
-        self._turns = {ch.device('cpu'): (f / (2 * math.pi)).repeat(axes)}
+        # turns per unit of position, in 64 bits whatever type the module is cast to: as floats, and in units of 2^-64 of a turn
+        turns = (f / (2 * math.pi)).repeat(axes)
+        steps = np.array([round(math.fmod(t, 1.0) * 2 ** 64) & (2 ** 64 - 1) for t in turns.tolist()], np.uint64)
+        self._turns = {ch.device('cpu'): ch.stack([turns, ch.from_numpy(steps.view(np.float64))])}
 
     def extra_repr(self):
         return f'head_dim={self.head_dim}, rotary_dim={self.rotary_dim}, layout={self.layout!r}, axes={self.axes}'
@@ -136,9 +139,9 @@ class RotaryPositions(ch.nn.Module):
             kv_heads = k.shape[2]
             kb, kt, kh, _ = k.stride()
             kob, kot, koh, _ = k_out.stride()
-        index = q.get_device()
+        index, turns = q.get_device(), self._turns_on(q.device).data_ptr()
         args = N.ROTARY.pack(
-            q.data_ptr(), N.ptr(k), q_out.data_ptr(), N.ptr(k_out), where.data_ptr(), self._turns_on(q.device).data_ptr(),
+            q.data_ptr(), N.ptr(k), q_out.data_ptr(), N.ptr(k_out), where.data_ptr(), turns, turns + 4 * self.rotary_dim,
             batch, tokens, heads, kv_heads, self.head_dim, self.rotary_dim, stride, qb, qt, qh, kb, kt, kh, qob, qot, qoh, kob, kot, koh,
             index, N.TYPES[q.dtype], where.dtype == ch.float32, self.axes, self.layout == 'interleaved', transpose, self.amplitude, 0)
         N.check(N.lib.ffcvb_rotary(args, N.raw_stream(index)))

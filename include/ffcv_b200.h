@@ -381,6 +381,7 @@ typedef struct {
     void *q_out, *k_out;
     const void *positions;  /* int64 or float [batch, tokens, axes], contiguous but for the batch stride (may be 0) */
     const double *turns;    /* [rotary_dim / 2], per unit of position */
+    const uint64_t *steps;  /* the same in units of 2^-64 of a turn, whole turns left out */
     int64_t batch, tokens, heads, kv_heads, head_dim, rotary_dim, positions_stride;
     int64_t q_stride[3], k_stride[3], q_out_stride[3], k_out_stride[3]; /* batch, token, head */
     int32_t device, type, positions_float, axes, interleaved, transpose;
