@@ -1,12 +1,14 @@
 // Cross entropy against labels, mixed labels or probabilities, with its gradient (sm_100a).
 //
 // With T the target's probabilities, S their sum and lse = log sum exp x, a row's loss is S * lse - sum T x and
-// its gradient S * exp(x - lse) - T.  A warp takes a row of up to 1024 logits, a CTA one of up to 56 KB, a cluster a longer one.  Every
+// its gradient S * exp(x - lse) - T.  Some lanes of a warp take a row of up to 8 KB, a CTA one of up to 56 KB, a cluster a longer one.  Every
 // thread copies its part of the row into shared memory, in places of its own; a pass over it keeps the largest logit so far and the
 // sum of exponentials relative to that (in 32 bits), which are joined over the row's threads; a second pass makes the gradient.  So
 // the row crosses HBM once each way, and several CTAs per SM load, compute and store at different times.
 #include "training.h"
 #include "two.h"
+
+#include <type_traits>
 
 namespace ffcvb {
 
@@ -89,20 +91,20 @@ struct Found {
         dot += d;
         mass += m;
     }
-    // joins those of groups of LANES lanes; `more`: dot and mass too
-    template <int LANES> __device__ __forceinline__ void join_lanes(bool more) {
+    // joins those of groups of LANES lanes, in each of which all are in `mask`; `more`: dot and mass too
+    template <int LANES> __device__ __forceinline__ void join_lanes(bool more, uint32_t mask) {
         float most = top;
 #pragma unroll
-        for (int o = LANES / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+        for (int o = LANES / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(mask, most, o));
         sum *= exp_of(top - most);
         top = most;
 #pragma unroll
-        for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(mask, sum, o);
         if (!more) return;
 #pragma unroll
-        for (int o = LANES / 2; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+        for (int o = LANES / 2; o > 0; o >>= 1) dot += __shfl_xor_sync(mask, dot, o);
 #pragma unroll
-        for (int o = LANES / 2; o > 0; o >>= 1) mass += __shfl_xor_sync(0xffffffffu, mass, o);
+        for (int o = LANES / 2; o > 0; o >>= 1) mass += __shfl_xor_sync(mask, mass, o);
     }
     template <int N> __device__ __forceinline__ void add(const float (&v)[N]) {
         float most = fmaxf(top, v[0]);
@@ -133,11 +135,12 @@ struct Deal {
 };
 
 // A row's packs of 16 bytes are dealt out to its threads in turn; the few logits before and behind them (all, where logits and
-// gradient lie differently to 16-byte boundaries) are taken one by one.  WARP: a row per warp, four warps per CTA; else a row per
-// CTA or cluster.  STAGED: the packs go through shared memory; else they are read where they are needed.
-template <typename T, bool STAGED, bool SOFT, bool WARP>
-__global__ void __launch_bounds__(WARP ? 128 : 256)
+// gradient lie differently to 16-byte boundaries) are taken one by one.  LANES: as many lanes of a warp (2 to 32) have a row, in CTAs of
+// four warps; 0: a row per CTA or cluster.  STAGED: the packs go through shared memory; else they are read where they are needed.
+template <typename T, bool STAGED, bool SOFT, int LANES>
+__global__ void __launch_bounds__(LANES ? 128 : 256)
 rows_kernel(const __grid_constant__ ffcvb_cross_entropy_args a, const Deal deal) {
+    constexpr bool WARP = LANES > 0;
     constexpr int N = kWide<T>, BATCH = STAGED ? 1 : 4; // packs that a thread has on their way
     __shared__ float4 s_part[8];
     __shared__ float4 s_there[8]; // from the cluster's CTAs
@@ -151,8 +154,9 @@ rows_kernel(const __grid_constant__ ffcvb_cross_entropy_args a, const Deal deal)
         asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
         if (ranks > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); // (this one has begun)
     }
-    const int thread = WARP ? threadIdx.x & 31 : threadIdx.x, threads = WARP ? 32 : blockDim.x;
-    const long long row = WARP ? blockIdx.x * 4ll + (threadIdx.x >> 5) : blockIdx.x / ranks;
+    const int thread = WARP ? threadIdx.x & (LANES - 1) : threadIdx.x, threads = WARP ? LANES : blockDim.x;
+    const long long row = WARP ? blockIdx.x * (128ll / (WARP ? LANES : 1)) + threadIdx.x / (WARP ? LANES : 1) : blockIdx.x / ranks;
+    const uint32_t mask = !WARP || LANES == 32 ? 0xffffffffu : ((1u << (LANES & 31)) - 1) << (threadIdx.x & 31 & -LANES); // lanes of the row
     if (WARP && row >= a.rows) return;
     const int classes = (int)a.classes;
     const T *x = static_cast<const T *>(a.logits) + row * a.logits_stride;
@@ -163,7 +167,7 @@ rows_kernel(const __grid_constant__ ffcvb_cross_entropy_args a, const Deal deal)
     const int packs = (classes - before) / N, singles = classes - packs * N;
     const int first = (int)rank * deal.part, count = max(0, min(packs - first, deal.part));
     const T *x0 = x + before + (long long)first * N;
-    const uint32_t mine = (uint32_t)__cvta_generic_to_shared(s_row + (WARP ? (threadIdx.x >> 5) * deal.part : 0) + thread);
+    const uint32_t mine = (uint32_t)__cvta_generic_to_shared(s_row + (WARP ? threadIdx.x / (WARP ? LANES : 1) * deal.part : 0) + thread);
     if (STAGED) {
         uint32_t to = mine;
         for (int k = thread; k < count; k += threads, to += threads * 16) copy16(to, x0 + (long long)k * N);
@@ -249,14 +253,14 @@ rows_kernel(const __grid_constant__ ffcvb_cross_entropy_args a, const Deal deal)
         if (STAGED) asm volatile("cp.async.wait_group 0;" ::: "memory");
         each_pack(take);
         const bool more = SOFT || p.flat > 0.0f;
-        f.join_lanes<32>(more);
+        f.join_lanes<WARP ? LANES : 32>(more, mask);
         if (!WARP) {
             const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
             if (lane == 0) s_part[threadIdx.x >> 5] = make_float4(f.top, f.sum, f.dot, f.mass);
             __syncthreads();
             const float4 other = (lane & 7) < warps ? s_part[lane & 7] : make_float4(kLowest, 0.0f, 0.0f, 0.0f); // (at most eight)
             f = Found{other.x, other.y, other.z, other.w};
-            f.join_lanes<8>(more);
+            f.join_lanes<8>(more, mask);
             if (ranks > 1) {
                 asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); // all have begun
                 if (threadIdx.x < ranks) {
@@ -287,7 +291,8 @@ rows_kernel(const __grid_constant__ ffcvb_cross_entropy_args a, const Deal deal)
                 probabilities<1>(t, a, soft_row + c, false);
                 mass += sure * t[0] + p.flat;
             }
-            mass = warp_sum(mass);
+#pragma unroll
+            for (int o = WARP ? LANES / 2 : 16; o > 0; o >>= 1) mass += __shfl_xor_sync(mask, mass, o);
             if (!WARP) {
                 const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
                 if (lane == 0) s_part[threadIdx.x >> 5].x = mass;
@@ -384,9 +389,12 @@ mean_kernel(const float *__restrict__ row_loss, long long rows, const float *cou
     }
 }
 
-constexpr long long kPartBytes = 56 * 1024; // of a row in a CTA's shared memory: four CTAs per SM
-constexpr long long kWarpClasses = 1024;    // of a row that a warp takes
-
+// Bytes of a row in a CTA's shared memory, of which an SM then has four or more, and at most, where eight CTAs have a row: 512 rows of 130000
+// logits in 32 bits 115 us, read twice 120; 1024 of 130001 in 16 bits 119 as eight parts, 126 as four.
+constexpr long long kPartBytes = 56 * 1024, kMostPartBytes = 72 * 1024;
+// Bytes of a row that a warp takes at most; a lane then has 16 packs.  (16384 rows of 2000 logits in 16 bits 36 us, 49 by CTAs; 8192 of 3500
+// 30 and 33.)
+constexpr long long kWarpBytes = 8192;
 template <typename T>
 void launch_rows(const ffcvb_cross_entropy_args &a, cudaStream_t stream) {
     constexpr int W = 16 / (int)sizeof(T);
@@ -412,22 +420,34 @@ void launch_rows(const ffcvb_cross_entropy_args &a, cudaStream_t stream) {
         }
         cudaLaunchKernelEx(&how, kernel, a, deal);
     };
-    if (a.classes <= kWarpClasses) {
+    if (a.classes * (long long)sizeof(T) <= kWarpBytes) {
+        // lanes of a row: one for every two packs, or for every two logits where there are no packs
+        const long long pieces = packs ? packs : a.classes;
+        const int lanes = pieces <= 4 ? 2 : pieces <= 16 ? 8 : 32;
         deal.part = (int)packs;
-        how.gridDim = dim3((unsigned)((a.rows + 3) / 4));
+        how.gridDim = dim3((unsigned)((a.rows * lanes + 127) / 128));
         how.blockDim = dim3(128);
-        how.dynamicSmemBytes = both ? 4 * packs * 16 : 0;
-        if (both)
-            run(soft ? rows_kernel<T, true, true, true> : rows_kernel<T, true, false, true>);
+        how.dynamicSmemBytes = both ? 128 / lanes * packs * 16 : 0;
+        auto by_lanes = [&](auto n) {
+            constexpr int L = decltype(n)::value;
+            if (both)
+                run(soft ? rows_kernel<T, true, true, L> : rows_kernel<T, true, false, L>);
+            else
+                run(soft ? rows_kernel<T, false, true, L> : rows_kernel<T, false, false, L>);
+        };
+        if (lanes == 2)
+            by_lanes(std::integral_constant<int, 2>{});
+        else if (lanes == 8)
+            by_lanes(std::integral_constant<int, 8>{});
         else
-            run(soft ? rows_kernel<T, false, true, true> : rows_kernel<T, false, false, true>);
+            by_lanes(std::integral_constant<int, 32>{});
         return;
     }
     // CTAs per row: until a part fits, and until there are two CTAs per SM (with few rows) of parts that are worth it
     int ctas = 1;
     while (ctas < 8 && ((both && (packs + ctas - 1) / ctas * 16 > kPartBytes) || (a.rows * ctas <= kSms && packs > 2048 * ctas))) ctas *= 2;
     deal.part = (int)((packs + ctas - 1) / ctas);
-    const bool staged = both && deal.part * 16ll <= kPartBytes; // (else the second pass reads what the caches still have)
+    const bool staged = both && deal.part * 16ll <= kMostPartBytes; // (else the second pass reads what the caches still have)
     const int threads = (deal.part / 14 + 31) / 32 * 32; // (14 packs each: 131 us for 8192 x 21841 in bf16, 134 with 16, 136 with 18)
     how.gridDim = dim3((unsigned)(a.rows * ctas));
     how.blockDim = dim3(!deal.wide || threads > 256 ? 256 : threads < 64 ? 64 : threads);
@@ -439,9 +459,9 @@ void launch_rows(const ffcvb_cross_entropy_args &a, cudaStream_t stream) {
         cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
     }
     if (staged)
-        run(soft ? rows_kernel<T, true, true, false> : rows_kernel<T, true, false, false>);
+        run(soft ? rows_kernel<T, true, true, 0> : rows_kernel<T, true, false, 0>);
     else
-        run(soft ? rows_kernel<T, false, true, false> : rows_kernel<T, false, false, false>);
+        run(soft ? rows_kernel<T, false, true, 0> : rows_kernel<T, false, false, 0>);
 }
 
 } // namespace
