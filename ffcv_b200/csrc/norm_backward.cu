@@ -30,7 +30,7 @@ backward_kernel(const __grid_constant__ Args a, const Deal deal, const Partials 
     const bool per_sample = FORM == kGated || (FORM == kAny && a.gate_kind == FFCVB_GATE_SAMPLE);
     const bool per_token = FORM == kAny && a.gate_kind == FFCVB_GATE_TOKEN;
     const bool branch = FORM != kAny || a.h, normed = FORM != kAny || a.norm != FFCVB_NORM_NONE;
-    const bool given_dy = FORM != kAny || a.dy, given_dz = FORM != kAny || a.dz, want_dx = FORM != kAny || a.dx, want_dh = FORM != kAny || a.dh;
+    const bool given_dy = FORM != kAny || a.dy, given_dz = FORM != kAny || a.dz, want_dx = FORM != kAny || a.dx, want_dh = a.dh;
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(s_ring), window_size = window_bytes<T>(c.threads);
     const uint32_t slot_size = shape.streams * (PACKS ? (8 / N) * blockDim.x * 16 : window_size);
     const int slots = PACKS ? shape.ahead : shape.ahead + 1;

@@ -14,37 +14,40 @@ namespace norms {
 
 namespace {
 
-// Adds up partial rows: 32 columns per CTA, 32 runs of rows side by side (of 576 rows of 1024 columns 6 us; with 8 columns and 128
-// runs 9).
+// Adds up partial rows: 32 columns per CTA, 32 rows at a time side by side (of 576 rows of 1024 columns 6 us; with 8 columns and 128 rows
+// 9).  blockIdx.z: a run of the rows, whose sum goes to a partial row of its own.
 struct Sums {
     const float *from[kColumns];
     void *to[kColumns];
-    long long width, count, stride; // rows to add, from one to the next
+    long long width, count, stride, run, to_z; // rows to add, from one to the next; rows of a run, and from one run's sum to the next one's
     int type;
 };
 __global__ void __launch_bounds__(1024)
 add_up_kernel(const __grid_constant__ Sums s) {
     __shared__ float s_part[32][33];
     wait_for_previous();
-    const int lane = threadIdx.x & 31, run = threadIdx.x >> 5;
+    let_next_begin();
+    const int lane = threadIdx.x & 31, beside = threadIdx.x >> 5;
     const long long c = blockIdx.x * 32ll + lane;
     const float *from = s.from[blockIdx.y];
+    const long long begin = blockIdx.z * s.run, end = begin + s.run < s.count ? begin + s.run : s.count;
     float v = 0.0f;
     if (c < s.width) {
 #pragma unroll 8
-        for (long long r = run; r < s.count; r += 32) v += from[r * s.stride + c];
+        for (long long r = begin + beside; r < end; r += 32) v += from[r * s.stride + c];
     }
-    s_part[run][lane] = v;
+    s_part[beside][lane] = v;
     __syncthreads();
-    v = warp_sum(s_part[lane][run]); // column `run`
-    const long long mine = blockIdx.x * 32ll + run;
+    v = warp_sum(s_part[lane][beside]); // column `beside`
+    const long long mine = blockIdx.x * 32ll + beside;
     if (lane == 0 && mine < s.width) {
+        const long long at = blockIdx.z * s.to_z + mine;
         if (s.type == FFCVB_TYPE_F32)
-            static_cast<float *>(s.to[blockIdx.y])[mine] = v;
+            static_cast<float *>(s.to[blockIdx.y])[at] = v;
         else if (s.type == FFCVB_TYPE_F16)
-            static_cast<__half *>(s.to[blockIdx.y])[mine] = __float2half_rn(v);
+            static_cast<__half *>(s.to[blockIdx.y])[at] = __float2half_rn(v);
         else
-            static_cast<__nv_bfloat16 *>(s.to[blockIdx.y])[mine] = __float2bfloat16_rn(v);
+            static_cast<__nv_bfloat16 *>(s.to[blockIdx.y])[at] = __float2bfloat16_rn(v);
     }
 }
 
@@ -119,6 +122,10 @@ Deal deal_of(const Args &a) {
     const int per = d.shape.rows_per_cta();
     if (d.units < most) d.shape.rows_at_once = (int)((d.units + per - 1) / per * per);
     for (const void *p : {a.dweight, a.dbias, a.dpost_weight, a.dpost_bias, a.dscale}) d.columns += p != nullptr;
+    // narrow rows have many partial rows and few columns: two steps then, the first with a CTA for every SM (128000 rows of 64 forward and
+    // backward 33 us, 45 in one step; 394 rows of 192 11 us, 10 in one)
+    const long long across = (a.width + 31) / 32 * d.columns, most_runs = across ? kSms / across : 0;
+    d.runs = most_runs >= 4 && d.shape.rows_at_once >= 1024 ? (int)(most_runs < d.shape.rows_at_once / 128 ? most_runs : d.shape.rows_at_once / 128) : 1;
     return d;
 }
 
@@ -172,7 +179,7 @@ int ffcvb_norm_residual(const ffcvb_norm_residual_args *args, void *stream) {
 int64_t ffcvb_norm_residual_workspace(const ffcvb_norm_residual_args *args) {
     if (!args || args->rows < 0 || args->width < 1 || (args->gate_kind == FFCVB_GATE_SAMPLE && args->tokens < 1)) return 0;
     const Deal d = deal_of(*args);
-    return ((int64_t)d.shape.rows_at_once * d.columns + (args->gate_kind == FFCVB_GATE_SAMPLE && d.splits > 1 ? d.units : 0)) * args->width * 4 + 16;
+    return (((int64_t)d.shape.rows_at_once + d.runs) * d.columns + (args->gate_kind == FFCVB_GATE_SAMPLE && d.splits > 1 ? d.units : 0)) * args->width * 4 + 16;
 }
 
 int ffcvb_norm_residual_backward(const ffcvb_norm_residual_args *args, void *stream) {
@@ -182,21 +189,39 @@ int ffcvb_norm_residual_backward(const ffcvb_norm_residual_args *args, void *str
     if (!here.ok()) return training_fail(FFCVB_E_NODEVICE, "ffcvb_norm_residual_backward: no device %d", a.device);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const Deal d = deal_of(a);
-    Partials part{static_cast<float *>(a.workspace), static_cast<float *>(a.workspace) + (long long)d.shape.rows_at_once * d.columns * a.width};
+    float *const room = static_cast<float *>(a.workspace);
+    const long long row = d.columns * a.width;
+    Partials part{room, room + d.shape.rows_at_once * row, room + (d.shape.rows_at_once + d.runs) * row};
     if (a.rows > 0) launch_backward(a, d, part, wide_rows(a), st);
-    Sums s{};
-    int n = 0;
-    for (void *p : {a.dweight, a.dbias, a.dpost_weight, a.dpost_bias, a.dscale})
-        if (p) {
-            s.from[n] = part.columns + n * a.width;
-            s.to[n++] = p;
+    if (d.columns) {
+        Sums s{};
+        int n = 0;
+        const bool twice = d.runs > 1 && a.rows > 0;
+        for (void *p : {a.dweight, a.dbias, a.dpost_weight, a.dpost_bias, a.dscale})
+            if (p) {
+                s.from[n] = part.columns + n * a.width;
+                s.to[n] = twice ? part.runs + n * a.width : p;
+                n++;
+            }
+        s.width = a.width;
+        s.count = a.rows > 0 ? d.shape.rows_at_once : 0;
+        s.stride = s.to_z = row;
+        s.run = twice ? (s.count + d.runs - 1) / d.runs : s.count;
+        s.type = twice ? FFCVB_TYPE_F32 : a.param_type;
+        const unsigned across = (unsigned)((a.width + 31) / 32);
+        launch_early(add_up_kernel, dim3(across, n, twice ? d.runs : 1), 1024, 0, st, s);
+        if (twice) {
+            n = 0;
+            for (void *p : {a.dweight, a.dbias, a.dpost_weight, a.dpost_bias, a.dscale})
+                if (p) {
+                    s.from[n] = part.runs + n * a.width;
+                    s.to[n++] = p;
+                }
+            s.count = s.run = d.runs;
+            s.type = a.param_type;
+            launch_early(add_up_kernel, dim3(across, n), 1024, 0, st, s);
         }
-    s.width = a.width;
-    s.count = a.rows > 0 ? d.shape.rows_at_once : 0;
-    s.stride = d.columns * a.width;
-    s.type = a.param_type;
-    const unsigned across = (unsigned)((a.width + 31) / 32);
-    if (n) launch_early(add_up_kernel, dim3(across, n), 1024, 0, st, s);
+    }
     if (a.dgate && a.gate_kind == FFCVB_GATE_SAMPLE && d.splits > 1 && a.rows > 0) // (then there are fewer samples than CTAs, or few splits)
         with_type(a.type, [&](auto zero) {
             using T = decltype(zero);

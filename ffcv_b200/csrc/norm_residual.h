@@ -323,19 +323,21 @@ struct Deal {
     Shape shape;
     long long samples, tokens, splits, units;
     int columns; // column sums of each cluster: weight, bias, post_weight, post_bias, scale
+    int runs;    // that their partial rows are added up in first, or 1
 };
-// Partial rows: [rows_at_once][columns][width] of the column sums, then [units][width] of the gate's with more than one split.
+// Partial rows: [rows_at_once][columns][width] of the column sums; [runs][columns][width] where those are added up in two steps; [units][width]
+// of the gate's with more than one split.
 struct Partials {
-    float *columns, *gate;
+    float *columns, *runs, *gate;
 };
 
 constexpr int kColumns = 5;
 
 // What is known of a call when its kernel is compiled: nothing; or that there are a branch, a norm behind it and (backward) gradients of both
-// results, and all streams' gradients wanted, with no gate or one per sample.
+// results, and that the stream's is wanted, with no gate or one per sample.
 enum Form { kAny, kPlain, kGated };
 inline Form form_of(const Args &a, bool backward) {
-    if (!a.h || a.norm == FFCVB_NORM_NONE || a.gate_kind == FFCVB_GATE_TOKEN || (backward && (!a.dy || !a.dz || !a.dx || !a.dh))) return kAny;
+    if (!a.h || a.norm == FFCVB_NORM_NONE || a.gate_kind == FFCVB_GATE_TOKEN || (backward && (!a.dy || !a.dz || !a.dx))) return kAny;
     return a.gate_kind == FFCVB_GATE_SAMPLE ? kGated : kPlain;
 }
 
