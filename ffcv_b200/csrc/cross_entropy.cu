@@ -196,28 +196,45 @@ rows_kernel(const __grid_constant__ ffcvb_cross_entropy_args a, const Deal deal)
         for (int k = 0; k < 2; k++)
             if (p.weight[k] != 0.0f) picked += p.weight[k] * to_float(x[p.label[k]]);
     }
-    // Calls f(values, class of the first) for this thread's packs, of which BATCH are on their way at a time.
+    // Calls f(values, class of the first) for this thread's packs: as many turns as all threads have, BATCH at a time, then what is left.
+    const int turns = count / threads;
     auto each_pack = [&](auto &&f) {
         uint32_t at = mine;
-        for (int k = thread; k < count; k += BATCH * threads, at += BATCH * threads * 16) {
+        const T *from = x0 + (long long)thread * N;
+        int c = before + (first + thread) * N;
+        const int step = threads * N;
+        auto load = [&](Pack<T, N> &pack, int i) {
+            if constexpr (STAGED) {
+                uint4 &r = pack.raw;
+                asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(at + i * threads * 16) : "memory");
+            } else {
+                pack.load(from + (long long)i * step);
+            }
+        };
+        auto work = [&](const Pack<T, N> &pack, int i) {
+            float v[N];
+            pack.get(v);
+            f(v, c + i * step);
+        };
+        int k = 0;
+        for (; k + BATCH <= turns; k += BATCH) {
             Pack<T, N> pack[BATCH];
 #pragma unroll
-            for (int i = 0; i < BATCH; i++)
-                if (k + i * threads < count) {
-                    if constexpr (STAGED) {
-                        uint4 &r = pack[i].raw;
-                        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(at + i * threads * 16) : "memory");
-                    } else {
-                        pack[i].load(x0 + (long long)(k + i * threads) * N);
-                    }
-                }
+            for (int i = 0; i < BATCH; i++) load(pack[i], i);
 #pragma unroll
-            for (int i = 0; i < BATCH; i++)
-                if (k + i * threads < count) {
-                    float v[N];
-                    pack[i].get(v);
-                    f(v, before + (first + k + i * threads) * N);
-                }
+            for (int i = 0; i < BATCH; i++) work(pack[i], i);
+            at += BATCH * threads * 16;
+            from += (long long)BATCH * step;
+            c += BATCH * step;
+        }
+        for (; k <= turns; k++) {
+            if (k == turns && turns * threads + thread >= count) break;
+            Pack<T, N> pack;
+            load(pack, 0);
+            work(pack, 0);
+            at += threads * 16;
+            from += step;
+            c += step;
         }
     };
     auto each_single = [&](auto &&f) {
