@@ -129,7 +129,7 @@ Deal deal_of(const Args &a) {
     return d;
 }
 
-int check(const Args *args, bool backward) {
+int check(const Args *args, bool backward, const void *workspace) {
     const char *name = backward ? "ffcvb_norm_residual_backward" : "ffcvb_norm_residual";
     if (!args) return training_fail(FFCVB_E_ARG, "%s: no arguments", name);
     const Args &a = *args;
@@ -146,7 +146,7 @@ int check(const Args *args, bool backward) {
         return training_fail(FFCVB_E_ARG, "%s: bad argument", name);
     if (!backward && a.rows > 0 && ((a.norm != FFCVB_NORM_NONE && !a.z) || (a.h && !a.y)))
         return training_fail(FFCVB_E_ARG, "%s: no room for the results", name);
-    if (backward && ((a.rows > 0 && !a.stats) || !a.workspace)) return training_fail(FFCVB_E_ARG, "%s: no statistics or workspace", name);
+    if (backward && ((a.rows > 0 && !a.stats) || !workspace)) return training_fail(FFCVB_E_ARG, "%s: no statistics or workspace", name);
     return FFCVB_OK;
 }
 
@@ -162,7 +162,7 @@ using namespace ffcvb::norms;
 extern "C" {
 
 int ffcvb_norm_residual(const ffcvb_norm_residual_args *args, void *stream) {
-    if (const int rc = check(args, false)) return rc;
+    if (const int rc = check(args, false, nullptr)) return rc;
     const Args &a = *args;
     if (a.rows == 0) return FFCVB_OK;
     OnDevice here(a.device);
@@ -177,19 +177,19 @@ int ffcvb_norm_residual(const ffcvb_norm_residual_args *args, void *stream) {
 }
 
 int64_t ffcvb_norm_residual_workspace(const ffcvb_norm_residual_args *args) {
-    if (!args || args->rows < 0 || args->width < 1 || (args->gate_kind == FFCVB_GATE_SAMPLE && args->tokens < 1)) return 0;
+    if (!args || args->rows < 0 || args->width < 1 || args->width > FFCVB_NORM_MAX_WIDTH || (args->gate_kind == FFCVB_GATE_SAMPLE && args->tokens < 1)) return 0;
     const Deal d = deal_of(*args);
     return (((int64_t)d.shape.rows_at_once + d.runs) * d.columns + (args->gate_kind == FFCVB_GATE_SAMPLE && d.splits > 1 ? d.units : 0)) * args->width * 4 + 16;
 }
 
-int ffcvb_norm_residual_backward(const ffcvb_norm_residual_args *args, void *stream) {
-    if (const int rc = check(args, true)) return rc;
+int ffcvb_norm_residual_backward(const ffcvb_norm_residual_args *args, void *workspace, void *stream) {
+    if (const int rc = check(args, true, workspace)) return rc;
     const Args &a = *args;
     OnDevice here(a.device);
     if (!here.ok()) return training_fail(FFCVB_E_NODEVICE, "ffcvb_norm_residual_backward: no device %d", a.device);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const Deal d = deal_of(a);
-    float *const room = static_cast<float *>(a.workspace);
+    float *const room = static_cast<float *>(workspace);
     const long long row = d.columns * a.width;
     Partials part{room, room + d.shape.rows_at_once * row, room + (d.shape.rows_at_once + d.runs) * row};
     if (a.rows > 0) launch_backward(a, d, part, wide_rows(a), st);

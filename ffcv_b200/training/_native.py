@@ -10,7 +10,7 @@ from ..libffcv import lib
 TYPES = {ch.float32: 0, ch.float16: 1, ch.bfloat16: 2}
 
 CROSS_ENTROPY = struct.Struct('=8Q6q8i2f')
-NORM_RESIDUAL = struct.Struct('=22Q8q6i2f')
+NORM_RESIDUAL = struct.Struct('=21Q8q6i2f')
 ROTARY = struct.Struct('=7Q19q6ifi')
 ADAMW = struct.Struct('=7Qq4id')
 ADAMW_GROUP = struct.Struct('=5d')
@@ -22,6 +22,7 @@ lib.ffcvb_training_error.restype = c_char_p
 for _name in ('ffcvb_cross_entropy', 'ffcvb_norm_residual', 'ffcvb_norm_residual_backward', 'ffcvb_rotary'):
     getattr(lib, _name).argtypes = [c_char_p, c_void_p]
     getattr(lib, _name).restype = c_int
+lib.ffcvb_norm_residual_backward.argtypes = [c_char_p, c_void_p, c_void_p]
 lib.ffcvb_norm_residual_workspace.argtypes = [c_char_p]
 lib.ffcvb_norm_residual_workspace.restype = c_int64
 lib.ffcvb_adamw_layout.argtypes = [c_int32, c_void_p, c_void_p, c_void_p]

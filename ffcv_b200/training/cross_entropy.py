@@ -50,19 +50,17 @@ class _Call:
         self.logits = logits if logits.stride(1) == 1 else logits.contiguous()
         self.target, self.ignore, self.mean, self.smoothing = target, ignore_index, reduction == 'mean', float(smoothing)
 
-    # loss: a value per sample, and one more for their mean or sum
-    def run(self, grad=None, loss=None, row_loss=None, stats=None, upstream=None, per_row=False, from_stats=False, scale=1.0):
-        x, t = self.logits, self.target
-        counted = ch.empty(1, device=x.device) if self.ignore is not None and self.mean else None
+    def run(self, grad, loss, one, stats=None, upstream=None, per_row=False, from_stats=False, scale=1.0):
+        """loss: a value per sample, and behind them, with `one`, room for their mean or sum."""
+        x, t, ignore = self.logits, self.target, self.ignore
+        rows, classes = x.shape
+        counted = ch.empty(1, dtype=ch.float32, device=x.device) if ignore is not None and self.mean else None
+        index, losses = x.get_device(), 0 if loss is None else loss.data_ptr()
         args = N.CROSS_ENTROPY.pack(
-            x.data_ptr(), t.data_ptr(), N.ptr(upstream), N.ptr(grad), 0 if loss is None else loss.data_ptr() + 4 * x.shape[0], N.ptr(row_loss), N.ptr(stats), N.ptr(counted),
-            x.shape[0], x.shape[1], x.stride(0), t.stride(0), x.shape[1], -1 if self.ignore is None else self.ignore,
-            x.get_device(), self.type, self.kind, self.target_type, self.ignore is not None, self.mean, per_row, from_stats,
-            self.smoothing, scale)
-        N.check(N.lib.ffcvb_cross_entropy(args, N.stream_of(x)))
-
-    def new_grad(self):
-        return N.new_like(self.logits)
+            x.data_ptr(), t.data_ptr(), N.ptr(upstream), N.ptr(grad), losses + 4 * rows if one else 0, losses, N.ptr(stats), N.ptr(counted),
+            rows, classes, x.stride(0), t.stride(0), classes, -1 if ignore is None else ignore,
+            index, self.type, self.kind, self.target_type, ignore is not None, self.mean, per_row, from_stats, self.smoothing, scale)
+        N.check(N.lib.ffcvb_cross_entropy(args, N.raw_stream(index)))
 
 
 def cross_entropy_with_grad(logits, labels=None, *, mixed=None, soft=None, label_smoothing=0.0, ignore_index=None,
@@ -93,9 +91,8 @@ def cross_entropy_with_grad(logits, labels=None, *, mixed=None, soft=None, label
     """
     call = _Call(logits, labels, mixed, soft, label_smoothing, ignore_index, reduction)
     n = logits.shape[0]
-    loss = ch.empty(n + 1, device=logits.device)  # a value per sample, and their mean or sum
-    grad = call.new_grad()
-    call.run(grad=grad, loss=None if reduction == 'none' else loss, row_loss=loss, scale=grad_scale)
+    loss, grad = ch.empty(n + 1, dtype=ch.float32, device=logits.device), N.new_like(call.logits)
+    call.run(grad, loss, reduction != 'none', scale=grad_scale)
     return loss[:n] if reduction == 'none' else loss[n], grad
 
 
@@ -103,8 +100,8 @@ class _CrossEntropy(ch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, call, reduction):
         n = logits.shape[0]
-        loss, stats = ch.empty(n + 1, device=logits.device), ch.empty((n, 2), device=logits.device)
-        call.run(loss=None if reduction == 'none' else loss, row_loss=loss, stats=stats)
+        loss, stats = (ch.empty(k, dtype=ch.float32, device=logits.device) for k in (n + 1, 2 * n))
+        call.run(None, loss, reduction != 'none', stats)
         ctx.per_row = reduction == 'none'
         ctx.save_for_backward(call.logits, call.target, stats)
         call.logits = call.target = None  # (autograd keeps them, and sees to it that nobody changes them)
@@ -116,9 +113,9 @@ class _CrossEntropy(ch.autograd.Function):
     def backward(ctx, upstream):
         call = ctx.call
         call.logits, call.target, stats = ctx.saved_tensors
-        grad = call.new_grad()
+        grad = N.new_like(call.logits)
         upstream = upstream.float().contiguous()
-        call.run(grad=grad, stats=stats, upstream=upstream, per_row=ctx.per_row, from_stats=True)
+        call.run(grad, None, False, stats, upstream, ctx.per_row, True)
         call.logits = call.target = None
         return grad, None, None
 

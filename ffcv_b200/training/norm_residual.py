@@ -7,6 +7,7 @@ from . import _native as N
 _NORMS = {None: 0, 'layer': 1, 'rms': 2}
 _NO_GATE, _SAMPLE, _TOKEN = range(3)
 _PARAMS = ('weight', 'bias', 'post_weight', 'post_bias', 'scale')
+_NAMES = ('x', 'h', 'weight', 'bias', 'post_weight', 'post_bias', 'gate', 'scale')
 
 
 def _gate_kind(x, gate):
@@ -94,21 +95,22 @@ class _Call:
         """Whether the branch is added as it is, so that its gradient is the stream's."""
         return self.post_norm == 0 and self.gate is None and self.scale is None and self.number == 1.0
 
-    def pack(self, stats, y=0, z=0, dy=0, dz=0, dx=0, dh=0, dgate=0, params=(0,) * 5, workspace=0, dy_stride=0, dz_stride=0):
+    def pack(self, stats, *places):
+        """places: y, z; dy, dz; dx, dh, dgate; the parameters' gradients; dy's and dz's strides."""
         return N.NORM_RESIDUAL.pack(
-            *self.given, stats.data_ptr(), y, z, dy, dz, dx, dh, dgate, *params, workspace, self.rows, self.width, self.tokens,
-            *self.strides, dy_stride, dz_stride, self.index, self.type, self.param_type, self.norm, self.post_norm, self.gate_kind,
-            self.eps, self.number)
+            *self.given, stats.data_ptr(), *places[:12], self.rows, self.width, self.tokens, *self.strides, *places[12:], self.index,
+            self.type, self.param_type, self.norm, self.post_norm, self.gate_kind, self.eps, self.number)
 
     def forward(self):
         x = self.x
         y, z = None if self.h is None else N.new_like(x), N.new_like(x) if self.norm else None
-        stats = ch.empty(4 * self.rows, device=x.device)
-        N.check(N.lib.ffcvb_norm_residual(self.pack(stats, N.ptr(y), N.ptr(z)), N.raw_stream(self.index)))
+        stats = ch.empty(4 * self.rows, dtype=ch.float32, device=x.device)
+        N.check(N.lib.ffcvb_norm_residual(self.pack(stats, N.ptr(y), N.ptr(z), 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0), N.raw_stream(self.index)))
         return y, z, stats
 
     def backward(self, stats, dy, dz, wanted):
-        """The gradients named in `wanted`, which holds only what the call was given."""
+        """The gradients of x, h, weight, bias, post_weight, post_bias, gate and scale, of which `wanted` says which ones (only such as
+        the call was given), else None."""
         x = self.x
         for name, g in (('dy', dy), ('dz', dz)):
             if g is not None and (N.require(g, name, x) != self.type or g.shape != x.shape):
@@ -119,25 +121,19 @@ class _Call:
             dz = ch.zeros_like(x, memory_format=ch.contiguous_format)
         dy_at, dy_stride = self.rows_of(dy)
         dz_at, dz_stride = self.rows_of(dz)
+        of_x, of_h, of_weight, of_bias, of_post_weight, of_post_bias, of_gate, of_scale = wanted
         plain = self.plain()
-        out = {}
-        if 'x' in wanted or (plain and 'h' in wanted):
-            out['x'] = N.new_like(x)
-        if 'h' in wanted:
-            out['h'] = out['x'] if plain else N.new_like(x)
-        params = [0] * 5
-        for k, name in enumerate(_PARAMS):
-            if name in wanted:
-                out[name] = g = ch.empty(self.width, dtype=self.param_dtype, device=x.device)
-                params[k] = g.data_ptr()
-        if 'gate' in wanted:
-            out['gate'] = N.new_like(self.gate)
-        how = dict(dy=dy_at, dz=dz_at, dx=N.ptr(out.get('x')), dh=0 if plain else N.ptr(out.get('h')), dgate=N.ptr(out.get('gate')),
-                   params=params, dy_stride=dy_stride, dz_stride=dz_stride)
-        room = N.lib.ffcvb_norm_residual_workspace(self.pack(stats, **how))
-        workspace = ch.empty(room, dtype=ch.uint8, device=x.device)
-        N.check(N.lib.ffcvb_norm_residual_backward(self.pack(stats, workspace=workspace.data_ptr(), **how), N.raw_stream(self.index)))
-        return out
+        dx = N.new_like(x) if of_x or (plain and of_h) else None
+        dh = None if not of_h else dx if plain else N.new_like(x)
+        dgate = N.new_like(self.gate) if of_gate else None
+        new, device = ch.empty, x.device
+        params = [new(self.width, dtype=self.param_dtype, device=device) if of else None
+                  for of in (of_weight, of_bias, of_post_weight, of_post_bias, of_scale)]
+        ptr = N.ptr
+        args = self.pack(stats, 0, 0, dy_at, dz_at, ptr(dx), 0 if plain else ptr(dh), ptr(dgate), *map(ptr, params), dy_stride, dz_stride)
+        workspace = new(N.lib.ffcvb_norm_residual_workspace(args), dtype=ch.uint8, device=device)
+        N.check(N.lib.ffcvb_norm_residual_backward(args, workspace.data_ptr(), N.raw_stream(self.index)))
+        return dx if of_x else None, dh, *params[:4], dgate, params[4]
 
 
 def norm_residual_forward(x, h=None, *, norm='layer', weight=None, bias=None, post_norm=None, post_weight=None, post_bias=None,
@@ -152,13 +148,11 @@ def norm_residual_backward(dy, dz, x, h, stats, *, norm='layer', weight=None, bi
     """Gradients of all tensors that :func:`norm_residual_forward` was given, by their names, from those of y and z (None: 0).
     Where the branch is added as it is, the entries 'x' and 'h' are one tensor."""
     call = _Call(x, h, norm, weight, bias, post_norm, post_weight, post_bias, gate, scale, eps)
-    given = dict(x=x, h=h, weight=weight, bias=bias, post_weight=post_weight, post_bias=post_bias, gate=gate, scale=call.scale)
-    return call.backward(stats, dy, dz, {name for name, t in given.items() if t is not None})
+    grads = call.backward(stats, dy, dz, [t is not None for t in (x, h, weight, bias, post_weight, post_bias, gate, call.scale)])
+    return {name: g for name, g in zip(_NAMES, grads) if g is not None}
 
 
 class _NormResidual(ch.autograd.Function):
-    NAMES = ('x', 'h', 'weight', 'bias', 'post_weight', 'post_bias', 'gate', 'scale')
-
     @staticmethod
     def forward(ctx, how, x, h, weight, bias, post_weight, post_bias, gate, scale):
         norm, post_norm, number, eps = how
@@ -177,9 +171,7 @@ class _NormResidual(ch.autograd.Function):
         if dy is None and dz is None:
             return (None,) * 9
         call = _Call(x, h, norm, weight, bias, post_norm, post_weight, post_bias, gate, scale if scale is not None else number, eps)
-        wanted = {name for name, needed in zip(_NormResidual.NAMES, ctx.needs_input_grad[1:]) if needed}
-        grads = call.backward(stats, dy, dz, wanted)
-        return (None,) + tuple(grads[name] if name in wanted else None for name in _NormResidual.NAMES)
+        return (None,) + tuple(call.backward(stats, dy, dz, ctx.needs_input_grad[1:]))
 
 
 def norm_residual(x, h=None, *, norm='layer', weight=None, bias=None, post_norm=None, post_weight=None, post_bias=None,

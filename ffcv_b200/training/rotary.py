@@ -87,9 +87,10 @@ class RotaryPositions(ch.nn.Module):
         return f'head_dim={self.head_dim}, rotary_dim={self.rotary_dim}, layout={self.layout!r}, axes={self.axes}'
 
     def _turns_on(self, device):
-        if device not in self._turns:
-            self._turns[device] = self._turns[ch.device('cpu')].to(device)
-        return self._turns[device]
+        turns = self._turns.get(device)
+        if turns is None:
+            turns = self._turns[device] = self._turns[ch.device('cpu')].to(device)
+        return turns
 
     def _where(self, q, positions):
         """Positions as the kernel reads them, and the stride from one sequence to the next."""

@@ -361,13 +361,13 @@ typedef struct {
     const void *dy, *dz;    /* gradients of y and z, or NULL: 0; backward only, like the following */
     void *dx, *dh, *dgate;  /* contiguous, or NULL: not wanted */
     void *dweight, *dbias, *dpost_weight, *dpost_bias, *dscale; /* of param_type, or NULL */
-    void *workspace;        /* ffcvb_norm_residual_workspace() bytes, 16-byte aligned; backward only */
     int64_t rows, width, tokens, x_stride, h_stride, gate_stride, dy_stride, dz_stride;
     int32_t device, type, param_type, norm, post_norm, gate_kind;
     float eps, number;
 } ffcvb_norm_residual_args;
 int ffcvb_norm_residual(const ffcvb_norm_residual_args *args, void *stream);
-int ffcvb_norm_residual_backward(const ffcvb_norm_residual_args *args, void *stream);
+/* workspace: ffcvb_norm_residual_workspace(args) bytes, 16-byte aligned. */
+int ffcvb_norm_residual_backward(const ffcvb_norm_residual_args *args, void *workspace, void *stream);
 int64_t ffcvb_norm_residual_workspace(const ffcvb_norm_residual_args *args);
 
 /* Rotary positions: pair i of a head's first rotary_dim values, (a, b), becomes

@@ -43,7 +43,7 @@ def test_bad_arguments_come_back_as_codes():
     """No exception and no abort leaves a C entry, whatever the host's arguments are; nothing is launched."""
     from ffcv_b200.training import _native as N
     lib = N.lib
-    for call in (lib.ffcvb_cross_entropy, lib.ffcvb_norm_residual, lib.ffcvb_norm_residual_backward, lib.ffcvb_rotary):
+    for call in (lib.ffcvb_cross_entropy, lib.ffcvb_norm_residual, lib.ffcvb_rotary, lambda args, stream: lib.ffcvb_norm_residual_backward(args, None, stream)):
         assert call(None, None) == -2
         assert b'no arguments' in lib.ffcvb_training_error()
     assert lib.ffcvb_norm_residual_workspace(None) == 0
@@ -54,13 +54,16 @@ def test_bad_arguments_come_back_as_codes():
                 loss(smoothing=math.nan)):
         assert lib.ffcvb_cross_entropy(bad, None) == -2
     norm = lambda rows=2, width=8, norm=1, post=0, gate=0, x=16, h=16, gate_at=0, tokens=1, type_=0, y=16: N.NORM_RESIDUAL.pack(  # noqa: E731
-        x, h, gate_at, 0, 0, 0, 0, 0, 16, y, 16, *([0] * 5), *([0] * 5), 0, rows, width, tokens, width, width, width, width, width, 0, type_, 0, norm, post, gate,
+        x, h, gate_at, 0, 0, 0, 0, 0, 16, y, 16, *([0] * 5), *([0] * 5), rows, width, tokens, width, width, width, width, width, 0, type_, 0, norm, post, gate,
         1e-6, 1.0)
     for bad in (norm(rows=-1), norm(width=0), norm(norm=3), norm(post=-1), norm(gate=3), norm(x=0), norm(gate=1, gate_at=0), norm(rows=3, gate=1, gate_at=16, tokens=2),
                 norm(type_=7), norm(y=0), norm(h=0, norm=0)):
         assert lib.ffcvb_norm_residual(bad, None) == -2
     assert lib.ffcvb_norm_residual(norm(width=16385), None) == -6
-    assert lib.ffcvb_norm_residual_backward(norm(), None) == -2  # no workspace
+    assert lib.ffcvb_norm_residual_backward(norm(), None, None) == -2  # no workspace
+    for odd in (norm(width=1 << 40), norm(width=0), norm(rows=-3), norm(gate=1, tokens=0)):
+        assert lib.ffcvb_norm_residual_workspace(odd) == 0
+    assert lib.ffcvb_norm_residual_workspace(norm(rows=0)) >= 0
     assert lib.ffcvb_norm_residual(norm(rows=0), None) == 0
     rotary = lambda head_dim=8, rotary_dim=8, axes=1, heads=2, q=16, tokens=3: N.ROTARY.pack(  # noqa: E731
         q, 0, 16, 0, 16, 16, 16, 1, tokens, heads, 0, head_dim, rotary_dim, 0, *([0] * 12), 0, 0, 0, axes, 0, 0, 1.0, 0)
@@ -73,7 +76,7 @@ def test_bad_arguments_come_back_as_codes():
 def test_structures_are_as_in_the_header():
     """The packed formats have no padding: their sizes are those of the C structures (members of 8 bytes first)."""
     from ffcv_b200.training import _native as N
-    for fmt, size in ((N.CROSS_ENTROPY, 8 * 8 + 6 * 8 + 8 * 4 + 2 * 4), (N.NORM_RESIDUAL, 22 * 8 + 8 * 8 + 6 * 4 + 2 * 4), (N.ROTARY, 7 * 8 + 19 * 8 + 8 * 4),
+    for fmt, size in ((N.CROSS_ENTROPY, 8 * 8 + 6 * 8 + 8 * 4 + 2 * 4), (N.NORM_RESIDUAL, 21 * 8 + 8 * 8 + 6 * 4 + 2 * 4), (N.ROTARY, 7 * 8 + 19 * 8 + 8 * 4),
                       (N.ADAMW, 8 * 8 + 4 * 4 + 8), (N.ADAMW_GROUP, 40)):
         assert fmt.size == size and size % 8 == 0
 
