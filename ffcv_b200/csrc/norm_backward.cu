@@ -28,7 +28,7 @@ backward_kernel(const __grid_constant__ Args a, const Deal deal, const Partials 
     const Columns<N, LANES> c(a.width, rank);
     const float over = 1.0f / (float)a.width;
     const bool per_sample = FORM == kGated || (FORM == kAny && a.gate_kind == FFCVB_GATE_SAMPLE);
-    const bool per_token = FORM == kAny && a.gate_kind == FFCVB_GATE_TOKEN;
+    const bool per_token = FORM == kToken || (FORM == kAny && a.gate_kind == FFCVB_GATE_TOKEN);
     const bool branch = FORM != kAny || a.h, normed = FORM != kAny || a.norm != FFCVB_NORM_NONE;
     const bool given_dy = FORM != kAny || a.dy, given_dz = FORM != kAny || a.dz, want_dx = FORM != kAny || a.dx, want_dh = a.dh;
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(s_ring), window_size = window_bytes<T>(c.threads);
@@ -287,22 +287,9 @@ void launch_backward(const Args &a, const Deal &d, const Partials &part, bool wi
     const size_t room = d.shape.ring + (size_t)d.shape.threads * ((post ? 64 : 0) + (a.gate_kind == FFCVB_GATE_SAMPLE ? 96 : 0));
     with_type(a.type, [&](auto zero) {
         using T = decltype(zero);
-        constexpr int W = 16 / (int)sizeof(T);
-        auto formed = [&](auto post_norm) {
-            constexpr bool P = decltype(post_norm)::value;
-            if (!wide)
-                sized<T, 1, P, kAny>(a, d, part, room, stream);
-            else if (form_of(a, true) == kPlain)
-                sized<T, W, P, kPlain>(a, d, part, room, stream);
-            else if (form_of(a, true) == kGated)
-                sized<T, W, P, kGated>(a, d, part, room, stream);
-            else
-                sized<T, W, P, kAny>(a, d, part, room, stream);
-        };
-        if (post)
-            formed(Int<1>{});
-        else
-            formed(Int<0>{});
+        with_form<T>(wide, post, form_of(a, true), [&](auto n, auto p, auto f) {
+            sized<T, decltype(n)::value, (bool)decltype(p)::value, decltype(f)::value>(a, d, part, room, stream);
+        });
     });
 }
 

@@ -18,7 +18,7 @@ forward_kernel(const __grid_constant__ Args a, const Shape shape) {
     int rank;
     const int cluster = first_row<LANES>(shape, rank);
     const bool branch = FORM != kAny || a.h, normed = FORM != kAny || a.norm != FFCVB_NORM_NONE;
-    const bool gated = FORM == kGated || (FORM == kAny && a.gate_kind != FFCVB_GATE_NONE);
+    const bool gated = FORM == kGated || FORM == kToken || (FORM == kAny && a.gate_kind != FFCVB_GATE_NONE);
     const bool per_sample = FORM == kGated || (FORM == kAny && a.gate_kind == FFCVB_GATE_SAMPLE);
     RowSum<LANES> sum{s_sum, shape.ctas_per_row};
     sum.begin();
@@ -186,22 +186,9 @@ void launch_forward(const Args &a, const Shape &shape, bool wide, cudaStream_t s
     const size_t room = shape.ring;
     with_type(a.type, [&](auto zero) {
         using T = decltype(zero);
-        constexpr int W = 16 / (int)sizeof(T);
-        auto formed = [&](auto post_norm) {
-            constexpr bool P = decltype(post_norm)::value;
-            if (!wide)
-                sized<T, 1, P, kAny>(a, shape, room, stream);
-            else if (form_of(a, false) == kPlain)
-                sized<T, W, P, kPlain>(a, shape, room, stream);
-            else if (form_of(a, false) == kGated)
-                sized<T, W, P, kGated>(a, shape, room, stream);
-            else
-                sized<T, W, P, kAny>(a, shape, room, stream);
-        };
-        if (post)
-            formed(Int<1>{});
-        else
-            formed(Int<0>{});
+        with_form<T>(wide, post, form_of(a, false), [&](auto n, auto p, auto f) {
+            sized<T, decltype(n)::value, (bool)decltype(p)::value, decltype(f)::value>(a, shape, room, stream);
+        });
     });
 }
 

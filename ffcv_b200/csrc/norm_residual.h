@@ -334,11 +334,35 @@ struct Partials {
 constexpr int kColumns = 5;
 
 // What is known of a call when its kernel is compiled: nothing; or that there are a branch, a norm behind it and (backward) gradients of both
-// results, and that the stream's is wanted, with no gate or one per sample.
-enum Form { kAny, kPlain, kGated };
+// results, and that the stream's is wanted, with no gate, one per sample or one per token.  (256 x 197 rows of 768 bf16 values, plain:
+// 48 and 74 us; as any call 62 and 96.)
+enum Form { kAny, kPlain, kGated, kToken };
 inline Form form_of(const Args &a, bool backward) {
-    if (!a.h || a.norm == FFCVB_NORM_NONE || a.gate_kind == FFCVB_GATE_TOKEN || (backward && (!a.dy || !a.dz || !a.dx))) return kAny;
-    return a.gate_kind == FFCVB_GATE_SAMPLE ? kGated : kPlain;
+    if (!a.h || a.norm == FFCVB_NORM_NONE || (backward && (!a.dy || !a.dz || !a.dx))) return kAny;
+    return a.gate_kind == FFCVB_GATE_SAMPLE ? kGated : a.gate_kind == FFCVB_GATE_TOKEN ? kToken : kPlain;
+}
+template <Form F> using FormOf = Int<(int)F>;
+// f(packs of N, post, form): for single values the gated forms are as any call.
+template <typename T, typename F> void with_form(bool wide, bool post, Form form, F &&f) {
+    using Wide = Int<16 / (int)sizeof(T)>;
+    auto formed = [&](auto post_norm) {
+        if (!wide && form == kPlain)
+            f(Int<1>{}, post_norm, FormOf<kPlain>{});
+        else if (!wide)
+            f(Int<1>{}, post_norm, FormOf<kAny>{});
+        else if (form == kPlain)
+            f(Wide{}, post_norm, FormOf<kPlain>{});
+        else if (form == kGated)
+            f(Wide{}, post_norm, FormOf<kGated>{});
+        else if (form == kToken)
+            f(Wide{}, post_norm, FormOf<kToken>{});
+        else
+            f(Wide{}, post_norm, FormOf<kAny>{});
+    };
+    if (post)
+        formed(Int<1>{});
+    else
+        formed(Int<0>{});
 }
 
 template <typename Kernel, typename... More>
