@@ -402,7 +402,7 @@ mean_kernel(const float *__restrict__ row_loss, long long rows, const float *cou
         sum = s_sum[threadIdx.x];
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (threadIdx.x == 0) *loss = (float)(mean ? sum / (counted ? fmax((double)*counted, 1.0) : (double)rows) : sum);
+        if (threadIdx.x == 0) *loss = (float)(mean ? sum / fmax(counted ? (double)*counted : (double)rows, 1.0) : sum);
     }
 }
 

@@ -152,6 +152,7 @@ class AdamW(ch.optim.Optimizer):
                             N.TYPES[dtype], self.state_bits, n, self.max_grad_norm or 0.0)
         N.check(N.lib.ffcvb_adamw_step(args, *self._host, struct.pack(f'={n}Q', *grads_at), groups, len(self.param_groups), N.raw_stream(index)))
         del kept
+        ch.autograd.graph.increment_version(params)  # (a later backward pass that needs what they were says so)
         return loss
 
     def state_dict(self):

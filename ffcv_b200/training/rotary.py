@@ -124,6 +124,8 @@ class RotaryPositions(ch.nn.Module):
                 raise ValueError(f'k must be {q.dtype} {tuple(q.shape[:2])} + (heads, {self.head_dim}), not {k.dtype} {tuple(k.shape)}')
 
     def _run(self, q, k, where, stride, transpose, inplace):
+        if inplace and ch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+            raise ValueError('in place is for tensors without a gradient: autograd would not know of the change')
         if inplace and (q.stride(3) != 1 or (k is not None and k.stride(3) != 1)):
             raise ValueError('in place the values of a head must lie next to one another')
         if q.stride(3) != 1:

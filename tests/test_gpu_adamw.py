@@ -315,6 +315,19 @@ def test_groups_added_later_keep_the_state():
         assert loss == 7 and opt._steps.tolist() == [2, 2, 1]
 
 
+def test_autograd_sees_the_step():
+    """A backward pass that needs a weight as it was before the step says so."""
+    from ffcv_b200.training import AdamW
+    p = ch.nn.Parameter(ch.ones(8, device='cuda'))
+    opt = AdamW([p])
+    x = ch.ones(8, device='cuda', requires_grad=True)
+    y = (x * p).sum()
+    p.grad = ch.ones_like(p)
+    opt.step()
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        y.backward()
+
+
 def test_learns_in_mixed_precision():
     """Least squares: with either state the loss falls to a hundredth."""
     from ffcv_b200.training import AdamW

@@ -135,6 +135,7 @@ def test_nothing_counted_and_no_rows():
     assert float(loss) == 0.0 and not grad.any()
     loss, grad = cross_entropy_with_grad(x[:0], ch.zeros(0, dtype=ch.long, device='cuda'), reduction='sum')
     assert float(loss) == 0.0 and grad.shape == (0, 9)
+    assert float(cross_entropy_with_grad(x[:0], ch.zeros(0, dtype=ch.long, device='cuda'))[0]) == 0.0
     x.requires_grad_()
     cross_entropy(x, ch.full((5,), -1, device='cuda'), ignore_index=-1).backward()
     assert not x.grad.any()

@@ -168,3 +168,5 @@ def test_refusals():
         RotaryPositions(64, axes=2).rotate(q)
     with pytest.raises(ValueError):
         rotary.rotate(q.transpose(2, 3).contiguous().transpose(2, 3), inplace=True)
+    with pytest.raises(ValueError):
+        rotary.rotate(q.clone().requires_grad_(), inplace=True)
