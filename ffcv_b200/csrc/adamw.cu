@@ -1,6 +1,6 @@
 // One AdamW step over many tensors (sm_100a), moments in 32 or in 8 bits.
 //
-// The tensors are cut into chunks, one CTA each; a table in device memory says which tensor a chunk belongs to, the
+// The tensors are cut into chunks; a table in device memory says which tensor a chunk belongs to, the
 // gradients' addresses, which change from step to step, travel as arguments of the kernel.  Moments and masters lie
 // in flat arrays in units of 256 values, a tensor's first value beginning a unit; a warp takes a unit.
 //
@@ -10,7 +10,11 @@
 // 1 - beta2 of its difference to g^2 per step, far less than half the distance of two e5m2 numbers, and would never
 // leave its place otherwise; and scales are powers of two, because a value that has not changed is then on the new
 // grid too and is not rounded again, which would add up to a noise of several times the value over 1 / (1 - beta2) steps.
-// Second moments above zero stay above zero.
+// A second moment above zero keeps the smallest code at least, except below 2^-128.
+//
+// Reading and writing bounds it: 28 bytes per value with moments in 32 bits, with 8-bit moments 16, masters of 16-bit weights included.
+// 409 M bf16 weights with 8-bit moments: 981 us (1002 at the rate of a copy); 101 M values in 32 bits with clipping, which reads the
+// gradients twice: 477 us (492 at that rate, had the caches kept nothing).
 #include "training.h"
 #include "two.h"
 
@@ -23,6 +27,7 @@ namespace {
 
 constexpr int kUnit = FFCVB_ADAMW_BLOCK;
 constexpr int kThreads = 256;
+constexpr int kPlaces = 4; // CTAs of an SM in a step with 8-bit moments
 constexpr int kSets = 16; // different (group, steps) of one launch
 
 struct Tensor {
@@ -33,13 +38,14 @@ struct Chunk {
     int32_t tensor, index;
 };
 
-// Values of a chunk: a unit for each warp, or four where there is a chunk of them for every place of a CTA (8 per SM): a long chunk saves
-// set-up (101 M values in 32 bits: 423 us, 447 with short ones), a short one latency (52 000 values: 8.8 us with long ones, 5.2).
+// Values of a chunk, of which the squares' kernel gives one to a CTA: with a chunk for every second SM four loads of 16 bytes a thread are
+// in flight at once instead of one (25 M values, squares and step: 124 us, 136 with short ones; 850 000: 8.8, 9.8); with fewer, short ones
+// bring more SMs in (500 000: 8.7 us, 9.1 with long ones; 51 000: 7.2, 8.0).
 constexpr long long kShort = 8 * kUnit, kLong = 32 * kUnit;
 long long chunk_size(int32_t n, const int64_t *numel) {
     int64_t all = 0;
     for (int32_t i = 0; i < n; i++) all += numel[i];
-    return all < kSms * 8 * kLong ? kShort : kLong;
+    return all < kSms / 2 * kLong ? kShort : kLong;
 }
 long long chunks_of(int64_t numel, long long chunk) { return (numel + chunk - 1) / chunk; }
 
@@ -79,25 +85,36 @@ __device__ __forceinline__ void four(Two *v, float4 f) {
 }
 __device__ __forceinline__ float4 four(const Two *v) { return make_float4(v[0].lo(), v[0].hi(), v[1].lo(), v[1].hi()); }
 
-// Four values from place `at` of a tensor of n; 0 beyond its end.  WHOLE: none is, and the tensor lies on boundaries of four values.
-template <bool WHOLE, typename T>
-__device__ __forceinline__ float4 load4(const T *p, long long at, long long n) {
-    if constexpr (WHOLE && sizeof(T) == 4) {
-        return *reinterpret_cast<const float4 *>(p + at);
-    } else if constexpr (WHOLE) {
-        const uint2 w = *reinterpret_cast<const uint2 *>(p + at);
+// Four values as they lie in memory.
+template <typename T> struct Words {
+    uint2 v;
+    __device__ __forceinline__ float4 get() const {
         float2 lo, hi;
         if constexpr (std::is_same<T, __half>::value) {
-            lo = __half22float2(*reinterpret_cast<const __half2 *>(&w.x));
-            hi = __half22float2(*reinterpret_cast<const __half2 *>(&w.y));
+            lo = __half22float2(*reinterpret_cast<const __half2 *>(&v.x));
+            hi = __half22float2(*reinterpret_cast<const __half2 *>(&v.y));
         } else {
-            lo = make_float2(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u));
-            hi = make_float2(__uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
+            lo = make_float2(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u));
+            hi = make_float2(__uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u));
         }
         return make_float4(lo.x, lo.y, hi.x, hi.y);
+    }
+};
+template <> struct Words<float> {
+    float4 v;
+    __device__ __forceinline__ float4 get() const { return v; }
+};
+// Those from place `at` of a tensor of n; 0 beyond its end.  WHOLE: none is, and the tensor lies on boundaries of four values.
+template <bool WHOLE, typename T>
+__device__ __forceinline__ Words<T> load4(const T *p, long long at, long long n) {
+    if constexpr (WHOLE) {
+        return *reinterpret_cast<const Words<T> *>(p + at);
+    } else if constexpr (sizeof(T) == 4) {
+        return {make_float4(at < n ? p[at] : 0.0f, at + 1 < n ? p[at + 1] : 0.0f, at + 2 < n ? p[at + 2] : 0.0f, at + 3 < n ? p[at + 3] : 0.0f)};
     } else {
-        return make_float4(at < n ? to_float(p[at]) : 0.0f, at + 1 < n ? to_float(p[at + 1]) : 0.0f,
-                           at + 2 < n ? to_float(p[at + 2]) : 0.0f, at + 3 < n ? to_float(p[at + 3]) : 0.0f);
+        const uint16_t *q = reinterpret_cast<const uint16_t *>(p);
+        const uint32_t v0 = at < n ? q[at] : 0, v1 = at + 1 < n ? q[at + 1] : 0, v2 = at + 2 < n ? q[at + 2] : 0, v3 = at + 3 < n ? q[at + 3] : 0;
+        return {make_uint2(v0 | v1 << 16, v2 | v3 << 16)};
     }
 }
 template <bool WHOLE, typename T>
@@ -151,27 +168,53 @@ __device__ __forceinline__ uint32_t top_bytes(const uint32_t *w) {
     return __byte_perm(__byte_perm(w[0], w[1], 0x0073), __byte_perm(w[2], w[3], 0x0073), 0x5410);
 }
 
-// One unit.  WHOLE: all of it inside a tensor on boundaries of four values.
+// What a lane reads of a unit: four neighbours in either half of it.  WHOLE: all of it inside a tensor on boundaries of four values.
+template <typename T, int BITS> struct Unit {
+    Words<T> g[2];
+    float4 w[2], m[BITS == 32 ? 2 : 1], v[BITS == 32 ? 2 : 1];
+    uint32_t mc[2], vc[2];
+    float2 scale;
+    template <bool WHOLE, typename Args>
+    __device__ __forceinline__ void load(const Args &a, const T *grad, const T *param, long long first, long long n, long long flat) {
+        const int lane = threadIdx.x & 31;
+        if (BITS == 8) scale = *reinterpret_cast<const float2 *>(a.scales + flat / kUnit * 2);
+#pragma unroll
+        for (int half = 0; half < 2; half++) {
+            const long long at = first + half * 128 + lane * 4, place = flat + half * 128 + lane * 4;
+            g[half] = load4<WHOLE>(grad, at, n);
+            if constexpr (sizeof(T) == 4)
+                w[half] = load4<WHOLE>(param, at, n).v;
+            else
+                w[half] = *reinterpret_cast<const float4 *>(a.master + place);
+            if constexpr (BITS == 32) {
+                m[half] = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.exp_avg) + place);
+                v[half] = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.exp_avg_sq) + place);
+            } else {
+                mc[half] = static_cast<const uint32_t *>(a.exp_avg)[place / 4];
+                vc[half] = static_cast<const uint32_t *>(a.exp_avg_sq)[place / 4];
+            }
+        }
+    }
+};
+
 template <typename T, int BITS, bool WHOLE, typename Args>
-__device__ __forceinline__ void step_unit(const Args &a, const Set &set, float clip, const T *grad, T *param, long long first, long long n, long long flat) {
+__device__ __forceinline__ void step_unit(const Args &a, const Unit<T, BITS> &unit, const Set &set, float clip, T *param, long long first, long long n, long long flat) {
     const int lane = threadIdx.x & 31;
     Two g[4], w[4], m[4], v[4];
     float *const exp_avg = static_cast<float *>(a.exp_avg), *const exp_avg_sq = static_cast<float *>(a.exp_avg_sq);
     uint32_t *const m_codes = static_cast<uint32_t *>(a.exp_avg), *const v_codes = static_cast<uint32_t *>(a.exp_avg_sq);
     uint32_t mc[2], vc[2];
-    float2 scale;
-    if (BITS == 8) scale = *reinterpret_cast<const float2 *>(a.scales + flat / kUnit * 2);
+    float2 scale = unit.scale;
 #pragma unroll
-    for (int half = 0; half < 2; half++) { // (a lane has four neighbours in either half of a unit)
-        const long long at = first + half * 128 + lane * 4, place = flat + half * 128 + lane * 4;
-        four(g + 2 * half, load4<WHOLE>(grad, at, n));
-        four(w + 2 * half, sizeof(T) == 4 ? load4<WHOLE>(param, at, n) : *reinterpret_cast<const float4 *>(a.master + place));
-        if (BITS == 32) {
-            four(m + 2 * half, *reinterpret_cast<const float4 *>(exp_avg + place));
-            four(v + 2 * half, *reinterpret_cast<const float4 *>(exp_avg_sq + place));
+    for (int half = 0; half < 2; half++) {
+        four(g + 2 * half, unit.g[half].get());
+        four(w + 2 * half, unit.w[half]);
+        if constexpr (BITS == 32) {
+            four(m + 2 * half, unit.m[half]);
+            four(v + 2 * half, unit.v[half]);
         } else {
-            mc[half] = m_codes[place / 4];
-            vc[half] = v_codes[place / 4];
+            mc[half] = unit.mc[half];
+            vc[half] = unit.vc[half];
         }
     }
     if (BITS == 8) {
@@ -243,12 +286,62 @@ __device__ __forceinline__ void step_unit(const Args &a, const Set &set, float c
     }
 }
 
-template <typename T, int BITS, int MOST>
-__global__ void __launch_bounds__(kThreads)
+// A whole unit on its way through a warp's part of shared memory.
+template <typename T> struct alignas(16) Staged {
+    T g[kUnit];
+    float w[kUnit];
+    uint32_t mc[kUnit / 4], vc[kUnit / 4];
+    float2 scale[2];
+    template <int BYTES>
+    static __device__ __forceinline__ void copy(void *to, const void *from) {
+        const uint32_t at = (uint32_t)__cvta_generic_to_shared(to);
+        if constexpr (BYTES == 16)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(from) : "memory");
+        else
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(at), "l"(from) : "memory");
+    }
+    template <typename Args>
+    __device__ __forceinline__ void begin(const Args &a, const T *grad, const T *param, long long first, long long flat) {
+        const int lane = threadIdx.x & 31, codes = (lane & 15) * 4;
+        const float *from;
+        if constexpr (sizeof(T) == 4)
+            from = param + first;
+        else
+            from = a.master + flat;
+#pragma unroll
+        for (int half = 0; half < 2; half++) {
+            const int at = half * 128 + lane * 4;
+            copy<4 * sizeof(T)>(g + at, grad + first + at);
+            copy<16>(w + at, from + at);
+        }
+        copy<16>((lane < 16 ? mc : vc) + codes, static_cast<const uint32_t *>(lane < 16 ? a.exp_avg : a.exp_avg_sq) + flat / 4 + codes);
+        if (lane == 0) copy<8>(scale, a.scales + flat / kUnit * 2);
+    }
+    __device__ __forceinline__ void read(Unit<T, 8> &u) const {
+        const int lane = threadIdx.x & 31;
+#pragma unroll
+        for (int half = 0; half < 2; half++) {
+            const int at = half * 128 + lane * 4;
+            u.g[half] = *reinterpret_cast<const Words<T> *>(g + at);
+            u.w[half] = *reinterpret_cast<const float4 *>(w + at);
+            u.mc[half] = mc[at / 4];
+            u.vc[half] = vc[at / 4];
+        }
+        u.scale = scale[0];
+    }
+};
+
+// STAGED: a CTA takes a whole chunk, with the next unit's copies under way while a warp works on one.  Otherwise it takes kShort values,
+// a warp a unit: in 32 bits, where the work is little, that keeps memory as busy (101 M bf16 values and their squares: 477 us).  With
+// 8-bit moments a warp that waits for each unit's loads leaves memory idle while it works: 409 M bf16 values take 981 us staged, 1143
+// without, 1114 with the next unit in registers, of which three CTAs fit instead of four.
+template <typename T, int BITS, int MOST, bool STAGED>
+__global__ void __launch_bounds__(kThreads, BITS == 8 ? kPlaces : 1)
 step_kernel(const __grid_constant__ Launch<MOST> a) {
     wait_for_previous();
     let_next_begin();
-    const Chunk chunk = a.chunks[blockIdx.x];
+    const unsigned parts = STAGED ? 1 : (unsigned)a.chunk / (unsigned)kShort;
+    const Chunk chunk = a.chunks[blockIdx.x / parts];
     const int local = chunk.tensor - a.first;
     const T *grad = static_cast<const T *>(a.grads[local]);
     if (!grad) return;
@@ -261,20 +354,49 @@ step_kernel(const __grid_constant__ Launch<MOST> a) {
     const Tensor tensor = a.tensors[local];
     const Set &set = a.sets[a.set[local]];
     T *param = reinterpret_cast<T *>(tensor.param);
+    const long long n = tensor.numel;
     const bool aligned = ((reinterpret_cast<uintptr_t>(grad) | reinterpret_cast<uintptr_t>(param)) & (4 * sizeof(T) - 1)) == 0;
-    for (int in_chunk = (threadIdx.x >> 5) * kUnit; in_chunk < a.chunk; in_chunk += kThreads / 32 * kUnit) {
-        const long long first = (long long)chunk.index * a.chunk + in_chunk; // in the tensor
-        if (first >= tensor.numel) break;
-        if (aligned && first + kUnit <= tensor.numel)
-            step_unit<T, BITS, true>(a, set, clip, grad, param, first, tensor.numel, tensor.start + first);
-        else
-            step_unit<T, BITS, false>(a, set, clip, grad, param, first, tensor.numel, tensor.start + first);
+    long long first = (long long)chunk.index * a.chunk + (blockIdx.x % parts) * kShort + (threadIdx.x >> 5) * kUnit; // in the tensor
+    Unit<T, BITS> unit;
+    if constexpr (STAGED) {
+        __shared__ Staged<T> s_staged[kThreads / 32][2];
+        Staged<T> *const mine = s_staged[threadIdx.x >> 5];
+        const long long end = min(n, (long long)(chunk.index + 1) * a.chunk);
+        auto whole = [&](long long at) { return aligned && at + kUnit <= end; };
+        auto begin = [&](int turn, long long at) {
+            if (whole(at)) mine[turn].begin(a, grad, param, at, tensor.start + at);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        begin(0, first);
+        for (int turn = 0; whole(first); first += kShort, turn ^= 1) {
+            __syncwarp(); // (all lanes have read what the next copies overwrite)
+            begin(turn ^ 1, first + kShort);
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
+            __syncwarp();
+            mine[turn].read(unit);
+            step_unit<T, BITS, true>(a, unit, set, clip, param, first, n, tensor.start + first);
+        }
+        for (; first < end; first += kShort) {
+            unit.template load<false>(a, grad, param, first, n, tensor.start + first);
+            step_unit<T, BITS, false>(a, unit, set, clip, param, first, n, tensor.start + first);
+        }
+    } else {
+        if (first >= n) return;
+        if (aligned && first + kUnit <= n) {
+            unit.template load<true>(a, grad, param, first, n, tensor.start + first);
+            step_unit<T, BITS, true>(a, unit, set, clip, param, first, n, tensor.start + first);
+        } else {
+            unit.template load<false>(a, grad, param, first, n, tensor.start + first);
+            step_unit<T, BITS, false>(a, unit, set, clip, param, first, n, tensor.start + first);
+        }
     }
 }
+// With 8-bit moments, where there is a long chunk for each place of a CTA: 6.5 M values take 21.5 us staged, 24.4 without; 1.1 M take
+// 10.3 and 5.8, as a CTA's four units are one after another.
+bool staged(int bits, long long values) { return bits == 8 && values >= kSms * kPlaces * kLong; }
 
 // The sum of squares of a chunk's gradients.  The last chunks come first: what the first ones leave in the caches the step begins with
-// (101 M values in 32 bits: squares and step together 505 us, 508 with the first chunks first; 500 and 494 without and with the caches'
-// default policy for all loads and stores instead of one for what is used once).
+// (101 M values in 32 bits: squares and step together 505 us, 508 with the first chunks first).
 template <typename T, int MOST>
 __global__ void __launch_bounds__(kThreads)
 squares_kernel(const __grid_constant__ Launch<MOST> a) {
@@ -292,14 +414,17 @@ squares_kernel(const __grid_constant__ Launch<MOST> a) {
         const long long first = (long long)chunk.index * a.chunk;
         constexpr int AT_ONCE = kLong / 4 / kThreads;
         if (aligned && first + a.chunk <= n && a.chunk == kLong) {
-            float4 g[AT_ONCE];
+            Words<T> w[AT_ONCE];
 #pragma unroll
-            for (int k = 0; k < AT_ONCE; k++) g[k] = load4<true>(grad, first + (k * kThreads + threadIdx.x) * 4, n);
+            for (int k = 0; k < AT_ONCE; k++) w[k] = load4<true>(grad, first + (k * kThreads + threadIdx.x) * 4, n);
 #pragma unroll
-            for (int k = 0; k < AT_ONCE; k++) sum += (g[k].x * g[k].x + g[k].y * g[k].y) + (g[k].z * g[k].z + g[k].w * g[k].w);
+            for (int k = 0; k < AT_ONCE; k++) {
+                const float4 g = w[k].get();
+                sum += (g.x * g.x + g.y * g.y) + (g.z * g.z + g.w * g.w);
+            }
         } else {
             for (int k = threadIdx.x; k < a.chunk / 4 && first + k * 4 < n; k += kThreads) {
-                const float4 g = load4<false>(grad, first + k * 4, n);
+                const float4 g = load4<false>(grad, first + k * 4, n).get();
                 sum += (g.x * g.x + g.y * g.y) + (g.z * g.z + g.w * g.w);
             }
         }
@@ -338,7 +463,7 @@ struct Tensors { // HOST
     const int64_t *steps;
     const int32_t *group_of;
     const ffcvb_adamw_group *groups;
-    long long chunks, chunk; // of all, and values of one
+    long long values, chunks, chunk; // of all, and values of one chunk
 };
 
 // Every launch takes as many tensors as its arguments have room for.
@@ -394,8 +519,9 @@ void launch_all(const ffcvb_adamw_args &args, const Tensors &t, bool squares, cu
         a.max_norm = (float)args.max_norm;
         a.partial = static_cast<float *>(args.workspace) + at;
         if (count > 0 && (any || squares)) {
-            auto step = args.bits == 8 ? step_kernel<T, 8, MOST> : step_kernel<T, 32, MOST>;
-            launch_early(squares ? squares_kernel<T, MOST> : step, (unsigned)count, kThreads, 0, st, a);
+            const bool long_ones = squares || staged(args.bits, t.values);
+            auto step = args.bits == 32 ? step_kernel<T, 32, MOST, false> : long_ones ? step_kernel<T, 8, MOST, true> : step_kernel<T, 8, MOST, false>;
+            launch_early(squares ? squares_kernel<T, MOST> : step, (unsigned)(long_ones ? count : count * (t.chunk / kShort)), kThreads, 0, st, a);
         }
         first += n;
         at += count;
@@ -447,12 +573,13 @@ int ffcvb_adamw_step(const ffcvb_adamw_args *args, const int64_t *numel, int64_t
         (a.bits == 8 && !a.scales) || (a.type != FFCVB_TYPE_F32 && (!a.master || (a.type != FFCVB_TYPE_F16 && a.type != FFCVB_TYPE_BF16))) ||
         (a.max_norm > 0.0 && (!a.norm || !a.workspace)))
         return training_fail(FFCVB_E_ARG, "ffcvb_adamw_step: bad argument");
-    Tensors t{numel, grads, steps, group_of, groups, 0, chunk_size(a.n_tensors, numel)};
+    Tensors t{numel, grads, steps, group_of, groups, 0, 0, chunk_size(a.n_tensors, numel)};
     for (int32_t i = 0; i < a.n_tensors; i++) {
         if (group_of[i] < 0 || group_of[i] >= n_groups) return training_fail(FFCVB_E_ARG, "ffcvb_adamw_step: tensor %d is in no group", i);
+        t.values += numel[i];
         t.chunks += chunks_of(numel[i], t.chunk);
     }
-    if (t.chunks > 0x7fffffff) return training_fail(FFCVB_E_LIMIT, "ffcvb_adamw_step: too many values");
+    if (t.chunks * (t.chunk / kShort) > 0x7fffffff) return training_fail(FFCVB_E_LIMIT, "ffcvb_adamw_step: too many values");
     OnDevice here(a.device);
     if (!here.ok()) return training_fail(FFCVB_E_NODEVICE, "ffcvb_adamw_step: no device %d", a.device);
     cudaStream_t st = static_cast<cudaStream_t>(stream);

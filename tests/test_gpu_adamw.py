@@ -197,6 +197,36 @@ def test_8_bit_moments(dtype):
             assert ch.equal(p.detach(), opt.state[p]['master'].to(dtype))
 
 
+@pytest.mark.parametrize('dtype', TYPES, ids=str)
+def test_8_bit_moments_of_many_values(dtype):
+    """As many as have their chunks worked on in turns, with tensors that end inside a turn, and a gradient at an odd place."""
+    from ffcv_b200.training import AdamW
+    shapes = [(1100, 2900), (7,), (1301, 1303), (8192,), (8193 + 255,), (2048 + 256,), (90001,), (6, 2048), (0,)]
+    assert sum(math.prod(s) for s in shapes) > 148 * 4 * 8192
+    params, gen = params_of(shapes, dtype, 6)
+    opt = AdamW(params, **HYPER, state_bits=8, seed=11, max_grad_norm=1e9)
+    b1, b2 = HYPER['betas']
+    plain = Eight(opt)
+    w = flat_of(opt, params, params).astype(np.float64)
+    for t in range(1, 4):
+        set_grads(params, gen, 10.0 ** -t)
+        params[6].grad = ch.randn(90002, generator=gen, device='cuda').to(dtype)[1:]
+        opt.step()
+        m, v = plain.step(flat_of(opt, params, [p.grad for p in params]), b1, b2, 11, t)
+        with np.errstate(invalid='ignore', divide='ignore'):
+            u = m.astype(np.float64) / (1 - b1 ** t) / (np.sqrt(v.astype(np.float64) / (1 - b2 ** t)) + HYPER['eps'])
+        w = w * (1 - HYPER['lr'] * HYPER['weight_decay']) - HYPER['lr'] * u
+        assert ch.equal(opt.exp_avg.view(ch.uint8).cpu(), plain.m.view(ch.uint8))
+        assert ch.equal(opt.exp_avg_sq.view(ch.uint8).cpu(), plain.v.view(ch.uint8))
+        assert ch.equal(opt.scales.cpu(), plain.scales)
+    masters = [opt.state[p]['master'] if 'master' in opt.state[p] else p for p in params]
+    got = flat_of(opt, params, masters)
+    assert np.all(np.abs(got - w) <= 3 * (2.0 ** -22 * np.abs(w) + 2.0 ** -18 * HYPER['lr'] * 10))
+    for p in params:
+        if 'master' in opt.state[p]:
+            assert ch.equal(p.detach(), opt.state[p]['master'].to(dtype))
+
+
 def test_8_bit_moments_follow_their_averages():
     """Thousands of steps of a constant gradient: the second moment comes to g^2, which it would not if values were rounded
     to the nearest, and a value's mean over many equal ones is right.  A step moves a value by up to (1 - b2) g^2 and rounding by a
