@@ -6,6 +6,10 @@
 // dx = t, the branch's gradient is du = t f, and the inner norm takes du on to dh by the same formula.  y is made
 // again from x and h, in 32 bits: its rounded copy would cost the weights' gradients their last digits.
 // Sums over columns of the gradient go through one partial row per CTA, added up in a fixed order by a second kernel.
+//
+// Reading and writing bounds it where rows are whole packs: 50432 bf16 rows of 768 with norm, branch and scale take 48 us
+// forward and 74 backward (47 and 71 at the rate of a copy), and 8 for the columns' sums.  With an inner norm and gates
+// (147520 rows of 1024) 218 and 310 us (184 and 276), where arithmetic and barriers between a row's sums show.
 #include "norm_residual.h"
 
 namespace ffcvb {
@@ -123,7 +127,7 @@ Deal deal_of(const Args &a) {
     if (d.units < most) d.shape.rows_at_once = (int)((d.units + per - 1) / per * per);
     for (const void *p : {a.dweight, a.dbias, a.dpost_weight, a.dpost_bias, a.dscale}) d.columns += p != nullptr;
     // narrow rows have many partial rows and few columns: two steps then, the first with a CTA for every SM (128000 rows of 64 forward and
-    // backward 33 us, 45 in one step; 394 rows of 192 11 us, 10 in one)
+    // backward 33 us, 47 in one step; 394 rows of 192 11 us, 10 in one)
     const long long across = (a.width + 31) / 32 * d.columns, most_runs = across ? kSms / across : 0;
     d.runs = most_runs >= 4 && d.shape.rows_at_once >= 1024 ? (int)(most_runs < d.shape.rows_at_once / 128 ? most_runs : d.shape.rows_at_once / 128) : 1;
     return d;
