@@ -4,6 +4,7 @@ import struct
 from ctypes import c_char_p, c_int, c_int32, c_int64, c_void_p
 
 import torch as ch
+from torch._C._dynamo.guards import TensorGuards
 
 from ..libffcv import lib
 
@@ -40,6 +41,12 @@ def check(rc):
 
 # The handle of a device's current stream, without the object around it that ch.cuda.current_stream makes (2 us a call).
 raw_stream = ch._C._cuda_getCurrentRawStream
+
+
+def layouts(tensors):
+    """What tensors are, whatever their values: ``layouts(a).check(*b)`` says whether sizes, strides, types and devices of b are those of a, of
+    148 tensors in 15 us (their strides, sizes and types as Python sees them take 40)."""
+    return TensorGuards(*tensors, dynamic_dims_sizes=None, dynamic_dims_strides=None)
 
 
 def stream_of(tensor):

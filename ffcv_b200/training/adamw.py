@@ -31,7 +31,9 @@ class AdamW(ch.optim.Optimizer):
     ``exp_avg_sq``, ``scales`` (8 bits) and ``master`` (16-bit parameters), of which ``state[p]`` has views; every
     parameter begins a block of 256 values, the rest of its last block is zero.  A parameter without a gradient is left alone,
     and its step is not counted.  The kernels read the current learning rates from the groups and take gradients and
-    parameters wherever they lie at the time of the step.
+    parameters wherever they lie at the time of the step.  Where the order of a parameter's values in memory has changed
+    (``model.to(memory_format=...)``) its state is brought into that order, moments in 8 bits rounded once more; a parameter of
+    another shape or type, on another device or with gaps is refused.
     """
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, state_bits=32, max_grad_norm=None,
@@ -43,6 +45,7 @@ class AdamW(ch.optim.Optimizer):
         self.state_bits, self.max_grad_norm, self.seed = state_bits, max_grad_norm, int(seed)
         self.exp_avg = self.exp_avg_sq = self.scales = self.master = self.grad_norm = None
         self._params, self._numel, self._steps = [], None, np.zeros(0, np.int64)
+        self._layouts = self._grad_layouts = None
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
 
     @staticmethod
@@ -57,6 +60,7 @@ class AdamW(ch.optim.Optimizer):
         group = self.param_groups[-1]
         try:
             self._check_group(group)
+            self._check_params()
             for p in group['params']:
                 N.require(p, 'parameter')
                 like = self._params[0] if self._params else group['params'][0]
@@ -69,12 +73,23 @@ class AdamW(ch.optim.Optimizer):
             raise
         self._lay_out()
 
+    def _check_params(self):
+        """Refuses parameters that are no longer what their state was made for."""
+        for p in self._params:
+            was = self.state[p]['exp_avg'].shape
+            if p.dtype != self._dtype or p.device != self.exp_avg.device or p.layout != ch.strided:
+                raise TypeError(f'a parameter is {p.dtype} {p.layout} on {p.device} now; the state was made for {self._dtype} on {self.exp_avg.device}')
+            if p.shape != was:
+                raise ValueError(f'a parameter of shape {tuple(was)} is of shape {tuple(p.shape)} now: its state belongs to the values it had')
+            if not _dense(p):
+                raise ValueError('parameters must lie together in memory, without gaps or overlaps')
+
     def _lay_out(self):
-        """Flat state for all parameters of all groups; what there was keeps its values."""
-        old = {id(p): (start, step) for p, start, step in zip(self._params, self._start if self._params else (), self._steps)}
-        before = self.exp_avg, self.exp_avg_sq, self.scales, self.master
+        """Flat state for all parameters of all groups, as they lie now; what there was keeps its values."""
+        old = {p: (self.state[p], int(step)) for p, step in zip(self._params, self._steps)}
         self._params = [p for group in self.param_groups for p in group['params']]
         n, device, dtype = len(self._params), self._params[0].device, self._params[0].dtype
+        self._dtype = dtype
         self._numel = np.array([p.numel() for p in self._params], np.int64)
         self._start, sizes = np.zeros(n, np.int64), np.zeros(2, np.int64)
         total = N.lib.ffcvb_adamw_layout(n, self._numel.ctypes.data, self._start.ctypes.data, sizes.ctypes.data)
@@ -87,27 +102,38 @@ class AdamW(ch.optim.Optimizer):
         self._table = ch.empty(int(sizes[0]), dtype=ch.uint8, device=device)
         self._workspace = ch.empty(max(16, int(sizes[1])), dtype=ch.uint8, device=device) if self.max_grad_norm else None
         self.grad_norm = ch.zeros((), device=device) if self.max_grad_norm else None
-        self._table_size, self._at, self._contiguous = int(sizes[0]), None, False
+        self._table_size, self._at = int(sizes[0]), None
+        self._layouts, self._grad_layouts = N.layouts(self._params), None
         self._group_of = np.repeat(np.arange(len(self.param_groups), dtype=np.int32), [len(g['params']) for g in self.param_groups])
         steps = np.zeros(n, np.int64)
         for i, p in enumerate(self._params):
-            a, b = int(self._start[i]), int(self._start[i]) + -(-p.numel() // _BLOCK) * _BLOCK
-            if id(p) in old:
-                was, steps[i] = old[id(p)]
-                for now, then in zip((self.exp_avg, self.exp_avg_sq, self.master), before[:2] + before[3:]):
-                    if now is not None:
-                        _bytes(now)[a * now.itemsize:b * now.itemsize].copy_(_bytes(then)[was * now.itemsize:(was + b - a) * now.itemsize])
-                if eight:
-                    self.scales[a // _BLOCK:b // _BLOCK].copy_(before[2][was // _BLOCK:(was + b - a) // _BLOCK])
-            elif self.master is not None:
-                self._of(self.master, i).copy_(p.detach())
-            entry = self.state[p] = dict(step=int(steps[i]), exp_avg=self._of(self.exp_avg, i), exp_avg_sq=self._of(self.exp_avg_sq, i))
+            entry = dict(step=0, exp_avg=self._of(self.exp_avg, i), exp_avg_sq=self._of(self.exp_avg_sq, i))
             if eight:
-                entry['scales'] = self.scales[a // _BLOCK:b // _BLOCK]
+                first = int(self._start[i]) // _BLOCK
+                entry['scales'] = self.scales[first:first - (-p.numel() // _BLOCK)]
             if self.master is not None:
                 entry['master'] = self._of(self.master, i)
+            if p in old:
+                was, steps[i] = old[p]
+                entry['step'] = int(steps[i])
+                self._take(entry, was)
+            elif self.master is not None:
+                entry['master'].copy_(p.detach())
+            self.state[p] = entry
         self._steps = steps
         self._host = self._numel.ctypes.data, self._steps.ctypes.data, self._group_of.ctypes.data
+
+    def _take(self, own, was):
+        """A parameter's state from another of the same shape, whatever order in memory either is in."""
+        if 'master' in own:
+            own['master'].copy_(was['master'])
+        if self.state_bits == 8 and _order(own['exp_avg']) != _order(was['exp_avg']):
+            for k, name in enumerate(('exp_avg', 'exp_avg_sq')):
+                _in_eight(own[name], own['scales'][:, k], _from_eight(was[name], was['scales'][:, k]))
+            return
+        for name in ('exp_avg', 'exp_avg_sq', 'scales'):
+            if name in own:
+                own[name].copy_(was[name])
 
     def _of(self, flat, i):
         """Parameter i's part of a flat tensor, in the parameter's shape and order in memory."""
@@ -118,6 +144,8 @@ class AdamW(ch.optim.Optimizer):
         """A gradient that is laid out as its parameter."""
         if g.layout != ch.strided or g.dtype != p.dtype or g.device != p.device:
             raise TypeError(f'gradients must be dense, of the parameters\' type and on their GPU, not {g.dtype} {g.layout} on {g.device}')
+        if g.shape != p.shape:
+            raise ValueError(f'a parameter of shape {tuple(p.shape)} has a gradient of shape {tuple(g.shape)}')
         return g if g.stride() == p.stride() else ch.empty_like(p).copy_(g)
 
     @ch.no_grad()
@@ -127,22 +155,27 @@ class AdamW(ch.optim.Optimizer):
             with ch.enable_grad():
                 loss = closure()
         params, n = self._params, len(self._params)
-        dtype, index = params[0].dtype, params[0].get_device()
+        if not self._layouts.check(*params):
+            self._check_params()
+            if any(_order(p) != _order(self.state[p]['exp_avg']) for p in params):
+                self._lay_out()
+            self._layouts = N.layouts(params)
+        dtype, index = self._dtype, params[0].get_device()
         at = [p.data_ptr() for p in params]
         # addresses of gradients, 0 without one
         grads, kept = [p.grad for p in params], None
-        if at == self._at and self._contiguous and all(
-                g is not None and g.dtype is dtype and g.is_contiguous() for g in grads):
+        if self._grad_layouts is not None and self._grad_layouts.check(*grads):
             grads_at = [g.data_ptr() for g in grads]
         else:
             kept = [None if g is None else self._as_parameter(p, g) for p, g in zip(params, grads)]
             grads_at = [N.ptr(g) for g in kept]
+            self._grad_layouts = N.layouts(kept) if all(g is not None and g is own for g, own in zip(kept, grads)) else None
         if at != self._at:  # the first step, or parameters that have moved
             host = np.empty(max(1, self._table_size), np.uint8)
             where = np.array(at, np.uint64)
             N.check(N.lib.ffcvb_adamw_table(n, self._numel.ctypes.data, where.ctypes.data, host.ctypes.data))
             self._table.copy_(ch.from_numpy(host[:self._table_size]))
-            self._at, self._contiguous = at, all(p.is_contiguous() for p in params)
+            self._at = at
         groups = b''
         for group in self.param_groups:
             self._check_group(group)
@@ -202,5 +235,37 @@ def _dense(p):
     return True
 
 
-def _bytes(t):
-    return t.view(-1).view(ch.uint8)
+def _order(t):
+    """The order of a dense tensor's values in memory."""
+    return [stride for stride, n in zip(t.stride(), t.shape) if n != 1]
+
+
+def _in_memory(t):
+    """A dense tensor's values in the order in which they lie in memory."""
+    return ch.as_strided(t, (t.numel(),), (1,))
+
+
+_TOP = {ch.float8_e4m3fn: 7, ch.float8_e5m2: 14}  # a block's largest value is 2^TOP .. 2^(TOP + 1) times its scale
+
+
+def _from_eight(codes, scales):
+    """A moment in 32 bits, in its codes' order in memory."""
+    values = ch.empty_like(codes, dtype=ch.float32)
+    _in_memory(values).copy_(_in_memory(codes).float() * scales.repeat_interleave(_BLOCK)[:codes.numel()])
+    return values
+
+
+def _in_eight(codes, scales, values):
+    """Writes a moment as codes and scales, as the kernel does but rounded to the nearest."""
+    if codes.numel() == 0:
+        return
+    own = ch.empty_like(codes, dtype=ch.float32).copy_(values)
+    blocks = ch.nn.functional.pad(_in_memory(own), (0, -codes.numel() % _BLOCK)).view(-1, _BLOCK).double()
+    top = _TOP[codes.dtype]
+    power = (ch.frexp(blocks.abs().amax(1))[1] - 1).clamp(min=-126)
+    finite = ch.isfinite(blocks).all(1)
+    scales.copy_(ch.where(finite, ch.ldexp(ch.ones_like(power, dtype=ch.float64), power - top), ch.nan))
+    scaled = ch.ldexp(blocks, (top - power)[:, None])
+    if codes.dtype == ch.float8_e5m2:  # (above zero it stays above zero)
+        scaled = ch.where(blocks > 0, scaled.clamp(min=2.0 ** -16), scaled)
+    _in_memory(codes).copy_(scaled.view(-1)[:codes.numel()].float().to(codes.dtype))
