@@ -219,9 +219,9 @@ class AdamW(ch.optim.Optimizer):
                     continue
                 if entry[name].shape != view.shape or entry[name].dtype != view.dtype:
                     raise ValueError(f'saved {name}: {entry[name].dtype} {tuple(entry[name].shape)}, not {view.dtype} {tuple(view.shape)}')
-                view.copy_(entry[name])
-            if 'master' in own and 'master' not in entry:
-                own['master'].copy_(p.detach())
+                if self.state_bits == 8 and not _dense(entry[name]):
+                    raise ValueError(f'saved {name}: values with gaps or overlaps have no blocks')
+            self._take(own, entry if 'master' in entry else dict(entry, master=p.detach()))
             self._steps[i] = int(entry['step'])
 
 

@@ -182,3 +182,37 @@ def test_frozen_between_steps_and_in_other_modes(monkeypatch):
         else:
             opt.step()
     assert lib.steps == 6 and want.near(p.detach()) and math.isclose(want.t, 6)
+
+
+@pytest.mark.parametrize('bits', [8, 32])
+@pytest.mark.parametrize('dtype', [ch.float32, ch.bfloat16], ids=str)
+def test_state_saved_in_another_order(monkeypatch, bits, dtype):
+    """A network that was trained with its channels last goes on with them first: moments in 8 bits have a scale per block of
+    neighbours in memory, which are others then."""
+    AdamW, lib = on_the_host(monkeypatch)
+    gen = ch.Generator().manual_seed(2)
+    p = ch.nn.Parameter(ch.randn((5, 30, 4, 3), generator=gen).to(dtype).to(memory_format=ch.channels_last))
+    opt = AdamW([p], **HYPER, state_bits=bits)
+    spread = ch.exp(2 * ch.randn((5, 30, 1, 1), generator=gen))  # (of another size in every channel)
+    for _ in range(3):
+        p.grad = (ch.randn(p.shape, generator=gen) * spread).to(dtype)
+        opt.step()
+    q = ch.nn.Parameter(p.detach().contiguous())
+    other = AdamW([q], **HYPER, state_bits=bits)
+    other.load_state_dict(opt.state_dict())
+    for k, (name, own, most) in enumerate((('exp_avg', 2.0 ** -4, 2.0 ** -10), ('exp_avg_sq', 2.0 ** -3, 2.0 ** -17))):
+        values = []
+        for o, t in ((opt, p), (other, q)):
+            v, shape = o.state[t][name], t.shape
+            assert v.stride() == t.stride()
+            if bits == 8:
+                flat = ch.as_strided(v, (v.numel(),), (1,)).float() * o.state[t]['scales'][:, k].repeat_interleave(256)[:v.numel()]
+                v = ch.as_strided(flat, shape, t.stride())
+            values.append(v)
+        was, now = values
+        if bits == 32:
+            assert ch.equal(was, now)
+        else:
+            assert bool(((now - was).abs() <= own * was.abs() + most * was.abs().max()).all())
+    if dtype != ch.float32:
+        assert ch.equal(opt.state[p]['master'], other.state[q]['master'])
