@@ -198,31 +198,40 @@ class AdamW(ch.optim.Optimizer):
     @ch.no_grad()
     def load_state_dict(self, saved):
         """State as :meth:`state_dict` gives it, of the same parameters in the same groups; with ``state_bits=32`` also
-        that of ``torch.optim.AdamW``.  Values are copied into the flat tensors."""
+        that of ``torch.optim.AdamW``.  Values are copied into the flat tensors; a parameter without saved state begins anew.  What
+        does not fit is refused before anything is changed."""
         groups = saved['param_groups']
         if [len(g['params']) for g in groups] != [len(g['params']) for g in self.param_groups]:
             raise ValueError('the saved state has other parameter groups')
         if saved.get('state_bits', 32) != self.state_bits:
             raise ValueError(f"the saved state has {saved.get('state_bits', 32)}-bit moments, not {self.state_bits}-bit ones")
-        for group, theirs in zip(self.param_groups, groups):
-            for key, value in theirs.items():
-                if key != 'params' and key in group:
-                    group[key] = value
+        options = [{key: theirs.get(key, value) for key, value in group.items() if key != 'params'}
+                   for group, theirs in zip(self.param_groups, groups)]
+        for group in options:
             self._check_group(group)
-        ids = [i for g in groups for i in g['params']]
-        for i, (p, key) in enumerate(zip(self._params, ids)):
-            entry, own = saved['state'].get(key), self.state[p]
-            if entry is None:
-                continue
-            for name, view in own.items():
+        entries = [saved['state'].get(i) for g in groups for i in g['params']]
+        for p, entry in zip(self._params, entries):
+            for name, view in self.state[p].items() if entry else ():
                 if name == 'step' or (name == 'master' and name not in entry):
                     continue
                 if entry[name].shape != view.shape or entry[name].dtype != view.dtype:
                     raise ValueError(f'saved {name}: {entry[name].dtype} {tuple(entry[name].shape)}, not {view.dtype} {tuple(view.shape)}')
                 if self.state_bits == 8 and not _dense(entry[name]):
                     raise ValueError(f'saved {name}: values with gaps or overlaps have no blocks')
-            self._take(own, entry if 'master' in entry else dict(entry, master=p.detach()))
-            self._steps[i] = int(entry['step'])
+        for group, values in zip(self.param_groups, options):
+            group.update(values)
+        for i, (p, entry) in enumerate(zip(self._params, entries)):
+            own = self.state[p]
+            if entry:
+                self._take(own, entry if 'master' in entry else dict(entry, master=p.detach()))
+            else:
+                for name in ('exp_avg', 'exp_avg_sq'):
+                    _in_memory(own[name]).view(ch.uint8).zero_()
+                if 'scales' in own:
+                    own['scales'].fill_(1.0)
+                if 'master' in own:
+                    own['master'].copy_(p.detach())
+            self._steps[i] = int(entry['step']) if entry else 0
 
 
 def _dense(p):
