@@ -27,7 +27,9 @@ class AdamW(ch.optim.Optimizer):
     seed : int
         Of the stochastic rounding: the same seed, steps and gradients give the same weights.
 
-    16-bit parameters have 32-bit masters, which the steps are made on.  The state lies in flat tensors, ``exp_avg``,
+    16-bit parameters have 32-bit masters, which the steps are made on.  Values that were written to a parameter since (by
+    ``load_state_dict`` of a network, by a swap for its average, by clamping) take their masters' place at the next step; what is written
+    through ``p.data`` autograd does not know of, and ``masters_from_parameters`` has to be called behind it.  The state lies in flat tensors, ``exp_avg``,
     ``exp_avg_sq``, ``scales`` (8 bits) and ``master`` (16-bit parameters), of which ``state[p]`` has views; every
     parameter begins a block of 256 values, the rest of its last block is zero.  A parameter without a gradient is left alone,
     and its step is not counted.  The kernels read the current learning rates from the groups and take gradients and
@@ -46,6 +48,7 @@ class AdamW(ch.optim.Optimizer):
         self.exp_avg = self.exp_avg_sq = self.scales = self.master = self.grad_norm = None
         self._params, self._numel, self._steps = [], None, np.zeros(0, np.int64)
         self._layouts = self._grad_layouts = None
+        self._seen = [], []  # 16-bit parameters' versions and addresses when their masters were last as they are
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
 
     @staticmethod
@@ -87,6 +90,7 @@ class AdamW(ch.optim.Optimizer):
     def _lay_out(self):
         """Flat state for all parameters of all groups, as they lie now; what there was keeps its values."""
         old = {p: (self.state[p], int(step)) for p, step in zip(self._params, self._steps)}
+        seen = dict(zip(self._params, zip(*self._seen)))
         self._params = [p for group in self.param_groups for p in group['params']]
         n, device, dtype = len(self._params), self._params[0].device, self._params[0].dtype
         self._dtype = dtype
@@ -121,7 +125,20 @@ class AdamW(ch.optim.Optimizer):
                 entry['master'].copy_(p.detach())
             self.state[p] = entry
         self._steps = steps
+        if self.master is not None:
+            both = [seen.get(p, (p._version, p.data_ptr())) for p in self._params]
+            self._seen = [version for version, _ in both], [place for _, place in both]
         self._host = self._numel.ctypes.data, self._steps.ctypes.data, self._group_of.ctypes.data
+
+    @ch.no_grad()
+    def masters_from_parameters(self, only=None):
+        """Makes masters follow 16-bit parameters that have been written to: where a value is not its master rounded, it becomes the
+        master.  ``only``: numbers of parameters, in the groups' order; default: all."""
+        for i in range(len(self._params)) if only is None and self.master is not None else only or ():
+            p = self._params[i].detach()
+            if p.numel():
+                master = self.state[self._params[i]]['master']
+                master.copy_(ch.where(master.to(p.dtype) == p, master, p.float()))
 
     def _take(self, own, was):
         """A parameter's state from another of the same shape, whatever order in memory either is in."""
@@ -162,6 +179,10 @@ class AdamW(ch.optim.Optimizer):
             self._layouts = N.layouts(params)
         dtype, index = self._dtype, params[0].get_device()
         at = [p.data_ptr() for p in params]
+        if self.master is not None:
+            seen = [p._version for p in params], at
+            if seen != self._seen:
+                self.masters_from_parameters([i for i, (now, then) in enumerate(zip(zip(*seen), zip(*self._seen))) if now != then])
         # addresses of gradients, 0 without one
         grads, kept = [p.grad for p in params], None
         if self._grad_layouts is not None and self._grad_layouts.check(*grads):
@@ -186,6 +207,8 @@ class AdamW(ch.optim.Optimizer):
         N.check(N.lib.ffcvb_adamw_step(args, *self._host, struct.pack(f'={n}Q', *grads_at), groups, len(self.param_groups), N.raw_stream(index)))
         del kept
         ch.autograd.graph.increment_version(params)  # (a later backward pass that needs what they were says so)
+        if self.master is not None:
+            self._seen = [p._version for p in params], at
         return loss
 
     def state_dict(self):
@@ -232,6 +255,7 @@ class AdamW(ch.optim.Optimizer):
                 if 'master' in own:
                     own['master'].copy_(p.detach())
             self._steps[i] = int(entry['step']) if entry else 0
+        self._seen = [None] * len(self._seen[0]), self._seen[1]  # (parameters may be others than those that the saved masters belong to)
 
 
 def _dense(p):

@@ -74,3 +74,88 @@ def test_what_does_not_fit_changes_nothing(monkeypatch):
             opt.load_state_dict(saved)
         assert all(ch.equal(x, y) for x, y in zip(before, bytes_of(opt)))
         assert opt.param_groups[0]['lr'] == HYPER['lr'] and opt._steps.tolist() == [1, 1, 1]
+
+
+def write_in_place(p, new):
+    with ch.no_grad():
+        p.copy_(new)
+
+
+def load_network(p, new):
+    net = ch.nn.Module()
+    net.p = p
+    net.load_state_dict(dict(p=new))
+
+
+def other_memory(p, new):
+    p.data = new.clone()
+
+
+def through_detach(p, new):
+    p.detach().copy_(new)
+
+
+@pytest.mark.parametrize('write', [write_in_place, load_network, other_memory, through_detach], ids=lambda f: f.__name__)
+@pytest.mark.parametrize('dtype', [ch.bfloat16, ch.float16], ids=str)
+@pytest.mark.parametrize('steps', [0, 2])
+@pytest.mark.parametrize('bits', [8, 32])
+def test_masters_follow_what_is_written(monkeypatch, write, dtype, steps, bits):
+    """Before the first step and between steps: the next step is made on the new values.  Values that were not changed keep the digits that
+    only their masters have."""
+    AdamW, lib = on_the_host(monkeypatch)
+    params, gen = params_of(dtype)
+    opt = AdamW(params, **HYPER, state_bits=bits)
+    for _ in range(steps):
+        set_grads(params, gen)
+        opt.step()
+    new = params[1].detach().clone()
+    new[3:9] = ch.randn((6, 30), generator=gen).to(dtype)
+    new[4, 2], new[5, 3] = 0.0, float('inf')
+    want = opt.state[params[1]]['master'].clone()
+    want[3:9] = ch.where(new[3:9] == params[1].detach()[3:9], want[3:9], new[3:9].float())
+    rest = [opt.state[p]['master'].clone() for p in (params[0], params[2])]
+    write(params[1], new)
+    for group in opt.param_groups:
+        group['lr'] = 0.0  # a step of no size: the masters stay as they are when it begins
+    set_grads(params, gen)
+    opt.step()
+    assert ch.equal(opt.state[params[1]]['master'], want) and ch.equal(params[1].detach(), new)
+    assert all(ch.equal(opt.state[p]['master'], r) for p, r in zip((params[0], params[2]), rest))
+    if steps:
+        assert not ch.equal(want[:3], new[:3].float())
+
+
+def test_masters_of_parameters_that_are_clamped_behind_autograds_back(monkeypatch):
+    AdamW, lib = on_the_host(monkeypatch)
+    params, gen = params_of(ch.bfloat16)
+    opt = AdamW(params, **HYPER)
+    set_grads(params, gen)
+    opt.step()
+    for p in params:
+        p.data.clamp_(-0.5, 0.5)
+    opt.masters_from_parameters()
+    for p in params:
+        master = opt.state[p]['master']
+        assert ch.equal(master.to(p.dtype), p.detach()) and float(master.abs().max()) <= 0.5 + 2.0 ** -9
+    plain, _ = params_of(ch.float32)
+    AdamW(plain).masters_from_parameters()  # (there are none)
+
+
+def test_loaded_masters_give_way_to_other_weights(monkeypatch):
+    """A saved optimizer's masters belong to its weights; other weights that are there when it is loaded stay."""
+    AdamW, lib = on_the_host(monkeypatch)
+    a, gen = params_of(ch.bfloat16)
+    opt = AdamW(a, **dict(HYPER, lr=0.0))
+    set_grads(a, gen)
+    opt.step()
+    saved = opt.state_dict()
+    b, _ = params_of(ch.bfloat16, 7)
+    with ch.no_grad():
+        b[0].copy_(a[0])
+    before = [p.detach().clone() for p in b]
+    other = AdamW(b, **HYPER)
+    other.load_state_dict(saved)
+    set_grads(b, gen)
+    other.step()
+    assert ch.equal(other.state[b[0]]['master'], saved['state'][0]['master'])
+    assert all(ch.equal(p.detach(), w) for p, w in zip(b, before))
