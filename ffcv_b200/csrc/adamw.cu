@@ -583,6 +583,10 @@ int ffcvb_adamw_step(const ffcvb_adamw_args *args, const int64_t *numel, int64_t
     OnDevice here(a.device);
     if (!here.ok()) return training_fail(FFCVB_E_NODEVICE, "ffcvb_adamw_step: no device %d", a.device);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(st, &capture) != cudaSuccess) return launched("ffcvb_adamw_step");
+    if (capture != cudaStreamCaptureStatusNone)
+        return training_fail(FFCVB_E_ARG, "ffcvb_adamw_step: a step cannot be captured: its number, rates and gradients' addresses are its kernels' arguments");
     for (int32_t i = 0; i < a.n_tensors; i++) steps[i] += grads[i] != 0;
     with_type(a.type, [&](auto zero) {
         using T = decltype(zero);

@@ -41,6 +41,8 @@ def check(rc):
 
 # The handle of a device's current stream, without the object around it that ch.cuda.current_stream makes (2 us a call).
 raw_stream = ch._C._cuda_getCurrentRawStream
+# Whether the current stream of the current device is being captured in a graph.
+capturing = ch._C._cuda_isCurrentStreamCapturing
 
 
 def layouts(tensors):

@@ -35,7 +35,8 @@ class AdamW(ch.optim.Optimizer):
     and its step is not counted.  The kernels read the current learning rates from the groups and take gradients and
     parameters wherever they lie at the time of the step.  Where the order of a parameter's values in memory has changed
     (``model.to(memory_format=...)``) its state is brought into that order, moments in 8 bits rounded once more; a parameter of
-    another shape or type, on another device or with gaps is refused.
+    another shape or type, on another device or with gaps is refused.  A step cannot be captured in a graph: its number, the rates and
+    the gradients' addresses come from the host.
     """
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, state_bits=32, max_grad_norm=None,
@@ -167,11 +168,13 @@ class AdamW(ch.optim.Optimizer):
 
     @ch.no_grad()
     def step(self, closure=None):
+        params, n = self._params, len(self._params)
+        if N.capturing():
+            raise RuntimeError('a step of AdamW cannot be captured in a graph: a replay would repeat its number, rates and gradients\' addresses')
         loss = None
         if closure is not None:
             with ch.enable_grad():
                 loss = closure()
-        params, n = self._params, len(self._params)
         if not self._layouts.check(*params):
             self._check_params()
             if any(_order(p) != _order(self.state[p]['exp_avg']) for p in params):

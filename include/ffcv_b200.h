@@ -397,7 +397,8 @@ int ffcvb_rotary(const ffcvb_rotary_args *args, void *stream);
  *   w = w (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps),
  * c = 1, or min(1, max_norm / (norm + 1e-6)) with max_norm > 0, norm being that of all gradients; where that is not
  * finite, nothing is changed.  8-bit moments are rounded stochastically: the numbers come from a hash of seed, t and
- * a value's place in the flat arrays.  Tensors whose gradient is NULL are left alone. */
+ * a value's place in the flat arrays.  Tensors whose gradient is NULL are left alone.  A step cannot be captured in a graph
+ * (FFCVB_E_ARG): t, the rates and the gradients' addresses are made on the host. */
 #define FFCVB_ADAMW_BLOCK 256
 typedef struct {
     double lr, beta1, beta2, eps, weight_decay;
