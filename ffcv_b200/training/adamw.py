@@ -209,7 +209,8 @@ class AdamW(ch.optim.Optimizer):
                             N.TYPES[dtype], self.state_bits, n, self.max_grad_norm or 0.0)
         N.check(N.lib.ffcvb_adamw_step(args, *self._host, struct.pack(f'={n}Q', *grads_at), groups, len(self.param_groups), N.raw_stream(index)))
         del kept
-        ch.autograd.graph.increment_version(params)  # (a later backward pass that needs what they were says so)
+        # (a later backward pass that needs what they were says so)
+        ch.autograd.graph.increment_version(params if all(grads_at) else [p for p, g in zip(params, grads_at) if g])
         if self.master is not None:
             self._seen = [p._version for p in params], at
         return loss

@@ -159,3 +159,20 @@ def test_loaded_masters_give_way_to_other_weights(monkeypatch):
     other.step()
     assert ch.equal(other.state[b[0]]['master'], saved['state'][0]['master'])
     assert all(ch.equal(p.detach(), w) for p, w in zip(b, before))
+
+
+def test_a_parameter_without_a_gradient_keeps_its_version(monkeypatch):
+    """A backward pass that needs it goes on; one that needs a parameter of the step does not."""
+    AdamW, lib = on_the_host(monkeypatch)
+    a, b = (ch.nn.Parameter(ch.ones(8)) for _ in range(2))
+    opt = AdamW([a, b], **HYPER)
+    x = ch.ones(8, requires_grad=True)
+    needs_a, needs_b = (x * a).sum(), (x * b).sum()
+    a.grad = ch.ones(8)
+    versions = a._version, b._version
+    opt.step()
+    assert a._version > versions[0] and b._version == versions[1]
+    needs_b.backward()
+    assert ch.equal(x.grad, ch.ones(8))
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        needs_a.backward()
