@@ -75,7 +75,8 @@ class AdamW(ch.optim.Optimizer):
         except Exception:
             self.param_groups.pop()
             raise
-        self._lay_out()
+        if self._params or group['params']:
+            self._lay_out()
 
     def _check_params(self):
         """Refuses parameters that are no longer what their state was made for."""
@@ -175,6 +176,8 @@ class AdamW(ch.optim.Optimizer):
         if closure is not None:
             with ch.enable_grad():
                 loss = closure()
+        if not params:
+            return loss
         if not self._layouts.check(*params):
             self._check_params()
             if any(_order(p) != _order(self.state[p]['exp_avg']) for p in params):

@@ -176,3 +176,28 @@ def test_a_parameter_without_a_gradient_keeps_its_version(monkeypatch):
     assert ch.equal(x.grad, ch.ones(8))
     with pytest.raises(RuntimeError, match='modified by an inplace operation'):
         needs_a.backward()
+
+
+def test_groups_without_parameters(monkeypatch):
+    """A network without vectors, say, whose group comes first, in between, last, or alone."""
+    AdamW, lib = on_the_host(monkeypatch)
+    params, gen = params_of(ch.bfloat16)
+    plain = [ch.nn.Parameter(p.detach().clone()) for p in params]
+    opt = AdamW([dict(params=[]), dict(params=params[:2]), dict(params=[], lr=1.0), dict(params=params[2:]), dict(params=[])], **HYPER)
+    want = AdamW(plain, **HYPER)
+    for _ in range(2):
+        set_grads(params, gen)
+        for p, q in zip(params, plain):
+            q.grad = p.grad.clone()
+        opt.step()
+        want.step()
+    assert all(ch.equal(p, q) for p, q in zip(params, plain))
+    opt.load_state_dict(opt.state_dict())
+    empty = AdamW([dict(params=[])], **HYPER)
+    assert empty.step(lambda: 3) == 3
+    empty.load_state_dict(empty.state_dict())
+    empty.masters_from_parameters()
+    empty.add_param_group(dict(params=params))
+    set_grads(params, gen)
+    empty.step()
+    assert empty._steps.tolist() == [1, 1, 1]
