@@ -1,5 +1,6 @@
 """AdamW over all tensors of a network in one launch, with moments in 32 or in 8 bits."""
 import struct
+from collections import defaultdict
 
 import numpy as np
 import torch as ch
@@ -46,11 +47,14 @@ class AdamW(ch.optim.Optimizer):
         if max_grad_norm is not None and not max_grad_norm > 0:
             raise ValueError(f'max_grad_norm must be positive, not {max_grad_norm}')
         self.state_bits, self.max_grad_norm, self.seed = state_bits, max_grad_norm, int(seed)
+        self._blank()
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+
+    def _blank(self):
         self.exp_avg = self.exp_avg_sq = self.scales = self.master = self.grad_norm = None
         self._params, self._numel, self._steps = [], None, np.zeros(0, np.int64)
         self._layouts = self._grad_layouts = None
         self._seen = [], []  # 16-bit parameters' versions and addresses when their masters were last as they are
-        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
 
     @staticmethod
     def _check_group(group):
@@ -218,12 +222,39 @@ class AdamW(ch.optim.Optimizer):
             self._seen = [p._version for p in params], at
         return loss
 
-    def state_dict(self):
+    def _count(self):
+        """Brings the steps in ``state`` up to date."""
         for p, step in zip(self._params, self._steps):
             self.state[p]['step'] = int(step)
+
+    def state_dict(self):
+        self._count()
         saved = super().state_dict()
         saved['state_bits'] = self.state_bits
         return saved
+
+    def __getstate__(self):
+        self._count()
+        saved = super().__getstate__()
+        if self.state_bits == 8:  # (as whole numbers: pickle has no codes)
+            saved['state'] = {p: {k: t.view(ch.uint8) if k.startswith('exp') else t for k, t in entry.items()} for p, entry in self.state.items()}
+        return dict(saved, _own=(self.state_bits, self.max_grad_norm, self.seed))
+
+    @ch.no_grad()
+    def __setstate__(self, saved):
+        """A copy (``copy.deepcopy``, ``pickle``) has flat state of its own."""
+        saved = dict(saved)
+        self.state_bits, self.max_grad_norm, self.seed = saved.pop('_own')
+        was, saved['state'] = saved['state'], defaultdict(dict)
+        super().__setstate__(saved)
+        self._blank()
+        if any(group['params'] for group in self.param_groups):
+            self._lay_out()
+        for i, p in enumerate(self._params):
+            own, entry = self.state[p], was[p]
+            self._take(own, {k: t.view(own[k].dtype) if k.startswith('exp') else t for k, t in entry.items()})
+            self._steps[i] = own['step'] = entry['step']
+        self._seen = [None] * len(self._params), [None] * len(self._params)
 
     @ch.no_grad()
     def load_state_dict(self, saved):
@@ -262,7 +293,7 @@ class AdamW(ch.optim.Optimizer):
                 if 'master' in own:
                     own['master'].copy_(p.detach())
             self._steps[i] = int(entry['step']) if entry else 0
-        self._seen = [None] * len(self._seen[0]), self._seen[1]  # (parameters may be others than those that the saved masters belong to)
+        self._seen = [None] * len(self._params), [None] * len(self._params)  # (parameters may be others than those that the saved masters belong to)
 
 
 def _dense(p):

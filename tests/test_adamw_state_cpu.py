@@ -1,4 +1,7 @@
 """The optimizer's state as it is kept, saved, loaded and copied, on the host: a step is the formula in numpy."""
+import copy
+import pickle
+
 import pytest
 import torch as ch
 
@@ -201,3 +204,41 @@ def test_groups_without_parameters(monkeypatch):
     set_grads(params, gen)
     empty.step()
     assert empty._steps.tolist() == [1, 1, 1]
+
+
+@pytest.mark.parametrize('how', ['deepcopy', 'pickle', 'copy.copy'])
+@pytest.mark.parametrize('bits', [8, 32])
+@pytest.mark.parametrize('dtype', [ch.float32, ch.bfloat16], ids=str)
+def test_copies_go_on_by_themselves(monkeypatch, bits, dtype, how):
+    """A copy of a network and its optimizer makes the steps that they would, on state of its own."""
+    AdamW, lib = on_the_host(monkeypatch)
+    params, gen = params_of(dtype)
+    opt = AdamW([dict(params=params[:2]), dict(params=params[2:], lr=1e-2)], **HYPER, state_bits=bits, seed=4)
+    for step in range(3):
+        set_grads(params, gen)
+        params[1].grad = None if step == 1 else params[1].grad
+        opt.step()
+    if how == 'copy.copy':  # (of the optimizer alone: the same parameters)
+        other = copy.copy(opt)
+        before = bytes_of(opt)
+        other.step()
+        assert other.param_groups[0]['params'][0] is params[0] and all(ch.equal(x, y) for x, y in zip(before, bytes_of(opt)))
+        assert opt._steps.tolist() == [3, 2, 3] and opt.state[params[0]]['exp_avg'].data_ptr() == opt.exp_avg.data_ptr()
+        return
+    both = params, opt
+    others, other = copy.deepcopy(both) if how == 'deepcopy' else pickle.loads(pickle.dumps(both))
+    assert type(other) is AdamW and (other.state_bits, other.seed, other._steps.tolist()) == (bits, 4, [3, 2, 3])
+    assert all(p is not q and p is r for p, q, r in zip(others, params, other._params))
+    assert all(ch.equal(x, y) for x, y in zip(bytes_of(opt), bytes_of(other)))
+    for _ in range(2):
+        set_grads(params, gen)
+        for p, q in zip(params, others):
+            q.grad = p.grad.clone()
+        before = bytes_of(other)
+        opt.step()
+        assert all(ch.equal(x, y) for x, y in zip(before, bytes_of(other)))
+        other.step()
+        assert all(ch.equal(p, q) for p, q in zip(params, others)) and all(ch.equal(x, y) for x, y in zip(bytes_of(opt), bytes_of(other)))
+    other.load_state_dict(opt.state_dict())
+    other.add_param_group(dict(params=[ch.nn.Parameter(ch.ones(5, dtype=dtype))]))
+    assert opt.state_dict()['state'][1]['step'] == 4
