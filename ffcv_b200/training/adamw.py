@@ -8,6 +8,7 @@ import torch as ch
 from . import _native as N
 
 _BLOCK = N.ADAMW_BLOCK
+_address = ch.Tensor.data_ptr
 
 
 class AdamW(ch.optim.Optimizer):
@@ -93,6 +94,7 @@ class AdamW(ch.optim.Optimizer):
             if not _dense(p):
                 raise ValueError('parameters must lie together in memory, without gaps or overlaps')
 
+    @ch.no_grad()
     def _lay_out(self):
         """Flat state for all parameters of all groups, as they lie now; what there was keeps its values."""
         old = {p: (self.state[p], int(step)) for p, step in zip(self._params, self._steps)}
@@ -169,9 +171,8 @@ class AdamW(ch.optim.Optimizer):
             raise TypeError(f'gradients must be dense, of the parameters\' type and on their GPU, not {g.dtype} {g.layout} on {g.device}')
         if g.shape != p.shape:
             raise ValueError(f'a parameter of shape {tuple(p.shape)} has a gradient of shape {tuple(g.shape)}')
-        return g if g.stride() == p.stride() else ch.empty_like(p).copy_(g)
+        return g if g.stride() == p.stride() else ch.empty_like(p, requires_grad=False).copy_(g.detach())
 
-    @ch.no_grad()
     def step(self, closure=None):
         params, n = self._params, len(self._params)
         if N.capturing():
@@ -188,7 +189,7 @@ class AdamW(ch.optim.Optimizer):
                 self._lay_out()
             self._layouts = N.layouts(params)
         dtype, index = self._dtype, params[0].get_device()
-        at = [p.data_ptr() for p in params]
+        at = list(map(_address, params))
         if self.master is not None:
             seen = [p._version for p in params], at
             if seen != self._seen:
@@ -196,7 +197,7 @@ class AdamW(ch.optim.Optimizer):
         # addresses of gradients, 0 without one
         grads, kept = [p.grad for p in params], None
         if self._grad_layouts is not None and self._grad_layouts.check(*grads):
-            grads_at = [g.data_ptr() for g in grads]
+            grads_at = list(map(_address, grads))
         else:
             kept = [None if g is None else self._as_parameter(p, g) for p, g in zip(params, grads)]
             grads_at = [N.ptr(g) for g in kept]
