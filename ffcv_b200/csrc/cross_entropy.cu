@@ -1,7 +1,8 @@
 // Cross entropy against labels, mixed labels or probabilities, with its gradient (sm_100a).
 //
 // With T the target's probabilities, S their sum and lse = log sum exp x, a row's loss is S * lse - sum T x and
-// its gradient S * exp(x - lse) - T.  Some lanes of a warp take a row of up to 8 KB, a CTA one of up to 56 KB, a cluster a longer one.  Every
+// its gradient S * exp(x - lse) - T.  With the largest logit taken off, S * log sum exp(x - top) + sum T (top - x), the loss has terms of
+// one sign alone, and no logit's size enters it.  Some lanes of a warp take a row of up to 8 KB, a CTA one of up to 56 KB, a cluster a longer one.  Every
 // thread copies its part of the row into shared memory, in places of its own; a pass over it keeps the largest logit so far and the
 // sum of exponentials relative to that (in 32 bits), which are joined over the row's threads; a second pass makes the gradient.  So
 // the row crosses HBM once each way, and several CTAs per SM load, compute and store at different times.
@@ -82,16 +83,20 @@ __device__ __forceinline__ void copy16(uint32_t to, const void *from) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
 }
 
-// The largest logit of a part of a row, at least kLowest, and the sum of exponentials relative to it; what else is summed up.  (Where all
-// logits are -inf the sum is 0: no difference here is that of two infinities of one sign, unless a logit is +inf.)
+// The largest logit of a part of a row, at least kLowest, and the sum of exponentials relative to it; with targets besides labels also the
+// sum of targets times logits, which are relative to it too, and the targets' sum.  (Where all logits are -inf the sum is 0: no difference
+// here is that of two infinities of one sign, unless a logit is +inf.)  Relative sums stay finite where several logits are the type's
+// lowest value, and keep the digits of logits that are all far from zero.
 constexpr float kLowest = -3.402823466e38f;
 struct Found {
     float top, sum, dot, mass;
+    // what a dot relative to `from` has more when it is relative to `to`, the larger (kept finite: there may be no mass yet)
+    static __device__ __forceinline__ float shift(float mass, float from, float to) { return mass * fmaxf(from - to, kLowest); }
     __device__ __forceinline__ void join(float t, float s, float d, float m) {
         const float most = fmaxf(top, t);
         sum = sum * exp_of(top - most) + s * exp_of(t - most);
+        dot = (dot + shift(mass, top, most)) + (d + shift(m, t, most));
         top = most;
-        dot += d;
         mass += m;
     }
     // joins those of groups of LANES lanes, in each of which all are in `mask`; `more`: dot and mass too
@@ -100,6 +105,7 @@ struct Found {
 #pragma unroll
         for (int o = LANES / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(mask, most, o));
         sum *= exp_of(top - most);
+        if (more) dot += shift(mass, top, most);
         top = most;
 #pragma unroll
         for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(mask, sum, o);
@@ -193,11 +199,11 @@ rows_kernel(const __grid_constant__ ffcvb_cross_entropy_args a, const Deal deal)
     }
     const long long soft_row = row * a.target_stride;
     const float sure = 1.0f - a.smoothing;
-    float picked = 0.0f; // of the labels' logits
+    float picked[2] = {0.0f, 0.0f}; // the labels' logits
     if (!SOFT && thread == 0 && rank == 0 && !a.from_stats) {
 #pragma unroll
         for (int k = 0; k < 2; k++)
-            if (p.weight[k] != 0.0f) picked += p.weight[k] * to_float(x[p.label[k]]);
+            if (p.weight[k] != 0.0f) picked[k] = to_float(x[p.label[k]]);
     }
     // Calls f(values, class of the first) for this thread's packs: as many turns as all threads have, BATCH at a time, then what is left.
     const int turns = count / threads;
@@ -249,22 +255,34 @@ rows_kernel(const __grid_constant__ ffcvb_cross_entropy_args a, const Deal deal)
         Found f{kLowest, 0.0f, 0.0f, 0.0f};
         auto take = [&](auto &v, int c) {
             constexpr int M = sizeof(v) / 4;
+            const float was = f.top;
+            float t[M];
+            if (SOFT) probabilities<M>(t, a, soft_row + c, deal.soft_wide);
+            f.add(v);
             if (SOFT) {
-                float t[M];
-                probabilities<M>(t, a, soft_row + c, deal.soft_wide);
+                f.dot += Found::shift(f.mass, was, f.top);
+                float part = 0.0f, mass = 0.0f;
 #pragma unroll
                 for (int j = 0; j < M; j++) {
                     t[j] = sure * t[j] + p.flat;
-                    f.mass += t[j];
-                    if (t[j] > 0.0f) f.dot += t[j] * v[j];
+                    mass += t[j];
+                    part += t[j] > 0.0f ? t[j] * (v[j] - f.top) : 0.0f;
                 }
+                f.dot += part;
+                f.mass += mass;
             } else if (p.flat > 0.0f) {
-                float part = v[0];
+                f.dot += Found::shift(f.mass, was, f.top);
+                f.mass += M * p.flat;
+                if constexpr (M == 1) {
+                    f.dot += p.flat * (v[0] - f.top);
+                } else { // (each times its target before they are added: the sum of two lowest values is none)
+                    const Two minus(-f.top, -f.top), flat(p.flat, p.flat);
+                    Two part(0.0f, 0.0f);
 #pragma unroll
-                for (int j = 1; j < M; j++) part += v[j];
-                f.dot += p.flat * part;
+                    for (int j = 0; j < M; j += 2) part = fma_rn(add_rn(Two(v[j], v[j + 1]), minus), flat, part);
+                    f.dot += part.lo() + part.hi();
+                }
             }
-            f.add(v);
         };
         each_single([&](int c) {
             const float v[1] = {to_float(x[c])};
@@ -297,7 +315,10 @@ rows_kernel(const __grid_constant__ ffcvb_cross_entropy_args a, const Deal deal)
         over = f.sum == 0.0f ? 0.0f : 1.0f / f.sum;
         if (SOFT) total = f.mass;
         if (thread == 0 && rank == 0) {
-            a.row_loss[row] = f.sum == 0.0f ? 0.0f : total * (row_top + logf(f.sum)) - (f.dot + picked);
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+                if (!SOFT && p.weight[k] != 0.0f) f.dot += p.weight[k] * (picked[k] - row_top);
+            a.row_loss[row] = f.sum == 0.0f ? 0.0f : total * logf(f.sum) - f.dot;
             if (a.stats) reinterpret_cast<float2 *>(a.stats)[row] = make_float2(row_top, over);
         }
     } else {
