@@ -154,8 +154,7 @@ rows_kernel(const __grid_constant__ ffcvb_cross_entropy_args a, const Deal deal)
     __shared__ float4 s_part[8];
     __shared__ float4 s_there[8]; // from the cluster's CTAs
     extern __shared__ uint4 s_row[];
-    const bool counted = a.has_ignore && a.mean; // by the kernel before this one, which waited for all before it
-    if (!counted) wait_for_previous();
+    wait_for_previous();
     let_next_begin();
     uint32_t rank = 0, ranks = 1;
     if (!WARP) {
@@ -194,7 +193,6 @@ rows_kernel(const __grid_constant__ ffcvb_cross_entropy_args a, const Deal deal)
         }
         if (STAGED) asm volatile("cp.async.wait_group 0;" ::: "memory");
         if (ranks > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
-        if (counted) wait_for_previous();
         return;
     }
     const long long soft_row = row * a.target_stride;
@@ -343,7 +341,6 @@ rows_kernel(const __grid_constant__ ffcvb_cross_entropy_args a, const Deal deal)
             total = mass;
         }
     }
-    if (counted) wait_for_previous();
     if (!g) return;
     float k_row = a.scale;
     if (a.upstream) k_row *= a.upstream[a.upstream_per_row ? row : 0];
@@ -399,7 +396,7 @@ __global__ void __launch_bounds__(1024)
 count_kernel(const int64_t *__restrict__ labels, long long rows, long long stride, long long ignore, float *counted) {
     __shared__ int s_count[32];
     wait_for_previous();
-    let_next_begin(); // (so all that is before this kernel has ended when the next one begins)
+    let_next_begin();
     int n = 0;
     for (long long i = threadIdx.x; i < rows; i += 1024) n += labels[i * stride] != ignore;
     n = __reduce_add_sync(0xffffffffu, n);
