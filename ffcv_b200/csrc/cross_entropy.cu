@@ -512,7 +512,8 @@ using namespace ffcvb;
 extern "C" int ffcvb_cross_entropy(const ffcvb_cross_entropy_args *args, void *stream) {
     if (!args) return training_fail(FFCVB_E_ARG, "ffcvb_cross_entropy: no arguments");
     const ffcvb_cross_entropy_args &a = *args;
-    if (a.rows < 0 || a.classes < 1 || a.rows > 0x0fffffff || a.classes > 0x7fffff00 || (a.type != FFCVB_TYPE_F32 && a.type != FFCVB_TYPE_F16 && a.type != FFCVB_TYPE_BF16))
+    // (classes are counted in 32 bits, by steps of up to 4 * 8 * 256 behind the last one)
+    if (a.rows < 0 || a.classes < 1 || a.rows > 0x0fffffff || a.classes > 0x7fff0000 || (a.type != FFCVB_TYPE_F32 && a.type != FFCVB_TYPE_F16 && a.type != FFCVB_TYPE_BF16))
         return training_fail(FFCVB_E_ARG, "ffcvb_cross_entropy: bad size or type");
     const bool needs_count = a.has_ignore && a.mean && a.target_kind == FFCVB_TARGET_LABELS;
     if (a.target_kind < FFCVB_TARGET_LABELS || a.target_kind > FFCVB_TARGET_SOFT || !(a.smoothing >= 0.0f && a.smoothing <= 1.0f) ||

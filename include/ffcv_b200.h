@@ -326,7 +326,7 @@ const char *ffcvb_training_error(void);
  *   grad_i = k_i * (S * exp(x - lse_i) - T),        k_i = scale * upstream / counted rows (mean) or * 1.
  * Rows with the label ignore_index (has_ignore) give 0 and a gradient of 0 and are not counted; rows whose logits
  * are all -inf give 0 and a gradient of 0 and are; rows with another label outside 0 .. classes - 1 give NaN.  Where no
- * row is counted the mean is 0. */
+ * row is counted the mean is 0.  At most 2^28 - 1 rows of at most 2^31 - 2^16 classes. */
 enum { FFCVB_TARGET_LABELS = 0, FFCVB_TARGET_MIXED = 1, FFCVB_TARGET_SOFT = 2 };
 typedef struct {
     const void *logits;     /* [rows, classes], neighbouring classes next to one another */
