@@ -50,14 +50,14 @@ class _Call:
         self.logits = logits if logits.stride(1) == 1 else logits.contiguous()
         self.target, self.ignore, self.mean, self.smoothing = target, ignore_index, reduction == 'mean', float(smoothing)
 
-    def run(self, grad, loss, one, stats=None, upstream=None, per_row=False, from_stats=False, scale=1.0):
-        """loss: a value per sample, and behind them, with `one`, room for their mean or sum."""
+    def run(self, grad, rows_at, loss_at, stats=None, upstream=None, per_row=False, from_stats=False, scale=1.0):
+        """rows_at, loss_at: addresses for a loss per sample, and for their mean or sum, or 0."""
         x, t, ignore = self.logits, self.target, self.ignore
         rows, classes = x.shape
         counted = ch.empty(1, dtype=ch.float32, device=x.device) if ignore is not None and self.mean else None
-        index, losses = x.get_device(), 0 if loss is None else loss.data_ptr()
+        index = x.get_device()
         args = N.CROSS_ENTROPY.pack(
-            x.data_ptr(), t.data_ptr(), N.ptr(upstream), N.ptr(grad), losses + 4 * rows if one else 0, losses, N.ptr(stats), N.ptr(counted),
+            x.data_ptr(), t.data_ptr(), N.ptr(upstream), N.ptr(grad), loss_at, rows_at, N.ptr(stats), N.ptr(counted),
             rows, classes, x.stride(0), t.stride(0), classes, -1 if ignore is None else ignore,
             index, self.type, self.kind, self.target_type, ignore is not None, self.mean, per_row, from_stats, self.smoothing, scale)
         N.check(N.lib.ffcvb_cross_entropy(args, N.raw_stream(index)))
@@ -92,7 +92,8 @@ def cross_entropy_with_grad(logits, labels=None, *, mixed=None, soft=None, label
     call = _Call(logits, labels, mixed, soft, label_smoothing, ignore_index, reduction)
     n = logits.shape[0]
     loss, grad = ch.empty(n + 1, dtype=ch.float32, device=logits.device), N.new_like(call.logits)
-    call.run(grad, loss, reduction != 'none', scale=grad_scale)
+    at = loss.data_ptr()
+    call.run(grad, at, 0 if reduction == 'none' else at + 4 * n, scale=grad_scale)
     return loss[:n] if reduction == 'none' else loss[n], grad
 
 
@@ -100,13 +101,15 @@ class _CrossEntropy(ch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, call, reduction):
         n = logits.shape[0]
-        loss, stats = (ch.empty(k, dtype=ch.float32, device=logits.device) for k in (n + 1, 2 * n))
-        call.run(None, loss, reduction != 'none', stats)
+        rows, stats = (ch.empty(k, dtype=ch.float32, device=logits.device) for k in (n, 2 * n))
         ctx.per_row = reduction == 'none'
+        # (a tensor of its own: a part of another one could not be changed in place)
+        loss = rows if ctx.per_row else ch.empty((), dtype=ch.float32, device=logits.device)
+        call.run(None, rows.data_ptr(), 0 if ctx.per_row else loss.data_ptr(), stats)
         ctx.save_for_backward(call.logits, call.target, stats)
         call.logits = call.target = None  # (autograd keeps them, and sees to it that nobody changes them)
         ctx.call = call
-        return loss[:n] if ctx.per_row else loss[n]
+        return loss
 
     @staticmethod
     @ch.autograd.function.once_differentiable
@@ -115,7 +118,7 @@ class _CrossEntropy(ch.autograd.Function):
         call.logits, call.target, stats = ctx.saved_tensors
         grad = N.new_like(call.logits)
         upstream = upstream.float().contiguous()
-        call.run(grad, None, False, stats, upstream, ctx.per_row, True)
+        call.run(grad, 0, 0, stats, upstream, ctx.per_row, True)
         call.logits = call.target = None
         return grad, None, None
 
