@@ -147,6 +147,8 @@ class RotaryPositions(ch.nn.Module):
             q.data_ptr(), N.ptr(k), q_out.data_ptr(), N.ptr(k_out), where.data_ptr(), turns, turns + 4 * self.rotary_dim,
             batch, tokens, heads, kv_heads, self.head_dim, self.rotary_dim, stride, qb, qt, qh, kb, kt, kh, qob, qot, qoh, kob, kot, koh,
             index, N.TYPES[q.dtype], where.dtype == ch.float32, self.axes, self.layout == 'interleaved', transpose, self.amplitude, 0)
+        if inplace:  # (a backward pass that needs what they were says so)
+            ch.autograd.graph.increment_version(q if k is None else (q, k))
         N.check(N.lib.ffcvb_rotary(args, N.raw_stream(index)))
         return q_out, k_out
 
