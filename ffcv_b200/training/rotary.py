@@ -14,6 +14,18 @@ def patch_positions(rows, cols, device=None):
     return ch.stack([r, c], 1)
 
 
+def _overlaps(t):
+    """Whether values of a tensor may share memory, as those of an expanded one do."""
+    reach = 0  # of the dimensions within
+    for stride, n in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n != 1):
+        if n == 0:
+            return False
+        if stride <= reach:
+            return True
+        reach += (n - 1) * stride
+    return False
+
+
 class _Rotate(ch.autograd.Function):
     @staticmethod
     def forward(ctx, rotary, positions, q, k):
@@ -128,6 +140,8 @@ class RotaryPositions(ch.nn.Module):
             raise ValueError('in place is for tensors without a gradient: autograd would not know of the change')
         if inplace and (q.stride(3) != 1 or (k is not None and k.stride(3) != 1)):
             raise ValueError('in place the values of a head must lie next to one another')
+        if inplace and (_overlaps(q) or (k is not None and (_overlaps(k) or (k.data_ptr() == q.data_ptr() and q.numel() and k.numel())))):
+            raise ValueError('in place no value may lie where another does: it would be turned more than once')
         if q.stride(3) != 1:
             q = q.contiguous()
         if k is not None and k.stride(3) != 1:
@@ -154,7 +168,8 @@ class RotaryPositions(ch.nn.Module):
 
     def rotate(self, q, k=None, positions=None, transpose=False, inplace=False):
         """``(q, k)`` turned, without autograd.  ``transpose`` turns the other way, which is the gradient's way: given the
-        gradients of what ``rotate`` returned, it returns those of what it was given."""
+        gradients of what ``rotate`` returned, it returns those of what it was given.  ``inplace`` writes over q and k, no value of which may
+        share memory with another."""
         self._check(q, k)
         return self._run(q, k, *self._where(q, positions), transpose, inplace)
 

@@ -37,3 +37,25 @@ def test_in_place_is_seen_by_autograd(which, keys):
         want = rotary.rotate(p)[0]
         rotary.rotate(p, inplace=True)
         assert ch.equal(p, want)
+
+
+def test_values_that_share_memory_are_not_turned_in_place():
+    from ffcv_b200.training import RotaryPositions
+    rotary = RotaryPositions(8)
+    one, fused = ch.randn(2, 3, 1, 8, device='cuda'), ch.randn(2, 3, 5, 8, device='cuda')
+    steps = ch.as_strided(fused, (2, 3, 4, 8), (120, 40, 4, 1))  # heads half over one another
+    before = one.clone(), fused.clone()
+    for args in ((one.expand(2, 3, 4, 8),), (fused, one.expand(2, 3, 4, 8)), (one.expand(2, 3, 1, 8)[:1].expand(2, 3, 1, 8),), (steps,), (fused, fused),
+                 (fused[:, :, :2], fused)):
+        with pytest.raises(ValueError, match='where another does'):
+            rotary.rotate(*args, inplace=True)
+    assert ch.equal(one, before[0]) and ch.equal(fused, before[1])
+    assert rotary.rotate(one.expand(2, 3, 4, 8))[0].shape == (2, 3, 4, 8)
+    want = rotary.rotate(fused[:, :, :4], fused[:, :, 4:])
+    rotary.rotate(fused[:, :, :4], fused[:, :, 4:], inplace=True)  # parts of one projection
+    assert ch.equal(fused[:, :, :4], want[0]) and ch.equal(fused[:, :, 4:], want[1])
+    turned = fused.transpose(1, 2).contiguous().transpose(1, 2)
+    want = rotary.rotate(turned)[0]
+    rotary.rotate(turned, inplace=True)
+    assert ch.equal(turned, want)
+    rotary.rotate(fused[:, :0], fused[:, :0], inplace=True)
