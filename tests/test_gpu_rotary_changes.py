@@ -59,3 +59,52 @@ def test_values_that_share_memory_are_not_turned_in_place():
     rotary.rotate(turned, inplace=True)
     assert ch.equal(turned, want)
     rotary.rotate(fused[:, :0], fused[:, :0], inplace=True)
+
+
+def plain(a, angle):
+    """Turned with sines and cosines that are made in 64 bits and rounded once, in 32 bits: the usual table."""
+    c, s = angle.cos().float()[..., None, :], angle.sin().float()[..., None, :]
+    x, y = a[..., :a.shape[-1] // 2], a[..., a.shape[-1] // 2:]
+    return ch.cat([x * c - y * s, y * c + x * s], -1)
+
+
+@pytest.mark.parametrize('transpose', [False, True])
+@pytest.mark.parametrize('kind', ['whole', 'float', 'patches'])
+def test_digits_in_32_bits(kind, transpose):
+    """The root of the mean square of the errors is that of the usual tables or less than a tenth more: whole and float positions of a
+    long sequence, and an image's patches."""
+    from ffcv_b200.training import RotaryPositions, patch_positions
+    gen = ch.Generator('cuda').manual_seed(1)
+    if kind == 'patches':
+        rotary, positions, batch = RotaryPositions(64, axes=2), patch_positions(14, 14, 'cuda'), 64
+    else:
+        rotary, batch = RotaryPositions(64), 1
+        positions = ch.arange(65536, device='cuda')
+        positions = positions if kind == 'whole' else positions.float() + 0.25
+    q = ch.randn((batch, positions.shape[0], 4, 64), generator=gen, device='cuda')
+    dim = 64 // rotary.axes
+    f = 10000.0 ** (-ch.arange(0, dim, 2, dtype=ch.float64, device='cuda') / dim)
+    angle = positions.double()[..., None] * f
+    angle = angle.flatten(-2) if kind == 'patches' else angle
+    angle = -angle if transpose else angle
+    turn = ch.polar(ch.ones_like(angle), angle)[:, None, :]
+    z = ch.complex(q[..., :32].double(), q[..., 32:].double()) * turn
+    want = ch.cat([z.real, z.imag], -1)
+    error = lambda t: math.sqrt(float((t.double() - want).square().mean()))  # noqa: E731
+    own, tables = error(rotary.rotate(q, None, positions, transpose=transpose)[0]), error(plain(q, angle))
+    assert own <= 1.1 * tables, (own, tables)
+
+
+def test_quarter_turns():
+    """Positions about the places where the nearest quarter turn changes, on either side of zero."""
+    from ffcv_b200.training import RotaryPositions
+    rotary = RotaryPositions(2, base=1.0)  # one radian per unit of position
+    near = ch.arange(-9, 10, device='cuda', dtype=ch.float64)[:, None] * (math.pi / 4) + ch.tensor([-1e-6, -1e-9, 0.0, 1e-9, 1e-6], device='cuda', dtype=ch.float64)
+    positions = ch.cat([near.flatten().float(), ch.arange(-700, 700, device='cuda').float()])
+    for where in (positions, ch.arange(-700, 700, device='cuda'), ch.tensor([-2 ** 40, 2 ** 40, -2 ** 53 + 1], device='cuda')):
+        q = ch.tensor([1.0, 0.0], device='cuda').expand(1, where.numel(), 1, 2)
+        got = rotary.rotate(q, None, where)[0][0, :, 0]
+        # (the product of a position with turns of 2^-64: 2^-65 of a position; floats: 2^-53 of the angle)
+        room = where.double().abs() * 2.0 ** -50 + 2.0 ** -23 + 2.0 ** -25
+        want = ch.stack([where.double().cos(), where.double().sin()], 1)
+        assert bool(((got.double() - want).abs() <= room[:, None]).all())
