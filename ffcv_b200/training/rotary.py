@@ -37,8 +37,12 @@ class _Rotate(ch.autograd.Function):
     @ch.autograd.function.once_differentiable
     def backward(ctx, dq, dk=None):
         positions, = ctx.saved_tensors
-        dq, dk = ctx.rotary._run(dq, dk, *ctx.rotary._where(dq, positions), True, False)
-        return None, None, dq, dk
+        wanted = [g if of else None for g, of in zip((dq, dk), ctx.needs_input_grad[2:])]
+        given = [g for g in wanted if g is not None]
+        if not given:
+            return (None,) * 4
+        turned = ctx.rotary._run(given[0], given[1] if len(given) > 1 else None, *ctx.rotary._where(given[0], positions), True, False)
+        return None, None, *(None if g is None else turned[g is not given[0]] for g in wanted)
 
 
 class RotaryPositions(ch.nn.Module):

@@ -108,3 +108,27 @@ def test_quarter_turns():
         room = where.double().abs() * 2.0 ** -50 + 2.0 ** -23 + 2.0 ** -25
         want = ch.stack([where.double().cos(), where.double().sin()], 1)
         assert bool(((got.double() - want).abs() <= room[:, None]).all())
+
+
+def test_only_wanted_gradients_are_made():
+    """Of queries or keys alone, if only they need one: as many values are allocated as are asked for.  What was turned and then not used
+    has a gradient of zeros."""
+    from ffcv_b200.training import RotaryPositions
+    rotary, where = RotaryPositions(64), ch.arange(256, device='cuda')
+    q, k = ch.randn(2, 256, 4, 64, device='cuda'), ch.randn(2, 256, 2, 64, device='cuda')
+    dq, dk = ch.randn_like(q), ch.randn_like(k)
+    want = rotary.rotate(dq, dk, where, transpose=True)
+    for needs in ((True, True), (True, False), (False, True)):
+        a, b = q.clone().requires_grad_(needs[0]), k.clone().requires_grad_(needs[1])
+        out, leaves = rotary(a, b, where), [t for t in (a, b) if t.requires_grad]
+        ch.cuda.synchronize()
+        ch.cuda.reset_peak_memory_stats()
+        before = ch.cuda.memory_allocated()
+        got = ch.autograd.grad(out, leaves, (dq, dk))
+        peak = ch.cuda.max_memory_allocated() - before
+        wanted = [w for w, need in zip(want, needs) if need]
+        assert all(ch.equal(g, w) for g, w in zip(got, wanted)) and peak <= sum(w.numel() * 4 for w in wanted) + 2048
+    a, b = q.clone().requires_grad_(), k.clone().requires_grad_()
+    for use in (0, 1):
+        got = ch.autograd.grad(rotary(a, b, where)[use], (a, b), (dq, dk)[use])
+        assert ch.equal(got[use], want[use]) and not got[1 - use].any()
