@@ -148,7 +148,7 @@ struct Deal {
 // four warps; 0: a row per CTA or cluster.  STAGED: the packs go through shared memory; else they are read where they are needed.  (Ten CTAs per
 // SM of lanes' rows: 16384 x 2000 bf16 with probabilities 56.4 us, 61.5 with the nine that the compiler's own choice of registers allows.)
 template <typename T, bool STAGED, bool SOFT, int LANES>
-__global__ void __launch_bounds__(LANES ? 128 : 256, LANES && STAGED ? 10 : 1)
+__global__ void __launch_bounds__(LANES ? 128 : 256, LANES && STAGED ? 10 : 0)
 rows_kernel(const __grid_constant__ ffcvb_cross_entropy_args a, const Deal deal) {
     constexpr bool WARP = LANES > 0;
     constexpr int N = kWide<T>, BATCH = STAGED ? 1 : 4; // packs that a thread has on their way
