@@ -454,7 +454,8 @@ void launch_rows(const ffcvb_cross_entropy_args &a, cudaStream_t stream) {
     how.numAttrs = 1;
     auto run = [&](auto kernel) {
         if (how.dynamicSmemBytes > 40 * 1024) {
-            cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)how.dynamicSmemBytes);
+            // (the limit is the kernel's, not the call's: another thread's call that needs less must not lower it)
+            cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMostPartBytes);
             cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
         }
         cudaLaunchKernelEx(&how, kernel, a, deal);

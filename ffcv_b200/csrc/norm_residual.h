@@ -365,10 +365,14 @@ template <typename T, typename F> void with_form(bool wide, bool post, Form form
         formed(Int<0>{});
 }
 
+// Shared memory that a CTA asks for at most, 213 KB (the general form backward, gated per sample, on 4096 odd columns of 32 bits), and room to the
+// 227 that it may have, the static part among them.  A kernel is allowed it once and for all: the limit is the kernel's, not the call's, and
+// another thread's call of it that needs less must not lower it in between.
+constexpr int kMostRoom = 226 * 1024;
 template <typename Kernel, typename... More>
 void launch(Kernel kernel, const Shape &shape, size_t room, cudaStream_t stream, const More &...more) {
     // (what a CTA may have without being asked includes the static part)
-    if (room > 40 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)room);
+    if (room > 40 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostRoom);
     cudaLaunchConfig_t how{};
     cudaLaunchAttribute with[2] = {};
     with[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
