@@ -71,6 +71,7 @@ class _Call:
                 self.kept.append(p)
             at[3 + k] = p.data_ptr()
         self.gate_kind, self.tokens = _gate_kind(x, gate)
+        self.tokens = max(1, self.tokens)  # (samples without tokens have no rows)
         if gate is not None and (N.require(gate, 'gate', x) != self.type or self.gate_kind is None):
             raise ValueError(f'gate must be {x.dtype}, with a row per row or per sample of {tuple(shape)}, not {gate.dtype} {tuple(gate.shape)}')
         at[0], x_stride = self.rows_of(x)
@@ -126,6 +127,8 @@ class _Call:
         dx = N.new_like(x) if of_x or (plain and of_h) else None
         dh = None if not of_h else dx if plain else N.new_like(x)
         dgate = N.new_like(self.gate) if of_gate else None
+        if of_gate and self.rows == 0:  # samples' gates may be there all the same
+            dgate.zero_()
         new, device = ch.empty, x.device
         params = [new(self.width, dtype=self.param_dtype, device=device) if of else None
                   for of in (of_weight, of_bias, of_post_weight, of_post_bias, of_scale)]
