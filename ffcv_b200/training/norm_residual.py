@@ -118,8 +118,6 @@ class _Call:
                 raise ValueError(f'{name} must be {x.dtype} {tuple(x.shape)}, not {g.dtype} {tuple(g.shape)}')
         if dz is not None and self.norm == 0:
             raise ValueError('dz goes with a norm')
-        if dz is None and self.norm:  # the kernel reads one where there is a norm
-            dz = ch.zeros_like(x, memory_format=ch.contiguous_format)
         dy_at, dy_stride = self.rows_of(dy)
         dz_at, dz_stride = self.rows_of(dz)
         of_x, of_h, of_weight, of_bias, of_post_weight, of_post_bias, of_gate, of_scale = wanted

@@ -34,3 +34,26 @@ def test_no_tokens(shape, gate, dtype):
     y, z = norm_residual(**leaves)
     (y.sum() + z.sum()).backward()
     assert all(t.grad is not None and not t.grad.any() for t in leaves.values())
+
+
+@pytest.mark.parametrize('post, gate', [(None, None), ('rms', 'sample'), ('layer', 'token')])
+@pytest.mark.parametrize('dtype, width', [(ch.float32, 96), (ch.bfloat16, 1024), (ch.float16, 333)], ids=str)
+def test_without_the_norms_gradient(dtype, width, post, gate):
+    """Where z had no use: as with a gradient of zeros, which nobody has to make."""
+    from ffcv_b200.training import norm_residual, norm_residual_backward, norm_residual_forward
+    v, dy, dz = make((3, 50, width), dtype, 'layer', post, gate, True)
+    how = {k: t for k, t in v.items() if k not in ('x', 'h')}
+    how.update(norm='layer', post_norm=post, eps=1e-6)
+    y, z, stats = norm_residual_forward(v['x'], v['h'], **how)
+    want = norm_residual_backward(dy, ch.zeros_like(dz), v['x'], v['h'], stats, **how)
+    got = norm_residual_backward(dy, None, v['x'], v['h'], stats, **how)
+    check(v, dy, ch.zeros_like(dz), 'layer', post, got=(y, z, got))
+    assert set(got) == set(want) and not got['weight'].any() and not got['bias'].any()
+    x, h = (t.clone().requires_grad_() for t in (v['x'], v['h']))
+    y, z = norm_residual(x, h)
+    ch.cuda.synchronize()
+    ch.cuda.reset_peak_memory_stats()
+    before = ch.cuda.memory_allocated()
+    dx, dh = ch.autograd.grad(y, (x, h), dy)
+    peak = ch.cuda.max_memory_allocated() - before
+    assert ch.equal(dx, dy) and ch.equal(dh, dy) and peak <= x.numel() * x.element_size() + 2048
