@@ -184,7 +184,8 @@ def norm_residual(x, h=None, *, norm='layer', weight=None, bias=None, post_norm=
     x : float32, float16 or bfloat16 CUDA tensor (..., tokens, width)
         The residual stream.
     h : the same, or None
-        The block's output.  Without it y is x.
+        The block's output.  Without it y is x.  A branch of another type than the stream's (of 16 bits beside 32, as automatic mixed
+        precision makes it): both are taken in the wider of the two.
     norm, post_norm : 'layer', 'rms' or None
         Norms over the last dimension, with ``weight`` and ``bias``, ``post_weight`` and ``post_bias`` (width,), each of
         which may be None.  Without ``norm`` z is None.
@@ -196,6 +197,9 @@ def norm_residual(x, h=None, *, norm='layer', weight=None, bias=None, post_norm=
 
     Everything is computed in 32 bits; y is rounded when it is stored, and z is made from what it was before.
     """
+    if all(isinstance(t, ch.Tensor) and t.dtype in N.TYPES for t in (x, h)) and h.dtype != x.dtype:
+        wide = ch.promote_types(x.dtype, h.dtype)
+        x, h = x.to(wide), h.to(wide)
     if gate is not None:
         gate = gate.to(x.dtype)
         if _gate_kind(x, gate)[0] is None:

@@ -57,3 +57,51 @@ def test_without_the_norms_gradient(dtype, width, post, gate):
     dx, dh = ch.autograd.grad(y, (x, h), dy)
     peak = ch.cuda.max_memory_allocated() - before
     assert ch.equal(dx, dy) and ch.equal(dh, dy) and peak <= x.numel() * x.element_size() + 2048
+
+
+@pytest.mark.parametrize('stream, branch', [(ch.float32, ch.bfloat16), (ch.float32, ch.float16), (ch.bfloat16, ch.float32), (ch.bfloat16, ch.float16)], ids=str)
+@pytest.mark.parametrize('gate', [None, 'sample'])
+def test_stream_and_branch_of_two_types(stream, branch, gate):
+    """As a sum takes them: in the wider type, with gradients in each one's own."""
+    from ffcv_b200.training import norm_residual
+    v, dy, dz = make((2, 9, 96), ch.float32, 'layer', 'rms', gate, True)
+    v['x'], v['h'] = v['x'].to(stream), v['h'].to(branch)
+    wide = ch.promote_types(stream, branch)
+    leaves = {k: t.clone().requires_grad_() for k, t in v.items()}
+    same = {k: (t.to(wide) if k in ('x', 'h') else t).detach().requires_grad_() for k, t in v.items()}
+    y, z = norm_residual(**leaves, post_norm='rms')
+    want = norm_residual(**same, post_norm='rms')
+    assert y.dtype == z.dtype == wide and ch.equal(y, want[0]) and ch.equal(z, want[1])
+    got = ch.autograd.grad((y, z), list(leaves.values()), (dy.to(wide), dz.to(wide)))
+    for k, g, w in zip(v, got, ch.autograd.grad(want, list(same.values()), (dy.to(wide), dz.to(wide)))):
+        assert g.dtype == v[k].dtype and ch.equal(g, w.to(g.dtype))
+
+
+def test_under_automatic_mixed_precision():
+    """A stream in 32 bits whose blocks' products are made in 16."""
+    from ffcv_b200.training import NormResidual
+    join, linear = NormResidual(64, scale=0.1).cuda(), ch.nn.Linear(64, 64).cuda()
+    x = ch.randn(2, 5, 64, device='cuda', requires_grad=True)
+    with ch.autocast('cuda', dtype=ch.bfloat16):
+        h = linear(x)
+        assert h.dtype == ch.bfloat16
+        y, z = join(x, h)
+        out = linear(z)
+    assert y.dtype == z.dtype == ch.float32 and out.dtype == ch.bfloat16
+    (out.float().square().mean() + y.mean()).backward()
+    assert all(p.grad is not None and bool(ch.isfinite(p.grad).all()) for p in (*join.parameters(), *linear.parameters(), x))
+
+
+def test_other_types_are_refused_as_before():
+    from ffcv_b200.training import norm_residual
+    x = ch.randn(2, 3, 16, device='cuda')
+    for a, b in ((x, x.double()), (x.double(), x), (x, x.int())):
+        with pytest.raises(TypeError):
+            norm_residual(a, b)
+    with pytest.raises(ValueError):
+        norm_residual(x, x.half()[:1])
+    for bad in (dict(h=[1.0]), dict(h=1.0)):
+        with pytest.raises(TypeError, match='not a tensor'):
+            norm_residual(x, **bad)
+    with pytest.raises(TypeError, match='not a tensor'):
+        norm_residual([1.0], x)
