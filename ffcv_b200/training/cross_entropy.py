@@ -101,11 +101,14 @@ class _CrossEntropy(ch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, call, reduction):
         n = logits.shape[0]
-        rows, stats = (ch.empty(k, dtype=ch.float32, device=logits.device) for k in (n, 2 * n))
         ctx.per_row = reduction == 'none'
-        # (a tensor of its own: a part of another one could not be changed in place)
-        loss = rows if ctx.per_row else ch.empty((), dtype=ch.float32, device=logits.device)
-        call.run(None, rows.data_ptr(), 0 if ctx.per_row else loss.data_ptr(), stats)
+        # the result is a tensor of its own (a part of another one could not be changed in place); losses of rows that are not are behind the statistics
+        loss = ch.empty(n if ctx.per_row else (), dtype=ch.float32, device=logits.device)
+        stats = ch.empty(2 * n if ctx.per_row else 3 * n, dtype=ch.float32, device=logits.device)
+        if ctx.per_row:
+            call.run(None, loss.data_ptr(), 0, stats)
+        else:
+            call.run(None, stats.data_ptr() + 8 * n, loss.data_ptr(), stats)
         ctx.save_for_backward(call.logits, call.target, stats)
         call.logits = call.target = None  # (autograd keeps them, and sees to it that nobody changes them)
         ctx.call = call
