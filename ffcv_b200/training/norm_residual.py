@@ -197,7 +197,7 @@ def norm_residual(x, h=None, *, norm='layer', weight=None, bias=None, post_norm=
 
     Everything is computed in 32 bits; y is rounded when it is stored, and z is made from what it was before.
     """
-    if all(isinstance(t, ch.Tensor) and t.dtype in N.TYPES for t in (x, h)) and h.dtype != x.dtype:
+    if isinstance(h, ch.Tensor) and isinstance(x, ch.Tensor) and h.dtype is not x.dtype and h.dtype in N.TYPES and x.dtype in N.TYPES:
         wide = ch.promote_types(x.dtype, h.dtype)
         x, h = x.to(wide), h.to(wide)
     if gate is not None:

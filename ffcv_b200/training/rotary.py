@@ -37,12 +37,12 @@ class _Rotate(ch.autograd.Function):
     @ch.autograd.function.once_differentiable
     def backward(ctx, dq, dk=None):
         positions, = ctx.saved_tensors
-        wanted = [g if of else None for g, of in zip((dq, dk), ctx.needs_input_grad[2:])]
-        given = [g for g in wanted if g is not None]
-        if not given:
-            return (None,) * 4
-        turned = ctx.rotary._run(given[0], given[1] if len(given) > 1 else None, *ctx.rotary._where(given[0], positions), True, False)
-        return None, None, *(None if g is None else turned[g is not given[0]] for g in wanted)
+        run, where = ctx.rotary._run, ctx.rotary._where(dq, positions)
+        _, _, of_q, of_k = ctx.needs_input_grad
+        if not of_q:
+            return None, None, None, run(dk, None, *where, True, False)[0] if of_k else None
+        dq, dk = run(dq, dk if of_k else None, *where, True, False)
+        return None, None, dq, dk
 
 
 class RotaryPositions(ch.nn.Module):
