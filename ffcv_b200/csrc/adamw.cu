@@ -438,6 +438,36 @@ squares_kernel(const __grid_constant__ Launch<MOST> a) {
         a.partial[which] = sum;
     }
 }
+// Masters of a chunk's weights that have been written to: where a weight is not its master rounded, it becomes the master.  A tensor's
+// place in the gradients is not 0 where it is to be looked at.  (290 tensors, 408 M bf16 values: 357 us, 374 at the rate
+// of a copy; the check of a loaded state by elementwise operations took 9.5 ms.)
+template <typename T, int MOST>
+__global__ void __launch_bounds__(kThreads)
+masters_kernel(const __grid_constant__ Launch<MOST> a) {
+    wait_for_previous();
+    let_next_begin();
+    const Chunk chunk = a.chunks[blockIdx.x];
+    const int local = chunk.tensor - a.first;
+    if (!a.grads[local]) return;
+    const Tensor tensor = a.tensors[local];
+    const T *param = reinterpret_cast<const T *>(tensor.param);
+    float *const master = a.master + tensor.start;
+    const long long n = tensor.numel, first = (long long)chunk.index * a.chunk;
+    const bool whole = (reinterpret_cast<uintptr_t>(param) & (4 * sizeof(T) - 1)) == 0 && first + a.chunk <= n;
+    for (int k = threadIdx.x; k < a.chunk / 4 && first + k * 4 < n; k += kThreads) {
+        const long long at = first + k * 4;
+        const float4 w = (whole ? load4<true>(param, at, n) : load4<false>(param, at, n)).get();
+        float4 m = *reinterpret_cast<const float4 *>(master + at); // (behind a tensor's last value both are 0)
+        auto keeps = [](float own, float weight) { return to_float(from_float<T>(own)) == weight; };
+        if (keeps(m.x, w.x) && keeps(m.y, w.y) && keeps(m.z, w.z) && keeps(m.w, w.w)) continue;
+        if (!keeps(m.x, w.x)) m.x = w.x;
+        if (!keeps(m.y, w.y)) m.y = w.y;
+        if (!keeps(m.z, w.z)) m.z = w.z;
+        if (!keeps(m.w, w.w)) m.w = w.w;
+        *reinterpret_cast<float4 *>(master + at) = m;
+    }
+}
+
 __global__ void __launch_bounds__(1024)
 norm_kernel(const float *__restrict__ partial, long long n, float *norm) {
     __shared__ double s_sum[32];
@@ -466,9 +496,11 @@ struct Tensors { // HOST
     long long values, chunks, chunk; // of all, and values of one chunk
 };
 
+enum Pass { kSquares, kStep, kMasters };
+
 // Every launch takes as many tensors as its arguments have room for.
 template <typename T, int MOST>
-void launch_all(const ffcvb_adamw_args &args, const Tensors &t, bool squares, cudaStream_t st) {
+void launch_all(const ffcvb_adamw_args &args, const Tensors &t, Pass pass, cudaStream_t st) {
     const Tensor *tensors = static_cast<const Tensor *>(args.tensors);
     const Chunk *chunks = reinterpret_cast<const Chunk *>(tensors + args.n_tensors);
     long long at = 0; // chunk
@@ -482,7 +514,7 @@ void launch_all(const ffcvb_adamw_args &args, const Tensors &t, bool squares, cu
             const int i = first + n;
             a.grads[n] = reinterpret_cast<const void *>(t.grads[i]);
             a.set[n] = 0;
-            if (a.grads[n] && !squares) {
+            if (a.grads[n] && pass == kStep) {
                 int s = 0;
                 while (s < sets && (group[s] != t.group_of[i] || steps[s] != t.steps[i])) s++;
                 if (s == sets) {
@@ -518,14 +550,25 @@ void launch_all(const ffcvb_adamw_args &args, const Tensors &t, bool squares, cu
         a.norm = args.max_norm > 0.0 ? args.norm : nullptr;
         a.max_norm = (float)args.max_norm;
         a.partial = static_cast<float *>(args.workspace) + at;
-        if (count > 0 && (any || squares)) {
-            const bool long_ones = squares || staged(args.bits, t.values);
-            auto step = args.bits == 32 ? step_kernel<T, 32, MOST, false> : long_ones ? step_kernel<T, 8, MOST, true> : step_kernel<T, 8, MOST, false>;
-            launch_early(squares ? squares_kernel<T, MOST> : step, (unsigned)(long_ones ? count : count * (t.chunk / kShort)), kThreads, 0, st, a);
+        if (count > 0 && (any || pass == kSquares)) {
+            const bool whole_chunks = pass != kStep || staged(args.bits, t.values);
+            auto step = args.bits == 32 ? step_kernel<T, 32, MOST, false> : whole_chunks ? step_kernel<T, 8, MOST, true> : step_kernel<T, 8, MOST, false>;
+            launch_early(pass == kSquares ? squares_kernel<T, MOST> : pass == kMasters ? masters_kernel<T, MOST> : step,
+                         (unsigned)(whole_chunks ? count : count * (t.chunk / kShort)), kThreads, 0, st, a);
         }
         first += n;
         at += count;
     }
+}
+
+void launch_pass(const ffcvb_adamw_args &a, const Tensors &t, Pass pass, cudaStream_t st) {
+    with_type(a.type, [&](auto zero) {
+        using T = decltype(zero);
+        if (a.n_tensors <= 64)
+            launch_all<T, 64>(a, t, pass, st);
+        else
+            launch_all<T, 1024>(a, t, pass, st);
+    });
 }
 
 } // namespace
@@ -588,21 +631,27 @@ int ffcvb_adamw_step(const ffcvb_adamw_args *args, const int64_t *numel, int64_t
     if (capture != cudaStreamCaptureStatusNone)
         return training_fail(FFCVB_E_ARG, "ffcvb_adamw_step: a step cannot be captured: its number, rates and gradients' addresses are its kernels' arguments");
     for (int32_t i = 0; i < a.n_tensors; i++) steps[i] += grads[i] != 0;
-    with_type(a.type, [&](auto zero) {
-        using T = decltype(zero);
-        auto all = [&](bool squares) {
-            if (a.n_tensors <= 64)
-                launch_all<T, 64>(a, t, squares, st);
-            else
-                launch_all<T, 1024>(a, t, squares, st);
-        };
-        if (a.max_norm > 0.0) {
-            all(true);
-            launch_early(norm_kernel, 1, 1024, 0, st, static_cast<const float *>(a.workspace), t.chunks, a.norm);
-        }
-        all(false);
-    });
+    if (a.max_norm > 0.0) {
+        launch_pass(a, t, kSquares, st);
+        launch_early(norm_kernel, 1, 1024, 0, st, static_cast<const float *>(a.workspace), t.chunks, a.norm);
+    }
+    launch_pass(a, t, kStep, st);
     return launched("ffcvb_adamw_step");
+}
+
+int ffcvb_adamw_masters(const ffcvb_adamw_args *args, const int64_t *numel, const uint64_t *which, void *stream) {
+    if (!args || args->n_tensors < 0) return training_fail(FFCVB_E_ARG, "ffcvb_adamw_masters: no arguments");
+    const ffcvb_adamw_args &a = *args;
+    if (a.n_tensors == 0) return FFCVB_OK;
+    if (!numel || !which || !a.tensors || !a.master || (a.type != FFCVB_TYPE_F16 && a.type != FFCVB_TYPE_BF16))
+        return training_fail(FFCVB_E_ARG, "ffcvb_adamw_masters: bad argument");
+    Tensors t{numel, which, nullptr, nullptr, nullptr, 0, 0, chunk_size(a.n_tensors, numel)};
+    for (int32_t i = 0; i < a.n_tensors; i++) t.chunks += chunks_of(numel[i], t.chunk);
+    if (t.chunks > 0x7fffffff) return training_fail(FFCVB_E_LIMIT, "ffcvb_adamw_masters: too many values");
+    OnDevice here(a.device);
+    if (!here.ok()) return training_fail(FFCVB_E_NODEVICE, "ffcvb_adamw_masters: no device %d", a.device);
+    launch_pass(a, t, kMasters, static_cast<cudaStream_t>(stream));
+    return launched("ffcvb_adamw_masters");
 }
 
 } // extern "C"

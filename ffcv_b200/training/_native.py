@@ -32,6 +32,8 @@ lib.ffcvb_adamw_table.argtypes = [c_int32, c_void_p, c_void_p, c_void_p]
 lib.ffcvb_adamw_table.restype = c_int
 lib.ffcvb_adamw_step.argtypes = [c_char_p, c_void_p, c_void_p, c_void_p, c_char_p, c_char_p, c_int32, c_void_p]
 lib.ffcvb_adamw_step.restype = c_int
+lib.ffcvb_adamw_masters.argtypes = [c_char_p, c_void_p, c_char_p, c_void_p]
+lib.ffcvb_adamw_masters.restype = c_int
 
 
 def check(rc):

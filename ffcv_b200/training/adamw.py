@@ -138,15 +138,38 @@ class AdamW(ch.optim.Optimizer):
             self._seen = [version for version, _ in both], [place for _, place in both]
         self._host = self._numel.ctypes.data, self._steps.ctypes.data, self._group_of.ctypes.data
 
-    @ch.no_grad()
-    def masters_from_parameters(self, only=None):
+    def masters_from_parameters(self):
         """Makes masters follow 16-bit parameters that have been written to: where a value is not its master rounded, it becomes the
-        master.  ``only``: numbers of parameters, in the groups' order; default: all."""
-        for i in range(len(self._params)) if only is None and self.master is not None else only or ():
-            p = self._params[i].detach()
-            if p.numel():
-                master = self.state[self._params[i]]['master']
-                master.copy_(ch.where(master.to(p.dtype) == p, master, p.float()))
+        master."""
+        if self.master is not None:
+            self._place()
+            self._follow([1] * len(self._params))
+
+    def _follow(self, which):
+        n = len(self._params)
+        N.check(N.lib.ffcvb_adamw_masters(self._args(), self._host[0], struct.pack(f'={n}Q', *which), N.raw_stream(self._params[0].get_device())))
+
+    def _place(self):
+        """Addresses of the parameters, which the table in device memory has too."""
+        params = self._params
+        if not self._layouts.check(*params):
+            self._check_params()
+            if any(_order(p) != _order(self.state[p]['exp_avg']) for p in params):
+                self._lay_out()
+            self._layouts = N.layouts(params)
+        at = list(map(_address, params))
+        if at != self._at:  # the first step, or parameters that have moved
+            host = np.empty(max(1, self._table_size), np.uint8)
+            where = np.array(at, np.uint64)
+            N.check(N.lib.ffcvb_adamw_table(len(params), self._numel.ctypes.data, where.ctypes.data, host.ctypes.data))
+            self._table.copy_(ch.from_numpy(host[:self._table_size]))
+            self._at = at
+        return at
+
+    def _args(self):
+        return N.ADAMW.pack(self._table.data_ptr(), self.exp_avg.data_ptr(), self.exp_avg_sq.data_ptr(), N.ptr(self.scales),
+                            N.ptr(self.master), N.ptr(self.grad_norm), N.ptr(self._workspace), self.seed, self._params[0].get_device(),
+                            N.TYPES[self._dtype], self.state_bits, len(self._params), self.max_grad_norm or 0.0)
 
     def _take(self, own, was):
         """A parameter's state from another of the same shape, whatever order in memory either is in."""
@@ -174,26 +197,20 @@ class AdamW(ch.optim.Optimizer):
         return g if g.stride() == p.stride() else ch.empty_like(p, requires_grad=False).copy_(g.detach())
 
     def step(self, closure=None):
-        params, n = self._params, len(self._params)
         if N.capturing():
             raise RuntimeError('a step of AdamW cannot be captured in a graph: a replay would repeat its number, rates and gradients\' addresses')
         loss = None
         if closure is not None:
             with ch.enable_grad():
                 loss = closure()
+        params, n = self._params, len(self._params)
         if not params:
             return loss
-        if not self._layouts.check(*params):
-            self._check_params()
-            if any(_order(p) != _order(self.state[p]['exp_avg']) for p in params):
-                self._lay_out()
-            self._layouts = N.layouts(params)
-        dtype, index = self._dtype, params[0].get_device()
-        at = list(map(_address, params))
+        at = self._place()
         if self.master is not None:
             seen = [p._version for p in params], at
             if seen != self._seen:
-                self.masters_from_parameters([i for i, (now, then) in enumerate(zip(zip(*seen), zip(*self._seen))) if now != then])
+                self._follow([now != then for now, then in zip(zip(*seen), zip(*self._seen))])
         # addresses of gradients, 0 without one
         grads, kept = [p.grad for p in params], None
         if self._grad_layouts is not None and self._grad_layouts.check(*grads):
@@ -202,20 +219,12 @@ class AdamW(ch.optim.Optimizer):
             kept = [None if g is None else self._as_parameter(p, g) for p, g in zip(params, grads)]
             grads_at = [N.ptr(g) for g in kept]
             self._grad_layouts = N.layouts(kept) if all(g is not None and g is own for g, own in zip(kept, grads)) else None
-        if at != self._at:  # the first step, or parameters that have moved
-            host = np.empty(max(1, self._table_size), np.uint8)
-            where = np.array(at, np.uint64)
-            N.check(N.lib.ffcvb_adamw_table(n, self._numel.ctypes.data, where.ctypes.data, host.ctypes.data))
-            self._table.copy_(ch.from_numpy(host[:self._table_size]))
-            self._at = at
         groups = b''
         for group in self.param_groups:
             self._check_group(group)
             groups += N.ADAMW_GROUP.pack(group['lr'], *group['betas'], group['eps'], group['weight_decay'])
-        args = N.ADAMW.pack(self._table.data_ptr(), self.exp_avg.data_ptr(), self.exp_avg_sq.data_ptr(), N.ptr(self.scales),
-                            N.ptr(self.master), N.ptr(self.grad_norm), N.ptr(self._workspace), self.seed, index,
-                            N.TYPES[dtype], self.state_bits, n, self.max_grad_norm or 0.0)
-        N.check(N.lib.ffcvb_adamw_step(args, *self._host, struct.pack(f'={n}Q', *grads_at), groups, len(self.param_groups), N.raw_stream(index)))
+        N.check(N.lib.ffcvb_adamw_step(self._args(), *self._host, struct.pack(f'={n}Q', *grads_at), groups, len(self.param_groups),
+                                       N.raw_stream(params[0].get_device())))
         del kept
         # (a later backward pass that needs what they were says so)
         ch.autograd.graph.increment_version(params if all(grads_at) else [p for p, g in zip(params, grads_at) if g])

@@ -423,6 +423,10 @@ int ffcvb_adamw_table(int32_t n, const int64_t *numel, const uint64_t *params, v
 int ffcvb_adamw_step(const ffcvb_adamw_args *args, const int64_t *numel, int64_t *steps, const int32_t *group_of,
                      const uint64_t *grads, const ffcvb_adamw_group *groups, int32_t n_groups, void *stream);
 
+/* Masters of tensors i with which[i] != 0 (HOST array) whose 16-bit weights have been written to: where a weight is not its master
+ * rounded, it becomes the master. */
+int ffcvb_adamw_masters(const ffcvb_adamw_args *args, const int64_t *numel, const uint64_t *which, void *stream);
+
 /* ---- decode without allocating -----------------------------------------------------------
  * No counterpart in the reference.  For callers that must not allocate GPU memory while they
  * run: a process that handed all device memory to its own pool at start-up, a plugin living

@@ -48,6 +48,17 @@ class HostLibrary:
                 self.moment(where, scales_at, k, start, count, bits, new)
         return 0
 
+    def ffcvb_adamw_masters(self, args, numel, which, stream):
+        table, _, _, _, master_at, _, _, _, _, kind, _, n, _ = self.native.ADAMW.unpack(args)
+        which, tensors = struct.unpack(f'={n}Q', which), at(table, 3 * n, np.int64).reshape(n, 3)
+        dtype = (None, ch.float16, ch.bfloat16)[kind]
+        for (param, count, start), asked in zip(tensors.tolist(), which):
+            if asked:
+                w, master = self.values(param, count, kind), at(master_at + 4 * start, count, np.float32)
+                rounded = ch.from_numpy(master.copy()).to(dtype).float().numpy()
+                master[:] = np.where(rounded == w, master, w)
+        return 0
+
     @staticmethod
     def values(address, n, kind, new=None):
         if kind == 0:

@@ -189,3 +189,51 @@ def test_copies_go_on_by_themselves(bits, dtype, how):
         for a, b in ((opt.exp_avg, other.exp_avg), (opt.exp_avg_sq, other.exp_avg_sq), (opt.master, other.master), (opt.scales, other.scales)):
             assert a is b is None or (a.data_ptr() != b.data_ptr() and ch.equal(a.view(ch.uint8), b.view(ch.uint8)))
         assert math.isclose(float(opt.grad_norm), float(other.grad_norm))
+
+
+@pytest.mark.parametrize('dtype', [ch.bfloat16, ch.float16], ids=str)
+@pytest.mark.parametrize('bits', [8, 32])
+@pytest.mark.parametrize('more', [0, 70, 1100])
+def test_masters_follow_parameters(dtype, bits, more):
+    """Against the rule in plain operations: tensors of all sizes, some at odd places, in more than one launch, some of them written to, with
+    infinities and what is no number; the others' masters are not touched."""
+    from ffcv_b200.training import AdamW
+    gen = ch.Generator('cuda').manual_seed(3)
+    r = lambda *s: ch.randn(s, generator=gen, device='cuda')  # noqa: E731
+    flat = r(40000).to(dtype)
+    params = [ch.nn.Parameter(r(*s).to(dtype)) for s in ((1,), (255,), (257,), (8192,), (8193,), (70, 301), (0,), (300000,))]
+    params += [ch.nn.Parameter(flat[1:20002]), ch.nn.Parameter(flat[20004:20007]), ch.nn.Parameter(r(9, 40).to(dtype).t())]
+    params += [ch.nn.Parameter(r(3 + i % 5).to(dtype)) for i in range(more)]
+    opt = AdamW(params, **HYPER, state_bits=bits)
+    for p in params:
+        p.grad = r(*p.shape).to(dtype)
+    opt.step()
+    want = [opt.state[p]['master'].clone() for p in params]
+    for i, p in enumerate(params):
+        if i % 3 == 0 or i == 8:  # (cut out of one tensor, the two odd ones share a version; what has not been written stays all the same)
+            new = p.detach().clone()
+            change = ch.rand(p.shape, generator=gen, device='cuda') < 0.3
+            new[change] = (r(*p.shape) * 4).to(dtype)[change]
+            if p.numel() > 50:
+                new.view(-1)[5:8] = ch.tensor([math.inf, -0.0, math.nan], device='cuda', dtype=dtype) if new.is_contiguous() else new.view(-1)[5:8]
+            want[i] = ch.where(new == p.detach(), want[i], new.float())
+            with ch.no_grad():
+                p.copy_(new)
+    values = [p.detach().clone() for p in params]
+    for group in opt.param_groups:
+        group['lr'] = 0.0
+    padding = opt.master.clone()
+    opt.step()
+    for p, w, v in zip(params, want, values):
+        kept = ~ch.isnan(w)
+        assert ch.equal(ch.isnan(opt.state[p]['master']), ~kept) and ch.equal(opt.state[p]['master'][kept], w[kept])
+        assert ch.equal(p.detach()[kept], v[kept])
+    starts = opt._start.tolist() + [opt.master.numel()]
+    for i, p in enumerate(params):  # behind a tensor's last value there are zeros
+        assert not opt.master[starts[i] + p.numel():starts[i + 1]].any() and not padding[starts[i] + p.numel():starts[i + 1]].any()
+    for p in params:  # behind autograd's back, and asked for
+        p.data.clamp_(-0.5, 0.5)
+    opt.masters_from_parameters()
+    for p in params:
+        master, finite = opt.state[p]['master'], ~ch.isnan(p.detach())
+        assert ch.equal(master.to(dtype)[finite], p.detach()[finite])
