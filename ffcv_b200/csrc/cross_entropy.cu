@@ -8,7 +8,7 @@
 // the row crosses HBM once each way, and several CTAs per SM load, compute and store at different times.
 //
 // What bounds it: two exponentials per logit and the instructions around them; 8192 x 21841 bf16 logits take 129 us, 109 at the rate
-// of a copy.
+// of a copy; with smoothing 130, with probabilities in 32 bits, which both passes read, 326.
 #include "training.h"
 #include "two.h"
 

@@ -7,9 +7,9 @@
 // again from x and h, in 32 bits: its rounded copy would cost the weights' gradients their last digits.
 // Sums over columns of the gradient go through one partial row per CTA, added up in a fixed order by a second kernel.
 //
-// Reading and writing bounds it where rows are whole packs: 50432 bf16 rows of 768 with norm, branch and scale take 48 us
-// forward and 74 backward (47 and 71 at the rate of a copy), and 8 for the columns' sums.  With an inner norm and gates
-// (147520 rows of 1024) 218 and 310 us (184 and 276), where arithmetic and barriers between a row's sums show.
+// Reading and writing bounds it where rows are whole packs: 50432 bf16 rows of 768 with norm, branch and scale take 137 us
+// forward and backward (118 at the rate of a copy), 8 of them for the columns' sums.  With an inner norm and gates
+// (147520 rows of 1024) 532 us (461), where arithmetic and barriers between a row's sums show.
 #include "norm_residual.h"
 
 namespace ffcvb {

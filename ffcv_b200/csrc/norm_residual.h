@@ -334,8 +334,10 @@ struct Partials {
 constexpr int kColumns = 5;
 
 // What is known of a call when its kernel is compiled: nothing; or that there are a branch, a norm behind it and (backward) gradients of both
-// results, and that the stream's is wanted, with no gate, one per sample or one per token.  (256 x 197 rows of 768 bf16 values, plain:
-// 48 and 74 us; as any call 62 and 96.)
+// results, and that the stream's is wanted, with no gate, one per sample or one per token.  (Forward and backward, bf16, as compiled and as
+// any call: 256 x 197 rows of 768, plain, 136 and 142 us, without a scale 124 and 137; 64 x 577 rows of 1024 with a gate per token 196 and
+// 214, an inner norm besides 179 and 196, a gate per sample and an inner norm 150 and 190; 128 x 197 rows of 387 values, one by one, plain,
+// 63 and 85, of 775 108 and 152.)
 enum Form { kAny, kPlain, kGated, kToken };
 inline Form form_of(const Args &a, bool backward) {
     if (!a.h || a.norm == FFCVB_NORM_NONE || (backward && (!a.dy || !a.dz || !a.dx))) return kAny;

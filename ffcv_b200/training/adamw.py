@@ -26,6 +26,7 @@ class AdamW(ch.optim.Optimizer):
     max_grad_norm : float
         Gradients are scaled down together so that their norm is at most this.  Where the norm is not finite, the step
         changes nothing (but counts).  ``grad_norm`` holds the last step's norm, on the GPU.
+        A value that is not finite, without such a bound, makes its block of 256 values none with 8-bit moments, and itself with 32.
     seed : int
         Of the stochastic rounding: the same seed, steps and gradients give the same weights.
 
