@@ -195,7 +195,7 @@ class AdamW(ch.optim.Optimizer):
             raise TypeError(f'gradients must be dense, of the parameters\' type and on their GPU, not {g.dtype} {g.layout} on {g.device}')
         if g.shape != p.shape:
             raise ValueError(f'a parameter of shape {tuple(p.shape)} has a gradient of shape {tuple(g.shape)}')
-        return g if g.stride() == p.stride() else ch.empty_like(p, requires_grad=False).copy_(g.detach())
+        return g if _order(g) == _order(p) else ch.empty_like(p, requires_grad=False).copy_(g.detach())
 
     def step(self, closure=None):
         if N.capturing():

@@ -16,10 +16,11 @@ def at(address, n, kind):
 
 
 class HostLibrary:
-    """Stands for ``libffcv_b200.so``: the host's functions are its own, a step is made here.  ``steps`` counts them."""
+    """Stands for ``libffcv_b200.so``: the host's functions are its own, a step is made here.  ``steps`` counts them, ``grads`` has the last
+    one's addresses of gradients."""
 
     def __init__(self, lib, native):
-        self.lib, self.native, self.steps = lib, native, 0
+        self.lib, self.native, self.steps, self.grads = lib, native, 0, None
 
     def __getattr__(self, name):
         return getattr(self.lib, name)
@@ -28,6 +29,7 @@ class HostLibrary:
         self.steps += 1
         table, m_at, v_at, scales_at, master_at, norm_at, _, seed, _, kind, bits, n, max_norm = self.native.ADAMW.unpack(args)
         assert max_norm == 0.0
+        self.grads = list(struct.unpack(f'={n}Q', grads))
         grads, numel, steps, group_of = struct.unpack(f'={n}Q', grads), at(numel, n, np.int64), at(steps, n, np.int64), at(group_of, n, np.int32)
         tensors = at(table, 3 * n, np.int64).reshape(n, 3)
         for i, (param, count, start) in enumerate(tensors.tolist()):

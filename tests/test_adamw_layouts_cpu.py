@@ -216,3 +216,27 @@ def test_state_saved_in_another_order(monkeypatch, bits, dtype):
             assert bool(((now - was).abs() <= own * was.abs() + most * was.abs().max()).all())
     if dtype != ch.float32:
         assert ch.equal(opt.state[p]['master'], other.state[q]['master'])
+
+
+def test_gradients_are_read_where_they_lie(monkeypatch):
+    """Also where dimensions of one value have other strides, as those of a convolution of 1 x 1 in another memory format; only another
+    order of values is copied, and sparse ones are refused."""
+    AdamW, lib = on_the_host(monkeypatch)
+    params = [ch.nn.Parameter(ch.randn(s)) for s in ((8, 4, 1, 1), (5, 1), (6, 7))]
+    opt, want = AdamW(params, **HYPER), [Formula(p) for p in params]
+    for step in range(3):
+        for p, w in zip(params, want):
+            p.grad = ch.randn(p.shape)
+            w.step(p.grad)
+        params[0].grad = params[0].grad.to(memory_format=ch.channels_last)
+        params[1].grad = ch.as_strided(params[1].grad, (5, 1), (1, 9))
+        if step == 2:
+            params[2].grad = params[2].grad.t().contiguous().t()
+        opt.step()
+        same = [a == p.grad.data_ptr() for a, p in zip(lib.grads, params)]
+        assert same == [True, True, step < 2] and (opt._grad_layouts is not None) == (step < 2)
+    assert all(w.near(p.detach()) for w, p in zip(want, params))
+    params[2].grad = ch.randn(6, 7).to_sparse()
+    with pytest.raises(TypeError, match='dense'):
+        opt.step()
+    assert lib.steps == 3
