@@ -9,57 +9,13 @@
 //
 // What bounds it: two exponentials per logit and the instructions around them; 8192 x 21841 bf16 logits take 129 us, 109 at the rate
 // of a copy; with smoothing 130, with probabilities in 32 bits, which both passes read, 326.
-#include "training.h"
-#include "two.h"
+#include "losses.h"
 
 #include <type_traits>
 
 namespace ffcvb {
 
 namespace {
-
-// (Differences are taken before the factor: a row masked with the type's lowest value has no product with it.)
-constexpr float kLog2e = 1.4426950408889634f;
-__device__ __forceinline__ float exp2_of(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ float exp_of(float x) { return exp2_of(x * kLog2e); }
-
-// What a row's target is besides probabilities per class: at most two classes with their weights, and the same
-// `flat` for all.
-struct Picks {
-    long long label[2];
-    float weight[2];
-    float flat;
-    float total;  // S
-    bool ignored, bad;
-};
-
-__device__ __forceinline__ Picks picks_of(const ffcvb_cross_entropy_args &a, long long row) {
-    Picks p{{-1, -1}, {0.0f, 0.0f}, a.smoothing / (float)a.classes, 0.0f, false, false};
-    const float sure = 1.0f - a.smoothing;
-    if (a.target_kind == FFCVB_TARGET_LABELS) {
-        p.label[0] = static_cast<const int64_t *>(a.target)[row * a.target_stride];
-        p.weight[0] = sure;
-        p.ignored = a.has_ignore && p.label[0] == a.ignore_index;
-        p.bad = p.label[0] < 0 || p.label[0] >= a.classes;
-        p.total = sure + a.smoothing;
-    } else if (a.target_kind == FFCVB_TARGET_MIXED) {
-        const float *m = static_cast<const float *>(a.target) + row * a.target_stride;
-        const float l0 = m[0], l1 = m[1], lam = m[2];
-        p.bad = !(l0 >= 0.0f && l0 < (float)a.classes && l1 >= 0.0f && l1 < (float)a.classes);
-        if (!p.bad) {
-            p.label[0] = (long long)l0;
-            p.label[1] = (long long)l1;
-        }
-        p.weight[0] = sure * lam;
-        p.weight[1] = sure * (1.0f - lam);
-        p.total = p.weight[0] + p.weight[1] + a.smoothing;
-    }
-    return p;
-}
 
 // N probabilities from class c of a row on.
 template <int N>
@@ -79,15 +35,10 @@ __device__ __forceinline__ void probabilities(float (&p)[N], const ffcvb_cross_e
                                                  : to_float(static_cast<const __nv_bfloat16 *>(a.target)[at + j]);
 }
 
-__device__ __forceinline__ void copy16(uint32_t to, const void *from) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
-}
-
 // The largest logit of a part of a row, at least kLowest, and the sum of exponentials relative to it; with targets besides labels also the
 // sum of targets times logits, which are relative to it too, and the targets' sum.  (Where all logits are -inf the sum is 0: no difference
 // here is that of two infinities of one sign, unless a logit is +inf.)  Relative sums stay finite where several logits are the type's
 // lowest value, and keep the digits of logits that are all far from zero.
-constexpr float kLowest = -3.402823466e38f;
 struct Found {
     float top, sum, dot, mass;
     // what a dot relative to `from` has more when it is relative to `to`, the larger (kept finite: there may be no mass yet)
@@ -506,6 +457,13 @@ void launch_rows(const ffcvb_cross_entropy_args &a, cudaStream_t stream) {
 
 } // namespace
 
+void launch_mean(const float *row_loss, int64_t rows, const float *counted, bool mean, float *loss, cudaStream_t stream) {
+    launch_early(mean_kernel, 1, 1024, 0, stream, row_loss, rows, counted, mean, loss);
+}
+void launch_count(const void *labels, int64_t rows, int64_t stride, int64_t ignore, float *counted, cudaStream_t stream) {
+    launch_early(count_kernel, 1, 1024, 0, stream, static_cast<const int64_t *>(labels), rows, stride, ignore, counted);
+}
+
 } // namespace ffcvb
 
 using namespace ffcvb;
@@ -524,8 +482,8 @@ extern "C" int ffcvb_cross_entropy(const ffcvb_cross_entropy_args *args, void *s
     OnDevice here(a.device);
     if (!here.ok()) return training_fail(FFCVB_E_NODEVICE, "ffcvb_cross_entropy: no device %d", a.device);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (needs_count) launch_early(count_kernel, 1, 1024, 0, st, static_cast<const int64_t *>(a.target), a.rows, a.target_stride, a.ignore_index, a.counted);
+    if (needs_count) launch_count(a.target, a.rows, a.target_stride, a.ignore_index, a.counted, st);
     if (a.rows > 0) with_type(a.type, [&](auto zero) { launch_rows<decltype(zero)>(a, st); });
-    if (a.loss && !a.from_stats) launch_early(mean_kernel, 1, 1024, 0, st, a.row_loss, a.rows, needs_count ? a.counted : nullptr, a.mean, a.loss);
+    if (a.loss && !a.from_stats) launch_mean(a.row_loss, a.rows, needs_count ? a.counted : nullptr, a.mean, a.loss, st);
     return launched("ffcvb_cross_entropy");
 }

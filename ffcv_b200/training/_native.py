@@ -11,6 +11,7 @@ from ..libffcv import lib
 TYPES = {ch.float32: 0, ch.float16: 1, ch.bfloat16: 2}
 
 CROSS_ENTROPY = struct.Struct('=8Q6q8i2f')
+LINEAR_CROSS_ENTROPY = struct.Struct('=11Q7q8i2f')
 NORM_RESIDUAL = struct.Struct('=21Q8q6i2f')
 ROTARY = struct.Struct('=7Q19q6ifi')
 ADAMW = struct.Struct('=7Qq4id')
@@ -26,6 +27,10 @@ for _name in ('ffcvb_cross_entropy', 'ffcvb_norm_residual', 'ffcvb_norm_residual
 lib.ffcvb_norm_residual_backward.argtypes = [c_char_p, c_void_p, c_void_p]
 lib.ffcvb_norm_residual_workspace.argtypes = [c_char_p]
 lib.ffcvb_norm_residual_workspace.restype = c_int64
+lib.ffcvb_linear_cross_entropy.argtypes = [c_char_p, c_void_p, c_void_p]
+lib.ffcvb_linear_cross_entropy.restype = c_int
+lib.ffcvb_linear_cross_entropy_workspace.argtypes = [c_char_p]
+lib.ffcvb_linear_cross_entropy_workspace.restype = c_int64
 lib.ffcvb_adamw_layout.argtypes = [c_int32, c_void_p, c_void_p, c_void_p]
 lib.ffcvb_adamw_layout.restype = c_int64
 lib.ffcvb_adamw_table.argtypes = [c_int32, c_void_p, c_void_p, c_void_p]

@@ -344,6 +344,28 @@ typedef struct {
 } ffcvb_cross_entropy_args;
 int ffcvb_cross_entropy(const ffcvb_cross_entropy_args *args, void *stream);
 
+/* The same loss of a linear layer's outputs, which are not kept: logits = hidden weight^T + bias, of 16-bit hidden [rows, width] and
+ * weight [classes, width], in 32 bits, made twice, the second time in pieces of the classes for the gradients; targets as labels or rows of
+ * LabelMixup, ignored rows and rows that give NaN as above.  Rows with the label ignore_index are not read.  A part of the gradient of the
+ * logits is held in 16 bits at a time; sums are of 32 bits, always in the same order.  At most 2^24 rows and classes, a width of 2^16. */
+typedef struct {
+    const void *hidden, *weight, *bias; /* of `type`, neighbours in a row next to one another; bias [classes] or NULL */
+    const void *target;
+    const float *upstream;
+    void *grad_hidden, *grad_weight, *grad_bias; /* of `type`, contiguous and 16-byte aligned, or NULL: not wanted */
+    float *loss;            /* one value, or NULL */
+    float *row_loss;        /* [rows]: written unless from_stats */
+    float *stats;           /* [rows, 4], 16-byte aligned: largest logit, 1 / sum exp(z - it), the labels' logits; written, or read with from_stats */
+    int64_t rows, classes, width, hidden_stride, weight_stride, target_stride, ignore_index;
+    int32_t device, type, target_kind, has_ignore, mean, upstream_per_row;
+    int32_t from_stats;     /* the gradients alone, with stats of an earlier call */
+    int32_t unused;
+    float smoothing, scale;
+} ffcvb_linear_cross_entropy_args;
+/* workspace: ffcvb_linear_cross_entropy_workspace(args) bytes, 256-byte aligned. */
+int ffcvb_linear_cross_entropy(const ffcvb_linear_cross_entropy_args *args, void *workspace, void *stream);
+int64_t ffcvb_linear_cross_entropy_workspace(const ffcvb_linear_cross_entropy_args *args);
+
 /* The seam between two blocks of a residual network, on rows of `width` values (at most FFCVB_NORM_MAX_WIDTH):
  *   u = post(h), or h;   y = x + scale * gate * u;   z = norm(y)
  * where a norm is (a - mean) / sqrt(var + eps) * weight + bias (layer) or a / sqrt(mean a^2 + eps) * weight (rms), in 32
