@@ -12,6 +12,8 @@ TYPES = {ch.float32: 0, ch.float16: 1, ch.bfloat16: 2}
 
 CROSS_ENTROPY = struct.Struct('=8Q6q8i2f')
 LINEAR_CROSS_ENTROPY = struct.Struct('=11Q7q8i2f')
+DISTILLATION = struct.Struct('=10Q9q10i4f')
+DISTILLATION_MOST = 1024
 NORM_RESIDUAL = struct.Struct('=21Q8q6i2f')
 ROTARY = struct.Struct('=7Q19q6ifi')
 ADAMW = struct.Struct('=7Qq4id')
@@ -21,7 +23,7 @@ NORM_MAX_WIDTH = 16384
 
 lib.ffcvb_training_error.argtypes = []
 lib.ffcvb_training_error.restype = c_char_p
-for _name in ('ffcvb_cross_entropy', 'ffcvb_norm_residual', 'ffcvb_norm_residual_backward', 'ffcvb_rotary'):
+for _name in ('ffcvb_cross_entropy', 'ffcvb_distillation', 'ffcvb_norm_residual', 'ffcvb_norm_residual_backward', 'ffcvb_rotary'):
     getattr(lib, _name).argtypes = [c_char_p, c_void_p]
     getattr(lib, _name).restype = c_int
 lib.ffcvb_norm_residual_backward.argtypes = [c_char_p, c_void_p, c_void_p]

@@ -366,6 +366,30 @@ typedef struct {
 int ffcvb_linear_cross_entropy(const ffcvb_linear_cross_entropy_args *args, void *workspace, void *stream);
 int64_t ffcvb_linear_cross_entropy_workspace(const ffcvb_linear_cross_entropy_args *args);
 
+/* Distillation: logits x [rows, classes] against a teacher's `kept` largest logits t of each row, of classes c (an entry whose class is below 0
+ * is none, as is one of -inf; classes may come more than once).  With q = softmax(t / temperature) over a row's entries and
+ * p = softmax(x / temperature) over all classes,
+ *   loss_i = (1 - hard) * temperature^2 * sum q (log q - log p_c) + hard * H,
+ * H being the cross entropy above of the same logits against labels or rows of LabelMixup.  A row without an entry has no first term; ignored
+ * rows, rows of -inf alone and labels outside the classes as above, and a teacher's class above the last one as such a label. */
+#define FFCVB_DISTILLATION_MOST 1024
+typedef struct {
+    const void *logits;     /* [rows, classes], neighbouring classes next to one another */
+    const void *teacher, *teacher_classes; /* [rows, kept]: of teacher_type; int32, or int64 (classes_wide) */
+    const void *target;     /* int64 [rows], float [rows, 3], or NULL */
+    const float *upstream;  /* one factor of the gradient, or one per row (upstream_per_row), or NULL */
+    void *grad;             /* [rows, classes] of the logits' type, or NULL: no gradient */
+    float *loss, *row_loss; /* as above */
+    float *stats;           /* [rows, 4], 16-byte aligned: written, or read with from_stats, or NULL */
+    float *counted;         /* one value of workspace; needed with has_ignore and mean */
+    int64_t rows, classes, kept, logits_stride, teacher_stride, classes_stride, target_stride, grad_stride, ignore_index;
+    int32_t device, type, teacher_type, classes_wide, target_kind, has_ignore, mean, upstream_per_row;
+    int32_t from_stats;     /* the gradient alone, with stats of an earlier call */
+    int32_t unused;
+    float temperature, hard, smoothing, scale;
+} ffcvb_distillation_args;
+int ffcvb_distillation(const ffcvb_distillation_args *args, void *stream);
+
 /* The seam between two blocks of a residual network, on rows of `width` values (at most FFCVB_NORM_MAX_WIDTH):
  *   u = post(h), or h;   y = x + scale * gate * u;   z = norm(y)
  * where a norm is (a - mean) / sqrt(var + eps) * weight + bias (layer) or a / sqrt(mean a^2 + eps) * weight (rms), in 32
