@@ -14,6 +14,7 @@ CROSS_ENTROPY = struct.Struct('=8Q6q8i2f')
 LINEAR_CROSS_ENTROPY = struct.Struct('=11Q7q8i2f')
 DISTILLATION = struct.Struct('=10Q9q10i4f')
 DISTILLATION_MOST = 1024
+GROUP_NORM = struct.Struct('=9Q8q4ifi')
 NORM_RESIDUAL = struct.Struct('=21Q8q6i2f')
 ROTARY = struct.Struct('=7Q19q6ifi')
 ADAMW = struct.Struct('=7Qq4id')
@@ -29,6 +30,10 @@ for _name in ('ffcvb_cross_entropy', 'ffcvb_distillation', 'ffcvb_norm_residual'
 lib.ffcvb_norm_residual_backward.argtypes = [c_char_p, c_void_p, c_void_p]
 lib.ffcvb_norm_residual_workspace.argtypes = [c_char_p]
 lib.ffcvb_norm_residual_workspace.restype = c_int64
+lib.ffcvb_group_norm.argtypes = lib.ffcvb_group_norm_backward.argtypes = [c_char_p, c_void_p, c_void_p]
+lib.ffcvb_group_norm.restype = lib.ffcvb_group_norm_backward.restype = c_int
+lib.ffcvb_group_norm_workspace.argtypes = [c_char_p, c_int]
+lib.ffcvb_group_norm_workspace.restype = c_int64
 lib.ffcvb_linear_cross_entropy.argtypes = [c_char_p, c_void_p, c_void_p]
 lib.ffcvb_linear_cross_entropy.restype = c_int
 lib.ffcvb_linear_cross_entropy_workspace.argtypes = [c_char_p]

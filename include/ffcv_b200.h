@@ -416,6 +416,30 @@ int ffcvb_norm_residual(const ffcvb_norm_residual_args *args, void *stream);
 int ffcvb_norm_residual_backward(const ffcvb_norm_residual_args *args, void *workspace, void *stream);
 int64_t ffcvb_norm_residual_workspace(const ffcvb_norm_residual_args *args);
 
+/* Group norm with an activation, of samples [positions, channels] with the channels next to one another: each group's channels / groups neighbouring
+ * channels at all positions have the mean and deviation that are taken off and out,
+ *   y = act((x - mean) / sqrt(var + eps) * weight + bias),
+ * in 32 bits throughout.  act is nothing, max(a, 0), a / (1 + exp(-a)), or a times the normal distribution's integral up to a.  At most
+ * 2^24 samples of 2^30 positions and 2^20 channels. */
+enum { FFCVB_ACT_NONE = 0, FFCVB_ACT_RELU = 1, FFCVB_ACT_SILU = 2, FFCVB_ACT_GELU = 3 };
+typedef struct {
+    const void *x;
+    const void *weight, *bias; /* [channels] of param_type, or NULL: 1, 0 */
+    float *stats;           /* [samples, groups, 2]: mean and 1 / deviation; written forward, read backward */
+    void *y;                /* contiguous; forward only */
+    const void *dy;         /* backward only, like the following */
+    void *dx;               /* contiguous, or NULL: not wanted */
+    void *dweight, *dbias;  /* of param_type, or NULL */
+    int64_t samples, positions, channels, groups, x_sample, x_position, dy_sample, dy_position; /* the last four strides */
+    int32_t device, type, param_type, activation;
+    float eps;
+    int32_t unused;
+} ffcvb_group_norm_args;
+/* workspace: ffcvb_group_norm_workspace(args, backward) bytes, 16-byte aligned; may be NULL where that is 0. */
+int ffcvb_group_norm(const ffcvb_group_norm_args *args, void *workspace, void *stream);
+int ffcvb_group_norm_backward(const ffcvb_group_norm_args *args, void *workspace, void *stream);
+int64_t ffcvb_group_norm_workspace(const ffcvb_group_norm_args *args, int backward);
+
 /* Rotary positions: pair i of a head's first rotary_dim values, (a, b), becomes
  *   amplitude * (a cos t - b sin t, a sin t + b cos t),   t = position * 2 pi * turns[i],
  * the other values are copied.  Pairs are neighbours (interleaved) or rotary_dim / 2 apart (half).  With two axes
