@@ -46,53 +46,124 @@ template <> struct Pack<__half, 2> {
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256, kHeldThreads = 128;
 constexpr int kMostGroups = 32; // of a CTA
 constexpr float kLog2e = 1.4426950408889634f;
 
-__device__ __forceinline__ float exp_of(float x) {
+__device__ __forceinline__ float exp2_of(float x) {
     float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * kLog2e));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// 1 / v, each at most 2^60: one reciprocal for two, of their product.
+__device__ __forceinline__ Two inverse(Two v) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v.lo() * v.hi()));
+    return mul_rn(Two(r, r), Two(v.hi(), v.lo()));
+}
+__device__ __forceinline__ Two all(float v) { return Two(v, v); }
 
-template <int N> __device__ __forceinline__ void activate(float (&v)[N], int kind) {
+// 1 / (1 + exp(-a)); 2^-60 instead of less.  (A NaN is none here, so that it stays with its own value; what the gate is multiplied with has it.)
+__device__ __forceinline__ Two gate_of(Two a) {
+    const Two t = mul_rn(a, all(-kLog2e));
+    return inverse(add_rn(Two(exp2_of(fminf(t.lo(), 60.0f)), exp2_of(fminf(t.hi(), 60.0f))), all(1.0f)));
+}
+// The normal distribution's density at a, and its integral up to a.  With z = |a| / sqrt(2) and t = 1 / (1 + 0.42 z) the integral up to -|a| is
+// t P(t) exp(-z^2) / 2; P is a polynomial fitted to that for z up to 6, to 3.3e-8 of the value.
+__device__ __forceinline__ void normal(Two a, Two &density, Two &integral) {
+    const Two size(fminf(fabsf(a.lo()), 30.0f), fminf(fabsf(a.hi()), 30.0f));
+    const Two t = inverse(fma_rn(size, all(0.42f * 0.70710678118654752f), all(1.0f)));
+    const Two square = mul_rn(mul_rn(a, a), all(-0.5f * kLog2e)), e(exp2_of(square.lo()), exp2_of(square.hi()));
+    Two p = fma_rn(all(0.5f * 0.076194151358683f), t, all(0.5f * -0.3458746854890851f));
+    p = fma_rn(p, t, all(0.5f * 0.4864512135112419f));
+    p = fma_rn(p, t, all(0.5f * -0.174528421558005f));
+    p = fma_rn(p, t, all(0.5f * 0.2932564906472867f));
+    p = fma_rn(p, t, all(0.5f * 0.18682665698819034f));
+    p = fma_rn(p, t, all(0.5f * 0.24094708374661222f));
+    p = fma_rn(p, t, all(0.5f * 0.23672753345776956f));
+    const Two tail = mul_rn(mul_rn(p, t), e);
+    integral = Two(a.lo() > 0.0f ? 1.0f - tail.lo() : tail.lo(), a.hi() > 0.0f ? 1.0f - tail.hi() : tail.hi());
+    density = mul_rn(e, all(0.39894228040143268f));
+}
+
+// act(a), in pairs
+template <int P> __device__ __forceinline__ void activate(Two (&v)[P], int kind) {
     if (kind == FFCVB_ACT_SILU) {
 #pragma unroll
-        for (int j = 0; j < N; j++) v[j] = __fdividef(v[j], 1.0f + exp_of(-v[j]));
+        for (int i = 0; i < P; i++) v[i] = mul_rn(v[i], gate_of(v[i]));
     } else if (kind == FFCVB_ACT_GELU) {
 #pragma unroll
-        for (int j = 0; j < N; j++) v[j] = 0.5f * v[j] * (1.0f + erff(v[j] * 0.70710678118654752f));
-    } else if (kind == FFCVB_ACT_RELU) {
+        for (int i = 0; i < P; i++) {
+            Two density, integral;
+            normal(v[i], density, integral);
+            v[i] = mul_rn(v[i], integral);
+        }
+    } else if (kind == FFCVB_ACT_RELU) { // (NaN stays)
 #pragma unroll
-        for (int j = 0; j < N; j++) v[j] = v[j] > 0.0f || v[j] != v[j] ? v[j] : 0.0f;
+        for (int i = 0; i < P; i++) v[i] = Two(v[i].lo() < 0.0f ? 0.0f : v[i].lo(), v[i].hi() < 0.0f ? 0.0f : v[i].hi());
     }
 }
 // act'(a) dy in the place of dy
-template <int N> __device__ __forceinline__ void slope(float (&d)[N], const float (&a)[N], int kind) {
+template <int P> __device__ __forceinline__ void slope(Two (&d)[P], const Two (&a)[P], int kind) {
     if (kind == FFCVB_ACT_SILU) {
 #pragma unroll
-        for (int j = 0; j < N; j++) {
-            const float gate = __fdividef(1.0f, 1.0f + exp_of(-a[j]));
-            d[j] *= gate * fmaf(a[j], 1.0f - gate, 1.0f);
+        for (int i = 0; i < P; i++) {
+            const Two gate = gate_of(a[i]), rest = sub_rn(all(1.0f), gate);
+            d[i] = mul_rn(mul_rn(d[i], gate), fma_rn(a[i], rest, all(1.0f)));
         }
     } else if (kind == FFCVB_ACT_GELU) {
 #pragma unroll
-        for (int j = 0; j < N; j++) d[j] *= fmaf(0.39894228040143268f * a[j], exp_of(-0.5f * a[j] * a[j]), 0.5f * (1.0f + erff(a[j] * 0.70710678118654752f)));
+        for (int i = 0; i < P; i++) {
+            Two density, integral;
+            normal(a[i], density, integral);
+            d[i] = mul_rn(d[i], fma_rn(a[i], density, integral));
+        }
     } else if (kind == FFCVB_ACT_RELU) {
 #pragma unroll
-        for (int j = 0; j < N; j++) d[j] = a[j] > 0.0f ? d[j] : 0.0f;
+        for (int i = 0; i < P; i++) d[i] = Two(a[i].lo() > 0.0f ? d[i].lo() : 0.0f, a[i].hi() > 0.0f ? d[i].hi() : 0.0f);
     }
 }
+
+// A pack's values in pairs; the one pair of a single value has a 0 beside it.
+template <int W> constexpr int kPairs = (W + 1) / 2;
+template <typename T, int W> __device__ __forceinline__ void get_pairs(Two (&v)[kPairs<W>], const Pack<T, W> &pack) {
+    float f[W];
+    pack.get(f);
+#pragma unroll
+    for (int i = 0; i < kPairs<W>; i++) v[i] = Two(f[2 * i], W == 1 ? 0.0f : f[(2 * i + 1) % W]);
+}
+template <typename T, int W> __device__ __forceinline__ void put_pairs(T *to, const Two (&v)[kPairs<W>]) {
+    float f[W];
+#pragma unroll
+    for (int j = 0; j < W; j++) f[j] = v[j / 2].half(j & 1);
+    Pack<T, W> pack;
+    pack.set(f);
+    pack.store(to);
+}
+
+// Which groups a pack's channels are of: `left` those before `split`, the next one the others (SPLIT; else all are of one).
+struct Groups {
+    int left, split;
+    __device__ __forceinline__ Groups(int pack, int w, int per) : left(pack * w / per), split(min(w, (pack * w / per + 1) * per - pack * w)) {}
+};
+// A number of a pack's groups for each of its channels.
+template <int W, bool SPLIT> struct Each {
+    Two v[SPLIT ? kPairs<W> : 1];
+    __device__ __forceinline__ void set(float left, float right, int split) {
+#pragma unroll
+        for (int i = 0; i < (SPLIT ? kPairs<W> : 1); i++) v[i] = Two(!SPLIT || 2 * i < split ? left : right, !SPLIT || 2 * i + 1 < split ? left : right);
+    }
+    __device__ __forceinline__ Two operator[](int i) const { return v[SPLIT ? i : 0]; }
+};
 
 // How many, their mean, and the sum of squares around it.
 struct Moments {
     float n, mean, squares;
     __device__ __forceinline__ void join(Moments o) {
-        const float all = n + o.n, share = o.n == 0.0f ? 0.0f : o.n / all, apart = o.mean - mean;
-        squares += o.squares + apart * apart * n * share;
-        mean += apart * share;
-        n = all;
+        const float both = n + o.n, share = __fdividef(o.n, fmaxf(both, 1.0f)), apart = o.mean - mean, step = apart * share;
+        squares += fmaf(apart * step, n, o.squares);
+        mean += step;
+        n = both;
     }
     // of a warp; lane 0 has the result
     __device__ __forceinline__ void join_lanes() {
@@ -103,35 +174,74 @@ struct Moments {
     __device__ __forceinline__ float rate(float eps) const { return rsqrtf(squares / n + eps); }
 };
 
-// Values of a thread, relative to its first one.
+// A thread's values of W channels, each relative to its first one.
 template <int W> struct Collected {
-    float first, sum, squares;
+    static constexpr int P = kPairs<W>;
+    Two first[P], sum[P], squares[P];
     int rows;
-    __device__ __forceinline__ void add(const float (&v)[W]) {
-        if (rows++ == 0) first = v[0], sum = squares = 0.0f;
+    __device__ __forceinline__ Collected() : rows(0) {
 #pragma unroll
-        for (int j = 0; j < W; j++) {
-            const float d = v[j] - first;
-            sum += d;
-            squares = fmaf(d, d, squares);
+        for (int i = 0; i < P; i++) first[i] = sum[i] = squares[i] = all(0.0f);
+    }
+    __device__ __forceinline__ void add(const Two (&v)[P]) {
+        if (rows++ == 0)
+#pragma unroll
+            for (int i = 0; i < P; i++) first[i] = v[i];
+#pragma unroll
+        for (int i = 0; i < P; i++) {
+            const Two d = sub_rn(v[i], first[i]);
+            sum[i] = add_rn(sum[i], d);
+            squares[i] = fma_rn(d, d, squares[i]);
         }
     }
-    __device__ __forceinline__ Moments moments() const {
-        if (rows == 0) return Moments{0.0f, 0.0f, 0.0f};
-        const float n = (float)(rows * W), mean = sum / n;
-        const float around = squares - sum * mean;
-        return Moments{n, first + mean, around < 0.0f ? 0.0f : around}; // (NaN stays)
+    // of channels from..to
+    __device__ __forceinline__ Moments moments(int from, int to) const {
+        if (rows == 0 || from >= to) return Moments{0.0f, 0.0f, 0.0f};
+        const float n = (float)rows, over = 1.0f / n;
+        float mean[W], around = 0.0f, base = 0.0f, level = 0.0f;
+#pragma unroll
+        for (int j = 0; j < W; j++) {
+            const float s = sum[j / 2].half(j & 1), away = s * over, left = squares[j / 2].half(j & 1) - s * away;
+            mean[j] = first[j / 2].half(j & 1) + away;
+            if (j == from) base = mean[j];
+            if (j < from || j >= to) continue;
+            around += left < 0.0f ? 0.0f : left; // (NaN stays)
+            level += mean[j] - base;
+        }
+        level = base + level / (float)(to - from);
+        float apart = 0.0f;
+#pragma unroll
+        for (int j = 0; j < W; j++)
+            if (j >= from && j < to) apart = fmaf(mean[j] - level, mean[j] - level, apart);
+        return Moments{n * (float)(to - from), level, fmaf(n, apart, around)};
     }
 };
 
-// W neighbouring parameters, or what stands for them.
-template <int W> __device__ __forceinline__ void parameters(float (&v)[W], const void *from, int type, long long c, float other) {
+// W neighbouring parameters in pairs, or what stands for them.
+__device__ __forceinline__ float parameter(const void *from, int type, long long c, float other) {
+    return !from                    ? other
+           : type == FFCVB_TYPE_F32 ? static_cast<const float *>(from)[c]
+           : type == FFCVB_TYPE_F16 ? to_float(static_cast<const __half *>(from)[c])
+                                    : to_float(static_cast<const __nv_bfloat16 *>(from)[c]);
+}
+template <int W> __device__ __forceinline__ void parameters(Two (&v)[kPairs<W>], const void *from, int type, long long c, float other) {
+    float f[W];
+    auto of = [&](auto *at) {
 #pragma unroll
-    for (int j = 0; j < W; j++)
-        v[j] = !from                        ? other
-               : type == FFCVB_TYPE_F32     ? static_cast<const float *>(from)[c + j]
-               : type == FFCVB_TYPE_F16     ? to_float(static_cast<const __half *>(from)[c + j])
-                                            : to_float(static_cast<const __nv_bfloat16 *>(from)[c + j]);
+        for (int j = 0; j < W; j++) f[j] = to_float(at[c + j]);
+    };
+    if (!from) {
+#pragma unroll
+        for (int j = 0; j < W; j++) f[j] = other;
+    } else if (type == FFCVB_TYPE_F32) {
+        of(static_cast<const float *>(from));
+    } else if (type == FFCVB_TYPE_F16) {
+        of(static_cast<const __half *>(from));
+    } else {
+        of(static_cast<const __nv_bfloat16 *>(from));
+    }
+#pragma unroll
+    for (int i = 0; i < kPairs<W>; i++) v[i] = Two(f[2 * i], W == 1 ? 0.0f : f[(2 * i + 1) % W]);
 }
 
 // A pack that a thread has copied for itself.
@@ -147,11 +257,6 @@ template <typename T, int W> __device__ __forceinline__ void copy_pack(Pack<T, W
 }
 __device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
-__device__ __forceinline__ uint32_t cluster_rank() {
-    uint32_t r;
-    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
 __device__ __forceinline__ void cluster_begun() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
@@ -165,58 +270,83 @@ __device__ __forceinline__ void store_there(const void *mine, uint32_t rank, flo
 
 // Groups of a CTA, packs of a position in them, of which `lanes` positions at once; positions of a CTA; CTAs of a cluster.
 struct Deal {
-    int groups, packs, lanes, rows, ctas;
+    int groups, packs, lanes, rows, ctas, per; // (per: channels of a group)
+};
+// Of a CTA: its cluster's rank, first group and sample; its thread's row and pack.
+struct Held {
+    int rank, group0, row, pack, first, last;
+    long long sample;
+    __device__ __forceinline__ Held(const Deal &deal, int positions) {
+        const int log = 31 - __clz(deal.ctas); // (1, 2, 4 or 8)
+        rank = blockIdx.x & (deal.ctas - 1);
+        group0 = (blockIdx.x >> log) * deal.groups;
+        sample = blockIdx.y;
+        row = threadIdx.x / deal.packs;
+        pack = threadIdx.x - row * deal.packs;
+        first = rank * deal.rows;
+        last = min(first + deal.rows, positions);
+    }
 };
 
-template <typename T, int W>
-__global__ void __launch_bounds__(kThreads) held_forward_kernel(const __grid_constant__ ffcvb_group_norm_args a, const Deal deal) {
-    __shared__ float s_moments[3][kThreads];
+template <typename T, int W, bool SPLIT>
+__global__ void __launch_bounds__(kHeldThreads) held_forward_kernel(const __grid_constant__ ffcvb_group_norm_args a, const Deal deal) {
+    constexpr int P = kPairs<W>, SIDES = SPLIT ? 2 : 1;
+    __shared__ float s_moments[SIDES][3][kHeldThreads];
     __shared__ Moments s_there[8][kMostGroups]; // of the cluster's CTAs
+    __shared__ float2 s_stats[kMostGroups];
     extern __shared__ uint4 s_held[];
     wait_for_previous();
     let_next_begin();
-    const uint32_t rank = deal.ctas > 1 ? cluster_rank() : 0;
     if (deal.ctas > 1) cluster_begun();
-    const int per = (int)(a.channels / a.groups), blocks = (int)a.groups / deal.groups, unit = blockIdx.x / deal.ctas;
-    const long long sample = unit / blocks;
-    const int group0 = unit % blocks * deal.groups, row = threadIdx.x / deal.packs, pack = threadIdx.x % deal.packs;
-    const int first = (int)rank * deal.rows, last = min(first + deal.rows, (int)a.positions);
-    const int group = pack * W / per, channel = group0 * per + pack * W;
+    const Held me(deal, (int)a.positions);
+    const int per = deal.per, rank = me.rank, group0 = me.group0, row = me.row, pack = me.pack, first = me.first, last = me.last;
+    const long long sample = me.sample;
+    const Groups groups(pack, W, per);
+    const int channel = group0 * per + pack * W;
     const bool used = row < deal.lanes;
     const T *x = static_cast<const T *>(a.x) + sample * a.x_sample + channel;
     Pack<T, W> *held = reinterpret_cast<Pack<T, W> *>(s_held) + threadIdx.x;
     if (used) {
+        const T *from = x + (first + row) * a.x_position;
+        const long long step = deal.lanes * a.x_position;
         Pack<T, W> *to = held;
-        for (int r = first + row; r < last; r += deal.lanes, to += kThreads) copy_pack(to, x + r * a.x_position);
+        for (int r = first + row; r < last; r += deal.lanes, to += kHeldThreads, from += step) copy_pack(to, from);
     }
-    float w[W], b[W];
+    Two w[P], b[P];
     if (used) {
-        parameters(w, a.weight, a.param_type, channel, 1.0f);
-        parameters(b, a.bias, a.param_type, channel, 0.0f);
+        parameters<W>(w, a.weight, a.param_type, channel, 1.0f);
+        parameters<W>(b, a.bias, a.param_type, channel, 0.0f);
     }
     copies_done();
-    Collected<W> values{0.0f, 0.0f, 0.0f, 0};
-    if (used) {
-        const Pack<T, W> *from = held;
-        for (int r = first + row; r < last; r += deal.lanes, from += kThreads) {
-            float v[W];
-            from->get(v);
-            values.add(v);
+    {
+        Collected<W> values;
+        if (used) {
+            const Pack<T, W> *from = held;
+#pragma unroll 2
+            for (int r = first + row; r < last; r += deal.lanes, from += kHeldThreads) {
+                Two v[P];
+                get_pairs<T, W>(v, *from);
+                values.add(v);
+            }
+        }
+#pragma unroll
+        for (int side = 0; side < SIDES; side++) {
+            const Moments mine = side ? values.moments(groups.split, W) : values.moments(0, SPLIT ? groups.split : W);
+            s_moments[side][0][threadIdx.x] = mine.n, s_moments[side][1][threadIdx.x] = mine.mean, s_moments[side][2][threadIdx.x] = mine.squares;
         }
     }
-    const Moments mine = values.moments();
-    s_moments[0][threadIdx.x] = mine.n, s_moments[1][threadIdx.x] = mine.mean, s_moments[2][threadIdx.x] = mine.squares;
     __syncthreads();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, each = per / W; // packs of a group
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (deal.ctas > 1) cluster_wait(); // all have begun
-    for (int g = warp; g < deal.groups; g += kThreads / 32) {
-        Moments all{0.0f, 0.0f, 0.0f};
+    for (int g = warp; g < deal.groups; g += kHeldThreads / 32) {
+        const int pack0 = g * per / W, each = ((g + 1) * per - 1) / W - pack0 + 1; // packs of a group
+        Moments found{0.0f, 0.0f, 0.0f};
         for (int e = lane; e < deal.lanes * each; e += 32) {
-            const int t = e / each * deal.packs + g * each + e % each;
-            all.join(Moments{s_moments[0][t], s_moments[1][t], s_moments[2][t]});
+            const int k = pack0 + e % each, t = e / each * deal.packs + k, side = SPLIT && k * W / per != g;
+            found.join(Moments{s_moments[side][0][t], s_moments[side][1][t], s_moments[side][2][t]});
         }
-        all.join_lanes();
-        const float n = __shfl_sync(0xffffffffu, all.n, 0), mean = __shfl_sync(0xffffffffu, all.mean, 0), squares = __shfl_sync(0xffffffffu, all.squares, 0);
+        found.join_lanes();
+        const float n = __shfl_sync(0xffffffffu, found.n, 0), mean = __shfl_sync(0xffffffffu, found.mean, 0), squares = __shfl_sync(0xffffffffu, found.squares, 0);
         if (lane < deal.ctas) {
             Moments *to = &s_there[rank][g];
             if (deal.ctas == 1) {
@@ -232,160 +362,218 @@ __global__ void __launch_bounds__(kThreads) held_forward_kernel(const __grid_con
         cluster_sync();
     else
         __syncthreads();
+    if (threadIdx.x < deal.groups) {
+        Moments whole = s_there[0][threadIdx.x];
+        for (int k = 1; k < deal.ctas; k++) whole.join(s_there[k][threadIdx.x]);
+        const float2 stats = make_float2(whole.mean, whole.rate(a.eps));
+        s_stats[threadIdx.x] = stats;
+        if (rank == 0) reinterpret_cast<float2 *>(a.stats)[sample * a.groups + group0 + threadIdx.x] = stats;
+    }
+    __syncthreads();
     if (!used) return;
-    Moments all = s_there[0][group];
-    for (int k = 1; k < deal.ctas; k++) all.join(s_there[k][group]);
-    const float rate = all.rate(a.eps);
-    if (rank == 0 && row == 0 && pack % each == 0) reinterpret_cast<float2 *>(a.stats)[sample * a.groups + group0 + group] = make_float2(all.mean, rate);
+    const float2 left = s_stats[groups.left], right = SPLIT ? s_stats[min(groups.left + 1, deal.groups - 1)] : left;
+    Each<W, SPLIT> less, rates;
+    less.set(left.x, right.x, groups.split);
+    rates.set(left.y, right.y, groups.split);
 #pragma unroll
-    for (int j = 0; j < W; j++) w[j] *= rate;
-    T *y = static_cast<T *>(a.y) + sample * a.positions * a.channels + channel;
+    for (int i = 0; i < P; i++) w[i] = mul_rn(w[i], rates[i]);
+    T *to = static_cast<T *>(a.y) + (sample * a.positions + first + row) * a.channels + channel;
+    const long long step = deal.lanes * a.channels;
     const Pack<T, W> *from = held;
-    for (int r = first + row; r < last; r += deal.lanes, from += kThreads) {
-        float v[W];
-        from->get(v);
+#pragma unroll 2
+    for (int r = first + row; r < last; r += deal.lanes, from += kHeldThreads, to += step) {
+        Two v[P];
+        get_pairs<T, W>(v, *from);
 #pragma unroll
-        for (int j = 0; j < W; j++) v[j] = fmaf(v[j] - all.mean, w[j], b[j]);
+        for (int i = 0; i < P; i++) v[i] = fma_rn(sub_rn(v[i], less[i]), w[i], b[i]);
         activate(v, a.activation);
-        Pack<T, W> out;
-        out.set(v);
-        out.store(y + r * a.channels);
+        put_pairs<T, W>(to, v);
     }
 }
 
-// Sums over positions of da and da hat: of a thread's channels joined over the rows of the CTA, in s_sums[channel]; `s_all` is room for all threads'.
-template <int W> __device__ __forceinline__ void channel_sums(const float2 (&mine)[W], bool used, int row, int pack, int lanes, int packs, float2 *s_all, float2 *s_sums) {
-    const int channels = packs * W;
-    if (used)
+// A thread's sums over its positions of da and of da hat, of W channels.
+template <int W> struct Sums {
+    static constexpr int P = kPairs<W>;
+    Two da[P], hat[P];
+    __device__ __forceinline__ Sums() {
 #pragma unroll
-        for (int j = 0; j < W; j++) s_all[row * channels + pack * W + j] = mine[j];
+        for (int i = 0; i < P; i++) da[i] = hat[i] = all(0.0f);
+    }
+    __device__ __forceinline__ void add(const Two (&h)[P], const Two (&d)[P]) {
+#pragma unroll
+        for (int i = 0; i < P; i++) {
+            da[i] = add_rn(da[i], d[i]);
+            hat[i] = fma_rn(d[i], h[i], hat[i]);
+        }
+    }
+    __device__ __forceinline__ float2 of(int j) const { return make_float2(da[j / 2].half(j & 1), hat[j / 2].half(j & 1)); }
+    // Lanes of a warp that have the same pack, `packs` (a power of two) apart: the lowest has the sum.
+    __device__ __forceinline__ void join_lanes(int packs) {
+        for (int o = 16; o >= packs; o >>= 1)
+#pragma unroll
+            for (int i = 0; i < P; i++) {
+                da[i] = add_rn(da[i], Two(__shfl_down_sync(0xffffffffu, da[i].lo(), o), __shfl_down_sync(0xffffffffu, da[i].hi(), o)));
+                hat[i] = add_rn(hat[i], Two(__shfl_down_sync(0xffffffffu, hat[i].lo(), o), __shfl_down_sync(0xffffffffu, hat[i].hi(), o)));
+            }
+    }
+};
+// Rows of partial sums that a CTA's threads leave in shared memory: one per warp where a warp's lanes can be joined, else one per position at once.
+__host__ __device__ constexpr bool joined(int packs) { return packs <= 32 && (packs & (packs - 1)) == 0; }
+__host__ __device__ constexpr int sum_rows(int packs, int lanes) { return joined(packs) ? kHeldThreads / 32 : lanes; }
+
+// Sums of a CTA's threads joined over its positions: s_sums[channel]; `s_all` is room for sum_rows() times the channels.
+template <int W> __device__ __forceinline__ void channel_sums(Sums<W> &mine, bool used, int row, int pack, int lanes, int packs, float2 *s_all, float2 *s_sums) {
+    const int channels = packs * W, rows = sum_rows(packs, lanes);
+    bool writes = used;
+    if (joined(packs)) {
+        mine.join_lanes(packs);
+        row = threadIdx.x >> 5;
+        writes = (threadIdx.x & 31) < packs;
+    }
+    if (writes)
+#pragma unroll
+        for (int j = 0; j < W; j++) s_all[row * channels + pack * W + j] = mine.of(j);
     __syncthreads();
-    // lanes are halved until one is left, always in the same order
-    for (int n = lanes; n > 1;) {
+    // rows are halved until one is left, always in the same order
+    for (int n = rows; n > 1;) {
         const int half = (n + 1) / 2;
-        for (int i = threadIdx.x; i < (n - half) * channels; i += kThreads) {
+        for (int i = threadIdx.x; i < (n - half) * channels; i += kHeldThreads) {
             s_all[i].x += s_all[i + half * channels].x;
             s_all[i].y += s_all[i + half * channels].y;
         }
         n = half;
         __syncthreads();
     }
-    for (int i = threadIdx.x; i < channels; i += kThreads) s_sums[i] = s_all[i];
+    for (int i = threadIdx.x; i < channels; i += kHeldThreads) s_sums[i] = s_all[i];
 }
 
-// room: 2 * kThreads * W floats for sums, of the cluster's CTAs as many channels' as there are; then x and dy
-template <typename T, int W>
-__global__ void __launch_bounds__(kThreads) held_backward_kernel(const __grid_constant__ ffcvb_group_norm_args a, const Deal deal, float2 *sums) {
+// What a thread needs for hat and da of W channels, and for dx.
+template <typename T, int W, bool SPLIT> struct Back {
+    static constexpr int P = kPairs<W>;
+    Two w[P], b[P];
+    Each<W, SPLIT> mean, rate;
+    int kind;
+    __device__ __forceinline__ Back() {}
+    __device__ __forceinline__ Back(const ffcvb_group_norm_args &a, long long sample, int channel, int group, const Groups &groups) : kind(a.activation) {
+        parameters<W>(w, a.weight, a.param_type, channel, 1.0f);
+        parameters<W>(b, a.bias, a.param_type, channel, 0.0f);
+        const float2 *stats = reinterpret_cast<const float2 *>(a.stats) + sample * a.groups;
+        const float2 left = stats[group], right = SPLIT ? stats[min(group + 1, (int)a.groups - 1)] : left;
+        mean.set(left.x, right.x, groups.split);
+        rate.set(left.y, right.y, groups.split);
+    }
+    __device__ __forceinline__ void row(const Pack<T, W> &x, const Pack<T, W> &dy, Two (&hat)[P], Two (&da)[P]) const {
+        get_pairs<T, W>(hat, x);
+        get_pairs<T, W>(da, dy);
+        Two v[P];
+#pragma unroll
+        for (int i = 0; i < P; i++) {
+            hat[i] = mul_rn(sub_rn(hat[i], mean[i]), rate[i]);
+            v[i] = fma_rn(hat[i], w[i], b[i]);
+        }
+        slope(da, v, kind);
+    }
+    // `less`: the means of da w and of da w hat
+    __device__ __forceinline__ void gradient(const Two (&hat)[P], Two (&da)[P], const Each<W, SPLIT> &less, const Each<W, SPLIT> &less_hat) const {
+#pragma unroll
+        for (int i = 0; i < P; i++) da[i] = mul_rn(sub_rn(sub_rn(mul_rn(da[i], w[i]), less[i]), mul_rn(hat[i], less_hat[i])), rate[i]);
+    }
+};
+
+// room: (sum_rows() + CTAs of the cluster) times the channels, of two floats; then x and dy
+template <typename T, int W, bool SPLIT>
+__global__ void __launch_bounds__(kHeldThreads) held_backward_kernel(const __grid_constant__ ffcvb_group_norm_args a, const Deal deal, float2 *sums) {
+    constexpr int P = kPairs<W>;
     __shared__ float2 s_group[kMostGroups];
     extern __shared__ uint4 s_held[];
     wait_for_previous();
     let_next_begin();
-    const uint32_t rank = deal.ctas > 1 ? cluster_rank() : 0;
     if (deal.ctas > 1) cluster_begun();
-    const int per = (int)(a.channels / a.groups), blocks = (int)a.groups / deal.groups, unit = blockIdx.x / deal.ctas;
-    const long long sample = unit / blocks;
-    const int group0 = unit % blocks * deal.groups, row = threadIdx.x / deal.packs, pack = threadIdx.x % deal.packs, channels = deal.packs * W;
-    const int first = (int)rank * deal.rows, last = min(first + deal.rows, (int)a.positions);
-    const int group = pack * W / per, channel = group0 * per + pack * W;
+    const Held me(deal, (int)a.positions);
+    const int per = deal.per, rank = me.rank, group0 = me.group0, row = me.row, pack = me.pack, first = me.first, last = me.last, channels = deal.packs * W;
+    const long long sample = me.sample;
+    const Groups groups(pack, W, per);
+    const int channel = group0 * per + pack * W;
     const bool used = row < deal.lanes;
-    const T *x = static_cast<const T *>(a.x) + sample * a.x_sample + channel, *dy = static_cast<const T *>(a.dy) + sample * a.dy_sample + channel;
-    float2 *s_all = reinterpret_cast<float2 *>(s_held), *s_there = s_all + deal.lanes * channels; // [ctas][channels]
-    Pack<T, W> *held = reinterpret_cast<Pack<T, W> *>(s_held + ((deal.lanes + deal.ctas) * channels + 1) / 2) + threadIdx.x;
+    float2 *s_all = reinterpret_cast<float2 *>(s_held), *s_there = s_all + sum_rows(deal.packs, deal.lanes) * channels; // [ctas][channels]
+    Pack<T, W> *held = reinterpret_cast<Pack<T, W> *>(s_held + ((sum_rows(deal.packs, deal.lanes) + deal.ctas) * channels + 1) / 2) + threadIdx.x;
     if (used) {
+        const T *x = static_cast<const T *>(a.x) + sample * a.x_sample + (first + row) * a.x_position + channel;
+        const T *dy = static_cast<const T *>(a.dy) + sample * a.dy_sample + (first + row) * a.dy_position + channel;
+        const long long x_step = deal.lanes * a.x_position, dy_step = deal.lanes * a.dy_position;
         Pack<T, W> *to = held;
-        for (int r = first + row; r < last; r += deal.lanes, to += 2 * kThreads) {
-            copy_pack(to, x + r * a.x_position);
-            copy_pack(to + kThreads, dy + r * a.dy_position);
+        for (int r = first + row; r < last; r += deal.lanes, to += 2 * kHeldThreads, x += x_step, dy += dy_step) {
+            copy_pack(to, x);
+            copy_pack(to + kHeldThreads, dy);
         }
     }
-    float w[W], b[W], mean = 0.0f, rate = 0.0f;
-    float2 mine[W];
-#pragma unroll
-    for (int j = 0; j < W; j++) mine[j] = make_float2(0.0f, 0.0f);
-    if (used) {
-        parameters(w, a.weight, a.param_type, channel, 1.0f);
-        parameters(b, a.bias, a.param_type, channel, 0.0f);
-        const float2 stats = reinterpret_cast<const float2 *>(a.stats)[sample * a.groups + group0 + group];
-        mean = stats.x, rate = stats.y;
-    }
+    Back<T, W, SPLIT> back;
+    if (used) back = Back<T, W, SPLIT>(a, sample, channel, group0 + groups.left, groups);
     copies_done();
-    // hat and da of a row
-    auto row_of = [&](const Pack<T, W> *from, float(&hat)[W], float(&da)[W]) {
-        from->get(hat);
-        from[kThreads].get(da);
-        float v[W];
-#pragma unroll
-        for (int j = 0; j < W; j++) {
-            hat[j] = (hat[j] - mean) * rate;
-            v[j] = fmaf(hat[j], w[j], b[j]);
-        }
-        slope(da, v, a.activation);
-    };
-    if (used) {
-        const Pack<T, W> *from = held;
-        for (int r = first + row; r < last; r += deal.lanes, from += 2 * kThreads) {
-            float hat[W], da[W];
-            row_of(from, hat, da);
-#pragma unroll
-            for (int j = 0; j < W; j++) {
-                mine[j].x += da[j];
-                mine[j].y = fmaf(da[j], hat[j], mine[j].y);
+    {
+        Sums<W> mine;
+        if (used) {
+            const Pack<T, W> *from = held;
+            for (int r = first + row; r < last; r += deal.lanes, from += 2 * kHeldThreads) {
+                Two hat[P], da[P];
+                back.row(from[0], from[kHeldThreads], hat, da);
+                mine.add(hat, da);
             }
         }
+        channel_sums<W>(mine, used, row, pack, deal.lanes, deal.packs, s_all, s_there + rank * channels);
     }
-    channel_sums<W>(mine, used, row, pack, deal.lanes, deal.packs, s_all, s_there + (deal.ctas > 1 ? (int)rank * channels : 0));
+    __syncthreads();
     if (deal.ctas > 1) {
-        __syncthreads();
         cluster_wait(); // all have begun
-        for (int i = threadIdx.x; i < channels * deal.ctas; i += kThreads) {
+        for (int i = threadIdx.x; i < channels * deal.ctas; i += kHeldThreads) {
             const int c = i % channels, to = i / channels;
             float2 *at = s_there + rank * channels + c;
-            if (to == (int)rank) continue;
+            if (to == rank) continue;
             const float2 v = *at;
             store_there(&at->x, to, v.x);
             store_there(&at->y, to, v.y);
         }
         cluster_sync();
-        for (int i = threadIdx.x; i < channels; i += kThreads) {
-            float2 all = s_there[i];
+        for (int i = threadIdx.x; i < channels; i += kHeldThreads) {
+            float2 whole = s_there[i];
             for (int k = 1; k < deal.ctas; k++) {
-                all.x += s_there[k * channels + i].x;
-                all.y += s_there[k * channels + i].y;
+                whole.x += s_there[k * channels + i].x;
+                whole.y += s_there[k * channels + i].y;
             }
-            s_all[i] = all;
+            s_all[i] = whole;
         }
+        __syncthreads();
     } else {
-        for (int i = threadIdx.x; i < channels; i += kThreads) s_all[i] = s_there[i]; // (each its own)
+        s_all = s_there;
     }
-    __syncthreads();
     if (rank == 0)
-        for (int i = threadIdx.x; i < channels; i += kThreads) sums[sample * a.channels + group0 * per + i] = s_all[i];
-    for (int g = threadIdx.x >> 5; g < deal.groups; g += kThreads / 32) {
-        float2 all = make_float2(0.0f, 0.0f);
+        for (int i = threadIdx.x; i < channels; i += kHeldThreads) sums[sample * a.channels + group0 * per + i] = s_all[i];
+    for (int g = threadIdx.x >> 5; g < deal.groups; g += kHeldThreads / 32) {
+        float2 mean = make_float2(0.0f, 0.0f);
         for (int c = threadIdx.x & 31; c < per; c += 32) {
-            float one[1];
-            parameters(one, a.weight, a.param_type, group0 * per + g * per + c, 1.0f);
-            all.x = fmaf(one[0], s_all[g * per + c].x, all.x);
-            all.y = fmaf(one[0], s_all[g * per + c].y, all.y);
+            const float one = parameter(a.weight, a.param_type, group0 * per + g * per + c, 1.0f);
+            mean.x = fmaf(one, s_all[g * per + c].x, mean.x);
+            mean.y = fmaf(one, s_all[g * per + c].y, mean.y);
         }
         const float over = 1.0f / ((float)a.positions * (float)per);
-        all.x = warp_sum(all.x) * over;
-        all.y = warp_sum(all.y) * over;
-        if ((threadIdx.x & 31) == 0) s_group[g] = all;
+        mean.x = warp_sum(mean.x) * over;
+        mean.y = warp_sum(mean.y) * over;
+        if ((threadIdx.x & 31) == 0) s_group[g] = mean;
     }
     __syncthreads();
     if (!used || !a.dx) return;
-    const float2 less = s_group[group];
-    T *dx = static_cast<T *>(a.dx) + sample * a.positions * a.channels + channel;
+    Each<W, SPLIT> less, less_hat;
+    const float2 left = s_group[groups.left], right = SPLIT ? s_group[min(groups.left + 1, deal.groups - 1)] : left;
+    less.set(left.x, right.x, groups.split);
+    less_hat.set(left.y, right.y, groups.split);
+    T *to = static_cast<T *>(a.dx) + (sample * a.positions + first + row) * a.channels + channel;
+    const long long step = deal.lanes * a.channels;
     const Pack<T, W> *from = held;
-    for (int r = first + row; r < last; r += deal.lanes, from += 2 * kThreads) {
-        float hat[W], da[W];
-        row_of(from, hat, da);
-#pragma unroll
-        for (int j = 0; j < W; j++) da[j] = rate * (fmaf(da[j], w[j], -less.x) - hat[j] * less.y);
-        Pack<T, W> out;
-        out.set(da);
-        out.store(dx + r * a.channels);
+    for (int r = first + row; r < last; r += deal.lanes, from += 2 * kHeldThreads, to += step) {
+        Two hat[P], da[P];
+        back.row(from[0], from[kHeldThreads], hat, da);
+        back.gradient(hat, da, less, less_hat);
+        put_pairs<T, W>(to, da);
     }
 }
 
@@ -416,143 +604,128 @@ __device__ __forceinline__ Place place_of(const Slabs &s, int positions, bool ba
     return p;
 }
 
-template <typename T, int W>
+// parts: [samples][slabs][packs][sides], mean and squares around it
+template <typename T, int W, bool SPLIT>
 __global__ void __launch_bounds__(kThreads) moments_kernel(const __grid_constant__ ffcvb_group_norm_args a, const Slabs s, float2 *parts) {
-    __shared__ Moments s_moments[kThreads];
+    constexpr int P = kPairs<W>, SIDES = SPLIT ? 2 : 1;
+    __shared__ Moments s_moments[SIDES][kThreads];
     wait_for_previous();
     let_next_begin();
     const Place p = place_of(s, (int)a.positions, false);
-    Collected<W> values{0.0f, 0.0f, 0.0f, 0};
+    const Groups groups(p.pack, W, (int)(a.channels / a.groups));
+    Collected<W> values;
     if (p.used) {
         const T *x = static_cast<const T *>(a.x) + p.sample * a.x_sample + p.pack * W;
 #pragma unroll 4
         for (int r = p.first + p.row; r < p.last; r += s.lanes) {
             Pack<T, W> pack;
-            float v[W];
+            Two v[P];
             pack.load(x + r * a.x_position);
-            pack.get(v);
+            get_pairs<T, W>(v, pack);
             values.add(v);
         }
     }
-    s_moments[threadIdx.x] = values.moments();
+#pragma unroll
+    for (int side = 0; side < SIDES; side++) s_moments[side][threadIdx.x] = side ? values.moments(groups.split, W) : values.moments(0, SPLIT ? groups.split : W);
     __syncthreads();
-    if (p.row != 0 || !p.used) return;
-    Moments all = s_moments[threadIdx.x];
-    for (int k = 1; k < s.lanes; k++) all.join(s_moments[k * s.columns + threadIdx.x]);
-    parts[(p.sample * s.slabs + p.slab) * s.packs + p.pack] = make_float2(all.mean, all.squares);
+    for (int i = threadIdx.x; i < s.columns * SIDES; i += kThreads) {
+        const int column = i % s.columns, side = i / s.columns, pack = blockIdx.y * s.columns + column;
+        if (pack >= s.packs) continue;
+        Moments whole = s_moments[side][column];
+        for (int k = 1; k < s.lanes; k++) whole.join(s_moments[side][k * s.columns + column]);
+        parts[((p.sample * s.slabs + p.slab) * s.packs + pack) * SIDES + side] = make_float2(whole.mean, whole.squares);
+    }
 }
 
-// One warp per group.
-template <int W> __global__ void __launch_bounds__(kThreads) join_moments_kernel(const __grid_constant__ ffcvb_group_norm_args a, const Slabs s, int samples, const float2 *parts) {
+// A CTA per group.
+template <int W, bool SPLIT> __global__ void __launch_bounds__(kThreads) join_moments_kernel(const __grid_constant__ ffcvb_group_norm_args a, const Slabs s, const float2 *parts) {
+    constexpr int SIDES = SPLIT ? 2 : 1;
+    __shared__ Moments s_part[kThreads / 32];
     wait_for_previous();
     let_next_begin();
-    const long long n = blockIdx.x * (kThreads / 32ll) + (threadIdx.x >> 5);
-    if (n >= samples * a.groups) return;
-    const long long sample = s.sample + n / a.groups;
-    const int group = (int)(n % a.groups), each = (int)(a.channels / a.groups) / W;
-    Moments all{0.0f, 0.0f, 0.0f};
-    for (long long e = threadIdx.x & 31; e < (long long)s.slabs * each; e += 32) {
-        const int slab = (int)(e / each);
-        const float2 part = parts[(sample * s.slabs + slab) * s.packs + group * each + e % each];
-        all.join(Moments{(float)(min(s.rows, (int)a.positions - slab * s.rows) * W), part.x, part.y});
+    const long long sample = s.sample + blockIdx.x / a.groups;
+    const int group = (int)(blockIdx.x % a.groups), per = (int)(a.channels / a.groups), pack0 = (int)((long long)group * per / W);
+    const int each = (int)(((long long)(group + 1) * per - 1) / W) - pack0 + 1;
+    Moments found{0.0f, 0.0f, 0.0f};
+    for (long long e = threadIdx.x; e < (long long)s.slabs * each; e += kThreads) {
+        const int slab = (int)(e / each), pack = pack0 + (int)(e % each);
+        const Groups groups(pack, W, per);
+        const int side = SPLIT && groups.left != group, there = !SPLIT ? W : side ? W - groups.split : groups.split;
+        const float2 part = parts[((sample * s.slabs + slab) * s.packs + pack) * SIDES + side];
+        found.join(Moments{(float)min(s.rows, (int)a.positions - slab * s.rows) * (float)there, part.x, part.y});
     }
-    all.join_lanes();
-    if ((threadIdx.x & 31) == 0) reinterpret_cast<float2 *>(a.stats)[sample * a.groups + group] = make_float2(all.mean, all.rate(a.eps));
+    found.join_lanes();
+    if ((threadIdx.x & 31) == 0) s_part[threadIdx.x >> 5] = found;
+    __syncthreads();
+    if (threadIdx.x) return;
+    for (int k = 1; k < kThreads / 32; k++) found.join(s_part[k]);
+    reinterpret_cast<float2 *>(a.stats)[sample * a.groups + group] = make_float2(found.mean, found.rate(a.eps));
 }
 
-template <typename T, int W>
+template <typename T, int W, bool SPLIT>
 __global__ void __launch_bounds__(kThreads) values_kernel(const __grid_constant__ ffcvb_group_norm_args a, const Slabs s) {
+    constexpr int P = kPairs<W>;
     wait_for_previous();
     let_next_begin();
     const Place p = place_of(s, (int)a.positions, true);
     if (!p.used) return;
-    const int channel = p.pack * W, group = channel / (int)(a.channels / a.groups);
-    float w[W], b[W];
-    parameters(w, a.weight, a.param_type, channel, 1.0f);
-    parameters(b, a.bias, a.param_type, channel, 0.0f);
-    const float2 stats = reinterpret_cast<const float2 *>(a.stats)[p.sample * a.groups + group];
+    const Groups groups(p.pack, W, (int)(a.channels / a.groups));
+    const int channel = p.pack * W;
+    Back<T, W, SPLIT> by(a, p.sample, channel, groups.left, groups);
 #pragma unroll
-    for (int j = 0; j < W; j++) w[j] *= stats.y;
+    for (int i = 0; i < P; i++) by.w[i] = mul_rn(by.w[i], by.rate[i]);
     const T *x = static_cast<const T *>(a.x) + p.sample * a.x_sample + channel;
     T *y = static_cast<T *>(a.y) + p.sample * a.positions * a.channels + channel;
 #pragma unroll 4
     for (int r = p.first + p.row; r < p.last; r += s.lanes) {
         Pack<T, W> pack;
-        float v[W];
+        Two v[P];
         pack.load(x + r * a.x_position);
-        pack.get(v);
+        get_pairs<T, W>(v, pack);
 #pragma unroll
-        for (int j = 0; j < W; j++) v[j] = fmaf(v[j] - stats.x, w[j], b[j]);
+        for (int i = 0; i < P; i++) v[i] = fma_rn(sub_rn(v[i], by.mean[i]), by.w[i], by.b[i]);
         activate(v, a.activation);
-        pack.set(v);
-        pack.store(y + r * a.channels);
+        put_pairs<T, W>(y + r * a.channels, v);
     }
 }
 
-// hat and da of W channels.
-template <typename T, int W> struct Back {
-    float w[W], b[W], mean, rate;
-    int kind;
-    __device__ __forceinline__ Back(const ffcvb_group_norm_args &a, long long sample, int channel) : kind(a.activation) {
-        parameters(w, a.weight, a.param_type, channel, 1.0f);
-        parameters(b, a.bias, a.param_type, channel, 0.0f);
-        const float2 stats = reinterpret_cast<const float2 *>(a.stats)[sample * a.groups + channel / (int)(a.channels / a.groups)];
-        mean = stats.x, rate = stats.y;
-    }
-    __device__ __forceinline__ void row(const T *x, const T *dy, float (&hat)[W], float (&da)[W]) const {
-        Pack<T, W> one, other;
-        one.load(x);
-        other.load(dy);
-        one.get(hat);
-        other.get(da);
-        float v[W];
-#pragma unroll
-        for (int j = 0; j < W; j++) {
-            hat[j] = (hat[j] - mean) * rate;
-            v[j] = fmaf(hat[j], w[j], b[j]);
-        }
-        slope(da, v, kind);
-    }
-};
-
 // parts: [samples][slabs][channels]
-template <typename T, int W>
+template <typename T, int W, bool SPLIT>
 __global__ void __launch_bounds__(kThreads) sums_kernel(const __grid_constant__ ffcvb_group_norm_args a, const Slabs s, float2 *parts) {
+    constexpr int P = kPairs<W>;
     __shared__ float2 s_all[kThreads * W];
     wait_for_previous();
     let_next_begin();
     const Place p = place_of(s, (int)a.positions, false);
-    float2 mine[W];
-#pragma unroll
-    for (int j = 0; j < W; j++) mine[j] = make_float2(0.0f, 0.0f);
+    Sums<W> mine;
     if (p.used) {
+        const Groups groups(p.pack, W, (int)(a.channels / a.groups));
         const int channel = p.pack * W;
-        const Back<T, W> back(a, p.sample, channel);
+        const Back<T, W, SPLIT> back(a, p.sample, channel, groups.left, groups);
         const T *x = static_cast<const T *>(a.x) + p.sample * a.x_sample + channel, *dy = static_cast<const T *>(a.dy) + p.sample * a.dy_sample + channel;
 #pragma unroll 2
         for (int r = p.first + p.row; r < p.last; r += s.lanes) {
-            float hat[W], da[W];
-            back.row(x + r * a.x_position, dy + r * a.dy_position, hat, da);
-#pragma unroll
-            for (int j = 0; j < W; j++) {
-                mine[j].x += da[j];
-                mine[j].y = fmaf(da[j], hat[j], mine[j].y);
-            }
+            Pack<T, W> one, other;
+            Two hat[P], da[P];
+            one.load(x + r * a.x_position);
+            other.load(dy + r * a.dy_position);
+            back.row(one, other, hat, da);
+            mine.add(hat, da);
         }
     }
     float2 *to = parts + (p.sample * s.slabs + p.slab) * a.channels + blockIdx.y * s.columns * W;
     const int channels = s.columns * W, there = min(channels, (int)a.channels - (int)blockIdx.y * channels);
     if (p.row < s.lanes)
 #pragma unroll
-        for (int j = 0; j < W; j++) s_all[p.row * channels + threadIdx.x % s.columns * W + j] = mine[j];
+        for (int j = 0; j < W; j++) s_all[p.row * channels + threadIdx.x % s.columns * W + j] = mine.of(j);
     __syncthreads();
     for (int c = threadIdx.x; c < there; c += kThreads) {
-        float2 all = s_all[c];
+        float2 whole = s_all[c];
         for (int k = 1; k < s.lanes; k++) {
-            all.x += s_all[k * channels + c].x;
-            all.y += s_all[k * channels + c].y;
+            whole.x += s_all[k * channels + c].x;
+            whole.y += s_all[k * channels + c].y;
         }
-        to[c] = all;
+        to[c] = whole;
     }
 }
 
@@ -565,19 +738,19 @@ __global__ void __launch_bounds__(kThreads) join_sums_kernel(const __grid_consta
     const long long sample = s.sample + blockIdx.x / a.groups;
     float2 mean = make_float2(0.0f, 0.0f);
     for (int c = group * per + warp; c < (group + 1) * per; c += kThreads / 32) {
-        float2 all = make_float2(0.0f, 0.0f);
+        float2 whole = make_float2(0.0f, 0.0f);
+#pragma unroll 4
         for (int k = lane; k < s.slabs; k += 32) {
             const float2 part = parts[(sample * s.slabs + k) * a.channels + c];
-            all.x += part.x;
-            all.y += part.y;
+            whole.x += part.x;
+            whole.y += part.y;
         }
-        all.x = warp_sum(all.x);
-        all.y = warp_sum(all.y);
-        float w[1];
-        parameters(w, a.weight, a.param_type, c, 1.0f);
-        mean.x = fmaf(w[0], all.x, mean.x);
-        mean.y = fmaf(w[0], all.y, mean.y);
-        if (lane == 0) sums[sample * a.channels + c] = all;
+        whole.x = warp_sum(whole.x);
+        whole.y = warp_sum(whole.y);
+        const float w = parameter(a.weight, a.param_type, c, 1.0f);
+        mean.x = fmaf(w, whole.x, mean.x);
+        mean.y = fmaf(w, whole.y, mean.y);
+        if (lane == 0) sums[sample * a.channels + c] = whole;
     }
     if (lane == 0) s_part[warp] = mean;
     __syncthreads();
@@ -590,50 +763,55 @@ __global__ void __launch_bounds__(kThreads) join_sums_kernel(const __grid_consta
     means[sample * a.groups + group] = make_float2(mean.x * over, mean.y * over);
 }
 
-template <typename T, int W>
+template <typename T, int W, bool SPLIT>
 __global__ void __launch_bounds__(kThreads) gradient_kernel(const __grid_constant__ ffcvb_group_norm_args a, const Slabs s, const float2 *means) {
+    constexpr int P = kPairs<W>;
     wait_for_previous();
     let_next_begin();
     const Place p = place_of(s, (int)a.positions, true);
     if (!p.used) return;
+    const Groups groups(p.pack, W, (int)(a.channels / a.groups));
     const int channel = p.pack * W;
-    const Back<T, W> back(a, p.sample, channel);
-    const float2 less = means[p.sample * a.groups + channel / (int)(a.channels / a.groups)];
+    const Back<T, W, SPLIT> back(a, p.sample, channel, groups.left, groups);
+    Each<W, SPLIT> less, less_hat;
+    const float2 left = means[p.sample * a.groups + groups.left], right = SPLIT ? means[p.sample * a.groups + min(groups.left + 1, (int)a.groups - 1)] : left;
+    less.set(left.x, right.x, groups.split);
+    less_hat.set(left.y, right.y, groups.split);
     const T *x = static_cast<const T *>(a.x) + p.sample * a.x_sample + channel, *dy = static_cast<const T *>(a.dy) + p.sample * a.dy_sample + channel;
     T *dx = static_cast<T *>(a.dx) + p.sample * a.positions * a.channels + channel;
 #pragma unroll 2
     for (int r = p.first + p.row; r < p.last; r += s.lanes) {
-        float hat[W], da[W];
-        back.row(x + r * a.x_position, dy + r * a.dy_position, hat, da);
-#pragma unroll
-        for (int j = 0; j < W; j++) da[j] = back.rate * (fmaf(da[j], back.w[j], -less.x) - hat[j] * less.y);
-        Pack<T, W> out;
-        out.set(da);
-        out.store(dx + r * a.channels);
+        Pack<T, W> one, other;
+        Two hat[P], da[P];
+        one.load(x + r * a.x_position);
+        other.load(dy + r * a.dy_position);
+        back.row(one, other, hat, da);
+        back.gradient(hat, da, less, less_hat);
+        put_pairs<T, W>(dx + r * a.channels, da);
     }
 }
 
 // The parameters' gradients: samples' sums added up, 32 channels per CTA.
-__global__ void __launch_bounds__(kThreads) samples_kernel(const __grid_constant__ ffcvb_group_norm_args a, const float2 *sums) {
-    __shared__ float2 s_part[kThreads / 32][32];
+__global__ void __launch_bounds__(1024) samples_kernel(const __grid_constant__ ffcvb_group_norm_args a, const float2 *sums) {
+    __shared__ float2 s_part[32][32];
     wait_for_previous();
     let_next_begin();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const long long c = blockIdx.x * 32ll + lane;
-    float2 all = make_float2(0.0f, 0.0f);
+    float2 whole = make_float2(0.0f, 0.0f);
     if (c < a.channels)
 #pragma unroll 4
-        for (long long n = warp; n < a.samples; n += kThreads / 32) {
+        for (long long n = warp; n < a.samples; n += 32) {
             const float2 part = sums[n * a.channels + c];
-            all.x += part.x;
-            all.y += part.y;
+            whole.x += part.x;
+            whole.y += part.y;
         }
-    s_part[warp][lane] = all;
+    s_part[warp][lane] = whole;
     __syncthreads();
     if (warp || c >= a.channels) return;
-    for (int k = 1; k < kThreads / 32; k++) {
-        all.x += s_part[k][lane].x;
-        all.y += s_part[k][lane].y;
+    for (int k = 1; k < 32; k++) {
+        whole.x += s_part[k][lane].x;
+        whole.y += s_part[k][lane].y;
     }
     auto put = [&](void *to, float v) {
         if (!to) return;
@@ -644,28 +822,29 @@ __global__ void __launch_bounds__(kThreads) samples_kernel(const __grid_constant
         else
             static_cast<__nv_bfloat16 *>(to)[c] = from_float<__nv_bfloat16>(v);
     };
-    put(a.dbias, all.x);
-    put(a.dweight, all.y);
+    put(a.dbias, whole.x);
+    put(a.dweight, whole.y);
 }
 
 // ---- the host's part -------------------------------------------------------------------------------------------------
 
 // Bytes that a CTA holds at most: two of them on an SM; and what it holds rather, so that four are.
-constexpr int64_t kMostHeld = 100 * 1024, kHeld = 52 * 1024;
+constexpr int64_t kMostHeld = 100 * 1024, kHeld = 51 * 1024;
 // Bytes of neighbouring channels that a CTA reads at least, where there are as many.
 constexpr int64_t kNeighbours = 64;
 // Bytes of x of a pass over all its slabs, before they are read again: what the caches keep.
 constexpr int64_t kCached = 40ll << 20;
 
-// Values of a pack: all of one group, and where they begin as their size has it.
+// Values of a pack: of one group or of two neighbouring ones (`split`), and where they begin as their size has it.
 int width_of(const ffcvb_group_norm_args &a, bool backward) {
     const int size = type_size(a.type);
     int w = 16 / size;
     auto fits = [&](const void *p, int64_t sample, int64_t position) {
         return reinterpret_cast<uintptr_t>(p) % (w * size) == 0 && (a.samples <= 1 || sample % w == 0) && (a.positions <= 1 || position % w == 0);
     };
+    const int64_t per = a.channels / a.groups;
     for (; w > 1; w /= 2)
-        if (a.channels / a.groups % w == 0 && fits(a.x, a.x_sample, a.x_position) &&
+        if (a.channels % w == 0 && (per >= w || w == 2 * per) && fits(a.x, a.x_sample, a.x_position) &&
             (backward ? fits(a.dy, a.dy_sample, a.dy_position) && (!a.dx || fits(a.dx, 0, 0)) : fits(a.y, 0, 0)))
             break;
     return w;
@@ -673,7 +852,7 @@ int width_of(const ffcvb_group_norm_args &a, bool backward) {
 
 struct Plan {
     int width;
-    bool held;
+    bool split, held;
     Deal deal;
     int64_t room;     // bytes of shared memory
     Slabs slabs;
@@ -685,42 +864,42 @@ Plan plan_of(const ffcvb_group_norm_args &a, bool backward) {
     Plan p{};
     const int size = type_size(a.type), w = p.width = width_of(a, backward);
     const int64_t per = a.channels / a.groups;
+    p.split = per % w != 0;
     Deal &d = p.deal;
     d.groups = 1;
-    while (d.groups * 2 <= kMostGroups && a.groups % (d.groups * 2) == 0 && d.groups * per * size < kNeighbours) d.groups *= 2;
+    while (d.groups * 2 <= kMostGroups && a.groups % (d.groups * 2) == 0 && (d.groups * per * size < kNeighbours || d.groups * per % w != 0)) d.groups *= 2;
     const int64_t packs = d.groups * per / w;
-    if (packs <= kThreads) {
+    if (packs <= kHeldThreads && d.groups * per % w == 0 && a.samples <= 65535) {
         d.packs = (int)packs;
-        d.lanes = (int)std::min<int64_t>(kThreads / packs, std::max<int64_t>(a.positions, 1));
+        d.per = (int)per;
+        d.lanes = (int)std::min<int64_t>(kHeldThreads / packs, std::max<int64_t>(a.positions, 1));
         auto room_of = [&](int ctas) {
             const int64_t rows = (a.positions + ctas - 1) / ctas, turns = (rows + d.lanes - 1) / d.lanes;
-            return turns * kThreads * w * size * (backward ? 2 : 1) + (backward ? ((d.lanes + ctas) * packs * w + 1) / 2 * 16 : 0);
+            return turns * kHeldThreads * w * size * (backward ? 2 : 1) + (backward ? ((sum_rows(d.packs, d.lanes) + ctas) * packs * w + 1) / 2 * 16 : 0);
         };
         for (d.ctas = 1; d.ctas < 8 && room_of(d.ctas) > kHeld; d.ctas *= 2) {}
         p.room = room_of(d.ctas);
         p.held = p.room <= kMostHeld;
         d.rows = (int)((a.positions + d.ctas - 1) / d.ctas);
-        p.held &= a.samples * (a.groups / d.groups) * d.ctas <= INT32_MAX;
     }
     Slabs &s = p.slabs;
     s.packs = (int)(a.channels / w);
     s.columns = std::min(s.packs, kThreads);
     s.lanes = std::max(1, kThreads / s.columns);
-    // slabs of 16 to 64 positions of a thread, as many as bring two rounds of CTAs to all SMs
-    const int64_t all = a.samples * ((s.packs + s.columns - 1) / s.columns);
-    int64_t turns = a.positions * all / std::max<int64_t>(1, (int64_t)s.lanes * kSms * 16);
-    turns = std::clamp<int64_t>(turns, 8, 64);
-    s.rows = (int)std::min<int64_t>(a.positions, turns * s.lanes);
-    s.slabs = s.rows ? (int)((a.positions + s.rows - 1) / s.rows) : 0;
     const int64_t sample_bytes = a.positions * a.channels * size * (backward ? 2 : 1);
     p.samples = std::clamp<int64_t>(kCached / std::max<int64_t>(1, sample_bytes), 1, a.samples);
+    // slabs of 4 to 64 positions of a thread, as many as bring five CTAs to every SM
+    const int64_t ctas = p.samples * ((s.packs + s.columns - 1) / s.columns);
+    const int64_t turns = std::clamp<int64_t>((a.positions * ctas + (int64_t)s.lanes * kSms * 5 - 1) / ((int64_t)s.lanes * kSms * 5), 4, 64);
+    s.rows = (int)std::min<int64_t>(a.positions, turns * s.lanes);
+    s.slabs = s.rows ? (int)((a.positions + s.rows - 1) / s.rows) : 0;
     int64_t at = 0;
     auto take = [&](bool wanted, int64_t bytes) {
         const int64_t here = at;
         if (wanted) at += (bytes + 255) / 256 * 256;
         return here;
     };
-    p.parts = take(!p.held, a.samples * s.slabs * (backward ? a.channels : s.packs) * 8);
+    p.parts = take(!p.held, a.samples * s.slabs * (backward ? a.channels : s.packs * (p.split ? 2 : 1)) * 8);
     p.means = take(!p.held && backward, a.samples * a.groups * 8);
     p.sums = take(backward, a.samples * a.channels * 8);
     p.bytes = at;
@@ -739,16 +918,23 @@ const char *wrong(const ffcvb_group_norm_args &a, bool backward) {
     return nullptr;
 }
 
-// Calls f with a value of the type, and the width, of a call's packs.
-template <typename T, typename F> void with_width(int w, F &&f) {
+// Calls f with a value of the type, the width of a call's packs, and whether they have two groups.
+template <int W> using Width = std::integral_constant<int, W>;
+template <typename T, typename F> void with_width(int w, bool split, F &&f) {
+    auto with = [&](auto width) {
+        if (split)
+            f(T{}, width, std::true_type{});
+        else
+            f(T{}, width, std::false_type{});
+    };
     if constexpr (sizeof(T) == 2)
-        if (w == 8) return f(T{}, std::integral_constant<int, 8>{});
-    if (w == 4) return f(T{}, std::integral_constant<int, 4>{});
-    if (w == 2) return f(T{}, std::integral_constant<int, 2>{});
-    f(T{}, std::integral_constant<int, 1>{});
+        if (w == 8) return with(Width<8>{});
+    if (w == 4) return with(Width<4>{});
+    if (w == 2) return with(Width<2>{});
+    f(T{}, Width<1>{}, std::false_type{});
 }
 
-template <typename... Params, typename... Given> void launch_cluster(void (*kernel)(Params...), int64_t ctas, int cluster, int64_t room, cudaStream_t stream, Given &&...given) {
+template <typename... Params, typename... Given> void launch_cluster(void (*kernel)(Params...), dim3 grid, int cluster, int64_t room, cudaStream_t stream, Given &&...given) {
     cudaLaunchConfig_t how{};
     cudaLaunchAttribute with[2] = {};
     with[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -756,8 +942,8 @@ template <typename... Params, typename... Given> void launch_cluster(void (*kern
     with[1].id = cudaLaunchAttributeClusterDimension;
     with[1].val.clusterDim.x = cluster;
     with[1].val.clusterDim.y = with[1].val.clusterDim.z = 1;
-    how.gridDim = dim3((unsigned)ctas);
-    how.blockDim = dim3(kThreads);
+    how.gridDim = grid;
+    how.blockDim = dim3(kHeldThreads);
     how.dynamicSmemBytes = room;
     how.stream = stream;
     how.attrs = with;
@@ -773,11 +959,12 @@ template <typename... Params, typename... Given> void launch_cluster(void (*kern
 void run_forward(const ffcvb_group_norm_args &a, uint8_t *room, cudaStream_t st) {
     const Plan p = plan_of(a, false);
     with_type(a.type, [&](auto zero) {
-        with_width<decltype(zero)>(p.width, [&](auto of, auto width) {
+        with_width<decltype(zero)>(p.width, p.split, [&](auto of, auto width, auto split) {
             using T = decltype(of);
             constexpr int W = decltype(width)::value;
+            constexpr bool SPLIT = decltype(split)::value;
             if (p.held) {
-                launch_cluster(held_forward_kernel<T, W>, a.samples * (a.groups / p.deal.groups) * p.deal.ctas, p.deal.ctas, p.room, st, a, p.deal);
+                launch_cluster(held_forward_kernel<T, W, SPLIT>, dim3((unsigned)(a.groups / p.deal.groups * p.deal.ctas), (unsigned)a.samples), p.deal.ctas, p.room, st, a, p.deal);
                 return;
             }
             float2 *parts = reinterpret_cast<float2 *>(room + p.parts);
@@ -785,9 +972,9 @@ void run_forward(const ffcvb_group_norm_args &a, uint8_t *room, cudaStream_t st)
             for (s.sample = 0; s.sample < a.samples; s.sample += p.samples) {
                 const int64_t samples = std::min(p.samples, a.samples - s.sample);
                 const dim3 grid((unsigned)(samples * s.slabs), (unsigned)((s.packs + s.columns - 1) / s.columns));
-                launch_early(moments_kernel<T, W>, grid, kThreads, 0, st, a, s, parts);
-                launch_early(join_moments_kernel<W>, (unsigned)((samples * a.groups + 7) / 8), kThreads, 0, st, a, s, (int)samples, parts);
-                launch_early(values_kernel<T, W>, grid, kThreads, 0, st, a, s);
+                launch_early(moments_kernel<T, W, SPLIT>, grid, kThreads, 0, st, a, s, parts);
+                launch_early(join_moments_kernel<W, SPLIT>, (unsigned)(samples * a.groups), kThreads, 0, st, a, s, parts);
+                launch_early(values_kernel<T, W, SPLIT>, grid, kThreads, 0, st, a, s);
             }
         });
     });
@@ -797,11 +984,12 @@ void run_backward(const ffcvb_group_norm_args &a, uint8_t *room, cudaStream_t st
     const Plan p = plan_of(a, true);
     float2 *sums = reinterpret_cast<float2 *>(room + p.sums);
     with_type(a.type, [&](auto zero) {
-        with_width<decltype(zero)>(p.width, [&](auto of, auto width) {
+        with_width<decltype(zero)>(p.width, p.split, [&](auto of, auto width, auto split) {
             using T = decltype(of);
             constexpr int W = decltype(width)::value;
+            constexpr bool SPLIT = decltype(split)::value;
             if (p.held) {
-                launch_cluster(held_backward_kernel<T, W>, a.samples * (a.groups / p.deal.groups) * p.deal.ctas, p.deal.ctas, p.room, st, a, p.deal, sums);
+                launch_cluster(held_backward_kernel<T, W, SPLIT>, dim3((unsigned)(a.groups / p.deal.groups * p.deal.ctas), (unsigned)a.samples), p.deal.ctas, p.room, st, a, p.deal, sums);
                 return;
             }
             float2 *parts = reinterpret_cast<float2 *>(room + p.parts), *means = reinterpret_cast<float2 *>(room + p.means);
@@ -809,13 +997,13 @@ void run_backward(const ffcvb_group_norm_args &a, uint8_t *room, cudaStream_t st
             for (s.sample = 0; s.sample < a.samples; s.sample += p.samples) {
                 const int64_t samples = std::min(p.samples, a.samples - s.sample);
                 const dim3 grid((unsigned)(samples * s.slabs), (unsigned)((s.packs + s.columns - 1) / s.columns));
-                launch_early(sums_kernel<T, W>, grid, kThreads, 0, st, a, s, parts);
+                launch_early(sums_kernel<T, W, SPLIT>, grid, kThreads, 0, st, a, s, parts);
                 launch_early(join_sums_kernel, (unsigned)(samples * a.groups), kThreads, 0, st, a, s, parts, sums, means);
-                if (a.dx) launch_early(gradient_kernel<T, W>, grid, kThreads, 0, st, a, s, means);
+                if (a.dx) launch_early(gradient_kernel<T, W, SPLIT>, grid, kThreads, 0, st, a, s, means);
             }
         });
     });
-    if (a.dweight || a.dbias) launch_early(samples_kernel, (unsigned)((a.channels + 31) / 32), kThreads, 0, st, a, sums);
+    if (a.dweight || a.dbias) launch_early(samples_kernel, (unsigned)((a.channels + 31) / 32), 1024, 0, st, a, sums);
 }
 
 int call(const ffcvb_group_norm_args *args, void *workspace, void *stream, bool backward) {
