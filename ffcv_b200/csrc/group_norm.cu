@@ -55,24 +55,23 @@ __device__ __forceinline__ float exp2_of(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// 1 / v, each at most 2^60: one reciprocal for two, of their product.
-__device__ __forceinline__ Two inverse(Two v) {
+__device__ __forceinline__ float inverse_of(float v) {
     float r;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v.lo() * v.hi()));
-    return mul_rn(Two(r, r), Two(v.hi(), v.lo()));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
 }
 __device__ __forceinline__ Two all(float v) { return Two(v, v); }
 
-// 1 / (1 + exp(-a)); 2^-60 instead of less.  (A NaN is none here, so that it stays with its own value; what the gate is multiplied with has it.)
+// 1 / (1 + exp(-a))
 __device__ __forceinline__ Two gate_of(Two a) {
-    const Two t = mul_rn(a, all(-kLog2e));
-    return inverse(add_rn(Two(exp2_of(fminf(t.lo(), 60.0f)), exp2_of(fminf(t.hi(), 60.0f))), all(1.0f)));
+    const Two t = mul_rn(a, all(-kLog2e)), e = add_rn(Two(exp2_of(t.lo()), exp2_of(t.hi())), all(1.0f));
+    return Two(inverse_of(e.lo()), inverse_of(e.hi()));
 }
 // The normal distribution's density at a, and its integral up to a.  With z = |a| / sqrt(2) and t = 1 / (1 + 0.42 z) the integral up to -|a| is
 // t P(t) exp(-z^2) / 2; P is a polynomial fitted to that for z up to 6, to 3.3e-8 of the value.
 __device__ __forceinline__ void normal(Two a, Two &density, Two &integral) {
-    const Two size(fminf(fabsf(a.lo()), 30.0f), fminf(fabsf(a.hi()), 30.0f));
-    const Two t = inverse(fma_rn(size, all(0.42f * 0.70710678118654752f), all(1.0f)));
+    const Two u = fma_rn(Two(fabsf(a.lo()), fabsf(a.hi())), all(0.42f * 0.70710678118654752f), all(1.0f));
+    const Two t(inverse_of(u.lo()), inverse_of(u.hi()));
     const Two square = mul_rn(mul_rn(a, a), all(-0.5f * kLog2e)), e(exp2_of(square.lo()), exp2_of(square.hi()));
     Two p = fma_rn(all(0.5f * 0.076194151358683f), t, all(0.5f * -0.3458746854890851f));
     p = fma_rn(p, t, all(0.5f * 0.4864512135112419f));
@@ -81,8 +80,8 @@ __device__ __forceinline__ void normal(Two a, Two &density, Two &integral) {
     p = fma_rn(p, t, all(0.5f * 0.18682665698819034f));
     p = fma_rn(p, t, all(0.5f * 0.24094708374661222f));
     p = fma_rn(p, t, all(0.5f * 0.23672753345776956f));
-    const Two tail = mul_rn(mul_rn(p, t), e);
-    integral = Two(a.lo() > 0.0f ? 1.0f - tail.lo() : tail.lo(), a.hi() > 0.0f ? 1.0f - tail.hi() : tail.hi());
+    const Two tail = mul_rn(mul_rn(p, t), e), rest = sub_rn(all(1.0f), tail);
+    integral = Two(a.lo() > 0.0f ? rest.lo() : tail.lo(), a.hi() > 0.0f ? rest.hi() : tail.hi());
     density = mul_rn(e, all(0.39894228040143268f));
 }
 
@@ -144,7 +143,8 @@ template <typename T, int W> __device__ __forceinline__ void put_pairs(T *to, co
 // Which groups a pack's channels are of: `left` those before `split`, the next one the others (SPLIT; else all are of one).
 struct Groups {
     int left, split;
-    __device__ __forceinline__ Groups(int pack, int w, int per) : left(pack * w / per), split(min(w, (pack * w / per + 1) * per - pack * w)) {}
+    // (the channel's middle over `per`: exact for as many channels as there may be)
+    __device__ __forceinline__ Groups(int pack, int w, int per) : left((int)(((float)(pack * w) + 0.5f) / (float)per)), split(min(w, (left + 1) * per - pack * w)) {}
 };
 // A number of a pack's groups for each of its channels.
 template <int W, bool SPLIT> struct Each {
@@ -165,57 +165,53 @@ struct Moments {
         mean += step;
         n = both;
     }
-    // of a warp; lane 0 has the result
-    __device__ __forceinline__ void join_lanes() {
+    // of groups of LANES lanes; the lowest has the result
+    template <int LANES = 32> __device__ __forceinline__ void join_lanes() {
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1)
+        for (int o = LANES / 2; o > 0; o >>= 1)
             join(Moments{__shfl_down_sync(0xffffffffu, n, o), __shfl_down_sync(0xffffffffu, mean, o), __shfl_down_sync(0xffffffffu, squares, o)});
     }
     __device__ __forceinline__ float rate(float eps) const { return rsqrtf(squares / n + eps); }
 };
 
-// A thread's values of W channels, each relative to its first one.
-template <int W> struct Collected {
+// A thread's values of W channels, added up relative to a pivot for each group.  With the mean of some of the values as the pivot, m of the n that are
+// added up, its square's distance from their mean is at most n / m variances, and the variance has so many roundings of 2^-24 of error at most: n / m is a
+// thread's number of positions here.
+template <int W, bool SPLIT> struct Collected {
     static constexpr int P = kPairs<W>;
-    Two first[P], sum[P], squares[P];
-    int rows;
-    __device__ __forceinline__ Collected() : rows(0) {
+    Each<W, SPLIT> pivot;
+    Two sum[P], squares[P];
+    __device__ __forceinline__ Collected() {
 #pragma unroll
-        for (int i = 0; i < P; i++) first[i] = sum[i] = squares[i] = all(0.0f);
+        for (int i = 0; i < P; i++) sum[i] = squares[i] = all(0.0f);
     }
     __device__ __forceinline__ void add(const Two (&v)[P]) {
-        if (rows++ == 0)
-#pragma unroll
-            for (int i = 0; i < P; i++) first[i] = v[i];
 #pragma unroll
         for (int i = 0; i < P; i++) {
-            const Two d = sub_rn(v[i], first[i]);
+            const Two d = sub_rn(v[i], pivot[i]);
             sum[i] = add_rn(sum[i], d);
             squares[i] = fma_rn(d, d, squares[i]);
         }
     }
-    // of channels from..to
-    __device__ __forceinline__ Moments moments(int from, int to) const {
-        if (rows == 0 || from >= to) return Moments{0.0f, 0.0f, 0.0f};
-        const float n = (float)rows, over = 1.0f / n;
-        float mean[W], around = 0.0f, base = 0.0f, level = 0.0f;
+    // Sums of the channels before `split`, or of those from it on.
+    static __device__ __forceinline__ float of(const Two (&v)[P], int split, bool right) {
+        if constexpr (!SPLIT) {
+            Two s = v[0];
 #pragma unroll
-        for (int j = 0; j < W; j++) {
-            const float s = sum[j / 2].half(j & 1), away = s * over, left = squares[j / 2].half(j & 1) - s * away;
-            mean[j] = first[j / 2].half(j & 1) + away;
-            if (j == from) base = mean[j];
-            if (j < from || j >= to) continue;
-            around += left < 0.0f ? 0.0f : left; // (NaN stays)
-            level += mean[j] - base;
+            for (int i = 1; i < P; i++) s = add_rn(s, v[i]);
+            return W == 1 ? s.lo() : s.lo() + s.hi();
         }
-        level = base + level / (float)(to - from);
-        float apart = 0.0f;
+        float s = 0.0f;
 #pragma unroll
-        for (int j = 0; j < W; j++)
-            if (j >= from && j < to) apart = fmaf(mean[j] - level, mean[j] - level, apart);
-        return Moments{n * (float)(to - from), level, fmaf(n, apart, around)};
+        for (int j = 0; j < W; j++) s += (j < split) != right ? v[j / 2].half(j & 1) : 0.0f;
+        return s;
     }
 };
+// What is left of sums of n values around a pivot.
+__device__ __forceinline__ Moments moments_of(float n, float pivot, float sum, float squares) {
+    const float away = __fdividef(sum, fmaxf(n, 1.0f)), around = squares - sum * away;
+    return Moments{n, pivot + away, around < 0.0f ? 0.0f : around}; // (NaN stays)
+}
 
 // W neighbouring parameters in pairs, or what stands for them.
 __device__ __forceinline__ float parameter(const void *from, int type, long long c, float other) {
@@ -227,6 +223,15 @@ __device__ __forceinline__ float parameter(const void *from, int type, long long
 template <int W> __device__ __forceinline__ void parameters(Two (&v)[kPairs<W>], const void *from, int type, long long c, float other) {
     float f[W];
     auto of = [&](auto *at) {
+        using T = std::remove_const_t<std::remove_pointer_t<decltype(at)>>;
+        if constexpr (W * sizeof(T) <= 16) {
+            if (reinterpret_cast<uintptr_t>(at) % 16 == 0) { // (c is a multiple of W)
+                Pack<T, W> pack;
+                pack.load(at + c);
+                pack.get(f);
+                return;
+            }
+        }
 #pragma unroll
         for (int j = 0; j < W; j++) f[j] = to_float(at[c + j]);
     };
@@ -268,30 +273,33 @@ __device__ __forceinline__ void store_there(const void *mine, uint32_t rank, flo
 
 // ---- held: a CTA or a cluster has some groups of a sample at all positions ---------------------------------------------
 
-// Groups of a CTA, packs of a position in them, of which `lanes` positions at once; positions of a CTA; CTAs of a cluster.
+// Groups of a CTA, packs of a position in them, of which `lanes` positions at once; positions of a CTA; CTAs of a cluster; channels of a group.
 struct Deal {
-    int groups, packs, lanes, rows, ctas, per; // (per: channels of a group)
+    int groups, packs, lanes, rows, ctas, per;
 };
 // Of a CTA: its cluster's rank, first group and sample; its thread's row and pack.
 struct Held {
     int rank, group0, row, pack, first, last;
     long long sample;
     __device__ __forceinline__ Held(const Deal &deal, int positions) {
-        const int log = 31 - __clz(deal.ctas); // (1, 2, 4 or 8)
-        rank = blockIdx.x & (deal.ctas - 1);
-        group0 = (blockIdx.x >> log) * deal.groups;
+        rank = blockIdx.x & (deal.ctas - 1); // (1, 2, 4 or 8)
+        group0 = (blockIdx.x >> (31 - __clz(deal.ctas))) * deal.groups;
         sample = blockIdx.y;
-        row = threadIdx.x / deal.packs;
+        row = (int)(((float)threadIdx.x + 0.5f) / (float)deal.packs);
         pack = threadIdx.x - row * deal.packs;
         first = rank * deal.rows;
         last = min(first + deal.rows, positions);
     }
 };
+// Lanes of a warp that have the same pack of a power of two of them can be joined; then a warp has one row of partial results, else each row has.
+__host__ __device__ constexpr bool joined(int packs) { return packs <= 32 && (packs & (packs - 1)) == 0; }
+__host__ __device__ constexpr int part_rows(int packs, int lanes, int threads) { return joined(packs) ? threads / 32 : lanes; }
 
+// s_moments[side][row][pack]: of a CTA's packs, from all its rows.
 template <typename T, int W, bool SPLIT>
 __global__ void __launch_bounds__(kHeldThreads) held_forward_kernel(const __grid_constant__ ffcvb_group_norm_args a, const Deal deal) {
-    constexpr int P = kPairs<W>, SIDES = SPLIT ? 2 : 1;
-    __shared__ float s_moments[SIDES][3][kHeldThreads];
+    constexpr int P = kPairs<W>, SIDES = SPLIT ? 2 : 1, N = kHeldThreads;
+    __shared__ Moments s_moments[SIDES][N];
     __shared__ Moments s_there[8][kMostGroups]; // of the cluster's CTAs
     __shared__ float2 s_stats[kMostGroups];
     extern __shared__ uint4 s_held[];
@@ -299,18 +307,15 @@ __global__ void __launch_bounds__(kHeldThreads) held_forward_kernel(const __grid
     let_next_begin();
     if (deal.ctas > 1) cluster_begun();
     const Held me(deal, (int)a.positions);
-    const int per = deal.per, rank = me.rank, group0 = me.group0, row = me.row, pack = me.pack, first = me.first, last = me.last;
-    const long long sample = me.sample;
-    const Groups groups(pack, W, per);
-    const int channel = group0 * per + pack * W;
-    const bool used = row < deal.lanes;
-    const T *x = static_cast<const T *>(a.x) + sample * a.x_sample + channel;
+    const Groups groups(me.pack, W, deal.per);
+    const int channel = me.group0 * deal.per + me.pack * W;
+    const bool used = me.row < deal.lanes;
     Pack<T, W> *held = reinterpret_cast<Pack<T, W> *>(s_held) + threadIdx.x;
     if (used) {
-        const T *from = x + (first + row) * a.x_position;
+        const T *from = static_cast<const T *>(a.x) + me.sample * a.x_sample + (me.first + me.row) * a.x_position + channel;
         const long long step = deal.lanes * a.x_position;
         Pack<T, W> *to = held;
-        for (int r = first + row; r < last; r += deal.lanes, to += kHeldThreads, from += step) copy_pack(to, from);
+        for (int r = me.first + me.row; r < me.last; r += deal.lanes, to += N, from += step) copy_pack(to, from);
     }
     Two w[P], b[P];
     if (used) {
@@ -319,42 +324,79 @@ __global__ void __launch_bounds__(kHeldThreads) held_forward_kernel(const __grid
     }
     copies_done();
     {
-        Collected<W> values;
-        if (used) {
-            const Pack<T, W> *from = held;
-#pragma unroll 2
-            for (int r = first + row; r < last; r += deal.lanes, from += kHeldThreads) {
-                Two v[P];
-                get_pairs<T, W>(v, *from);
-                values.add(v);
-            }
+        Collected<W, SPLIT> values;
+        const int turns = used && me.first + me.row < me.last ? (me.last - me.first - me.row - 1) / deal.lanes + 1 : 0;
+        // the pivots: means of the thread's first values; of those of the warp's lanes with the same pack, where they are joined
+        const float there[2] = {SPLIT ? (float)groups.split : (float)W, (float)(W - groups.split)};
+        float pivot[2] = {0.0f, 0.0f}, n[2];
+        if (turns) {
+            Two v[P];
+            get_pairs<T, W>(v, *held);
+#pragma unroll
+            for (int side = 0; side < SIDES; side++) pivot[side] = values.of(v, groups.split, side);
         }
 #pragma unroll
         for (int side = 0; side < SIDES; side++) {
-            const Moments mine = side ? values.moments(groups.split, W) : values.moments(0, SPLIT ? groups.split : W);
-            s_moments[side][0][threadIdx.x] = mine.n, s_moments[side][1][threadIdx.x] = mine.mean, s_moments[side][2][threadIdx.x] = mine.squares;
+            float m = turns ? there[side] : 0.0f;
+            n[side] = (float)turns * there[side];
+            if (joined(deal.packs))
+                for (int o = 16; o >= deal.packs; o >>= 1) {
+                    pivot[side] += __shfl_xor_sync(0xffffffffu, pivot[side], o);
+                    m += __shfl_xor_sync(0xffffffffu, m, o);
+                    n[side] += __shfl_xor_sync(0xffffffffu, n[side], o);
+                }
+            pivot[side] = __fdividef(pivot[side], fmaxf(m, 1.0f));
+        }
+        values.pivot.set(pivot[0], pivot[SIDES - 1], groups.split);
+        const Pack<T, W> *from = held;
+#pragma unroll 2
+        for (int k = 0; k < turns; k++, from += N) {
+            Two v[P];
+            get_pairs<T, W>(v, *from);
+            values.add(v);
+        }
+#pragma unroll
+        for (int side = 0; side < SIDES; side++) {
+            float sum = values.of(values.sum, groups.split, side), squares = values.of(values.squares, groups.split, side);
+            int at = threadIdx.x; // (row by row)
+            bool writes = used;
+            if (joined(deal.packs)) {
+                for (int o = 16; o >= deal.packs; o >>= 1) {
+                    sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                    squares += __shfl_xor_sync(0xffffffffu, squares, o);
+                }
+                at = (threadIdx.x >> 5) * deal.packs + (threadIdx.x & 31);
+                writes = (threadIdx.x & 31) < deal.packs;
+            }
+            if (writes) s_moments[side][at] = moments_of(n[side], pivot[side], sum, squares);
         }
     }
     __syncthreads();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (deal.ctas > 1) cluster_wait(); // all have begun
-    for (int g = warp; g < deal.groups; g += kHeldThreads / 32) {
-        const int pack0 = g * per / W, each = ((g + 1) * per - 1) / W - pack0 + 1; // packs of a group
+    // a quarter of a warp has a group: its packs, in all rows of partial results
+    const int rows = part_rows(deal.packs, deal.lanes, N);
+    for (int g0 = threadIdx.x >> 5 << 2; g0 < deal.groups; g0 += N / 8) {
+        const int g = g0 + (threadIdx.x & 31) / 8, e0 = threadIdx.x & 7;
         Moments found{0.0f, 0.0f, 0.0f};
-        for (int e = lane; e < deal.lanes * each; e += 32) {
-            const int k = pack0 + e % each, t = e / each * deal.packs + k, side = SPLIT && k * W / per != g;
-            found.join(Moments{s_moments[side][0][t], s_moments[side][1][t], s_moments[side][2][t]});
+        if (g < deal.groups) {
+            const int pack0 = g * deal.per / W, each = ((g + 1) * deal.per - 1) / W - pack0 + 1;
+            for (int k = pack0; k < pack0 + each; k++) {
+                const int side = SPLIT && Groups(k, W, deal.per).left != g;
+                for (int r = e0; r < rows; r += 8) found.join(s_moments[side][r * deal.packs + k]);
+            }
         }
-        found.join_lanes();
-        const float n = __shfl_sync(0xffffffffu, found.n, 0), mean = __shfl_sync(0xffffffffu, found.mean, 0), squares = __shfl_sync(0xffffffffu, found.squares, 0);
-        if (lane < deal.ctas) {
-            Moments *to = &s_there[rank][g];
+        found.join_lanes<8>();
+        found.n = __shfl_sync(0xffffffffu, found.n, threadIdx.x & 24);
+        found.mean = __shfl_sync(0xffffffffu, found.mean, threadIdx.x & 24);
+        found.squares = __shfl_sync(0xffffffffu, found.squares, threadIdx.x & 24);
+        if (g < deal.groups && e0 < deal.ctas) {
+            Moments *to = &s_there[me.rank][g];
             if (deal.ctas == 1) {
-                *to = Moments{n, mean, squares};
+                *to = found;
             } else {
-                store_there(&to->n, lane, n);
-                store_there(&to->mean, lane, mean);
-                store_there(&to->squares, lane, squares);
+                store_there(&to->n, e0, found.n);
+                store_there(&to->mean, e0, found.mean);
+                store_there(&to->squares, e0, found.squares);
             }
         }
     }
@@ -367,7 +409,7 @@ __global__ void __launch_bounds__(kHeldThreads) held_forward_kernel(const __grid
         for (int k = 1; k < deal.ctas; k++) whole.join(s_there[k][threadIdx.x]);
         const float2 stats = make_float2(whole.mean, whole.rate(a.eps));
         s_stats[threadIdx.x] = stats;
-        if (rank == 0) reinterpret_cast<float2 *>(a.stats)[sample * a.groups + group0 + threadIdx.x] = stats;
+        if (me.rank == 0) reinterpret_cast<float2 *>(a.stats)[me.sample * a.groups + me.group0 + threadIdx.x] = stats;
     }
     __syncthreads();
     if (!used) return;
@@ -377,11 +419,11 @@ __global__ void __launch_bounds__(kHeldThreads) held_forward_kernel(const __grid
     rates.set(left.y, right.y, groups.split);
 #pragma unroll
     for (int i = 0; i < P; i++) w[i] = mul_rn(w[i], rates[i]);
-    T *to = static_cast<T *>(a.y) + (sample * a.positions + first + row) * a.channels + channel;
+    T *to = static_cast<T *>(a.y) + (me.sample * a.positions + me.first + me.row) * a.channels + channel;
     const long long step = deal.lanes * a.channels;
     const Pack<T, W> *from = held;
 #pragma unroll 2
-    for (int r = first + row; r < last; r += deal.lanes, from += kHeldThreads, to += step) {
+    for (int r = me.first + me.row; r < me.last; r += deal.lanes, from += N, to += step) {
         Two v[P];
         get_pairs<T, W>(v, *from);
 #pragma unroll
@@ -406,6 +448,11 @@ template <int W> struct Sums {
             hat[i] = fma_rn(d[i], h[i], hat[i]);
         }
     }
+    // (from sums of da c)
+    template <bool SPLIT> __device__ __forceinline__ void times(const Each<W, SPLIT> &rate) {
+#pragma unroll
+        for (int i = 0; i < P; i++) hat[i] = mul_rn(hat[i], rate[i]);
+    }
     __device__ __forceinline__ float2 of(int j) const { return make_float2(da[j / 2].half(j & 1), hat[j / 2].half(j & 1)); }
     // Lanes of a warp that have the same pack, `packs` (a power of two) apart: the lowest has the sum.
     __device__ __forceinline__ void join_lanes(int packs) {
@@ -417,13 +464,10 @@ template <int W> struct Sums {
             }
     }
 };
-// Rows of partial sums that a CTA's threads leave in shared memory: one per warp where a warp's lanes can be joined, else one per position at once.
-__host__ __device__ constexpr bool joined(int packs) { return packs <= 32 && (packs & (packs - 1)) == 0; }
-__host__ __device__ constexpr int sum_rows(int packs, int lanes) { return joined(packs) ? kHeldThreads / 32 : lanes; }
 
-// Sums of a CTA's threads joined over its positions: s_sums[channel]; `s_all` is room for sum_rows() times the channels.
+// Sums of a CTA's threads joined over its positions: s_sums[channel]; `s_all` is room for part_rows() times the channels.
 template <int W> __device__ __forceinline__ void channel_sums(Sums<W> &mine, bool used, int row, int pack, int lanes, int packs, float2 *s_all, float2 *s_sums) {
-    const int channels = packs * W, rows = sum_rows(packs, lanes);
+    const int channels = packs * W, rows = part_rows(packs, lanes, kHeldThreads);
     bool writes = used;
     if (joined(packs)) {
         mine.join_lanes(packs);
@@ -434,8 +478,9 @@ template <int W> __device__ __forceinline__ void channel_sums(Sums<W> &mine, boo
 #pragma unroll
         for (int j = 0; j < W; j++) s_all[row * channels + pack * W + j] = mine.of(j);
     __syncthreads();
-    // rows are halved until one is left, always in the same order
-    for (int n = rows; n > 1;) {
+    // rows are halved until at most four are left, always in the same order
+    int n = rows;
+    while (n > 4) {
         const int half = (n + 1) / 2;
         for (int i = threadIdx.x; i < (n - half) * channels; i += kHeldThreads) {
             s_all[i].x += s_all[i + half * channels].x;
@@ -444,13 +489,20 @@ template <int W> __device__ __forceinline__ void channel_sums(Sums<W> &mine, boo
         n = half;
         __syncthreads();
     }
-    for (int i = threadIdx.x; i < channels; i += kHeldThreads) s_sums[i] = s_all[i];
+    for (int i = threadIdx.x; i < channels; i += kHeldThreads) {
+        float2 sum = s_all[i];
+        for (int k = 1; k < n; k++) {
+            sum.x += s_all[k * channels + i].x;
+            sum.y += s_all[k * channels + i].y;
+        }
+        s_sums[i] = sum;
+    }
 }
 
-// What a thread needs for hat and da of W channels, and for dx.
+// What a thread needs for da of W channels, with c = x - mean: a = c (w r) + b; and for dx = w r da - r mean(da w) - c r^2 mean(da w hat).
 template <typename T, int W, bool SPLIT> struct Back {
     static constexpr int P = kPairs<W>;
-    Two w[P], b[P];
+    Two w[P], b[P]; // (w r)
     Each<W, SPLIT> mean, rate;
     int kind;
     __device__ __forceinline__ Back() {}
@@ -461,77 +513,97 @@ template <typename T, int W, bool SPLIT> struct Back {
         const float2 left = stats[group], right = SPLIT ? stats[min(group + 1, (int)a.groups - 1)] : left;
         mean.set(left.x, right.x, groups.split);
         rate.set(left.y, right.y, groups.split);
+#pragma unroll
+        for (int i = 0; i < P; i++) w[i] = mul_rn(w[i], rate[i]);
     }
-    __device__ __forceinline__ void row(const Pack<T, W> &x, const Pack<T, W> &dy, Two (&hat)[P], Two (&da)[P]) const {
-        get_pairs<T, W>(hat, x);
-        get_pairs<T, W>(da, dy);
-        Two v[P];
+    // c and a
+    __device__ __forceinline__ void row(const Pack<T, W> &x, Two (&c)[P], Two (&v)[P]) const {
+        get_pairs<T, W>(c, x);
 #pragma unroll
         for (int i = 0; i < P; i++) {
-            hat[i] = mul_rn(sub_rn(hat[i], mean[i]), rate[i]);
-            v[i] = fma_rn(hat[i], w[i], b[i]);
+            c[i] = sub_rn(c[i], mean[i]);
+            v[i] = fma_rn(c[i], w[i], b[i]);
         }
+    }
+    // c and da
+    __device__ __forceinline__ void row(const Pack<T, W> &x, const Pack<T, W> &dy, Two (&c)[P], Two (&da)[P]) const {
+        Two v[P];
+        row(x, c, v);
+        get_pairs<T, W>(da, dy);
         slope(da, v, kind);
     }
-    // `less`: the means of da w and of da w hat
-    __device__ __forceinline__ void gradient(const Two (&hat)[P], Two (&da)[P], const Each<W, SPLIT> &less, const Each<W, SPLIT> &less_hat) const {
+    // `less`: r mean(da w) and -r^2 mean(da w hat)
+    __device__ __forceinline__ void gradient(const Two (&c)[P], Two (&da)[P], const Each<W, SPLIT> &less, const Each<W, SPLIT> &less_c) const {
 #pragma unroll
-        for (int i = 0; i < P; i++) da[i] = mul_rn(sub_rn(sub_rn(mul_rn(da[i], w[i]), less[i]), mul_rn(hat[i], less_hat[i])), rate[i]);
+        for (int i = 0; i < P; i++) da[i] = fma_rn(c[i], less_c[i], fma_rn(da[i], w[i], less[i]));
+    }
+    // those from the groups' means
+    __device__ __forceinline__ void means(Each<W, SPLIT> &less, Each<W, SPLIT> &less_c, float2 left, float2 right, int split) const {
+        less.set(left.x, right.x, split);
+        less_c.set(left.y, right.y, split);
+#pragma unroll
+        for (int i = 0; i < (SPLIT ? P : 1); i++) {
+            const Two r = mul_rn(rate.v[i], all(-1.0f));
+            less.v[i] = mul_rn(less.v[i], r);
+            less_c.v[i] = mul_rn(mul_rn(less_c.v[i], r), rate.v[i]);
+        }
     }
 };
 
-// room: (sum_rows() + CTAs of the cluster) times the channels, of two floats; then x and dy
+// room: (part_rows() + CTAs of the cluster) times the channels, of two floats; then, for each turn of the threads, x and dy
 template <typename T, int W, bool SPLIT>
 __global__ void __launch_bounds__(kHeldThreads) held_backward_kernel(const __grid_constant__ ffcvb_group_norm_args a, const Deal deal, float2 *sums) {
-    constexpr int P = kPairs<W>;
+    constexpr int P = kPairs<W>, N = kHeldThreads;
     __shared__ float2 s_group[kMostGroups];
     extern __shared__ uint4 s_held[];
     wait_for_previous();
     let_next_begin();
     if (deal.ctas > 1) cluster_begun();
     const Held me(deal, (int)a.positions);
-    const int per = deal.per, rank = me.rank, group0 = me.group0, row = me.row, pack = me.pack, first = me.first, last = me.last, channels = deal.packs * W;
-    const long long sample = me.sample;
-    const Groups groups(pack, W, per);
-    const int channel = group0 * per + pack * W;
-    const bool used = row < deal.lanes;
-    float2 *s_all = reinterpret_cast<float2 *>(s_held), *s_there = s_all + sum_rows(deal.packs, deal.lanes) * channels; // [ctas][channels]
-    Pack<T, W> *held = reinterpret_cast<Pack<T, W> *>(s_held + ((sum_rows(deal.packs, deal.lanes) + deal.ctas) * channels + 1) / 2) + threadIdx.x;
+    const int channels = deal.packs * W, rows = part_rows(deal.packs, deal.lanes, kHeldThreads);
+    const Groups groups(me.pack, W, deal.per);
+    const int channel = me.group0 * deal.per + me.pack * W;
+    const bool used = me.row < deal.lanes;
+    float2 *s_all = reinterpret_cast<float2 *>(s_held), *s_there = s_all + rows * channels; // [ctas][channels]
+    Pack<T, W> *held = reinterpret_cast<Pack<T, W> *>(s_held + ((rows + deal.ctas) * channels + 1) / 2) + threadIdx.x;
     if (used) {
-        const T *x = static_cast<const T *>(a.x) + sample * a.x_sample + (first + row) * a.x_position + channel;
-        const T *dy = static_cast<const T *>(a.dy) + sample * a.dy_sample + (first + row) * a.dy_position + channel;
+        const T *x = static_cast<const T *>(a.x) + me.sample * a.x_sample + (me.first + me.row) * a.x_position + channel;
+        const T *dy = static_cast<const T *>(a.dy) + me.sample * a.dy_sample + (me.first + me.row) * a.dy_position + channel;
         const long long x_step = deal.lanes * a.x_position, dy_step = deal.lanes * a.dy_position;
         Pack<T, W> *to = held;
-        for (int r = first + row; r < last; r += deal.lanes, to += 2 * kHeldThreads, x += x_step, dy += dy_step) {
+        for (int r = me.first + me.row; r < me.last; r += deal.lanes, to += 2 * N, x += x_step, dy += dy_step) {
             copy_pack(to, x);
-            copy_pack(to + kHeldThreads, dy);
+            copy_pack(to + N, dy);
         }
     }
     Back<T, W, SPLIT> back;
-    if (used) back = Back<T, W, SPLIT>(a, sample, channel, group0 + groups.left, groups);
+    if (used) back = Back<T, W, SPLIT>(a, me.sample, channel, me.group0 + groups.left, groups);
     copies_done();
     {
         Sums<W> mine;
         if (used) {
             const Pack<T, W> *from = held;
-            for (int r = first + row; r < last; r += deal.lanes, from += 2 * kHeldThreads) {
-                Two hat[P], da[P];
-                back.row(from[0], from[kHeldThreads], hat, da);
-                mine.add(hat, da);
+#pragma unroll 2
+            for (int r = me.first + me.row; r < me.last; r += deal.lanes, from += 2 * N) {
+                Two c[P], da[P];
+                back.row(from[0], from[N], c, da);
+                mine.add(c, da);
             }
+            mine.times(back.rate);
         }
-        channel_sums<W>(mine, used, row, pack, deal.lanes, deal.packs, s_all, s_there + rank * channels);
+        channel_sums<W>(mine, used, me.row, me.pack, deal.lanes, deal.packs, s_all, s_there + me.rank * channels);
     }
     __syncthreads();
     if (deal.ctas > 1) {
         cluster_wait(); // all have begun
-        for (int i = threadIdx.x; i < channels * deal.ctas; i += kHeldThreads) {
-            const int c = i % channels, to = i / channels;
-            float2 *at = s_there + rank * channels + c;
-            if (to == rank) continue;
+        for (int i = threadIdx.x; i < channels; i += kHeldThreads) {
+            float2 *at = s_there + me.rank * channels + i;
             const float2 v = *at;
-            store_there(&at->x, to, v.x);
-            store_there(&at->y, to, v.y);
+            for (int to = 0; to < deal.ctas; to++) {
+                if (to == me.rank) continue;
+                store_there(&at->x, to, v.x);
+                store_there(&at->y, to, v.y);
+            }
         }
         cluster_sync();
         for (int i = threadIdx.x; i < channels; i += kHeldThreads) {
@@ -546,43 +618,41 @@ __global__ void __launch_bounds__(kHeldThreads) held_backward_kernel(const __gri
     } else {
         s_all = s_there;
     }
-    if (rank == 0)
-        for (int i = threadIdx.x; i < channels; i += kHeldThreads) sums[sample * a.channels + group0 * per + i] = s_all[i];
+    if (me.rank == 0)
+        for (int i = threadIdx.x; i < channels; i += kHeldThreads) sums[me.sample * a.channels + me.group0 * deal.per + i] = s_all[i];
     for (int g = threadIdx.x >> 5; g < deal.groups; g += kHeldThreads / 32) {
         float2 mean = make_float2(0.0f, 0.0f);
-        for (int c = threadIdx.x & 31; c < per; c += 32) {
-            const float one = parameter(a.weight, a.param_type, group0 * per + g * per + c, 1.0f);
-            mean.x = fmaf(one, s_all[g * per + c].x, mean.x);
-            mean.y = fmaf(one, s_all[g * per + c].y, mean.y);
+        for (int c = threadIdx.x & 31; c < deal.per; c += 32) {
+            const float one = parameter(a.weight, a.param_type, me.group0 * deal.per + g * deal.per + c, 1.0f);
+            mean.x = fmaf(one, s_all[g * deal.per + c].x, mean.x);
+            mean.y = fmaf(one, s_all[g * deal.per + c].y, mean.y);
         }
-        const float over = 1.0f / ((float)a.positions * (float)per);
+        const float over = 1.0f / ((float)a.positions * (float)deal.per);
         mean.x = warp_sum(mean.x) * over;
         mean.y = warp_sum(mean.y) * over;
         if ((threadIdx.x & 31) == 0) s_group[g] = mean;
     }
     __syncthreads();
     if (!used || !a.dx) return;
-    Each<W, SPLIT> less, less_hat;
-    const float2 left = s_group[groups.left], right = SPLIT ? s_group[min(groups.left + 1, deal.groups - 1)] : left;
-    less.set(left.x, right.x, groups.split);
-    less_hat.set(left.y, right.y, groups.split);
-    T *to = static_cast<T *>(a.dx) + (sample * a.positions + first + row) * a.channels + channel;
+    Each<W, SPLIT> less, less_c;
+    back.means(less, less_c, s_group[groups.left], s_group[min(groups.left + 1, deal.groups - 1)], groups.split);
+    T *to = static_cast<T *>(a.dx) + (me.sample * a.positions + me.first + me.row) * a.channels + channel;
     const long long step = deal.lanes * a.channels;
     const Pack<T, W> *from = held;
-    for (int r = first + row; r < last; r += deal.lanes, from += 2 * kHeldThreads, to += step) {
-        Two hat[P], da[P];
-        back.row(from[0], from[kHeldThreads], hat, da);
-        back.gradient(hat, da, less, less_hat);
+#pragma unroll 2
+    for (int r = me.first + me.row; r < me.last; r += deal.lanes, from += 2 * N, to += step) {
+        Two c[P], da[P];
+        back.row(from[0], from[N], c, da);
+        back.gradient(c, da, less, less_c);
         put_pairs<T, W>(to, da);
     }
 }
 
 // ---- not held: sums of slabs of positions, joined; then the values -------------------------------------------------------
 
-// Packs of a position, of which a CTA has `columns`, and `lanes` positions at once; positions of a slab, and slabs.  Samples from `sample` on.
+// Packs of a position, of which a CTA has `columns`, and `lanes` positions at once; positions of a slab, and slabs.
 struct Slabs {
     int packs, columns, lanes, rows, slabs;
-    int64_t sample;
 };
 
 struct Place {
@@ -597,11 +667,36 @@ __device__ __forceinline__ Place place_of(const Slabs &s, int positions, bool ba
     p.pack = blockIdx.y * s.columns + threadIdx.x % s.columns;
     const long long n = backwards ? (long long)gridDim.x - 1 - blockIdx.x : blockIdx.x;
     p.slab = (int)(n % s.slabs);
-    p.sample = s.sample + n / s.slabs;
+    p.sample = n / s.slabs;
     p.first = p.slab * s.rows;
     p.last = min(p.first + s.rows, positions);
     p.used = p.row < s.lanes && p.pack < s.packs;
     return p;
+}
+
+// Calls f(pack of x, pack of dy, position) for a thread's positions, four of them loaded before the first is used (two with dy).
+template <typename T, int W, bool TWO, typename F>
+__device__ __forceinline__ void each_position(const Place &p, int lanes, const T *x, long long x_step, const T *dy, long long dy_step, F &&f) {
+    constexpr int BATCH = TWO ? 2 : 4;
+    int r = p.first + p.row;
+    x += r * x_step;
+    dy += r * dy_step;
+    for (; r + (BATCH - 1) * lanes < p.last; r += BATCH * lanes) {
+        Pack<T, W> one[BATCH], other[BATCH];
+#pragma unroll
+        for (int i = 0; i < BATCH; i++, x += lanes * x_step, dy += lanes * dy_step) {
+            one[i].load(x);
+            if (TWO) other[i].load(dy);
+        }
+#pragma unroll
+        for (int i = 0; i < BATCH; i++) f(one[i], other[i], r + i * lanes);
+    }
+    for (; r < p.last; r += lanes, x += lanes * x_step, dy += lanes * dy_step) {
+        Pack<T, W> one, other;
+        one.load(x);
+        if (TWO) other.load(dy);
+        f(one, other, r);
+    }
 }
 
 // parts: [samples][slabs][packs][sides], mean and squares around it
@@ -613,20 +708,31 @@ __global__ void __launch_bounds__(kThreads) moments_kernel(const __grid_constant
     let_next_begin();
     const Place p = place_of(s, (int)a.positions, false);
     const Groups groups(p.pack, W, (int)(a.channels / a.groups));
-    Collected<W> values;
-    if (p.used) {
+    Collected<W, SPLIT> values;
+    float pivot[2] = {0.0f, 0.0f}, n[2] = {0.0f, 0.0f};
+    if (p.used && p.first + p.row < p.last) {
         const T *x = static_cast<const T *>(a.x) + p.sample * a.x_sample + p.pack * W;
-#pragma unroll 4
-        for (int r = p.first + p.row; r < p.last; r += s.lanes) {
-            Pack<T, W> pack;
+        const float turns = (float)((p.last - p.first - p.row - 1) / s.lanes + 1);
+        Pack<T, W> pack;
+        Two v[P];
+        pack.load(x + (p.first + p.row) * a.x_position);
+        get_pairs<T, W>(v, pack);
+#pragma unroll
+        for (int side = 0; side < SIDES; side++) {
+            const float there = !SPLIT ? (float)W : side ? (float)(W - groups.split) : (float)groups.split;
+            pivot[side] = __fdividef(values.of(v, groups.split, side), fmaxf(there, 1.0f));
+            n[side] = turns * there;
+        }
+        values.pivot.set(pivot[0], pivot[SIDES - 1], groups.split);
+        each_position<T, W, false>(p, s.lanes, x, a.x_position, x, 0, [&](const Pack<T, W> &pack, const Pack<T, W> &, int) {
             Two v[P];
-            pack.load(x + r * a.x_position);
             get_pairs<T, W>(v, pack);
             values.add(v);
-        }
+        });
     }
 #pragma unroll
-    for (int side = 0; side < SIDES; side++) s_moments[side][threadIdx.x] = side ? values.moments(groups.split, W) : values.moments(0, SPLIT ? groups.split : W);
+    for (int side = 0; side < SIDES; side++)
+        s_moments[side][threadIdx.x] = moments_of(n[side], pivot[side], values.of(values.sum, groups.split, side), values.of(values.squares, groups.split, side));
     __syncthreads();
     for (int i = threadIdx.x; i < s.columns * SIDES; i += kThreads) {
         const int column = i % s.columns, side = i / s.columns, pack = blockIdx.y * s.columns + column;
@@ -643,7 +749,7 @@ template <int W, bool SPLIT> __global__ void __launch_bounds__(kThreads) join_mo
     __shared__ Moments s_part[kThreads / 32];
     wait_for_previous();
     let_next_begin();
-    const long long sample = s.sample + blockIdx.x / a.groups;
+    const long long sample = blockIdx.x / a.groups;
     const int group = (int)(blockIdx.x % a.groups), per = (int)(a.channels / a.groups), pack0 = (int)((long long)group * per / W);
     const int each = (int)(((long long)(group + 1) * per - 1) / W) - pack0 + 1;
     Moments found{0.0f, 0.0f, 0.0f};
@@ -671,27 +777,20 @@ __global__ void __launch_bounds__(kThreads) values_kernel(const __grid_constant_
     if (!p.used) return;
     const Groups groups(p.pack, W, (int)(a.channels / a.groups));
     const int channel = p.pack * W;
-    Back<T, W, SPLIT> by(a, p.sample, channel, groups.left, groups);
-#pragma unroll
-    for (int i = 0; i < P; i++) by.w[i] = mul_rn(by.w[i], by.rate[i]);
+    const Back<T, W, SPLIT> by(a, p.sample, channel, groups.left, groups);
     const T *x = static_cast<const T *>(a.x) + p.sample * a.x_sample + channel;
     T *y = static_cast<T *>(a.y) + p.sample * a.positions * a.channels + channel;
-#pragma unroll 4
-    for (int r = p.first + p.row; r < p.last; r += s.lanes) {
-        Pack<T, W> pack;
-        Two v[P];
-        pack.load(x + r * a.x_position);
-        get_pairs<T, W>(v, pack);
-#pragma unroll
-        for (int i = 0; i < P; i++) v[i] = fma_rn(sub_rn(v[i], by.mean[i]), by.w[i], by.b[i]);
+    each_position<T, W, false>(p, s.lanes, x, a.x_position, x, 0, [&](const Pack<T, W> &pack, const Pack<T, W> &, int r) {
+        Two c[P], v[P];
+        by.row(pack, c, v);
         activate(v, a.activation);
         put_pairs<T, W>(y + r * a.channels, v);
-    }
+    });
 }
 
 // parts: [samples][slabs][channels]
 template <typename T, int W, bool SPLIT>
-__global__ void __launch_bounds__(kThreads) sums_kernel(const __grid_constant__ ffcvb_group_norm_args a, const Slabs s, float2 *parts) {
+__global__ void __launch_bounds__(kThreads, 3) sums_kernel(const __grid_constant__ ffcvb_group_norm_args a, const Slabs s, float2 *parts) {
     constexpr int P = kPairs<W>;
     __shared__ float2 s_all[kThreads * W];
     wait_for_previous();
@@ -703,15 +802,12 @@ __global__ void __launch_bounds__(kThreads) sums_kernel(const __grid_constant__ 
         const int channel = p.pack * W;
         const Back<T, W, SPLIT> back(a, p.sample, channel, groups.left, groups);
         const T *x = static_cast<const T *>(a.x) + p.sample * a.x_sample + channel, *dy = static_cast<const T *>(a.dy) + p.sample * a.dy_sample + channel;
-#pragma unroll 2
-        for (int r = p.first + p.row; r < p.last; r += s.lanes) {
-            Pack<T, W> one, other;
-            Two hat[P], da[P];
-            one.load(x + r * a.x_position);
-            other.load(dy + r * a.dy_position);
-            back.row(one, other, hat, da);
-            mine.add(hat, da);
-        }
+        each_position<T, W, true>(p, s.lanes, x, a.x_position, dy, a.dy_position, [&](const Pack<T, W> &one, const Pack<T, W> &other, int) {
+            Two c[P], da[P];
+            back.row(one, other, c, da);
+            mine.add(c, da);
+        });
+        mine.times(back.rate);
     }
     float2 *to = parts + (p.sample * s.slabs + p.slab) * a.channels + blockIdx.y * s.columns * W;
     const int channels = s.columns * W, there = min(channels, (int)a.channels - (int)blockIdx.y * channels);
@@ -735,7 +831,7 @@ __global__ void __launch_bounds__(kThreads) join_sums_kernel(const __grid_consta
     wait_for_previous();
     let_next_begin();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, per = (int)(a.channels / a.groups), group = (int)(blockIdx.x % a.groups);
-    const long long sample = s.sample + blockIdx.x / a.groups;
+    const long long sample = blockIdx.x / a.groups;
     float2 mean = make_float2(0.0f, 0.0f);
     for (int c = group * per + warp; c < (group + 1) * per; c += kThreads / 32) {
         float2 whole = make_float2(0.0f, 0.0f);
@@ -764,7 +860,7 @@ __global__ void __launch_bounds__(kThreads) join_sums_kernel(const __grid_consta
 }
 
 template <typename T, int W, bool SPLIT>
-__global__ void __launch_bounds__(kThreads) gradient_kernel(const __grid_constant__ ffcvb_group_norm_args a, const Slabs s, const float2 *means) {
+__global__ void __launch_bounds__(kThreads, 3) gradient_kernel(const __grid_constant__ ffcvb_group_norm_args a, const Slabs s, const float2 *means) {
     constexpr int P = kPairs<W>;
     wait_for_previous();
     let_next_begin();
@@ -773,22 +869,16 @@ __global__ void __launch_bounds__(kThreads) gradient_kernel(const __grid_constan
     const Groups groups(p.pack, W, (int)(a.channels / a.groups));
     const int channel = p.pack * W;
     const Back<T, W, SPLIT> back(a, p.sample, channel, groups.left, groups);
-    Each<W, SPLIT> less, less_hat;
-    const float2 left = means[p.sample * a.groups + groups.left], right = SPLIT ? means[p.sample * a.groups + min(groups.left + 1, (int)a.groups - 1)] : left;
-    less.set(left.x, right.x, groups.split);
-    less_hat.set(left.y, right.y, groups.split);
+    Each<W, SPLIT> less, less_c;
+    back.means(less, less_c, means[p.sample * a.groups + groups.left], means[p.sample * a.groups + min(groups.left + 1, (int)a.groups - 1)], groups.split);
     const T *x = static_cast<const T *>(a.x) + p.sample * a.x_sample + channel, *dy = static_cast<const T *>(a.dy) + p.sample * a.dy_sample + channel;
     T *dx = static_cast<T *>(a.dx) + p.sample * a.positions * a.channels + channel;
-#pragma unroll 2
-    for (int r = p.first + p.row; r < p.last; r += s.lanes) {
-        Pack<T, W> one, other;
-        Two hat[P], da[P];
-        one.load(x + r * a.x_position);
-        other.load(dy + r * a.dy_position);
-        back.row(one, other, hat, da);
-        back.gradient(hat, da, less, less_hat);
+    each_position<T, W, true>(p, s.lanes, x, a.x_position, dy, a.dy_position, [&](const Pack<T, W> &one, const Pack<T, W> &other, int r) {
+        Two c[P], da[P];
+        back.row(one, other, c, da);
+        back.gradient(c, da, less, less_c);
         put_pairs<T, W>(dx + r * a.channels, da);
-    }
+    });
 }
 
 // The parameters' gradients: samples' sums added up, 32 channels per CTA.
@@ -828,12 +918,13 @@ __global__ void __launch_bounds__(1024) samples_kernel(const __grid_constant__ f
 
 // ---- the host's part -------------------------------------------------------------------------------------------------
 
-// Bytes that a CTA holds at most: two of them on an SM; and what it holds rather, so that four are.
-constexpr int64_t kMostHeld = 100 * 1024, kHeld = 51 * 1024;
-// Bytes of neighbouring channels that a CTA reads at least, where there are as many.
-constexpr int64_t kNeighbours = 64;
-// Bytes of x of a pass over all its slabs, before they are read again: what the caches keep.
-constexpr int64_t kCached = 40ll << 20;
+// Bytes that a CTA holds at most; of one that is not alone rather so much that there are four on an SM, in clusters of up to eight.
+constexpr int64_t kMostHeld = 74 * 1024, kHeld = 51 * 1024;
+// Bytes of neighbouring channels that a CTA reads at least, where there are as many; and what it holds rather of small images, as long as there are six CTAs for
+// every SM.
+constexpr int64_t kNeighbours = 64, kSmall = 32 * 1024;
+// Positions of a thread in a slab: as many as bring eight CTAs to every SM.
+constexpr int64_t kLeastTurns = 4, kMostTurns = 16;
 
 // Values of a pack: of one group or of two neighbouring ones (`split`), and where they begin as their size has it.
 int width_of(const ffcvb_group_norm_args &a, bool backward) {
@@ -856,7 +947,6 @@ struct Plan {
     Deal deal;
     int64_t room;     // bytes of shared memory
     Slabs slabs;
-    int64_t samples;  // at once
     int64_t parts, means, sums, bytes; // offsets in the workspace
 };
 
@@ -867,17 +957,23 @@ Plan plan_of(const ffcvb_group_norm_args &a, bool backward) {
     p.split = per % w != 0;
     Deal &d = p.deal;
     d.groups = 1;
-    while (d.groups * 2 <= kMostGroups && a.groups % (d.groups * 2) == 0 && (d.groups * per * size < kNeighbours || d.groups * per % w != 0)) d.groups *= 2;
+    while (d.groups * 2 <= kMostGroups && a.groups % (d.groups * 2) == 0 && 
+           (d.groups * per * size < kNeighbours || d.groups * per % w != 0 ||
+            (d.groups * 2 * per * size * a.positions <= kSmall && d.groups * 2 * per / w <= 64 && a.samples * a.groups / (d.groups * 2) >= kSms * 6)))
+        d.groups *= 2;
+    constexpr int threads = kHeldThreads;
     const int64_t packs = d.groups * per / w;
-    if (packs <= kHeldThreads && d.groups * per % w == 0 && a.samples <= 65535) {
+    if (packs <= threads && d.groups * per % w == 0 && a.samples <= 65535) {
         d.packs = (int)packs;
         d.per = (int)per;
-        d.lanes = (int)std::min<int64_t>(kHeldThreads / packs, std::max<int64_t>(a.positions, 1));
+        d.lanes = (int)std::min<int64_t>(threads / packs, std::max<int64_t>(a.positions, 1));
         auto room_of = [&](int ctas) {
             const int64_t rows = (a.positions + ctas - 1) / ctas, turns = (rows + d.lanes - 1) / d.lanes;
-            return turns * kHeldThreads * w * size * (backward ? 2 : 1) + (backward ? ((sum_rows(d.packs, d.lanes) + ctas) * packs * w + 1) / 2 * 16 : 0);
+            return turns * threads * w * size * (backward ? 2 : 1) + (backward ? ((part_rows(d.packs, d.lanes, threads) + ctas) * packs * w + 1) / 2 * 16 : 0);
         };
-        for (d.ctas = 1; d.ctas < 8 && room_of(d.ctas) > kHeld; d.ctas *= 2) {}
+        d.ctas = 1;
+        if (room_of(1) > kMostHeld)
+            while (d.ctas < 8 && room_of(d.ctas) > kHeld) d.ctas *= 2;
         p.room = room_of(d.ctas);
         p.held = p.room <= kMostHeld;
         d.rows = (int)((a.positions + d.ctas - 1) / d.ctas);
@@ -886,12 +982,8 @@ Plan plan_of(const ffcvb_group_norm_args &a, bool backward) {
     s.packs = (int)(a.channels / w);
     s.columns = std::min(s.packs, kThreads);
     s.lanes = std::max(1, kThreads / s.columns);
-    const int64_t sample_bytes = a.positions * a.channels * size * (backward ? 2 : 1);
-    p.samples = std::clamp<int64_t>(kCached / std::max<int64_t>(1, sample_bytes), 1, a.samples);
-    // slabs of 4 to 64 positions of a thread, as many as bring five CTAs to every SM
-    const int64_t ctas = p.samples * ((s.packs + s.columns - 1) / s.columns);
-    const int64_t turns = std::clamp<int64_t>((a.positions * ctas + (int64_t)s.lanes * kSms * 5 - 1) / ((int64_t)s.lanes * kSms * 5), 4, 64);
-    s.rows = (int)std::min<int64_t>(a.positions, turns * s.lanes);
+    const int64_t ctas = a.samples * ((s.packs + s.columns - 1) / s.columns), fair = (a.positions * ctas + (int64_t)s.lanes * kSms * 8 - 1) / ((int64_t)s.lanes * kSms * 8);
+    s.rows = (int)std::min<int64_t>(a.positions, std::clamp(fair, kLeastTurns, kMostTurns) * s.lanes);
     s.slabs = s.rows ? (int)((a.positions + s.rows - 1) / s.rows) : 0;
     int64_t at = 0;
     auto take = [&](bool wanted, int64_t bytes) {
@@ -915,6 +1007,7 @@ const char *wrong(const ffcvb_group_norm_args &a, bool backward) {
     if (a.activation < FFCVB_ACT_NONE || a.activation > FFCVB_ACT_GELU || !(a.eps >= 0.0f)) return "bad argument";
     if (a.samples > 0 && a.positions > 0 && (!a.x || !a.stats || (backward ? !a.dy : !a.y))) return "an address is missing";
     if (backward && !a.dx && !a.dweight && !a.dbias) return "nothing to do";
+    if (a.samples > 0 && a.positions > 0 && a.samples * plan_of(a, backward).slabs.slabs > INT32_MAX) return "too many values";
     return nullptr;
 }
 
@@ -934,7 +1027,7 @@ template <typename T, typename F> void with_width(int w, bool split, F &&f) {
     f(T{}, Width<1>{}, std::false_type{});
 }
 
-template <typename... Params, typename... Given> void launch_cluster(void (*kernel)(Params...), dim3 grid, int cluster, int64_t room, cudaStream_t stream, Given &&...given) {
+template <typename... Params, typename... Given> void launch_cluster(void (*kernel)(Params...), dim3 grid, int threads, int cluster, int64_t room, cudaStream_t stream, Given &&...given) {
     cudaLaunchConfig_t how{};
     cudaLaunchAttribute with[2] = {};
     with[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -943,7 +1036,7 @@ template <typename... Params, typename... Given> void launch_cluster(void (*kern
     with[1].val.clusterDim.x = cluster;
     with[1].val.clusterDim.y = with[1].val.clusterDim.z = 1;
     how.gridDim = grid;
-    how.blockDim = dim3(kHeldThreads);
+    how.blockDim = dim3(threads);
     how.dynamicSmemBytes = room;
     how.stream = stream;
     how.attrs = with;
@@ -964,18 +1057,15 @@ void run_forward(const ffcvb_group_norm_args &a, uint8_t *room, cudaStream_t st)
             constexpr int W = decltype(width)::value;
             constexpr bool SPLIT = decltype(split)::value;
             if (p.held) {
-                launch_cluster(held_forward_kernel<T, W, SPLIT>, dim3((unsigned)(a.groups / p.deal.groups * p.deal.ctas), (unsigned)a.samples), p.deal.ctas, p.room, st, a, p.deal);
+                launch_cluster(held_forward_kernel<T, W, SPLIT>, dim3((unsigned)(a.groups / p.deal.groups * p.deal.ctas), (unsigned)a.samples), kHeldThreads, p.deal.ctas, p.room, st, a, p.deal);
                 return;
             }
             float2 *parts = reinterpret_cast<float2 *>(room + p.parts);
-            Slabs s = p.slabs;
-            for (s.sample = 0; s.sample < a.samples; s.sample += p.samples) {
-                const int64_t samples = std::min(p.samples, a.samples - s.sample);
-                const dim3 grid((unsigned)(samples * s.slabs), (unsigned)((s.packs + s.columns - 1) / s.columns));
-                launch_early(moments_kernel<T, W, SPLIT>, grid, kThreads, 0, st, a, s, parts);
-                launch_early(join_moments_kernel<W, SPLIT>, (unsigned)(samples * a.groups), kThreads, 0, st, a, s, parts);
-                launch_early(values_kernel<T, W, SPLIT>, grid, kThreads, 0, st, a, s);
-            }
+            const Slabs &s = p.slabs;
+            const dim3 grid((unsigned)(a.samples * s.slabs), (unsigned)((s.packs + s.columns - 1) / s.columns));
+            launch_early(moments_kernel<T, W, SPLIT>, grid, kThreads, 0, st, a, s, parts);
+            launch_early(join_moments_kernel<W, SPLIT>, (unsigned)(a.samples * a.groups), kThreads, 0, st, a, s, parts);
+            launch_early(values_kernel<T, W, SPLIT>, grid, kThreads, 0, st, a, s);
         });
     });
 }
@@ -989,18 +1079,15 @@ void run_backward(const ffcvb_group_norm_args &a, uint8_t *room, cudaStream_t st
             constexpr int W = decltype(width)::value;
             constexpr bool SPLIT = decltype(split)::value;
             if (p.held) {
-                launch_cluster(held_backward_kernel<T, W, SPLIT>, dim3((unsigned)(a.groups / p.deal.groups * p.deal.ctas), (unsigned)a.samples), p.deal.ctas, p.room, st, a, p.deal, sums);
+                launch_cluster(held_backward_kernel<T, W, SPLIT>, dim3((unsigned)(a.groups / p.deal.groups * p.deal.ctas), (unsigned)a.samples), kHeldThreads, p.deal.ctas, p.room, st, a, p.deal, sums);
                 return;
             }
             float2 *parts = reinterpret_cast<float2 *>(room + p.parts), *means = reinterpret_cast<float2 *>(room + p.means);
-            Slabs s = p.slabs;
-            for (s.sample = 0; s.sample < a.samples; s.sample += p.samples) {
-                const int64_t samples = std::min(p.samples, a.samples - s.sample);
-                const dim3 grid((unsigned)(samples * s.slabs), (unsigned)((s.packs + s.columns - 1) / s.columns));
-                launch_early(sums_kernel<T, W, SPLIT>, grid, kThreads, 0, st, a, s, parts);
-                launch_early(join_sums_kernel, (unsigned)(samples * a.groups), kThreads, 0, st, a, s, parts, sums, means);
-                if (a.dx) launch_early(gradient_kernel<T, W, SPLIT>, grid, kThreads, 0, st, a, s, means);
-            }
+            const Slabs &s = p.slabs;
+            const dim3 grid((unsigned)(a.samples * s.slabs), (unsigned)((s.packs + s.columns - 1) / s.columns));
+            launch_early(sums_kernel<T, W, SPLIT>, grid, kThreads, 0, st, a, s, parts);
+            launch_early(join_sums_kernel, (unsigned)(a.samples * a.groups), kThreads, 0, st, a, s, parts, sums, means);
+            if (a.dx) launch_early(gradient_kernel<T, W, SPLIT>, grid, kThreads, 0, st, a, s, means);
         });
     });
     if (a.dweight || a.dbias) launch_early(samples_kernel, (unsigned)((a.channels + 31) / 32), 1024, 0, st, a, sums);
