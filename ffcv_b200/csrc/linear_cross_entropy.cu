@@ -25,18 +25,20 @@ template <int BN> constexpr uint32_t kStageBytes = kRowsBytes + BN * 128;
 template <int BN> constexpr uint32_t kRoom = kStages<BN> * kStageBytes<BN> + kStagingBytes + 1024 + 256 + 1024;
 
 enum { kStatistics, kGradient, kProducts };      // what a kernel makes of its products
-enum { kWritten, kWritten32, kAdded32 };         // how products leave: as they are to be, or as parts in 32 bits
+enum { kWritten, kWritten32, kAdded32 };         // how products leave: as they are to be, or in 32 bits
 enum { kFixed, kRowsCounted, kSumCounted };      // what depends on the number of rows that count
 
-// One product A B of matrices, in tiles of 128 by BN, the sum in `splits` parts.
+// One product A B of matrices, in tiles of 128 by BN.
 struct alignas(64) Product {
     CUtensorMap a, b, c;
-    int row_tiles, column_tiles, sum_blocks, splits;
-    int a_along_sum; // A's rows in memory run along the sum
+    void *out;           // what C is a map of (kProducts)
+    int64_t out_stride;
+    int row_tiles, column_tiles, sum_blocks;
+    int a_along_sum;     // A's rows in memory run along the sum
     int leaves, counted;
-    int b_first;     // where B begins along the sum (kProducts), or its rows (else)
-    int c_rows, c_last; // C's rows of a part; and of those there are
-    int unused[6];
+    int b_first;         // where B begins along the sum (kProducts), or its rows (else)
+    int c_last;          // C's rows
+    int unused[4];
 };
 
 struct Head {
@@ -44,18 +46,22 @@ struct Head {
     const int *map;      // rows that count, or NULL: all
     const int *place;    // a row's place among them, or -1
     const float *counted;
-    float2 *parts;       // [classes / (BN / 2)][rows_pad]: largest logit and sum of exponentials
+    float2 *parts;       // [classes / part_columns][rows_pad]: largest logit and sum of exponentials
     float *parts_apart;  // the same: sum of logits relative to the largest; with smoothing
     float *bias_parts;   // [rows_pad / 32][chunk]
     const float *most;   // largest upstream of a row
     int rows_pad, first, columns; // classes of this chunk
-    int part_count, part_columns;
+    int part_count, part_columns, chunk;
 };
 
+// Products that one launch makes.  The blocks of all tiles' sums, in their order, are dealt out to the CTAs in equal runs, so that all end at once; what a CTA
+// has of a tile that is not its own alone it leaves as a part in 32 bits, the first one of its run or the last.
 struct Products {
     Product of[2];
-    int count;
-    int unused[15];
+    CUtensorMap part;    // [2 * CTAs * 128, BN]
+    const float *parts;
+    int count, ctas, lanes;
+    int unused[11];
     Head head;
 };
 
@@ -83,37 +89,86 @@ template <typename T> __device__ __forceinline__ float gradient_scale(const Head
     return k;
 }
 
-// A tile: of which product, where, and its part of the sum.
+// A tile, or a run of its sum: of which product and where; whether it is the whole.
 struct Tile {
-    int product, row, column, from, to, split;
+    int product, row, column, from, to;
+    bool whole;
 };
-template <int MODE> __device__ __forceinline__ bool tile_at(const Products &p, long long t, int rows, Tile &tile) {
-    for (int i = 0; i < (MODE == kProducts ? p.count : 1); i++) {
-        const Product &w = p.of[i];
-        const int row_tiles = w.counted == kRowsCounted ? (rows + 127) / 128 : w.row_tiles;
-        const long long here = (long long)row_tiles * w.column_tiles * w.splits;
-        if (t >= here) {
-            t -= here;
-            continue;
-        }
-        tile.product = i;
-        if (MODE == kProducts) { // tiles of the same rows beside one another
-            tile.column = (int)(t % w.column_tiles);
-            t /= w.column_tiles;
-            tile.row = (int)(t % row_tiles);
-            tile.split = (int)(t / row_tiles);
-        } else { // tiles of the same weights
-            tile.row = (int)(t % row_tiles);
-            tile.column = (int)(t / row_tiles);
-            tile.split = 0;
-        }
-        const int blocks = w.counted == kSumCounted ? (rows + kSum - 1) / kSum : w.sum_blocks, each = (blocks + w.splits - 1) / w.splits;
-        tile.from = min(tile.split * each, blocks);
-        tile.to = min(tile.from + each, blocks);
+__device__ __forceinline__ int row_tiles_of(const Product &w, int rows) { return w.counted == kRowsCounted ? (rows + 127) / 128 : w.row_tiles; }
+// (a sum without terms is one block long, all the same)
+__device__ __forceinline__ int sum_blocks_of(const Product &w, int rows) { return w.counted == kSumCounted ? max(1, (rows + kSum - 1) / kSum) : w.sum_blocks; }
+// Blocks of runs, at least: shorter ones cost more than they save.
+constexpr int kLeastRun = 4;
+// How blocks are dealt out: with few columns of tiles those of each column, in the same way to as many CTAs, so that CTAs with the same rows read A at the same time;
+// else of all tiles, those of the same columns one after another.
+struct Runs {
+    int lanes, all, ctas; // columns that are dealt out apart; blocks, and CTAs with a run, of each
+    int each, more;       // blocks of a run, and runs with one more
+    __device__ __forceinline__ Runs(const Products &p, int rows) : lanes(p.lanes), all(0) {
+        for (int i = 0; i < p.count; i++) all += row_tiles_of(p.of[i], rows) * sum_blocks_of(p.of[i], rows);
+        if (lanes == 1) all *= p.of[0].column_tiles;
+        ctas = min(p.ctas / lanes, max(1, all / kLeastRun));
+        each = all / ctas;
+        more = all - each * ctas;
+    }
+    __device__ __forceinline__ int begin(int n) const { return each * n + min(n, more); }
+    __device__ __forceinline__ int lane(int cta) const { return cta % lanes; }
+    __device__ __forceinline__ int place(int cta) const { return cta / lanes; }
+};
+// The tile that block `at` of a lane's is in, from that block on.
+__device__ __forceinline__ Tile tile_of(const Products &p, const Runs &runs, int lane, int at, int rows) {
+    Tile tile;
+    tile.product = 0;
+    const int columns = runs.lanes == 1 ? p.of[0].column_tiles : 1;
+    if (p.count > 1) {
+        const int here = row_tiles_of(p.of[0], rows) * sum_blocks_of(p.of[0], rows) * columns;
+        if (at >= here) at -= here, tile.product = 1;
+    }
+    const Product &w = p.of[tile.product];
+    const int blocks = sum_blocks_of(w, rows), row_tiles = row_tiles_of(w, rows), t = at / blocks;
+    tile.from = at - t * blocks;
+    tile.to = blocks;
+    tile.column = columns == 1 ? 0 : t / row_tiles;
+    tile.row = t - tile.column * row_tiles;
+    if (runs.lanes > 1) tile.column = lane;
+    tile.whole = tile.from == 0;
+    return tile;
+}
+// A CTA's tiles one after another.
+template <int MODE> struct Walk {
+    long long at, end;
+    __device__ __forceinline__ Walk(const Products &p, int rows) {
+        at = blockIdx.x;
+        end = (long long)row_tiles_of(p.of[0], rows) * p.of[0].column_tiles;
+    }
+    __device__ __forceinline__ bool next(const Products &p, int rows, Tile &tile) { // tiles of the same weights one after another
+        if (at >= end) return false;
+        const int row_tiles = row_tiles_of(p.of[0], rows), column = (int)(at / row_tiles);
+        tile = Tile{0, (int)(at - (long long)column * row_tiles), column, 0, p.of[0].sum_blocks, true};
+        at += gridDim.x;
         return true;
     }
-    return false;
-}
+};
+template <> struct Walk<kProducts> {
+    Runs runs;
+    int lane, at, end;
+    __device__ __forceinline__ Walk(const Products &p, int rows) : runs(p, rows) {
+        const int place = runs.place(blockIdx.x);
+        lane = runs.lane(blockIdx.x);
+        at = place < runs.ctas ? runs.begin(place) : 0;
+        end = place < runs.ctas ? runs.begin(place + 1) : 0;
+    }
+    __device__ __forceinline__ bool next(const Products &p, int rows, Tile &tile) {
+        if (at >= end) return false;
+        tile = tile_of(p, runs, lane, at, rows);
+        if (end - at < tile.to - tile.from) {
+            tile.to = tile.from + end - at;
+            tile.whole = false;
+        }
+        at += tile.to - tile.from;
+        return true;
+    }
+};
 
 // A CTA per SM that takes tile after tile.  Products of the next tile go into the other half of TMEM while eight warps, two for each 32 rows, take
 // the last one's.  A wait that does not end makes the CTA give up: all that it has not finished is NaN, and it ends.
@@ -154,7 +209,7 @@ __global__ void __launch_bounds__(kThreads, 1) products_kernel(const __grid_cons
         if (lane == 0) {
             uint32_t n = 0; // stages filled so far
             bool fine = true;
-            for (long long t = blockIdx.x; fine && tile_at<MODE>(p, t, rows, tile); t += gridDim.x) {
+            for (Walk<MODE> walk(p, rows); fine && walk.next(p, rows, tile);) {
                 const Product &w = p.of[tile.product];
                 for (int k = tile.from; k < tile.to; k++, n++) {
                     const uint32_t s = n % STAGES, at = room + s * kStageBytes<BN>, bar = full + 8 * s;
@@ -188,8 +243,7 @@ __global__ void __launch_bounds__(kThreads, 1) products_kernel(const __grid_cons
         if (lane == 0) {
             uint32_t n = 0, m = 0; // stages and tiles multiplied so far
             bool fine = true;
-            for (long long t = blockIdx.x; fine && tile_at<MODE>(p, t, rows, tile); t += gridDim.x) {
-                if (tile.from >= tile.to) continue;
+            for (Walk<MODE> walk(p, rows); fine && walk.next(p, rows, tile);) {
                 const bool a_along_sum = MODE == kProducts && p.of[tile.product].a_along_sum;
                 const uint32_t kind = product_kind(sizeof(T) == 2 && kHeld<T> == 1.0f, BN, a_along_sum, MODE == kProducts), half = m & 1;
                 fine = m < 2 || barrier_wait(taken + 8 * half, (m / 2 - 1) & 1, s_gave_up);
@@ -223,9 +277,8 @@ __global__ void __launch_bounds__(kThreads, 1) products_kernel(const __grid_cons
         const uint32_t from = tmem + ((uint32_t)quarter << 21) + side * HALF;
         const float k_all = MODE == kProducts ? gradient_scale<T>(h) : 0.0f;
         uint32_t m = 0;
-        for (long long t = blockIdx.x; tile_at<MODE>(p, t, rows, tile); t += gridDim.x) {
+        for (Walk<MODE> walk(p, rows); walk.next(p, rows, tile);) {
             const Product &w = p.of[tile.product];
-            const bool nothing = tile.from >= tile.to;
             const uint32_t half = m & 1, at = from + half * BN;
             const int row = tile.row * 128 + quarter * 32 + lane, column = tile.column * BN + side * HALF; // (of the lane; the first)
             if (MODE != kProducts) { // the columns' bias; classes that there are not have a logit of -inf
@@ -236,15 +289,11 @@ __global__ void __launch_bounds__(kThreads, 1) products_kernel(const __grid_cons
                 }
                 asm volatile("bar.sync 1, 256;" ::: "memory");
             }
-            bool fine = true;
-            if (!nothing) {
-                fine = barrier_wait(done + 8 * half, m / 2 & 1, s_gave_up);
-                fine = __all_sync(0xffffffffu, fine);
-                tmem_after_sync();
-                m++;
-            }
+            bool fine = barrier_wait(done + 8 * half, m / 2 & 1, s_gave_up);
+            fine = __all_sync(0xffffffffu, fine);
+            tmem_after_sync();
+            m++;
             auto give_back = [&] { // behind the last load of the tile
-                if (nothing) return;
                 tmem_before_sync();
                 __syncwarp();
                 if (lane == 0) barrier_arrive(taken + 8 * half);
@@ -262,6 +311,7 @@ __global__ void __launch_bounds__(kThreads, 1) products_kernel(const __grid_cons
                 for (int c = 0; c < HALF; c += 32) {
                     uint32_t raw[32];
                     tmem_load(raw, at + c);
+                    tmem_wait(raw);
                     Two z[16];
 #pragma unroll
                     for (int j = 0; j < 32; j += 4) {
@@ -343,13 +393,16 @@ __global__ void __launch_bounds__(kThreads, 1) products_kernel(const __grid_cons
                     }
                     if (!fine) factor = NAN;
                 }
-                const bool blank = nothing || (MODE == kGradient && row >= rows); // (what is there is no number, perhaps)
-                const Two minus(-row_top, -row_top), log2e(kLog2e, kLog2e), times(factor, factor), less(-flat, -flat);
-                const int row0 = tile.row * 128 + quarter * 32 + (MODE == kProducts ? tile.split * w.c_rows : 0);
+                // (what is there is no number, perhaps)
+                const bool blank = MODE == kGradient ? row >= rows : w.counted == kSumCounted && rows == 0;
+                const bool part = MODE == kProducts && !tile.whole;
+                const float times_it = part || (MODE == kProducts && w.leaves != kWritten) ? 1.0f : factor;
+                const Two minus(-row_top, -row_top), log2e(kLog2e, kLog2e), times(times_it, times_it), less(-flat, -flat);
+                // a part's place: the run's first, or its last
+                const int row0 = (part ? (2 * (int)blockIdx.x + (tile.from == 0)) * 128 : tile.row * 128) + quarter * 32;
+                const int x0 = part ? side * HALF : column, x_last = part ? BN : MODE == kGradient ? h.columns : (int)h.a.width;
                 // 32 columns from c on
-                auto values = [&](Two(&v)[16], int c) {
-                    uint32_t raw[32];
-                    tmem_load(raw, at + c);
+                auto values = [&](Two(&v)[16], const uint32_t(&raw)[32], int c) {
 #pragma unroll
                     for (int j = 0; j < 32; j += 4) {
                         Two a(__uint_as_float(raw[j]), __uint_as_float(raw[j + 1])), b(__uint_as_float(raw[j + 2]), __uint_as_float(raw[j + 3]));
@@ -359,7 +412,7 @@ __global__ void __launch_bounds__(kThreads, 1) products_kernel(const __grid_cons
                             b = mul_rn(add_rn(add_rn(b, Two(bias.z, bias.w)), minus), log2e);
                             a = fma_rn(Two(exp2_of(a.lo()), exp2_of(a.hi())), times, less);
                             b = fma_rn(Two(exp2_of(b.lo()), exp2_of(b.hi())), times, less);
-                        } else if (w.leaves == kWritten) {
+                        } else {
                             a = mul_rn(a, times);
                             b = mul_rn(b, times);
                         }
@@ -380,32 +433,38 @@ __global__ void __launch_bounds__(kThreads, 1) products_kernel(const __grid_cons
                 auto piece = [&](int j, uint4 v) {
                     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(my_row + ((j ^ (lane & 7)) << 4)), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
                 };
-                const int x_last = MODE == kGradient ? h.columns : (int)h.a.width;
-                auto leave = [&](int x) {
+                auto leave = [&](int c) {
                     shared_to_copies();
                     __syncwarp();
-                    if (lane == 0 && x < x_last && row0 < w.c_last) {
-                        if (MODE == kProducts && w.leaves == kAdded32)
-                            add_box(&w.c, x, row0, mine);
+                    if (lane == 0 && x0 + c < x_last && (part || row0 < w.c_last)) {
+                        if (part)
+                            store_box(&p.part, x0 + c, row0, mine);
+                        else if (MODE == kProducts && w.leaves == kAdded32)
+                            add_box(&w.c, x0 + c, row0, mine);
                         else
-                            store_box(&w.c, x, row0, mine);
+                            store_box(&w.c, x0 + c, row0, mine);
                         boxes_commit();
                     }
                 };
-                if (MODE == kGradient || w.leaves == kWritten) {
+                if (MODE == kGradient || (w.leaves == kWritten && !part)) {
 #pragma unroll 1
                     for (int c = 0; c < HALF; c += 64) {
-                        room_free();
+                        uint32_t raw[2][32], out[32];
+                        tmem_load(raw[0], at + c);
+                        tmem_load(raw[1], at + c + 32);
+                        tmem_wait(raw[0]);
+                        tmem_wait(raw[1]);
+                        if (c + 64 >= HALF) give_back();
 #pragma unroll
                         for (int i = 0; i < 2; i++) {
                             Two v[16];
-                            values(v, c + 32 * i);
+                            values(v, raw[i], c + 32 * i);
 #pragma unroll
-                            for (int j = 0; j < 4; j++)
-                                piece(4 * i + j, make_uint4(two_of<T>(v[4 * j].lo(), v[4 * j].hi()), two_of<T>(v[4 * j + 1].lo(), v[4 * j + 1].hi()),
-                                                            two_of<T>(v[4 * j + 2].lo(), v[4 * j + 2].hi()), two_of<T>(v[4 * j + 3].lo(), v[4 * j + 3].hi())));
+                            for (int j = 0; j < 16; j++) out[16 * i + j] = two_of<T>(v[j].lo(), v[j].hi());
                         }
-                        if (c + 64 >= HALF) give_back();
+                        room_free(); // (the last box has been read meanwhile)
+#pragma unroll
+                        for (int j = 0; j < 8; j++) piece(j, make_uint4(out[4 * j], out[4 * j + 1], out[4 * j + 2], out[4 * j + 3]));
                         if constexpr (MODE == kGradient) {
 #pragma unroll
                             for (int k = 0; k < 2; k++) {
@@ -415,38 +474,46 @@ __global__ void __launch_bounds__(kThreads, 1) products_kernel(const __grid_cons
                                 asm volatile("st.shared.b16 [%0], %1;" ::"r"(my_row + ((l / 8 ^ (lane & 7)) << 4) + l % 8 * 2), "h"((uint16_t)two) : "memory");
                             }
                         }
-                        leave(column + c);
+                        leave(c);
                         if constexpr (MODE == kGradient) {
-                            if (h.bias_parts) { // sums of these 32 rows, two columns for a lane
-                                float2 s = make_float2(0.0f, 0.0f);
-#pragma unroll 8
-                                for (int r = 0; r < 32; r++) {
-                                    uint32_t two;
-                                    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(two) : "r"(mine + r * 128 + ((lane / 4 ^ (r & 7)) << 4) + lane % 4 * 4) : "memory");
+                            if (h.bias_parts) { // sums of these 32 rows: four columns for a lane, of every other row
+                                Two s0(0.0f, 0.0f), s1(0.0f, 0.0f);
+#pragma unroll
+                                for (int r = 0; r < 32; r += 2) {
+                                    const int rr = r + lane / 16;
                                     Pack<T, 4> pack;
-                                    pack.raw = make_uint2(two, 0);
                                     float f[4];
+                                    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];"
+                                                 : "=r"(pack.raw.x), "=r"(pack.raw.y)
+                                                 : "r"(mine + rr * 128 + ((lane % 16 / 2 ^ (rr & 7)) << 4) + lane % 2 * 8)
+                                                 : "memory");
                                     pack.get(f);
-                                    s.x += f[0];
-                                    s.y += f[1];
+                                    s0 = add_rn(s0, Two(f[0], f[1]));
+                                    s1 = add_rn(s1, Two(f[2], f[3]));
                                 }
-                                const int x = column + c + 2 * lane;
-                                float *to = h.bias_parts + (long long)(tile.row * 4 + quarter) * w.c_rows + x;
-                                if (x < w.c_rows) *reinterpret_cast<float2 *>(to) = s;
+                                float s[4] = {s0.lo(), s0.hi(), s1.lo(), s1.hi()};
+#pragma unroll
+                                for (int i = 0; i < 4; i++) s[i] += __shfl_down_sync(0xffffffffu, s[i], 16);
+                                const int x = column + c + 4 * lane;
+                                if (lane < 16 && x < h.chunk)
+                                    *reinterpret_cast<float4 *>(h.bias_parts + (long long)(tile.row * 4 + quarter) * h.chunk + x) = make_float4(s[0], s[1], s[2], s[3]);
                             }
                         }
                     }
                 } else {
 #pragma unroll 1
                     for (int c = 0; c < HALF; c += 32) {
-                        room_free();
+                        uint32_t raw[32];
+                        tmem_load(raw, at + c);
+                        tmem_wait(raw);
+                        if (c + 32 >= HALF) give_back();
                         Two v[16];
-                        values(v, c);
+                        values(v, raw, c);
+                        room_free();
 #pragma unroll
                         for (int j = 0; j < 8; j++)
                             piece(j, make_uint4(__float_as_uint(v[2 * j].lo()), __float_as_uint(v[2 * j].hi()), __float_as_uint(v[2 * j + 1].lo()), __float_as_uint(v[2 * j + 1].hi())));
-                        if (c + 32 >= HALF) give_back();
-                        leave(column + c);
+                        leave(c);
                     }
                 }
             }
@@ -459,46 +526,47 @@ __global__ void __launch_bounds__(kThreads, 1) products_kernel(const __grid_cons
     if (warp == 1) tmem_free(tmem, 2 * BN);
 }
 
-// Rows' statistics joined over the classes: 32 rows per CTA, whose eight warps each take every eighth part.
-__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Head h) {
-    __shared__ float s_part[8][3][32];
+// Rows' statistics joined over the classes: 32 rows per CTA, whose 32 warps each take every 32nd part.
+__global__ void __launch_bounds__(1024) join_kernel(const __grid_constant__ Head h) {
+    __shared__ float s_top[32][33], s_sum[32][33], s_away[32][33];
     wait_for_previous();
     let_next_begin();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.x * 32 + lane, rows = rows_counted(h);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rows = rows_counted(h);
     if (blockIdx.x * 32 >= rows) return;
     const bool apart = h.a.smoothing > 0.0f;
-    const int each = h.part_columns;
-    float top = kLowest, sum = 0.0f, away = 0.0f, mass = 0.0f;
-#pragma unroll 4
-    for (int k = warp; k < h.part_count; k += 8) {
-        const long long at = (long long)k * h.rows_pad + row;
-        const float2 one = h.parts[at];
-        const float most = fmaxf(top, one.x);
-        sum = sum * exp_of(top - most) + one.y * exp_of(one.x - most);
+    float top = kLowest, sum = 0.0f, away = 0.0f, mass = 0.0f; // (mass: classes seen)
+    auto add = [&](float t, float s, float d, float there) {
+        const float most = fmaxf(top, t);
+        sum = sum * exp_of(top - most) + s * exp_of(t - most);
         if (apart) {
-            const float there = (float)max(0, min(each, (int)h.a.classes - k * each));
-            away = away + mass * fmaxf(top - most, kLowest) + h.parts_apart[at] + there * fmaxf(one.x - most, kLowest);
+            away += mass * fmaxf(top - most, kLowest) + d + there * fmaxf(t - most, kLowest);
             mass += there;
         }
         top = most;
-        if (one.x != one.x) sum = NAN;
+    };
+    auto there_of = [&](int k) { return (float)max(0, min(h.part_columns, (int)h.a.classes - k * h.part_columns)); };
+    {
+        const int row = blockIdx.x * 32 + lane;
+#pragma unroll 4
+        for (int k = warp; k < h.part_count; k += 32) {
+            const long long at = (long long)k * h.rows_pad + row;
+            const float2 one = h.parts[at];
+            add(one.x, one.x != one.x ? NAN : one.y, apart ? h.parts_apart[at] : 0.0f, there_of(k));
+        }
     }
-    s_part[warp][0][lane] = top;
-    s_part[warp][1][lane] = sum;
-    s_part[warp][2][lane] = away;
+    s_top[warp][lane] = top, s_sum[warp][lane] = sum, s_away[warp][lane] = away;
     __syncthreads();
-    if (warp || row >= rows) return;
-    float most = top;
-    for (int k = 1; k < 8; k++) most = fmaxf(most, s_part[k][0][lane]);
-    sum = away = 0.0f;
-    for (int k = 0; k < 8; k++) {
-        const float t = s_part[k][0][lane];
-        sum += s_part[k][1][lane] * exp_of(t - most);
-        if (!apart) continue;
-        long long there = 0; // classes that the warp has joined
-        for (int part = k; part < h.part_count; part += 8) there += max(0, min(each, (int)h.a.classes - part * each));
-        away += s_part[k][2][lane] + (float)there * fmaxf(t - most, kLowest);
+    // now a warp has a row, and a lane what a warp had of it
+    const int row = blockIdx.x * 32 + warp;
+    if (row >= rows) return;
+    const float mine = s_top[lane][warp], most = warp_max(mine);
+    sum = warp_sum(s_sum[lane][warp] * exp_of(mine - most));
+    if (apart) {
+        long long seen = 0;
+        for (int k = lane; k < h.part_count; k += 32) seen += (int)there_of(k);
+        away = warp_sum(s_away[lane][warp] + (float)seen * fmaxf(mine - most, kLowest));
     }
+    if (lane) return;
     const long long orig = h.map ? h.map[row] : row;
     const Picks p = picks_of(h.a, orig);
     float4 *stats = reinterpret_cast<float4 *>(h.a.stats) + orig;
@@ -516,37 +584,61 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Head 
     stats->y = over;
 }
 
-// Which rows count, in their order: the place of each, or -1; a row for each place.  One CTA; rows that do not count get a loss of 0.
+// Which rows count, in their order: the place of each, or -1; a row for each place.  One cluster; rows that do not count get a loss of 0.
+constexpr int kPlacesCtas = 8;
 __global__ void __launch_bounds__(1024) places_kernel(const __grid_constant__ ffcvb_linear_cross_entropy_args a, int *map, int *place, float *counted) {
-    __shared__ int s_count[33];
+    __shared__ int s_count[32], s_before[kPlacesCtas];
     wait_for_previous();
     let_next_begin();
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); // (this one has begun)
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t *labels = static_cast<const int64_t *>(a.target);
-    // a warp has a run of rows, 32 at a time
-    const int run = (int)((a.rows + 1023) / 1024) * 32, first = warp * run, last = min(first + run, (int)a.rows);
+    // a warp has a run of rows, 32 at a time, eight loads ahead
+    const int run = (int)((a.rows + kPlacesCtas * 1024 - 1) / (kPlacesCtas * 1024)) * 32, first = (blockIdx.x * 32 + warp) * run, last = min(first + run, (int)a.rows);
+    auto counting = [&](int r0) {
+        int64_t label[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) label[i] = r0 + 32 * i + lane < last ? labels[(r0 + 32 * i + lane) * a.target_stride] : a.ignore_index;
+        uint32_t bits = 0;
+#pragma unroll
+        for (int i = 0; i < 8; i++) bits |= (label[i] != a.ignore_index ? 1u : 0u) << i;
+        return bits;
+    };
     int n = 0;
-    for (int r = first + lane; r < last; r += 32) n += labels[r * a.target_stride] != a.ignore_index;
+    for (int r0 = first; r0 < last; r0 += 256) n += __popc(counting(r0));
     n = __reduce_add_sync(0xffffffffu, n);
     if (lane == 0) s_count[warp] = n;
     __syncthreads();
     int before = __reduce_add_sync(0xffffffffu, lane < warp ? s_count[lane] : 0);
-    for (int r0 = first; r0 < last; r0 += 32) {
-        const int r = r0 + lane;
-        const bool counts = r < last && labels[r * a.target_stride] != a.ignore_index;
-        const uint32_t those = __ballot_sync(0xffffffffu, counts);
-        const int here = before + __popc(those & ((1u << lane) - 1));
-        if (counts) map[here] = r;
-        if (r < last) {
-            place[r] = counts ? here : -1;
-            if (!counts && !a.from_stats) {
-                if (a.row_loss) a.row_loss[r] = 0.0f;
-                reinterpret_cast<float4 *>(a.stats)[r] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            }
-        }
-        before += __popc(those);
+    const int whole = __reduce_add_sync(0xffffffffu, s_count[lane]);
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); // all have begun
+    if (threadIdx.x < kPlacesCtas) {
+        uint32_t there;
+        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(shared_address(s_before + blockIdx.x)), "r"(threadIdx.x));
+        asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(there), "r"(whole) : "memory");
     }
-    if (warp == 31 && lane == 0) *counted = (float)before;
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    for (int k = 0; k < (int)blockIdx.x; k++) before += s_before[k];
+    if (blockIdx.x == kPlacesCtas - 1 && warp == 31 && lane == 0) *counted = (float)(before + n);
+    for (int r0 = first; r0 < last; r0 += 256) {
+        const uint32_t bits = counting(r0);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int r = r0 + 32 * i + lane;
+            const bool counts = bits >> i & 1;
+            const uint32_t those = __ballot_sync(0xffffffffu, counts);
+            const int here = before + __popc(those & ((1u << lane) - 1));
+            if (counts) map[here] = r;
+            if (r < last) {
+                place[r] = counts ? here : -1;
+                if (!counts && !a.from_stats) {
+                    if (a.row_loss) a.row_loss[r] = 0.0f;
+                    reinterpret_cast<float4 *>(a.stats)[r] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                }
+            }
+            before += __popc(those);
+        }
+    }
 }
 
 // Rows of `width` values of 16 bits in places that the copies can begin at; rows behind those that count, up to the next 128, and columns behind
@@ -597,34 +689,29 @@ __global__ void __launch_bounds__(1024) most_kernel(const float *__restrict__ up
     }
 }
 
-// Gradients from parts of sums in 32 bits, or of rows that count from 16 bits: out[r] = sum of parts[place of r]; rows without a place are 0.
-template <typename T, typename Part>
-__global__ void __launch_bounds__(256) settle_kernel(const __grid_constant__ Head h, const Part *__restrict__ parts, long long part_size, int splits, int pad, const int *place,
-                                                     T *__restrict__ out, int rows, int width) {
+// Gradients from sums in 32 bits, or of rows that count from 16 bits: out[r] = from[place of r]; rows without a place are 0.
+template <typename T, typename From>
+__global__ void __launch_bounds__(256) settle_kernel(const __grid_constant__ Head h, const From *__restrict__ sums, int pad, const int *place, T *__restrict__ out, int rows, int width) {
     wait_for_previous();
     let_next_begin();
-    const float k = sizeof(Part) == 4 ? gradient_scale<T>(h) : 1.0f;
+    const float k = sizeof(From) == 4 ? gradient_scale<T>(h) : 1.0f;
     const int packs = (width + 7) / 8;
     const bool wide = width % 8 == 0;
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < (long long)rows * packs; i += (long long)gridDim.x * 256) {
-        const int r = (int)(i / packs), c = (int)(i % packs) * 8, from = place ? place[r] : r;
+        const int r = (int)(i / packs), c = (int)(i - (long long)r * packs) * 8, from = place ? place[r] : r;
         float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
         if (from >= 0) {
-            const Part *at = parts + (long long)from * pad + c;
-            for (int s = 0; s < splits; s++, at += part_size) {
-                constexpr int N = kWide<Part>;
+            const From *at = sums + (long long)from * pad + c;
+            constexpr int N = kWide<From>;
 #pragma unroll
-                for (int j = 0; j < 8; j += N) {
-                    Pack<Part, N> pack;
-                    float f[N];
-                    pack.load(at + j);
-                    pack.get(f);
+            for (int j = 0; j < 8; j += N) {
+                Pack<From, N> pack;
+                float f[N];
+                pack.load(at + j);
+                pack.get(f);
 #pragma unroll
-                    for (int l = 0; l < N; l++) v[j + l] += f[l];
-                }
+                for (int l = 0; l < N; l++) v[j + l] = f[l] * k;
             }
-#pragma unroll
-            for (int j = 0; j < 8; j++) v[j] *= k;
         }
         T *to = out + (long long)r * width + c;
         if (wide) {
@@ -637,57 +724,91 @@ __global__ void __launch_bounds__(256) settle_kernel(const __grid_constant__ Hea
     }
 }
 
-// The bias' gradient: sums over 32 rows each added up, 32 columns per CTA.
-template <typename T>
-__global__ void __launch_bounds__(256) bias_kernel(const __grid_constant__ Head h, int pad) {
+// What is left to do behind a chunk's products: tiles that several CTAs have parts of, added up in their order; and the bias' gradient.  The first CTAs have
+// a quarter each of the tile that a run begins in the middle of (the first such run of a tile); of the others each has 32 classes, whose sums over 32 rows it
+// adds up.
+template <typename T, int BN>
+__global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Products p) {
     __shared__ float s_sum[8][32];
     wait_for_previous();
     let_next_begin();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
-    const int parts = (rows_counted(h) + 127) / 128 * 4;
-    float sum = 0.0f;
-    if (c < h.columns) {
-#pragma unroll 8
-        for (int k = warp; k < parts; k += 8) sum += h.bias_parts[(long long)k * pad + c];
+    const Head &h = p.head;
+    const int rows = rows_counted(h), tiles = p.count ? p.ctas * 4 : 0;
+    if ((int)blockIdx.x >= tiles) {
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = ((int)blockIdx.x - tiles) * 32 + lane, parts = (rows + 127) / 128 * 4;
+        float sum = 0.0f;
+        if (c < h.columns) {
+#pragma unroll 16
+            for (int k = warp; k < parts; k += 8) sum += h.bias_parts[(long long)k * h.chunk + c];
+        }
+        s_sum[warp][lane] = sum;
+        __syncthreads();
+        if (warp || c >= h.columns) return;
+        for (int k = 1; k < 8; k++) sum += s_sum[k][lane];
+        static_cast<T *>(h.a.grad_bias)[h.first + c] = from_float<T>(sum * gradient_scale<T>(h));
+        return;
     }
-    s_sum[warp][lane] = sum;
-    __syncthreads();
-    if (warp || c >= h.columns) return;
-    for (int k = 1; k < 8; k++) sum += s_sum[k][lane];
-    static_cast<T *>(h.a.grad_bias)[h.first + c] = from_float<T>(sum * gradient_scale<T>(h));
+    const Runs runs(p, rows);
+    const int cta = (int)blockIdx.x / 4, quarter = blockIdx.x & 3, place = runs.place(cta), lane = runs.lane(cta);
+    if (place == 0 || place >= runs.ctas) return;
+    const int begin = runs.begin(place);
+    const Tile tile = tile_of(p, runs, lane, begin, rows);
+    if (tile.from == 0 || begin - runs.begin(place - 1) < tile.from) return; // (a run's own tile; one that an earlier run has begun in the middle of)
+    int last = place; // the last run with a part
+    while (last + 1 < runs.ctas && runs.begin(last + 1) - begin < tile.to - tile.from) last++;
+    const Product &w = p.of[tile.product];
+    const float k = w.leaves == kWritten ? gradient_scale<T>(h) : 1.0f;
+    const bool blank = w.counted == kSumCounted && rows == 0;
+    for (int i = threadIdx.x; i < 32 * BN / 8; i += 256) {
+        const int r = quarter * 32 + i / (BN / 8), c = i % (BN / 8) * 8, row = tile.row * 128 + r, column = tile.column * BN + c;
+        if (row >= w.c_last || column >= h.a.width) continue;
+        float v[8];
+        auto take = [&](int part, bool first) {
+            const float *at = p.parts + ((long long)part * 128 + r) * BN + c;
+#pragma unroll
+            for (int j = 0; j < 8; j += 4) {
+                const float4 f = *reinterpret_cast<const float4 *>(at + j);
+                v[j] = first ? f.x : v[j] + f.x;
+                v[j + 1] = first ? f.y : v[j + 1] + f.y;
+                v[j + 2] = first ? f.z : v[j + 2] + f.z;
+                v[j + 3] = first ? f.w : v[j + 3] + f.w;
+            }
+        };
+        take(2 * (cta - runs.lanes) + 1, true);
+#pragma unroll 4
+        for (int other = place; other <= last; other++) take(2 * (cta + (other - place) * runs.lanes), false);
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = blank ? 0.0f : v[j] * k;
+        if (w.leaves == kWritten) {
+            Pack<T, 8> pack;
+            pack.set(v);
+            pack.store(static_cast<T *>(w.out) + row * w.out_stride + column);
+            continue;
+        }
+        float *to = static_cast<float *>(w.out) + row * w.out_stride + column;
+#pragma unroll
+        for (int j = 0; j < 8; j++) to[j] = w.leaves == kAdded32 ? to[j] + v[j] : v[j];
+    }
 }
 
 // ---- the host's part -------------------------------------------------------------------------------------------------
 
 inline int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 
-// A gradient product: how its tiles are cut, and how it leaves.
-struct Cut {
-    int splits = 1;
-    bool direct = true;
-};
-
 // What a call does, and where in the workspace (offsets in bytes).
 struct Plan {
     int64_t rows_pad, width_pad, chunk, chunks;  // (classes at once)
     bool counted, lay_hidden, lay_weight, grads, hidden_grad, weight_grad, bias_grad;
     int stat_columns, sum_columns;               // BN
-    Cut of_hidden, of_weight;
-    int64_t map, place, count, most, hidden, weight, parts, apart, grad, hidden_parts, hidden_rows, weight_parts, bias_parts, bytes;
+    bool hidden_direct, weight_direct;           // products leave as they are to be
+    int ctas;
+    int64_t map, place, count, most, hidden, weight, parts, apart, grad, hidden_sums, hidden_rows, weight_sums, bias_parts, tile_parts, bytes;
 };
 
 // G's bytes at most.  (So many classes at once that dw's tiles and the sum over classes fill the GPU; 8 GB of HBM would hold 32 times as much.)
 constexpr int64_t kMostGradient = 256ll << 20;
 
 bool aligned(const void *p, int64_t stride) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && stride % 8 == 0; }
-
-// Tiles of a product, and parts of its sum where there are too few of them: parts of at least eight blocks.
-Cut cut_of(int64_t tiles, int64_t others, int64_t blocks, bool direct) {
-    Cut cut;
-    if (tiles > 0 && tiles + others < kSms && blocks >= 16) cut.splits = (int)std::min<int64_t>(blocks / 8, std::max<int64_t>(1, kSms / (tiles + others)));
-    cut.direct = direct && cut.splits == 1;
-    return cut;
-}
 
 Plan plan_of(const ffcvb_linear_cross_entropy_args &a) {
     Plan p{};
@@ -703,16 +824,10 @@ Plan plan_of(const ffcvb_linear_cross_entropy_args &a) {
     p.chunks = (a.classes * p.rows_pad * 2 + kMostGradient - 1) / kMostGradient;
     p.chunk = up((a.classes + p.chunks - 1) / p.chunks, 256);
     p.chunks = (a.classes + p.chunk - 1) / p.chunk;
-    // columns of the gradients' tiles: those that need the fewer steps
-    auto cost = [&](int64_t bn) {
-        const int64_t tiles = (row_tiles + p.chunk / 128) * ((a.width + bn - 1) / bn);
-        return (tiles + kSms - 1) / kSms * bn;
-    };
-    p.sum_columns = cost(128) < cost(256) ? 128 : 256;
-    const int64_t column_tiles = (a.width + p.sum_columns - 1) / p.sum_columns;
-    const int64_t hidden_tiles = p.hidden_grad ? row_tiles * column_tiles : 0, weight_tiles = p.weight_grad ? p.chunk / 128 * column_tiles : 0;
-    p.of_hidden = cut_of(hidden_tiles, weight_tiles, p.chunk / kSum, p.chunks == 1 && (p.counted || a.width % 8 == 0));
-    p.of_weight = cut_of(weight_tiles, hidden_tiles, (a.rows + kSum - 1) / kSum, a.width % 8 == 0);
+    p.sum_columns = a.width <= 128 ? 128 : 256;
+    p.ctas = kSms;
+    p.hidden_direct = p.chunks == 1 && (p.counted || a.width % 8 == 0);
+    p.weight_direct = a.width % 8 == 0;
     int64_t at = 0;
     auto take = [&](bool wanted, int64_t bytes) {
         const int64_t here = at;
@@ -730,9 +845,10 @@ Plan plan_of(const ffcvb_linear_cross_entropy_args &a) {
     p.apart = take(!a.from_stats && a.smoothing > 0.0f, parts * 4);
     p.grad = take(p.grads, p.rows_pad * p.chunk * 2);
     const int64_t wide = up(a.width, 32); // (boxes of 32 values)
-    p.hidden_parts = take(p.hidden_grad && !p.of_hidden.direct, p.of_hidden.splits * p.rows_pad * wide * 4);
-    p.hidden_rows = take(p.hidden_grad && p.of_hidden.direct && p.counted, p.rows_pad * p.width_pad * 2);
-    p.weight_parts = take(p.weight_grad && !p.of_weight.direct, p.of_weight.splits * p.chunk * wide * 4);
+    p.hidden_sums = take(p.hidden_grad && !p.hidden_direct, p.rows_pad * wide * 4);
+    p.hidden_rows = take(p.hidden_grad && p.hidden_direct && p.counted, p.rows_pad * p.width_pad * 2);
+    p.weight_sums = take(p.weight_grad && !p.weight_direct, p.chunk * wide * 4);
+    p.tile_parts = take(p.hidden_grad || p.weight_grad, 2ll * p.ctas * 128 * p.sum_columns * 4);
     p.bias_parts = take(p.bias_grad, p.rows_pad / 32 * p.chunk * 4);
     p.bytes = at;
     return p;
@@ -776,7 +892,21 @@ template <typename T> int run(const ffcvb_linear_cross_entropy_args &a, uint8_t 
     h.parts_apart = static_cast<float *>(at(p.apart));
     h.part_columns = p.stat_columns / 2;
     h.part_count = (int)(up(a.classes, p.stat_columns) / h.part_columns);
-    if (p.counted) launch_early(places_kernel, 1, 1024, 0, st, a, static_cast<int *>(at(p.map)), static_cast<int *>(at(p.place)), static_cast<float *>(at(p.count)));
+    if (p.counted) {
+        cudaLaunchConfig_t how{};
+        cudaLaunchAttribute with[2] = {};
+        with[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        with[0].val.programmaticStreamSerializationAllowed = 1;
+        with[1].id = cudaLaunchAttributeClusterDimension;
+        with[1].val.clusterDim.x = kPlacesCtas;
+        with[1].val.clusterDim.y = with[1].val.clusterDim.z = 1;
+        how.gridDim = dim3(kPlacesCtas);
+        how.blockDim = dim3(1024);
+        how.stream = st;
+        how.attrs = with;
+        how.numAttrs = 2;
+        cudaLaunchKernelEx(&how, places_kernel, a, static_cast<int *>(at(p.map)), static_cast<int *>(at(p.place)), static_cast<float *>(at(p.count)));
+    }
     auto lay = [&](const void *from, int64_t stride, int64_t rows, const int *map, const float *counted, void *to) {
         const unsigned ctas = (unsigned)std::min<int64_t>((up(rows, 128) * (p.width_pad / 8) + 255) / 256, kSms * 8);
         launch_early(lay_kernel, ctas, 256, 0, st, static_cast<const uint16_t *>(from), (long long)stride, (int)rows, (int)a.width, map, counted, static_cast<uint16_t *>(to),
@@ -804,7 +934,6 @@ template <typename T> int run(const ffcvb_linear_cross_entropy_args &a, uint8_t 
         w.row_tiles = (int)row_tiles;
         w.column_tiles = (int)((count + columns - 1) / columns);
         w.sum_blocks = sum_blocks;
-        w.splits = 1;
         w.a_along_sum = 0;
         w.counted = p.counted ? kRowsCounted : kFixed;
         w.b_first = (int)first;
@@ -818,7 +947,7 @@ template <typename T> int run(const ffcvb_linear_cross_entropy_args &a, uint8_t 
         if (!mapped) return training_fail(FFCVB_E_CUDA, "ffcvb_linear_cross_entropy: no map of a matrix");
         g.of[0].b_first = 0;
         fine &= launch_products<kStatistics, T>(p.stat_columns, g, tiles, st);
-        launch_early(join_kernel, (unsigned)(p.rows_pad / 32), 256, 0, st, h);
+        launch_early(join_kernel, (unsigned)(p.rows_pad / 32), 1024, 0, st, h);
         if (a.loss) launch_mean(a.row_loss, a.rows, h.counted, a.mean, a.loss, st);
     }
     if (!p.grads) return fine ? launched("ffcvb_linear_cross_entropy") : training_fail(FFCVB_E_CUDA, "ffcvb_linear_cross_entropy: %s", cudaGetErrorString(cudaGetLastError()));
@@ -830,70 +959,73 @@ template <typename T> int run(const ffcvb_linear_cross_entropy_args &a, uint8_t 
         const int columns = row_tiles * ((count + 255) / 256) < kSms ? 128 : 256;
         int64_t tiles = logits(columns, first, count);
         mapped &= matrix_map(&g.of[0].c, type, at(p.grad), p.counted ? p.rows_pad : a.rows, count, p.chunk, 32);
-        g.of[0].c_rows = (int)p.chunk; // (of the bias' sums: columns)
         g.of[0].c_last = (int)(p.counted ? p.rows_pad : a.rows);
         h.bias_parts = p.bias_grad ? static_cast<float *>(at(p.bias_parts)) : nullptr;
+        h.chunk = (int)p.chunk;
         if (!mapped) break;
         fine &= launch_products<kGradient, T>(columns, g, tiles, st);
-        if (p.bias_grad) launch_early(bias_kernel<T>, (unsigned)((count + 31) / 32), 256, 0, st, h, (int)p.chunk);
         const int column_tiles = (int)((a.width + p.sum_columns - 1) / p.sum_columns);
         g.count = 0;
-        tiles = 0;
+        g.ctas = p.ctas;
+        g.lanes = column_tiles <= 16 ? column_tiles : 1; // (few CTAs are left without one)
+        // C: in what it is to be, in rows that count, or in 32 bits
+        auto leaves_as = [&](Product &w, int how, void *out, int64_t rows, int64_t stride) {
+            w.leaves = how;
+            w.out = out;
+            w.out_stride = stride;
+            w.c_last = (int)rows;
+            w.column_tiles = column_tiles;
+            mapped &= matrix_map(&w.c, how == kWritten ? type : FFCVB_TYPE_F32, out, rows, how == kWritten ? a.width : wide, stride, 32);
+        };
         if (p.hidden_grad) {
             Product &w = g.of[g.count++];
             mapped &= matrix_map(&w.a, type, at(p.grad), p.counted ? p.rows_pad : a.rows, count, p.chunk, 128);
             mapped &= matrix_map(&w.b, type, weight, a.classes, a.width, weight_stride, kSum);
-            if (!p.of_hidden.direct)
-                mapped &= matrix_map(&w.c, FFCVB_TYPE_F32, at(p.hidden_parts), p.of_hidden.splits * p.rows_pad, wide, wide, 32);
+            if (!p.hidden_direct)
+                leaves_as(w, chunk ? kAdded32 : kWritten32, at(p.hidden_sums), p.rows_pad, wide);
             else if (p.counted)
-                mapped &= matrix_map(&w.c, type, at(p.hidden_rows), p.rows_pad, a.width, p.width_pad, 32);
+                leaves_as(w, kWritten, at(p.hidden_rows), p.rows_pad, p.width_pad);
             else
-                mapped &= matrix_map(&w.c, type, a.grad_hidden, a.rows, a.width, a.width, 32);
+                leaves_as(w, kWritten, a.grad_hidden, a.rows, a.width);
             w.row_tiles = (int)row_tiles;
-            w.column_tiles = column_tiles;
             w.sum_blocks = (int)((count + kSum - 1) / kSum);
-            w.splits = p.of_hidden.splits;
             w.a_along_sum = 0;
-            w.leaves = p.of_hidden.direct ? kWritten : chunk ? kAdded32 : kWritten32;
             w.counted = p.counted ? kRowsCounted : kFixed;
             w.b_first = (int)first;
-            w.c_rows = (int)p.rows_pad;
-            w.c_last = (int)(!p.of_hidden.direct ? p.of_hidden.splits * p.rows_pad : p.counted ? p.rows_pad : a.rows);
-            tiles += row_tiles * column_tiles * w.splits;
         }
         if (p.weight_grad) {
             Product &w = g.of[g.count++];
             mapped &= matrix_map(&w.a, type, at(p.grad), p.counted ? p.rows_pad : a.rows, count, p.chunk, kSum);
             mapped &= matrix_map(&w.b, type, hidden, hidden_rows, a.width, hidden_stride, kSum);
-            if (p.of_weight.direct)
-                mapped &= matrix_map(&w.c, type, static_cast<T *>(a.grad_weight) + first * a.width, count, a.width, a.width, 32);
+            if (p.weight_direct)
+                leaves_as(w, kWritten, static_cast<T *>(a.grad_weight) + first * a.width, count, a.width);
             else
-                mapped &= matrix_map(&w.c, FFCVB_TYPE_F32, at(p.weight_parts), p.of_weight.splits * p.chunk, wide, wide, 32);
+                leaves_as(w, kWritten32, at(p.weight_sums), p.chunk, wide);
             w.row_tiles = (int)((count + 127) / 128);
-            w.column_tiles = column_tiles;
             w.sum_blocks = (int)((a.rows + kSum - 1) / kSum);
-            w.splits = p.of_weight.splits;
             w.a_along_sum = 1;
-            w.leaves = p.of_weight.direct ? kWritten : kWritten32;
             w.counted = p.counted ? kSumCounted : kFixed;
             w.b_first = 0;
-            w.c_rows = (int)p.chunk;
-            w.c_last = (int)(p.of_weight.direct ? count : p.of_weight.splits * p.chunk);
-            tiles += (int64_t)w.row_tiles * column_tiles * w.splits;
+        }
+        if (g.count) {
+            g.parts = static_cast<float *>(at(p.tile_parts));
+            mapped &= matrix_map(&g.part, FFCVB_TYPE_F32, at(p.tile_parts), 2 * p.ctas * 128, p.sum_columns, p.sum_columns, 32);
         }
         if (!mapped) break;
-        if (g.count) fine &= launch_products<kProducts, T>(p.sum_columns, g, tiles, st);
-        if (p.weight_grad && !p.of_weight.direct)
-            launch_early(settle_kernel<T, float>, ctas_for(count), 256, 0, st, h, static_cast<const float *>(at(p.weight_parts)), (long long)(p.chunk * wide),
-                         p.of_weight.splits, (int)wide, (const int *)nullptr, static_cast<T *>(a.grad_weight) + first * a.width, (int)count, (int)a.width);
+        if (g.count) fine &= launch_products<kProducts, T>(p.sum_columns, g, p.ctas, st);
+        const unsigned finish = (unsigned)((g.count ? p.ctas * 4 : 0) + (p.bias_grad ? (count + 31) / 32 : 0));
+        if (finish) launch_early(p.sum_columns == 256 ? finish_kernel<T, 256> : finish_kernel<T, 128>, finish, 256, 0, st, g);
+        if (p.weight_grad && !p.weight_direct)
+            launch_early(settle_kernel<T, float>, ctas_for(count), 256, 0, st, h, static_cast<const float *>(at(p.weight_sums)), (int)wide, (const int *)nullptr,
+                         static_cast<T *>(a.grad_weight) + first * a.width, (int)count, (int)a.width);
     }
     if (!mapped) return training_fail(FFCVB_E_CUDA, "ffcvb_linear_cross_entropy: no map of a matrix");
-    if (p.hidden_grad && !p.of_hidden.direct)
-        launch_early(settle_kernel<T, float>, ctas_for(a.rows), 256, 0, st, h, static_cast<const float *>(at(p.hidden_parts)), (long long)(p.rows_pad * wide), p.of_hidden.splits,
-                     (int)wide, h.place, static_cast<T *>(a.grad_hidden), (int)a.rows, (int)a.width);
+    if (p.hidden_grad && !p.hidden_direct)
+        launch_early(settle_kernel<T, float>, ctas_for(a.rows), 256, 0, st, h, static_cast<const float *>(at(p.hidden_sums)), (int)wide, h.place, static_cast<T *>(a.grad_hidden),
+                     (int)a.rows, (int)a.width);
     else if (p.hidden_grad && p.counted)
-        launch_early(settle_kernel<T, T>, ctas_for(a.rows), 256, 0, st, h, static_cast<const T *>(at(p.hidden_rows)), 0ll, 1, (int)p.width_pad, h.place,
-                     static_cast<T *>(a.grad_hidden), (int)a.rows, (int)a.width);
+        launch_early(settle_kernel<T, T>, ctas_for(a.rows), 256, 0, st, h, static_cast<const T *>(at(p.hidden_rows)), (int)p.width_pad, h.place, static_cast<T *>(a.grad_hidden),
+                     (int)a.rows, (int)a.width);
     return fine ? launched("ffcvb_linear_cross_entropy") : training_fail(FFCVB_E_CUDA, "ffcvb_linear_cross_entropy: %s", cudaGetErrorString(cudaGetLastError()));
 }
 
