@@ -11,6 +11,7 @@
 // class may come twice.  So the row crosses HBM once each way.
 #include "losses.h"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace ffcvb {
@@ -40,15 +41,22 @@ struct Sums {
         seen += o.seen;
     }
     // joins those of groups of LANES lanes
-    template <int LANES> __device__ __forceinline__ void join_lanes(float rate) {
+    template <int LANES, bool HARD> __device__ __forceinline__ void join_lanes(float rate, bool spread) {
         float most = top;
 #pragma unroll
         for (int o = LANES / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-        to(most, rate);
+        soft *= exp2_of((top - most) * rate);
+        if (HARD) hard *= exp_of(top - most);
+        if (spread) away += shift(seen, top, most);
+        top = most;
 #pragma unroll
         for (int o = LANES / 2; o > 0; o >>= 1) {
             soft += __shfl_xor_sync(0xffffffffu, soft, o);
-            hard += __shfl_xor_sync(0xffffffffu, hard, o);
+            if (HARD) hard += __shfl_xor_sync(0xffffffffu, hard, o);
+        }
+        if (!spread) return;
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) {
             away += __shfl_xor_sync(0xffffffffu, away, o);
             seen += __shfl_xor_sync(0xffffffffu, seen, o);
         }
@@ -85,31 +93,9 @@ __device__ __forceinline__ float logit_of(const ffcvb_distillation_args &a, long
                                               : to_float(static_cast<const __nv_bfloat16 *>(a.teacher)[at]);
 }
 
-// How rows are dealt out: whether logits and gradient lie alike to 16-byte boundaries; packs of a CTA's part of a row; places of the table of classes.
+// How rows are dealt out: whether logits and gradient lie alike to 16-byte boundaries; packs of a CTA's part of a row.
 struct Deal {
-    int wide, part, slots;
-};
-
-// A table of the classes that a row has entries of, open addressing: the class, and the first entry with it.
-struct Table {
-    int *key, *first;
-    int slots; // a power of two, more than there are entries
-    __device__ __forceinline__ int start(int c) const { return (int)((uint32_t)c * 2654435761u >> 7) & (slots - 1); }
-    // whether the class was there before
-    __device__ __forceinline__ bool insert(int c, int entry) const {
-        for (int s = start(c);; s = (s + 1) & (slots - 1)) {
-            const int was = atomicCAS(key + s, -1, c);
-            if (was != -1 && was != c) continue;
-            atomicMin(first + s, entry);
-            return was == c;
-        }
-    }
-    // its first entry, or -1
-    __device__ __forceinline__ int find(int c) const {
-        for (int s = start(c); key[s] != -1; s = (s + 1) & (slots - 1))
-            if (key[s] == c) return first[s];
-        return -1;
-    }
+    int wide, part;
 };
 
 // WARP: a row per warp, one entry per lane, in CTAs of four; else a row per CTA or cluster.  STAGED: packs go through shared memory; else they are read
@@ -119,8 +105,7 @@ __global__ void __launch_bounds__(WARP ? 128 : 256)
 distill_kernel(const __grid_constant__ ffcvb_distillation_args a, const Deal deal) {
     constexpr int N = kWide<T>, BATCH = STAGED ? 1 : 4; // packs that a thread has on their way
     __shared__ float s_part[8][8], s_there[8][8];       // of the CTA's warps, of the cluster's CTAs
-    __shared__ float s_soft[8];
-    __shared__ int s_twice, s_bad;
+    __shared__ int s_bad;
     extern __shared__ uint4 s_row[];
     wait_for_previous();
     let_next_begin();
@@ -142,15 +127,22 @@ distill_kernel(const __grid_constant__ ffcvb_distillation_args a, const Deal dea
     const int packs = (classes - before) / N, singles = classes - packs * N;
     const int first = (int)rank * deal.part, count = max(0, min(packs - first, deal.part));
     const T *x0 = x + before + (long long)first * N;
-    // entries' classes, shares and table lie before the row's packs
-    int *s_class = reinterpret_cast<int *>(s_row);
-    float *s_share = reinterpret_cast<float *>(s_class + kept);
-    const Table table{s_class + 2 * kept, s_class + 2 * kept + deal.slots, deal.slots};
-    const int head = WARP ? 0 : (2 * kept + 2 * deal.slots + 3) / 4;
-    const uint32_t mine = (uint32_t)__cvta_generic_to_shared(s_row + head + (WARP ? threadIdx.x / 32 * deal.part : 0) + thread);
+    // before the row's packs: entries' classes, teacher's logits over the temperature, own logits; of each thread a list of those entries whose classes it writes
+    int *s_class = reinterpret_cast<int *>(s_row), *s_next = s_class + 3 * kept, *s_first = s_next + kept;
+    float *s_given = reinterpret_cast<float *>(s_class + kept), *s_logit = s_given + kept;
+    const int head = WARP ? 0 : (4 * kept + threads + 3) / 4;
+    // (a CTA's threads keep their first pack in registers: so much less shared memory, five CTAs of 21841 logits on an SM and not four)
+    constexpr bool OWN = STAGED && !WARP;
+    const uint32_t mine = (uint32_t)__cvta_generic_to_shared(s_row + head + (WARP ? threadIdx.x / 32 * deal.part : 0) + thread) - (OWN ? threads * 16 : 0);
+    Pack<T, N> own;
     if (STAGED) {
         uint32_t to = mine;
-        for (int k = thread; k < count; k += threads, to += threads * 16) copy16(to, x0 + (long long)k * N);
+        for (int k = thread; k < count; k += threads, to += threads * 16) {
+            if (OWN && k == thread)
+                own.load(x0 + (long long)k * N);
+            else
+                copy16(to, x0 + (long long)k * N);
+        }
         asm volatile("cp.async.commit_group;" ::: "memory");
     }
     auto single = [&](int k) { return k < before ? k : k + packs * N; }; // class of the k-th besides packs
@@ -163,35 +155,62 @@ distill_kernel(const __grid_constant__ ffcvb_distillation_args a, const Deal dea
     const float tau = a.temperature, rate = kLog2e / tau;
     Given given{kLowest, 0.0f};
     int my_class = -1; // (WARP)
-    float my_logit = 0.0f;
+    float my_logit = 0.0f, my_x = 0.0f;
     bool bad = p.bad;
     if (WARP) {
         if (lane < kept) {
             const long long c = class_of(a, row, lane);
             bad |= c >= classes;
             my_class = c < 0 || c >= classes ? -1 : (int)c;
-            if (my_class >= 0) given.add(my_logit = logit_of(a, row, lane) / tau);
+            if (my_class >= 0) {
+                my_x = to_float(x[my_class]);
+                given.add(my_logit = logit_of(a, row, lane) / tau);
+            }
         }
         bad = __any_sync(0xffffffffu, bad);
         given.join_lanes<32>();
     } else {
-        if (thread == 0) s_twice = s_bad = 0;
-        for (int s = thread; s < deal.slots; s += threads) table.key[s] = -1, table.first[s] = kMostKept;
+        if (thread == 0) s_bad = 0;
+        s_first[thread] = -1;
         __syncthreads();
-        for (int k = thread; k < kept; k += threads) {
+    }
+    // The thread that writes a class, or -1: one of another CTA.
+    auto writer = [&](int c) {
+        const int in = c - before;
+        if (in >= 0 && in < packs * N) {
+            const int mine = in / N - first;
+            return mine < 0 || mine >= count ? -1 : mine % threads;
+        }
+        const int k = in < 0 ? c : c - packs * N;
+        return k / threads % (int)ranks == (int)rank ? k % threads : -1;
+    };
+    // (WARP not:) A thread's first entry is loaded ahead, its class at once, its logit here once the row is, and taken behind the first pass.
+    const long long ahead = !WARP && thread < kept ? class_of(a, row, thread) : -1;
+    float ahead_logit = !WARP && thread < kept ? logit_of(a, row, thread) : 0.0f, ahead_x = 0.0f;
+    auto take_entry = [&](int k, long long c, float t, float v) {
+        bad |= c >= classes;
+        const int here = c < 0 || c >= classes || t == -INFINITY ? -1 : (int)c; // (rows that are filled up with one class have no long lists)
+        s_class[k] = here;
+        if (here < 0) return;
+        s_given[k] = t / tau;
+        s_logit[k] = v;
+        given.add(t / tau);
+        const int by = writer(here);
+        if (by >= 0) s_next[k] = atomicExch(s_first + by, k);
+    };
+    auto load_ahead = [&] {
+        if (!WARP && ahead >= 0 && ahead < classes) ahead_x = to_float(x[ahead]);
+    };
+    auto take_entries = [&] {
+        if (WARP) return;
+        if (thread < kept) take_entry(thread, ahead, ahead_logit, ahead_x);
+        for (int k = thread + threads; k < kept; k += threads) {
             const long long c = class_of(a, row, k);
-            bad |= c >= classes;
-            const int here = c < 0 || c >= classes ? -1 : (int)c;
-            s_class[k] = here;
-            if (here < 0) continue;
-            const float t = logit_of(a, row, k) / tau;
-            s_share[k] = t;
-            given.add(t);
-            if (table.insert(here, k)) s_twice = 1;
+            take_entry(k, c, logit_of(a, row, k), c >= 0 && c < classes ? to_float(x[c]) : 0.0f);
         }
         if (bad) s_bad = 1;
         given.join_lanes<32>();
-    }
+    };
     if (p.ignored) { // (all of a row's threads alike)
         const T zero = from_float<T>(0.0f);
         if (g)
@@ -211,8 +230,11 @@ distill_kernel(const __grid_constant__ ffcvb_distillation_args a, const Deal dea
         const T *from = x0 + (long long)thread * N;
         int c = before + (first + thread) * N;
         const int step = threads * N;
+        int k = 0;
         auto load = [&](Pack<T, N> &pack, int i) {
-            if constexpr (STAGED) {
+            if (OWN && k + i == 0) {
+                pack = own;
+            } else if constexpr (STAGED) {
                 uint4 &r = pack.raw;
                 asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(at + i * threads * 16) : "memory");
             } else {
@@ -224,7 +246,6 @@ distill_kernel(const __grid_constant__ ffcvb_distillation_args a, const Deal dea
             pack.get(v);
             f(v, c + i * step);
         };
-        int k = 0;
         for (; k + BATCH <= turns; k += BATCH) {
             Pack<T, N> pack[BATCH];
 #pragma unroll
@@ -290,8 +311,13 @@ distill_kernel(const __grid_constant__ ffcvb_distillation_args a, const Deal dea
             take(v, c);
         });
         if (STAGED) asm volatile("cp.async.wait_group 0;" ::: "memory");
+        load_ahead();
         each_pack(take);
-        sums.join_lanes<32>(rate);
+        take_entries();
+        sums.join_lanes<32, HARD>(rate, spread);
+    } else {
+        load_ahead();
+        take_entries();
     }
     if (!WARP) {
         const int warps = blockDim.x >> 5;
@@ -304,7 +330,7 @@ distill_kernel(const __grid_constant__ ffcvb_distillation_args a, const Deal dea
         const bool there = (lane & 7) < warps; // (at most eight)
         sums = there ? Sums{from[0], from[1], from[2], from[3], from[4]} : Sums{kLowest, 0.0f, 0.0f, 0.0f, 0.0f};
         given = there ? Given{from[5], from[6]} : Given{kLowest, 0.0f};
-        sums.join_lanes<8>(rate);
+        sums.join_lanes<8, HARD>(rate, spread);
         given.join_lanes<8>();
         bad = s_bad != 0;
         if (ranks > 1) {
@@ -349,25 +375,35 @@ distill_kernel(const __grid_constant__ ffcvb_distillation_args a, const Deal dea
         if (HARD) out += times_hard * exp_of(d);
         return out;
     };
-    // Shares of the entries, and the soft loss: sum q (log q - log p).
-    float loss = 0.0f;
-    auto entry = [&](int c, float t) {
-        const float less = t - given.top, q = exp_of(less) * over_given;
-        if (q != 0.0f && !a.from_stats) loss += q * (less - (to_float(x[c]) - top) / tau);
-        return q;
-    };
-    float my_share = 0.0f;
-    if (WARP) {
-        if (my_class >= 0 && !bad) my_share = entry(my_class, my_logit);
-    } else if (!bad) {
-        for (int k = thread; k < kept; k += threads)
-            if (s_class[k] >= 0) s_share[k] = entry(s_class[k], s_share[k]);
-    }
-    if (!a.from_stats) {
+    auto share_of = [&](float t) { return exp_of(t - given.top) * over_given; };
+    if (thread < 32 && rank == 0 && !a.from_stats) { // a warp has the loss
+        // the soft one is sum q (log q - log p); log q has the teacher's sum, log p the student's, both once for all shares
+        float loss = 0.0f;
+        auto add = [&](float t, float v) {
+            const float q = share_of(t);
+            if (q != 0.0f) loss += q * ((t - given.top) - (v - top) / tau);
+        };
+        if (WARP) {
+            if (my_class >= 0) add(my_logit, my_x);
+        } else {
+            for (int k = lane; k < kept; k += 32)
+                if (s_class[k] >= 0) add(s_given[k], s_logit[k]);
+        }
         loss = warp_sum(loss);
-        if (!WARP && lane == 0) s_soft[threadIdx.x >> 5] = loss;
+        if (lane == 0) {
+            float out = soft == 0.0f || all == 0.0f ? 0.0f : soft * tau * tau * (loss + logf(sums.soft) - logf(given.sum));
+            if (HARD) {
+                float dot = spread ? p.flat * sums.away : 0.0f;
+#pragma unroll
+                for (int k = 0; k < 2; k++)
+                    if (p.weight[k] != 0.0f && !bad) dot += p.weight[k] * (to_float(x[p.label[k]]) - top);
+                out += hard * (p.total * logf(sums.hard) - dot);
+            }
+            a.row_loss[row] = bad ? NAN : blank ? 0.0f : out;
+        }
     }
-    if (g) {
+    if (!g) return;
+    {
         each_single([&](int c) { g[c] = from_float<T>(common(to_float(x[c]))); });
         const Two minus(-top, -top), rates(rate, rate), log2e(kLog2e, kLog2e), less(-flat, -flat), soft2(times_soft, times_soft), hard2(times_hard, times_hard);
         each_pack([&](float(&v)[N], int c) {
@@ -387,35 +423,10 @@ distill_kernel(const __grid_constant__ ffcvb_distillation_args a, const Deal dea
             pack.store(g + c);
         });
     }
-    if (WARP)
-        __syncwarp();
-    else
-        __syncthreads();
-    if (thread == 0 && rank == 0 && !a.from_stats) {
-        if (!WARP)
-            for (int k = 1; k < (int)blockDim.x >> 5; k++) loss += s_soft[k];
-        // (log q has the teacher's sum, log p the student's, both once for all shares)
-        float out = soft == 0.0f || all == 0.0f ? 0.0f : soft * tau * tau * (loss + logf(sums.soft) - logf(given.sum));
-        if (HARD) {
-            float dot = spread ? p.flat * sums.away : 0.0f;
-#pragma unroll
-            for (int k = 0; k < 2; k++)
-                if (p.weight[k] != 0.0f && !bad) dot += p.weight[k] * (to_float(x[p.label[k]]) - top);
-            out += hard * (p.total * logf(sums.hard) - dot);
-        }
-        a.row_loss[row] = bad ? NAN : blank ? 0.0f : out;
-    }
-    if (!g || bad) return;
-    // Classes with entries or labels once more.  Of a cluster the CTA does it that has written the class before.
-    auto written_here = [&](int c) {
-        if (WARP || ranks == 1) return true;
-        const int in = c - before;
-        if (in >= 0 && in < packs * N) return in / N / deal.part == (int)rank;
-        const int k = in < 0 ? c : c - packs * N;
-        return k / threads % (int)ranks == (int)rank;
-    };
-    auto again = [&](int c, float share) {
-        float v = common(to_float(x[c])) - k_soft * share;
+    if (bad) return;
+    // Classes with entries or labels once more, by the thread that has written them (or the warp), with the shares of all entries of a class in their order.
+    auto again = [&](int c, float logit, float share) {
+        float v = common(logit) - k_soft * share;
         if (HARD) {
 #pragma unroll
             for (int k = 0; k < 2; k++)
@@ -423,34 +434,41 @@ distill_kernel(const __grid_constant__ ffcvb_distillation_args a, const Deal dea
         }
         g[c] = from_float<T>(v);
     };
-    bool alone[2]; // labels without an entry
+    bool alone[2]; // labels without an entry, which this thread writes
     if (WARP) {
+        __syncwarp();
+        const float mine_share = my_class >= 0 ? share_of(my_logit) : 0.0f;
         const uint32_t same = __match_any_sync(0xffffffffu, my_class);
         float share = 0.0f;
         for (int k = 0; k < kept; k++) { // (all lanes take part)
-            const float s = __shfl_sync(0xffffffffu, my_share, k);
+            const float s = __shfl_sync(0xffffffffu, mine_share, k);
             if (same >> k & 1) share += s;
         }
-        if (my_class >= 0 && lane == __ffs(same) - 1) again(my_class, share);
+        if (my_class >= 0 && lane == __ffs(same) - 1) again(my_class, my_x, share);
 #pragma unroll
-        for (int k = 0; k < 2; k++) alone[k] = HARD && !__any_sync(0xffffffffu, my_class >= 0 && my_class == (int)p.label[k]);
+        for (int k = 0; k < 2; k++) alone[k] = HARD && !__any_sync(0xffffffffu, my_class >= 0 && my_class == (int)p.label[k]) && thread == k;
     } else {
-        for (int k = thread; k < kept; k += threads) {
-            const int c = s_class[k];
-            if (c < 0 || !written_here(c) || table.find(c) != k) continue;
-            float share = s_share[k];
-            if (s_twice)
-                for (int j = k + 1; j < kept; j++)
-                    if (s_class[j] == c) share += s_share[j];
-            again(c, share);
-        }
 #pragma unroll
-        for (int k = 0; k < 2; k++) alone[k] = HARD && thread == k && p.label[k] >= 0 && table.find((int)p.label[k]) < 0 && written_here((int)p.label[k]);
+        for (int k = 0; k < 2; k++) alone[k] = HARD && p.label[k] >= 0 && writer((int)p.label[k]) == thread;
+        for (int k = s_first[thread]; k >= 0; k = s_next[k]) {
+            const int c = s_class[k];
+#pragma unroll
+            for (int l = 0; l < 2; l++) alone[l] = alone[l] && c != (int)p.label[l];
+            bool earlier = false, later = false; // entries of the same class: they are in the same list
+            for (int j = s_first[thread]; j >= 0 && !earlier; j = s_next[j])
+                if (j != k && s_class[j] == c) (j < k ? earlier : later) = true;
+            if (earlier) continue;
+            float share = share_of(s_given[k]);
+            if (later)
+                for (int j = k + 1; j < kept; j++)
+                    if (s_class[j] == c) share += share_of(s_given[j]);
+            again(c, s_logit[k], share);
+        }
     }
     if (HARD) {
 #pragma unroll
         for (int k = 0; k < 2; k++)
-            if (thread == k && alone[k] && p.label[k] >= 0 && !(k == 1 && p.label[0] == p.label[1])) again((int)p.label[k], 0.0f);
+            if (alone[k] && p.label[k] >= 0 && !(k == 1 && p.label[0] == p.label[1])) again((int)p.label[k], to_float(x[p.label[k]]), 0.0f);
     }
 }
 
@@ -494,13 +512,11 @@ template <typename T, bool HARD> void launch_rows(const ffcvb_distillation_args 
     int ctas = 1;
     while (ctas < 8 && ((both && (packs + ctas - 1) / ctas * 16 > kPartBytes) || (a.rows * ctas <= kSms && packs > 2048 * ctas))) ctas *= 2;
     deal.part = (int)((packs + ctas - 1) / ctas);
-    deal.slots = 64;
-    while (deal.slots * 2 < a.kept * 3) deal.slots *= 2;
     const bool staged = both && deal.part * 16ll <= kMostPartBytes; // (else the second pass reads what the caches still have)
     const int threads = (deal.part / 14 + 31) / 32 * 32;
     how.gridDim = dim3((unsigned)(a.rows * ctas));
     how.blockDim = dim3(!deal.wide || threads > 256 ? 256 : threads < 64 ? 64 : threads);
-    how.dynamicSmemBytes = (2 * a.kept + 2 * deal.slots + 3) / 4 * 16 + (staged ? deal.part * 16ll : 0);
+    how.dynamicSmemBytes = (4 * a.kept + how.blockDim.x + 3) / 4 * 16 + (staged ? std::max(0, deal.part - (int)how.blockDim.x) * 16ll : 0);
     if (ctas > 1) {
         cudaLaunchAttribute &cluster = with[how.numAttrs++];
         cluster.id = cudaLaunchAttributeClusterDimension;

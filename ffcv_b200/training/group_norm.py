@@ -10,7 +10,11 @@ _NAMES = ('x', 'weight', 'bias')
 def _strides(t):
     """Strides of samples and positions of (samples, channels, ...) whose channels lie together and whose positions are evenly apart, or
     None.  Dimensions of one value may have any stride."""
-    samples, channels, *sides = t.shape
+    shape = t.shape
+    if len(shape) == 4 and t.is_contiguous(memory_format=ch.channels_last):  # (as most are: 1 us and not 3)
+        channels = shape[1]
+        return shape[2] * shape[3] * channels, channels
+    samples, channels, *sides = shape
     if t.numel() == 0:
         return 0, channels
     stride = t.stride()
@@ -38,6 +42,8 @@ def _last(t):
 
 def _new(t):
     """Room for a dense result of a tensor's shape, channels last."""
+    if t.dim() == 4:
+        return ch.empty(t.shape, dtype=t.dtype, device=t.device, memory_format=ch.channels_last)
     samples, channels, *sides = t.shape
     return ch.empty((samples, *sides, channels), dtype=t.dtype, device=t.device).movedim(-1, 1)
 
