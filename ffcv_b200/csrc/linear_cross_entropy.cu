@@ -19,16 +19,17 @@ namespace {
 constexpr int kThreads = 320; // a warp that copies, one that multiplies, eight that take the results
 constexpr int kSum = 64;      // of the sum's terms in a stage: 128 bytes
 constexpr uint32_t kRowsBytes = 128 * 128, kStagingBytes = 8 * 4096;
-template <int BN> constexpr int kStages = BN == 256 ? 4 : 6;
-template <int BN> constexpr uint32_t kStageBytes = kRowsBytes + BN * 128;
+// (of a pair's 256 columns each CTA has 128)
+template <int BN, bool PAIR> constexpr uint32_t kStageBytes = kRowsBytes + (PAIR ? BN / 2 : BN) * 128;
+template <int BN, bool PAIR> constexpr int kStages = 6 * 32768 / kStageBytes<BN, PAIR>;
 // stages, the eight warps' staging, the bias of a tile, barriers; and what it takes to begin on 1024 bytes
-template <int BN> constexpr uint32_t kRoom = kStages<BN> * kStageBytes<BN> + kStagingBytes + 1024 + 256 + 1024;
+template <int BN, bool PAIR> constexpr uint32_t kRoom = kStages<BN, PAIR> * kStageBytes<BN, PAIR> + kStagingBytes + 1024 + 256 + 1024;
 
 enum { kStatistics, kGradient, kProducts };      // what a kernel makes of its products
 enum { kWritten, kWritten32, kAdded32 };         // how products leave: as they are to be, or in 32 bits
 enum { kFixed, kRowsCounted, kSumCounted };      // what depends on the number of rows that count
 
-// One product A B of matrices, in tiles of 128 by BN.
+// One product A B of matrices, in tiles of 128, or a pair's 256, by BN.
 struct alignas(64) Product {
     CUtensorMap a, b, c;
     void *out;           // what C is a map of (kProducts)
@@ -60,8 +61,9 @@ struct Products {
     Product of[2];
     CUtensorMap part;    // [2 * CTAs * 128, BN]
     const float *parts;
-    int count, ctas, lanes;
-    int unused[11];
+    int count, units, lanes; // (units: CTAs or pairs)
+    int high;                // rows of a tile
+    int unused[10];
     Head head;
 };
 
@@ -94,26 +96,26 @@ struct Tile {
     int product, row, column, from, to;
     bool whole;
 };
-__device__ __forceinline__ int row_tiles_of(const Product &w, int rows) { return w.counted == kRowsCounted ? (rows + 127) / 128 : w.row_tiles; }
+__device__ __forceinline__ int row_tiles_of(const Products &p, const Product &w, int rows) { return w.counted == kRowsCounted ? (rows + p.high - 1) / p.high : w.row_tiles; }
 // (a sum without terms is one block long, all the same)
 __device__ __forceinline__ int sum_blocks_of(const Product &w, int rows) { return w.counted == kSumCounted ? max(1, (rows + kSum - 1) / kSum) : w.sum_blocks; }
 // Blocks of runs, at least: shorter ones cost more than they save.
 constexpr int kLeastRun = 4;
-// How blocks are dealt out: with few columns of tiles those of each column, in the same way to as many CTAs, so that CTAs with the same rows read A at the same time;
+// How blocks are dealt out: with few columns of tiles those of each column, in the same way to as many CTAs or pairs, so that those with the same rows read A at the same time;
 // else of all tiles, those of the same columns one after another.
 struct Runs {
-    int lanes, all, ctas; // columns that are dealt out apart; blocks, and CTAs with a run, of each
+    int lanes, all, units; // columns that are dealt out apart; blocks, and CTAs or pairs with a run, of each
     int each, more;       // blocks of a run, and runs with one more
     __device__ __forceinline__ Runs(const Products &p, int rows) : lanes(p.lanes), all(0) {
-        for (int i = 0; i < p.count; i++) all += row_tiles_of(p.of[i], rows) * sum_blocks_of(p.of[i], rows);
+        for (int i = 0; i < p.count; i++) all += row_tiles_of(p, p.of[i], rows) * sum_blocks_of(p.of[i], rows);
         if (lanes == 1) all *= p.of[0].column_tiles;
-        ctas = min(p.ctas / lanes, max(1, all / kLeastRun));
-        each = all / ctas;
-        more = all - each * ctas;
+        units = min(p.units / lanes, max(1, all / kLeastRun));
+        each = all / units;
+        more = all - each * units;
     }
     __device__ __forceinline__ int begin(int n) const { return each * n + min(n, more); }
-    __device__ __forceinline__ int lane(int cta) const { return cta % lanes; }
-    __device__ __forceinline__ int place(int cta) const { return cta / lanes; }
+    __device__ __forceinline__ int lane(int unit) const { return unit % lanes; }
+    __device__ __forceinline__ int place(int unit) const { return unit / lanes; }
 };
 // The tile that block `at` of a lane's is in, from that block on.
 __device__ __forceinline__ Tile tile_of(const Products &p, const Runs &runs, int lane, int at, int rows) {
@@ -121,11 +123,11 @@ __device__ __forceinline__ Tile tile_of(const Products &p, const Runs &runs, int
     tile.product = 0;
     const int columns = runs.lanes == 1 ? p.of[0].column_tiles : 1;
     if (p.count > 1) {
-        const int here = row_tiles_of(p.of[0], rows) * sum_blocks_of(p.of[0], rows) * columns;
+        const int here = row_tiles_of(p, p.of[0], rows) * sum_blocks_of(p.of[0], rows) * columns;
         if (at >= here) at -= here, tile.product = 1;
     }
     const Product &w = p.of[tile.product];
-    const int blocks = sum_blocks_of(w, rows), row_tiles = row_tiles_of(w, rows), t = at / blocks;
+    const int blocks = sum_blocks_of(w, rows), row_tiles = row_tiles_of(p, w, rows), t = at / blocks;
     tile.from = at - t * blocks;
     tile.to = blocks;
     tile.column = columns == 1 ? 0 : t / row_tiles;
@@ -137,26 +139,27 @@ __device__ __forceinline__ Tile tile_of(const Products &p, const Runs &runs, int
 // A CTA's tiles one after another.
 template <int MODE> struct Walk {
     long long at, end;
-    __device__ __forceinline__ Walk(const Products &p, int rows) {
-        at = blockIdx.x;
-        end = (long long)row_tiles_of(p.of[0], rows) * p.of[0].column_tiles;
+    int step;
+    __device__ __forceinline__ Walk(const Products &p, int rows, int unit) : step(p.units) {
+        at = unit;
+        end = (long long)row_tiles_of(p, p.of[0], rows) * p.of[0].column_tiles;
     }
     __device__ __forceinline__ bool next(const Products &p, int rows, Tile &tile) { // tiles of the same weights one after another
         if (at >= end) return false;
-        const int row_tiles = row_tiles_of(p.of[0], rows), column = (int)(at / row_tiles);
+        const int row_tiles = row_tiles_of(p, p.of[0], rows), column = (int)(at / row_tiles);
         tile = Tile{0, (int)(at - (long long)column * row_tiles), column, 0, p.of[0].sum_blocks, true};
-        at += gridDim.x;
+        at += step;
         return true;
     }
 };
 template <> struct Walk<kProducts> {
     Runs runs;
     int lane, at, end;
-    __device__ __forceinline__ Walk(const Products &p, int rows) : runs(p, rows) {
-        const int place = runs.place(blockIdx.x);
-        lane = runs.lane(blockIdx.x);
-        at = place < runs.ctas ? runs.begin(place) : 0;
-        end = place < runs.ctas ? runs.begin(place + 1) : 0;
+    __device__ __forceinline__ Walk(const Products &p, int rows, int unit) : runs(p, rows) {
+        const int place = runs.place(unit);
+        lane = runs.lane(unit);
+        at = place < runs.units ? runs.begin(place) : 0;
+        end = place < runs.units ? runs.begin(place + 1) : 0;
     }
     __device__ __forceinline__ bool next(const Products &p, int rows, Tile &tile) {
         if (at >= end) return false;
@@ -172,11 +175,12 @@ template <> struct Walk<kProducts> {
 
 // A CTA per SM that takes tile after tile.  Products of the next tile go into the other half of TMEM while eight warps, two for each 32 rows, take
 // the last one's.  A wait that does not end makes the CTA give up: all that it has not finished is NaN, and it ends.
-template <int MODE, typename T, int BN>
+template <int MODE, typename T, int BN, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1) products_kernel(const __grid_constant__ Products p) {
-    constexpr int STAGES = kStages<BN>, HALF = BN / 2;
+    constexpr int STAGES = kStages<BN, PAIR>, HALF = BN / 2, CTAS = PAIR ? 2 : 1;
+    constexpr uint32_t STAGE = kStageBytes<BN, PAIR>;
     extern __shared__ uint8_t s_room[];
-    const uint32_t room = (shared_address(s_room) + 1023) & ~1023u, staging = room + STAGES * kStageBytes<BN>;
+    const uint32_t room = (shared_address(s_room) + 1023) & ~1023u, staging = room + STAGES * STAGE;
     float *s_bias = (float *)(s_room + (staging + kStagingBytes - shared_address(s_room)));
     volatile int *s_gave_up = (volatile int *)(s_bias + 256);
     const uint32_t s_tmem = shared_address(s_bias + 257), bars = shared_address(s_bias + 260);
@@ -189,50 +193,61 @@ __global__ void __launch_bounds__(kThreads, 1) products_kernel(const __grid_cons
         }
         for (int s = 0; s < 2; s++) {
             barrier_init(done + 8 * s, 1);
-            barrier_init(taken + 8 * s, 8);
+            barrier_init(taken + 8 * s, 8 * CTAS);
         }
         barrier_init(drained, 1);
         *s_gave_up = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 1) tmem_alloc(s_tmem, 2 * BN);
+    __syncwarp();
+    if (warp == 1) tmem_alloc<PAIR>(s_tmem, 2 * BN);
     tmem_before_sync();
+    if (PAIR) cluster_sync(); // (both CTAs' barriers are there)
     __syncthreads();
     tmem_after_sync();
     wait_for_previous();
     let_next_begin();
     const Head &h = p.head;
     const uint32_t tmem = *(volatile uint32_t *)(s_bias + 257);
-    const int rows = rows_counted(h);
+    const int rows = rows_counted(h), rank = blockIdx.x % CTAS, unit = blockIdx.x / CTAS;
+    const uint32_t first_full = PAIR ? there(full, 0) : full, first_taken = PAIR ? there(taken, 0) : taken;
+    auto copy = [&](uint32_t to, const CUtensorMap *map, int x, int y, uint32_t bar) {
+        if (PAIR)
+            copy_box_of_pair(to, map, x, y, bar);
+        else
+            copy_box(to, map, x, y, bar);
+    };
     Tile tile;
     if (warp == 0) {
         if (lane == 0) {
             uint32_t n = 0; // stages filled so far
             bool fine = true;
-            for (Walk<MODE> walk(p, rows); fine && walk.next(p, rows, tile);) {
+            for (Walk<MODE> walk(p, rows, unit); fine && walk.next(p, rows, tile);) {
                 const Product &w = p.of[tile.product];
                 for (int k = tile.from; k < tile.to; k++, n++) {
-                    const uint32_t s = n % STAGES, at = room + s * kStageBytes<BN>, bar = full + 8 * s;
+                    const uint32_t s = n % STAGES, at = room + s * STAGE, bar = first_full + 8 * s;
+                    const int row = tile.row * (128 * CTAS) + rank * 128, column = tile.column * BN + rank * (BN / CTAS); // of this CTA
                     fine = n < STAGES || barrier_wait(empty + 8 * s, (n / STAGES - 1) & 1, s_gave_up);
                     if (!fine) break;
-                    barrier_expect(bar, kStageBytes<BN>);
+                    if (rank == 0) barrier_expect(full + 8 * s, CTAS * STAGE);
                     if (MODE == kProducts) {
                         if (w.a_along_sum) {
-                            copy_box(at, &w.a, tile.row * 128, k * kSum, bar);
-                            copy_box(at + kRowsBytes / 2, &w.a, tile.row * 128 + 64, k * kSum, bar);
+                            copy(at, &w.a, row, k * kSum, bar);
+                            copy(at + kRowsBytes / 2, &w.a, row + 64, k * kSum, bar);
                         } else {
-                            copy_box(at, &w.a, k * kSum, tile.row * 128, bar);
+                            copy(at, &w.a, k * kSum, row, bar);
                         }
 #pragma unroll
-                        for (int j = 0; j < BN / 64; j++)
-                            copy_box(at + kRowsBytes + j * (kSum * 128), &w.b, tile.column * BN + 64 * j, w.b_first + k * kSum, bar);
+                        for (int j = 0; j < BN / CTAS / 64; j++) copy(at + kRowsBytes + j * (kSum * 128), &w.b, column + 64 * j, w.b_first + k * kSum, bar);
                     } else {
-                        copy_box(at, &w.a, k * kSum, tile.row * 128, bar);
-                        copy_box(at + kRowsBytes, &w.b, k * kSum, w.b_first + tile.column * BN, bar);
+                        copy(at, &w.a, k * kSum, row, bar);
+                        copy(at + kRowsBytes, &w.b, k * kSum, w.b_first + column, bar);
                     }
                 }
             }
-            if (!fine) // no copy arrives behind the CTA's end
+            if (PAIR && fine) // nor does the word that a stage is free, from the other CTA
+                for (uint32_t k = n < STAGES ? 0 : n - STAGES; k < n; k++) barrier_wait(empty + 8 * (k % STAGES), k / STAGES & 1, s_gave_up);
+            if (!fine && rank == 0) // no copy arrives behind the CTA's end (or the pair's)
                 for (uint32_t k = n < STAGES ? 0 : n - STAGES; k < n; k++) {
                     volatile int patient = 0;
                     barrier_wait(full + 8 * (k % STAGES), k / STAGES & 1, &patient);
@@ -240,33 +255,33 @@ __global__ void __launch_bounds__(kThreads, 1) products_kernel(const __grid_cons
         }
         __syncwarp();
     } else if (warp == 1) {
-        if (lane == 0) {
+        if (lane == 0 && rank == 0) {
             uint32_t n = 0, m = 0; // stages and tiles multiplied so far
             bool fine = true;
-            for (Walk<MODE> walk(p, rows); fine && walk.next(p, rows, tile);) {
+            for (Walk<MODE> walk(p, rows, unit); fine && walk.next(p, rows, tile);) {
                 const bool a_along_sum = MODE == kProducts && p.of[tile.product].a_along_sum;
-                const uint32_t kind = product_kind(sizeof(T) == 2 && kHeld<T> == 1.0f, BN, a_along_sum, MODE == kProducts), half = m & 1;
+                const uint32_t kind = product_kind(sizeof(T) == 2 && kHeld<T> == 1.0f, 128 * CTAS, BN, a_along_sum, MODE == kProducts), half = m & 1;
                 fine = m < 2 || barrier_wait(taken + 8 * half, (m / 2 - 1) & 1, s_gave_up);
                 if (!fine) break;
                 tmem_after_sync();
                 for (int k = tile.from; k < tile.to; k++, n++) {
-                    const uint32_t s = n % STAGES, at = room + s * kStageBytes<BN>;
+                    const uint32_t s = n % STAGES, at = room + s * STAGE;
                     fine = barrier_wait(full + 8 * s, n / STAGES & 1, s_gave_up);
                     if (!fine) break;
                     tmem_after_sync();
                     const uint64_t a = operand(at, kSum * 128), b = operand(at + kRowsBytes, kSum * 128);
 #pragma unroll
                     for (int i = 0; i < kSum / 16; i++) // 16 terms: 32 bytes along a box's rows, or 16 of them
-                        multiply(tmem + half * BN, a + i * (a_along_sum ? 128 : 2), b + i * (MODE == kProducts ? 128 : 2), kind, k > tile.from || i > 0);
-                    when_multiplied(empty + 8 * s);
+                        multiply<PAIR>(tmem + half * BN, a + i * (a_along_sum ? 128 : 2), b + i * (MODE == kProducts ? 128 : 2), kind, k > tile.from || i > 0);
+                    when_multiplied<PAIR>(empty + 8 * s);
                 }
                 if (!fine) break;
-                when_multiplied(done + 8 * half);
+                when_multiplied<PAIR>(done + 8 * half);
                 m++;
             }
             if (!fine) {
                 volatile int patient = 0;
-                when_multiplied(drained);
+                when_multiplied<PAIR>(drained);
                 barrier_wait(drained, 0, &patient);
             }
         }
@@ -277,10 +292,10 @@ __global__ void __launch_bounds__(kThreads, 1) products_kernel(const __grid_cons
         const uint32_t from = tmem + ((uint32_t)quarter << 21) + side * HALF;
         const float k_all = MODE == kProducts ? gradient_scale<T>(h) : 0.0f;
         uint32_t m = 0;
-        for (Walk<MODE> walk(p, rows); walk.next(p, rows, tile);) {
+        for (Walk<MODE> walk(p, rows, unit); walk.next(p, rows, tile);) {
             const Product &w = p.of[tile.product];
             const uint32_t half = m & 1, at = from + half * BN;
-            const int row = tile.row * 128 + quarter * 32 + lane, column = tile.column * BN + side * HALF; // (of the lane; the first)
+            const int row_tile = tile.row * CTAS + rank, row = row_tile * 128 + quarter * 32 + lane, column = tile.column * BN + side * HALF; // (of the lane; the first)
             if (MODE != kProducts) { // the columns' bias; classes that there are not have a logit of -inf
                 asm volatile("bar.sync 1, 256;" ::: "memory");
                 if (threadIdx.x - 64 < BN) {
@@ -296,7 +311,11 @@ __global__ void __launch_bounds__(kThreads, 1) products_kernel(const __grid_cons
             auto give_back = [&] { // behind the last load of the tile
                 tmem_before_sync();
                 __syncwarp();
-                if (lane == 0) barrier_arrive(taken + 8 * half);
+                if (lane != 0) return;
+                if (PAIR)
+                    barrier_arrive_there(first_taken + 8 * half);
+                else
+                    barrier_arrive(taken + 8 * half);
             };
             const float4 *bias4 = reinterpret_cast<const float4 *>(s_bias + side * HALF);
             if constexpr (MODE == kStatistics) {
@@ -399,7 +418,7 @@ __global__ void __launch_bounds__(kThreads, 1) products_kernel(const __grid_cons
                 const float times_it = part || (MODE == kProducts && w.leaves != kWritten) ? 1.0f : factor;
                 const Two minus(-row_top, -row_top), log2e(kLog2e, kLog2e), times(times_it, times_it), less(-flat, -flat);
                 // a part's place: the run's first, or its last
-                const int row0 = (part ? (2 * (int)blockIdx.x + (tile.from == 0)) * 128 : tile.row * 128) + quarter * 32;
+                const int row0 = (part ? 2 * (int)blockIdx.x + (tile.from == 0) : row_tile) * 128 + quarter * 32;
                 const int x0 = part ? side * HALF : column, x_last = part ? BN : MODE == kGradient ? h.columns : (int)h.a.width;
                 // 32 columns from c on
                 auto values = [&](Two(&v)[16], const uint32_t(&raw)[32], int c) {
@@ -496,7 +515,7 @@ __global__ void __launch_bounds__(kThreads, 1) products_kernel(const __grid_cons
                                 for (int i = 0; i < 4; i++) s[i] += __shfl_down_sync(0xffffffffu, s[i], 16);
                                 const int x = column + c + 4 * lane;
                                 if (lane < 16 && x < h.chunk)
-                                    *reinterpret_cast<float4 *>(h.bias_parts + (long long)(tile.row * 4 + quarter) * h.chunk + x) = make_float4(s[0], s[1], s[2], s[3]);
+                                    *reinterpret_cast<float4 *>(h.bias_parts + (long long)(row_tile * 4 + quarter) * h.chunk + x) = make_float4(s[0], s[1], s[2], s[3]);
                             }
                         }
                     }
@@ -519,11 +538,13 @@ __global__ void __launch_bounds__(kThreads, 1) products_kernel(const __grid_cons
             }
         }
         if (MODE != kStatistics && lane == 0) boxes_written();
+        __syncwarp();
     }
     tmem_before_sync();
     __syncthreads();
+    if (PAIR) cluster_sync(); // (nothing of the other CTA's arrives here any more)
     tmem_after_sync();
-    if (warp == 1) tmem_free(tmem, 2 * BN);
+    if (warp == 1) tmem_free<PAIR>(tmem, 2 * BN);
 }
 
 // Rows' statistics joined over the classes: 32 rows per CTA, whose 32 warps each take every 32nd part.
@@ -725,7 +746,7 @@ __global__ void __launch_bounds__(256) settle_kernel(const __grid_constant__ Hea
 }
 
 // What is left to do behind a chunk's products: tiles that several CTAs have parts of, added up in their order; and the bias' gradient.  The first CTAs have
-// a quarter each of the tile that a run begins in the middle of (the first such run of a tile); of the others each has 32 classes, whose sums over 32 rows it
+// 32 rows each of the tile that a run begins in the middle of (the first such run of a tile); of the others each has 32 classes, whose sums over 32 rows it
 // adds up.
 template <typename T, int BN>
 __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Products p) {
@@ -733,7 +754,7 @@ __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Pro
     wait_for_previous();
     let_next_begin();
     const Head &h = p.head;
-    const int rows = rows_counted(h), tiles = p.count ? p.ctas * 4 : 0;
+    const int rows = rows_counted(h), pieces = p.high / 32, tiles = p.count ? p.units * pieces : 0;
     if ((int)blockIdx.x >= tiles) {
         const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = ((int)blockIdx.x - tiles) * 32 + lane, parts = (rows + 127) / 128 * 4;
         float sum = 0.0f;
@@ -749,21 +770,22 @@ __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Pro
         return;
     }
     const Runs runs(p, rows);
-    const int cta = (int)blockIdx.x / 4, quarter = blockIdx.x & 3, place = runs.place(cta), lane = runs.lane(cta);
-    if (place == 0 || place >= runs.ctas) return;
+    const int unit = (int)blockIdx.x / pieces, piece = (int)blockIdx.x - unit * pieces, place = runs.place(unit), lane = runs.lane(unit);
+    if (place == 0 || place >= runs.units) return;
     const int begin = runs.begin(place);
     const Tile tile = tile_of(p, runs, lane, begin, rows);
     if (tile.from == 0 || begin - runs.begin(place - 1) < tile.from) return; // (a run's own tile; one that an earlier run has begun in the middle of)
     int last = place; // the last run with a part
-    while (last + 1 < runs.ctas && runs.begin(last + 1) - begin < tile.to - tile.from) last++;
+    while (last + 1 < runs.units && runs.begin(last + 1) - begin < tile.to - tile.from) last++;
     const Product &w = p.of[tile.product];
     const float k = w.leaves == kWritten ? gradient_scale<T>(h) : 1.0f;
     const bool blank = w.counted == kSumCounted && rows == 0;
     for (int i = threadIdx.x; i < 32 * BN / 8; i += 256) {
-        const int r = quarter * 32 + i / (BN / 8), c = i % (BN / 8) * 8, row = tile.row * 128 + r, column = tile.column * BN + c;
+        const int r = piece % 4 * 32 + i / (BN / 8), c = i % (BN / 8) * 8, row = tile.row * p.high + piece * 32 + i / (BN / 8), column = tile.column * BN + c;
         if (row >= w.c_last || column >= h.a.width) continue;
         float v[8];
-        auto take = [&](int part, bool first) {
+        auto take = [&](int unit, int end, bool first) { // (of a pair's CTA)
+            const int part = 2 * (unit * (p.high / 128) + piece / 4) + end;
             const float *at = p.parts + ((long long)part * 128 + r) * BN + c;
 #pragma unroll
             for (int j = 0; j < 8; j += 4) {
@@ -774,9 +796,9 @@ __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Pro
                 v[j + 3] = first ? f.w : v[j + 3] + f.w;
             }
         };
-        take(2 * (cta - runs.lanes) + 1, true);
+        take(unit - runs.lanes, 1, true);
 #pragma unroll 4
-        for (int other = place; other <= last; other++) take(2 * (cta + (other - place) * runs.lanes), false);
+        for (int other = place; other <= last; other++) take(unit + (other - place) * runs.lanes, 0, false);
 #pragma unroll
         for (int j = 0; j < 8; j++) v[j] = blank ? 0.0f : v[j] * k;
         if (w.leaves == kWritten) {
@@ -801,7 +823,7 @@ struct Plan {
     bool counted, lay_hidden, lay_weight, grads, hidden_grad, weight_grad, bias_grad;
     int stat_columns, sum_columns;               // BN
     bool hidden_direct, weight_direct;           // products leave as they are to be
-    int ctas;
+    bool pairs;                                  // of CTAs
     int64_t map, place, count, most, hidden, weight, parts, apart, grad, hidden_sums, hidden_rows, weight_sums, bias_parts, tile_parts, bytes;
 };
 
@@ -812,20 +834,19 @@ bool aligned(const void *p, int64_t stride) { return (reinterpret_cast<uintptr_t
 
 Plan plan_of(const ffcvb_linear_cross_entropy_args &a) {
     Plan p{};
-    p.rows_pad = up(a.rows, 128);
+    p.pairs = a.rows > 128;
+    p.rows_pad = up(a.rows, p.pairs ? 256 : 128);
     p.width_pad = up(a.width, 8);
     p.counted = a.has_ignore && a.target_kind == FFCVB_TARGET_LABELS;
     p.lay_hidden = p.counted || !aligned(a.hidden, a.hidden_stride);
     p.lay_weight = !aligned(a.weight, a.weight_stride);
     p.hidden_grad = a.grad_hidden, p.weight_grad = a.grad_weight, p.bias_grad = a.grad_bias;
     p.grads = p.hidden_grad || p.weight_grad || p.bias_grad;
-    const int64_t row_tiles = p.rows_pad / 128;
-    p.stat_columns = row_tiles * ((a.classes + 255) / 256) < kSms ? 128 : 256;
+    p.stat_columns = p.pairs || (a.classes + 255) / 256 >= kSms ? 256 : 128;
     p.chunks = (a.classes * p.rows_pad * 2 + kMostGradient - 1) / kMostGradient;
     p.chunk = up((a.classes + p.chunks - 1) / p.chunks, 256);
     p.chunks = (a.classes + p.chunk - 1) / p.chunk;
-    p.sum_columns = a.width <= 128 ? 128 : 256;
-    p.ctas = kSms;
+    p.sum_columns = p.pairs || a.width > 128 ? 256 : 128;
     p.hidden_direct = p.chunks == 1 && (p.counted || a.width % 8 == 0);
     p.weight_direct = a.width % 8 == 0;
     int64_t at = 0;
@@ -848,7 +869,7 @@ Plan plan_of(const ffcvb_linear_cross_entropy_args &a) {
     p.hidden_sums = take(p.hidden_grad && !p.hidden_direct, p.rows_pad * wide * 4);
     p.hidden_rows = take(p.hidden_grad && p.hidden_direct && p.counted, p.rows_pad * p.width_pad * 2);
     p.weight_sums = take(p.weight_grad && !p.weight_direct, p.chunk * wide * 4);
-    p.tile_parts = take(p.hidden_grad || p.weight_grad, 2ll * p.ctas * 128 * p.sum_columns * 4);
+    p.tile_parts = take(p.hidden_grad || p.weight_grad, 2ll * kSms * 128 * p.sum_columns * 4);
     p.bias_parts = take(p.bias_grad, p.rows_pad / 32 * p.chunk * 4);
     p.bytes = at;
     return p;
@@ -866,21 +887,39 @@ const char *wrong(const ffcvb_linear_cross_entropy_args &a) {
     return nullptr;
 }
 
-template <int MODE, typename T, int BN> bool launch_products(const Products &p, int64_t tiles, cudaStream_t stream) {
-    auto *kernel = products_kernel<MODE, T, BN>;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kRoom<BN>) != cudaSuccess) return false;
-    return launch_early(kernel, (unsigned)std::min<int64_t>(tiles, kSms), kThreads, kRoom<BN>, stream, p) == cudaSuccess;
+template <int MODE, typename T, int BN, bool PAIR> bool launch_products(Products &p, int64_t tiles, cudaStream_t stream) {
+    auto *kernel = products_kernel<MODE, T, BN, PAIR>;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kRoom<BN, PAIR>) != cudaSuccess) return false;
+    constexpr int CTAS = PAIR ? 2 : 1;
+    p.units = (int)std::min<int64_t>(tiles, kSms / CTAS);
+    cudaLaunchConfig_t how{};
+    cudaLaunchAttribute with[2] = {};
+    with[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    with[0].val.programmaticStreamSerializationAllowed = 1;
+    with[1].id = cudaLaunchAttributeClusterDimension;
+    with[1].val.clusterDim.x = CTAS;
+    with[1].val.clusterDim.y = with[1].val.clusterDim.z = 1;
+    how.gridDim = dim3((unsigned)(p.units * CTAS));
+    how.blockDim = dim3(kThreads);
+    how.dynamicSmemBytes = kRoom<BN, PAIR>;
+    how.stream = stream;
+    how.attrs = with;
+    how.numAttrs = PAIR ? 2 : 1;
+    return cudaLaunchKernelEx(&how, kernel, p) == cudaSuccess;
 }
-template <int MODE, typename T> bool launch_products(int columns, const Products &p, int64_t tiles, cudaStream_t stream) {
-    return columns == 256 ? launch_products<MODE, T, 256>(p, tiles, stream) : launch_products<MODE, T, 128>(p, tiles, stream);
+template <int MODE, typename T> bool launch_products(int columns, bool pairs, Products &p, int64_t tiles, cudaStream_t stream) {
+    if (pairs) return launch_products<MODE, T, 256, true>(p, tiles, stream);
+    return columns == 256 ? launch_products<MODE, T, 256, false>(p, tiles, stream) : launch_products<MODE, T, 128, false>(p, tiles, stream);
 }
 
 template <typename T> int run(const ffcvb_linear_cross_entropy_args &a, uint8_t *room, cudaStream_t st) {
     const Plan p = plan_of(a);
     const int type = a.type;
-    const int64_t row_tiles = p.rows_pad / 128;
+    const int high = p.pairs ? 256 : 128;
+    const int64_t row_tiles = p.rows_pad / high;
     auto at = [&](int64_t offset) { return static_cast<void *>(room + offset); };
     Products g{};
+    g.high = high;
     Head &h = g.head;
     h.a = a;
     h.rows_pad = (int)p.rows_pad;
@@ -930,7 +969,7 @@ template <typename T> int run(const ffcvb_linear_cross_entropy_args &a, uint8_t 
     auto logits = [&](int columns, int64_t first, int64_t count) {
         Product &w = g.of[0];
         mapped &= matrix_map(&w.a, type, hidden, hidden_rows, a.width, hidden_stride, 128);
-        mapped &= matrix_map(&w.b, type, weight, a.classes, a.width, weight_stride, columns);
+        mapped &= matrix_map(&w.b, type, weight, a.classes, a.width, weight_stride, p.pairs ? columns / 2 : columns);
         w.row_tiles = (int)row_tiles;
         w.column_tiles = (int)((count + columns - 1) / columns);
         w.sum_blocks = sum_blocks;
@@ -946,7 +985,7 @@ template <typename T> int run(const ffcvb_linear_cross_entropy_args &a, uint8_t 
         const int64_t tiles = logits(p.stat_columns, 0, a.classes);
         if (!mapped) return training_fail(FFCVB_E_CUDA, "ffcvb_linear_cross_entropy: no map of a matrix");
         g.of[0].b_first = 0;
-        fine &= launch_products<kStatistics, T>(p.stat_columns, g, tiles, st);
+        fine &= launch_products<kStatistics, T>(p.stat_columns, p.pairs, g, tiles, st);
         launch_early(join_kernel, (unsigned)(p.rows_pad / 32), 1024, 0, st, h);
         if (a.loss) launch_mean(a.row_loss, a.rows, h.counted, a.mean, a.loss, st);
     }
@@ -956,17 +995,16 @@ template <typename T> int run(const ffcvb_linear_cross_entropy_args &a, uint8_t 
     auto ctas_for = [&](int64_t rows) { return (unsigned)std::min<int64_t>((rows * ((a.width + 7) / 8) + 255) / 256, kSms * 8); };
     for (int64_t chunk = 0; chunk < p.chunks; chunk++) {
         const int64_t first = chunk * p.chunk, count = std::min(p.chunk, a.classes - first);
-        const int columns = row_tiles * ((count + 255) / 256) < kSms ? 128 : 256;
+        const int columns = p.pairs || (count + 255) / 256 >= kSms ? 256 : 128;
         int64_t tiles = logits(columns, first, count);
         mapped &= matrix_map(&g.of[0].c, type, at(p.grad), p.counted ? p.rows_pad : a.rows, count, p.chunk, 32);
         g.of[0].c_last = (int)(p.counted ? p.rows_pad : a.rows);
         h.bias_parts = p.bias_grad ? static_cast<float *>(at(p.bias_parts)) : nullptr;
         h.chunk = (int)p.chunk;
         if (!mapped) break;
-        fine &= launch_products<kGradient, T>(columns, g, tiles, st);
+        fine &= launch_products<kGradient, T>(columns, p.pairs, g, tiles, st);
         const int column_tiles = (int)((a.width + p.sum_columns - 1) / p.sum_columns);
         g.count = 0;
-        g.ctas = p.ctas;
         g.lanes = column_tiles <= 16 ? column_tiles : 1; // (few CTAs are left without one)
         // C: in what it is to be, in rows that count, or in 32 bits
         auto leaves_as = [&](Product &w, int how, void *out, int64_t rows, int64_t stride) {
@@ -1001,7 +1039,7 @@ template <typename T> int run(const ffcvb_linear_cross_entropy_args &a, uint8_t 
                 leaves_as(w, kWritten, static_cast<T *>(a.grad_weight) + first * a.width, count, a.width);
             else
                 leaves_as(w, kWritten32, at(p.weight_sums), p.chunk, wide);
-            w.row_tiles = (int)((count + 127) / 128);
+            w.row_tiles = (int)((count + high - 1) / high);
             w.sum_blocks = (int)((a.rows + kSum - 1) / kSum);
             w.a_along_sum = 1;
             w.counted = p.counted ? kSumCounted : kFixed;
@@ -1009,11 +1047,11 @@ template <typename T> int run(const ffcvb_linear_cross_entropy_args &a, uint8_t 
         }
         if (g.count) {
             g.parts = static_cast<float *>(at(p.tile_parts));
-            mapped &= matrix_map(&g.part, FFCVB_TYPE_F32, at(p.tile_parts), 2 * p.ctas * 128, p.sum_columns, p.sum_columns, 32);
+            mapped &= matrix_map(&g.part, FFCVB_TYPE_F32, at(p.tile_parts), 2 * kSms * 128, p.sum_columns, p.sum_columns, 32);
         }
         if (!mapped) break;
-        if (g.count) fine &= launch_products<kProducts, T>(p.sum_columns, g, p.ctas, st);
-        const unsigned finish = (unsigned)((g.count ? p.ctas * 4 : 0) + (p.bias_grad ? (count + 31) / 32 : 0));
+        if (g.count) fine &= launch_products<kProducts, T>(p.sum_columns, p.pairs, g, kSms, st);
+        const unsigned finish = (unsigned)((g.count ? g.units * (high / 32) : 0) + (p.bias_grad ? (count + 31) / 32 : 0));
         if (finish) launch_early(p.sum_columns == 256 ? finish_kernel<T, 256> : finish_kernel<T, 128>, finish, 256, 0, st, g);
         if (p.weight_grad && !p.weight_direct)
             launch_early(settle_kernel<T, float>, ctas_for(count), 256, 0, st, h, static_cast<const float *>(at(p.weight_sums)), (int)wide, (const int *)nullptr,

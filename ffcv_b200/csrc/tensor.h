@@ -23,6 +23,14 @@ __device__ __forceinline__ uint64_t nanoseconds() {
 
 __device__ __forceinline__ void barrier_init(uint32_t bar, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory"); }
 __device__ __forceinline__ void barrier_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+// The same place in the shared memory of the cluster's CTA `rank`.
+__device__ __forceinline__ uint32_t there(uint32_t at, uint32_t rank) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(at), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void barrier_arrive_there(uint32_t bar) { asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ void barrier_expect(uint32_t bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
@@ -56,6 +64,12 @@ __device__ __forceinline__ void copy_box(uint32_t to, const CUtensorMap *map, in
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(to), "l"(map), "r"(x), "r"(y), "r"(bar)
                  : "memory");
 }
+// By one of a pair of CTAs, whose barrier is the first one's.
+__device__ __forceinline__ void copy_box_of_pair(uint32_t to, const CUtensorMap *map, int x, int y, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], [%4];" ::"r"(to), "l"(map), "r"(x), "r"(y),
+                 "r"(bar)
+                 : "memory");
+}
 __device__ __forceinline__ void store_box(const CUtensorMap *map, int x, int y, uint32_t from) {
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x), "r"(y), "r"(from) : "memory");
 }
@@ -67,11 +81,21 @@ __device__ __forceinline__ void boxes_read() { asm volatile("cp.async.bulk.wait_
 __device__ __forceinline__ void boxes_written() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 __device__ __forceinline__ void shared_to_copies() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-__device__ __forceinline__ void tmem_alloc(uint32_t to, uint32_t columns) {
+// (PAIR, here and below: of both CTAs of a pair, each of which calls these.)
+template <bool PAIR> __device__ __forceinline__ void tmem_alloc(uint32_t to, uint32_t columns) {
+    if constexpr (PAIR) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(to), "r"(columns) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        return;
+    }
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(to), "r"(columns) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void tmem_free(uint32_t at, uint32_t columns) {
+template <bool PAIR> __device__ __forceinline__ void tmem_free(uint32_t at, uint32_t columns) {
+    if constexpr (PAIR) {
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(at), "r"(columns) : "memory");
+        return;
+    }
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(at), "r"(columns) : "memory");
 }
 __device__ __forceinline__ void tmem_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -83,17 +107,28 @@ __device__ __forceinline__ uint64_t operand(uint32_t at, uint32_t across) {
     constexpr uint64_t kEight = 1024 >> 4; // from eight of a box's rows to the next
     return (uint64_t)(at >> 4) | (uint64_t)(across >> 4) << 16 | kEight << 32 | 1ull << 46 | 2ull << 61;
 }
-// The instruction's sizes and types: products of 16 bits, sums of 32; 128 rows.
-__device__ __forceinline__ uint32_t product_kind(bool bf16, int columns, bool a_along_sum, bool b_along_sum) {
-    return 1u << 4 | (bf16 ? 1u << 7 | 1u << 10 : 0u) | (a_along_sum ? 1u << 15 : 0u) | (b_along_sum ? 1u << 16 : 0u) | (uint32_t)(columns >> 3) << 17 | (128u >> 4) << 24;
+// The instruction's sizes and types: products of 16 bits, sums of 32; 128 rows, or a pair's 256.
+__device__ __forceinline__ uint32_t product_kind(bool bf16, int rows, int columns, bool a_along_sum, bool b_along_sum) {
+    return 1u << 4 | (bf16 ? 1u << 7 | 1u << 10 : 0u) | (a_along_sum ? 1u << 15 : 0u) | (b_along_sum ? 1u << 16 : 0u) | (uint32_t)(columns >> 3) << 17 | (uint32_t)(rows >> 4) << 24;
 }
-__device__ __forceinline__ void multiply(uint32_t tmem, uint64_t a, uint64_t b, uint32_t kind, bool add) {
+// One thread multiplies; a pair's first CTA does it for both, which have 128 rows of A and half of B's columns each, in the same places, and get their rows' sums.
+template <bool PAIR> __device__ __forceinline__ void multiply(uint32_t tmem, uint64_t a, uint64_t b, uint32_t kind, bool add) {
+    if constexpr (PAIR) {
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem), "l"(a), "l"(b), "r"(kind),
+                     "r"((uint32_t)add)
+                     : "memory");
+        return;
+    }
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem), "l"(a), "l"(b), "r"(kind),
                  "r"((uint32_t)add)
                  : "memory");
 }
-// The barrier is arrived at once all multiplications issued so far are done.
-__device__ __forceinline__ void when_multiplied(uint32_t bar) {
+// The barrier is arrived at once all multiplications issued so far are done: a pair's, in both CTAs.
+template <bool PAIR> __device__ __forceinline__ void when_multiplied(uint32_t bar) {
+    if constexpr (PAIR) {
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
+        return;
+    }
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 
