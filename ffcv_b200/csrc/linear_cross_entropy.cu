@@ -67,9 +67,9 @@ struct Products {
     Head head;
 };
 
-// G is held times this: in fp16 shares of less than 2^-24 of a row would be lost.
+// G, whose values are at most 1 with targets that are shares, is held times this: in fp16 those of less than 2^-24 would be lost.
 template <typename T> constexpr float kHeld = 1.0f;
-template <> constexpr float kHeld<__half> = 32768.0f;
+template <> constexpr float kHeld<__half> = 16384.0f;
 
 template <typename T> __device__ __forceinline__ uint32_t two_of(float lo, float hi);
 template <> __device__ __forceinline__ uint32_t two_of<__half>(float lo, float hi) {
@@ -884,6 +884,7 @@ const char *wrong(const ffcvb_linear_cross_entropy_args &a) {
     if (a.rows > 0 && (!a.hidden || !a.weight || !a.target || !a.stats || (!a.from_stats && !a.row_loss))) return "an address is missing";
     if (a.from_stats && !a.grad_hidden && !a.grad_weight && !a.grad_bias) return "nothing to do";
     if (a.grad_bias && !a.bias) return "no bias";
+    if (((reinterpret_cast<uintptr_t>(a.grad_hidden) | reinterpret_cast<uintptr_t>(a.grad_weight) | reinterpret_cast<uintptr_t>(a.stats)) & 15) != 0) return "gradients and stats begin on 16 bytes";
     return nullptr;
 }
 

@@ -42,8 +42,8 @@ def _last(t):
 
 def _new(t):
     """Room for a dense result of a tensor's shape, channels last."""
-    if t.dim() == 4:
-        return ch.empty(t.shape, dtype=t.dtype, device=t.device, memory_format=ch.channels_last)
+    if t.dim() == 4 and t.is_contiguous(memory_format=ch.channels_last):
+        return ch.empty_like(t)
     samples, channels, *sides = t.shape
     return ch.empty((samples, *sides, channels), dtype=t.dtype, device=t.device).movedim(-1, 1)
 
@@ -115,7 +115,7 @@ class _Call:
             raise ValueError('stats must be what the forward pass of the same call gave')
         dy, dy_strides = self.laid(dy)
         dx = _new(x) if wanted[0] else None
-        dweight, dbias = (ch.empty(x.shape[1], dtype=self.param_dtype, device=x.device) if w else None for w in wanted[1:])
+        dweight, dbias = (ch.empty_like(p) if w else None for p, w in zip((self.weight, self.bias), wanted[1:]))
         if dx is not None or dweight is not None or dbias is not None:
             args = self.pack(stats, None, dy, dx, dweight, dbias, dy_strides)
             workspace = self.room(args, 1)

@@ -149,7 +149,11 @@ class _LinearCrossEntropy(ch.autograd.Function):
 
 def linear_cross_entropy(hidden, weight, labels=None, *, mixed=None, bias=None, label_smoothing=0.0, ignore_index=None, reduction='mean'):
     """The loss as a function of hidden values, weights and bias that autograd knows; see :func:`linear_cross_entropy_with_grad`
-    for the arguments.  The gradients are made in the backward pass, where a loss scale is known."""
+    for the arguments.  The gradients are made in the backward pass, where a loss scale is known.  Under autocast hidden values, weights and
+    bias are taken in its type, as a linear layer takes them."""
+    if ch.is_autocast_enabled('cuda'):
+        dtype = ch.get_autocast_dtype('cuda')
+        hidden, weight, bias = (t.to(dtype) if isinstance(t, ch.Tensor) and t.is_cuda and t.dtype in N.TYPES else t for t in (hidden, weight, bias))
     call = _Call(hidden, weight, labels, mixed, bias, label_smoothing, ignore_index, reduction)
     return _LinearCrossEntropy.apply(call.hidden, call.weight, call.bias, call, reduction)
 
