@@ -2,11 +2,17 @@
 
     python examples/train_image_transformer.py                       # on synthetic images, a minute on one GPU
     python examples/train_image_transformer.py --data train.beton --classes 1000 --width 384 --layers 12
+    python examples/train_image_transformer.py --stem convolutions --head whole     # for label sets of many classes
+    python examples/train_image_transformer.py --teacher 5                          # from a teacher's best logits
 
 The loader decodes, crops, flips and mixes the images on the GPU and hands the mixed labels over as [label, partner's
 label, lambda] rows, which the loss reads as they are.  The resolution grows from epoch to epoch; patches have rotary
 positions by row and column, which do not depend on it.  Every residual join is one kernel with the norm before the
 next block; AdamW keeps 32-bit masters of the bfloat16 weights and moments in 8 bits.
+
+With ``--stem convolutions`` patches are made by convolutions with group norms between them; with ``--head whole`` the
+last layer makes its loss itself, without logits in memory; with ``--teacher K`` every sample of the synthetic set has the
+K best logits of a teacher stored beside its label, which the loss is taken against too (images are not mixed then).
 """
 import argparse
 import json
@@ -42,23 +48,45 @@ class Colours:
         return np.clip(rng.normal(colour, 30, (h, w, 3)), 0, 255).astype(np.uint8), label
 
 
-def write(path, count, classes):
+class Taught(Colours):
+    """The same, with what a teacher thinks of each image: its best logits, of 16 bits, and their classes."""
+
+    def __init__(self, count, classes, kept):
+        super().__init__(count, classes)
+        self.kept = kept
+
+    def __getitem__(self, k):
+        image, label = super().__getitem__(k)
+        logits = np.random.default_rng([9, k]).normal(0, 1, self.classes)
+        logits[label] += 5
+        best = np.argsort(-logits)[:self.kept]
+        return image, label, logits[best].astype(np.float16), best.astype(np.int32)
+
+
+def write(path, count, classes, kept=0):
     from ffcv_b200 import DatasetWriter
-    from ffcv_b200.fields import IntField, RGBImageField
-    DatasetWriter(path, {'image': RGBImageField(write_mode='jpg', jpeg_quality=90), 'label': IntField()},
-                  num_workers=1).from_indexed_dataset(Colours(count, classes))
+    from ffcv_b200.fields import IntField, NDArrayField, RGBImageField
+    fields = {'image': RGBImageField(write_mode='jpg', jpeg_quality=90), 'label': IntField()}
+    if kept:
+        fields.update(best=NDArrayField(np.dtype('float16'), (kept,)), where=NDArrayField(np.dtype('int32'), (kept,)))
+    DatasetWriter(path, fields, num_workers=1).from_indexed_dataset(Taught(count, classes, kept) if kept else Colours(count, classes))
 
 
-def loader_of(path, batch, side, mixup, seed):
+def loader_of(path, batch, side, mixup, seed, teacher=0):
     from ffcv_b200 import Loader, OrderOption
-    from ffcv_b200.fields.decoders import IntDecoder, RandomResizedCropRGBImageDecoder
-    from ffcv_b200.transforms import (ImageMixup, LabelMixup, NormalizeImage, RandomHorizontalFlip, ToDevice, ToTensor,
-                                      ToTorchImage)
+    from ffcv_b200.fields.decoders import IntDecoder, NDArrayDecoder, RandomResizedCropRGBImageDecoder
+    from ffcv_b200.transforms import (ImageMixup, LabelMixup, NormalizeImage, RandomHorizontalFlip, Squeeze, ToDevice,
+                                      ToTensor, ToTorchImage)
     device = torch.device('cuda', torch.cuda.current_device())
     image = [RandomResizedCropRGBImageDecoder((side, side)), RandomHorizontalFlip(), ImageMixup(mixup, False), ToTensor(),
              ToDevice(device), ToTorchImage(), NormalizeImage(MEAN, STD, np.float16)]
     label = [IntDecoder(), LabelMixup(mixup, False), ToTensor(), ToDevice(device)]
-    return Loader(path, batch_size=batch, order=OrderOption.RANDOM, seed=seed, pipelines={'image': image, 'label': label})
+    pipelines = {'image': image, 'label': label}
+    if teacher:  # its logits are those of one image: nothing is mixed
+        pipelines['image'] = [op for op in image if not isinstance(op, ImageMixup)]
+        pipelines['label'] = [IntDecoder(), ToTensor(), ToDevice(device), Squeeze()]
+        pipelines.update({name: [NDArrayDecoder(), ToTensor(), ToDevice(device)] for name in ('best', 'where')})
+    return Loader(path, batch_size=batch, order=OrderOption.RANDOM, seed=seed, pipelines=pipelines)
 
 
 class Block(nn.Module):
@@ -82,26 +110,52 @@ class Block(nn.Module):
         return self.join_perceptron(stream, self.down(F.gelu(self.up(normed))))
 
 
-class ImageTransformer(nn.Module):
-    def __init__(self, classes, patch, width, layers, heads):
-        from ffcv_b200.training import NormResidual, RotaryPositions
+class Stem(nn.Module):
+    """Patches by convolutions that halve the sides, each but the last with a group norm and an activation behind it; all channels last, as the
+    loader's images are."""
+
+    def __init__(self, patch, width):
+        from ffcv_b200.training import GroupNormAct
         super().__init__()
-        self.patch, self.embed = patch, nn.Linear(3 * patch * patch, width)
+        channels, layers = 3, []
+        while patch > 2:
+            more = 32 if channels == 3 else min(2 * channels, 256)
+            layers += [nn.Conv2d(channels, more, 3, 2, 1), GroupNormAct(8, more, 'silu')]
+            channels, patch = more, patch // 2
+        self.layers = nn.Sequential(*layers, nn.Conv2d(channels, width, patch, patch)).to(memory_format=torch.channels_last)
+
+    def forward(self, images):
+        return self.layers(images.contiguous(memory_format=torch.channels_last)).flatten(2).transpose(1, 2)
+
+
+class ImageTransformer(nn.Module):
+    def __init__(self, classes, patch, width, layers, heads, stem='patches', head='logits'):
+        from ffcv_b200.training import LinearCrossEntropy, NormResidual, RotaryPositions
+        super().__init__()
+        self.patch, self.embed = patch, Stem(patch, width) if stem == 'convolutions' else nn.Linear(3 * patch * patch, width)
         self.first = NormResidual(width)
         rotary = RotaryPositions(width // heads, axes=2)
         self.blocks = nn.ModuleList([Block(width, heads, rotary) for _ in range(layers)])
-        self.head = nn.Linear(width, classes)
+        self.head = LinearCrossEntropy(width, classes, label_smoothing=0.1) if head == 'whole' else nn.Linear(width, classes)
 
-    def forward(self, images):
+    def hidden(self, images):
         from ffcv_b200.training import patch_positions
         batch, channels, height, width = images.shape
         rows, cols = height // self.patch, width // self.patch
-        patches = images.reshape(batch, channels, rows, self.patch, cols, self.patch).permute(0, 2, 4, 1, 3, 5)
-        stream, normed = self.first(self.embed(patches.reshape(batch, rows * cols, -1)))
+        if isinstance(self.embed, Stem):
+            embedded = self.embed(images)
+        else:
+            patches = images.reshape(batch, channels, rows, self.patch, cols, self.patch).permute(0, 2, 4, 1, 3, 5)
+            embedded = self.embed(patches.reshape(batch, rows * cols, -1))
+        stream, normed = self.first(embedded)
         positions = patch_positions(rows, cols, images.device)
         for block in self.blocks:
             stream, normed = block(stream, normed, positions)
-        return self.head(normed.mean(1))
+        return normed.mean(1)
+
+    def forward(self, images):
+        hidden = self.hidden(images)
+        return self.head(hidden) if isinstance(self.head, nn.Linear) else self.head.logits(hidden)
 
 
 def main():
@@ -119,29 +173,40 @@ def main():
     ap.add_argument('--lr', type=float, default=1e-3)
     ap.add_argument('--mixup', type=float, default=0.2)
     ap.add_argument('--state-bits', type=int, default=8, choices=(8, 32))
+    ap.add_argument('--stem', default='patches', choices=('patches', 'convolutions'))
+    ap.add_argument('--head', default='logits', choices=('logits', 'whole'), help='whole: the last layer and its loss in one')
+    ap.add_argument('--teacher', type=int, default=0, metavar='K', help="best logits of a teacher that every sample has (fields best and where)")
     a = ap.parse_args()
+    if a.teacher and a.head == 'whole':
+        ap.error('--teacher needs logits')
 
     own = None
     if a.data is None:  # (before the process touches the GPU: the writer forks)
         own = tempfile.TemporaryDirectory(dir='/dev/shm' if os.path.isdir('/dev/shm') else None)
         a.data = os.path.join(own.name, 'colours.beton')
-        write(a.data, a.count, a.classes)
+        write(a.data, a.count, a.classes, a.teacher)
 
-    from ffcv_b200.training import AdamW, MixupCrossEntropy
+    from ffcv_b200.training import AdamW, Distillation, MixupCrossEntropy
     torch.manual_seed(0)
-    model = ImageTransformer(a.classes, a.patch, a.width, a.layers, a.heads).cuda().bfloat16()
+    model = ImageTransformer(a.classes, a.patch, a.width, a.layers, a.heads, a.stem, a.head).cuda().bfloat16()
     matrices = [p for p in model.parameters() if p.dim() > 1]
     vectors = [p for p in model.parameters() if p.dim() <= 1]
     opt = AdamW([dict(params=matrices), dict(params=vectors, weight_decay=0.0)], lr=a.lr, weight_decay=0.05,
                 state_bits=a.state_bits, max_grad_norm=1.0)
-    loss_of = MixupCrossEntropy(label_smoothing=0.1)
+    loss_of, taught = MixupCrossEntropy(label_smoothing=0.1), Distillation(temperature=2.0, hard_weight=0.5, label_smoothing=0.1)
     means = []
     for epoch in range(a.epochs):
         share = epoch / max(1, a.epochs - 1)
         side = int(round((a.sides[0] + share * (a.sides[1] - a.sides[0])) / a.patch)) * a.patch
         losses = []
-        for images, labels in loader_of(a.data, a.batch, side, a.mixup, epoch):
-            loss = loss_of(model(images.bfloat16()), labels)
+        for images, labels, *teacher in loader_of(a.data, a.batch, side, a.mixup, epoch, a.teacher):
+            images = images.bfloat16()
+            if a.teacher:
+                loss = taught(model(images), *teacher, labels)
+            elif a.head == 'whole':
+                loss = model.head(model.hidden(images), labels)
+            else:
+                loss = loss_of(model(images), labels)
             opt.zero_grad()
             loss.backward()
             opt.step()

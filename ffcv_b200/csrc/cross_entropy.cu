@@ -366,6 +366,7 @@ mean_kernel(const float *__restrict__ row_loss, long long rows, const float *cou
     __shared__ double s_sum[32];
     wait_for_previous();
     double sum = 0.0;
+#pragma unroll 8
     for (long long i = threadIdx.x; i < rows; i += 1024) sum += row_loss[i];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);

@@ -41,7 +41,7 @@ struct Sums {
         seen += o.seen;
     }
     // joins those of groups of LANES lanes
-    template <int LANES, bool HARD> __device__ __forceinline__ void join_lanes(float rate, bool spread) {
+    template <int LANES, int HARD> __device__ __forceinline__ void join_lanes(float rate, bool spread) {
         float most = top;
 #pragma unroll
         for (int o = LANES / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
@@ -98,9 +98,23 @@ struct Deal {
     int wide, part;
 };
 
+// The loss against labels: none; with exponentials of its own; or with those at the temperature, to the power of 1, 2 or 4, which the temperature then is (two instead of
+// four exponentials for a logit).
+enum { kNoHard, kOwn, kFirst, kSecond, kFourth };
+template <int HARD> __device__ __forceinline__ float hard_exp(float d, float soft) {
+    return HARD == kFirst ? soft : HARD == kSecond ? soft * soft : HARD == kFourth ? (soft * soft) * (soft * soft) : exp_of(d);
+}
+template <int HARD> __device__ __forceinline__ Two hard_exp(Two d, Two soft) {
+    if constexpr (HARD == kFirst) return soft;
+    if constexpr (HARD == kSecond) return mul_rn(soft, soft);
+    if constexpr (HARD == kFourth) return mul_rn(mul_rn(soft, soft), mul_rn(soft, soft));
+    const Two h = mul_rn(d, Two(kLog2e, kLog2e));
+    return Two(exp2_of(h.lo()), exp2_of(h.hi()));
+}
+
 // WARP: a row per warp, one entry per lane, in CTAs of four; else a row per CTA or cluster.  STAGED: packs go through shared memory; else they are read
 // where they are needed.  HARD: with the loss against labels.
-template <typename T, bool STAGED, bool WARP, bool HARD>
+template <typename T, bool STAGED, bool WARP, int HARD>
 __global__ void __launch_bounds__(WARP ? 128 : 256)
 distill_kernel(const __grid_constant__ ffcvb_distillation_args a, const Deal deal) {
     constexpr int N = kWide<T>, BATCH = STAGED ? 1 : 4; // packs that a thread has on their way
@@ -283,21 +297,19 @@ distill_kernel(const __grid_constant__ ffcvb_distillation_args a, const Deal dea
             if (spread) sums.away += Sums::shift(sums.seen, sums.top, most);
             sums.top = most;
             if constexpr (M == 1) {
-                const float d = v[0] - most;
-                sums.soft += exp2_of(d * rate);
-                if (HARD) sums.hard += exp_of(d);
+                const float d = v[0] - most, e = exp2_of(d * rate);
+                sums.soft += e;
+                if (HARD) sums.hard += hard_exp<HARD>(d, e);
                 if (spread) sums.away += d;
             } else {
-                const Two minus(-most, -most), rates(rate, rate), log2e(kLog2e, kLog2e);
+                const Two minus(-most, -most), rates(rate, rate);
                 Two soft(0.0f, 0.0f), hard(0.0f, 0.0f), away(0.0f, 0.0f);
 #pragma unroll
                 for (int j = 0; j < M; j += 2) {
                     const Two d = add_rn(Two(v[j], v[j + 1]), minus), s = mul_rn(d, rates);
-                    soft = add_rn(soft, Two(exp2_of(s.lo()), exp2_of(s.hi())));
-                    if (HARD) {
-                        const Two h = mul_rn(d, log2e);
-                        hard = add_rn(hard, Two(exp2_of(h.lo()), exp2_of(h.hi())));
-                    }
+                    const Two e(exp2_of(s.lo()), exp2_of(s.hi()));
+                    soft = add_rn(soft, e);
+                    if (HARD) hard = add_rn(hard, hard_exp<HARD>(d, e));
                     if (spread) away = add_rn(away, d);
                 }
                 sums.soft += soft.lo() + soft.hi();
@@ -370,9 +382,9 @@ distill_kernel(const __grid_constant__ ffcvb_distillation_args a, const Deal dea
     const float times_soft = bad ? NAN : k_soft * all * over_soft, times_hard = k_hard * p.total * over_hard, flat = k_hard * p.flat;
     // what a class has of the gradient besides entries and labels
     auto common = [&](float v) {
-        const float d = v - top;
-        float out = times_soft * exp2_of(d * rate) - flat;
-        if (HARD) out += times_hard * exp_of(d);
+        const float d = v - top, e = exp2_of(d * rate);
+        float out = times_soft * e - flat;
+        if (HARD) out += times_hard * hard_exp<HARD>(d, e);
         return out;
     };
     auto share_of = [&](float t) { return exp_of(t - given.top) * over_given; };
@@ -405,18 +417,16 @@ distill_kernel(const __grid_constant__ ffcvb_distillation_args a, const Deal dea
     if (!g) return;
     {
         each_single([&](int c) { g[c] = from_float<T>(common(to_float(x[c]))); });
-        const Two minus(-top, -top), rates(rate, rate), log2e(kLog2e, kLog2e), less(-flat, -flat), soft2(times_soft, times_soft), hard2(times_hard, times_hard);
+        const Two minus(-top, -top), rates(rate, rate), less(-flat, -flat), soft2(times_soft, times_soft), hard2(times_hard, times_hard);
         each_pack([&](float(&v)[N], int c) {
 #pragma unroll
             for (int j = 0; j < N; j += 2) {
                 const Two d = add_rn(Two(v[j], v[j + 1]), minus), s = mul_rn(d, rates);
-                Two e = fma_rn(Two(exp2_of(s.lo()), exp2_of(s.hi())), soft2, less);
-                if (HARD) {
-                    const Two h = mul_rn(d, log2e);
-                    e = fma_rn(Two(exp2_of(h.lo()), exp2_of(h.hi())), hard2, e);
-                }
-                v[j] = e.lo();
-                v[j + 1] = e.hi();
+                const Two e(exp2_of(s.lo()), exp2_of(s.hi()));
+                Two out = fma_rn(e, soft2, less);
+                if (HARD) out = fma_rn(hard_exp<HARD>(d, e), hard2, out);
+                v[j] = out.lo();
+                v[j + 1] = out.hi();
             }
             Pack<T, N> pack;
             pack.set(v);
@@ -475,7 +485,7 @@ distill_kernel(const __grid_constant__ ffcvb_distillation_args a, const Deal dea
 // As for the cross entropy's rows: bytes of a row in a CTA's shared memory, at most where eight CTAs have a row, and in a warp's.
 constexpr long long kPartBytes = 56 * 1024, kMostPartBytes = 72 * 1024, kWarpBytes = 8192;
 
-template <typename T, bool HARD> void launch_rows(const ffcvb_distillation_args &a, cudaStream_t stream) {
+template <typename T, int HARD> void launch_rows(const ffcvb_distillation_args &a, cudaStream_t stream) {
     constexpr int W = 16 / (int)sizeof(T);
     const uintptr_t apart = reinterpret_cast<uintptr_t>(a.logits) ^ reinterpret_cast<uintptr_t>(a.grad);
     const bool both = a.grad && !a.from_stats; // (both passes)
@@ -560,10 +570,17 @@ extern "C" int ffcvb_distillation(const ffcvb_distillation_args *args, void *str
     if (a.counted) launch_count(a.target, a.rows, a.target_stride, a.ignore_index, a.counted, st);
     if (a.rows > 0)
         with_type(a.type, [&](auto zero) {
-            if (a.hard > 0.0f)
-                launch_rows<decltype(zero), true>(a, st);
+            using T = decltype(zero);
+            if (!(a.hard > 0.0f))
+                launch_rows<T, kNoHard>(a, st);
+            else if (a.temperature == 1.0f)
+                launch_rows<T, kFirst>(a, st);
+            else if (a.temperature == 2.0f)
+                launch_rows<T, kSecond>(a, st);
+            else if (a.temperature == 4.0f)
+                launch_rows<T, kFourth>(a, st);
             else
-                launch_rows<decltype(zero), false>(a, st);
+                launch_rows<T, kOwn>(a, st);
         });
     if (a.loss && !a.from_stats) launch_mean(a.row_loss, a.rows, a.counted, a.mean, a.loss, st);
     return launched("ffcvb_distillation");

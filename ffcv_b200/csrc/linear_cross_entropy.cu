@@ -547,12 +547,12 @@ __global__ void __launch_bounds__(kThreads, 1) products_kernel(const __grid_cons
     if (warp == 1) tmem_free<PAIR>(tmem, 2 * BN);
 }
 
-// Rows' statistics joined over the classes: 32 rows per CTA, whose 32 warps each take every 32nd part.
+// Rows' statistics joined over the classes: 32 rows per CTA, whose warps (eight, or 32 where there are few rows) take the parts in turn.
 __global__ void __launch_bounds__(1024) join_kernel(const __grid_constant__ Head h) {
-    __shared__ float s_top[32][33], s_sum[32][33], s_away[32][33];
+    __shared__ float s_top[32][33], s_sum[32][33], s_away[32][33], s_row[3][32];
     wait_for_previous();
     let_next_begin();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rows = rows_counted(h);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, rows = rows_counted(h);
     if (blockIdx.x * 32 >= rows) return;
     const bool apart = h.a.smoothing > 0.0f;
     float top = kLowest, sum = 0.0f, away = 0.0f, mass = 0.0f; // (mass: classes seen)
@@ -569,7 +569,7 @@ __global__ void __launch_bounds__(1024) join_kernel(const __grid_constant__ Head
     {
         const int row = blockIdx.x * 32 + lane;
 #pragma unroll 4
-        for (int k = warp; k < h.part_count; k += 32) {
+        for (int k = warp; k < h.part_count; k += warps) {
             const long long at = (long long)k * h.rows_pad + row;
             const float2 one = h.parts[at];
             add(one.x, one.x != one.x ? NAN : one.y, apart ? h.parts_apart[at] : 0.0f, there_of(k));
@@ -577,28 +577,34 @@ __global__ void __launch_bounds__(1024) join_kernel(const __grid_constant__ Head
     }
     s_top[warp][lane] = top, s_sum[warp][lane] = sum, s_away[warp][lane] = away;
     __syncthreads();
-    // now a warp has a row, and a lane what a warp had of it
-    const int row = blockIdx.x * 32 + warp;
-    if (row >= rows) return;
-    const float mine = s_top[lane][warp], most = warp_max(mine);
-    sum = warp_sum(s_sum[lane][warp] * exp_of(mine - most));
-    if (apart) {
-        long long seen = 0;
-        for (int k = lane; k < h.part_count; k += 32) seen += (int)there_of(k);
-        away = warp_sum(s_away[lane][warp] + (float)seen * fmaxf(mine - most, kLowest));
+    // now a warp has a row at a time, and a lane what a warp had of it
+    for (int r = warp; r < 32; r += warps) {
+        const float mine = lane < warps ? s_top[lane][r] : kLowest, most = warp_max(mine);
+        const float whole = warp_sum(lane < warps ? s_sum[lane][r] * exp_of(mine - most) : 0.0f);
+        float apart_all = 0.0f;
+        if (apart) {
+            float seen = 0.0f;
+            if (lane < warps)
+                for (int k = lane; k < h.part_count; k += warps) seen += there_of(k);
+            apart_all = warp_sum(lane < warps ? s_away[lane][r] + seen * fmaxf(mine - most, kLowest) : 0.0f);
+        }
+        if (lane == 0) s_row[0][r] = most, s_row[1][r] = whole, s_row[2][r] = apart_all;
     }
-    if (lane) return;
+    __syncthreads();
+    const int row = blockIdx.x * 32 + lane;
+    if (warp || row >= rows) return;
+    const float most = s_row[0][lane], whole = s_row[1][lane];
     const long long orig = h.map ? h.map[row] : row;
     const Picks p = picks_of(h.a, orig);
     float4 *stats = reinterpret_cast<float4 *>(h.a.stats) + orig;
     float loss = NAN, over = NAN;
     if (!p.bad) {
         const float picked[2] = {stats->z, stats->w};
-        float dot = p.flat > 0.0f ? p.flat * away : 0.0f;
+        float dot = p.flat > 0.0f ? p.flat * s_row[2][lane] : 0.0f;
         for (int k = 0; k < 2; k++)
             if (p.weight[k] != 0.0f) dot += p.weight[k] * (picked[k] - most);
-        loss = sum == 0.0f ? 0.0f : p.total * logf(sum) - dot;
-        over = sum == 0.0f ? 0.0f : 1.0f / sum;
+        loss = whole == 0.0f ? 0.0f : p.total * logf(whole) - dot;
+        over = whole == 0.0f ? 0.0f : 1.0f / whole;
     }
     h.a.row_loss[orig] = loss;
     stats->x = most;
@@ -746,17 +752,16 @@ __global__ void __launch_bounds__(256) settle_kernel(const __grid_constant__ Hea
 }
 
 // What is left to do behind a chunk's products: tiles that several CTAs have parts of, added up in their order; and the bias' gradient.  The first CTAs have
-// 32 rows each of the tile that a run begins in the middle of (the first such run of a tile); of the others each has 32 classes, whose sums over 32 rows it
-// adds up.
+// 32 classes each, whose sums over 32 rows they add up; the others 32 rows each of the tile that a run begins in the middle of (the first such run of a tile).
 template <typename T, int BN>
 __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Products p) {
     __shared__ float s_sum[8][32];
     wait_for_previous();
     let_next_begin();
     const Head &h = p.head;
-    const int rows = rows_counted(h), pieces = p.high / 32, tiles = p.count ? p.units * pieces : 0;
-    if ((int)blockIdx.x >= tiles) {
-        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = ((int)blockIdx.x - tiles) * 32 + lane, parts = (rows + 127) / 128 * 4;
+    const int rows = rows_counted(h), pieces = p.high / 32, biases = h.bias_parts ? (h.columns + 31) / 32 : 0;
+    if ((int)blockIdx.x < biases) {
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = (int)blockIdx.x * 32 + lane, parts = (rows + 127) / 128 * 4;
         float sum = 0.0f;
         if (c < h.columns) {
 #pragma unroll 16
@@ -770,7 +775,7 @@ __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Pro
         return;
     }
     const Runs runs(p, rows);
-    const int unit = (int)blockIdx.x / pieces, piece = (int)blockIdx.x - unit * pieces, place = runs.place(unit), lane = runs.lane(unit);
+    const int n = (int)blockIdx.x - biases, unit = n / pieces, piece = n - unit * pieces, place = runs.place(unit), lane = runs.lane(unit);
     if (place == 0 || place >= runs.units) return;
     const int begin = runs.begin(place);
     const Tile tile = tile_of(p, runs, lane, begin, rows);
@@ -987,7 +992,7 @@ template <typename T> int run(const ffcvb_linear_cross_entropy_args &a, uint8_t 
         if (!mapped) return training_fail(FFCVB_E_CUDA, "ffcvb_linear_cross_entropy: no map of a matrix");
         g.of[0].b_first = 0;
         fine &= launch_products<kStatistics, T>(p.stat_columns, p.pairs, g, tiles, st);
-        launch_early(join_kernel, (unsigned)(p.rows_pad / 32), 1024, 0, st, h);
+        launch_early(join_kernel, (unsigned)(p.rows_pad / 32), p.rows_pad / 32 >= 2 * kSms ? 256 : 1024, 0, st, h);
         if (a.loss) launch_mean(a.row_loss, a.rows, h.counted, a.mean, a.loss, st);
     }
     if (!p.grads) return fine ? launched("ffcvb_linear_cross_entropy") : training_fail(FFCVB_E_CUDA, "ffcvb_linear_cross_entropy: %s", cudaGetErrorString(cudaGetLastError()));
