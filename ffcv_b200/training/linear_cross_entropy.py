@@ -61,16 +61,25 @@ class _Call:
         self.hidden, self.weight, self.bias, self.target = _rows(hidden), _rows(weight), bias, target
         self.ignore, self.mean, self.smoothing, self.sizes = ignore_index, reduction == 'mean', float(smoothing), (n, classes, width)
 
-    def run(self, grads, rows_at, loss_at, stats, upstream=None, per_row=False, from_stats=False, scale=1.0):
-        """grads: of hidden, weight and bias, or None; rows_at, loss_at: addresses for a loss per sample, and for their mean or sum, or 0."""
+    def run(self, grads, rows_at, loss_at, stats=None, upstream=None, per_row=False, from_stats=False, scale=1.0):
+        """grads: of hidden, weight and bias, or None; rows_at, loss_at: addresses for a loss per sample, and for their mean or sum, or 0; without
+        `stats` they are in the workspace."""
         x, w, t, ignore = self.hidden, self.weight, self.target, self.ignore
         index = x.get_device()
-        args = N.LINEAR_CROSS_ENTROPY.pack(
-            x.data_ptr(), w.data_ptr(), N.ptr(self.bias), t.data_ptr(), N.ptr(upstream), *map(N.ptr, grads), loss_at, rows_at, stats.data_ptr(),
-            *self.sizes, x.stride(0), w.stride(0), t.stride(0), -1 if ignore is None else ignore,
-            index, self.type, self.kind, ignore is not None, self.mean, per_row, from_stats, 0, self.smoothing, scale)
-        workspace = ch.empty(N.lib.ffcvb_linear_cross_entropy_workspace(args), dtype=ch.uint8, device=x.device)
-        N.check(N.lib.ffcvb_linear_cross_entropy(args, workspace.data_ptr(), N.raw_stream(index)))
+
+        def pack(stats_at):
+            return N.LINEAR_CROSS_ENTROPY.pack(
+                x.data_ptr(), w.data_ptr(), N.ptr(self.bias), t.data_ptr(), N.ptr(upstream), *map(N.ptr, grads), loss_at, rows_at, stats_at,
+                *self.sizes, x.stride(0), w.stride(0), t.stride(0), -1 if ignore is None else ignore,
+                index, self.type, self.kind, ignore is not None, self.mean, per_row, from_stats, 0, self.smoothing, scale)
+
+        args = pack(16 if stats is None else stats.data_ptr())
+        size = N.lib.ffcvb_linear_cross_entropy_workspace(args)
+        workspace = ch.empty(size if stats is not None else size + 16 * self.sizes[0], dtype=ch.uint8, device=x.device)
+        at = workspace.data_ptr()
+        if stats is None:
+            args = pack(at + size)
+        N.check(N.lib.ffcvb_linear_cross_entropy(args, at, N.raw_stream(index)))
 
     def room_for(self, wanted):
         """Room for the gradients of hidden, weight and bias that are wanted."""
@@ -113,9 +122,8 @@ def linear_cross_entropy_with_grad(hidden, weight, labels=None, *, mixed=None, b
     n = hidden.shape[0]
     grads = call.room_for((True, True, True))
     loss = ch.empty(n + 1, dtype=ch.float32, device=hidden.device)
-    stats = ch.empty(4 * n, dtype=ch.float32, device=hidden.device)
     at = loss.data_ptr()
-    call.run(grads, at, 0 if reduction == 'none' else at + 4 * n, stats, scale=grad_scale)
+    call.run(grads, at, 0 if reduction == 'none' else at + 4 * n, scale=grad_scale)
     return (loss[:n] if reduction == 'none' else loss[n], *grads)
 
 
