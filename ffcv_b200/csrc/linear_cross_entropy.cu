@@ -844,9 +844,16 @@ constexpr int64_t kMostGradient = 256ll << 20;
 
 bool aligned(const void *p, int64_t stride) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && stride % 8 == 0; }
 
+// Columns of the logits' tiles: 256, but 128 where single CTAs would leave more than every other SM without a tile. Microseconds with 256 and with 128 columns: 4096 x
+// 1000 x 768 55 and 60, 16384 x 200 x 768 66 and 70, 128 x 21841 x 1024 82 and 89; below the bound 64 x 1000 x 384 35 and 33, 64 x 100 x 128 27 and 24.
+int columns_of(const Plan &p, int64_t classes) { return p.pairs || p.rows_pad / 128 * ((classes + 255) / 256) >= kSms / 2 ? 256 : 128; }
+
 Plan plan_of(const ffcvb_linear_cross_entropy_args &a) {
     Plan p{};
-    p.pairs = a.rows > 128;
+    // Pairs where there are rows for the second CTA and a tile of 256 x 256 logits for every SM: 1021 x 21841 x 768 takes 132 us, 166 by single CTAs; 512 x 10000 x
+    // 1024 (80 tiles) takes 79 either way, 1000 x 5000 x 512 (80 tiles) 55 by single CTAs and 64 by pairs, 128 x 21841 x 1024 (86 tiles, one of the two CTAs idle) 71
+    // and 108.
+    p.pairs = a.rows > 128 && (a.rows + 255) / 256 * ((a.classes + 255) / 256) >= kSms;
     p.rows_pad = up(a.rows, p.pairs ? 256 : 128);
     p.width_pad = up(a.width, 8);
     p.counted = a.has_ignore && a.target_kind == FFCVB_TARGET_LABELS;
@@ -854,11 +861,11 @@ Plan plan_of(const ffcvb_linear_cross_entropy_args &a) {
     p.lay_weight = !aligned(a.weight, a.weight_stride);
     p.hidden_grad = a.grad_hidden, p.weight_grad = a.grad_weight, p.bias_grad = a.grad_bias;
     p.grads = p.hidden_grad || p.weight_grad || p.bias_grad;
-    p.stat_columns = p.pairs || (a.classes + 255) / 256 >= kSms ? 256 : 128;
+    p.stat_columns = columns_of(p, a.classes);
     p.chunks = (a.classes * p.rows_pad * 2 + kMostGradient - 1) / kMostGradient;
     p.chunk = up((a.classes + p.chunks - 1) / p.chunks, 256);
     p.chunks = (a.classes + p.chunk - 1) / p.chunk;
-    p.sum_columns = p.pairs || a.width > 128 ? 256 : 128;
+    p.sum_columns = p.pairs ? 256 : 128; // (single CTAs with 128 and with 256 columns: 64 x 1000 x 384 29 us and 33, 4096 x 100 x 384 41 and 49, 128 x 21841 x 1024 77 and 89)
     p.hidden_direct = p.chunks == 1 && (p.counted || a.width % 8 == 0);
     p.weight_direct = a.width % 8 == 0;
     int64_t at = 0;
@@ -1014,7 +1021,7 @@ template <typename T> int run(const ffcvb_linear_cross_entropy_args &a, uint8_t 
     auto ctas_for = [&](int64_t rows) { return (unsigned)std::min<int64_t>((rows * ((a.width + 7) / 8) + 255) / 256, kSms * 8); };
     for (int64_t chunk = 0; chunk < p.chunks; chunk++) {
         const int64_t first = chunk * p.chunk, count = std::min(p.chunk, a.classes - first);
-        const int columns = p.pairs || (count + 255) / 256 >= kSms ? 256 : 128;
+        const int columns = columns_of(p, count);
         int64_t tiles = logits(columns, first, count);
         mapped &= matrix_map(&g.of[0].c, type, at(p.grad), p.counted ? p.rows_pad : a.rows, count, p.chunk, 32);
         g.of[0].c_last = (int)(p.counted ? p.rows_pad : a.rows);
