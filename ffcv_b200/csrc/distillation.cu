@@ -9,6 +9,10 @@
 // are joined over the row's threads together with the teacher's; a second pass makes the part of the gradient that all classes have; then the
 // classes with entries, or labels, are written once more, each by one thread, with the shares of all entries of that class, in their order: the same
 // class may come twice.  So the row crosses HBM once each way.
+//
+// What bounds it: exponentials, two for a logit, or three with the hard loss (one of them from the other where the temperature is 1, 2 or 4; else four), and the
+// instructions around them.  8192 x 21841 bf16 logits with 64 entries take 156 us, 110 at the rate of a copy; the unit for exponentials is busy for 63 % of it and 61 % of the
+// turns to issue are used, by five CTAs on an SM.  1531 x 50021 fp16 logits with 200 entries and labels take 121 us (65 %), 47 at the rate of a copy.  512 x 10 take 8 us: two launches.
 #include "losses.h"
 
 #include <algorithm>
@@ -482,7 +486,8 @@ distill_kernel(const __grid_constant__ ffcvb_distillation_args a, const Deal dea
     }
 }
 
-// As for the cross entropy's rows: bytes of a row in a CTA's shared memory, at most where eight CTAs have a row, and in a warp's.
+// As for the cross entropy's rows: bytes of a row in a CTA's shared memory (8192 x 21841 in 16 bits 156 us, 181 with 40 KB, 157 with 100; 1531 x 50021 124, 132 and
+// 124), at most where eight CTAs have a row, and in a warp's (16384 x 2000 in 16 bits 54 us, 88 by CTAs; 8192 x 3500 35 and 45; 16384 x 300 in 32 bits 27 and 73).
 constexpr long long kPartBytes = 56 * 1024, kMostPartBytes = 72 * 1024, kWarpBytes = 8192;
 
 template <typename T, int HARD> void launch_rows(const ffcvb_distillation_args &a, cudaStream_t stream) {
@@ -518,12 +523,13 @@ template <typename T, int HARD> void launch_rows(const ffcvb_distillation_args &
             run(distill_kernel<T, false, true, HARD>);
         return;
     }
-    // CTAs per row: until a part fits, and until there are two CTAs per SM (with few rows) of parts that are worth it
+    // CTAs per row: until a part fits, and until there is one for every SM (with few rows) of parts that are worth it (the loss alone of 8 x 200000 10.4 us, 18.5 by a
+    // CTA for each row; 8 x 24000 10.4 by two, 8.4 by one; 64 x 50000 10.4 either way)
     int ctas = 1;
-    while (ctas < 8 && ((both && (packs + ctas - 1) / ctas * 16 > kPartBytes) || (a.rows * ctas <= kSms && packs > 2048 * ctas))) ctas *= 2;
+    while (ctas < 8 && ((both && (packs + ctas - 1) / ctas * 16 > kPartBytes) || (a.rows * ctas <= kSms && packs > 4096 * ctas))) ctas *= 2;
     deal.part = (int)((packs + ctas - 1) / ctas);
     const bool staged = both && deal.part * 16ll <= kMostPartBytes; // (else the second pass reads what the caches still have)
-    const int threads = (deal.part / 14 + 31) / 32 * 32;
+    const int threads = (deal.part / 14 + 31) / 32 * 32; // (20000 x 6000 125 us, 207 by 256 threads each; 4096 x 8000 66 and 88; with 28 packs each within two in a hundred)
     how.gridDim = dim3((unsigned)(a.rows * ctas));
     how.blockDim = dim3(!deal.wide || threads > 256 ? 256 : threads < 64 ? 64 : threads);
     how.dynamicSmemBytes = (4 * a.kept + how.blockDim.x + 3) / 4 * 16 + (staged ? std::max(0, deal.part - (int)how.blockDim.x) * 16ll : 0);

@@ -7,6 +7,10 @@
 // What fits is held: some groups of a sample (channels of 64 bytes or more), at all positions, in the shared memory of a CTA or of a cluster's, so that x
 // (backward x and dy) is read once.  Threads copy what they use themselves, in places of their own, and exchange moments or sums
 // across the CTA and the cluster.  What does not fit is read twice, by kernels for the sums, for joining them, and for the values.
+//
+// What bounds it: instructions, for the activation above all.  256 x 56 x 56 x 256 bf16 values with SiLU take 179 us forward and 359 backward, 125 and 188 at the rate of a copy: 15 and 32
+// instructions for a value, 45 % of the turns to issue used by 16 warps on an SM, the rest waits for copies and for the group's last value.  What is read twice is bound by HBM:
+// 4 x 512 x 512 x 128 forward 159 us, 123 at the rate of a copy.  2 x 7 x 7 x 512 take 11 us for both directions: three launches.
 // Variances are joined from means and squares around them (of a thread's values relative to its first), which loses no digits where means are large.
 #include "training.h"
 #include "two.h"
@@ -46,6 +50,7 @@ template <> struct Pack<__half, 2> {
 
 namespace {
 
+// (What is held, by CTAs of 128: 56 x 56 x 256 forward and backward 187 and 385 us, 250 and 449 by CTAs of 256, which wait for more of their own.)
 constexpr int kThreads = 256, kHeldThreads = 128;
 constexpr int kMostGroups = 32; // of a CTA
 constexpr float kLog2e = 1.4426950408889634f;
@@ -551,6 +556,7 @@ template <typename T, int W, bool SPLIT> struct Back {
 };
 
 // room: (part_rows() + CTAs of the cluster) times the channels, of two floats; then, for each turn of the threads, x and dy
+// act' is computed in both passes: kept in 32 bits between them da takes the room that other CTAs need (56 x 56 x 256 520 us, 385 computed twice).
 template <typename T, int W, bool SPLIT>
 __global__ void __launch_bounds__(kHeldThreads) held_backward_kernel(const __grid_constant__ ffcvb_group_norm_args a, const Deal deal, float2 *sums) {
     constexpr int P = kPairs<W>, N = kHeldThreads;
@@ -649,6 +655,9 @@ __global__ void __launch_bounds__(kHeldThreads) held_backward_kernel(const __gri
 }
 
 // ---- not held: sums of slabs of positions, joined; then the values -------------------------------------------------------
+//
+// All samples' slabs in one launch, the values' from the last one back: 4 x 512 x 512 x 128 forward 236 us as built first, 298 to 336 in launches over as many samples as L2 holds,
+// which end and begin too often.  Three CTAs on an SM of the two kernels that read x and dy: backward 431 us, 507 with the registers that the compiler chooses.
 
 // Packs of a position, of which a CTA has `columns`, and `lanes` positions at once; positions of a slab, and slabs.
 struct Slabs {
@@ -918,13 +927,15 @@ __global__ void __launch_bounds__(1024) samples_kernel(const __grid_constant__ f
 
 // ---- the host's part -------------------------------------------------------------------------------------------------
 
-// Bytes that a CTA holds at most; of one that is not alone rather so much that there are four on an SM, in clusters of up to eight.
+// Bytes that a CTA holds at most; of one that is not alone rather so much that there are four on an SM, in clusters of up to eight.  (14 x 14 x 1024 backward by single CTAs of up to
+// 74 KB 177 us, 190 in clusters; 56 x 56 x 256 forward with 51 KB 187 us, 206 with 72, 204 with 26.)
 constexpr int64_t kMostHeld = 74 * 1024, kHeld = 51 * 1024;
 // Bytes of neighbouring channels that a CTA reads at least, where there are as many; and what it holds rather of small images, as long as there are six CTAs for
-// every SM.
+// every SM.  (56 x 56 x 256 forward and backward 187 and 385 us, 223 and 477 with 32 bytes; small images: 14 x 14 x 1024 forward 87 us, 119 with 64 bytes, 7 x 7 x 2048 83 and 195.)
 constexpr int64_t kNeighbours = 64, kSmall = 32 * 1024;
-// Positions of a thread in a slab: as many as bring eight CTAs to every SM.
-constexpr int64_t kLeastTurns = 4, kMostTurns = 16;
+// Positions of a thread in a slab: as many as bring eight CTAs to every SM.  (Forward and backward: 1 x 256 x 256 x 64 13 and 23 us, 17 and 28 with one position at least; 2 x 64 x 64 x 320
+// 12 and 23, 12 and 35; 4 x 512 x 512 x 128 159 and 307, 162 and 310 with 16 at most, 183 and 359 with 8.)
+constexpr int64_t kLeastTurns = 4, kMostTurns = 64;
 
 // Values of a pack: of one group or of two neighbouring ones (`split`), and where they begin as their size has it.
 int width_of(const ffcvb_group_norm_args &a, bool backward) {
@@ -957,7 +968,7 @@ Plan plan_of(const ffcvb_group_norm_args &a, bool backward) {
     p.split = per % w != 0;
     Deal &d = p.deal;
     d.groups = 1;
-    while (d.groups * 2 <= kMostGroups && a.groups % (d.groups * 2) == 0 && 
+    while (d.groups * 2 <= kMostGroups && a.groups % (d.groups * 2) == 0 &&
            (d.groups * per * size < kNeighbours || d.groups * per % w != 0 ||
             (d.groups * 2 * per * size * a.positions <= kSmall && d.groups * 2 * per / w <= 64 && a.samples * a.groups / (d.groups * 2) >= kSms * 6)))
         d.groups *= 2;

@@ -7,6 +7,11 @@
 // tiles leave as G, rounded to 16 bits (one rounding of at most 2^-9 (bf16) of a value that is multiplied and added with thousands of others), for as many
 // classes at once as the workspace has room for; of these dx's part is added up and dw's rows are finished.  So 8 * rows * classes * width
 // operations instead of 6 are done, and the logits, of any size, take a bounded workspace.
+//
+// What bounds it: the tensor cores, and in long runs the clock that their power leaves.  8192 x 21841 x 1024 in bf16 with all gradients takes 1.04 ms in a short run and
+// 1.19 in a long one; 880 us is the 8 * rows * classes * width at the rate of a large library product, 660 the 6.  Of it the statistics take 236 us (1550 TFLOP/s), the
+// joining 9, and each of the two chunks of 10921 classes 130 for G (1410), 240 for its products (1530) and 10 for what is left of them.  Kept in 16 bits
+// instead the logits would be 358 MB written and read, and rounded before the exponentials.  64 x 1000 x 384 takes 29 us: six launches, which wait for one another.
 #include "losses.h"
 #include "tensor.h"
 
@@ -99,10 +104,12 @@ struct Tile {
 __device__ __forceinline__ int row_tiles_of(const Products &p, const Product &w, int rows) { return w.counted == kRowsCounted ? (rows + p.high - 1) / p.high : w.row_tiles; }
 // (a sum without terms is one block long, all the same)
 __device__ __forceinline__ int sum_blocks_of(const Product &w, int rows) { return w.counted == kSumCounted ? max(1, (rows + kSum - 1) / kSum) : w.sum_blocks; }
-// Blocks of runs, at least: shorter ones cost more than they save.
+// Blocks of runs, at least: shorter ones cost more than they save.  (64 x 1000 x 384 33 us, 42 with 1, 41 with 16; 4096 x 100 x 384 54, 67 and 58; 2048 x 1000 x 768
+// 54, 54 and 49; larger ones within one in a hundred.)
 constexpr int kLeastRun = 4;
 // How blocks are dealt out: with few columns of tiles those of each column, in the same way to as many CTAs or pairs, so that those with the same rows read A at the same time;
-// else of all tiles, those of the same columns one after another.
+// else of all tiles, those of the same columns one after another.  (The products of 8192 x 10921 x 1024, four columns: 240 us, 450 where neighbouring CTAs read different
+// rows; 2048 x 8000 x 2560, ten columns: 246 us in all, 251 with all tiles in a line.)
 struct Runs {
     int lanes, all, units; // columns that are dealt out apart; blocks, and CTAs or pairs with a run, of each
     int each, more;       // blocks of a run, and runs with one more
@@ -175,6 +182,11 @@ template <> struct Walk<kProducts> {
 
 // A CTA per SM that takes tile after tile.  Products of the next tile go into the other half of TMEM while eight warps, two for each 32 rows, take
 // the last one's.  A wait that does not end makes the CTA give up: all that it has not finished is NaN, and it ends.
+//
+// A CTA of a pair copies its own 128 rows of A and half of the columns of B, 32 KB for 64 terms, and the first one's instruction multiplies both: half of the
+// shared memory's traffic for B.  (8192 x 10921 x 1024: products 240 us, 263 by single CTAs.)  Six stages of 32 KB, 192 KB, leave room for 32 KB of results, which
+// leave as boxes of 32 rows by 128 bytes; written by the threads themselves G takes 140 us instead of 128.  For the statistics a thread has half a row of a tile: one exponential
+// for a logit, whose 256 x 256 for a pair take half as long as 1024 terms of the product; below 512 terms they bound it.
 template <int MODE, typename T, int BN, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1) products_kernel(const __grid_constant__ Products p) {
     constexpr int STAGES = kStages<BN, PAIR>, HALF = BN / 2, CTAS = PAIR ? 2 : 1;
@@ -547,7 +559,7 @@ __global__ void __launch_bounds__(kThreads, 1) products_kernel(const __grid_cons
     if (warp == 1) tmem_free<PAIR>(tmem, 2 * BN);
 }
 
-// Rows' statistics joined over the classes: 32 rows per CTA, whose warps (eight, or 32 where there are few rows) take the parts in turn.
+// Rows' statistics joined over the classes: 32 rows per CTA, whose warps take the parts in turn: of 8192 x 171 16 MB, 9 us.
 __global__ void __launch_bounds__(1024) join_kernel(const __grid_constant__ Head h) {
     __shared__ float s_top[32][33], s_sum[32][33], s_away[32][33], s_row[3][32];
     wait_for_previous();
@@ -611,7 +623,8 @@ __global__ void __launch_bounds__(1024) join_kernel(const __grid_constant__ Head
     stats->y = over;
 }
 
-// Which rows count, in their order: the place of each, or -1; a row for each place.  One cluster; rows that do not count get a loss of 0.
+// Which rows count, in their order: the place of each, or -1; a row for each place.  Rows that do not count get a loss of 0.  One cluster of eight CTAs, which tell one
+// another how many they have: 50176 rows 9 us, 49 by one CTA.
 constexpr int kPlacesCtas = 8;
 __global__ void __launch_bounds__(1024) places_kernel(const __grid_constant__ ffcvb_linear_cross_entropy_args a, int *map, int *place, float *counted) {
     __shared__ int s_count[32], s_before[kPlacesCtas];
@@ -669,7 +682,7 @@ __global__ void __launch_bounds__(1024) places_kernel(const __grid_constant__ ff
 }
 
 // Rows of `width` values of 16 bits in places that the copies can begin at; rows behind those that count, up to the next 128, and columns behind
-// the last one are 0.
+// the last one are 0.  A copy: 50176 x 768 11 us where 40 % of the rows count.
 __global__ void __launch_bounds__(256) lay_kernel(const uint16_t *__restrict__ from, long long stride, int rows, int width, const int *map, const float *counted,
                                                   uint16_t *__restrict__ to, int pad, int wide) {
     wait_for_previous();
@@ -716,7 +729,8 @@ __global__ void __launch_bounds__(1024) most_kernel(const float *__restrict__ up
     }
 }
 
-// Gradients from sums in 32 bits, or of rows that count from 16 bits: out[r] = from[place of r]; rows without a place are 0.
+// Gradients from sums in 32 bits, or of rows that count from 16 bits: out[r] = from[place of r]; rows without a place are 0.  Bound by HBM: 8192 x 1024 sums 9 us, 50176 x 768
+// from 40 % as many sums 22.
 template <typename T, typename From>
 __global__ void __launch_bounds__(256) settle_kernel(const __grid_constant__ Head h, const From *__restrict__ sums, int pad, const int *place, T *__restrict__ out, int rows, int width) {
     wait_for_previous();
@@ -753,6 +767,7 @@ __global__ void __launch_bounds__(256) settle_kernel(const __grid_constant__ Hea
 
 // What is left to do behind a chunk's products: tiles that several CTAs have parts of, added up in their order; and the bias' gradient.  The first CTAs have
 // 32 classes each, whose sums over 32 rows they add up; the others 32 rows each of the tile that a run begins in the middle of (the first such run of a tile).
+// 7 to 16 us, for which all runs end at once: whole tiles dealt out to 148 CTAs leave up to half of them idle in the last turn (8192 x 21841 x 1024: 1720 us and 1348).
 template <typename T, int BN>
 __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Products p) {
     __shared__ float s_sum[8][32];
@@ -839,7 +854,8 @@ struct Plan {
     int64_t map, place, count, most, hidden, weight, parts, apart, grad, hidden_sums, hidden_rows, weight_sums, bias_parts, tile_parts, bytes;
 };
 
-// G's bytes at most.  (So many classes at once that dw's tiles and the sum over classes fill the GPU; 8 GB of HBM would hold 32 times as much.)
+// G's bytes at most: so many classes at once that the sum over classes of dx's few tiles is long and few parts are joined.  (8192 x 21841 x 1024, 358 MB in two chunks: 1038 us,
+// 1080 with 128 MB, 1184 with 64, 1192 with 512, which is one chunk; 50176 x 8192 x 768, 822 MB: 2374, 2736, 2866 and 2522.)
 constexpr int64_t kMostGradient = 256ll << 20;
 
 bool aligned(const void *p, int64_t stride) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && stride % 8 == 0; }
@@ -1012,6 +1028,7 @@ template <typename T> int run(const ffcvb_linear_cross_entropy_args &a, uint8_t 
         if (!mapped) return training_fail(FFCVB_E_CUDA, "ffcvb_linear_cross_entropy: no map of a matrix");
         g.of[0].b_first = 0;
         fine &= launch_products<kStatistics, T>(p.stat_columns, p.pairs, g, tiles, st);
+        // (32 warps, or eight where there are two CTAs for every SM: 1021 x 21841 x 768 130 us and 136, 50176 x 1000 x 256 195 and 187)
         launch_early(join_kernel, (unsigned)(p.rows_pad / 32), p.rows_pad / 32 >= 2 * kSms ? 256 : 1024, 0, st, h);
         if (a.loss) launch_mean(a.row_loss, a.rows, h.counted, a.mean, a.loss, st);
     }
