@@ -8,8 +8,8 @@
 // (backward x and dy) is read once.  Threads copy what they use themselves, in places of their own, and exchange moments or sums
 // across the CTA and the cluster.  What does not fit is read twice, by kernels for the sums, for joining them, and for the values.
 //
-// What bounds it: instructions, for the activation above all.  256 x 56 x 56 x 256 bf16 values with SiLU take 179 us forward and 359 backward, 125 and 188 at the rate of a copy: 15 and 32
-// instructions for a value, 45 % of the turns to issue used by 16 warps on an SM, the rest waits for copies and for the group's last value.  What is read twice is bound by HBM:
+// What bounds it: instructions, for the activation above all.  256 x 56 x 56 x 256 bf16 values with SiLU take 172 us forward and 321 backward, 125 and 188 at the rate of a copy: about 15 and 28
+// instructions for a value, of which half the turns to issue are used, and the unit for exponentials and reciprocals 50 % of the time; the rest waits for copies and for the group's last value.  What is read twice is bound by HBM:
 // 4 x 512 x 512 x 128 forward 159 us, 123 at the rate of a copy.  2 x 7 x 7 x 512 take 11 us for both directions: three launches.
 // Variances are joined from means and squares around them (of a thread's values relative to its first), which loses no digits where means are large.
 #include "training.h"
@@ -52,6 +52,7 @@ namespace {
 
 // (What is held, by CTAs of 128: 56 x 56 x 256 forward and backward 187 and 385 us, 250 and 449 by CTAs of 256, which wait for more of their own.)
 constexpr int kThreads = 256, kHeldThreads = 128;
+constexpr int kAhead = 6;       // packs of x that a thread has on their way a second time
 constexpr int kMostGroups = 32; // of a CTA
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -521,6 +522,12 @@ template <typename T, int W, bool SPLIT> struct Back {
 #pragma unroll
         for (int i = 0; i < P; i++) w[i] = mul_rn(w[i], rate[i]);
     }
+    // c
+    __device__ __forceinline__ void center(const Pack<T, W> &x, Two (&c)[P]) const {
+        get_pairs<T, W>(c, x);
+#pragma unroll
+        for (int i = 0; i < P; i++) c[i] = sub_rn(c[i], mean[i]);
+    }
     // c and a
     __device__ __forceinline__ void row(const Pack<T, W> &x, Two (&c)[P], Two (&v)[P]) const {
         get_pairs<T, W>(c, x);
@@ -555,8 +562,37 @@ template <typename T, int W, bool SPLIT> struct Back {
     }
 };
 
+// da in 32 bits in the place of a pack of x and one of dy; in the place of dy alone, where that has as many bits.
+template <typename T, int W> __device__ __forceinline__ void keep_pairs(Pack<T, W> *x, Pack<T, W> *dy, const Two (&v)[kPairs<W>]) {
+    if constexpr (sizeof(T) == 4) {
+        put_pairs<T, W>(reinterpret_cast<T *>(dy), v);
+    } else if constexpr (W > 1) {
+        float f[W];
+#pragma unroll
+        for (int i = 0; i < W; i++) f[i] = v[i / 2].half(i & 1);
+        Pack<float, W / 2> half;
+        half.set(reinterpret_cast<float(&)[W / 2]>(f[0]));
+        half.store(reinterpret_cast<float *>(x));
+        half.set(reinterpret_cast<float(&)[W / 2]>(f[W / 2]));
+        half.store(reinterpret_cast<float *>(dy));
+    }
+}
+template <typename T, int W> __device__ __forceinline__ void kept_pairs(Two (&v)[kPairs<W>], const Pack<T, W> *x, const Pack<T, W> *dy) {
+    if constexpr (sizeof(T) == 4) {
+        get_pairs<T, W>(v, *dy);
+    } else if constexpr (W > 1) {
+        float f[W];
+        reinterpret_cast<const Pack<float, W / 2> *>(x)->get(reinterpret_cast<float(&)[W / 2]>(f[0]));
+        reinterpret_cast<const Pack<float, W / 2> *>(dy)->get(reinterpret_cast<float(&)[W / 2]>(f[W / 2]));
+#pragma unroll
+        for (int i = 0; i < W / 2; i++) v[i] = Two(f[2 * i], f[2 * i + 1]);
+    }
+}
+
 // room: (part_rows() + CTAs of the cluster) times the channels, of two floats; then, for each turn of the threads, x and dy
-// act' is computed in both passes: kept in 32 bits between them da takes the room that other CTAs need (56 x 56 x 256 520 us, 385 computed twice).
+// Behind SiLU and GELU da stays for the second pass, in 32 bits where x and dy were, and of 16 bits x is read once more, out of L2, ahead of its use: backward 56 x 56 x 256 321 us,
+// 359 where da is computed twice, 520 where it has room of its own beside x and dy, which other CTAs need; with 2, 4 and 8 packs ahead 332, 329 and 322 (28 x 28 x 512
+// 174 with 6, 177 with 8).
 template <typename T, int W, bool SPLIT>
 __global__ void __launch_bounds__(kHeldThreads) held_backward_kernel(const __grid_constant__ ffcvb_group_norm_args a, const Deal deal, float2 *sums) {
     constexpr int P = kPairs<W>, N = kHeldThreads;
@@ -585,20 +621,30 @@ __global__ void __launch_bounds__(kHeldThreads) held_backward_kernel(const __gri
     Back<T, W, SPLIT> back;
     if (used) back = Back<T, W, SPLIT>(a, me.sample, channel, me.group0 + groups.left, groups);
     copies_done();
+    const bool keep = (sizeof(T) == 4 || W > 1) && (a.activation == FFCVB_ACT_SILU || a.activation == FFCVB_ACT_GELU);
     {
         Sums<W> mine;
         if (used) {
-            const Pack<T, W> *from = held;
+            Pack<T, W> *from = held;
 #pragma unroll 2
             for (int r = me.first + me.row; r < me.last; r += deal.lanes, from += 2 * N) {
                 Two c[P], da[P];
                 back.row(from[0], from[N], c, da);
                 mine.add(c, da);
+                if (keep) keep_pairs<T, W>(from, from + N, da);
             }
             mine.times(back.rate);
         }
         channel_sums<W>(mine, used, me.row, me.pack, deal.lanes, deal.packs, s_all, s_there + me.rank * channels);
     }
+    // (x's values of the first turns once more)
+    const T *again = static_cast<const T *>(a.x) + me.sample * a.x_sample + (me.first + me.row) * a.x_position + channel;
+    const long long again_step = deal.lanes * a.x_position;
+    Pack<T, W> ahead[kAhead];
+    if (sizeof(T) == 2 && keep && used)
+#pragma unroll
+        for (int j = 0; j < kAhead; j++)
+            if (me.first + me.row + j * deal.lanes < me.last) ahead[j].load(again + j * again_step);
     __syncthreads();
     if (deal.ctas > 1) {
         cluster_wait(); // all have begun
@@ -645,10 +691,33 @@ __global__ void __launch_bounds__(kHeldThreads) held_backward_kernel(const __gri
     T *to = static_cast<T *>(a.dx) + (me.sample * a.positions + me.first + me.row) * a.channels + channel;
     const long long step = deal.lanes * a.channels;
     const Pack<T, W> *from = held;
+    if (sizeof(T) == 2 && keep) {
+        again += kAhead * again_step;
+#pragma unroll 1
+        for (int r = me.first + me.row; r < me.last; r += kAhead * deal.lanes) {
+#pragma unroll
+            for (int j = 0; j < kAhead; j++) {
+                if (r + j * deal.lanes >= me.last) break;
+                Two c[P], da[P];
+                back.center(ahead[j], c);
+                if (r + (j + kAhead) * deal.lanes < me.last) ahead[j].load(again);
+                kept_pairs<T, W>(da, from, from + N);
+                back.gradient(c, da, less, less_c);
+                put_pairs<T, W>(to, da);
+                from += 2 * N, to += step, again += again_step;
+            }
+        }
+        return;
+    }
 #pragma unroll 2
     for (int r = me.first + me.row; r < me.last; r += deal.lanes, from += 2 * N, to += step) {
         Two c[P], da[P];
-        back.row(from[0], from[N], c, da);
+        if (sizeof(T) == 4 && keep) {
+            back.center(from[0], c);
+            kept_pairs<T, W>(da, from, from + N);
+        } else {
+            back.row(from[0], from[N], c, da);
+        }
         back.gradient(c, da, less, less_c);
         put_pairs<T, W>(to, da);
     }
@@ -927,9 +996,10 @@ __global__ void __launch_bounds__(1024) samples_kernel(const __grid_constant__ f
 
 // ---- the host's part -------------------------------------------------------------------------------------------------
 
-// Bytes that a CTA holds at most; of one that is not alone rather so much that there are four on an SM, in clusters of up to eight.  (14 x 14 x 1024 backward by single CTAs of up to
-// 74 KB 177 us, 190 in clusters; 56 x 56 x 256 forward with 51 KB 187 us, 206 with 72, 204 with 26.)
-constexpr int64_t kMostHeld = 74 * 1024, kHeld = 51 * 1024;
+// Bytes that a CTA holds at most; of one that is not alone rather so little that there are many on an SM, in clusters of up to eight.  (Forward and backward: 512 x 14 x 14 x 1024 84 and 134
+// us, 84 and 161 with single CTAs of up to 51 KB; 1024 x 7 x 7 x 2048 88 and 167, 88 and 391; 256 x 56 x 56 x 256 with parts of 51 KB 180 and 321, of 36 172 and 321; up to 72 KB by themselves
+// 206 forward.  Clusters of 16: 184 and 319, and 128 x 64 x 64 x 320, which is read twice, backward 538 where it takes 421.)
+constexpr int64_t kMostHeld = 74 * 1024, kHeld = 36 * 1024;
 // Bytes of neighbouring channels that a CTA reads at least, where there are as many; and what it holds rather of small images, as long as there are six CTAs for
 // every SM.  (56 x 56 x 256 forward and backward 187 and 385 us, 223 and 477 with 32 bytes; small images: 14 x 14 x 1024 forward 87 us, 119 with 64 bytes, 7 x 7 x 2048 83 and 195.)
 constexpr int64_t kNeighbours = 64, kSmall = 32 * 1024;
