@@ -1,5 +1,6 @@
-"""Operators of the training step that the loader's batches go into: a loss for mixed labels, the norms and
-residual joins of a network's blocks, positions of image patches, and the optimizer.  No counterpart in the
+"""Operators of the training step that the loader's batches go into: losses for mixed labels, for a linear layer's
+outputs that are not kept and for a teacher's logits, the norms and residual joins of a network's blocks, the group
+norm of convolutions with its activation, positions of image patches, and the optimizer.  No counterpart in the
 reference, whose work ends with the batch.
 
 Every operator is a hand-written kernel behind a call of ``libffcv_b200.so`` and runs on the current stream of its
