@@ -55,7 +55,7 @@ struct Head {
     float2 *parts;       // [classes / part_columns][rows_pad]: largest logit and sum of exponentials
     float *parts_apart;  // the same: sum of logits relative to the largest; with smoothing
     float *bias_parts;   // [rows_pad / 32][chunk]
-    const float *most;   // largest upstream of a row
+    const float *most;   // largest upstream of a row that counts
     int rows_pad, first, columns; // classes of this chunk
     int part_count, part_columns, chunk;
 };
@@ -399,8 +399,8 @@ __global__ void __launch_bounds__(kThreads, 1) products_kernel(const __grid_cons
                         const float4 stats = reinterpret_cast<const float4 *>(h.a.stats)[orig];
                         held = kHeld<T>;
                         if (h.a.upstream && h.a.upstream_per_row) {
-                            const float most = *h.most;
-                            held *= most == 0.0f ? 0.0f : h.a.upstream[orig] / most;
+                            const float most = *h.most, mine = h.a.upstream[orig];
+                            held *= !(fabsf(mine) < INFINITY) ? NAN : most == 0.0f ? 0.0f : mine / most;
                         }
                         row_top = stats.x;
                         if (stats.y == 0.0f) held = 0.0f; // (no logit but -inf)
@@ -708,24 +708,23 @@ __global__ void __launch_bounds__(256) lay_kernel(const uint16_t *__restrict__ f
     }
 }
 
-// The largest size of the rows' upstream gradients.
-__global__ void __launch_bounds__(1024) most_kernel(const float *__restrict__ upstream, long long rows, float *most) {
+// The largest size of the upstream gradients of rows that count (place: as of places_kernel, or NULL).  One that is no number or has no end is left out: it is
+// its own row's, whose G is NaN, and not the scale of the others.
+__global__ void __launch_bounds__(1024) most_kernel(const float *__restrict__ upstream, const int *__restrict__ place, long long rows, float *most) {
     __shared__ float s_most[32];
     wait_for_previous();
     let_next_begin();
     float m = 0.0f;
-    bool bad = false;
     for (long long i = threadIdx.x; i < rows; i += 1024) {
         const float v = fabsf(upstream[i]);
-        bad |= v != v;
-        m = fmaxf(m, v);
+        if (v < INFINITY && (!place || place[i] >= 0)) m = fmaxf(m, v);
     }
     m = warp_max(m);
     if ((threadIdx.x & 31) == 0) s_most[threadIdx.x >> 5] = m;
-    bad = __syncthreads_or(bad);
+    __syncthreads();
     if (threadIdx.x < 32) {
         m = warp_max(s_most[threadIdx.x]);
-        if (threadIdx.x == 0) *most = bad ? NAN : m;
+        if (threadIdx.x == 0) *most = m;
     }
 }
 
@@ -1033,7 +1032,7 @@ template <typename T> int run(const ffcvb_linear_cross_entropy_args &a, uint8_t 
         if (a.loss) launch_mean(a.row_loss, a.rows, h.counted, a.mean, a.loss, st);
     }
     if (!p.grads) return fine ? launched("ffcvb_linear_cross_entropy") : training_fail(FFCVB_E_CUDA, "ffcvb_linear_cross_entropy: %s", cudaGetErrorString(cudaGetLastError()));
-    if (a.upstream && a.upstream_per_row) launch_early(most_kernel, 1, 1024, 0, st, a.upstream, a.rows, static_cast<float *>(at(p.most)));
+    if (a.upstream && a.upstream_per_row) launch_early(most_kernel, 1, 1024, 0, st, a.upstream, h.place, a.rows, static_cast<float *>(at(p.most)));
     const int64_t wide = up(a.width, 32);
     auto ctas_for = [&](int64_t rows) { return (unsigned)std::min<int64_t>((rows * ((a.width + 7) / 8) + 255) / 256, kSms * 8); };
     for (int64_t chunk = 0; chunk < p.chunks; chunk++) {
