@@ -8,7 +8,7 @@ CSRC = os.path.join(HERE, 'csrc')
 LIB = os.path.join(HERE, 'libffcv_b200.so')
 SOURCES = ['context.cu', 'entropy.cu', 'idct.cu', 'gather.cu', 'resize.cu', 'pixel_ops.cu', 'static_decode.cu', 'training.cu',
            'cross_entropy.cu', 'linear_cross_entropy.cu', 'distillation.cu', 'norm_residual.cu', 'norm_forward.cu', 'norm_backward.cu', 'group_norm.cu', 'rotary.cu', 'adamw.cu', 'jpeg_header.cpp']
-HEADERS = ['types.h', 'kernels.h', 'jpeg_header.h', 'huffman.h', 'color.h', 'two.h', 'decode_index.h', 'table_store.h', 'training.h', 'losses.h', 'tensor.h', 'norm_residual.h',
+HEADERS = ['types.h', 'kernels.h', 'jpeg_header.h', 'huffman.h', 'color.h', 'two.h', 'decode_index.h', 'table_store.h', 'training.h', 'losses.h', 'tensor.h', 'waits.h', 'norm_residual.h',
            os.path.join('..', '..', 'include', 'ffcv_b200.h')]
 
 

@@ -230,17 +230,17 @@ __global__ void __launch_bounds__(kThreads, 1) products_kernel(const __grid_cons
             copy_box(to, map, x, y, bar);
     };
     Tile tile;
+    Waiter waiter(s_gave_up);
+    const bool &fine = waiter.fine;
     if (warp == 0) {
         if (lane == 0) {
             uint32_t n = 0; // stages filled so far
-            bool fine = true;
             for (Walk<MODE> walk(p, rows, unit); fine && walk.next(p, rows, tile);) {
                 const Product &w = p.of[tile.product];
                 for (int k = tile.from; k < tile.to; k++, n++) {
                     const uint32_t s = n % STAGES, at = room + s * STAGE, bar = first_full + 8 * s;
                     const int row = tile.row * (128 * CTAS) + rank * 128, column = tile.column * BN + rank * (BN / CTAS); // of this CTA
-                    fine = n < STAGES || barrier_wait(empty + 8 * s, (n / STAGES - 1) & 1, s_gave_up);
-                    if (!fine) break;
+                    if (n >= STAGES && !barrier_wait(waiter, empty + 8 * s, (n / STAGES - 1) & 1)) break;
                     if (rank == 0) barrier_expect(full + 8 * s, CTAS * STAGE);
                     if (MODE == kProducts) {
                         if (w.a_along_sum) {
@@ -258,28 +258,26 @@ __global__ void __launch_bounds__(kThreads, 1) products_kernel(const __grid_cons
                 }
             }
             if (PAIR && fine) // nor does the word that a stage is free, from the other CTA
-                for (uint32_t k = n < STAGES ? 0 : n - STAGES; k < n; k++) barrier_wait(empty + 8 * (k % STAGES), k / STAGES & 1, s_gave_up);
-            if (!fine && rank == 0) // no copy arrives behind the CTA's end (or the pair's)
+                for (uint32_t k = n < STAGES ? 0 : n - STAGES; k < n; k++) barrier_wait(waiter, empty + 8 * (k % STAGES), k / STAGES & 1);
+            else if (!fine && rank == 0) // no copy arrives behind the CTA's end (or the pair's)
                 for (uint32_t k = n < STAGES ? 0 : n - STAGES; k < n; k++) {
-                    volatile int patient = 0;
-                    barrier_wait(full + 8 * (k % STAGES), k / STAGES & 1, &patient);
+                    volatile int mine = 0;
+                    Waiter patient(&mine);
+                    barrier_wait(patient, full + 8 * (k % STAGES), k / STAGES & 1);
                 }
         }
         __syncwarp();
     } else if (warp == 1) {
         if (lane == 0 && rank == 0) {
             uint32_t n = 0, m = 0; // stages and tiles multiplied so far
-            bool fine = true;
             for (Walk<MODE> walk(p, rows, unit); fine && walk.next(p, rows, tile);) {
                 const bool a_along_sum = MODE == kProducts && p.of[tile.product].a_along_sum;
                 const uint32_t kind = product_kind(sizeof(T) == 2 && kHeld<T> == 1.0f, 128 * CTAS, BN, a_along_sum, MODE == kProducts), half = m & 1;
-                fine = m < 2 || barrier_wait(taken + 8 * half, (m / 2 - 1) & 1, s_gave_up);
-                if (!fine) break;
+                if (m >= 2 && !barrier_wait(waiter, taken + 8 * half, (m / 2 - 1) & 1)) break;
                 tmem_after_sync();
                 for (int k = tile.from; k < tile.to; k++, n++) {
                     const uint32_t s = n % STAGES, at = room + s * STAGE;
-                    fine = barrier_wait(full + 8 * s, n / STAGES & 1, s_gave_up);
-                    if (!fine) break;
+                    if (!barrier_wait(waiter, full + 8 * s, n / STAGES & 1)) break;
                     tmem_after_sync();
                     const uint64_t a = operand(at, kSum * 128), b = operand(at + kRowsBytes, kSum * 128);
 #pragma unroll
@@ -292,9 +290,10 @@ __global__ void __launch_bounds__(kThreads, 1) products_kernel(const __grid_cons
                 m++;
             }
             if (!fine) {
-                volatile int patient = 0;
+                volatile int mine = 0;
+                Waiter patient(&mine);
                 when_multiplied<PAIR>(drained);
-                barrier_wait(drained, 0, &patient);
+                barrier_wait(patient, drained, 0);
             }
         }
         __syncwarp();
@@ -316,8 +315,8 @@ __global__ void __launch_bounds__(kThreads, 1) products_kernel(const __grid_cons
                 }
                 asm volatile("bar.sync 1, 256;" ::: "memory");
             }
-            bool fine = barrier_wait(done + 8 * half, m / 2 & 1, s_gave_up);
-            fine = __all_sync(0xffffffffu, fine);
+            barrier_wait(waiter, done + 8 * half, m / 2 & 1);
+            waiter.fine = __all_sync(0xffffffffu, fine); // (and stays so for all tiles that are left)
             tmem_after_sync();
             m++;
             auto give_back = [&] { // behind the last load of the tile

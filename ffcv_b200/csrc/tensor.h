@@ -5,6 +5,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "waits.h"
+
 namespace ffcvb {
 
 // A map of a matrix [rows, cols] of 16- or 32-bit values, rows `stride` values apart, whose boxes are 128 bytes wide and `box` rows high and lie
@@ -42,22 +44,8 @@ __device__ __forceinline__ bool barrier_passed(uint32_t bar, uint32_t parity) {
                  : "memory");
     return done != 0;
 }
-// Waits two seconds at most.  `gave_up` is the CTA's: whoever waits longer sets it, and no wait lasts once it is set.
-constexpr uint64_t kLongestWait = 2000000000ull;
-__device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, volatile int *gave_up) {
-    if (barrier_passed(bar, parity)) return true;
-    uint64_t since = 0;
-    for (uint32_t tries = 1;; tries++) {
-        if (barrier_passed(bar, parity)) return true;
-        if ((tries & 63) != 0) continue;
-        if (*gave_up) return false;
-        const uint64_t now = nanoseconds();
-        if (since == 0) since = now;
-        if (now - since > kLongestWait) {
-            *gave_up = 1;
-            return false;
-        }
-    }
+__device__ __forceinline__ bool barrier_wait(Waiter &waiter, uint32_t bar, uint32_t parity) {
+    return waiter([&] { return barrier_passed(bar, parity); }, nanoseconds);
 }
 
 __device__ __forceinline__ void copy_box(uint32_t to, const CUtensorMap *map, int x, int y, uint32_t bar) {
