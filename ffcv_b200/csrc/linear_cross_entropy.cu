@@ -319,10 +319,10 @@ __global__ void __launch_bounds__(kThreads, 1) products_kernel(const __grid_cons
             waiter.fine = __all_sync(0xffffffffu, fine); // (and stays so for all tiles that are left)
             tmem_after_sync();
             m++;
-            auto give_back = [&] { // behind the last load of the tile
+            auto give_back = [&] { // behind the last load of the tile (one that has given up would be ahead of the others, and their half multiplied over)
                 tmem_before_sync();
                 __syncwarp();
-                if (lane != 0) return;
+                if (lane != 0 || !fine) return;
                 if (PAIR)
                     barrier_arrive_there(first_taken + 8 * half);
                 else

@@ -1,8 +1,10 @@
 """Waits for barriers that end (csrc/waits.h), compiled on its own for a barrier and a clock of the test's."""
 import os
+import re
 import subprocess
 
 import pytest
+from test_training_sources_cpu import kernels
 
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), 'ffcv_b200', 'csrc')
 BEGIN = r'''
@@ -75,3 +77,11 @@ def test_waits(what, tmp_path):
     subprocess.run(['g++', '-std=c++17', '-O2', '-Wall', '-Werror', '-I', CSRC, '-o', str(program), str(source)], check=True)
     run = subprocess.run([str(program)], capture_output=True, text=True, timeout=120)
     assert run.returncode == 0, run.stdout
+
+
+def test_who_has_given_up_gives_nothing_back():
+    """A half of the results is multiplied over once eight warps have arrived for it: arrivals for tiles that a warp has not waited for would stand for those
+    of warps that still read theirs."""
+    body = dict(kernels('linear_cross_entropy.cu'))['products_kernel']
+    give_back = re.search(r'auto give_back = \[&\] \{(.*?)\n {12}\};', body, re.S).group(1)
+    assert give_back.index('|| !fine) return;') < give_back.index('barrier_arrive')
