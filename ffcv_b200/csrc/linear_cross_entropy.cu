@@ -257,9 +257,9 @@ __global__ void __launch_bounds__(kThreads, 1) products_kernel(const __grid_cons
                     }
                 }
             }
-            if (PAIR && fine) // nor does the word that a stage is free, from the other CTA
+            if (PAIR) // nothing arrives behind the pair's end: no word that a stage is free, from the other CTA
                 for (uint32_t k = n < STAGES ? 0 : n - STAGES; k < n; k++) barrier_wait(waiter, empty + 8 * (k % STAGES), k / STAGES & 1);
-            else if (!fine && rank == 0) // no copy arrives behind the CTA's end (or the pair's)
+            if (rank == 0 && !(PAIR && fine)) // nor a copy (or the other CTA's), which nobody has waited for where the others have given up
                 for (uint32_t k = n < STAGES ? 0 : n - STAGES; k < n; k++) {
                     volatile int mine = 0;
                     Waiter patient(&mine);

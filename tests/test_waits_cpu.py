@@ -79,9 +79,22 @@ def test_waits(what, tmp_path):
     assert run.returncode == 0, run.stdout
 
 
+def products_kernel():
+    body, = (body for _, body in kernels('linear_cross_entropy.cu') if 'multiply<' in body)
+    return body
+
+
 def test_who_has_given_up_gives_nothing_back():
     """A half of the results is multiplied over once eight warps have arrived for it: arrivals for tiles that a warp has not waited for would stand for those
     of warps that still read theirs."""
-    body, = (body for _, body in kernels('linear_cross_entropy.cu') if 'multiply<' in body)
-    give_back = re.search(r'auto give_back = \[&\] \{(.*?)\n {12}\};', body, re.S).group(1)
+    give_back = re.search(r'auto give_back = \[&\] \{(.*?)\n {12}\};', products_kernel(), re.S).group(1)
     assert give_back.index('|| !fine) return;') < give_back.index('barrier_arrive')
+
+
+def test_copies_are_waited_for_whoever_has_given_up():
+    """A block that ends has no copy on its way, even if all were issued before others gave up: its shared memory is another's then.  (Those of a pair whose stages have
+    all been freed have been multiplied.)"""
+    copying = products_kernel().split('} else if (warp == 1) {')[0]
+    last = re.search(r'\n {12}if \(rank == 0 && !\(PAIR && fine\)\)[^\n]*\n(.*?)\n {12}\S', copying + '\n            .', re.S).group(1)
+    assert 'patient(&mine)' in last and 'barrier_wait(patient, full' in last
+    assert copying.index('for (Walk<MODE> walk') < copying.index('barrier_wait(waiter, empty + 8 * (k') < copying.index('barrier_wait(patient, full')
