@@ -12,6 +12,8 @@
 namespace ffcvb {
 
 constexpr uint64_t kLongestWait = 2000000000ull; // ns
+// What counts as waiting between two looks at the clock, at most: a longer time is one in which the whole block was not on the GPU.
+constexpr uint64_t kLongestLook = 100000000ull;
 constexpr uint32_t kTriesForALook = 64;
 
 // One that waits for barriers' phases, one after another.  `gave_up` is all waiters' of a block: whoever waits longer than kLongestWait sets it, and no wait that has to try
@@ -25,14 +27,15 @@ struct Waiter {
     template <typename Passed, typename Now> FFCVB_EVERYWHERE bool operator()(Passed passed, Now now) {
         if (!fine) return false;
         if (passed()) return true;
-        uint64_t since = 0;
+        uint64_t last = 0, waited = 0;
         for (uint32_t tries = 1;; tries++) {
             if (passed()) return true;
             if (tries % kTriesForALook != 0) continue;
             if (*gave_up) return fine = false;
-            const uint64_t time = now();
-            if (since == 0) since = time;
-            if (time - since > kLongestWait) {
+            const uint64_t time = now(), more = time - last;
+            if (last != 0) waited += more < kLongestLook ? more : kLongestLook;
+            last = time;
+            if (waited > kLongestWait) {
                 *gave_up = 1;
                 return fine = false;
             }

@@ -49,7 +49,7 @@ int main() {
     'a wait ends': r'''
 int main() {
     Barrier done;
-    for (uint64_t each = 100; each <= 10000000; each *= 10) {
+    for (uint64_t each = 100; each <= 1000000; each *= 10) {
         a_try = each;
         volatile int gave_up = 0;
         Waiter one(&gave_up), other(&gave_up);
@@ -64,6 +64,30 @@ int main() {
         CHECK(lucky([&] { return done.passed(0); }, now) && lucky.fine);
         done.over++;
     }
+    return 0;
+}
+''',
+    'time off the GPU is not waited': r'''
+int main() {
+    for (int tries = 0; tries < 3000; tries += 7) { // (the block is off the GPU for an hour, after so many tries)
+        Barrier done;
+        volatile int gave_up = 0;
+        Waiter waiter(&gave_up);
+        a_try = 100;
+        int left = tries;
+        const bool fine = waiter([&] {
+            if (left-- == 0) the_time += 3600000000000ull;
+            if (left == -1000) done.over++;
+            return done.passed(0);
+        }, now);
+        CHECK(fine && !gave_up);
+    }
+    // but one that is on and off again and again does not wait for good
+    Barrier never;
+    volatile int gave_up = 0;
+    Waiter waiter(&gave_up);
+    int tries = 0;
+    CHECK(!waiter([&] { tries++, the_time += 3600000000000ull; return never.passed(0); }, now) && tries <= 64 * 23);
     return 0;
 }
 ''',
