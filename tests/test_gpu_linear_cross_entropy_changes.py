@@ -1,5 +1,5 @@
-"""Cross entropy of a linear layer: upstream gradients that are no numbers or very large, against the formulas in 64 bits and with the
-tolerances of test_gpu_linear_cross_entropy."""
+"""Cross entropy of a linear layer: upstream gradients that are no numbers or very large, smoothing beside masked classes, against the formulas in 64 bits and with
+the tolerances of test_gpu_linear_cross_entropy."""
 import math
 
 import pytest
@@ -53,3 +53,43 @@ def test_an_upstream_that_is_no_number_is_its_own_rows(n, classes, width, dtype,
     want, (dx_want, *_), (sizes, *_), z = formula(x, w, b, reduction='none', upstream=quiet, **target)
     dx[17] = 0.0
     near([dx], [dx_want], [(sizes[0] + 2.0 ** -38 * 1.5 * w.double().abs().sum(0), sizes[1])], dtype)
+
+
+@pytest.mark.parametrize('masked', [-math.inf, torch.finfo(BF16).min])
+@pytest.mark.parametrize('smoothing', [0.1, 1.0])
+@pytest.mark.parametrize('target', ['labels', 'mixed'])
+@pytest.mark.parametrize('n,classes,width', [(3, 2, 8), (40, 50, 32), (150, 700, 64), (300, 20000, 72)])
+def test_smoothing_beside_masked_classes(n, classes, width, target, smoothing, masked):
+    """Classes masked by their bias have a share of a smoothed target: with -inf the loss has no end, with the type's lowest value it is as large as the formula has it.
+    Such a loss is a sum of terms of one sign, each off by 2^-24 of itself for a difference, a product and the share's own rounding; so it is
+    right to 2^-24 (classes / 32 + 100) of itself, which allows an addition for each of 32 classes that a thread has and those of all trees."""
+    from ffcv_b200.training import linear_cross_entropy, linear_cross_entropy_with_grad
+    x, w, b, how = make(n, classes, width, BF16, True, target)
+    b[1::2] = masked
+    b[:classes // 3] = masked
+    b[classes // 2 // 2 * 2] = 0.5
+    b[0] = 0.25
+    if target == 'labels':
+        how['labels'] = torch.where(torch.arange(n, device='cuda') % 2 == 0, 0, classes // 2 // 2 * 2)
+    else:
+        how['mixed'][:, 0], how['mixed'][:, 1] = 0, classes // 2 // 2 * 2
+    rows, dx, dw, db = linear_cross_entropy_with_grad(x, w, bias=b, label_smoothing=smoothing, reduction='none', **how)
+    again = linear_cross_entropy(x, w, bias=b, label_smoothing=smoothing, reduction='none', **how)
+    want, grads_want, sizes, z = formula(x, w, b, smoothing=smoothing, reduction='none', **how)
+    assert torch.equal(rows, again)
+    if masked == -math.inf:
+        assert bool((want == math.inf).all()) and torch.equal(rows, want.float())
+    else:
+        assert bool(want.float().isfinite().all())
+        assert bool(((rows.double() - want).abs() <= 2.0 ** -24 * (classes / 32 + 100) * want).all()), ((rows.double() - want) / want).abs().max()
+    near((dx, dw, db), grads_want, sizes, BF16)
+
+
+def test_rows_of_the_lowest_value_are_uniform():
+    """Nothing but masked classes: a uniform row, as where logits are kept."""
+    from ffcv_b200.training import linear_cross_entropy
+    for n, classes, width in ((40, 50, 32), (300, 20000, 72)):
+        x, w, b, target = make(n, classes, width, BF16, True, 'labels')
+        b[:] = torch.finfo(BF16).min
+        rows = linear_cross_entropy(x, w, bias=b, label_smoothing=0.1, reduction='none', **target)
+        assert bool(((rows - math.log(classes)).abs() < 1e-5).all())
