@@ -24,15 +24,15 @@ namespace {
 
 constexpr int kMostKept = FFCVB_DISTILLATION_MOST;
 
-// Of a part of a row: the largest logit, at least kLowest; sums of exponentials relative to it, at the temperature and (HARD) at 1; with smoothing the sum of logits
-// relative to it and how many they are.
+// Of a part of a row: the largest logit, at least kLowest; sums of exponentials relative to it, at the temperature and (HARD) at 1; with smoothing what its classes have of the
+// target, and the sum of that times the logits relative to the largest (of differences themselves to logits of the type's lowest value, which mask classes, it would not be finite).
 struct Sums {
-    float top, soft, hard, away, seen;
-    static __device__ __forceinline__ float shift(float seen, float from, float to) { return seen * fmaxf(from - to, kLowest); }
+    float top, soft, hard, away, mass;
+    static __device__ __forceinline__ float shift(float mass, float from, float to) { return mass * fmaxf(from - to, kLowest); }
     __device__ __forceinline__ void to(float most, float rate) {
         soft *= exp2_of((top - most) * rate);
         hard *= exp_of(top - most);
-        away += shift(seen, top, most);
+        away += shift(mass, top, most);
         top = most;
     }
     __device__ __forceinline__ void join(Sums o, float rate) {
@@ -42,7 +42,7 @@ struct Sums {
         soft += o.soft;
         hard += o.hard;
         away += o.away;
-        seen += o.seen;
+        mass += o.mass;
     }
     // joins those of groups of LANES lanes
     template <int LANES, int HARD> __device__ __forceinline__ void join_lanes(float rate, bool spread) {
@@ -51,7 +51,7 @@ struct Sums {
         for (int o = LANES / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
         soft *= exp2_of((top - most) * rate);
         if (HARD) hard *= exp_of(top - most);
-        if (spread) away += shift(seen, top, most);
+        if (spread) away += shift(mass, top, most);
         top = most;
 #pragma unroll
         for (int o = LANES / 2; o > 0; o >>= 1) {
@@ -62,7 +62,7 @@ struct Sums {
 #pragma unroll
         for (int o = LANES / 2; o > 0; o >>= 1) {
             away += __shfl_xor_sync(0xffffffffu, away, o);
-            seen += __shfl_xor_sync(0xffffffffu, seen, o);
+            mass += __shfl_xor_sync(0xffffffffu, mass, o);
         }
     }
 };
@@ -298,15 +298,15 @@ distill_kernel(const __grid_constant__ ffcvb_distillation_args a, const Deal dea
             const float less = sums.top - most;
             sums.soft *= exp2_of(less * rate);
             if (HARD) sums.hard *= exp_of(less);
-            if (spread) sums.away += Sums::shift(sums.seen, sums.top, most);
+            if (spread) sums.away += Sums::shift(sums.mass, sums.top, most);
             sums.top = most;
             if constexpr (M == 1) {
                 const float d = v[0] - most, e = exp2_of(d * rate);
                 sums.soft += e;
                 if (HARD) sums.hard += hard_exp<HARD>(d, e);
-                if (spread) sums.away += d;
+                if (spread) sums.away += p.flat * d;
             } else {
-                const Two minus(-most, -most), rates(rate, rate);
+                const Two minus(-most, -most), rates(rate, rate), flat(p.flat, p.flat);
                 Two soft(0.0f, 0.0f), hard(0.0f, 0.0f), away(0.0f, 0.0f);
 #pragma unroll
                 for (int j = 0; j < M; j += 2) {
@@ -314,13 +314,13 @@ distill_kernel(const __grid_constant__ ffcvb_distillation_args a, const Deal dea
                     const Two e(exp2_of(s.lo()), exp2_of(s.hi()));
                     soft = add_rn(soft, e);
                     if (HARD) hard = add_rn(hard, hard_exp<HARD>(d, e));
-                    if (spread) away = add_rn(away, d);
+                    if (spread) away = fma_rn(d, flat, away);
                 }
                 sums.soft += soft.lo() + soft.hi();
                 if (HARD) sums.hard += hard.lo() + hard.hi();
                 if (spread) sums.away += away.lo() + away.hi();
             }
-            if (spread) sums.seen += M;
+            if (spread) sums.mass += M * p.flat;
         };
         each_single([&](int c) {
             const float v[1] = {to_float(x[c])};
@@ -339,7 +339,7 @@ distill_kernel(const __grid_constant__ ffcvb_distillation_args a, const Deal dea
         const int warps = blockDim.x >> 5;
         if (lane == 0) {
             float *to = s_part[threadIdx.x >> 5];
-            to[0] = sums.top, to[1] = sums.soft, to[2] = sums.hard, to[3] = sums.away, to[4] = sums.seen, to[5] = given.top, to[6] = given.sum;
+            to[0] = sums.top, to[1] = sums.soft, to[2] = sums.hard, to[3] = sums.away, to[4] = sums.mass, to[5] = given.top, to[6] = given.sum;
         }
         __syncthreads();
         const float *from = s_part[lane & 7];
@@ -354,7 +354,7 @@ distill_kernel(const __grid_constant__ ffcvb_distillation_args a, const Deal dea
             if (threadIdx.x < ranks) {
                 uint32_t to;
                 asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"((uint32_t)__cvta_generic_to_shared(s_there[rank])), "r"(threadIdx.x));
-                const float v[5] = {sums.top, sums.soft, sums.hard, sums.away, sums.seen};
+                const float v[5] = {sums.top, sums.soft, sums.hard, sums.away, sums.mass};
 #pragma unroll
                 for (int i = 0; i < 5; i++) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 4 * i), "f"(v[i]) : "memory");
             }
@@ -409,7 +409,7 @@ distill_kernel(const __grid_constant__ ffcvb_distillation_args a, const Deal dea
         if (lane == 0) {
             float out = soft == 0.0f || all == 0.0f ? 0.0f : soft * tau * tau * (loss + logf(sums.soft) - logf(given.sum));
             if (HARD) {
-                float dot = spread ? p.flat * sums.away : 0.0f;
+                float dot = spread ? sums.away : 0.0f;
 #pragma unroll
                 for (int k = 0; k < 2; k++)
                     if (p.weight[k] != 0.0f && !bad) dot += p.weight[k] * (to_float(x[p.label[k]]) - top);
