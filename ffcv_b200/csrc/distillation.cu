@@ -67,19 +67,19 @@ struct Sums {
     }
 };
 
-// The same of the teacher's logits over the temperature.
+// The same of the teacher's logits, at the temperature.  (Differences are divided by it, not logits: one below 1 would leave the type's lowest value infinite.)
 struct Given {
     float top, sum;
-    __device__ __forceinline__ void add(float t) {
+    __device__ __forceinline__ void add(float t, float rate) {
         const float most = fmaxf(top, t);
-        sum = sum * exp_of(top - most) + exp_of(t - most);
+        sum = sum * exp2_of((top - most) * rate) + exp2_of((t - most) * rate);
         top = most;
     }
-    template <int LANES> __device__ __forceinline__ void join_lanes() {
+    template <int LANES> __device__ __forceinline__ void join_lanes(float rate) {
         float most = top;
 #pragma unroll
         for (int o = LANES / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-        sum *= exp_of(top - most);
+        sum *= exp2_of((top - most) * rate);
         top = most;
 #pragma unroll
         for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -145,7 +145,7 @@ distill_kernel(const __grid_constant__ ffcvb_distillation_args a, const Deal dea
     const int packs = (classes - before) / N, singles = classes - packs * N;
     const int first = (int)rank * deal.part, count = max(0, min(packs - first, deal.part));
     const T *x0 = x + before + (long long)first * N;
-    // before the row's packs: entries' classes, teacher's logits over the temperature, own logits; of each thread a list of those entries whose classes it writes
+    // before the row's packs: entries' classes, teacher's logits, own logits; of each thread a list of those entries whose classes it writes
     int *s_class = reinterpret_cast<int *>(s_row), *s_next = s_class + 3 * kept, *s_first = s_next + kept;
     float *s_given = reinterpret_cast<float *>(s_class + kept), *s_logit = s_given + kept;
     const int head = WARP ? 0 : (4 * kept + threads + 3) / 4;
@@ -182,11 +182,11 @@ distill_kernel(const __grid_constant__ ffcvb_distillation_args a, const Deal dea
             my_class = c < 0 || c >= classes ? -1 : (int)c;
             if (my_class >= 0) {
                 my_x = to_float(x[my_class]);
-                given.add(my_logit = logit_of(a, row, lane) / tau);
+                given.add(my_logit = logit_of(a, row, lane), rate);
             }
         }
         bad = __any_sync(0xffffffffu, bad);
-        given.join_lanes<32>();
+        given.join_lanes<32>(rate);
     } else {
         if (thread == 0) s_bad = 0;
         s_first[thread] = -1;
@@ -210,9 +210,9 @@ distill_kernel(const __grid_constant__ ffcvb_distillation_args a, const Deal dea
         const int here = c < 0 || c >= classes || t == -INFINITY ? -1 : (int)c; // (rows that are filled up with one class have no long lists)
         s_class[k] = here;
         if (here < 0) return;
-        s_given[k] = t / tau;
+        s_given[k] = t;
         s_logit[k] = v;
-        given.add(t / tau);
+        given.add(t, rate);
         const int by = writer(here);
         if (by >= 0) s_next[k] = atomicExch(s_first + by, k);
     };
@@ -227,7 +227,7 @@ distill_kernel(const __grid_constant__ ffcvb_distillation_args a, const Deal dea
             take_entry(k, c, logit_of(a, row, k), c >= 0 && c < classes ? to_float(x[c]) : 0.0f);
         }
         if (bad) s_bad = 1;
-        given.join_lanes<32>();
+        given.join_lanes<32>(rate);
     };
     if (p.ignored) { // (all of a row's threads alike)
         const T zero = from_float<T>(0.0f);
@@ -347,7 +347,7 @@ distill_kernel(const __grid_constant__ ffcvb_distillation_args a, const Deal dea
         sums = there ? Sums{from[0], from[1], from[2], from[3], from[4]} : Sums{kLowest, 0.0f, 0.0f, 0.0f, 0.0f};
         given = there ? Given{from[5], from[6]} : Given{kLowest, 0.0f};
         sums.join_lanes<8, HARD>(rate, spread);
-        given.join_lanes<8>();
+        given.join_lanes<8>(rate);
         bad = s_bad != 0;
         if (ranks > 1) {
             asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); // all have begun
@@ -391,13 +391,13 @@ distill_kernel(const __grid_constant__ ffcvb_distillation_args a, const Deal dea
         if (HARD) out += times_hard * hard_exp<HARD>(d, e);
         return out;
     };
-    auto share_of = [&](float t) { return exp_of(t - given.top) * over_given; };
+    auto share_of = [&](float t) { return exp2_of((t - given.top) * rate) * over_given; };
     if (thread < 32 && rank == 0 && !a.from_stats) { // a warp has the loss
-        // the soft one is sum q (log q - log p); log q has the teacher's sum, log p the student's, both once for all shares
+        // the soft one is tau^2 sum q (log q - log p); log q has the teacher's sum, log p the student's, both once for all shares
         float loss = 0.0f;
         auto add = [&](float t, float v) {
             const float q = share_of(t);
-            if (q != 0.0f) loss += q * ((t - given.top) - (v - top) / tau);
+            if (q != 0.0f) loss += q * ((t - given.top) - (v - top));
         };
         if (WARP) {
             if (my_class >= 0) add(my_logit, my_x);
@@ -407,7 +407,7 @@ distill_kernel(const __grid_constant__ ffcvb_distillation_args a, const Deal dea
         }
         loss = warp_sum(loss);
         if (lane == 0) {
-            float out = soft == 0.0f || all == 0.0f ? 0.0f : soft * tau * tau * (loss + logf(sums.soft) - logf(given.sum));
+            float out = soft == 0.0f || all == 0.0f ? 0.0f : soft * tau * (loss + tau * (logf(sums.soft) - logf(given.sum)));
             if (HARD) {
                 float dot = spread ? sums.away : 0.0f;
 #pragma unroll
