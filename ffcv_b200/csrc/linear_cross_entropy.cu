@@ -53,9 +53,12 @@ struct Head {
     const int *place;    // a row's place among them, or -1
     const float *counted;
     float2 *parts;       // [classes / part_columns][rows_pad]: largest logit and sum of exponentials
-    float *parts_apart;  // the same: share_of_all() times the sum of logits relative to the largest; with smoothing
+    float *parts_apart;  // the same: `share` times the sum of logits relative to the largest; with smoothing
     float *bias_parts;   // [rows_pad / 32][chunk]
     const float *most;   // largest upstream of a row that counts
+    // What smoothing gives every class of the target.  (It multiplies differences before they are added up: a sum of those to logits of the type's lowest value, which mask
+    // classes, would not be finite, the loss is.)
+    float share;
     int rows_pad, first, columns; // classes of this chunk
     int part_count, part_columns, chunk;
 };
@@ -85,10 +88,6 @@ template <> __device__ __forceinline__ uint32_t two_of<__nv_bfloat16>(float lo, 
     const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t *>(&v);
 }
-
-// What smoothing gives every class of the target.  (It multiplies differences before they are added up: a sum of those to logits of the type's lowest value, which mask
-// classes, would not be finite, the loss is.)
-__device__ __forceinline__ float share_of_all(const Head &h) { return h.a.smoothing / (float)h.a.classes; }
 
 __device__ __forceinline__ int rows_counted(const Head &h) { return h.counted ? (int)*h.counted : (int)h.a.rows; }
 
@@ -339,7 +338,6 @@ __global__ void __launch_bounds__(kThreads, 1) products_kernel(const __grid_cons
                 Picks picks{{-1, -1}, {0.0f, 0.0f}, 0.0f, 0.0f, false, true};
                 if (there) picks = picks_of(h.a, orig);
                 const bool apart = h.a.smoothing > 0.0f;
-                const float share = share_of_all(h);
                 const int left = (int)h.a.classes - (h.first + column); // classes from the first column on
                 float top = kLowest, sum = 0.0f, away = 0.0f;
 #pragma unroll 1
@@ -358,7 +356,7 @@ __global__ void __launch_bounds__(kThreads, 1) products_kernel(const __grid_cons
 #pragma unroll
                     for (int j = 0; j < 16; j++) most = fmaxf(most, fmaxf(z[j].lo(), z[j].hi()));
                     sum *= exp_of(top - most);
-                    if (apart) away += share * (float)min(c, max(left, 0)) * fmaxf(top - most, kLowest);
+                    if (apart) away += h.share * (float)min(c, max(left, 0)) * fmaxf(top - most, kLowest);
                     top = most;
                     const Two minus(-top, -top), log2e(kLog2e, kLog2e);
                     Two part[2] = {Two(0.0f, 0.0f), Two(0.0f, 0.0f)};
@@ -373,7 +371,7 @@ __global__ void __launch_bounds__(kThreads, 1) products_kernel(const __grid_cons
                     if (apart) {
                         float all = 0.0f;
 #pragma unroll
-                        for (int j = 0; j < 16; j++) all += share * (c + 2 * j < left ? z[j].lo() : 0.0f) + share * (c + 2 * j + 1 < left ? z[j].hi() : 0.0f);
+                        for (int j = 0; j < 16; j++) all += h.share * (c + 2 * j < left ? z[j].lo() : 0.0f) + h.share * (c + 2 * j + 1 < left ? z[j].hi() : 0.0f);
                         away += all;
                     }
                 }
@@ -571,7 +569,6 @@ __global__ void __launch_bounds__(1024) join_kernel(const __grid_constant__ Head
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, rows = rows_counted(h);
     if (blockIdx.x * 32 >= rows) return;
     const bool apart = h.a.smoothing > 0.0f;
-    const float share = share_of_all(h);
     float top = kLowest, sum = 0.0f, away = 0.0f, mass = 0.0f; // (mass: what the classes seen have of the target by smoothing)
     auto add = [&](float t, float s, float d, float there) {
         const float most = fmaxf(top, t);
@@ -582,7 +579,7 @@ __global__ void __launch_bounds__(1024) join_kernel(const __grid_constant__ Head
         }
         top = most;
     };
-    auto there_of = [&](int k) { return share * (float)max(0, min(h.part_columns, (int)h.a.classes - k * h.part_columns)); };
+    auto there_of = [&](int k) { return h.share * (float)max(0, min(h.part_columns, (int)h.a.classes - k * h.part_columns)); };
     {
         const int row = blockIdx.x * 32 + lane;
 #pragma unroll 4
@@ -962,6 +959,7 @@ template <typename T> int run(const ffcvb_linear_cross_entropy_args &a, uint8_t 
     g.high = high;
     Head &h = g.head;
     h.a = a;
+    h.share = a.smoothing / (float)a.classes;
     h.rows_pad = (int)p.rows_pad;
     h.map = p.counted ? static_cast<int *>(at(p.map)) : nullptr;
     h.place = p.counted ? static_cast<int *>(at(p.place)) : nullptr;
