@@ -89,6 +89,24 @@ template <> __device__ __forceinline__ uint32_t two_of<__nv_bfloat16>(float lo, 
     return *reinterpret_cast<const uint32_t *>(&v);
 }
 
+// Sums over a warp's rows, a row per lane, of 32 columns; a lane gets its column's.  Lanes exchange halves of what they have left, in 31 shuffles.  (1021 x 21841 x 768 140
+// us with them, 142 by way of shared memory in 32 bits, 135 where the rounded boxes were read back, 131 without a bias; 16384 x 21841 x 128 1010, 1036, 932 and 882.)
+__device__ __forceinline__ float sum_rows(Two (&v)[16]) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int turn = 0; turn < 4; turn++) {
+        const int n = 8 >> turn;
+        const bool upper = lane & 2 * n;
+#pragma unroll
+        for (int j = 0; j < n; j++) {
+            const Two keep = upper ? v[j + n] : v[j], give = upper ? v[j] : v[j + n];
+            v[j] = add_rn(keep, Two(__shfl_xor_sync(0xffffffffu, give.lo(), 2 * n), __shfl_xor_sync(0xffffffffu, give.hi(), 2 * n)));
+        }
+    }
+    const bool upper = lane & 1;
+    return (upper ? v[0].hi() : v[0].lo()) + __shfl_xor_sync(0xffffffffu, upper ? v[0].lo() : v[0].hi(), 1);
+}
+
 __device__ __forceinline__ int rows_counted(const Head &h) { return h.counted ? (int)*h.counted : (int)h.a.rows; }
 
 // What all gradients are multiplied by behind the sums.
@@ -494,6 +512,22 @@ __global__ void __launch_bounds__(kThreads, 1) products_kernel(const __grid_cons
                             values(v, raw[i], c + 32 * i);
 #pragma unroll
                             for (int j = 0; j < 16; j++) out[16 * i + j] = two_of<T>(v[j].lo(), v[j].hi());
+                            if constexpr (MODE == kGradient) {
+                                if (h.bias_parts) { // sums of these 32 rows, before they are rounded
+#pragma unroll
+                                    for (int k = 0; k < 2; k++) {
+                                        const int l = label[k] < 0 ? -1 : label[k] - c - 32 * i;
+                                        const float one = fine ? written[k] : NAN;
+                                        if (__any_sync(0xffffffffu, l >= 0 && l < 32)) {
+#pragma unroll
+                                            for (int j = 0; j < 16; j++) v[j] = Two(l == 2 * j ? one : v[j].lo(), l == 2 * j + 1 ? one : v[j].hi());
+                                        }
+                                    }
+                                    const int x = column + c + 32 * i + lane;
+                                    const float sum = sum_rows(v);
+                                    if (x < h.chunk) h.bias_parts[(long long)(row_tile * 4 + quarter) * h.chunk + x] = sum;
+                                }
+                            }
                         }
                         room_free(); // (the last box has been read meanwhile)
 #pragma unroll
@@ -508,30 +542,6 @@ __global__ void __launch_bounds__(kThreads, 1) products_kernel(const __grid_cons
                             }
                         }
                         leave(c);
-                        if constexpr (MODE == kGradient) {
-                            if (h.bias_parts) { // sums of these 32 rows: four columns for a lane, of every other row
-                                Two s0(0.0f, 0.0f), s1(0.0f, 0.0f);
-#pragma unroll
-                                for (int r = 0; r < 32; r += 2) {
-                                    const int rr = r + lane / 16;
-                                    Pack<T, 4> pack;
-                                    float f[4];
-                                    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];"
-                                                 : "=r"(pack.raw.x), "=r"(pack.raw.y)
-                                                 : "r"(mine + rr * 128 + ((lane % 16 / 2 ^ (rr & 7)) << 4) + lane % 2 * 8)
-                                                 : "memory");
-                                    pack.get(f);
-                                    s0 = add_rn(s0, Two(f[0], f[1]));
-                                    s1 = add_rn(s1, Two(f[2], f[3]));
-                                }
-                                float s[4] = {s0.lo(), s0.hi(), s1.lo(), s1.hi()};
-#pragma unroll
-                                for (int i = 0; i < 4; i++) s[i] += __shfl_down_sync(0xffffffffu, s[i], 16);
-                                const int x = column + c + 4 * lane;
-                                if (lane < 16 && x < h.chunk)
-                                    *reinterpret_cast<float4 *>(h.bias_parts + (long long)(row_tile * 4 + quarter) * h.chunk + x) = make_float4(s[0], s[1], s[2], s[3]);
-                            }
-                        }
                     }
                 } else {
 #pragma unroll 1

@@ -116,7 +116,8 @@ def linear_cross_entropy_with_grad(hidden, weight, labels=None, *, mixed=None, b
     grad_scale : float
         Factor of the gradients, applied before they are rounded to 16 bits: with float16 the loss scale.
 
-    The loss is float32.  The gradient of the logits is rounded to 16 bits before it is multiplied with weights and hidden values.  With a gradient
+    The loss is float32.  The gradient of the logits is rounded to 16 bits before it is multiplied with weights and hidden values; the
+    bias' is the sum of it as it was before.  With a gradient
     per sample from behind (``reduction='none'`` and autograd) it is held relative to the largest of these among the samples that count: in
     float16 in steps of 2^-38 of that, so a sample with a billionth of the largest keeps few digits.  One that is infinite or NaN
     makes its own sample's hidden gradient NaN, and those of the weights and the bias, which are sums over the samples.

@@ -93,3 +93,18 @@ def test_rows_of_the_lowest_value_are_uniform():
         b[:] = torch.finfo(BF16).min
         rows = linear_cross_entropy(x, w, bias=b, label_smoothing=0.1, reduction='none', **target)
         assert bool(((rows - math.log(classes)).abs() < 1e-5).all())
+
+
+@pytest.mark.parametrize('n,classes,width', [(1, 5, 8), (3, 130, 16), (40, 1000, 64), (129, 257, 72), (300, 20000, 72), (1021, 3001, 200)])
+@pytest.mark.parametrize('dtype', [BF16, F16])
+@pytest.mark.parametrize('target', ['labels', 'mixed'])
+def test_gradient_of_the_bias_is_rounded_once(n, classes, width, dtype, target):
+    """It is a sum of 32-bit values: off by 4e-6 of what is added up, as the logits' gradients are, and by half a step of itself."""
+    x, w, b, how = make(n, classes, width, dtype, True, target)
+    from ffcv_b200.training import linear_cross_entropy_with_grad
+    scale = 256.0  # (fp16's smallest numbers have few digits)
+    db = linear_cross_entropy_with_grad(x, w, bias=b, label_smoothing=0.05, grad_scale=scale, **how)[3].double()
+    want, sizes = (v[2] for v in formula(x, w, b, smoothing=0.05, **how)[1:3])
+    small = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    room = torch.finfo(dtype).eps / 2 * (want * scale).abs() + 4e-6 * sizes[1] * scale + small
+    assert bool(((db - want * scale).abs() <= room).all()), float(((db - want * scale).abs() / room).max())
