@@ -1186,7 +1186,9 @@ int call(const ffcvb_group_norm_args *args, void *workspace, void *stream, bool 
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (some) {
         (backward ? run_backward : run_forward)(a, static_cast<uint8_t *>(workspace), st);
-    } else if (backward) {
+    } else if (!backward) { // (a mean of nothing is no number, and all bits of a NaN may be set)
+        if (a.stats && a.samples > 0) cudaMemsetAsync(a.stats, 0xff, (size_t)(a.samples * a.groups * 8), st);
+    } else {
         if (a.dweight) cudaMemsetAsync(a.dweight, 0, (size_t)(a.channels * type_size(a.param_type)), st);
         if (a.dbias) cudaMemsetAsync(a.dbias, 0, (size_t)(a.channels * type_size(a.param_type)), st);
     }
