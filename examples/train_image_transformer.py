@@ -111,14 +111,14 @@ class Block(nn.Module):
 
 
 class Stem(nn.Module):
-    """Patches by convolutions that halve the sides, each but the last with a group norm and an activation behind it; all channels last, as the
-    loader's images are."""
+    """Patches by convolutions that halve the sides as often as the patch can be halved, each with a group norm and an activation behind it, and one that
+    takes what is left of a patch; all channels last, as the loader's images are."""
 
     def __init__(self, patch, width):
         from ffcv_b200.training import GroupNormAct
         super().__init__()
         channels, layers = 3, []
-        while patch > 2:
+        while patch > 2 and patch % 2 == 0:
             more = 32 if channels == 3 else min(2 * channels, 256)
             layers += [nn.Conv2d(channels, more, 3, 2, 1), GroupNormAct(8, more, 'silu')]
             channels, patch = more, patch // 2
