@@ -5,8 +5,8 @@
 // matrix products on the tensor cores with sums of 32 bits: x w^T a first time, whose tiles never leave the SM: of 128 logits of a row the
 // largest and the sum of exponentials relative to it are left; joined, they give the loss and lse.  Then x w^T a second time, whose
 // tiles leave as G, rounded to 16 bits (one rounding of at most 2^-9 (bf16) of a value that is multiplied and added with thousands of others), for as many
-// classes at once as the workspace has room for; of these dx's part is added up and dw's rows are finished.  So 8 * rows * classes * width
-// operations instead of 6 are done, and the logits, of any size, take a bounded workspace.
+// classes at once as 256 MB hold (256 classes of all rows at least); of these dx's part is added up and dw's rows are finished.  So 8 * rows * classes * width
+// operations instead of 6 are done, and no logits are kept; the first time leaves 8 bytes (12 with smoothing) for 128 logits of a row, or for 64 with narrow tiles.
 //
 // What bounds it: the tensor cores, and in long runs the clock that their power leaves.  8192 x 21841 x 1024 in bf16 with all gradients takes 1.04 ms in a short run and
 // 1.19 in a long one; 880 us is the 8 * rows * classes * width at the rate of a large library product, 660 the 6.  Of it the statistics take 236 us (1550 TFLOP/s), the
@@ -865,7 +865,7 @@ struct Plan {
     int64_t map, place, count, most, hidden, weight, parts, apart, grad, hidden_sums, hidden_rows, weight_sums, bias_parts, tile_parts, bytes;
 };
 
-// G's bytes at most: so many classes at once that the sum over classes of dx's few tiles is long and few parts are joined.  (8192 x 21841 x 1024, 358 MB in two chunks: 1038 us,
+// G's bytes at most, or those of 256 classes of all rows: so many classes at once that the sum over classes of dx's few tiles is long and few parts are joined.  (8192 x 21841 x 1024, 358 MB in two chunks: 1038 us,
 // 1080 with 128 MB, 1184 with 64, 1192 with 512, which is one chunk; 50176 x 8192 x 768, 822 MB: 2374, 2736, 2866 and 2522.)
 constexpr int64_t kMostGradient = 256ll << 20;
 
