@@ -4,7 +4,7 @@
 // (see cross_entropy.cu) and G = S exp(z - lse) - T the gradient of its logits; then dx = G w, dw = G^T x, db = sum of G's rows.  All are
 // matrix products on the tensor cores with sums of 32 bits: x w^T a first time, whose tiles never leave the SM: of 128 logits of a row the
 // largest and the sum of exponentials relative to it are left; joined, they give the loss and lse.  Then x w^T a second time, whose
-// tiles leave as G, rounded to 16 bits (one rounding of at most 2^-9 (bf16) of a value that is multiplied and added with thousands of others), for as many
+// tiles leave as G, rounded to 16 bits (one rounding of at most 2^-8 (bf16) of a value that is multiplied and added with thousands of others), for as many
 // classes at once as 256 MB hold (256 classes of all rows at least); of these dx's part is added up and dw's rows are finished.  So 8 * rows * classes * width
 // operations instead of 6 are done, and no logits are kept; the first time leaves 8 bytes (12 with smoothing) for 128 logits of a row, or for 64 with narrow tiles.
 //
@@ -89,22 +89,26 @@ template <> __device__ __forceinline__ uint32_t two_of<__nv_bfloat16>(float lo, 
     return *reinterpret_cast<const uint32_t *>(&v);
 }
 
-// Sums over a warp's rows, a row per lane, of 32 columns; a lane gets its column's.  Lanes exchange halves of what they have left, in 31 shuffles.  (1021 x 21841 x 768 140
-// us with them, 142 by way of shared memory in 32 bits, 135 where the rounded boxes were read back, 131 without a bias; 16384 x 21841 x 128 1010, 1036, 932 and 882.)
-__device__ __forceinline__ float sum_rows(Two (&v)[16]) {
+// Sums over a warp's rows, a row per lane, of two times 32 columns; a lane gets its column's of either.  Lanes exchange halves of what they have left, in 31 shuffles for 32 columns.
+// (1021 x 21841 x 768 136 us with them, 139 with 32 columns at a time, 142 by way of shared memory in 32 bits, 135 where the rounded boxes were read back, 131 without a bias;
+// 16384 x 21841 x 128 962, 1012, 1036, 932 and 880.)
+__device__ __forceinline__ void sum_rows(Two (&v)[2][16], float (&sum)[2]) {
     const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int turn = 0; turn < 4; turn++) {
         const int n = 8 >> turn;
         const bool upper = lane & 2 * n;
 #pragma unroll
-        for (int j = 0; j < n; j++) {
-            const Two keep = upper ? v[j + n] : v[j], give = upper ? v[j] : v[j + n];
-            v[j] = add_rn(keep, Two(__shfl_xor_sync(0xffffffffu, give.lo(), 2 * n), __shfl_xor_sync(0xffffffffu, give.hi(), 2 * n)));
-        }
+        for (int j = 0; j < n; j++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const Two keep = upper ? v[i][j + n] : v[i][j], give = upper ? v[i][j] : v[i][j + n];
+                v[i][j] = add_rn(keep, Two(__shfl_xor_sync(0xffffffffu, give.lo(), 2 * n), __shfl_xor_sync(0xffffffffu, give.hi(), 2 * n)));
+            }
     }
     const bool upper = lane & 1;
-    return (upper ? v[0].hi() : v[0].lo()) + __shfl_xor_sync(0xffffffffu, upper ? v[0].lo() : v[0].hi(), 1);
+#pragma unroll
+    for (int i = 0; i < 2; i++) sum[i] = (upper ? v[i][0].hi() : v[i][0].lo()) + __shfl_xor_sync(0xffffffffu, upper ? v[i][0].lo() : v[i][0].hi(), 1);
 }
 
 __device__ __forceinline__ int rows_counted(const Head &h) { return h.counted ? (int)*h.counted : (int)h.a.rows; }
@@ -501,6 +505,7 @@ __global__ void __launch_bounds__(kThreads, 1) products_kernel(const __grid_cons
 #pragma unroll 1
                     for (int c = 0; c < HALF; c += 64) {
                         uint32_t raw[2][32], out[32];
+                        Two v[2][16];
                         tmem_load(raw[0], at + c);
                         tmem_load(raw[1], at + c + 32);
                         tmem_wait(raw[0]);
@@ -508,26 +513,9 @@ __global__ void __launch_bounds__(kThreads, 1) products_kernel(const __grid_cons
                         if (c + 64 >= HALF) give_back();
 #pragma unroll
                         for (int i = 0; i < 2; i++) {
-                            Two v[16];
-                            values(v, raw[i], c + 32 * i);
+                            values(v[i], raw[i], c + 32 * i);
 #pragma unroll
-                            for (int j = 0; j < 16; j++) out[16 * i + j] = two_of<T>(v[j].lo(), v[j].hi());
-                            if constexpr (MODE == kGradient) {
-                                if (h.bias_parts) { // sums of these 32 rows, before they are rounded
-#pragma unroll
-                                    for (int k = 0; k < 2; k++) {
-                                        const int l = label[k] < 0 ? -1 : label[k] - c - 32 * i;
-                                        const float one = fine ? written[k] : NAN;
-                                        if (__any_sync(0xffffffffu, l >= 0 && l < 32)) {
-#pragma unroll
-                                            for (int j = 0; j < 16; j++) v[j] = Two(l == 2 * j ? one : v[j].lo(), l == 2 * j + 1 ? one : v[j].hi());
-                                        }
-                                    }
-                                    const int x = column + c + 32 * i + lane;
-                                    const float sum = sum_rows(v);
-                                    if (x < h.chunk) h.bias_parts[(long long)(row_tile * 4 + quarter) * h.chunk + x] = sum;
-                                }
-                            }
+                            for (int j = 0; j < 16; j++) out[16 * i + j] = two_of<T>(v[i][j].lo(), v[i][j].hi());
                         }
                         room_free(); // (the last box has been read meanwhile)
 #pragma unroll
@@ -542,6 +530,26 @@ __global__ void __launch_bounds__(kThreads, 1) products_kernel(const __grid_cons
                             }
                         }
                         leave(c);
+                        if constexpr (MODE == kGradient) {
+                            if (h.bias_parts) { // sums of these 32 rows, before they are rounded
+#pragma unroll
+                                for (int k = 0; k < 2; k++) {
+                                    const int l = label[k] < 0 ? -1 : label[k] - c;
+                                    const float one = fine ? written[k] : NAN;
+                                    if (__any_sync(0xffffffffu, l >= 0 && l < 64)) {
+#pragma unroll
+                                        for (int j = 0; j < 32; j++)
+                                            v[j / 16][j % 16] = Two(l == 2 * j ? one : v[j / 16][j % 16].lo(), l == 2 * j + 1 ? one : v[j / 16][j % 16].hi());
+                                    }
+                                }
+                                float sum[2];
+                                sum_rows(v, sum);
+                                float *to = h.bias_parts + (long long)(row_tile * 4 + quarter) * h.chunk + column + c + lane;
+#pragma unroll
+                                for (int i = 0; i < 2; i++)
+                                    if (column + c + 32 * i + lane < h.chunk) to[32 * i] = sum[i];
+                            }
+                        }
                     }
                 } else {
 #pragma unroll 1
