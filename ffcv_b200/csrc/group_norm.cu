@@ -1087,6 +1087,7 @@ const char *wrong(const ffcvb_group_norm_args &a, bool backward) {
     if (a.x_sample < 0 || a.x_position < 0 || a.dy_sample < 0 || a.dy_position < 0) return "bad stride";
     if (a.activation < FFCVB_ACT_NONE || a.activation > FFCVB_ACT_GELU || !(a.eps >= 0.0f)) return "bad argument";
     if (a.samples > 0 && a.positions > 0 && (!a.x || !a.stats || (backward ? !a.dy : !a.y))) return "an address is missing";
+    if ((reinterpret_cast<uintptr_t>(a.stats) & 7) != 0) return "stats begin on 8 bytes";
     if (backward && !a.dx && !a.dweight && !a.dbias) return "nothing to do";
     if (a.samples > 0 && a.positions > 0 && a.samples * plan_of(a, backward).slabs.slabs > INT32_MAX) return "too many values";
     return nullptr;

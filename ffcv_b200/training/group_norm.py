@@ -113,6 +113,8 @@ class _Call:
             raise ValueError(f'dy must be {x.dtype} {tuple(x.shape)}, not {dy.dtype} {tuple(dy.shape)}')
         if stats.shape != (self.sizes[0], self.sizes[3], 2) or stats.dtype != ch.float32 or not stats.is_contiguous() or stats.device != x.device:
             raise ValueError('stats must be what the forward pass of the same call gave')
+        if stats.data_ptr() % 8:  # (kept in the middle of another tensor)
+            stats = stats.clone()
         dy, dy_strides = self.laid(dy)
         dx = _new(x) if wanted[0] else None
         dweight, dbias = (ch.empty_like(p) if w else None for p, w in zip((self.weight, self.bias), wanted[1:]))

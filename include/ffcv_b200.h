@@ -425,7 +425,7 @@ enum { FFCVB_ACT_NONE = 0, FFCVB_ACT_RELU = 1, FFCVB_ACT_SILU = 2, FFCVB_ACT_GEL
 typedef struct {
     const void *x;
     const void *weight, *bias; /* [channels] of param_type, or NULL: 1, 0 */
-    float *stats;           /* [samples, groups, 2]: mean and 1 / deviation (NaN without positions); written forward, read backward */
+    float *stats;           /* [samples, groups, 2], 8-byte aligned: mean and 1 / deviation (NaN without positions); written forward, read backward */
     void *y;                /* contiguous; forward only */
     const void *dy;         /* backward only, like the following */
     void *dx;               /* contiguous, or NULL: not wanted */

@@ -1,4 +1,4 @@
-"""Group norm: statistics of samples without positions."""
+"""Group norm: statistics of samples without positions, and those that were kept elsewhere."""
 import pytest
 
 torch = pytest.importorskip('torch')
@@ -16,3 +16,16 @@ def test_statistics_of_nothing_are_no_numbers(samples, channels, groups, sides):
         assert y.shape == x.shape and stats.shape == (samples, groups, 2) and bool(stats.isnan().all())
         grads = group_norm_act_backward(y, x, stats, groups, weight=w)
         assert grads['x'].shape == x.shape and not grads['weight'].any()
+
+
+@pytest.mark.parametrize('sides', [(6, 7), (170, 171)])
+@pytest.mark.parametrize('offset', [0, 1, 2, 3])
+def test_statistics_kept_in_another_tensor(sides, offset):
+    from ffcv_b200.training import group_norm_act_backward, group_norm_act_forward
+    x, dy = (torch.randn(2, *sides, 32, device='cuda').movedim(-1, 1) for _ in range(2))
+    _, stats = group_norm_act_forward(x, 4, activation='silu')
+    kept = torch.zeros(stats.numel() + offset, device='cuda')[offset:].view(stats.shape)
+    kept.copy_(stats)
+    assert kept.data_ptr() % 8 == offset % 2 * 4
+    want, got = (group_norm_act_backward(dy, x, s, 4, activation='silu')['x'] for s in (stats, kept))
+    assert torch.equal(got, want)
