@@ -556,6 +556,7 @@ const char *wrong(const ffcvb_distillation_args &a) {
     if (a.rows > 0 && (!a.logits || !a.teacher || !a.teacher_classes || (a.hard > 0.0f && !a.target) || (a.from_stats ? !a.stats || !a.grad : !a.row_loss)))
         return "an address is missing";
     if (a.has_ignore && a.mean && !a.counted) return "no room for the count";
+    if ((reinterpret_cast<uintptr_t>(a.stats) & 15) != 0) return "stats begin on 16 bytes";
     return nullptr;
 }
 

@@ -7,3 +7,10 @@ def test_group_norm():
     for call in (lib.ffcvb_group_norm, lib.ffcvb_group_norm_backward):
         for at in (257, 258, 260, 263):
             assert call(group_norm(stats=at), 256, None) == -2 and b'stats begin on 8 bytes' in lib.ffcvb_training_error()
+
+
+def test_distillation():
+    from ffcv_b200.training import _native as N
+    for at in (257, 260, 264, 271):
+        args = N.DISTILLATION.pack(16, 16, 16, 16, 0, 16, 0, 16, at, 16, 4, 50, 5, 50, 5, 5, 1, 50, -1, 0, 0, 0, 0, 0, 0, 1, 0, 0, 0, 1.0, 0.0, 0.0, 1.0)
+        assert N.lib.ffcvb_distillation(args, None) == -2 and b'stats begin on 16 bytes' in N.lib.ffcvb_training_error()
