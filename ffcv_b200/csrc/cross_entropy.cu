@@ -480,6 +480,7 @@ extern "C" int ffcvb_cross_entropy(const ffcvb_cross_entropy_args *args, void *s
         (a.rows > 0 && (!a.logits || !a.target || (a.from_stats ? !a.stats || !a.grad : !a.row_loss))) || (needs_count && !a.counted) ||
         (a.has_ignore && a.target_kind != FFCVB_TARGET_LABELS))
         return training_fail(FFCVB_E_ARG, "ffcvb_cross_entropy: bad argument");
+    if ((reinterpret_cast<uintptr_t>(a.stats) & 7) != 0) return training_fail(FFCVB_E_ARG, "ffcvb_cross_entropy: stats begin on 8 bytes");
     OnDevice here(a.device);
     if (!here.ok()) return training_fail(FFCVB_E_NODEVICE, "ffcvb_cross_entropy: no device %d", a.device);
     cudaStream_t st = static_cast<cudaStream_t>(stream);

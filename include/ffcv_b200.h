@@ -335,7 +335,7 @@ typedef struct {
     void *grad;             /* [rows, classes] of the logits' type, or NULL: no gradient */
     float *loss;            /* one value, the mean or the sum, or NULL */
     float *row_loss;        /* [rows]: written unless from_stats */
-    float *stats;           /* [rows, 2]: largest logit and 1 / sum exp(x - it); written, or read with from_stats, or NULL */
+    float *stats;           /* [rows, 2], 8-byte aligned: largest logit and 1 / sum exp(x - it); written, or read with from_stats, or NULL */
     float *counted;         /* one value of workspace; needed with has_ignore and mean */
     int64_t rows, classes, logits_stride, target_stride, grad_stride, ignore_index;
     int32_t device, type, target_kind, target_type, has_ignore, mean, upstream_per_row;

@@ -14,3 +14,10 @@ def test_distillation():
     for at in (257, 260, 264, 271):
         args = N.DISTILLATION.pack(16, 16, 16, 16, 0, 16, 0, 16, at, 16, 4, 50, 5, 50, 5, 5, 1, 50, -1, 0, 0, 0, 0, 0, 0, 1, 0, 0, 0, 1.0, 0.0, 0.0, 1.0)
         assert N.lib.ffcvb_distillation(args, None) == -2 and b'stats begin on 16 bytes' in N.lib.ffcvb_training_error()
+
+
+def test_cross_entropy():
+    from ffcv_b200.training import _native as N
+    for at in (257, 260, 263):
+        args = N.CROSS_ENTROPY.pack(16, 16, 0, 16, 0, 16, at, 0, 4, 5, 5, 1, 5, 0, 0, 0, 0, 0, 0, 1, 0, 0, 0.0, 1.0)
+        assert N.lib.ffcvb_cross_entropy(args, None) == -2 and b'stats begin on 8 bytes' in N.lib.ffcvb_training_error()
