@@ -151,6 +151,7 @@ int check(const Args *args, bool backward, const void *workspace) {
     if (!backward && a.rows > 0 && ((a.norm != FFCVB_NORM_NONE && !a.z) || (a.h && !a.y)))
         return training_fail(FFCVB_E_ARG, "%s: no room for the results", name);
     if (backward && ((a.rows > 0 && !a.stats) || !workspace)) return training_fail(FFCVB_E_ARG, "%s: no statistics or workspace", name);
+    if ((reinterpret_cast<uintptr_t>(a.stats) & 15) != 0) return training_fail(FFCVB_E_ARG, "%s: stats begin on 16 bytes", name);
     return FFCVB_OK;
 }
 

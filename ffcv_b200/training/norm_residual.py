@@ -149,6 +149,10 @@ def norm_residual_backward(dy, dz, x, h, stats, *, norm='layer', weight=None, bi
     """Gradients of all tensors that :func:`norm_residual_forward` was given, by their names, from those of y and z (None: 0).
     Where the branch is added as it is, the entries 'x' and 'h' are one tensor."""
     call = _Call(x, h, norm, weight, bias, post_norm, post_weight, post_bias, gate, scale, eps)
+    if not isinstance(stats, ch.Tensor) or stats.shape != (4 * call.rows,) or stats.dtype != ch.float32 or not stats.is_contiguous() or stats.device != x.device:
+        raise ValueError('stats must be what the forward pass of the same call gave')
+    if stats.data_ptr() % 16:  # (kept in the middle of another tensor)
+        stats = stats.clone()
     grads = call.backward(stats, dy, dz, [t is not None for t in (x, h, weight, bias, post_weight, post_bias, gate, call.scale)])
     return {name: g for name, g in zip(_NAMES, grads) if g is not None}
 

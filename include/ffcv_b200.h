@@ -402,7 +402,7 @@ enum { FFCVB_GATE_NONE = 0, FFCVB_GATE_SAMPLE = 1, FFCVB_GATE_TOKEN = 2 };
 typedef struct {
     const void *x, *h, *gate;
     const void *weight, *bias, *post_weight, *post_bias, *scale;
-    float *stats;           /* [rows, 4]: mean and 1 / deviation of y and of h; written forward, read backward */
+    float *stats;           /* [rows, 4], 16-byte aligned: mean and 1 / deviation of y and of h; written forward, read backward */
     void *y, *z;            /* contiguous; forward only */
     const void *dy, *dz;    /* gradients of y and z, or NULL: 0; backward only, like the following */
     void *dx, *dh, *dgate;  /* contiguous, or NULL: not wanted */

@@ -21,3 +21,11 @@ def test_cross_entropy():
     for at in (257, 260, 263):
         args = N.CROSS_ENTROPY.pack(16, 16, 0, 16, 0, 16, at, 0, 4, 5, 5, 1, 5, 0, 0, 0, 0, 0, 0, 1, 0, 0, 0.0, 1.0)
         assert N.lib.ffcvb_cross_entropy(args, None) == -2 and b'stats begin on 8 bytes' in N.lib.ffcvb_training_error()
+
+
+def test_norm_residual():
+    from ffcv_b200.training import _native as N
+    for at in (257, 260, 264, 271):
+        args = N.NORM_RESIDUAL.pack(16, 16, 0, 0, 0, 0, 0, 0, at, 16, 16, *([0] * 5), *([0] * 5), 2, 8, 1, 8, 8, 8, 8, 8, 0, 0, 0, 1, 0, 0, 1e-6, 1.0)
+        for call in (lambda: N.lib.ffcvb_norm_residual(args, None), lambda: N.lib.ffcvb_norm_residual_backward(args, 256, None)):
+            assert call() == -2 and b'stats begin on 16 bytes' in N.lib.ffcvb_training_error()
