@@ -10,9 +10,10 @@
 // classes with entries, or labels, are written once more, each by one thread, with the shares of all entries of that class, in their order: the same
 // class may come twice.  So the row crosses HBM once each way.
 //
-// What bounds it: exponentials, two for a logit, or three with the hard loss (one of them from the other where the temperature is 1, 2 or 4; else four), and the
-// instructions around them.  8192 x 21841 bf16 logits with 64 entries take 156 us, 110 at the rate of a copy; the unit for exponentials is busy for 63 % of it and 61 % of the
-// turns to issue are used, by five CTAs on an SM.  1531 x 50021 fp16 logits with 200 entries and labels take 121 us (65 %), 47 at the rate of a copy.  512 x 10 take 8 us: two launches.
+// What bounds it: exponentials and the instructions around them, and that a row's passes wait for one another.  A logit has two exponentials, one in each pass; four with the hard loss, but
+// where the temperature is 1, 2 or 4, whose one exponential gives the other.  8192 x 21841 bf16 logits with 64 entries take 158 to 164 us, 110 at the rate of a copy; the unit for exponentials
+// is busy for 67 % of it and 65 % of the turns to issue are used, by five CTAs on an SM, whose warps wait for one another's results and at barriers most.  1531 x 50021 fp16 logits with 200
+// entries and labels at 3.5 take 118 to 121 us, 47 at the rate of a copy (80 % of the unit's time with 8192 x 21841).  512 x 10 take 8 us: two launches.
 #include "losses.h"
 
 #include <algorithm>
@@ -487,7 +488,8 @@ distill_kernel(const __grid_constant__ ffcvb_distillation_args a, const Deal dea
 }
 
 // As for the cross entropy's rows: bytes of a row in a CTA's shared memory (8192 x 21841 in 16 bits 156 us, 181 with 40 KB, 157 with 100; 1531 x 50021 124, 132 and
-// 124), at most where eight CTAs have a row, and in a warp's (16384 x 2000 in 16 bits 54 us, 88 by CTAs; 8192 x 3500 35 and 45; 16384 x 300 in 32 bits 27 and 73).
+// 124; with 56, 40 and 72 KB 3413 x 24000 87, 89 and 87, 2730 x 30000 86, 86 and 93, 1637 x 50021 91, 88 and 91, 1170 x 70000 87, 87 and 92, 409 x 200000 89 each, in
+// 32 bits 4818 x 17000 139, 140 and 142, 3750 x 21841 142, 150 and 142), at most where eight CTAs have a row, and in a warp's (16384 x 2000 in 16 bits 54 us, 88 by CTAs; 8192 x 3500 35 and 45; 16384 x 300 in 32 bits 27 and 73).
 constexpr long long kPartBytes = 56 * 1024, kMostPartBytes = 72 * 1024, kWarpBytes = 8192;
 
 template <typename T, int HARD> void launch_rows(const ffcvb_distillation_args &a, cudaStream_t stream) {

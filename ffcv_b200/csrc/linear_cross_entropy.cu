@@ -9,9 +9,9 @@
 // operations instead of 6 are done, and no logits are kept; the first time leaves 8 bytes (12 with smoothing) for 128 logits of a row, or for 64 with narrow tiles.
 //
 // What bounds it: the tensor cores, and in long runs the clock that their power leaves.  8192 x 21841 x 1024 in bf16 with all gradients takes 1.04 ms in a short run and
-// 1.19 in a long one; 880 us is the 8 * rows * classes * width at the rate of a large library product, 660 the 6.  Of it the statistics take 236 us (1550 TFLOP/s), the
-// joining 9, and each of the two chunks of 10921 classes 130 for G (1410), 240 for its products (1530) and 10 for what is left of them.  Kept in 16 bits
-// instead the logits would be 358 MB written and read, and rounded before the exponentials.  64 x 1000 x 384 takes 29 us: six launches, which wait for one another.
+// 1.2 to 1.26 in a long one; 880 us is the 8 * rows * classes * width at the rate of a large library product, 660 the 6.  Of it the statistics take 236 us (1550 TFLOP/s), the
+// joining 9, and each of the two chunks of 10921 classes 130 for G (1410; 142 with the bias' sums), 240 for its products (1530) and 10 for what is left of them.  Kept in 16 bits
+// instead the logits would be 358 MB written and read, and rounded before the exponentials.  64 x 1000 x 384 takes 29 to 32 us: six launches, which wait for one another.
 #include "losses.h"
 #include "tensor.h"
 
@@ -129,7 +129,7 @@ struct Tile {
 __device__ __forceinline__ int row_tiles_of(const Products &p, const Product &w, int rows) { return w.counted == kRowsCounted ? (rows + p.high - 1) / p.high : w.row_tiles; }
 // (a sum without terms is one block long, all the same)
 __device__ __forceinline__ int sum_blocks_of(const Product &w, int rows) { return w.counted == kSumCounted ? max(1, (rows + kSum - 1) / kSum) : w.sum_blocks; }
-// Blocks of runs, at least: shorter ones cost more than they save.  (64 x 1000 x 384 33 us, 42 with 1, 41 with 16; 4096 x 100 x 384 54, 67 and 58; 2048 x 1000 x 768
+// Blocks of runs, at least: shorter ones cost more than they save.  (As built then, 64 x 1000 x 384 33 us, 42 with 1, 41 with 16; 4096 x 100 x 384 54, 67 and 58; 2048 x 1000 x 768
 // 54, 54 and 49; larger ones within one in a hundred.)
 constexpr int kLeastRun = 4;
 // How blocks are dealt out: with few columns of tiles those of each column, in the same way to as many CTAs or pairs, so that those with the same rows read A at the same time;

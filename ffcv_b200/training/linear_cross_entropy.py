@@ -121,6 +121,9 @@ def linear_cross_entropy_with_grad(hidden, weight, labels=None, *, mixed=None, b
     per sample from behind (``reduction='none'`` and autograd) it is held relative to the largest of these among the samples that count: in
     float16 in steps of 2^-38 of that, so a sample with a billionth of the largest keeps few digits.  One that is infinite or NaN
     makes its own sample's hidden gradient NaN, and those of the weights and the bias, which are sums over the samples.
+
+    A kernel whose own copies or products do not come to an end gives up after two seconds; the call has returned by then, and what is missing is
+    NaN, in the loss too.
     """
     call = _Call(hidden, weight, labels, mixed, bias, label_smoothing, ignore_index, reduction)
     n = hidden.shape[0]

@@ -347,7 +347,9 @@ int ffcvb_cross_entropy(const ffcvb_cross_entropy_args *args, void *stream);
 /* The same loss of a linear layer's outputs, which are not kept: logits = hidden weight^T + bias, of 16-bit hidden [rows, width] and
  * weight [classes, width], in 32 bits, made twice, the second time in pieces of the classes for the gradients; targets as labels or rows of
  * LabelMixup, ignored rows and rows that give NaN as above.  Rows with the label ignore_index are not read.  A part of the gradient of the
- * logits is held in 16 bits at a time; sums are of 32 bits, always in the same order.  At most 2^24 rows and classes, a width of 2^16. */
+ * logits is held in 16 bits at a time, with upstream_per_row relative to the largest finite upstream of a row that counts (one that is not finite makes its own row's
+ * grad_hidden NaN, and grad_weight and grad_bias); grad_bias is of it as it was before.  Sums are of 32 bits, always in the same order.  A kernel whose copies or products
+ * do not end gives up after two seconds: the call has returned FFCVB_OK by then, and what is missing is NaN.  At most 2^24 rows and classes, a width of 2^16. */
 typedef struct {
     const void *hidden, *weight, *bias; /* of `type`, neighbours in a row next to one another; bias [classes] or NULL */
     const void *target;
